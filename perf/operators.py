@@ -18,6 +18,7 @@ even index in the low half, exponents (biased by 127) in [pages, kv heads, 2, pa
 
 from __future__ import annotations
 
+import functools
 import math
 import sys
 from pathlib import Path
@@ -31,6 +32,7 @@ LEVELS = (0.0, 0.5, 1.0, 1.5, 2.0, 3.0, 4.0, 6.0)
 EPS = 1e-6
 
 
+@functools.lru_cache(maxsize=None)
 def _tattn():
     pkg = str(Path(__file__).resolve().parent.parent / "triton-attn_amd")
     if pkg not in sys.path:
