@@ -170,6 +170,39 @@ enum tattn_pick {
 int tattn_picked(int kernel, const int64_t k_strides[4], const int64_t v_strides[4], int64_t Z, int64_t H,
                  int64_t N, int64_t D, int dtype, int causal, float sm_scale);
 
+/*
+ * Operators around attention. No counterpart in the reference. Pointers may be null where their
+ * tensor has no elements; a call without work (no tokens, no requests) launches nothing and returns 0.
+ *
+ * Pages for the tokens that R requests add: request r holds lens[r] tokens, adds new_tokens[r], and its
+ * pages are tables[r * table_stride ..] (P entries). Pages past ceil(lens[r] / page_size) come from
+ * free_pages (F of them) in request order and are entered into the table. For the T tokens in request order:
+ * slots (page * page_size + offset) and positions; starts[R + 1] is where each request's tokens begin and
+ * taken[0] how many pages they need. A token without a page (free list or table row exhausted, or an
+ * entry of the table below 0) has slot -1; tokens past T are not placed, entries of T behind the last request hold
+ * slot -1, position 0. Negative lengths count as 0. page_size: a power of two, 16 to 1024. lens is not updated.
+ */
+int tattn_page_tables(const int32_t* lens, const int32_t* new_tokens, int32_t* tables, const int32_t* free_pages,
+                      int64_t* slots, int32_t* positions, int32_t* starts, int32_t* taken, int64_t R, int64_t P,
+                      int64_t table_stride, int64_t F, int64_t T, int64_t page_size, void* stream);
+
+/*
+ * A key/value cache in 4 bits (TATTN_F16 or TATTN_BF16 values; D = 32, 64 or 128). codes:
+ * [pages, H, 2, page_size, D / 2] bytes (2: keys, values; an even d in the low four bits), e2m1: sign, two
+ * exponent bits, one mantissa bit. scales: [pages, H, 2, page_size, D / 32] bytes, exponents biased by 127 of
+ * the blocks of 32 values along d: the smallest at which the block's largest magnitude rounds to 6 or less (and
+ * at which 6 * 2^e is finite in the element type); 255
+ * marks a block that held an infinity or a NaN and reads as NaN. Magnitudes below 2^-120 count as zero.
+ * write: k, v [T, H, D] with (token, head) strides in elements, unit d stride, 16-byte aligned rows,
+ * into `slots`; read: what the cache holds for `slots`, contiguous [T, H, D]. Slots outside the cache (a batch's
+ * padding has -1) are not written and read as zeros. No two tokens of a write may have one slot.
+ */
+int tattn_cache4_write(uint8_t* codes, uint8_t* scales, const void* k, const void* v, const int64_t* slots,
+                       const int64_t k_strides[2], const int64_t v_strides[2], int64_t T, int64_t H, int64_t D,
+                       int64_t pages, int64_t page_size, int dtype, void* stream);
+int tattn_cache4_read(const uint8_t* codes, const uint8_t* scales, void* k, void* v, const int64_t* slots, int64_t T,
+                      int64_t H, int64_t D, int64_t pages, int64_t page_size, int dtype, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

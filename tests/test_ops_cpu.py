@@ -1,0 +1,135 @@
+"""Refusals of the operators around attention, checked before anything reaches a GPU: the Python
+wrappers' messages and the C entry points' codes."""
+
+import ctypes
+
+import pytest
+import torch
+
+import tattn
+from tattn import _lib
+
+
+def i32(*x):
+    return torch.tensor(x, dtype=torch.int32)
+
+
+# ---- page_tables ---------------------------------------------------------------------------------
+
+def _tables(**kw):
+    a = dict(lens=i32(3, 0), new_tokens=i32(1, 5), tables=torch.zeros(2, 4, dtype=torch.int32), free_pages=i32(5, 6, 7),
+             page_size=16, tokens=8)
+    a.update(kw)
+    return tattn.page_tables(**a)
+
+
+@pytest.mark.parametrize("bad,msg", [
+    (dict(lens=torch.zeros(2, dtype=torch.int64)), "lens must be int32"),
+    (dict(lens=torch.zeros(2, 1, dtype=torch.int32)), "lens must be int32"),
+    (dict(new_tokens=i32(1)), "new_tokens must be int32 of shape"),
+    (dict(tables=torch.zeros(3, 4, dtype=torch.int32)), "tables must be int32 of shape"),
+    (dict(tables=torch.zeros(4, dtype=torch.int32)), "tables must be int32"),
+    (dict(tables=torch.zeros(4, 2, dtype=torch.int32).t()), "updated in place"),
+    (dict(tables=torch.zeros(1, 4, dtype=torch.int32).expand(2, 4)), "updated in place"),
+    (dict(free_pages=torch.zeros(3)), "free_pages must be int32"),
+    (dict(page_size=24), "page size"),
+    (dict(page_size=8), "page size"),
+    (dict(page_size=2048), "page size"),
+    (dict(tokens=-1), "tokens out of range"),
+    (dict(tokens=1 << 31), "tokens out of range"),
+    (dict(new_tokens=torch.zeros(2, dtype=torch.int32, device="meta")), "must be on cpu"),
+])
+def test_page_tables_refuses(bad, msg):
+    with pytest.raises(ValueError, match=msg):
+        _tables(**bad)
+
+
+def test_page_tables_has_no_cpu_path():
+    with pytest.raises(RuntimeError, match="gfx950"):
+        _tables()
+
+
+@pytest.mark.parametrize("bad,msg", [
+    (dict(page=20), "page size"), (dict(page=0), "page size"), (dict(T=-1), "tokens out of range"),
+    (dict(R=1 << 31), "requests out of range"), (dict(lens=None), "lens is a null pointer"),
+    (dict(slots=12), "slots must be 8-byte aligned"), (dict(taken=None), "taken is a null pointer"),
+    (dict(stride=3), "rows overlap"),
+])
+def test_page_tables_entry_point_refuses(bad, msg):
+    a = dict(lens=16, add=16, tables=16, free=16, slots=16, pos=16, starts=16, taken=16, R=2, P=4, stride=4, F=3, T=8,
+             page=16, stream=None)
+    a.update(bad)
+    assert _lib.load().tattn_page_tables(*a.values()) == 1
+    assert msg in _lib.last_error()
+
+
+# ---- the cache in 4 bits ------------------------------------------------------------------------
+
+def _cache(dtype=torch.float16, page=16, d=64):
+    return tattn.Cache4.empty(3, page, 2, d, dtype=dtype, device="cpu")
+
+
+def test_cache4_describes_itself():
+    c = _cache()
+    assert (c.pages, c.page_size, c.kv_heads, c.head_dim, c.dtype) == (3, 16, 2, 64, torch.float16)
+    assert c.codes.shape == (3, 2, 2, 16, 32) and c.scales.shape == (3, 2, 2, 16, 2)
+
+
+@pytest.mark.parametrize("kw,msg", [
+    (dict(d=16), "head dim"), (dict(d=256), "head dim"), (dict(page=20), "page size"), (dict(page=8), "page size"),
+    (dict(dtype=torch.float32), "dtype"),
+])
+def test_cache4_refuses(kw, msg):
+    with pytest.raises(ValueError, match=msg):
+        _cache(**kw)
+
+
+def test_cache4_refuses_buffers_that_do_not_belong_together():
+    c = _cache()
+    with pytest.raises(ValueError, match="codes must be uint8"):
+        tattn.Cache4(c.codes[0], c.scales, c.dtype)
+    with pytest.raises(ValueError, match="scales must be uint8"):
+        tattn.Cache4(c.codes, c.scales[..., :1], c.dtype)
+    with pytest.raises(ValueError, match="contiguous"):
+        tattn.Cache4(c.codes[:, :, :, ::1].transpose(0, 1).contiguous().transpose(0, 1), c.scales, c.dtype)
+    with pytest.raises(ValueError, match="scales must be on"):
+        tattn.Cache4(c.codes, c.scales.to("meta"), c.dtype)
+
+
+@pytest.mark.parametrize("bad,msg", [
+    (dict(k=torch.zeros(5, 2, 32, dtype=torch.float16)), "expected k, v"),
+    (dict(k=torch.zeros(4, 2, 64, dtype=torch.float16)), "expected k, v"),
+    (dict(v=torch.zeros(5, 2, 64, dtype=torch.bfloat16)), "dtype"),
+    (dict(slots=torch.zeros(5, dtype=torch.int32)), "slots must be int64"),
+    (dict(slots=torch.zeros(4, dtype=torch.int64)), "slots must be int64"),
+    (dict(slots=torch.zeros(5, dtype=torch.int64, device="meta")), "slots must be on"),
+])
+def test_cache4_write_refuses(bad, msg):
+    a = dict(k=torch.zeros(5, 2, 64, dtype=torch.float16), v=torch.zeros(5, 2, 64, dtype=torch.float16),
+             slots=torch.zeros(5, dtype=torch.int64))
+    a.update(bad)
+    with pytest.raises(ValueError, match=msg):
+        tattn.cache4_write(_cache(), **a)
+
+
+def test_cache4_read_refuses():
+    for bad in (torch.zeros(5, dtype=torch.int32), torch.zeros(5, 1, dtype=torch.int64)):
+        with pytest.raises(ValueError, match="slots must be int64"):
+            tattn.cache4_read(_cache(), bad)
+    with pytest.raises(RuntimeError, match="gfx950"):
+        tattn.cache4_read(_cache(), torch.zeros(5, dtype=torch.int64))
+
+
+@pytest.mark.parametrize("bad,msg", [
+    (dict(D=16), "head dim"), (dict(dtype=_lib.F32), "dtype"), (dict(page=48), "page size"), (dict(pages=-1), "pages out of range"),
+    (dict(codes=None), "codes is a null pointer"), (dict(codes=24), "codes must be 16-byte aligned"),
+    (dict(k=8), "k must be 16-byte aligned"), (dict(ks=(ctypes.c_int64 * 2)(128, 60)), "k stride"),
+    (dict(vs=None), "v strides are null"), (dict(T=1 << 31), "tokens out of range"),
+])
+def test_cache4_write_entry_point_refuses(bad, msg):
+    st = (ctypes.c_int64 * 2)(128, 64)
+    a = dict(codes=16, scales=16, k=16, v=16, slots=16, ks=st, vs=st, T=4, H=2, D=64, pages=3, page=16, dtype=_lib.F16,
+             stream=None)
+    a.update(bad)
+    assert _lib.load().tattn_cache4_write(*a.values()) == 1
+    assert msg in _lib.last_error()

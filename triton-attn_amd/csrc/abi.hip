@@ -10,6 +10,7 @@
 
 #include "../../include/tattn.h"
 #include "launch.h"
+#include "ops.h"
 #include "tiles.h"
 
 namespace tattn {
@@ -361,6 +362,9 @@ int check_config(int kernel, int64_t D, int dtype, int id) {
 }
 
 }  // namespace
+
+int require_device() { return device_check(); }
+
 }  // namespace tattn
 
 using namespace tattn;

@@ -1,0 +1,117 @@
+// C ABI of the operators around attention (declared in include/tattn.h): argument checks, then the
+// launchers of ops.h.
+#include <hip/hip_runtime.h>
+
+#include "../../include/tattn.h"
+#include "ops.h"
+
+namespace tattn {
+namespace {
+
+bool aligned(const void* p, unsigned bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0; }
+
+// A pointer that may be null only where the tensor has no elements.
+int check_ptr(const char* name, const void* p, int64_t elements, unsigned align) {
+  if (elements > 0 && !p) return set_error(TATTN_E_ARG, "%s is a null pointer", name);
+  if (!aligned(p, align)) return set_error(TATTN_E_ARG, "%s must be %u-byte aligned", name, align);
+  return TATTN_OK;
+}
+
+// Strides (in elements) of dimensions before the unit-stride d: whole 16-byte rows.
+int check_rows(const char* name, const int64_t* st, int n, int sz) {
+  if (!st) return set_error(TATTN_E_ARG, "%s strides are null", name);
+  for (int i = 0; i < n; ++i)
+    if (st[i] < 0 || (st[i] * sz) % 16 != 0)
+      return set_error(TATTN_E_ARG, "%s stride %lld must be a multiple of %d elements", name, (long long)st[i], 16 / sz);
+  return TATTN_OK;
+}
+
+int check_page(int64_t page_size, int32_t* shift) {
+  if (page_size < 16 || page_size > 1024 || (page_size & (page_size - 1)))
+    return set_error(TATTN_E_ARG, "page size must be a power of two from 16 to 1024, got %lld", (long long)page_size);
+  *shift = __builtin_ctzll((unsigned long long)page_size);
+  return TATTN_OK;
+}
+
+int check_count(const char* name, int64_t x) {
+  if (x < 0 || x > 0x7fffffff - 4096) return set_error(TATTN_E_ARG, "%s out of range: %lld", name, (long long)x);
+  return TATTN_OK;
+}
+
+int cache4_common(Cache4Params& p, const void* codes, const void* scales, const int64_t* slots, int64_t T, int64_t H,
+                  int64_t D, int64_t pages, int64_t page_size, int dtype) {
+  int rc;
+  if (dtype != TATTN_F16 && dtype != TATTN_BF16)
+    return set_error(TATTN_E_ARG, "dtype must be TATTN_F16 or TATTN_BF16, got %d", dtype);
+  if (D != 32 && D != 64 && D != 128) return set_error(TATTN_E_ARG, "head dim must be 32, 64 or 128, got %lld", (long long)D);
+  if ((rc = check_page(page_size, &p.shift)) || (rc = check_count("tokens", T)) || (rc = check_count("heads", H)) ||
+      (rc = check_count("pages", pages)))
+    return rc;
+  if ((rc = check_ptr("codes", codes, pages * H, 16)) || (rc = check_ptr("scales", scales, pages * H, 4)) ||
+      (rc = check_ptr("slots", slots, T, 8)))
+    return rc;
+  p.codes = (uint8_t*)codes;
+  p.scales = (uint8_t*)scales;
+  p.slots = slots;
+  p.T = (int32_t)T;
+  p.H = (int32_t)H;
+  p.total = pages * page_size;
+  return TATTN_OK;
+}
+
+}  // namespace
+}  // namespace tattn
+
+using namespace tattn;
+
+extern "C" {
+
+int tattn_page_tables(const int32_t* lens, const int32_t* new_tokens, int32_t* tables, const int32_t* free_pages,
+                      int64_t* slots, int32_t* positions, int32_t* starts, int32_t* taken, int64_t R, int64_t P,
+                      int64_t table_stride, int64_t F, int64_t T, int64_t page_size, void* stream) {
+  TablesParams p{};
+  int rc;
+  if ((rc = check_page(page_size, &p.shift)) || (rc = check_count("requests", R)) || (rc = check_count("table width", P)) ||
+      (rc = check_count("free pages", F)) || (rc = check_count("tokens", T)))
+    return rc;
+  if ((rc = check_ptr("lens", lens, R, 4)) || (rc = check_ptr("new_tokens", new_tokens, R, 4)) ||
+      (rc = check_ptr("tables", tables, R * P, 4)) || (rc = check_ptr("free_pages", free_pages, F, 4)) ||
+      (rc = check_ptr("slots", slots, T, 8)) || (rc = check_ptr("positions", positions, T, 4)) ||
+      (rc = check_ptr("starts", starts, 1, 4)) || (rc = check_ptr("taken", taken, 1, 4)))
+    return rc;
+  if (R > 1 && table_stride < P) return set_error(TATTN_E_ARG, "table rows overlap: stride %lld", (long long)table_stride);
+  if ((rc = require_device())) return rc;
+  p.lens = lens; p.add = new_tokens; p.tables = tables; p.free_pages = free_pages;
+  p.slots = slots; p.positions = positions; p.starts = starts; p.taken = taken;
+  p.table_stride = table_stride;
+  p.R = (int32_t)R; p.P = (int32_t)P; p.F = (int32_t)F; p.T = (int32_t)T;
+  return launch_page_tables(p, (hipStream_t)stream);
+}
+
+int tattn_cache4_write(uint8_t* codes, uint8_t* scales, const void* k, const void* v, const int64_t* slots,
+                       const int64_t k_strides[2], const int64_t v_strides[2], int64_t T, int64_t H, int64_t D,
+                       int64_t pages, int64_t page_size, int dtype, void* stream) {
+  Cache4Params p{};
+  int rc;
+  if ((rc = cache4_common(p, codes, scales, slots, T, H, D, pages, page_size, dtype))) return rc;
+  if ((rc = check_ptr("k", k, T * H, 16)) || (rc = check_ptr("v", v, T * H, 16)) || (rc = check_rows("k", k_strides, 2, 2)) ||
+      (rc = check_rows("v", v_strides, 2, 2)) || (rc = require_device()))
+    return rc;
+  if (T == 0 || H == 0 || pages == 0) return TATTN_OK;
+  p.k = k; p.v = v;
+  for (int i = 0; i < 2; ++i) p.sk[i] = k_strides[i], p.sv[i] = v_strides[i];
+  return launch_cache4_write(p, (int)D, dtype, (hipStream_t)stream);
+}
+
+int tattn_cache4_read(const uint8_t* codes, const uint8_t* scales, void* k, void* v, const int64_t* slots, int64_t T,
+                      int64_t H, int64_t D, int64_t pages, int64_t page_size, int dtype, void* stream) {
+  Cache4Params p{};
+  int rc;
+  if ((rc = cache4_common(p, codes, scales, slots, T, H, D, pages, page_size, dtype))) return rc;
+  if ((rc = check_ptr("k", k, T * H, 16)) || (rc = check_ptr("v", v, T * H, 16)) || (rc = require_device())) return rc;
+  if (T == 0 || H == 0) return TATTN_OK;
+  p.ko = k; p.vo = v;
+  return launch_cache4_read(p, (int)D, dtype, (hipStream_t)stream);
+}
+
+}  // extern "C"

@@ -1,0 +1,47 @@
+// Host-side launchers of the operators around attention: page bookkeeping, the cache in 4 bits,
+// norms with rotation, window attention. Arguments are checked by the entry points (abi_ops.hip).
+#pragma once
+
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include "launch.h"
+
+namespace tattn {
+
+// The current device runs these kernels: TATTN_OK or an error code with its message.
+int require_device();
+
+struct TablesParams {
+  const int32_t* lens;
+  const int32_t* add;
+  int32_t* tables;
+  const int32_t* free_pages;
+  int64_t* slots;
+  int32_t* positions;
+  int32_t* starts;
+  int32_t* taken;
+  int64_t table_stride;
+  int32_t R, P, F, T;
+  int32_t shift;  // log2 of the page size
+};
+int launch_page_tables(const TablesParams& p, hipStream_t st);
+
+// The cache in 4 bits: codes [pages, heads, 2, page, d / 2], scales [pages, heads, 2, page, d / 32].
+struct Cache4Params {
+  uint8_t* codes;
+  uint8_t* scales;
+  const void* k;  // written: [T, heads, d] with the strides below
+  const void* v;
+  void* ko;  // read: [T, heads, d] contiguous
+  void* vo;
+  const int64_t* slots;
+  int64_t sk[2], sv[2];  // (token, head) strides of k and v in elements
+  int64_t total;         // slots of the cache
+  int32_t T, H;
+  int32_t shift;  // log2 of the page size
+};
+int launch_cache4_write(const Cache4Params& p, int D, int dtype, hipStream_t st);
+int launch_cache4_read(const Cache4Params& p, int D, int dtype, hipStream_t st);
+
+}  // namespace tattn

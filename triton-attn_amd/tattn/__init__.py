@@ -4,5 +4,7 @@ Drop-in for amaanmithani/triton-attn's `tattn` package (src/tattn/__init__.py:3-
 """
 
 from tattn.api import attention, autotune_cache, configs, hip_available, set_autotune, triton_available
+from tattn.paged import Cache4, PageTables, cache4_read, cache4_write, page_tables
 
-__all__ = ["attention", "triton_available", "hip_available", "configs", "set_autotune", "autotune_cache"]
+__all__ = ["attention", "triton_available", "hip_available", "configs", "set_autotune", "autotune_cache",
+           "page_tables", "PageTables", "Cache4", "cache4_write", "cache4_read"]

@@ -24,6 +24,7 @@ EXPORTS = (
     "tattn_abi_version", "tattn_last_error", "tattn_device_supported", "tattn_fwd",
     "tattn_bwd_preprocess", "tattn_bwd_dkdv", "tattn_bwd_dq", "tattn_bwd", "tattn_bwd_layouts", "tattn_bwd_noalloc",
     "tattn_num_configs", "tattn_config_desc", "tattn_pick_config", "tattn_picked",
+    "tattn_page_tables", "tattn_cache4_write", "tattn_cache4_read",
 )
 
 # Kernels outside the tables, as `picked` reports them.
@@ -67,6 +68,9 @@ _SIGS = {
     "tattn_config_desc": (_I, [_I, _I64, _I, _I, ctypes.POINTER(TattnConfig)]),
     "tattn_pick_config": (_I, [_I, _I64, _I, _I, _I64]),
     "tattn_picked": (_I, [_I, _STR4, _STR4, _I64, _I64, _I64, _I64, _I, _I, _F]),
+    "tattn_page_tables": (_I, [_P] * 8 + [_I64] * 6 + [_P]),
+    "tattn_cache4_write": (_I, [_P] * 5 + [_STR4, _STR4] + [_I64] * 5 + [_I, _P]),
+    "tattn_cache4_read": (_I, [_P] * 5 + [_I64] * 5 + [_I, _P]),
 }
 
 _lib: ctypes.CDLL | None = None
