@@ -203,6 +203,31 @@ int tattn_cache4_write(uint8_t* codes, uint8_t* scales, const void* k, const voi
 int tattn_cache4_read(const uint8_t* codes, const uint8_t* scales, void* k, void* v, const int64_t* slots, int64_t T,
                       int64_t H, int64_t D, int64_t pages, int64_t page_size, int dtype, void* stream);
 
+/*
+ * Root-mean-square norm of every head of q [Z, H, N, D] and k [Z, Hk, N, D], its weights, and the position
+ * rotation: y = x / sqrt(mean(x^2) + eps) * weight, then pairs (i, i + D / 2) of y, or (2i, 2i + 1) when
+ * interleaved, turned by the angle whose cosine and sine are cos[position][i], sin[position][i] (float32
+ * [P, D / 2], contiguous). positions: [N] (pos_stride 0) or one row per z, pos_stride apart; null: n. A position
+ * outside [0, P) gives a row of NaN. dtype: any; D: 16, 32, 64, 128; w_dtype: dtype or TATTN_F32. Tensor strides
+ * are (z, h, n, d) in elements, unit d stride, 16-byte aligned rows; everything is float32 up to one rounding per result.
+ *
+ * The backward gives dq, dk and, unless workspace is null, both weights' gradients in w_dtype (sums in a fixed
+ * order, no atomics). workspace: float32 [TATTN_NORM_ROPE_ROWS, D]. Without tokens nothing is written.
+ */
+#define TATTN_NORM_ROPE_ROWS 512
+int tattn_norm_rope_fwd(const void* q, const void* k, const void* q_weight, const void* k_weight, const float* cos,
+                        const float* sin, const int32_t* positions, void* q_out, void* k_out, const int64_t q_strides[4],
+                        const int64_t k_strides[4], const int64_t qo_strides[4], const int64_t ko_strides[4],
+                        int64_t pos_stride, int64_t Z, int64_t H, int64_t Hk, int64_t N, int64_t D, int64_t P, int dtype,
+                        int w_dtype, int interleaved, float eps, void* stream);
+int tattn_norm_rope_bwd(const void* q, const void* k, const void* q_weight, const void* k_weight, const float* cos,
+                        const float* sin, const int32_t* positions, const void* dq_out, const void* dk_out, void* dq,
+                        void* dk, void* dq_weight, void* dk_weight, float* workspace, const int64_t q_strides[4],
+                        const int64_t k_strides[4], const int64_t dqo_strides[4], const int64_t dko_strides[4],
+                        const int64_t dq_strides[4], const int64_t dk_strides[4], int64_t pos_stride, int64_t Z, int64_t H,
+                        int64_t Hk, int64_t N, int64_t D, int64_t P, int dtype, int w_dtype, int interleaved, float eps,
+                        void* stream);
+
 #ifdef __cplusplus
 }
 #endif

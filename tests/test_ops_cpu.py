@@ -133,3 +133,60 @@ def test_cache4_write_entry_point_refuses(bad, msg):
     a.update(bad)
     assert _lib.load().tattn_cache4_write(*a.values()) == 1
     assert msg in _lib.last_error()
+
+
+# ---- qk_norm_rope --------------------------------------------------------------------------------
+
+def _norm_rope(**kw):
+    a = dict(q=torch.zeros(2, 4, 8, 32), k=torch.zeros(2, 2, 8, 32), q_weight=torch.ones(32), k_weight=torch.ones(32),
+             cos=torch.ones(8, 16), sin=torch.ones(8, 16))
+    a.update(kw)
+    return tattn.qk_norm_rope(**a)
+
+
+@pytest.mark.parametrize("bad,msg", [
+    (dict(q=torch.zeros(4, 8, 32)), "expected q"),
+    (dict(k=torch.zeros(2, 2, 9, 32)), "expected q"),
+    (dict(k=torch.zeros(2, 0, 8, 32)), "at least one head"),
+    (dict(q=torch.zeros(2, 4, 8, 48), k=torch.zeros(2, 2, 8, 48)), "head dim"),
+    (dict(q=torch.zeros(2, 4, 8, 32).half()), "dtype"),
+    (dict(q_weight=torch.ones(16)), "q_weight must have shape"),
+    (dict(k_weight=torch.ones(32).half()), "k_weight must have shape"),
+    (dict(cos=torch.ones(8, 32)), "cos must be float32"),
+    (dict(sin=torch.ones(8, 16).half()), "sin must be float32"),
+    (dict(sin=torch.ones(7, 16)), "sin must be float32"),
+    (dict(cos=torch.ones(7, 16), sin=torch.ones(7, 16)), "7 rows for 8 positions"),
+    (dict(cos=torch.ones(0, 16), sin=torch.ones(0, 16), positions=torch.zeros(8, dtype=torch.int32)), "no rows"),
+    (dict(positions=torch.zeros(8, dtype=torch.int64)), "positions must be int32"),
+    (dict(positions=torch.zeros(1, 8, dtype=torch.int32)), "positions must be int32"),
+    (dict(cos=torch.ones(8, 16, device="meta")), "cos must be on"),
+])
+def test_qk_norm_rope_refuses(bad, msg):
+    with pytest.raises(ValueError, match=msg):
+        _norm_rope(**bad)
+
+
+def test_qk_norm_rope_has_no_cpu_path():
+    with pytest.raises(RuntimeError, match="gfx950"):
+        _norm_rope()
+
+
+@pytest.mark.parametrize("bad,msg", [
+    (dict(D=48), "head dim"), (dict(dtype=9), "unknown dtype"), (dict(wd=_lib.BF16), "weights must be"), (dict(Hk=0), "heads must be positive"),
+    (dict(q=8), "q must be 16-byte aligned"), (dict(cos=None), "cos is a null pointer"), (dict(P=0), "no rows"),
+    (dict(ks=(ctypes.c_int64 * 4)(64, 60, 32, 1)), "k stride"), (dict(ko=None), "k_out is a null pointer"),
+    (dict(Z=1 << 20, N=1 << 20), "too many tokens"),
+])
+def test_norm_rope_entry_point_refuses(bad, msg):
+    st = (ctypes.c_int64 * 4)(1024, 256, 32, 1)
+    a = dict(q=16, k=16, qw=16, kw=16, cos=16, sin=16, pos=None, qo=16, ko=16, qs=st, ks=st, qos=st, kos=st, ps=0, Z=2, H=4,
+             Hk=2, N=8, D=32, P=8, dtype=_lib.F16, wd=_lib.F16, il=0, eps=1e-6, stream=None)
+    a.update(bad)
+    assert _lib.load().tattn_norm_rope_fwd(*a.values()) == 1
+    assert msg in _lib.last_error()
+
+
+def test_norm_rope_workspace_rows_match_the_header():
+    from test_abi import HEADER
+
+    assert f"#define TATTN_NORM_ROPE_ROWS {_lib.NORM_ROPE_ROWS}" in HEADER.read_text()

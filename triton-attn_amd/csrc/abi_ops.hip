@@ -59,6 +59,42 @@ int cache4_common(Cache4Params& p, const void* codes, const void* scales, const 
   return TATTN_OK;
 }
 
+// Everything the norm's two directions share; no work is left when N or Z is 0.
+int norm_rope_common(NormRopeParams& p, const void* q, const void* k, const void* qw, const void* kw, const float* cos,
+                     const float* sin, const int32_t* positions, const int64_t* sq, const int64_t* sk, int64_t pos_stride,
+                     int64_t Z, int64_t H, int64_t Hk, int64_t N, int64_t D, int64_t P, int dtype, int w_dtype, float eps) {
+  int rc;
+  if (dtype != TATTN_F16 && dtype != TATTN_F32 && dtype != TATTN_BF16) return set_error(TATTN_E_ARG, "unknown dtype %d", dtype);
+  if (w_dtype != dtype && w_dtype != TATTN_F32) return set_error(TATTN_E_ARG, "weights must be of the tensors' dtype or float32");
+  if (D != 16 && D != 32 && D != 64 && D != 128)
+    return set_error(TATTN_E_ARG, "head dim must be 16, 32, 64 or 128, got %lld", (long long)D);
+  if ((rc = check_count("batch", Z)) || (rc = check_count("heads", H)) || (rc = check_count("key heads", Hk)) ||
+      (rc = check_count("length", N)) || (rc = check_count("table rows", P)))
+    return rc;
+  if (H < 1 || Hk < 1) return set_error(TATTN_E_ARG, "heads must be positive, got %lld and %lld", (long long)H, (long long)Hk);
+  p.per_q = (uint32_t)((H + 3) / 4);
+  p.per_k = (uint32_t)((Hk + 3) / 4);
+  if (Z > 0 && N > 0 && (double)Z * (double)N * (double)(p.per_q + p.per_k) >= 2147483648.0)
+    return set_error(TATTN_E_ARG, "too many tokens: %lld x %lld with %lld + %lld heads", (long long)Z, (long long)N,
+                     (long long)H, (long long)Hk);
+  const int64_t rows = Z * N;
+  const int sz = dtype == TATTN_F32 ? 4 : 2;
+  if ((rc = check_ptr("q", q, rows, 16)) || (rc = check_ptr("k", k, rows, 16)) || (rc = check_ptr("q_weight", qw, 1, 16)) ||
+      (rc = check_ptr("k_weight", kw, 1, 16)) || (rc = check_ptr("cos", cos, P, 16)) || (rc = check_ptr("sin", sin, P, 16)) ||
+      (rc = check_ptr("positions", positions, 0, 4)) || (rc = check_rows("q", sq, 3, sz)) || (rc = check_rows("k", sk, 3, sz)))
+    return rc;
+  if (rows > 0 && P < 1) return set_error(TATTN_E_ARG, "cos and sin have no rows");
+  p.q = q; p.k = k; p.qw = qw; p.kw = kw; p.cos = cos; p.sin = sin; p.positions = positions;
+  for (int i = 0; i < 3; ++i) p.sq[i] = sq[i], p.sk[i] = sk[i];
+  p.pos_stride = pos_stride;
+  p.Z = (int32_t)Z; p.H = (int32_t)H; p.Hk = (int32_t)Hk; p.N = (int32_t)N; p.P = (int32_t)P;
+  p.wide_w = dtype != TATTN_F32 && w_dtype == TATTN_F32;
+  p.eps = eps;
+  p.units_q = (uint32_t)rows * p.per_q;
+  p.units_k = (uint32_t)rows * p.per_k;
+  return TATTN_OK;
+}
+
 }  // namespace
 }  // namespace tattn
 
@@ -112,6 +148,61 @@ int tattn_cache4_read(const uint8_t* codes, const uint8_t* scales, void* k, void
   if (T == 0 || H == 0) return TATTN_OK;
   p.ko = k; p.vo = v;
   return launch_cache4_read(p, (int)D, dtype, (hipStream_t)stream);
+}
+
+int tattn_norm_rope_fwd(const void* q, const void* k, const void* q_weight, const void* k_weight, const float* cos,
+                        const float* sin, const int32_t* positions, void* q_out, void* k_out, const int64_t q_strides[4],
+                        const int64_t k_strides[4], const int64_t qo_strides[4], const int64_t ko_strides[4],
+                        int64_t pos_stride, int64_t Z, int64_t H, int64_t Hk, int64_t N, int64_t D, int64_t P, int dtype,
+                        int w_dtype, int interleaved, float eps, void* stream) {
+  NormRopeParams p{};
+  int rc;
+  if ((rc = norm_rope_common(p, q, k, q_weight, k_weight, cos, sin, positions, q_strides, k_strides, pos_stride, Z, H, Hk,
+                             N, D, P, dtype, w_dtype, eps)))
+    return rc;
+  const int sz = dtype == TATTN_F32 ? 4 : 2;
+  if ((rc = check_ptr("q_out", q_out, Z * N, 16)) || (rc = check_ptr("k_out", k_out, Z * N, 16)) ||
+      (rc = check_rows("q_out", qo_strides, 3, sz)) || (rc = check_rows("k_out", ko_strides, 3, sz)) || (rc = require_device()))
+    return rc;
+  if (Z == 0 || N == 0) return TATTN_OK;
+  p.qo = q_out; p.ko = k_out;
+  for (int i = 0; i < 3; ++i) p.sqo[i] = qo_strides[i], p.sko[i] = ko_strides[i];
+  return launch_norm_rope(p, (int)D, dtype, interleaved != 0, false, (hipStream_t)stream);
+}
+
+int tattn_norm_rope_bwd(const void* q, const void* k, const void* q_weight, const void* k_weight, const float* cos,
+                        const float* sin, const int32_t* positions, const void* dq_out, const void* dk_out, void* dq,
+                        void* dk, void* dq_weight, void* dk_weight, float* workspace, const int64_t q_strides[4],
+                        const int64_t k_strides[4], const int64_t dqo_strides[4], const int64_t dko_strides[4],
+                        const int64_t dq_strides[4], const int64_t dk_strides[4], int64_t pos_stride, int64_t Z, int64_t H,
+                        int64_t Hk, int64_t N, int64_t D, int64_t P, int dtype, int w_dtype, int interleaved, float eps,
+                        void* stream) {
+  NormRopeParams p{};
+  int rc;
+  if ((rc = norm_rope_common(p, q, k, q_weight, k_weight, cos, sin, positions, q_strides, k_strides, pos_stride, Z, H, Hk,
+                             N, D, P, dtype, w_dtype, eps)))
+    return rc;
+  const int sz = dtype == TATTN_F32 ? 4 : 2;
+  const int64_t rows = Z * N;
+  if ((rc = check_ptr("dq_out", dq_out, rows, 16)) || (rc = check_ptr("dk_out", dk_out, rows, 16)) ||
+      (rc = check_ptr("dq", dq, rows, 16)) || (rc = check_ptr("dk", dk, rows, 16)) ||
+      (rc = check_rows("dq_out", dqo_strides, 3, sz)) || (rc = check_rows("dk_out", dko_strides, 3, sz)) ||
+      (rc = check_rows("dq", dq_strides, 3, sz)) || (rc = check_rows("dk", dk_strides, 3, sz)))
+    return rc;
+  if (workspace) {
+    if ((rc = check_ptr("dq_weight", dq_weight, 1, 2)) || (rc = check_ptr("dk_weight", dk_weight, 1, 2)) ||
+        (rc = check_ptr("workspace", workspace, 1, 16)))
+      return rc;
+  } else if (dq_weight || dk_weight) {
+    return set_error(TATTN_E_ARG, "weight gradients need the workspace");
+  }
+  if ((rc = require_device())) return rc;
+  if (rows == 0) return TATTN_OK;
+  p.gq = dq_out; p.gk = dk_out; p.qo = dq; p.ko = dk; p.dqw = dq_weight; p.dkw = dk_weight; p.partial = workspace;
+  for (int i = 0; i < 3; ++i) {
+    p.sqo[i] = dq_strides[i]; p.sko[i] = dk_strides[i]; p.sgq[i] = dqo_strides[i]; p.sgk[i] = dko_strides[i];
+  }
+  return launch_norm_rope(p, (int)D, dtype, interleaved != 0, true, (hipStream_t)stream);
 }
 
 }  // extern "C"

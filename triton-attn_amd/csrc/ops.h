@@ -44,4 +44,32 @@ struct Cache4Params {
 int launch_cache4_write(const Cache4Params& p, int D, int dtype, hipStream_t st);
 int launch_cache4_read(const Cache4Params& p, int D, int dtype, hipStream_t st);
 
+// Norm and rotation of q [Z, H, N, D] and k [Z, Hk, N, D]; strides (z, h, n) in elements, unit d stride.
+constexpr int kNormRopeRows = 512;  // most workgroups of the backward: rows of its workspace
+struct NormRopeParams {
+  const void* q;
+  const void* k;
+  const void* qw;
+  const void* kw;
+  const float* cos;  // [P, D / 2]
+  const float* sin;
+  const int32_t* positions;  // [N] or [Z, N]; null: n
+  const void* gq;            // backward: gradients of the outputs
+  const void* gk;
+  void* qo;  // outputs; backward: gradients of q and k
+  void* ko;
+  void* dqw;
+  void* dkw;
+  float* partial;  // [kNormRopeRows, D]; null: no weight gradients
+  int64_t sq[3], sk[3], sqo[3], sko[3], sgq[3], sgk[3];
+  int64_t pos_stride;  // of z
+  int32_t Z, H, Hk, N, P;
+  int32_t wide_w;  // weights are float32 (else the tensors' type)
+  float eps;
+  uint32_t per_q, per_k;      // lane groups' work units per token
+  uint32_t units_q, units_k;
+  int32_t blocks_q, blocks_k;
+};
+int launch_norm_rope(const NormRopeParams& p, int D, int dtype, bool interleaved, bool bwd, hipStream_t st);
+
 }  // namespace tattn

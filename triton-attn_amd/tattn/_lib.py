@@ -25,11 +25,15 @@ EXPORTS = (
     "tattn_bwd_preprocess", "tattn_bwd_dkdv", "tattn_bwd_dq", "tattn_bwd", "tattn_bwd_layouts", "tattn_bwd_noalloc",
     "tattn_num_configs", "tattn_config_desc", "tattn_pick_config", "tattn_picked",
     "tattn_page_tables", "tattn_cache4_write", "tattn_cache4_read",
+    "tattn_norm_rope_fwd", "tattn_norm_rope_bwd",
 )
 
 # Kernels outside the tables, as `picked` reports them.
 PICK_COOP, PICK_PLANES, PICK_SHORT = 1000, 1001, 1002
 PICK_NAMES = {PICK_COOP: "coop", PICK_PLANES: "planes", PICK_SHORT: "short"}
+
+
+NORM_ROPE_ROWS = 512  # TATTN_NORM_ROPE_ROWS
 
 
 class TattnConfig(ctypes.Structure):
@@ -71,6 +75,8 @@ _SIGS = {
     "tattn_page_tables": (_I, [_P] * 8 + [_I64] * 6 + [_P]),
     "tattn_cache4_write": (_I, [_P] * 5 + [_STR4, _STR4] + [_I64] * 5 + [_I, _P]),
     "tattn_cache4_read": (_I, [_P] * 5 + [_I64] * 5 + [_I, _P]),
+    "tattn_norm_rope_fwd": (_I, [_P] * 9 + [_STR4] * 4 + [_I64] * 7 + [_I, _I, _I, _F, _P]),
+    "tattn_norm_rope_bwd": (_I, [_P] * 14 + [_STR4] * 6 + [_I64] * 7 + [_I, _I, _I, _F, _P]),
 }
 
 _lib: ctypes.CDLL | None = None
@@ -134,6 +140,18 @@ def stride_block(*ts: torch.Tensor):
         arr = (ctypes.c_int64 * (4 * len(ts)))(*(s for st in key for s in st))
         base = ctypes.addressof(arr)
         hit = _stride_blocks[key] = (arr, [base + 32 * i for i in range(len(ts))])
+    return hit
+
+
+def stride_rows(key: tuple) -> tuple:
+    """The same for tuples of up to four strides (missing ones are 0)."""
+    hit = _stride_blocks.get(key)
+    if hit is None:
+        if len(_stride_blocks) > 1024:
+            _stride_blocks.clear()
+        arr = (ctypes.c_int64 * (4 * len(key)))(*(s for st in key for s in (*st, 0, 0, 0, 0)[:4]))
+        base = ctypes.addressof(arr)
+        hit = _stride_blocks[key] = (arr, [base + 32 * i for i in range(len(key))])
     return hit
 
 

@@ -11,29 +11,17 @@ the cache is skipped, as documented per call.
 
 from __future__ import annotations
 
-import ctypes
 from typing import NamedTuple
 
 import torch
 
 from tattn import _lib
+from tattn._args import check_index, rows, same_device, strides
 from tattn.api import _on_device, _require_gpu, _stream
 
 _DTYPES = {torch.float16: _lib.F16, torch.bfloat16: _lib.BF16}
 
 PAGE_SIZES = (16, 32, 64, 128, 256, 512, 1024)
-
-
-def _same_device(first: torch.Tensor, **others: torch.Tensor) -> None:
-    for name, t in others.items():
-        if t.device != first.device:
-            raise ValueError(f"{name} must be on {first.device}, got {t.device}")
-
-
-def _check_index(name: str, t: torch.Tensor, dtype: torch.dtype, shape: tuple) -> None:
-    if t.dtype != dtype or tuple(t.shape) != shape:
-        raise ValueError(f"{name} must be {str(dtype).removeprefix('torch.')} of shape {list(shape)}, "
-                         f"got {str(t.dtype).removeprefix('torch.')} {list(t.shape)}")
 
 
 def _check_page_size(page_size: int) -> None:
@@ -61,10 +49,10 @@ def page_tables(lens: torch.Tensor, new_tokens: torch.Tensor, tables: torch.Tens
     if lens.dim() != 1 or lens.dtype != torch.int32:
         raise ValueError(f"lens must be int32 [requests], got {lens.dtype} {list(lens.shape)}")
     r = lens.shape[0]
-    _check_index("new_tokens", new_tokens, torch.int32, (r,))
+    check_index("new_tokens", new_tokens, torch.int32, (r,))
     if tables.dim() != 2:
         raise ValueError(f"tables must be int32 [requests, width], got {list(tables.shape)}")
-    _check_index("tables", tables, torch.int32, (r, tables.shape[1]))
+    check_index("tables", tables, torch.int32, (r, tables.shape[1]))
     if free_pages.dim() != 1 or free_pages.dtype != torch.int32:
         raise ValueError(f"free_pages must be int32 [pages], got {free_pages.dtype} {list(free_pages.shape)}")
     if tables.numel() and ((tables.shape[1] > 1 and tables.stride(1) != 1) or (r > 1 and tables.stride(0) < tables.shape[1])):
@@ -72,7 +60,7 @@ def page_tables(lens: torch.Tensor, new_tokens: torch.Tensor, tables: torch.Tens
     _check_page_size(page_size)
     if not 0 <= tokens < (1 << 31) - 4096:
         raise ValueError(f"tokens out of range: {tokens}")
-    _same_device(lens, new_tokens=new_tokens, tables=tables, free_pages=free_pages)
+    same_device(lens, new_tokens=new_tokens, tables=tables, free_pages=free_pages)
     _require_gpu(lens)
     lens, new_tokens, free_pages = lens.contiguous(), new_tokens.contiguous(), free_pages.contiguous()
     slots = lens.new_empty(tokens, dtype=torch.int64)
@@ -102,11 +90,11 @@ class Cache4:
         pages, heads, _, page, half = codes.shape
         if 2 * half not in (32, 64, 128):
             raise ValueError(f"head dim must be 32, 64 or 128, got {2 * half}")
-        _check_index("scales", scales, torch.uint8, (pages, heads, 2, page, half // 16))
+        check_index("scales", scales, torch.uint8, (pages, heads, 2, page, half // 16))
         _check_page_size(page)
         if dtype not in _DTYPES:
             raise ValueError(f"dtype must be float16 or bfloat16, got {dtype}")
-        _same_device(codes, scales=scales)
+        same_device(codes, scales=scales)
         if not (codes.is_contiguous() and scales.is_contiguous()) or codes.data_ptr() % 16 or scales.data_ptr() % 4:
             raise ValueError("codes and scales must be contiguous, codes 16-byte and scales 4-byte aligned")
         self.codes, self.scales, self.dtype = codes, scales, dtype
@@ -121,13 +109,6 @@ class Cache4:
                    torch.zeros((*shape, head_dim // 32), dtype=torch.uint8, device=device), dtype)
 
 
-def _rows(t: torch.Tensor) -> torch.Tensor:
-    """t itself where the kernels read its rows (unit d stride, 16-byte aligned), else an aligned contiguous copy."""
-    if t.stride(-1) == 1 and t.data_ptr() % 16 == 0 and all(s % 8 == 0 and s >= 0 for s in t.stride()[:-1]):
-        return t
-    return t.clone(memory_format=torch.contiguous_format)
-
-
 def cache4_write(cache: Cache4, k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor) -> None:
     """Writes keys and values [tokens, kv_heads, head_dim] (the cache's dtype, any token and head strides) into
     `slots` (int64 [tokens], as page_tables gives them). Slots outside the cache, such as a padded token's -1,
@@ -136,15 +117,14 @@ def cache4_write(cache: Cache4, k: torch.Tensor, v: torch.Tensor, slots: torch.T
         raise ValueError(f"expected k, v of shape [tokens, {cache.kv_heads}, {cache.head_dim}]; got {list(k.shape)}, {list(v.shape)}")
     if k.dtype != cache.dtype or v.dtype != cache.dtype:
         raise ValueError(f"k and v must have the cache's dtype {cache.dtype}, got {k.dtype}, {v.dtype}")
-    _check_index("slots", slots, torch.int64, (k.shape[0],))
-    _same_device(cache.codes, k=k, v=v, slots=slots)
+    check_index("slots", slots, torch.int64, (k.shape[0],))
+    same_device(cache.codes, k=k, v=v, slots=slots)
     _require_gpu(k)
-    k, v, slots = _rows(k), _rows(v), slots.contiguous()
-    strides = (ctypes.c_int64 * 4)(*k.stride()[:2], *v.stride()[:2])
-    at = ctypes.addressof(strides)
+    k, v, slots = rows(k), rows(v), slots.contiguous()
+    _, st = strides(k, v)
     with _on_device(k):
         rc = _lib.load().tattn_cache4_write(
-            cache.codes.data_ptr(), cache.scales.data_ptr(), k.data_ptr(), v.data_ptr(), slots.data_ptr(), at, at + 16,
+            cache.codes.data_ptr(), cache.scales.data_ptr(), k.data_ptr(), v.data_ptr(), slots.data_ptr(), *st,
             k.shape[0], cache.kv_heads, cache.head_dim, cache.pages, cache.page_size, _DTYPES[cache.dtype], _stream(k))
     _lib.check(rc, "tattn_cache4_write")
 
@@ -154,8 +134,8 @@ def cache4_read(cache: Cache4, slots: torch.Tensor) -> tuple[torch.Tensor, torch
     outside it. For prompts that continue a cached prefix, and to see what 4 bits made of a tensor."""
     if slots.dim() != 1:
         raise ValueError(f"slots must be int64 [tokens], got {list(slots.shape)}")
-    _check_index("slots", slots, torch.int64, (slots.shape[0],))
-    _same_device(cache.codes, slots=slots)
+    check_index("slots", slots, torch.int64, (slots.shape[0],))
+    same_device(cache.codes, slots=slots)
     _require_gpu(slots)
     slots = slots.contiguous()
     shape = (slots.shape[0], cache.kv_heads, cache.head_dim)
