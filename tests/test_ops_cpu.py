@@ -190,3 +190,65 @@ def test_norm_rope_workspace_rows_match_the_header():
     from test_abi import HEADER
 
     assert f"#define TATTN_NORM_ROPE_ROWS {_lib.NORM_ROPE_ROWS}" in HEADER.read_text()
+
+
+# ---- window_attention ----------------------------------------------------------------------------
+
+def _window(**kw):
+    a = dict(q=torch.zeros(2, 4, 8, 32).half(), k=torch.zeros(2, 2, 8, 32).half(), v=torch.zeros(2, 2, 8, 32).half(), window=4)
+    a.update(kw)
+    return tattn.window_attention(**a)
+
+
+@pytest.mark.parametrize("bad,msg", [
+    (dict(q=torch.zeros(4, 8, 32).half()), "expected q"),
+    (dict(v=torch.zeros(2, 2, 9, 32).half()), "expected q"),
+    (dict(q=torch.zeros(1, 4, 8, 32).half()), "expected q"),
+    (dict(q=torch.zeros(2, 3, 8, 32).half()), "multiple of kv heads"),
+    (dict(q=torch.zeros(2, 4, 9, 32).half()), "9 queries for 8 keys"),
+    (dict(q=torch.zeros(2, 4, 8, 48).half(), k=torch.zeros(2, 2, 8, 48).half(), v=torch.zeros(2, 2, 8, 48).half()), "head dim"),
+    (dict(q=torch.zeros(2, 4, 8, 32)), "dtype"),
+    (dict(window=0), "window must be positive"),
+    (dict(sinks=-1), "sinks not negative"),
+    (dict(lens=torch.zeros(2, dtype=torch.int64)), "lens must be int32"),
+    (dict(lens=torch.zeros(3, dtype=torch.int32)), "lens must be int32"),
+    (dict(lens=torch.zeros(2, dtype=torch.int32, device="meta")), "lens must be on"),
+    (dict(lens=torch.zeros(2, dtype=torch.int32), q=torch.zeros(2, 4, 8, 32).half().requires_grad_()), "no gradients with lens"),
+])
+def test_window_attention_refuses(bad, msg):
+    with pytest.raises(ValueError, match=msg):
+        _window(**bad)
+
+
+def test_window_attention_has_no_cpu_path():
+    with pytest.raises(RuntimeError, match="gfx950"):
+        _window()
+
+
+@pytest.mark.parametrize("bad,msg", [
+    (dict(D=48), "head dim"), (dict(dtype=_lib.F32), "dtype"), (dict(Hk=3), "evenly"), (dict(S=7), "8 queries for 7 keys"),
+    (dict(window=0), "window must be positive"), (dict(sinks=-1), "sinks must not be negative"), (dict(N=0), "positive"),
+    (dict(k=None), "k is a null pointer"), (dict(v=8), "v must be 16-byte aligned"),
+    (dict(ks=(ctypes.c_int64 * 4)(512, 256, 16, 1)), "k rows overlap"), (dict(ks=(ctypes.c_int64 * 4)(512, 256, 36, 1)), "multiple of"),
+    (dict(ks=(ctypes.c_int64 * 4)(512, 256, 1 << 25, 1)), "2 GiB"), (dict(os=None), "o strides are null"),
+    (dict(Z=1 << 20, H=1 << 20, Hk=1), "too many rows"),
+])
+def test_window_entry_point_refuses(bad, msg):
+    st = (ctypes.c_int64 * 4)(1024, 256, 32, 1)
+    a = dict(q=16, k=16, v=16, o=16, m=None, lens=None, work=None, qs=st, ks=st, vs=st, os=st, Z=2, H=4, Hk=2, N=8, S=8, D=32,
+             window=4, sinks=0, dtype=_lib.F16, scale=0.1, stream=None)
+    a.update(bad)
+    assert _lib.load().tattn_window_fwd(*a.values()) == 1
+    assert msg in _lib.last_error()
+
+
+def test_window_workspace_is_asked_for_where_keys_are_split():
+    lib, n = _lib.load(), ctypes.c_int64(-1)
+    assert lib.tattn_window_workspace(0, 64, 32, 8, 4096, 4096, 64, 1024, 4, ctypes.byref(n)) == 0 and n.value == 0
+    assert lib.tattn_window_workspace(0, 1, 8, 2, 1, 8192, 64, 8192, 0, ctypes.byref(n)) == 0 and n.value > 0
+    st = (ctypes.c_int64 * 4)(1 << 20, 1 << 19, 64, 1)
+    assert lib.tattn_window_fwd(16, 16, 16, 16, None, None, None, st, st, st, st, 1, 8, 2, 1, 8192, 64, 8192, 0, _lib.F16, 0.1, None) == 1
+    assert "workspace is a null pointer" in _lib.last_error()
+    assert lib.tattn_window_workspace(1, 1, 8, 2, 16384, 16384, 64, 128, 4, ctypes.byref(n)) == 0 and n.value > 0
+    assert lib.tattn_window_workspace(1, 1, 8, 2, 16384, 16384, 64, 128, 0, ctypes.byref(n)) == 0 and n.value == 0
+    assert lib.tattn_window_workspace(1, 1, 8, 2, 16384, 100, 64, 128, 0, ctypes.byref(n)) == 1

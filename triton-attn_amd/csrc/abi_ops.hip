@@ -95,6 +95,47 @@ int norm_rope_common(NormRopeParams& p, const void* q, const void* k, const void
   return TATTN_OK;
 }
 
+// Window attention: sizes, window and first keys.
+int window_common(WindowParams& p, int64_t Z, int64_t H, int64_t Hk, int64_t N, int64_t S, int64_t D, int64_t window,
+                  int64_t sinks, bool lens) {
+  int rc;
+  if (D != 16 && D != 32 && D != 64 && D != 128)
+    return set_error(TATTN_E_ARG, "head dim must be 16, 32, 64 or 128, got %lld", (long long)D);
+  if ((rc = check_count("batch", Z)) || (rc = check_count("heads", H)) || (rc = check_count("length", N)) ||
+      (rc = check_count("key length", S)))
+    return rc;
+  if (Z < 1 || H < 1 || N < 1 || S < 1) return set_error(TATTN_E_ARG, "sizes must be positive");
+  if (Hk < 1 || H % Hk) return set_error(TATTN_E_ARG, "%lld heads do not share %lld key heads evenly", (long long)H, (long long)Hk);
+  if (!lens && S < N) return set_error(TATTN_E_ARG, "%lld queries for %lld keys", (long long)N, (long long)S);
+  if (window < 1) return set_error(TATTN_E_ARG, "window must be positive, got %lld", (long long)window);
+  if (sinks < 0) return set_error(TATTN_E_ARG, "sinks must not be negative, got %lld", (long long)sinks);
+  if ((double)H * (double)N > 1073741824.0 || (double)Z * (double)H * (double)((N + 31) / 32) > 67108864.0)
+    return set_error(TATTN_E_ARG, "too many rows: %lld x %lld x %lld", (long long)Z, (long long)H, (long long)N);
+  p.Z = (int32_t)Z; p.H = (int32_t)H; p.Hk = (int32_t)Hk; p.G = (int32_t)(H / Hk); p.N = (int32_t)N; p.S = (int32_t)S;
+  p.window = (int32_t)(window < S ? window : S);
+  p.sinks = (int32_t)(sinks < S ? sinks : S);
+  return TATTN_OK;
+}
+
+// A tensor that the kernels read in tiles of 32 rows: strides (z, h, n), rows that do not overlap, slices that 31-bit
+// byte offsets span with a step's rows to spare. A dimension of one row gets the stride of whole rows.
+int check_tiles(const char* name, const void* ptr, const int64_t* st, int64_t rows, int64_t D, int64_t (&out)[3]) {
+  int rc;
+  if ((rc = check_ptr(name, ptr, 1, 16)) || (rc = check_rows(name, st, 3, 2))) return rc;
+  for (int i = 0; i < 3; ++i) out[i] = st[i];
+  if (rows == 1) out[2] = D;
+  if (out[2] < D) return set_error(TATTN_E_ARG, "%s rows overlap: stride %lld", name, (long long)out[2]);
+  if (out[2] > (1ll << 24) || (rows + 256) * out[2] * 2 >= 0x7fffff00ll)
+    return set_error(TATTN_E_ARG, "a head of %s spans 2 GiB or more", name);
+  return TATTN_OK;
+}
+
+int check_16bit(int dtype) {
+  if (dtype != TATTN_F16 && dtype != TATTN_BF16)
+    return set_error(TATTN_E_ARG, "dtype must be TATTN_F16 or TATTN_BF16, got %d", dtype);
+  return TATTN_OK;
+}
+
 }  // namespace
 }  // namespace tattn
 
@@ -203,6 +244,66 @@ int tattn_norm_rope_bwd(const void* q, const void* k, const void* q_weight, cons
     p.sqo[i] = dq_strides[i]; p.sko[i] = dk_strides[i]; p.sgq[i] = dqo_strides[i]; p.sgk[i] = dko_strides[i];
   }
   return launch_norm_rope(p, (int)D, dtype, interleaved != 0, true, (hipStream_t)stream);
+}
+
+int tattn_window_workspace(int backward, int64_t Z, int64_t H, int64_t Hk, int64_t N, int64_t S, int64_t D, int64_t window,
+                           int64_t sinks, int64_t* floats) {
+  WindowParams p{};
+  int rc;
+  if (!floats) return set_error(TATTN_E_ARG, "floats is a null pointer");
+  if ((rc = window_common(p, Z, H, Hk, N, S, D, window, sinks, !backward))) return rc;
+  if (backward) {
+    *floats = window_bwd_part_floats(p, (int)D);
+  } else {
+    const int splits = window_fwd_splits(p);
+    *floats = splits > 1 ? window_part_floats(Z * Hk, N * p.G, splits, D) : 0;
+  }
+  return TATTN_OK;
+}
+
+int tattn_window_fwd(const void* q, const void* k, const void* v, void* o, float* m, const int32_t* lens, float* workspace,
+                     const int64_t q_strides[4], const int64_t k_strides[4], const int64_t v_strides[4],
+                     const int64_t o_strides[4], int64_t Z, int64_t H, int64_t Hk, int64_t N, int64_t S, int64_t D,
+                     int64_t window, int64_t sinks, int dtype, float sm_scale, void* stream) {
+  WindowParams p{};
+  int rc;
+  if ((rc = window_common(p, Z, H, Hk, N, S, D, window, sinks, lens != nullptr)) || (rc = check_16bit(dtype)) ||
+      (rc = check_tiles("q", q, q_strides, N, D, p.sq)) || (rc = check_tiles("k", k, k_strides, S, D, p.sk)) ||
+      (rc = check_tiles("v", v, v_strides, S, D, p.sv)) || (rc = check_tiles("o", o, o_strides, N, D, p.sout)) ||
+      (rc = check_ptr("m", m, 0, 4)) || (rc = check_ptr("lens", lens, 0, 4)))
+    return rc;
+  p.splits = window_fwd_splits(p);
+  if ((rc = check_ptr("workspace", workspace, p.splits > 1, 16)) || (rc = require_device())) return rc;
+  p.q = q; p.k = k; p.v = v; p.out = o; p.m = m; p.lens = lens; p.part = workspace;
+  p.c = sm_scale * kLog2e;
+  p.scale = sm_scale;
+  return launch_window_fwd(p, (int)D, dtype, (hipStream_t)stream);
+}
+
+int tattn_window_bwd(const void* q, const void* k, const void* v, const void* o, const void* dout, void* dq, void* dk,
+                     void* dv, const float* m, float* delta, float* workspace, const int64_t q_strides[4],
+                     const int64_t k_strides[4], const int64_t v_strides[4], const int64_t o_strides[4],
+                     const int64_t do_strides[4], const int64_t dq_strides[4], const int64_t dk_strides[4],
+                     const int64_t dv_strides[4], int64_t Z, int64_t H, int64_t Hk, int64_t N, int64_t S, int64_t D,
+                     int64_t window, int64_t sinks, int dtype, float sm_scale, void* stream) {
+  WindowParams p{};
+  int rc;
+  if ((rc = window_common(p, Z, H, Hk, N, S, D, window, sinks, false)) || (rc = check_16bit(dtype)) ||
+      (rc = check_tiles("q", q, q_strides, N, D, p.sq)) || (rc = check_tiles("k", k, k_strides, S, D, p.sk)) ||
+      (rc = check_tiles("v", v, v_strides, S, D, p.sv)) || (rc = check_tiles("o", o, o_strides, N, D, p.so)) ||
+      (rc = check_tiles("do", dout, do_strides, N, D, p.sd)) || (rc = check_tiles("dq", dq, dq_strides, N, D, p.sout)) ||
+      (rc = check_tiles("dk", dk, dk_strides, S, D, p.sdk)) || (rc = check_tiles("dv", dv, dv_strides, S, D, p.sdv)) ||
+      (rc = check_ptr("m", m, 1, 4)) || (rc = check_ptr("delta", delta, 1, 4)))
+    return rc;
+  p.splits = window_bwd_splits(p, (int)D);
+  if ((rc = check_ptr("workspace", workspace, p.splits > 1, 16)) || (rc = require_device())) return rc;
+  p.q = q; p.k = k; p.v = v; p.o = o; p.dout = dout; p.out = dq; p.dk = dk; p.dv = dv;
+  p.m = const_cast<float*>(m);
+  p.delta = delta;
+  p.part = workspace;
+  p.c = sm_scale * kLog2e;
+  p.scale = sm_scale;
+  return launch_window_bwd(p, (int)D, dtype, (hipStream_t)stream);
 }
 
 }  // extern "C"

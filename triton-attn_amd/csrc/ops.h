@@ -72,4 +72,40 @@ struct NormRopeParams {
 };
 int launch_norm_rope(const NormRopeParams& p, int D, int dtype, bool interleaved, bool bwd, hipStream_t st);
 
+// Attention over a window and the first keys (window.h). q, o, do, dq: [Z, H, N, D]; k, v, dk, dv: [Z, Hk, S, D].
+struct WindowParams {
+  const void* q;
+  const void* k;
+  const void* v;
+  const void* o;  // backward: the forward's output
+  const void* dout;
+  void* out;  // forward: O; backward: dQ
+  void* dk;
+  void* dv;
+  float* m;      // [Z, H, N] base-2 log-sum-exp, or null
+  float* delta;  // [Z, H, N]
+  const int32_t* lens;  // [Z] keys of each sequence, or null: S
+  float* part;          // partial rows of a split forward, see window_part_floats; partial dK, dV of the first keys
+  int64_t sq[3], sk[3], sv[3], so[3], sd[3], sout[3], sdk[3], sdv[3];
+  int32_t Z, H, Hk, G, N, S;
+  int32_t window, sinks;
+  int32_t nblk;
+  int32_t splits;  // forward: parts of a row's keys; backward: parts of the first keys' queries
+  int32_t runs;    // window_coord
+  float c, scale;
+};
+
+// Partial rows of a forward split `splits` ways: for each split and row D sums, then its max and sum.
+inline int64_t window_part_floats(int64_t slices, int64_t rows, int64_t splits, int64_t D) {
+  return slices * rows * splits * (D + 2);
+}
+int window_fwd_splits(const WindowParams& p);  // 0: no parts and two row tiles per workgroup
+int window_bwd_splits(const WindowParams& p, int D);
+int64_t window_bwd_part_floats(const WindowParams& p, int D);
+int launch_window_fwd(WindowParams p, int D, int dtype, hipStream_t st);
+int launch_window_bwd(WindowParams p, int D, int dtype, hipStream_t st);
+// O of rows whose keys were split: part as laid out above, out [slices / Hk, H, N, D] with strides (z, h, n).
+int launch_combine(const float* part, void* out, float* m, const int64_t so[3], int64_t slices, int Hk, int G, int N,
+                   int splits, int D, int dtype, hipStream_t st);
+
 }  // namespace tattn

@@ -1,0 +1,77 @@
+// Window attention: parameters, and device code shared by its kernels and the one over the 4-bit cache.
+//
+// Query n of sequence z is at position p = len_z - N + n and sees key j if j <= p and (p - j < window or
+// j < sinks). The G query heads of one key head share its keys: their rows are laid one after the other, row
+// R = n * G + g, so that a 32-row tile holds whole queries with all their heads where G allows. A tile then spans 32 / G
+// positions, which trims the masked ends of its window, and a single token's heads fill one tile.
+#pragma once
+
+#include "bwd_pipe.h"
+#include "common.h"
+#include "ops.h"
+
+namespace tattn {
+
+// Score below every score: the running max before the first visible key. Finite, so that rescaling a
+// sum that holds nothing yet multiplies by 0 and never subtracts infinities.
+constexpr float kNoMax = -3.0e38f;
+
+// The key tiles (32 keys) that rows at positions [p0, p1] see: the tiles of the first `sinks` keys, then those of
+// the window.
+struct TileList {
+  int lo;     // first key of the window
+  int sink_tiles, first, n;
+  __device__ __forceinline__ void init(int p0, int p1, int window, int sinks) {
+    lo = max(0, p0 - window + 1);
+    first = lo >> 5;
+    sink_tiles = min((min(sinks, lo) + 31) >> 5, first);
+    n = p1 < 0 ? 0 : sink_tiles + (p1 >> 5) - first + 1;
+  }
+  __device__ __forceinline__ int at(int i) const { return i < sink_tiles ? i : i - sink_tiles + first; }
+};
+
+// What a lane's row at position p hides in a tile: register r of lane-half h2 is key 32 t + 8 h2 + 16 (r / 8) + r % 8.
+struct RowMask {
+  int hi, lb, sk;
+  __device__ __forceinline__ RowMask(int p, int t, int h2, int window, int sinks) {
+    const int base = 32 * t + 8 * h2;
+    hi = p - base;
+    lb = hi - window + 1;
+    sk = sinks - base;
+  }
+  __device__ __forceinline__ bool hides(int r) const {
+    const int off = 16 * (r >> 3) + (r & 7);
+    return off > hi || (off < lb && off >= sk);
+  }
+};
+
+// Whether rows at positions [p0, p1] see nothing of tile t, or all of it.
+__device__ __forceinline__ bool tile_hidden(int p0, int p1, int t, int window, int sinks) {
+  return 32 * t > p1 || (32 * t + 31 < p0 - window + 1 && 32 * t >= sinks);
+}
+__device__ __forceinline__ bool tile_masked(int p0, int p1, int t, int window, int sinks) {
+  return 32 * t + 31 > p0 || (32 * t < p1 - window + 1 && 32 * t + 31 >= sinks);
+}
+
+// Everything this wave has in flight has landed, its LDS reads are done, then the barrier.
+__device__ __forceinline__ void all_landed_barrier() {
+  __builtin_amdgcn_s_waitcnt(0x0070);  // vmcnt(0), lgkmcnt(0)
+  __atomic_signal_fence(__ATOMIC_SEQ_CST);
+  __builtin_amdgcn_s_barrier();
+  __atomic_signal_fence(__ATOMIC_SEQ_CST);
+}
+
+// Workgroup -> (slice, block); false past the last. Workgroups go round-robin over the 8 XCDs. runs: an XCD takes
+// consecutive blocks, which read overlapping keys through its L2; else consecutive workgroups take consecutive slices.
+__device__ __forceinline__ bool window_coord(int slices, int nblk, bool runs, int& slice, int& blk) {
+  const int64_t total = (int64_t)slices * nblk;
+  int64_t i = blockIdx.x;
+  if (runs) i = (i & 7) * ((total + 7) >> 3) + (i >> 3);
+  if (i >= total) return false;
+  if (!runs) i = (i % slices) * nblk + i / slices;
+  slice = (int)(i / nblk);
+  blk = (int)(i % nblk);
+  return true;
+}
+
+}  // namespace tattn
