@@ -253,6 +253,21 @@ int tattn_window_bwd(const void* q, const void* k, const void* v, const void* o,
                      const int64_t dv_strides[4], int64_t Z, int64_t H, int64_t Hk, int64_t N, int64_t S, int64_t D,
                      int64_t window, int64_t sinks, int dtype, float sm_scale, void* stream);
 
+/*
+ * Attention of one token per request over the cache in 4 bits: q, o [R, H, D] with (request, head) strides in elements, H a
+ * multiple of the cache's Hk heads (head h reads key head h / (H / Hk)), D = 32, 64 or 128, dtype of the cache's values.
+ * Request r sees its first lens[r] tokens (clamped to [0, width * page_size]) through tables[r * table_stride ..]
+ * (width pages); with a window (0: none) only the last `window` of them and the first `sinks`. Pages that no visible token
+ * lies in are not looked up; tokens on a page outside [0, pages) are hidden. A request that sees no token gives zeros.
+ * workspace: float32, 16-byte aligned, as many as tattn_cache4_attention_workspace gives (null where 0).
+ */
+int tattn_cache4_attention_workspace(int64_t R, int64_t H, int64_t Hk, int64_t D, int64_t width, int64_t page_size,
+                                     int64_t window, int64_t sinks, int64_t* floats);
+int tattn_cache4_attention(const void* q, void* o, const uint8_t* codes, const uint8_t* scales, const int32_t* tables,
+                           const int32_t* lens, float* workspace, const int64_t q_strides[2], const int64_t o_strides[2],
+                           int64_t table_stride, int64_t R, int64_t H, int64_t Hk, int64_t D, int64_t width, int64_t pages,
+                           int64_t page_size, int64_t window, int64_t sinks, int dtype, float sm_scale, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -252,3 +252,51 @@ def test_window_workspace_is_asked_for_where_keys_are_split():
     assert lib.tattn_window_workspace(1, 1, 8, 2, 16384, 16384, 64, 128, 4, ctypes.byref(n)) == 0 and n.value > 0
     assert lib.tattn_window_workspace(1, 1, 8, 2, 16384, 16384, 64, 128, 0, ctypes.byref(n)) == 0 and n.value == 0
     assert lib.tattn_window_workspace(1, 1, 8, 2, 16384, 100, 64, 128, 0, ctypes.byref(n)) == 1
+
+
+# ---- cache4_attention ----------------------------------------------------------------------------
+
+def _attend(**kw):
+    a = dict(q=torch.zeros(2, 4, 64).half(), cache=_cache(), tables=torch.zeros(2, 3, dtype=torch.int32),
+             lens=torch.zeros(2, dtype=torch.int32))
+    a.update(kw)
+    return tattn.cache4_attention(**a)
+
+
+@pytest.mark.parametrize("bad,msg", [
+    (dict(q=torch.zeros(2, 4, 1, 64).half()), "expected q"),
+    (dict(q=torch.zeros(2, 4, 32).half()), "expected q"),
+    (dict(q=torch.zeros(2, 3, 64).half()), "multiple of 2 heads"),
+    (dict(q=torch.zeros(2, 0, 64).half()), "expected q"),
+    (dict(q=torch.zeros(2, 4, 64).bfloat16()), "cache's dtype"),
+    (dict(tables=torch.zeros(2, 3)), "tables must be int32"),
+    (dict(tables=torch.zeros(3, 3, dtype=torch.int32)), "tables must be int32"),
+    (dict(lens=torch.zeros(2, dtype=torch.int64)), "lens must be int32"),
+    (dict(window=0), "window must be positive"),
+    (dict(sinks=-1), "sinks not negative"),
+    (dict(lens=torch.zeros(2, dtype=torch.int32, device="meta")), "lens must be on"),
+    (dict(q=torch.zeros(2, 4, 64).half().requires_grad_()), "no gradients"),
+])
+def test_cache4_attention_refuses(bad, msg):
+    with pytest.raises(ValueError, match=msg):
+        _attend(**bad)
+
+
+def test_cache4_attention_has_no_cpu_path():
+    with pytest.raises(RuntimeError, match="gfx950"):
+        _attend()
+
+
+@pytest.mark.parametrize("bad,msg", [
+    (dict(D=16), "head dim"), (dict(H=3), "evenly"), (dict(dtype=_lib.F32), "dtype"), (dict(page=40), "page size"),
+    (dict(pages=0), "no pages"), (dict(width=1 << 28), "2^31 tokens"), (dict(window=-1), "must not be negative"),
+    (dict(lens=None), "lens is a null pointer"), (dict(codes=8), "codes must be 16-byte aligned"),
+    (dict(qs=(ctypes.c_int64 * 2)(256, 63)), "q stride"), (dict(width=1 << 12), "workspace is a null pointer"),
+])
+def test_cache4_attention_entry_point_refuses(bad, msg):
+    st = (ctypes.c_int64 * 2)(256, 64)
+    a = dict(q=16, o=16, codes=16, scales=16, tables=16, lens=16, work=None, qs=st, os=st, ts=3, R=2, H=4, Hk=2, D=64, width=3,
+             pages=3, page=16, window=0, sinks=0, dtype=_lib.F16, scale=0.1, stream=None)
+    a.update(bad)
+    assert _lib.load().tattn_cache4_attention(*a.values()) == 1
+    assert msg in _lib.last_error()

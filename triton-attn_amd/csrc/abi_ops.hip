@@ -136,6 +136,27 @@ int check_16bit(int dtype) {
   return TATTN_OK;
 }
 
+int cache4_attn_common(Cache4AttnParams& p, int64_t R, int64_t H, int64_t Hk, int64_t D, int64_t width, int64_t page_size,
+                       int64_t window, int64_t sinks) {
+  int rc;
+  if (D != 32 && D != 64 && D != 128) return set_error(TATTN_E_ARG, "head dim must be 32, 64 or 128, got %lld", (long long)D);
+  if ((rc = check_page(page_size, &p.shift)) || (rc = check_count("requests", R)) || (rc = check_count("heads", H)) ||
+      (rc = check_count("table width", width)))
+    return rc;
+  if (Hk < 1 || H < 1 || H % Hk)
+    return set_error(TATTN_E_ARG, "%lld heads do not share %lld key heads evenly", (long long)H, (long long)Hk);
+  if (width * page_size > 0x7fffffff - 4096)
+    return set_error(TATTN_E_ARG, "a table row of %lld pages holds 2^31 tokens or more", (long long)width);
+  if (window < 0 || sinks < 0) return set_error(TATTN_E_ARG, "window and sinks must not be negative");
+  p.R = (int32_t)R; p.Hk = (int32_t)Hk; p.G = (int32_t)(H / Hk); p.groups = (p.G + 31) / 32;
+  if ((double)R * (double)Hk * p.groups > 67108864.0) return set_error(TATTN_E_ARG, "too many requests: %lld", (long long)R);
+  p.most = (int32_t)(width * page_size);
+  p.window = window == 0 || window > p.most ? p.most + 1 : (int32_t)window;
+  p.sinks = (int32_t)(sinks < p.most ? sinks : p.most);
+  cache4_chunks(p);
+  return TATTN_OK;
+}
+
 }  // namespace
 }  // namespace tattn
 
@@ -304,6 +325,40 @@ int tattn_window_bwd(const void* q, const void* k, const void* v, const void* o,
   p.c = sm_scale * kLog2e;
   p.scale = sm_scale;
   return launch_window_bwd(p, (int)D, dtype, (hipStream_t)stream);
+}
+
+int tattn_cache4_attention_workspace(int64_t R, int64_t H, int64_t Hk, int64_t D, int64_t width, int64_t page_size,
+                                     int64_t window, int64_t sinks, int64_t* floats) {
+  Cache4AttnParams p{};
+  int rc;
+  if (!floats) return set_error(TATTN_E_ARG, "floats is a null pointer");
+  if ((rc = cache4_attn_common(p, R, H, Hk, D, width, page_size, window, sinks))) return rc;
+  *floats = p.splits > 1 ? window_part_floats(R * Hk, p.G, p.splits, D) : 0;
+  return TATTN_OK;
+}
+
+int tattn_cache4_attention(const void* q, void* o, const uint8_t* codes, const uint8_t* scales, const int32_t* tables,
+                           const int32_t* lens, float* workspace, const int64_t q_strides[2], const int64_t o_strides[2],
+                           int64_t table_stride, int64_t R, int64_t H, int64_t Hk, int64_t D, int64_t width, int64_t pages,
+                           int64_t page_size, int64_t window, int64_t sinks, int dtype, float sm_scale, void* stream) {
+  Cache4AttnParams p{};
+  int rc;
+  if ((rc = cache4_attn_common(p, R, H, Hk, D, width, page_size, window, sinks)) || (rc = check_16bit(dtype)) ||
+      (rc = check_count("pages", pages)) || (rc = check_ptr("q", q, R, 16)) || (rc = check_ptr("o", o, R, 16)) ||
+      (rc = check_rows("q", q_strides, 2, 2)) || (rc = check_rows("o", o_strides, 2, 2)) ||
+      (rc = check_ptr("codes", codes, R, 16)) || (rc = check_ptr("scales", scales, R, 4)) ||
+      (rc = check_ptr("tables", tables, R * width, 4)) || (rc = check_ptr("lens", lens, R, 4)) ||
+      (rc = check_ptr("workspace", workspace, R > 0 && p.splits > 1, 16)))
+    return rc;
+  if (pages < 1) return set_error(TATTN_E_ARG, "the cache has no pages");
+  if ((rc = require_device())) return rc;
+  if (R == 0) return TATTN_OK;
+  p.q = q; p.out = o; p.codes = codes; p.scales = scales; p.tables = tables; p.lens = lens; p.part = workspace;
+  for (int i = 0; i < 2; ++i) p.sq[i] = q_strides[i], p.so[i] = o_strides[i];
+  p.table_stride = table_stride;
+  p.pages = (int32_t)pages;
+  p.c = sm_scale * kLog2e;
+  return launch_cache4_attention(p, (int)D, dtype, (hipStream_t)stream);
 }
 
 }  // extern "C"

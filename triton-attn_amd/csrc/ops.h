@@ -108,4 +108,26 @@ int launch_window_bwd(WindowParams p, int D, int dtype, hipStream_t st);
 int launch_combine(const float* part, void* out, float* m, const int64_t so[3], int64_t slices, int Hk, int G, int N,
                    int splits, int D, int dtype, hipStream_t st);
 
+// One token per request over the cache in 4 bits.
+struct Cache4AttnParams {
+  const void* q;  // [R, H, D], strides (r, h)
+  void* out;
+  const uint8_t* codes;
+  const uint8_t* scales;
+  const int32_t* tables;
+  const int32_t* lens;
+  float* part;  // window_part_floats(R * Hk, G, splits, D)
+  int64_t sq[2], so[2];
+  int64_t table_stride;
+  int32_t R, Hk, G, pages;
+  int32_t groups;  // of 32 query heads of a key head
+  int32_t shift;   // log2 of the page size
+  int32_t most;    // tokens that a table row holds
+  int32_t window, sinks;
+  int32_t chunk, splits;  // key tiles per workgroup, workgroups per request and key head
+  float c;
+};
+void cache4_chunks(Cache4AttnParams& p);  // sets chunk and splits
+int launch_cache4_attention(const Cache4AttnParams& p, int D, int dtype, hipStream_t st);
+
 }  // namespace tattn

@@ -1,6 +1,7 @@
 // Pages of a key/value cache on gfx950: which page and slot every new token gets, and the tokens'
 // keys and values into and out of a cache held in 4 bits.
 #include "common.h"
+#include "fp4.h"
 #include "ops.h"
 
 namespace tattn {
@@ -145,34 +146,6 @@ __global__ __launch_bounds__(256) void page_tables_kernel(const TablesParams p) 
 // Bound by bytes: 16 values a thread (two 16-byte loads, one 8-byte store), a workgroup takes one head of
 // 2048 / D consecutive tokens, keys and values, so that its codes and exponents fill whole lines of a page.
 
-template <typename T> struct Fp4;
-template <> struct Fp4<f16> {
-  static constexpr uint32_t kInf = 0x7c00, kTop = 127 + 13;  // 6 * 2^13 is finite, 4 * 2^14 is not
-  static __device__ __forceinline__ uint32_t exponent(uint32_t mag) {  // fp32 bits of a magnitude
-    return __builtin_bit_cast(uint32_t, (float)__builtin_bit_cast(f16, (uint16_t)mag));
-  }
-  template <int SEL>
-  static __device__ __forceinline__ uint32_t pack(uint32_t old, uint32_t two, float scale) {
-    return __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(old, __builtin_bit_cast(f16x2, two), scale, SEL);
-  }
-  template <int SEL>
-  static __device__ __forceinline__ uint32_t unpack(uint32_t codes, float scale) {
-    return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(codes, scale, SEL));
-  }
-};
-template <> struct Fp4<bf16> {
-  static constexpr uint32_t kInf = 0x7f80, kTop = 127 + 125;
-  static __device__ __forceinline__ uint32_t exponent(uint32_t mag) { return mag << 16; }
-  template <int SEL>
-  static __device__ __forceinline__ uint32_t pack(uint32_t old, uint32_t two, float scale) {
-    return __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(old, __builtin_bit_cast(bf16x2, two), scale, SEL);
-  }
-  template <int SEL>
-  static __device__ __forceinline__ uint32_t unpack(uint32_t codes, float scale) {
-    return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, scale, SEL));
-  }
-};
-
 // Row x of a workgroup's 256 / (D / 16) rows: token, K (0) or V (1), and the thread's 16 values.
 template <int D>
 struct Rows {
@@ -253,7 +226,6 @@ __global__ __launch_bounds__(256) void cache4_read_kernel(const Cache4Params p) 
     for (int i = 0; i < 2; ++i) {
       x[i] = u32x4{F::template unpack<0>(c[i], scale), F::template unpack<1>(c[i], scale),
                    F::template unpack<2>(c[i], scale), F::template unpack<3>(c[i], scale)};
-      if (e == 255) x[i] = u32x4{} - 1u;  // NaN in either type
     }
   }
   T* dst = (T*)(r.kv ? p.vo : p.ko) + ((int64_t)r.t * p.H + h) * D + 16 * r.c;

@@ -351,8 +351,9 @@ __global__ __launch_bounds__(256) void combine_kernel(const float* part, T* out,
 #pragma unroll 4
   for (int s = 0; s < splits; ++s) {
     const int64_t at = first + (int64_t)s * rows;
-    const float w = fast_exp2(ml[at * 2] - mall);
-    l = __builtin_fmaf(w, ml[at * 2 + 1], l);
+    const float w = fast_exp2(ml[at * 2] - mall), ls = ml[at * 2 + 1];
+    if (ls == 0.0f) continue;  // no visible key: the sums of such a part may not be there
+    l = __builtin_fmaf(w, ls, l);
     const f32x4 y = *reinterpret_cast<const f32x4*>(part + at * D + d0);
 #pragma unroll
     for (int e = 0; e < 4; ++e) x[e] = __builtin_fmaf(w, y[e], x[e]);

@@ -26,6 +26,7 @@ EXPORTS = (
     "tattn_num_configs", "tattn_config_desc", "tattn_pick_config", "tattn_picked",
     "tattn_page_tables", "tattn_cache4_write", "tattn_cache4_read",
     "tattn_norm_rope_fwd", "tattn_norm_rope_bwd", "tattn_window_workspace", "tattn_window_fwd", "tattn_window_bwd",
+    "tattn_cache4_attention_workspace", "tattn_cache4_attention",
 )
 
 # Kernels outside the tables, as `picked` reports them.
@@ -76,6 +77,8 @@ _SIGS = {
     "tattn_cache4_write": (_I, [_P] * 5 + [_STR4, _STR4] + [_I64] * 5 + [_I, _P]),
     "tattn_cache4_read": (_I, [_P] * 5 + [_I64] * 5 + [_I, _P]),
     "tattn_norm_rope_fwd": (_I, [_P] * 9 + [_STR4] * 4 + [_I64] * 7 + [_I, _I, _I, _F, _P]),
+    "tattn_cache4_attention_workspace": (_I, [_I64] * 8 + [ctypes.POINTER(_I64)]),
+    "tattn_cache4_attention": (_I, [_P] * 7 + [_STR4] * 2 + [_I64] * 10 + [_I, _F, _P]),
     "tattn_window_workspace": (_I, [_I] + [_I64] * 8 + [ctypes.POINTER(_I64)]),
     "tattn_window_fwd": (_I, [_P] * 7 + [_STR4] * 4 + [_I64] * 8 + [_I, _F, _P]),
     "tattn_window_bwd": (_I, [_P] * 11 + [_STR4] * 8 + [_I64] * 8 + [_I, _F, _P]),

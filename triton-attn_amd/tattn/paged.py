@@ -3,6 +3,7 @@
     tables, slots, ... = page_tables(...)     # pages and slots of the tokens that requests add
     cache4_write(cache, k, v, slots)          # their keys and values into the cache
     cache4_read(cache, slots)                 # what the cache holds for them
+    cache4_attention(q, cache, tables, lens)  # one token per request over its pages
 
 No counterpart in the reference. Lengths, tables and slots stay on the GPU: no call waits for it, and
 every call can be captured into a graph. Values the GPU alone knows are checked there: a slot or page outside
@@ -11,6 +12,9 @@ the cache is skipped, as documented per call.
 
 from __future__ import annotations
 
+import ctypes
+import functools
+import math
 from typing import NamedTuple
 
 import torch
@@ -146,3 +150,59 @@ def cache4_read(cache: Cache4, slots: torch.Tensor) -> tuple[torch.Tensor, torch
             cache.kv_heads, cache.head_dim, cache.pages, cache.page_size, _DTYPES[cache.dtype], _stream(slots))
     _lib.check(rc, "tattn_cache4_read")
     return k, v
+
+
+@functools.lru_cache(maxsize=4096)
+def _workspace(r: int, h: int, hk: int, d: int, width: int, page: int, window: int, sinks: int) -> int:
+    """Float32 values of workspace that a cache4_attention call of these sizes needs."""
+    out = ctypes.c_int64()
+    _lib.check(_lib.load().tattn_cache4_attention_workspace(r, h, hk, d, width, page, window, sinks, ctypes.byref(out)),
+               "tattn_cache4_attention_workspace")
+    return out.value
+
+
+def cache4_attention(
+    q: torch.Tensor, cache: Cache4, tables: torch.Tensor, lens: torch.Tensor, window: int | None = None, sinks: int = 0,
+    sm_scale: float | None = None,
+) -> torch.Tensor:
+    """Attention of one token per request over the cache: q [requests, heads, head_dim] (the cache's dtype; heads a
+    multiple of its kv heads, consecutive heads sharing one; any request and head strides), tables int32 [requests, width]
+    as page_tables keeps them, lens int32 [requests]: tokens each request sees, the newest one included (clamped to what its
+    table row holds). With a window only the last `window` tokens and the first `sinks` are seen, and pages without a seen
+    token are not looked up (they may have been given away). Tokens on a page number outside the cache are hidden; a request
+    that sees nothing gives zeros. sm_scale defaults to 1 / sqrt(head_dim). For serving: refuses a q that requires gradients."""
+    if q.dim() != 3 or q.shape[2] != cache.head_dim or q.shape[1] < 1 or q.shape[1] % cache.kv_heads:
+        raise ValueError(f"expected q [requests, heads, {cache.head_dim}] with a multiple of {cache.kv_heads} heads; got {list(q.shape)}")
+    r, h, d = q.shape
+    if q.dtype != cache.dtype:
+        raise ValueError(f"q must have the cache's dtype {cache.dtype}, got {q.dtype}")
+    if tables.dim() != 2:
+        raise ValueError(f"tables must be int32 [requests, width], got {list(tables.shape)}")
+    width = tables.shape[1]
+    check_index("tables", tables, torch.int32, (r, width))
+    check_index("lens", lens, torch.int32, (r,))
+    if (window is not None and window < 1) or sinks < 0:
+        raise ValueError(f"window must be positive and sinks not negative, got {window} and {sinks}")
+    same_device(q, cache=cache.codes, tables=tables, lens=lens)
+    if torch.is_grad_enabled() and q.requires_grad:
+        raise ValueError("cache4_attention has no gradients: call it under torch.no_grad()")
+    _require_gpu(q)
+    q, lens = rows(q), lens.contiguous()
+    o = torch.empty_like(q)
+    if q.numel() == 0 or width == 0 or cache.pages == 0:
+        return o.zero_()
+    if width > 1 and tables.stride(1) != 1:
+        tables = tables.contiguous()
+    held = width * cache.page_size
+    sizes = (0 if window is None else min(window, held), min(sinks, held))
+    n = _workspace(r, h, cache.kv_heads, d, width, cache.page_size, *sizes)
+    work = q.new_empty(n, dtype=torch.float32) if n else None
+    _, st = strides(q, o)
+    with _on_device(q):
+        rc = _lib.load().tattn_cache4_attention(
+            q.data_ptr(), o.data_ptr(), cache.codes.data_ptr(), cache.scales.data_ptr(), tables.data_ptr(), lens.data_ptr(),
+            None if work is None else work.data_ptr(), *st, tables.stride(0), r, h, cache.kv_heads, d, width, cache.pages,
+            cache.page_size, *sizes, _DTYPES[cache.dtype], float(sm_scale) if sm_scale is not None else 1.0 / math.sqrt(d),
+            _stream(q))
+    _lib.check(rc, "tattn_cache4_attention")
+    return o
