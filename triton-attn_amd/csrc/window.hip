@@ -1,11 +1,10 @@
 // Attention over a sliding window and the first keys, 16-bit, forward and backward, on gfx950.
 //
-// The waves of a workgroup share row tiles and key tiles as in the kernels for few rows: NW = RW * CS waves own RW
-// 32-row tiles; a step stages CS tiles of the other dimension by LDS DMA (buffer_load ... lds, swizzled rows) into one of
-// two stages while the other is worked on; wave (rw, cs) works on tile cs of the step for row tile rw, and the CS partial
-// results of a row tile are added through LDS at the end. What differs is the list of tiles: only those that some
-// row of the workgroup sees are walked (TileList), only those at the ends of a row's window pay for masks, and a wave
-// passes over tiles that none of its own rows sees.
+// A workgroup's NW = RW * CS waves own RW 32-row tiles; a step stages CS * TP tiles of the other dimension by LDS DMA
+// (buffer_load ... lds, swizzled rows) into one of two stages while the other is worked on. With many rows CS is 1 and each wave
+// works on all TP tiles of a step for its own rows; with few, wave (rw, cs) takes every CS-th tile, and the CS partial
+// results of a row tile are added through LDS at the end. Only tiles that some row of the workgroup sees are walked
+// (TileList), only those at the ends of a row's window pay for masks, and a wave passes over tiles that none of its own rows sees.
 //
 // Rows that nobody in the workgroup sees (before the window, behind the last key) are fetched from beyond the end of
 // the buffer, which reads as zero: whatever a cache holds there cannot reach a sum.
@@ -17,47 +16,45 @@
 namespace tattn {
 namespace {
 
-template <int D, int NW, int CS>
+// A stage: NT tiles of each of two tensors. Each wave fetches TW whole tiles of a step, the first half of the waves of
+// the first tensor.
+template <int D, int NW, int NT>
 struct WinRing {
-  static constexpr int RB = Swz<D>::RB, TILE = 32 * RB, PIECES = TILE / 1024;
-  static constexpr int HALF = CS * TILE;        // bytes of one tensor's tiles
+  static constexpr int RB = Swz<D>::RB, TILE = 32 * RB, PIECES = TILE / 1024;  // 1 KB DMA pieces
+  static constexpr int HALF = NT * TILE;  // bytes of one tensor's tiles
   static constexpr int STAGE = 2 * HALF;
-  static constexpr int PW = STAGE / 1024 / NW;  // 1 KB DMA pieces per wave and step
-  static_assert(PW >= 1 && PW * NW * 1024 == STAGE && NW % 2 == 0, "whole pieces, one tensor per wave");
+  static constexpr int TW = 2 * NT / NW;
+  static_assert(TW >= 1 && TW * NW == 2 * NT && NW % 2 == 0, "whole tiles, one tensor per wave");
 };
 
 constexpr uint32_t kBeyond = 0x7fffffffu;  // byte offset past every slice: reads as zero
 
-// DMA of tile pairs: the first half of the waves loads the first tensor, the other half the second.
-template <int D, int NW, int CS>
+template <int D, int NW, int NT>
 struct WinLoader {
-  using R = WinRing<D, NW, CS>;
-  uint32_t go[R::PW];
+  using R = WinRing<D, NW, NT>;
+  uint32_t go[R::PIECES];
   uint32_t tile_bytes;
-  int base, g0, lane;
+  int first, base, lane;  // first tile of the wave's TW, and its place in a stage
   bool second;
   __device__ __forceinline__ void init(int64_t sa, int64_t sb, int wu, int lane_) {
     lane = lane_;
     second = wu >= NW / 2;
     const int64_t st = second ? sb : sa;
     tile_bytes = uniform32((uint32_t)(st * 64));
-    base = wu * R::PW * 1024;
-    g0 = (wu * R::PW) % (CS * R::PIECES);
+    first = wu % (NW / 2) * R::TW;
+    base = (second ? R::HALF : 0) + first * R::TILE;
     constexpr int CPR = R::RB / 16;
 #pragma unroll
-    for (int i = 0; i < R::PW; ++i) {
-      const int j = 64 * ((g0 + i) % R::PIECES) + lane;
+    for (int i = 0; i < R::PIECES; ++i) {
+      const int j = 64 * i + lane;
       const int row = j / CPR, cc = ((j % CPR) ^ Swz<D>::f(row)) & (D / 8 - 1);
       go[i] = (uint32_t)(perm32(row) * st * 2 + cc * 16);
     }
   }
-  // Which of the step's CS tiles piece i belongs to, and the row of that tile the lane fetches.
-  __device__ __forceinline__ int slot(int i) const { return (g0 + i) / R::PIECES; }
-  __device__ __forceinline__ int row(int i) const {
-    return perm32((64 * ((g0 + i) % R::PIECES) + lane) / (R::RB / 16));
-  }
-  __device__ __forceinline__ void fetch(__amdgpu_buffer_rsrc_t rs, char* stage, int i, uint32_t off) const {
-    __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (TATTN_LDS void*)(stage + base + 1024 * i), 16, (int)off, 0, 0, 0);
+  // Row of a tile that the lane fetches in piece i.
+  __device__ __forceinline__ int row(int i) const { return perm32((64 * i + lane) / (R::RB / 16)); }
+  __device__ __forceinline__ void fetch(__amdgpu_buffer_rsrc_t rs, char* stage, int x, int i, uint32_t off) const {
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (TATTN_LDS void*)(stage + base + x * R::TILE + 1024 * i), 16, (int)off, 0, 0, 0);
   }
 };
 
@@ -110,37 +107,44 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t win_rsrc(const void* base, int
   return slice_rsrc((const T*)base + off, rows > 0 ? slice_bytes(rows, stride, D) : 0);
 }
 
-// K and V tiles of list entries [i0, i0 + CS) into `stage`; entries from i1 on are not fetched.
-template <int D, int NW, int CS>
-__device__ __forceinline__ void fetch_keys(const WinLoader<D, NW, CS>& ld, __amdgpu_buffer_rsrc_t rs, char* stage,
+// K and V tiles of list entries [i0, i0 + NT) into `stage`; entries from i1 on are not fetched.
+template <int D, int NW, int NT>
+__device__ __forceinline__ void fetch_keys(const WinLoader<D, NW, NT>& ld, __amdgpu_buffer_rsrc_t rs, char* stage,
                                            const TileList& list, int i0, int i1, int top, int sinks) {
+  using R = WinRing<D, NW, NT>;
 #pragma unroll
-  for (int i = 0; i < WinRing<D, NW, CS>::PW; ++i) {
-    const int at = i0 + ld.slot(i);
-    if (at >= i1) continue;
+  for (int x = 0; x < R::TW; ++x) {
+    const int at = i0 + ld.first + x;
+    if (at >= i1) break;
     const int t = list.at(at);
-    uint32_t o = ld.go[i] + (uint32_t)t * ld.tile_bytes;
+    const uint32_t o = (uint32_t)t * ld.tile_bytes;
     if (32 * t + 31 > top || (32 * t < list.lo && 32 * t + 31 >= sinks)) {
-      const int key = 32 * t + ld.row(i);
-      if (key > top || (key < list.lo && key >= sinks)) o = kBeyond;
+#pragma unroll
+      for (int i = 0; i < R::PIECES; ++i) {
+        const int key = 32 * t + ld.row(i);
+        const bool dead = key > top || (key < list.lo && key >= sinks);
+        ld.fetch(rs, stage, x, i, dead ? kBeyond : ld.go[i] + o);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < R::PIECES; ++i) ld.fetch(rs, stage, x, i, ld.go[i] + o);
     }
-    ld.fetch(rs, stage, i, o);
   }
 }
 
 // ---- forward -----------------------------------------------------------------------------------
-template <typename T, int D, int RW, int CS, int OCC, bool SPLIT>
+template <typename T, int D, int RW, int CS, int TP, int OCC, bool SPLIT>
 __global__ __launch_bounds__(RW * CS * 64, OCC) void window_fwd_kernel(const WindowParams p) {
   using H = H16<T>;
   using V8 = typename H::V8;
   using V4 = typename H::V4;
   using V2 = typename H::V2;
-  constexpr int NW = RW * CS, NSD = D / 16, DT = (D + 31) / 32;
-  using R = WinRing<D, NW, CS>;
+  constexpr int NW = RW * CS, NT = CS * TP, NSD = D / 16, DT = (D + 31) / 32;
+  using R = WinRing<D, NW, NT>;
   // Two arrays: a DMA into one stage does not alias reads of the other.
   __shared__ __attribute__((aligned(1024))) char s0[R::STAGE];
   __shared__ __attribute__((aligned(1024))) char s1[R::STAGE];
-  __shared__ float red[2][NW][32];
+  __shared__ float red[2][CS > 1 || SPLIT ? NW : 1][32];
 
   const int tid = threadIdx.x;
   const int lane = tid & 63, h2 = lane >> 5, l32 = lane & 31;
@@ -156,15 +160,15 @@ __global__ __launch_bounds__(RW * CS * 64, OCC) void window_fwd_kernel(const Win
   list.init(b.p0, b.p1, p.window, p.sinks);
   const int i0 = SPLIT ? (int)((int64_t)list.n * split / p.splits) : 0;
   const int i1 = SPLIT ? (int)((int64_t)list.n * (split + 1) / p.splits) : list.n;
-  const int nsteps = (i1 - i0 + CS - 1) / CS;
+  const int nsteps = (i1 - i0 + NT - 1) / NT;
 
-  WinLoader<D, NW, CS> ld;
+  WinLoader<D, NW, NT> ld;
   ld.init(p.sk[2], p.sv[2], wu, lane);
   const __amdgpu_buffer_rsrc_t rs =
       ld.second ? win_rsrc<T, D>(p.v, b.z * p.sv[0] + b.hk * p.sv[1], b.len, p.sv[2])
                 : win_rsrc<T, D>(p.k, b.z * p.sk[0] + b.hk * p.sk[1], b.len, p.sk[2]);
   auto issue = [&](char* stage, int step) __attribute__((always_inline)) {
-    fetch_keys<D, NW, CS>(ld, rs, stage, list, i0 + step * CS, i1, b.top, p.sinks);
+    fetch_keys<D, NW, NT>(ld, rs, stage, list, i0 + step * NT, i1, b.top, p.sinks);
   };
   if (nsteps > 0) issue(s0, 0);
 
@@ -201,6 +205,12 @@ __global__ __launch_bounds__(RW * CS * 64, OCC) void window_fwd_kernel(const Win
     f32x16 s = f32x16{};
 #pragma unroll
     for (int sd = 0; sd < NSD; ++sd) s = Elt<T>::mfma(lds8<T>(st + at.nat[sd]), qop[sd], s);
+    // Masked: scaled scores with hidden ones at -inf, whatever lies there (the running max is finite).
+    if (MASK) {
+#pragma unroll
+      for (int r = 0; r < 16; ++r) s[r] = hide.hides(r) ? -__builtin_inff() : s[r] * c;
+    }
+    const float cc = MASK ? 1.0f : c;
     V8 x[2];
     auto probs = [&]() __attribute__((always_inline)) {
       float ps = 0.0f;
@@ -209,12 +219,7 @@ __global__ __launch_bounds__(RW * CS * 64, OCC) void window_fwd_kernel(const Win
 #pragma unroll
         for (int i = 0; i < 8; i += 2) {
           const int r = 8 * sg + i;
-          float e0 = fast_exp2(__builtin_fmaf(s[r], c, -mrow)), e1 = fast_exp2(__builtin_fmaf(s[r + 1], c, -mrow));
-          if (MASK) {
-            e0 = hide.hides(r) ? 0.0f : e0;
-            e1 = hide.hides(r + 1) ? 0.0f : e1;
-          }
-          const V2 pr = H::pack(e0, e1);
+          const V2 pr = H::pack(fast_exp2(__builtin_fmaf(s[r], cc, -mrow)), fast_exp2(__builtin_fmaf(s[r + 1], cc, -mrow)));
           ps = H::sum2(pr, ps);
           x[sg][i] = pr[0];
           x[sg][i + 1] = pr[1];
@@ -227,7 +232,7 @@ __global__ __launch_bounds__(RW * CS * 64, OCC) void window_fwd_kernel(const Win
     if (__builtin_amdgcn_ballot_w64(!(ps <= 4096.0f))) {
       float mx = kNoMax;
 #pragma unroll
-      for (int r = 0; r < 16; ++r) mx = MASK && hide.hides(r) ? mx : __builtin_fmaxf(mx, s[r] * c);
+      for (int r = 0; r < 16; ++r) mx = __builtin_fmaxf(mx, s[r] * cc);
       const float cand = max_halves(mx);
       const float mnew = cand > mrow + kRescaleLog2 ? cand : mrow;
       const float alpha = fast_exp2(mrow - mnew);
@@ -248,13 +253,14 @@ __global__ __launch_bounds__(RW * CS * 64, OCC) void window_fwd_kernel(const Win
   };
   auto step = [&](int i, char* cur, char* nxt) __attribute__((always_inline)) {
     if (i + 1 < nsteps) issue(nxt, i + 1);
-    const int k = i0 + i * CS + cs;
-    if (k < i1) {
-      const int t = list.at(k);
-      if (!tile_hidden(wp0, wp1, t, p.window, p.sinks)) {
-        if (tile_masked(wp0, wp1, t, p.window, p.sinks)) tile(cur, t, std::true_type{});
-        else tile(cur, t, std::false_type{});
-      }
+    const int k = i0 + i * NT + cs;
+#pragma unroll 1
+    for (int x = 0; x < TP; ++x) {
+      if (k + x * CS >= i1) break;
+      const int t = list.at(k + x * CS);
+      if (tile_hidden(wp0, wp1, t, p.window, p.sinks)) continue;
+      if (tile_masked(wp0, wp1, t, p.window, p.sinks)) tile(cur + x * CS * R::TILE, t, std::true_type{});
+      else tile(cur + x * CS * R::TILE, t, std::false_type{});
     }
     all_landed_barrier();
   };
@@ -270,6 +276,24 @@ __global__ __launch_bounds__(RW * CS * 64, OCC) void window_fwd_kernel(const Win
   // DMA is in flight). A split keeps the sums as they are; otherwise they are divided by the row's sum, and rows
   // that see no key become 0.
   const float lt = sum_halves(lrow);
+  if constexpr (CS == 1 && !SPLIT) {
+    const float inv = lt == 0.0f ? 0.0f : 1.0f / lt;
+    if (!live) return;
+    T* orow = (T*)p.out + b.z * p.sout[0] + (b.hk * p.G + g) * p.sout[1] + n * p.sout[2];
+#pragma unroll
+    for (int u = 0; u < DT; ++u)
+#pragma unroll
+      for (int gr = 0; gr < 4; ++gr) {
+        const int d0 = 32 * u + 8 * gr + 4 * h2;
+        if (d0 >= D) continue;
+        V4 y;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) y[e] = (T)(acc[u][4 * gr + e] * inv);
+        *reinterpret_cast<V4*>(orow + d0) = y;
+      }
+    if (h2 == 0 && p.m) p.m[((int64_t)b.z * p.H + b.hk * p.G + g) * p.N + n] = mrow + __log2f(lt);
+    return;
+  }
   if (h2 == 0) {
     red[0][wu][l32] = mrow;
     red[1][wu][l32] = lt;
@@ -285,7 +309,7 @@ __global__ __launch_bounds__(RW * CS * 64, OCC) void window_fwd_kernel(const Win
   if (!SPLIT) wgt = lall == 0.0f ? 0.0f : wgt / lall;
   constexpr int PART = DT * 16 * 64 * 4;  // bytes of one wave's partial O^T
   constexpr int PER = R::STAGE / PART;    // partials per stage array
-  static_assert(2 * PER >= NW, "partials fit the stages");
+  static_assert((CS == 1 && !SPLIT) || 2 * PER >= NW, "partials fit the stages");
   auto part = [&](int k) { return (TATTN_LDS float*)(k < PER ? s0 + k * PART : s1 + (k - PER) * PART); };
   {
     TATTN_LDS float* dst = part(wu) + lane;
@@ -368,15 +392,15 @@ __global__ __launch_bounds__(256) void combine_kernel(const float* part, T* out,
 }
 
 // ---- dQ ------------------------------------------------------------------------------------------
-// Rows and key tiles as in the forward; computes delta = rowsum(dO * O) on the way and stores it for dK / dV.
-template <typename T, int D, int RW, int CS, int OCC>
+// Rows and key tiles as in the forward; computes delta = rowsum(dO * O) on the way and stores -delta for dK / dV.
+template <typename T, int D, int RW, int CS, int TP, int OCC>
 __global__ __launch_bounds__(RW * CS * 64, OCC) void window_dq_kernel(const WindowParams p) {
   using H = H16<T>;
   using V8 = typename H::V8;
   using V4 = typename H::V4;
   using V2 = typename H::V2;
-  constexpr int NW = RW * CS, NSD = D / 16, DT = (D + 31) / 32;
-  using R = WinRing<D, NW, CS>;
+  constexpr int NW = RW * CS, NT = CS * TP, NSD = D / 16, DT = (D + 31) / 32;
+  using R = WinRing<D, NW, NT>;
   __shared__ __attribute__((aligned(1024))) char s0[R::STAGE];
   __shared__ __attribute__((aligned(1024))) char s1[R::STAGE];
 
@@ -391,15 +415,15 @@ __global__ __launch_bounds__(RW * CS * 64, OCC) void window_dq_kernel(const Wind
   b.init(p, slice, p.nblk - 1 - blk, RW);
   TileList list;
   list.init(b.p0, b.p1, p.window, p.sinks);
-  const int nsteps = (list.n + CS - 1) / CS;
+  const int nsteps = (list.n + NT - 1) / NT;
 
-  WinLoader<D, NW, CS> ld;
+  WinLoader<D, NW, NT> ld;
   ld.init(p.sk[2], p.sv[2], wu, lane);
   const __amdgpu_buffer_rsrc_t rs =
       ld.second ? win_rsrc<T, D>(p.v, b.z * p.sv[0] + b.hk * p.sv[1], b.len, p.sv[2])
                 : win_rsrc<T, D>(p.k, b.z * p.sk[0] + b.hk * p.sk[1], b.len, p.sk[2]);
   auto issue = [&](char* stage, int step) __attribute__((always_inline)) {
-    fetch_keys<D, NW, CS>(ld, rs, stage, list, step * CS, list.n, b.top, p.sinks);
+    fetch_keys<D, NW, NT>(ld, rs, stage, list, step * NT, list.n, b.top, p.sinks);
   };
   if (nsteps > 0) issue(s0, 0);
 
@@ -425,7 +449,7 @@ __global__ __launch_bounds__(RW * CS * 64, OCC) void window_dq_kernel(const Wind
       sd[s] = chunk_dot(*reinterpret_cast<const V8*>(os + 16 * s), y);
     }
     dl = row_delta(sd);
-    if (live && h2 == 0 && cs == 0) p.delta[mrow] = dl;
+    if (live && h2 == 0 && cs == 0) p.delta[mrow] = -dl;
     if (!live) dl = 0.0f;
   }
   const float nm = live ? -p.m[mrow] : 0.0f;
@@ -471,13 +495,14 @@ __global__ __launch_bounds__(RW * CS * 64, OCC) void window_dq_kernel(const Wind
   };
   auto step = [&](int i, char* cur, char* nxt) __attribute__((always_inline)) {
     if (i + 1 < nsteps) issue(nxt, i + 1);
-    const int k = i * CS + cs;
-    if (k < list.n) {
-      const int t = list.at(k);
-      if (!tile_hidden(wp0, wp1, t, p.window, p.sinks)) {
-        if (tile_masked(wp0, wp1, t, p.window, p.sinks)) tile(cur, t, std::true_type{});
-        else tile(cur, t, std::false_type{});
-      }
+    const int k = i * NT + cs;
+#pragma unroll 1
+    for (int x = 0; x < TP; ++x) {
+      if (k + x * CS >= list.n) break;
+      const int t = list.at(k + x * CS);
+      if (tile_hidden(wp0, wp1, t, p.window, p.sinks)) continue;
+      if (tile_masked(wp0, wp1, t, p.window, p.sinks)) tile(cur + x * CS * R::TILE, t, std::true_type{});
+      else tile(cur + x * CS * R::TILE, t, std::false_type{});
     }
     all_landed_barrier();
   };
@@ -489,9 +514,25 @@ __global__ __launch_bounds__(RW * CS * 64, OCC) void window_dq_kernel(const Wind
   }
   if (i < nsteps) step(i, s0, s1);
 
+  if constexpr (CS == 1) {
+    if (!live) return;
+    T* orow = (T*)p.out + b.z * p.sout[0] + h * p.sout[1] + n * p.sout[2];
+#pragma unroll
+    for (int u = 0; u < DT; ++u)
+#pragma unroll
+      for (int gr = 0; gr < 4; ++gr) {
+        const int d0 = 32 * u + 8 * gr + 4 * h2;
+        if (d0 >= D) continue;
+        V4 y;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) y[e] = (T)(dq[u][4 * gr + e] * p.scale);
+        *reinterpret_cast<V4*>(orow + d0) = y;
+      }
+    return;
+  }
   constexpr int PART = DT * 16 * 64 * 4;
   constexpr int PER = R::STAGE / PART;
-  static_assert(2 * PER >= NW, "partials fit the stages");
+  static_assert(CS == 1 || 2 * PER >= NW, "partials fit the stages");
   auto part = [&](int k) { return (TATTN_LDS float*)(k < PER ? s0 + k * PART : s1 + (k - PER) * PART); };
   {
     TATTN_LDS float* dst = part(wu) + lane;
@@ -581,22 +622,23 @@ __global__ __launch_bounds__(RW * CS * 64, OCC) void window_dkdv_kernel(const Wi
   const uint32_t qbytes = (uint32_t)slice_bytes(p.N, ld.second ? p.sd[2] : p.sq[2], D);
   auto issue = [&](char* stage, int step) __attribute__((always_inline)) {
 #pragma unroll
-    for (int i = 0; i < R::PW; ++i) {
-      const int k = i0 + step * CS + ld.slot(i);
-      if (k >= i1) continue;
+    for (int x = 0; x < R::TW; ++x) {
+      const int k = i0 + step * CS + ld.first + x;
+      if (k >= i1) break;
       const int g = k / nq, qt = qt0 + k % nq;
       // Rows past the head's last query lie past the end of its slice and read as zero.
-      ld.fetch(slice_rsrc(qbase + g * head_bytes, qbytes), stage, i, ld.go[i] + (uint32_t)qt * ld.tile_bytes);
+      const __amdgpu_buffer_rsrc_t rs = slice_rsrc(qbase + g * head_bytes, qbytes);
+#pragma unroll
+      for (int i = 0; i < R::PIECES; ++i) ld.fetch(rs, stage, x, i, ld.go[i] + (uint32_t)qt * ld.tile_bytes);
     }
   };
   if (nsteps > 0) issue(s0, 0);
-  // Lanes 0-31 fetch M and lanes 32-63 delta of the wave's tile; zero past the end.
+  // Lanes 0-31 fetch M and lanes 32-63 -delta of the wave's tile; zero past the end.
   const float* mdsrc = (h2 ? p.delta : p.m) + ((int64_t)z * p.H + hk * p.G) * p.N;
   auto md_load = [&](int step) {
     const int k = i0 + step * CS + cs;
     const int q = k < i1 ? 32 * (qt0 + k % nq) + l32 : p.N;
-    const float x = q < p.N ? mdsrc[(int64_t)(k / nq) * p.N + q] : 0.0f;
-    return h2 ? -x : x;
+    return q < p.N ? mdsrc[(int64_t)(k / nq) * p.N + q] : 0.0f;
   };
   md[wu][0][lane] = nsteps > 0 ? md_load(0) : 0.0f;
   const int kt = kb * RW + rw, key = 32 * kt + l32;
@@ -744,6 +786,260 @@ __global__ __launch_bounds__(RW * CS * 64, OCC) void window_dkdv_kernel(const Wi
   reduce(dv, 1.0f, (T*)p.dv + z * p.sdv[0] + hk * p.sdv[1], p.sdv[2], fdst + 32 * RW * D);
 }
 
+// dK / dV at head dims 64 and 128: two waves per 32-key tile. Over each 32-query tile wave j (role A) computes S = Q K^T,
+// P = 2^(S c - M), dV += P^T dO, and wave j + 4 (role B) dP - delta = dO V^T - delta, dS = P (dP - delta), dK += dS^T Q,
+// taking P from A through LDS in float32. Each keeps one of K / V and one accumulator set: half the registers of a wave that
+// does both, so that two (head dim 128) or four waves (64) share a SIMD; as many matrix instructions in either role.
+// Step i, one barrier each: A runs S of tile i + 1 and dV of tile i - 1 on the matrix cores while its vector unit forms P of
+// tile i; B runs dP of tile i, then forms dS of tile i - 1 and runs its dK. Tile i + 2 is on its way to the fourth stage.
+template <typename T, int D, int OCC>
+__global__ __launch_bounds__(512, OCC) void window_dkdv_pair_kernel(const WindowParams p) {
+  using H = H16<T>;
+  using V8 = typename H::V8;
+  using V2 = typename H::V2;
+  constexpr int RW = 4, NW = 8, NSD = D / 16, DT = D / 32, RB = Swz<D>::RB, TILE = 32 * RB;
+  constexpr int PW = 2 * TILE / 1024 / NW;          // 1 KB pieces per wave and step
+  constexpr int STAGE = 2 * TILE + 256;             // Q, dO, M[32], -delta[32]
+  constexpr int XB = 32 * 32 * 4;                   // P of a pair
+  // Arrays of their own: a DMA into one does not alias reads of the others.
+  __shared__ __attribute__((aligned(1024))) char st0[STAGE], st1[STAGE], st2[STAGE], st3[STAGE];
+  __shared__ __attribute__((aligned(1024))) char x0[RW * XB], x1[RW * XB];
+  auto stage = [&](auto tag) __attribute__((always_inline)) -> char* {
+    constexpr int I = decltype(tag)::value & 3;
+    return I == 0 ? st0 : I == 1 ? st1 : I == 2 ? st2 : st3;
+  };
+
+  const int tid = threadIdx.x;
+  const int lane = tid & 63, h2 = lane >> 5, l32 = lane & 31;
+  const int wu = (int)uniform32((uint32_t)(tid >> 6));
+  const int pr = wu & 3;
+  const bool role_b = wu >= 4;
+  const float c = p.c;
+  const KeyBlocks<RW> kbs(p.S, p.sinks, p.splits);
+  int slice, kb, split = 0;
+  if (!window_coord(p.Z * p.Hk, kbs.items, p.runs, slice, kb)) return;
+  const bool parted = kb < kbs.sink_blocks * p.splits;
+  if (parted) split = kb % p.splits, kb /= p.splits;
+  else kb = kb - kbs.sink_blocks * p.splits + kbs.sink_blocks;
+  const int z = slice / p.Hk, hk = slice % p.Hk, off = p.S - p.N;
+  const int k0 = 32 * RW * kb, k1 = k0 + 32 * RW - 1;
+  // Queries that see a key of the block, as tiles of 32 of each head in turn.
+  const int nlo = max(0, k0 - off);
+  const int nhi = k0 < p.sinks ? p.N - 1 : min(p.N - 1, k1 + p.window - 1 - off);
+  const int qt0 = nlo >> 5, nq = nhi < nlo ? 0 : (nhi >> 5) - qt0 + 1;
+  const int total = nq * p.G;
+  const int i0 = parted ? (int)((int64_t)total * split / p.splits) : 0;
+  const int i1 = parted ? (int)((int64_t)total * (split + 1) / p.splits) : total;
+  const int n = i1 - i0;
+  const int wk0 = 32 * (kb * RW + pr), wk1 = wk0 + 31, key = wk0 + l32;
+
+  // The wave's operand: K rows (A) or V rows (B).
+  V8 kv[NSD];
+  {
+    const T* src = role_b ? (const T*)p.v + z * p.sv[0] + hk * p.sv[1] + (int64_t)(key < p.S ? key : 0) * p.sv[2]
+                          : (const T*)p.k + z * p.sk[0] + hk * p.sk[1] + (int64_t)(key < p.S ? key : 0) * p.sk[2];
+#pragma unroll
+    for (int s = 0; s < NSD; ++s) {
+      const V8 a = *reinterpret_cast<const V8*>(src + 16 * s + 8 * h2);
+      kv[s] = key < p.S ? a : V8{};
+    }
+  }
+
+  // Fetching: pieces wu * PW .. of the step's Q tile (waves 0-3) and dO tile (4-7), and by wave 0 M and -delta.
+  const int64_t head = (role_b ? p.sd[1] : p.sq[1]) * 2, rowst = role_b ? p.sd[2] : p.sq[2];
+  const char* base = role_b ? (const char*)((const T*)p.dout + z * p.sd[0] + (int64_t)hk * p.G * p.sd[1])
+                            : (const char*)((const T*)p.q + z * p.sq[0] + (int64_t)hk * p.G * p.sq[1]);
+  const uint32_t bytes = (uint32_t)slice_bytes(p.N, rowst, D), tile_bytes = uniform32((uint32_t)(rowst * 64));
+  const float* md = (h2 ? p.delta : p.m) + ((int64_t)z * p.H + hk * p.G) * p.N;
+  uint32_t go[PW];
+#pragma unroll
+  for (int i = 0; i < PW; ++i) {
+    constexpr int CPR = RB / 16;
+    const int j = 64 * ((wu & 3) * PW + i) + lane, row = j / CPR;
+    go[i] = (uint32_t)(perm32(row) * rowst * 2 + (((j % CPR) ^ Swz<D>::f(row)) & (D / 8 - 1)) * 16);
+  }
+  int fg = nq > 0 ? i0 / nq : 0, fq = qt0 + (nq > 0 ? i0 % nq : 0), fi = 0;  // next tile to fetch
+  auto fetch = [&](char* st) __attribute__((always_inline)) {
+    if (fi < n) {
+      const __amdgpu_buffer_rsrc_t rs = slice_rsrc(base + fg * head, bytes);  // rows past the last query read as zero
+#pragma unroll
+      for (int i = 0; i < PW; ++i)
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (TATTN_LDS void*)(st + (wu * PW + i) * 1024), 16,
+                                                 (int)(go[i] + (uint32_t)fq * tile_bytes), 0, 0, 0);
+      if (wu == 0) {
+        const float* src = md + (int64_t)fg * p.N + min(32 * fq + l32, p.N - 1);
+        __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)src,
+                                         (TATTN_LDS void*)(st + 2 * TILE), 4, 0, 0);
+      }
+    }
+    ++fi;
+    if (++fq == qt0 + nq) fq = qt0, ++fg;
+  };
+
+  int nat[NSD], lo[DT], hi[DT];
+#pragma unroll
+  for (int s = 0; s < NSD; ++s) nat[s] = Swz<D>::addr(l32, (16 * s + 8 * h2) * 2);
+#pragma unroll
+  for (int u = 0; u < DT; ++u) tr_addrs<D>(0, u, lane, lo[u], hi[u]);
+  f32x16 acc[DT];  // dV (A) or dK (B)
+#pragma unroll
+  for (int u = 0; u < DT; ++u) acc[u] = f32x16{};
+
+  // What the pair does with a query tile: nothing, all of it, or with a mask.
+  struct Look {
+    int qt;
+    bool live, masked;
+  };
+  auto look = [&](int qt, bool in) __attribute__((always_inline)) {
+    const int q0 = off + 32 * qt, q1 = q0 + 31;
+    Look l;
+    l.qt = qt;
+    l.live = in && wk0 < p.S && q1 >= wk0 && (q0 - wk1 < p.window || wk0 < p.sinks);
+    l.masked = q0 < wk1 || (q1 - wk0 >= p.window && wk1 >= p.sinks) || 32 * qt + 32 > p.N;
+    return l;
+  };
+
+  auto run = [&](auto role_tag) __attribute__((always_inline)) {
+    constexpr bool RB_ = decltype(role_tag)::value;
+    // S (A) of a stage's tile, or dP - delta (B).
+    auto first = [&](f32x16& s, const char* st) __attribute__((always_inline)) {
+      if constexpr (RB_) {
+        const TATTN_LDS char* nd = (const TATTN_LDS char*)st + 2 * TILE + 128 + 32 * h2;
+#pragma unroll
+        for (int a = 0; a < 4; ++a) {
+          const f32x4 v = *reinterpret_cast<const TATTN_LDS f32x4*>(nd + 64 * (a >> 1) + 16 * (a & 1));
+#pragma unroll
+          for (int e = 0; e < 4; ++e) s[4 * a + e] = v[e];
+        }
+      } else {
+        s = f32x16{};
+      }
+#pragma unroll
+      for (int sd = 0; sd < NSD; ++sd) s = Elt<T>::mfma(lds8<T>(st + (RB_ ? TILE : 0) + nat[sd]), kv[sd], s);
+    };
+    // dV += P^T dO (A), dK += dS^T Q (B).
+    auto grad = [&](const V8 (&op)[2], const char* st) __attribute__((always_inline)) {
+#pragma unroll
+      for (int sl = 0; sl < 2; ++sl)
+#pragma unroll
+        for (int u = 0; u < DT; ++u)
+          acc[u] = Elt<T>::mfma(op[sl], tr_pair<T>(st + (RB_ ? 0 : TILE) + 16 * sl * RB, lo[u], hi[u]), acc[u]);
+    };
+    auto probs = [&](f32x16& s, V8 (&pp)[2], const char* st, char* x, const Look& l, auto mask_tag) __attribute__((always_inline)) {
+      constexpr bool MASK = decltype(mask_tag)::value;
+      const int gap0 = off + 32 * l.qt + 8 * h2 - key, left = p.N - 32 * l.qt - 8 * h2;
+#pragma unroll
+      for (int a = 0; a < 4; ++a) {
+        const f32x4 m = *reinterpret_cast<const TATTN_LDS f32x4*>((const TATTN_LDS char*)st + 2 * TILE + 32 * h2 + 64 * (a >> 1) + 16 * (a & 1));
+        f32x4 pv;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int o = 16 * (a >> 1) + 4 * (a & 1) + e;
+          pv[e] = fast_exp2(__builtin_fmaf(s[4 * a + e], c, -m[e]));
+          if (MASK) {
+            const int gap = gap0 + o;
+            pv[e] = gap < 0 || (gap >= p.window && key >= p.sinks) || o >= left ? 0.0f : pv[e];
+          }
+        }
+        *reinterpret_cast<TATTN_LDS f32x4*>((TATTN_LDS char*)x + pr * XB + 1024 * a + 16 * lane) = pv;
+        const V2 a0 = H::pack(pv[0], pv[1]), a1 = H::pack(pv[2], pv[3]);
+        V8& o8 = pp[a >> 1];
+        o8[4 * (a & 1)] = a0[0], o8[4 * (a & 1) + 1] = a0[1], o8[4 * (a & 1) + 2] = a1[0], o8[4 * (a & 1) + 3] = a1[1];
+      }
+    };
+    auto dsv = [&](const f32x16& dp, V8 (&ds)[2], const char* x, auto mask_tag) __attribute__((always_inline)) {
+      constexpr bool MASK = decltype(mask_tag)::value;
+#pragma unroll
+      for (int a = 0; a < 4; ++a) {
+        const f32x4 pv = *reinterpret_cast<const TATTN_LDS f32x4*>((const TATTN_LDS char*)x + pr * XB + 1024 * a + 16 * lane);
+        float d[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) d[e] = MASK && pv[e] == 0.0f ? 0.0f : pv[e] * dp[4 * a + e];
+        const V2 a0 = H::pack(d[0], d[1]), a1 = H::pack(d[2], d[3]);
+        V8& o8 = ds[a >> 1];
+        o8[4 * (a & 1)] = a0[0], o8[4 * (a & 1) + 1] = a0[1], o8[4 * (a & 1) + 2] = a1[0], o8[4 * (a & 1) + 3] = a1[1];
+      }
+    };
+    f32x16 sa = f32x16{}, sb = f32x16{};
+    V8 pa[2] = {V8{}, V8{}}, pb[2] = {V8{}, V8{}};
+    int q = nq > 0 ? qt0 + i0 % nq : 0;
+    auto next_q = [&](int x) { return x + 1 == qt0 + nq ? qt0 : x + 1; };
+    Look prev{0, false, false}, cur = look(q, 0 < n);
+    if (!RB_ && cur.live) first(sa, st0);
+    // Step i at stage I = i % 4. A: s0 = S_i, s1 <- S_{i+1}; o0 = P_{i-1}, o1 <- P_i. B: s0 = dP_{i-1}, s1 <- dP_i.
+    auto step = [&](int i, auto tag, f32x16& s0, f32x16& s1, V8 (&o0)[2], V8 (&o1)[2]) __attribute__((always_inline)) {
+      constexpr int I = decltype(tag)::value;
+      char* xc = (I & 1) ? x1 : x0;
+      char* xp = (I & 1) ? x0 : x1;
+      q = next_q(q);
+      const Look nxt = look(q, i + 1 < n);
+      fetch(stage(IC<I + 2>{}));
+      if constexpr (!RB_) {
+        if (nxt.live) first(s1, stage(IC<I + 1>{}));
+        if (prev.live) grad(o0, stage(IC<I + 3>{}));
+        if (cur.live) {
+          if (cur.masked) probs(s0, o1, stage(IC<I>{}), xc, cur, std::true_type{});
+          else probs(s0, o1, stage(IC<I>{}), xc, cur, std::false_type{});
+        }
+      } else {
+        if (cur.live) first(s1, stage(IC<I>{}));
+        if (prev.live) {
+          if (prev.masked) dsv(s0, o1, xp, std::true_type{});
+          else dsv(s0, o1, xp, std::false_type{});
+          grad(o1, stage(IC<I + 3>{}));
+        }
+      }
+      prev = cur;
+      cur = nxt;
+      all_landed_barrier();
+    };
+    for (int i = 0; i <= n; i += 4) {  // step n finishes the last tile; steps past it are empty
+      step(i, IC<0>{}, sa, sb, pa, pb);
+      step(i + 1, IC<1>{}, sb, sa, pb, pa);
+      step(i + 2, IC<2>{}, sa, sb, pa, pb);
+      step(i + 3, IC<3>{}, sb, sa, pb, pa);
+    }
+  };
+  fetch(st0);
+  fetch(st1);
+  all_landed_barrier();
+  if (role_b) run(std::true_type{});
+  else run(std::false_type{});
+
+  // Every wave has passed the last barrier and nothing is in flight. C register r of a lane: key 8 (r / 4) + 4 h2 + r % 4 of
+  // the tile, column 32 u + l32. A part's sums go out in float32; otherwise the tile is turned into rows through LDS.
+  const float mul = role_b ? p.scale : 1.0f;
+  if (parted) {
+    float* dst = p.part + (((int64_t)slice * kbs.sink_blocks + kb) * p.splits + split) * (2 * 32 * RW * D) +
+                 (role_b ? 0 : 32 * RW * D) + (int64_t)32 * pr * D;
+#pragma unroll
+    for (int u = 0; u < DT; ++u)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) dst[(8 * (r >> 2) + 4 * h2 + (r & 3)) * D + 32 * u + l32] = acc[u][r];
+    return;
+  }
+  T* dst = role_b ? (T*)p.dk + z * p.sdk[0] + hk * p.sdk[1] : (T*)p.dv + z * p.sdv[0] + hk * p.sdv[1];
+  const int64_t dst_row = role_b ? p.sdk[2] : p.sdv[2];
+  constexpr int PER = STAGE / TILE;  // whole tiles per stage array: 2
+  static_assert(PER * 4 >= NW, "a block of rows per wave");
+  char* mine = (wu >> 1) == 0 ? st0 : (wu >> 1) == 1 ? st1 : (wu >> 1) == 2 ? st2 : st3;
+  mine += (wu & 1) * TILE;
+#pragma unroll
+  for (int u = 0; u < DT; ++u)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      const int row = 8 * (r >> 2) + 4 * h2 + (r & 3);
+      *reinterpret_cast<TATTN_LDS T*>((TATTN_LDS char*)mine + Swz<D>::addr(row, (32 * u + l32) * 2)) = (T)(acc[u][r] * mul);
+    }
+  constexpr int CPR = D / 8;
+#pragma unroll
+  for (int i = 0; i < 32 * CPR / 64; ++i) {
+    const int j = 64 * i + lane, row = j / CPR, cc = j % CPR;
+    const u32x4 v = *reinterpret_cast<const TATTN_LDS u32x4*>((const TATTN_LDS char*)mine + Swz<D>::addr(row, 16 * cc));
+    if (wk0 + row < p.S) st16(dst + (int64_t)(wk0 + row) * dst_row + 8 * cc, v);
+  }
+}
+
 // dK and dV of the key blocks whose queries were cut into parts.
 template <typename T, int D, int RW>
 __global__ __launch_bounds__(256) void window_first_keys_kernel(const WindowParams p) {
@@ -766,9 +1062,9 @@ __global__ __launch_bounds__(256) void window_first_keys_kernel(const WindowPara
 }
 
 // ---- launch ----------------------------------------------------------------------------------------
-// Row tiles per workgroup and tiles of the other dimension per step.
-template <int D> struct WinShape { static constexpr int RW = 2, CS = D == 128 ? 2 : 4; };
-template <int D> struct KeyShape { static constexpr int RW = D == 128 ? 4 : 2, CS = D == 128 ? 2 : 4; };
+// Row tiles per workgroup and key tiles per step.
+template <int D> struct WinShape { static constexpr int RW = 4, TP = 2, OCC = D == 128 ? 2 : 4; };
+template <int D> struct KeyShape { static constexpr int RW = D >= 64 ? 4 : 2, CS = 4; };
 
 int grid_of(int64_t slices, int64_t per_slice, unsigned* out) {
   const int64_t blocks = slices * per_slice + 8;
@@ -797,18 +1093,17 @@ int fwd_d(WindowParams p, hipStream_t st) {
     p.nblk = (int)((rows + 31) / 32);
     if ((rc = grid_of(slices, (int64_t)p.nblk * p.splits, &blocks))) return rc;
     if (p.splits == 1) {
-      window_fwd_kernel<T, D, 1, 4, D == 128 ? 1 : 2, false><<<dim3(blocks), dim3(256), 0, st>>>(p);
+      window_fwd_kernel<T, D, 1, 4, 1, D == 128 ? 1 : 2, false><<<dim3(blocks), dim3(256), 0, st>>>(p);
       return check_launch("tattn_window_fwd");
     }
-    window_fwd_kernel<T, D, 1, 4, D == 128 ? 1 : 2, true><<<dim3(blocks), dim3(256), 0, st>>>(p);
+    window_fwd_kernel<T, D, 1, 4, 1, D == 128 ? 1 : 2, true><<<dim3(blocks), dim3(256), 0, st>>>(p);
     if ((rc = check_launch("tattn_window_fwd"))) return rc;
     return launch_combine(p.part, p.out, p.m, p.sout, slices, p.Hk, p.G, p.N, p.splits, D, std::is_same_v<T, bf16> ? 2 : 0, st);
   }
   using S = WinShape<D>;
   p.nblk = (int)((rows + 32 * S::RW - 1) / (32 * S::RW));
   if ((rc = grid_of(slices, p.nblk, &blocks))) return rc;
-  constexpr int OCC = D == 128 ? 2 : 4;
-  window_fwd_kernel<T, D, S::RW, S::CS, OCC, false><<<dim3(blocks), dim3(S::RW * S::CS * 64), 0, st>>>(p);
+  window_fwd_kernel<T, D, S::RW, 1, S::TP, S::OCC, false><<<dim3(blocks), dim3(S::RW * 64), 0, st>>>(p);
   return check_launch("tattn_window_fwd");
 }
 
@@ -823,11 +1118,14 @@ int bwd_d(WindowParams p, hipStream_t st) {
   p.runs = in_runs(p);
   p.nblk = (int)((rows + 32 * S::RW - 1) / (32 * S::RW));
   if ((rc = grid_of(slices, p.nblk, &blocks))) return rc;
-  window_dq_kernel<T, D, S::RW, S::CS, D >= 64 ? 2 : 4><<<dim3(blocks), dim3(S::RW * S::CS * 64), 0, st>>>(p);
+  window_dq_kernel<T, D, S::RW, 1, S::TP, D >= 64 ? 2 : 4><<<dim3(blocks), dim3(S::RW * 64), 0, st>>>(p);
   if ((rc = check_launch("tattn_window_bwd"))) return rc;
   const KeyBlocks<K::RW> kbs(p.S, p.sinks, splits);
   if ((rc = grid_of(slices, kbs.items, &blocks))) return rc;
-  window_dkdv_kernel<T, D, K::RW, K::CS, D >= 64 ? 2 : D == 32 ? 3 : 4><<<dim3(blocks), dim3(K::RW * K::CS * 64), 0, st>>>(p);
+  if constexpr (D >= 64)
+    window_dkdv_pair_kernel<T, D, D == 64 ? 4 : 2><<<dim3(blocks), dim3(512), 0, st>>>(p);
+  else
+    window_dkdv_kernel<T, D, K::RW, K::CS, D == 32 ? 3 : 4><<<dim3(blocks), dim3(K::RW * K::CS * 64), 0, st>>>(p);
   if ((rc = check_launch("tattn_window_bwd")) || !kbs.sink_blocks) return rc;
   const int64_t n = slices * kbs.sink_blocks * 2 * 32 * K::RW * D;
   window_first_keys_kernel<T, D, K::RW><<<dim3((unsigned)((n + 255) / 256)), dim3(256), 0, st>>>(p);
@@ -868,7 +1166,7 @@ int window_fwd_splits(const WindowParams& p) {
 // work over four workgroups per CU where that is more.
 int window_bwd_splits(const WindowParams& p, int D) {
   if (p.sinks == 0) return 1;
-  const int64_t rw = D == 128 ? KeyShape<128>::RW : KeyShape<64>::RW, keys = 32 * rw;
+  const int64_t rw = D >= 64 ? KeyShape<64>::RW : KeyShape<32>::RW, keys = 32 * rw;
   const int64_t all = (int64_t)p.G * ((p.N + 31) / 32);
   const int64_t list = std::min<int64_t>(all, (int64_t)p.G * (std::min<int64_t>(p.window, p.S) / 32 + rw + 1));
   const int64_t share = (int64_t)p.Z * p.Hk * ((p.S + keys - 1) / keys) * list / 1024;
@@ -879,9 +1177,9 @@ int window_bwd_splits(const WindowParams& p, int D) {
 int64_t window_bwd_part_floats(const WindowParams& p, int D) {
   const int splits = window_bwd_splits(p, D);
   if (splits == 1) return 0;
-  const int64_t rw = D == 128 ? KeyShape<128>::RW : KeyShape<64>::RW;
-  const int64_t blocks = D == 128 ? KeyBlocks<KeyShape<128>::RW>(p.S, p.sinks, splits).sink_blocks
-                                  : KeyBlocks<KeyShape<64>::RW>(p.S, p.sinks, splits).sink_blocks;
+  const int64_t rw = D >= 64 ? KeyShape<64>::RW : KeyShape<32>::RW;
+  const int64_t blocks = D >= 64 ? KeyBlocks<KeyShape<64>::RW>(p.S, p.sinks, splits).sink_blocks
+                                 : KeyBlocks<KeyShape<32>::RW>(p.S, p.sinks, splits).sink_blocks;
   return (int64_t)p.Z * p.Hk * blocks * splits * 2 * 32 * rw * D;
 }
 
