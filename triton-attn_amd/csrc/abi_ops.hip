@@ -130,6 +130,10 @@ int check_tiles(const char* name, const void* ptr, const int64_t* st, int64_t ro
   return TATTN_OK;
 }
 
+// Scores to base-2 exponents. A scale of 0 becomes one so small that all exponents are 0 for finite scores below 1e22, because
+// hidden keys are marked by scores whose scaled value is -inf.
+float window_exponent_scale(float sm_scale) { return sm_scale == 0.0f ? 1.0e-30f : sm_scale * kLog2e; }
+
 int check_16bit(int dtype) {
   if (dtype != TATTN_F16 && dtype != TATTN_BF16)
     return set_error(TATTN_E_ARG, "dtype must be TATTN_F16 or TATTN_BF16, got %d", dtype);
@@ -296,7 +300,7 @@ int tattn_window_fwd(const void* q, const void* k, const void* v, void* o, float
   p.splits = window_fwd_splits(p);
   if ((rc = check_ptr("workspace", workspace, p.splits > 1, 16)) || (rc = require_device())) return rc;
   p.q = q; p.k = k; p.v = v; p.out = o; p.m = m; p.lens = lens; p.part = workspace;
-  p.c = sm_scale * kLog2e;
+  p.c = window_exponent_scale(sm_scale);
   p.scale = sm_scale;
   return launch_window_fwd(p, (int)D, dtype, (hipStream_t)stream);
 }
@@ -322,7 +326,7 @@ int tattn_window_bwd(const void* q, const void* k, const void* v, const void* o,
   p.m = const_cast<float*>(m);
   p.delta = delta;
   p.part = workspace;
-  p.c = sm_scale * kLog2e;
+  p.c = window_exponent_scale(sm_scale);
   p.scale = sm_scale;
   return launch_window_bwd(p, (int)D, dtype, (hipStream_t)stream);
 }

@@ -30,7 +30,12 @@ struct TileList {
   __device__ __forceinline__ int at(int i) const { return i < sink_tiles ? i : i - sink_tiles + first; }
 };
 
-// What a lane's row at position p hides in a tile: register r of lane-half h2 is key 32 t + 8 h2 + 16 (r / 8) + r % 8.
+// The raw score of a hidden key: its scaled value is -inf, so its probability is 0 whatever the row's max or log-sum-exp
+// (the entry points replace a scale of 0, where no such score exists, by a tiny one).
+__device__ __forceinline__ float hidden_score(float c) { return c < 0.0f ? __builtin_inff() : -__builtin_inff(); }
+
+
+// What a lane's row at position p hides in a tile of S^T: register r of lane-half h2 is key 32 t + 8 h2 + 16 (r / 8) + r % 8.
 struct RowMask {
   int hi, lb, sk;
   __device__ __forceinline__ RowMask(int p, int t, int h2, int window, int sinks) {
@@ -39,9 +44,30 @@ struct RowMask {
     lb = hi - window + 1;
     sk = sinks - base;
   }
-  __device__ __forceinline__ bool hides(int r) const {
-    const int off = 16 * (r >> 3) + (r & 7);
-    return off > hi || (off < lb && off >= sk);
+  __device__ __forceinline__ void hide(f32x16& s, float hidden) const {
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      const int off = 16 * (r >> 3) + (r & 7);
+      s[r] = off > hi || (off < lb && off >= sk) ? hidden : s[r];
+    }
+  }
+};
+
+// The same where the lane is a key and register r a query of a tile of S: `gap` from the key to the tile's first
+// position, `rows` left from there to the last query.
+struct ColMask {
+  int gap, window, rows;
+  __device__ __forceinline__ ColMask(int gap_, int key, int rows_, int h2, int window_, int sinks) {
+    gap = gap_ + 8 * h2;
+    rows = rows_ - 8 * h2;
+    window = key < sinks ? 0x7fffffff : window_;
+  }
+  __device__ __forceinline__ void hide(f32x16& s, float hidden) const {
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      const int off = 16 * (r >> 3) + (r & 7);
+      s[r] = gap + off < 0 || gap + off >= window || off >= rows ? hidden : s[r];
+    }
   }
 };
 

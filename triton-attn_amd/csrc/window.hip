@@ -191,26 +191,21 @@ __global__ __launch_bounds__(RW * CS * 64, OCC) void window_fwd_kernel(const Win
   WinOp<D> at;
   at.init(cs * R::TILE, lane);
 
+  const float hidden = hidden_score(c);
   float mrow = kNoMax, lrow = 0.0f;
   f32x16 acc[DT];
 #pragma unroll
   for (int u = 0; u < DT; ++u) acc[u] = f32x16{};
 
   // Tile t, staged in `st`. Probabilities against the running max as it stands; a lane whose 16 probabilities sum above
-  // 2^12 (its first visible tile among them) sends the wave through the row max and a rescale. The branch is
-  // one-sided (state updated first, undone inside): a two-sided one makes the allocator hold two copies of it.
-  auto tile = [&](const char* st, int t, auto mask_tag) __attribute__((always_inline)) {
-    constexpr bool MASK = decltype(mask_tag)::value;
-    const RowMask hide(pos, t, h2, p.window, p.sinks);
+  // 2^12 (its first visible tile among them) sends the wave through the row max and a rescale. The branches are
+  // one-sided (state updated first, undone inside): two-sided ones make the allocator hold two copies of it and copy the
+  // accumulators in every tile.
+  auto tile = [&](const char* st, int t) __attribute__((always_inline)) {
     f32x16 s = f32x16{};
 #pragma unroll
     for (int sd = 0; sd < NSD; ++sd) s = Elt<T>::mfma(lds8<T>(st + at.nat[sd]), qop[sd], s);
-    // Masked: scaled scores with hidden ones at -inf, whatever lies there (the running max is finite).
-    if (MASK) {
-#pragma unroll
-      for (int r = 0; r < 16; ++r) s[r] = hide.hides(r) ? -__builtin_inff() : s[r] * c;
-    }
-    const float cc = MASK ? 1.0f : c;
+    if (tile_masked(wp0, wp1, t, p.window, p.sinks)) RowMask(pos, t, h2, p.window, p.sinks).hide(s, hidden);
     V8 x[2];
     auto probs = [&]() __attribute__((always_inline)) {
       float ps = 0.0f;
@@ -219,7 +214,7 @@ __global__ __launch_bounds__(RW * CS * 64, OCC) void window_fwd_kernel(const Win
 #pragma unroll
         for (int i = 0; i < 8; i += 2) {
           const int r = 8 * sg + i;
-          const V2 pr = H::pack(fast_exp2(__builtin_fmaf(s[r], cc, -mrow)), fast_exp2(__builtin_fmaf(s[r + 1], cc, -mrow)));
+          const V2 pr = H::pack(fast_exp2(__builtin_fmaf(s[r], c, -mrow)), fast_exp2(__builtin_fmaf(s[r + 1], c, -mrow)));
           ps = H::sum2(pr, ps);
           x[sg][i] = pr[0];
           x[sg][i + 1] = pr[1];
@@ -232,7 +227,7 @@ __global__ __launch_bounds__(RW * CS * 64, OCC) void window_fwd_kernel(const Win
     if (__builtin_amdgcn_ballot_w64(!(ps <= 4096.0f))) {
       float mx = kNoMax;
 #pragma unroll
-      for (int r = 0; r < 16; ++r) mx = __builtin_fmaxf(mx, s[r] * cc);
+      for (int r = 0; r < 16; ++r) mx = __builtin_fmaxf(mx, s[r] * c);
       const float cand = max_halves(mx);
       const float mnew = cand > mrow + kRescaleLog2 ? cand : mrow;
       const float alpha = fast_exp2(mrow - mnew);
@@ -259,8 +254,7 @@ __global__ __launch_bounds__(RW * CS * 64, OCC) void window_fwd_kernel(const Win
       if (k + x * CS >= i1) break;
       const int t = list.at(k + x * CS);
       if (tile_hidden(wp0, wp1, t, p.window, p.sinks)) continue;
-      if (tile_masked(wp0, wp1, t, p.window, p.sinks)) tile(cur + x * CS * R::TILE, t, std::true_type{});
-      else tile(cur + x * CS * R::TILE, t, std::false_type{});
+      tile(cur + x * CS * R::TILE, t);
     }
     all_landed_barrier();
   };
@@ -459,9 +453,8 @@ __global__ __launch_bounds__(RW * CS * 64, OCC) void window_dq_kernel(const Wind
 #pragma unroll
   for (int u = 0; u < DT; ++u) dq[u] = f32x16{};
 
-  auto tile = [&](const char* st, int t, auto mask_tag) __attribute__((always_inline)) {
-    constexpr bool MASK = decltype(mask_tag)::value;
-    const RowMask hide(pos, t, h2, p.window, p.sinks);
+  const float hidden = hidden_score(c);
+  auto tile = [&](const char* st, int t) __attribute__((always_inline)) {
     f32x16 s = f32x16{}, dp;
 #pragma unroll
     for (int r = 0; r < 16; ++r) dp[r] = -dl;  // seeds dP - delta
@@ -470,11 +463,9 @@ __global__ __launch_bounds__(RW * CS * 64, OCC) void window_dq_kernel(const Wind
       s = Elt<T>::mfma(lds8<T>(st + at.nat[sd]), qop[sd], s);
       dp = Elt<T>::mfma(lds8<T>(st + R::HALF + at.nat[sd]), dop[sd], dp);
     }
+    if (tile_masked(wp0, wp1, t, p.window, p.sinks)) RowMask(pos, t, h2, p.window, p.sinks).hide(s, hidden);
 #pragma unroll
-    for (int r = 0; r < 16; ++r) {
-      s[r] = fast_exp2(__builtin_fmaf(s[r], c, nm)) * dp[r];
-      if (MASK) s[r] = hide.hides(r) ? 0.0f : s[r];
-    }
+    for (int r = 0; r < 16; ++r) s[r] = fast_exp2(__builtin_fmaf(s[r], c, nm)) * dp[r];
     V8 ds[2];
 #pragma unroll
     for (int sl = 0; sl < 2; ++sl)
@@ -501,8 +492,7 @@ __global__ __launch_bounds__(RW * CS * 64, OCC) void window_dq_kernel(const Wind
       if (k + x * CS >= list.n) break;
       const int t = list.at(k + x * CS);
       if (tile_hidden(wp0, wp1, t, p.window, p.sinks)) continue;
-      if (tile_masked(wp0, wp1, t, p.window, p.sinks)) tile(cur + x * CS * R::TILE, t, std::true_type{});
-      else tile(cur + x * CS * R::TILE, t, std::false_type{});
+      tile(cur + x * CS * R::TILE, t);
     }
     all_landed_barrier();
   };
@@ -560,6 +550,216 @@ __global__ __launch_bounds__(RW * CS * 64, OCC) void window_dq_kernel(const Wind
       *reinterpret_cast<V4*>(orow + d0) = y;
     }
   }
+}
+
+// dQ at head dims 64 and 128: two waves per row tile, as for dK / dV below. Over each key tile wave j (role A) computes
+// S^T = K Q^T and P = 2^(S c - M) for B, and wave j + 4 (role B) dP - delta, dS = P (dP - delta) and dQ^T += K^T dS^T. Both share
+// a SIMD, so that A's exponentials run beside B's matrix instructions. In step i A takes tile i, B tile i - 1; tiles i + 1 and
+// i + 2 are on their way.
+template <typename T, int D, int OCC>
+__global__ __launch_bounds__(512, OCC) void window_dq_pair_kernel(const WindowParams p) {
+  using H = H16<T>;
+  using V8 = typename H::V8;
+  using V4 = typename H::V4;
+  using V2 = typename H::V2;
+  constexpr int RW = 4, NW = 8, NSD = D / 16, DT = D / 32, RB = Swz<D>::RB, TILE = 32 * RB;
+  constexpr int PW = 2 * TILE / 1024 / NW;  // 1 KB pieces per wave and step
+  constexpr int STAGE = 2 * TILE;
+  constexpr int XB = 32 * 32 * 4;           // P of a pair
+  __shared__ __attribute__((aligned(1024))) char st0[STAGE], st1[STAGE], st2[STAGE], st3[STAGE];
+  __shared__ __attribute__((aligned(1024))) char x0[RW * XB], x1[RW * XB];
+  auto stage = [&](auto tag) __attribute__((always_inline)) -> char* {
+    constexpr int I = decltype(tag)::value & 3;
+    return I == 0 ? st0 : I == 1 ? st1 : I == 2 ? st2 : st3;
+  };
+
+  const int tid = threadIdx.x;
+  const int lane = tid & 63, h2 = lane >> 5, l32 = lane & 31;
+  const int wu = (int)uniform32((uint32_t)(tid >> 6));
+  const int pr = wu & 3;
+  const bool role_b = wu >= 4;
+  const float c = p.c;
+  int slice, blk;
+  if (!window_coord(p.Z * p.Hk, p.nblk, p.runs, slice, blk)) return;
+  WinRows b;
+  b.init(p, slice, p.nblk - 1 - blk, RW);
+  TileList list;
+  list.init(b.p0, b.p1, p.window, p.sinks);
+  const int nt = list.n;
+
+  const int64_t rowst = role_b ? p.sv[2] : p.sk[2];
+  const __amdgpu_buffer_rsrc_t rs = role_b ? win_rsrc<T, D>(p.v, b.z * p.sv[0] + b.hk * p.sv[1], b.len, rowst)
+                                           : win_rsrc<T, D>(p.k, b.z * p.sk[0] + b.hk * p.sk[1], b.len, rowst);
+  const uint32_t tile_bytes = uniform32((uint32_t)(rowst * 64));
+  uint32_t go[PW];
+  int krow[PW];
+#pragma unroll
+  for (int i = 0; i < PW; ++i) {
+    constexpr int CPR = RB / 16;
+    const int j = 64 * ((wu & 3) * PW + i) + lane, row = j / CPR;
+    krow[i] = perm32(row);
+    go[i] = (uint32_t)(perm32(row) * rowst * 2 + (((j % CPR) ^ Swz<D>::f(row)) & (D / 8 - 1)) * 16);
+  }
+  // Entry i, or past the end the last one again, into a stage that nobody reads: every step has as many loads in flight.
+  auto fetch = [&](char* st, int i) __attribute__((always_inline)) {
+    const int t = list.at(min(i, nt - 1));
+    const uint32_t o = (uint32_t)t * tile_bytes;
+    const bool edge = 32 * t + 31 > b.top || (32 * t < list.lo && 32 * t + 31 >= p.sinks);
+#pragma unroll
+    for (int x = 0; x < PW; ++x) {
+      uint32_t at = go[x] + o;
+      if (edge) {
+        const int key = 32 * t + krow[x];
+        if (key > b.top || (key < list.lo && key >= p.sinks)) at = kBeyond;
+      }
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (TATTN_LDS void*)(st + (wu * PW + x) * 1024), 16, (int)at, 0, 0, 0);
+    }
+  };
+  // End of a step: the loads of the step before have landed, this step's may stay in flight; LDS accesses are done.
+  auto step_end = [&]() __attribute__((always_inline)) {
+    __builtin_amdgcn_s_waitcnt(0x0070 | PW);
+    __atomic_signal_fence(__ATOMIC_SEQ_CST);
+    __builtin_amdgcn_s_barrier();
+    __atomic_signal_fence(__ATOMIC_SEQ_CST);
+  };
+  if (nt > 0) {
+    fetch(st0, 0);
+    fetch(st1, 1);
+  }
+
+  const int tile0 = 32 * (b.tile0 + pr);
+  const int row = tile0 + l32;
+  const bool live = row < b.rows;
+  const int n = (live ? row : 0) / p.G, g = (live ? row : 0) % p.G, h = b.hk * p.G + g;
+  const int pos = b.off + n;
+  const int wp0 = b.off + tile0 / p.G, wp1 = tile0 < b.rows ? b.off + min(tile0 + 31, b.rows - 1) / p.G : -1;
+  const int64_t mrow = ((int64_t)b.z * p.H + h) * p.N + n;
+  V8 op[NSD];       // Q (A) or dO (B)
+  float seed;       // -M (A) or -delta (B)
+  {
+    const T* src = role_b ? (const T*)p.dout + b.z * p.sd[0] + h * p.sd[1] + n * p.sd[2] + 8 * h2
+                          : (const T*)p.q + b.z * p.sq[0] + h * p.sq[1] + n * p.sq[2] + 8 * h2;
+#pragma unroll
+    for (int s = 0; s < NSD; ++s) {
+      const V8 x = *reinterpret_cast<const V8*>(src + 16 * s);
+      op[s] = live ? x : V8{};
+    }
+    if (role_b) {
+      const T* os = (const T*)p.o + b.z * p.so[0] + h * p.so[1] + n * p.so[2] + 8 * h2;
+      float sd[NSD];
+#pragma unroll
+      for (int s = 0; s < NSD; ++s) sd[s] = chunk_dot(*reinterpret_cast<const V8*>(os + 16 * s), op[s]);
+      seed = live ? -row_delta(sd) : 0.0f;
+      if (live && h2 == 0) p.delta[mrow] = seed;
+    } else {
+      seed = live ? -p.m[mrow] : 0.0f;
+    }
+  }
+  int nat[NSD], lo[DT], hi[DT];
+#pragma unroll
+  for (int s = 0; s < NSD; ++s) nat[s] = Swz<D>::addr(l32, (16 * s + 8 * h2) * 2);
+#pragma unroll
+  for (int u = 0; u < DT; ++u) tr_addrs<D>(0, u, lane, lo[u], hi[u]);
+  const float hidden = hidden_score(c);
+  f32x16 dq[DT];
+#pragma unroll
+  for (int u = 0; u < DT; ++u) dq[u] = f32x16{};
+
+  struct Look {
+    int t;
+    bool live, masked;
+  };
+  auto look = [&](int i) __attribute__((always_inline)) {
+    Look l{0, false, false};
+    if (i < nt) {
+      l.t = list.at(i);
+      l.live = !tile_hidden(wp0, wp1, l.t, p.window, p.sinks);
+      l.masked = tile_masked(wp0, wp1, l.t, p.window, p.sinks);
+    }
+    return l;
+  };
+  auto run = [&](auto role_tag) __attribute__((always_inline)) {
+    constexpr bool RB_ = decltype(role_tag)::value;
+    auto first = [&](f32x16& s, const char* st) __attribute__((always_inline)) {
+#pragma unroll
+      for (int r = 0; r < 16; ++r) s[r] = RB_ ? seed : 0.0f;
+#pragma unroll
+      for (int sd = 0; sd < NSD; ++sd) s = Elt<T>::mfma(lds8<T>(st + (RB_ ? TILE : 0) + nat[sd]), op[sd], s);
+    };
+    auto probs = [&](const f32x16& s, char* x) __attribute__((always_inline)) {
+#pragma unroll
+      for (int a = 0; a < 4; ++a) {
+        f32x4 pv;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) pv[e] = fast_exp2(__builtin_fmaf(s[4 * a + e], c, seed));
+        *reinterpret_cast<TATTN_LDS f32x4*>((TATTN_LDS char*)x + pr * XB + 1024 * a + 16 * lane) = pv;
+      }
+    };
+    auto dsv = [&](const f32x16& dp, V8 (&ds)[2], const char* x) __attribute__((always_inline)) {
+#pragma unroll
+      for (int a = 0; a < 4; ++a) {
+        const f32x4 pv = *reinterpret_cast<const TATTN_LDS f32x4*>((const TATTN_LDS char*)x + pr * XB + 1024 * a + 16 * lane);
+        float d[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) d[e] = pv[e] * dp[4 * a + e];
+        const V2 a0 = H::pack(d[0], d[1]), a1 = H::pack(d[2], d[3]);
+        V8& o8 = ds[a >> 1];
+        o8[4 * (a & 1)] = a0[0], o8[4 * (a & 1) + 1] = a0[1], o8[4 * (a & 1) + 2] = a1[0], o8[4 * (a & 1) + 3] = a1[1];
+      }
+    };
+    auto grad = [&](const V8 (&ds)[2], const char* st) __attribute__((always_inline)) {
+#pragma unroll
+      for (int sl = 0; sl < 2; ++sl)
+#pragma unroll
+        for (int u = 0; u < DT; ++u) dq[u] = Elt<T>::mfma(tr_pair<T>(st + 16 * sl * RB, lo[u], hi[u]), ds[sl], dq[u]);
+    };
+    Look prev{0, false, false};
+    auto step = [&](int i, auto tag) __attribute__((always_inline)) {
+      constexpr int I = decltype(tag)::value;
+      if (i > nt) return;
+      fetch(stage(IC<I + 2>{}), i + 2);
+      const Look cur = look(i);
+      if constexpr (!RB_) {
+        if (cur.live) {
+          f32x16 s;
+          first(s, stage(IC<I>{}));
+          if (cur.masked) RowMask(pos, cur.t, h2, p.window, p.sinks).hide(s, hidden);
+          probs(s, (I & 1) ? x1 : x0);
+        }
+      } else if (prev.live) {
+        f32x16 dp;
+        V8 ds[2];
+        first(dp, stage(IC<I + 3>{}));
+        dsv(dp, ds, (I & 1) ? x0 : x1);
+        grad(ds, stage(IC<I + 3>{}));
+      }
+      prev = cur;
+      step_end();
+    };
+    for (int i = 0; i <= nt; i += 4) {  // in step nt B finishes the last tile; none follows
+      step(i, IC<0>{});
+      step(i + 1, IC<1>{});
+      step(i + 2, IC<2>{});
+      step(i + 3, IC<3>{});
+    }
+  };
+  all_landed_barrier();
+  if (nt > 0) {
+    if (role_b) run(std::true_type{});
+    else run(std::false_type{});
+  }
+  __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0): no DMA may be in flight when the workgroup's LDS is released
+  if (!role_b || !live) return;
+  T* orow = (T*)p.out + b.z * p.sout[0] + h * p.sout[1] + n * p.sout[2];
+#pragma unroll
+  for (int u = 0; u < DT; ++u)
+#pragma unroll
+    for (int gr = 0; gr < 4; ++gr) {
+      V4 y;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) y[e] = (T)(dq[u][4 * gr + e] * p.scale);
+      *reinterpret_cast<V4*>(orow + 32 * u + 8 * gr + 4 * h2) = y;
+    }
 }
 
 // ---- dK / dV -------------------------------------------------------------------------------------
@@ -665,8 +865,8 @@ __global__ __launch_bounds__(RW * CS * 64, OCC) void window_dkdv_kernel(const Wi
 #pragma unroll
   for (int u = 0; u < DT; ++u) dk[u] = dv[u] = f32x16{};
 
-  auto tile = [&](const char* st, const float* mdw, int qt, auto mask_tag) __attribute__((always_inline)) {
-    constexpr bool MASK = decltype(mask_tag)::value;
+  const float hidden = hidden_score(c);
+  auto tile = [&](const char* st, const float* mdw, int qt, bool masked) __attribute__((always_inline)) {
     f32x16 s = f32x16{}, dp;
     float mv[16];
 #pragma unroll
@@ -688,18 +888,9 @@ __global__ __launch_bounds__(RW * CS * 64, OCC) void window_dkdv_kernel(const Wi
       else vo = vop[sd];
       dp = Elt<T>::mfma(lds8<T>(st + R::HALF + at.nat[sd]), vo, dp);
     }
-    // Register r is query 32 qt + 8 h2 + 16 (r / 8) + r % 8 at position `off` further, the lane's key is `key`.
-    const int first = off + 32 * qt + 8 * h2 - key;
+    if (masked) ColMask(off + 32 * qt - key, key, p.N - 32 * qt, h2, p.window, p.sinks).hide(s, hidden);
 #pragma unroll
-    for (int r = 0; r < 16; ++r) {
-      s[r] = fast_exp2(__builtin_fmaf(s[r], c, -mv[r]));
-      if (MASK) {
-        const int gap = first + 16 * (r >> 3) + (r & 7);
-        const bool hide = gap < 0 || (gap >= p.window && key >= p.sinks) || 16 * (r >> 3) + (r & 7) >= p.N - 32 * qt - 8 * h2;
-        s[r] = hide ? 0.0f : s[r];
-        dp[r] = hide ? 0.0f : dp[r];
-      }
-    }
+    for (int r = 0; r < 16; ++r) s[r] = fast_exp2(__builtin_fmaf(s[r], c, -mv[r]));
     V8 pp[2], ds[2];
 #pragma unroll
     for (int sl = 0; sl < 2; ++sl)
@@ -734,8 +925,7 @@ __global__ __launch_bounds__(RW * CS * 64, OCC) void window_dkdv_kernel(const Wi
     if (k < i1 && wk0 < p.S) {
       const int qt = qt0 + k % nq, q0 = off + 32 * qt, q1 = q0 + 31;
       if (q1 >= wk0 && (q0 - wk1 < p.window || wk0 < p.sinks)) {
-        if (q0 < wk1 || (q1 - wk0 >= p.window && wk1 >= p.sinks) || 32 * qt + 32 > p.N) tile(cur, md[wu][par], qt, std::true_type{});
-        else tile(cur, md[wu][par], qt, std::false_type{});
+        tile(cur, md[wu][par], qt, q0 < wk1 || (q1 - wk0 >= p.window && wk1 >= p.sinks) || 32 * qt + 32 > p.N);
       }
     }
     md[wu][par ^ 1][lane] = mdn;  // the wave's own rows: no barrier needed
@@ -790,8 +980,8 @@ __global__ __launch_bounds__(RW * CS * 64, OCC) void window_dkdv_kernel(const Wi
 // P = 2^(S c - M), dV += P^T dO, and wave j + 4 (role B) dP - delta = dO V^T - delta, dS = P (dP - delta), dK += dS^T Q,
 // taking P from A through LDS in float32. Each keeps one of K / V and one accumulator set: half the registers of a wave that
 // does both, so that two (head dim 128) or four waves (64) share a SIMD; as many matrix instructions in either role.
-// Step i, one barrier each: A runs S of tile i + 1 and dV of tile i - 1 on the matrix cores while its vector unit forms P of
-// tile i; B runs dP of tile i, then forms dS of tile i - 1 and runs its dK. Tile i + 2 is on its way to the fourth stage.
+// Step i, one barrier each: A takes tile i, B tile i - 1, and tiles i + 1 and i + 2 are on their way. Nothing is
+// pipelined inside a wave: the waves of a SIMD overlap each other's matrix and vector work.
 template <typename T, int D, int OCC>
 __global__ __launch_bounds__(512, OCC) void window_dkdv_pair_kernel(const WindowParams p) {
   using H = H16<T>;
@@ -858,22 +1048,32 @@ __global__ __launch_bounds__(512, OCC) void window_dkdv_pair_kernel(const Window
     const int j = 64 * ((wu & 3) * PW + i) + lane, row = j / CPR;
     go[i] = (uint32_t)(perm32(row) * rowst * 2 + (((j % CPR) ^ Swz<D>::f(row)) & (D / 8 - 1)) * 16);
   }
-  int fg = nq > 0 ? i0 / nq : 0, fq = qt0 + (nq > 0 ? i0 % nq : 0), fi = 0;  // next tile to fetch
+  // Next tile to fetch. Past the last one its rows come again, into a stage that nobody reads: every step has as many
+  // loads in flight.
+  int fg = nq > 0 ? i0 / nq : 0, fq = qt0 + (nq > 0 ? i0 % nq : 0), fi = 1;
   auto fetch = [&](char* st) __attribute__((always_inline)) {
-    if (fi < n) {
-      const __amdgpu_buffer_rsrc_t rs = slice_rsrc(base + fg * head, bytes);  // rows past the last query read as zero
+    const __amdgpu_buffer_rsrc_t rs = slice_rsrc(base + fg * head, bytes);  // rows past the last query read as zero
 #pragma unroll
-      for (int i = 0; i < PW; ++i)
-        __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (TATTN_LDS void*)(st + (wu * PW + i) * 1024), 16,
-                                                 (int)(go[i] + (uint32_t)fq * tile_bytes), 0, 0, 0);
-      if (wu == 0) {
-        const float* src = md + (int64_t)fg * p.N + min(32 * fq + l32, p.N - 1);
-        __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)src,
-                                         (TATTN_LDS void*)(st + 2 * TILE), 4, 0, 0);
-      }
+    for (int i = 0; i < PW; ++i)
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (TATTN_LDS void*)(st + (wu * PW + i) * 1024), 16,
+                                               (int)(go[i] + (uint32_t)fq * tile_bytes), 0, 0, 0);
+    if (wu == 0) {
+      const float* src = md + (int64_t)fg * p.N + min(32 * fq + l32, p.N - 1);
+      __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)src,
+                                       (TATTN_LDS void*)(st + 2 * TILE), 4, 0, 0);
     }
-    ++fi;
-    if (++fq == qt0 + nq) fq = qt0, ++fg;
+    if (fi < n) {
+      ++fi;
+      if (++fq == qt0 + nq) fq = qt0, ++fg;
+    }
+  };
+  // End of a step: the loads of the step before have landed, this step's may stay in flight; LDS accesses are done.
+  auto step_end = [&]() __attribute__((always_inline)) {
+    if (wu == 0) __builtin_amdgcn_s_waitcnt(0x0070 | (PW + 1));
+    else __builtin_amdgcn_s_waitcnt(0x0070 | PW);
+    __atomic_signal_fence(__ATOMIC_SEQ_CST);
+    __builtin_amdgcn_s_barrier();
+    __atomic_signal_fence(__ATOMIC_SEQ_CST);
   };
 
   int nat[NSD], lo[DT], hi[DT];
@@ -881,6 +1081,7 @@ __global__ __launch_bounds__(512, OCC) void window_dkdv_pair_kernel(const Window
   for (int s = 0; s < NSD; ++s) nat[s] = Swz<D>::addr(l32, (16 * s + 8 * h2) * 2);
 #pragma unroll
   for (int u = 0; u < DT; ++u) tr_addrs<D>(0, u, lane, lo[u], hi[u]);
+  const float hidden = hidden_score(c);
   f32x16 acc[DT];  // dV (A) or dK (B)
 #pragma unroll
   for (int u = 0; u < DT; ++u) acc[u] = f32x16{};
@@ -925,86 +1126,73 @@ __global__ __launch_bounds__(512, OCC) void window_dkdv_pair_kernel(const Window
         for (int u = 0; u < DT; ++u)
           acc[u] = Elt<T>::mfma(op[sl], tr_pair<T>(st + (RB_ ? 0 : TILE) + 16 * sl * RB, lo[u], hi[u]), acc[u]);
     };
-    auto probs = [&](f32x16& s, V8 (&pp)[2], const char* st, char* x, const Look& l, auto mask_tag) __attribute__((always_inline)) {
-      constexpr bool MASK = decltype(mask_tag)::value;
-      const int gap0 = off + 32 * l.qt + 8 * h2 - key, left = p.N - 32 * l.qt - 8 * h2;
+    auto probs = [&](const f32x16& s, V8 (&pp)[2], const char* st, char* x) __attribute__((always_inline)) {
 #pragma unroll
       for (int a = 0; a < 4; ++a) {
         const f32x4 m = *reinterpret_cast<const TATTN_LDS f32x4*>((const TATTN_LDS char*)st + 2 * TILE + 32 * h2 + 64 * (a >> 1) + 16 * (a & 1));
         f32x4 pv;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int o = 16 * (a >> 1) + 4 * (a & 1) + e;
-          pv[e] = fast_exp2(__builtin_fmaf(s[4 * a + e], c, -m[e]));
-          if (MASK) {
-            const int gap = gap0 + o;
-            pv[e] = gap < 0 || (gap >= p.window && key >= p.sinks) || o >= left ? 0.0f : pv[e];
-          }
-        }
+        for (int e = 0; e < 4; ++e) pv[e] = fast_exp2(__builtin_fmaf(s[4 * a + e], c, -m[e]));
         *reinterpret_cast<TATTN_LDS f32x4*>((TATTN_LDS char*)x + pr * XB + 1024 * a + 16 * lane) = pv;
         const V2 a0 = H::pack(pv[0], pv[1]), a1 = H::pack(pv[2], pv[3]);
         V8& o8 = pp[a >> 1];
         o8[4 * (a & 1)] = a0[0], o8[4 * (a & 1) + 1] = a0[1], o8[4 * (a & 1) + 2] = a1[0], o8[4 * (a & 1) + 3] = a1[1];
       }
     };
-    auto dsv = [&](const f32x16& dp, V8 (&ds)[2], const char* x, auto mask_tag) __attribute__((always_inline)) {
-      constexpr bool MASK = decltype(mask_tag)::value;
+    auto dsv = [&](const f32x16& dp, V8 (&ds)[2], const char* x) __attribute__((always_inline)) {
 #pragma unroll
       for (int a = 0; a < 4; ++a) {
         const f32x4 pv = *reinterpret_cast<const TATTN_LDS f32x4*>((const TATTN_LDS char*)x + pr * XB + 1024 * a + 16 * lane);
         float d[4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) d[e] = MASK && pv[e] == 0.0f ? 0.0f : pv[e] * dp[4 * a + e];
+        for (int e = 0; e < 4; ++e) d[e] = pv[e] * dp[4 * a + e];
         const V2 a0 = H::pack(d[0], d[1]), a1 = H::pack(d[2], d[3]);
         V8& o8 = ds[a >> 1];
         o8[4 * (a & 1)] = a0[0], o8[4 * (a & 1) + 1] = a0[1], o8[4 * (a & 1) + 2] = a1[0], o8[4 * (a & 1) + 3] = a1[1];
       }
     };
-    f32x16 sa = f32x16{}, sb = f32x16{};
-    V8 pa[2] = {V8{}, V8{}}, pb[2] = {V8{}, V8{}};
     int q = nq > 0 ? qt0 + i0 % nq : 0;
-    auto next_q = [&](int x) { return x + 1 == qt0 + nq ? qt0 : x + 1; };
-    Look prev{0, false, false}, cur = look(q, 0 < n);
-    if (!RB_ && cur.live) first(sa, st0);
-    // Step i at stage I = i % 4. A: s0 = S_i, s1 <- S_{i+1}; o0 = P_{i-1}, o1 <- P_i. B: s0 = dP_{i-1}, s1 <- dP_i.
-    auto step = [&](int i, auto tag, f32x16& s0, f32x16& s1, V8 (&o0)[2], V8 (&o1)[2]) __attribute__((always_inline)) {
+    Look prev{0, false, false};
+    auto step = [&](int i, auto tag) __attribute__((always_inline)) {
       constexpr int I = decltype(tag)::value;
-      char* xc = (I & 1) ? x1 : x0;
-      char* xp = (I & 1) ? x0 : x1;
-      q = next_q(q);
-      const Look nxt = look(q, i + 1 < n);
+      if (i > n) return;
       fetch(stage(IC<I + 2>{}));
+      const Look cur = look(q, i < n);
+      q = q + 1 == qt0 + nq ? qt0 : q + 1;
       if constexpr (!RB_) {
-        if (nxt.live) first(s1, stage(IC<I + 1>{}));
-        if (prev.live) grad(o0, stage(IC<I + 3>{}));
         if (cur.live) {
-          if (cur.masked) probs(s0, o1, stage(IC<I>{}), xc, cur, std::true_type{});
-          else probs(s0, o1, stage(IC<I>{}), xc, cur, std::false_type{});
+          f32x16 s;
+          V8 pp[2];
+          first(s, stage(IC<I>{}));
+          if (cur.masked) ColMask(off + 32 * cur.qt - key, key, p.N - 32 * cur.qt, h2, p.window, p.sinks).hide(s, hidden);
+          probs(s, pp, stage(IC<I>{}), (I & 1) ? x1 : x0);
+          grad(pp, stage(IC<I>{}));
         }
-      } else {
-        if (cur.live) first(s1, stage(IC<I>{}));
-        if (prev.live) {
-          if (prev.masked) dsv(s0, o1, xp, std::true_type{});
-          else dsv(s0, o1, xp, std::false_type{});
-          grad(o1, stage(IC<I + 3>{}));
-        }
+      } else if (prev.live) {
+        f32x16 dp;
+        V8 ds[2];
+        first(dp, stage(IC<I + 3>{}));
+        dsv(dp, ds, (I & 1) ? x0 : x1);
+        grad(ds, stage(IC<I + 3>{}));
       }
       prev = cur;
-      cur = nxt;
-      all_landed_barrier();
+      step_end();
     };
-    for (int i = 0; i <= n; i += 4) {  // step n finishes the last tile; steps past it are empty
-      step(i, IC<0>{}, sa, sb, pa, pb);
-      step(i + 1, IC<1>{}, sb, sa, pb, pa);
-      step(i + 2, IC<2>{}, sa, sb, pa, pb);
-      step(i + 3, IC<3>{}, sb, sa, pb, pa);
+    for (int i = 0; i <= n; i += 4) {  // in step n B finishes the last tile; none follows
+      step(i, IC<0>{});
+      step(i + 1, IC<1>{});
+      step(i + 2, IC<2>{});
+      step(i + 3, IC<3>{});
     }
   };
-  fetch(st0);
-  fetch(st1);
-  all_landed_barrier();
-  if (role_b) run(std::true_type{});
-  else run(std::false_type{});
+  if (n > 0) {
+    fetch(st0);
+    fetch(st1);
+    all_landed_barrier();
+    if (role_b) run(std::true_type{});
+    else run(std::false_type{});
+    all_landed_barrier();
+  }
 
   // Every wave has passed the last barrier and nothing is in flight. C register r of a lane: key 8 (r / 4) + 4 h2 + r % 4 of
   // the tile, column 32 u + l32. A part's sums go out in float32; otherwise the tile is turned into rows through LDS.
@@ -1118,7 +1306,10 @@ int bwd_d(WindowParams p, hipStream_t st) {
   p.runs = in_runs(p);
   p.nblk = (int)((rows + 32 * S::RW - 1) / (32 * S::RW));
   if ((rc = grid_of(slices, p.nblk, &blocks))) return rc;
-  window_dq_kernel<T, D, S::RW, 1, S::TP, D >= 64 ? 2 : 4><<<dim3(blocks), dim3(S::RW * 64), 0, st>>>(p);
+  if constexpr (D >= 64)
+    window_dq_pair_kernel<T, D, D == 64 ? 4 : 2><<<dim3(blocks), dim3(512), 0, st>>>(p);
+  else
+    window_dq_kernel<T, D, S::RW, 1, S::TP, 4><<<dim3(blocks), dim3(S::RW * 64), 0, st>>>(p);
   if ((rc = check_launch("tattn_window_bwd"))) return rc;
   const KeyBlocks<K::RW> kbs(p.S, p.sinks, splits);
   if ((rc = grid_of(slices, kbs.items, &blocks))) return rc;
