@@ -552,216 +552,6 @@ __global__ __launch_bounds__(RW * CS * 64, OCC) void window_dq_kernel(const Wind
   }
 }
 
-// dQ at head dims 64 and 128: two waves per row tile, as for dK / dV below. Over each key tile wave j (role A) computes
-// S^T = K Q^T and P = 2^(S c - M) for B, and wave j + 4 (role B) dP - delta, dS = P (dP - delta) and dQ^T += K^T dS^T. Both share
-// a SIMD, so that A's exponentials run beside B's matrix instructions. In step i A takes tile i, B tile i - 1; tiles i + 1 and
-// i + 2 are on their way.
-template <typename T, int D, int OCC>
-__global__ __launch_bounds__(512, OCC) void window_dq_pair_kernel(const WindowParams p) {
-  using H = H16<T>;
-  using V8 = typename H::V8;
-  using V4 = typename H::V4;
-  using V2 = typename H::V2;
-  constexpr int RW = 4, NW = 8, NSD = D / 16, DT = D / 32, RB = Swz<D>::RB, TILE = 32 * RB;
-  constexpr int PW = 2 * TILE / 1024 / NW;  // 1 KB pieces per wave and step
-  constexpr int STAGE = 2 * TILE;
-  constexpr int XB = 32 * 32 * 4;           // P of a pair
-  __shared__ __attribute__((aligned(1024))) char st0[STAGE], st1[STAGE], st2[STAGE], st3[STAGE];
-  __shared__ __attribute__((aligned(1024))) char x0[RW * XB], x1[RW * XB];
-  auto stage = [&](auto tag) __attribute__((always_inline)) -> char* {
-    constexpr int I = decltype(tag)::value & 3;
-    return I == 0 ? st0 : I == 1 ? st1 : I == 2 ? st2 : st3;
-  };
-
-  const int tid = threadIdx.x;
-  const int lane = tid & 63, h2 = lane >> 5, l32 = lane & 31;
-  const int wu = (int)uniform32((uint32_t)(tid >> 6));
-  const int pr = wu & 3;
-  const bool role_b = wu >= 4;
-  const float c = p.c;
-  int slice, blk;
-  if (!window_coord(p.Z * p.Hk, p.nblk, p.runs, slice, blk)) return;
-  WinRows b;
-  b.init(p, slice, p.nblk - 1 - blk, RW);
-  TileList list;
-  list.init(b.p0, b.p1, p.window, p.sinks);
-  const int nt = list.n;
-
-  const int64_t rowst = role_b ? p.sv[2] : p.sk[2];
-  const __amdgpu_buffer_rsrc_t rs = role_b ? win_rsrc<T, D>(p.v, b.z * p.sv[0] + b.hk * p.sv[1], b.len, rowst)
-                                           : win_rsrc<T, D>(p.k, b.z * p.sk[0] + b.hk * p.sk[1], b.len, rowst);
-  const uint32_t tile_bytes = uniform32((uint32_t)(rowst * 64));
-  uint32_t go[PW];
-  int krow[PW];
-#pragma unroll
-  for (int i = 0; i < PW; ++i) {
-    constexpr int CPR = RB / 16;
-    const int j = 64 * ((wu & 3) * PW + i) + lane, row = j / CPR;
-    krow[i] = perm32(row);
-    go[i] = (uint32_t)(perm32(row) * rowst * 2 + (((j % CPR) ^ Swz<D>::f(row)) & (D / 8 - 1)) * 16);
-  }
-  // Entry i, or past the end the last one again, into a stage that nobody reads: every step has as many loads in flight.
-  auto fetch = [&](char* st, int i) __attribute__((always_inline)) {
-    const int t = list.at(min(i, nt - 1));
-    const uint32_t o = (uint32_t)t * tile_bytes;
-    const bool edge = 32 * t + 31 > b.top || (32 * t < list.lo && 32 * t + 31 >= p.sinks);
-#pragma unroll
-    for (int x = 0; x < PW; ++x) {
-      uint32_t at = go[x] + o;
-      if (edge) {
-        const int key = 32 * t + krow[x];
-        if (key > b.top || (key < list.lo && key >= p.sinks)) at = kBeyond;
-      }
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (TATTN_LDS void*)(st + (wu * PW + x) * 1024), 16, (int)at, 0, 0, 0);
-    }
-  };
-  // End of a step: the loads of the step before have landed, this step's may stay in flight; LDS accesses are done.
-  auto step_end = [&]() __attribute__((always_inline)) {
-    __builtin_amdgcn_s_waitcnt(0x0070 | PW);
-    __atomic_signal_fence(__ATOMIC_SEQ_CST);
-    __builtin_amdgcn_s_barrier();
-    __atomic_signal_fence(__ATOMIC_SEQ_CST);
-  };
-  if (nt > 0) {
-    fetch(st0, 0);
-    fetch(st1, 1);
-  }
-
-  const int tile0 = 32 * (b.tile0 + pr);
-  const int row = tile0 + l32;
-  const bool live = row < b.rows;
-  const int n = (live ? row : 0) / p.G, g = (live ? row : 0) % p.G, h = b.hk * p.G + g;
-  const int pos = b.off + n;
-  const int wp0 = b.off + tile0 / p.G, wp1 = tile0 < b.rows ? b.off + min(tile0 + 31, b.rows - 1) / p.G : -1;
-  const int64_t mrow = ((int64_t)b.z * p.H + h) * p.N + n;
-  V8 op[NSD];       // Q (A) or dO (B)
-  float seed;       // -M (A) or -delta (B)
-  {
-    const T* src = role_b ? (const T*)p.dout + b.z * p.sd[0] + h * p.sd[1] + n * p.sd[2] + 8 * h2
-                          : (const T*)p.q + b.z * p.sq[0] + h * p.sq[1] + n * p.sq[2] + 8 * h2;
-#pragma unroll
-    for (int s = 0; s < NSD; ++s) {
-      const V8 x = *reinterpret_cast<const V8*>(src + 16 * s);
-      op[s] = live ? x : V8{};
-    }
-    if (role_b) {
-      const T* os = (const T*)p.o + b.z * p.so[0] + h * p.so[1] + n * p.so[2] + 8 * h2;
-      float sd[NSD];
-#pragma unroll
-      for (int s = 0; s < NSD; ++s) sd[s] = chunk_dot(*reinterpret_cast<const V8*>(os + 16 * s), op[s]);
-      seed = live ? -row_delta(sd) : 0.0f;
-      if (live && h2 == 0) p.delta[mrow] = seed;
-    } else {
-      seed = live ? -p.m[mrow] : 0.0f;
-    }
-  }
-  int nat[NSD], lo[DT], hi[DT];
-#pragma unroll
-  for (int s = 0; s < NSD; ++s) nat[s] = Swz<D>::addr(l32, (16 * s + 8 * h2) * 2);
-#pragma unroll
-  for (int u = 0; u < DT; ++u) tr_addrs<D>(0, u, lane, lo[u], hi[u]);
-  const float hidden = hidden_score(c);
-  f32x16 dq[DT];
-#pragma unroll
-  for (int u = 0; u < DT; ++u) dq[u] = f32x16{};
-
-  struct Look {
-    int t;
-    bool live, masked;
-  };
-  auto look = [&](int i) __attribute__((always_inline)) {
-    Look l{0, false, false};
-    if (i < nt) {
-      l.t = list.at(i);
-      l.live = !tile_hidden(wp0, wp1, l.t, p.window, p.sinks);
-      l.masked = tile_masked(wp0, wp1, l.t, p.window, p.sinks);
-    }
-    return l;
-  };
-  auto run = [&](auto role_tag) __attribute__((always_inline)) {
-    constexpr bool RB_ = decltype(role_tag)::value;
-    auto first = [&](f32x16& s, const char* st) __attribute__((always_inline)) {
-#pragma unroll
-      for (int r = 0; r < 16; ++r) s[r] = RB_ ? seed : 0.0f;
-#pragma unroll
-      for (int sd = 0; sd < NSD; ++sd) s = Elt<T>::mfma(lds8<T>(st + (RB_ ? TILE : 0) + nat[sd]), op[sd], s);
-    };
-    auto probs = [&](const f32x16& s, char* x) __attribute__((always_inline)) {
-#pragma unroll
-      for (int a = 0; a < 4; ++a) {
-        f32x4 pv;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) pv[e] = fast_exp2(__builtin_fmaf(s[4 * a + e], c, seed));
-        *reinterpret_cast<TATTN_LDS f32x4*>((TATTN_LDS char*)x + pr * XB + 1024 * a + 16 * lane) = pv;
-      }
-    };
-    auto dsv = [&](const f32x16& dp, V8 (&ds)[2], const char* x) __attribute__((always_inline)) {
-#pragma unroll
-      for (int a = 0; a < 4; ++a) {
-        const f32x4 pv = *reinterpret_cast<const TATTN_LDS f32x4*>((const TATTN_LDS char*)x + pr * XB + 1024 * a + 16 * lane);
-        float d[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) d[e] = pv[e] * dp[4 * a + e];
-        const V2 a0 = H::pack(d[0], d[1]), a1 = H::pack(d[2], d[3]);
-        V8& o8 = ds[a >> 1];
-        o8[4 * (a & 1)] = a0[0], o8[4 * (a & 1) + 1] = a0[1], o8[4 * (a & 1) + 2] = a1[0], o8[4 * (a & 1) + 3] = a1[1];
-      }
-    };
-    auto grad = [&](const V8 (&ds)[2], const char* st) __attribute__((always_inline)) {
-#pragma unroll
-      for (int sl = 0; sl < 2; ++sl)
-#pragma unroll
-        for (int u = 0; u < DT; ++u) dq[u] = Elt<T>::mfma(tr_pair<T>(st + 16 * sl * RB, lo[u], hi[u]), ds[sl], dq[u]);
-    };
-    Look prev{0, false, false};
-    auto step = [&](int i, auto tag) __attribute__((always_inline)) {
-      constexpr int I = decltype(tag)::value;
-      if (i > nt) return;
-      fetch(stage(IC<I + 2>{}), i + 2);
-      const Look cur = look(i);
-      if constexpr (!RB_) {
-        if (cur.live) {
-          f32x16 s;
-          first(s, stage(IC<I>{}));
-          if (cur.masked) RowMask(pos, cur.t, h2, p.window, p.sinks).hide(s, hidden);
-          probs(s, (I & 1) ? x1 : x0);
-        }
-      } else if (prev.live) {
-        f32x16 dp;
-        V8 ds[2];
-        first(dp, stage(IC<I + 3>{}));
-        dsv(dp, ds, (I & 1) ? x0 : x1);
-        grad(ds, stage(IC<I + 3>{}));
-      }
-      prev = cur;
-      step_end();
-    };
-    for (int i = 0; i <= nt; i += 4) {  // in step nt B finishes the last tile; none follows
-      step(i, IC<0>{});
-      step(i + 1, IC<1>{});
-      step(i + 2, IC<2>{});
-      step(i + 3, IC<3>{});
-    }
-  };
-  all_landed_barrier();
-  if (nt > 0) {
-    if (role_b) run(std::true_type{});
-    else run(std::false_type{});
-  }
-  __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0): no DMA may be in flight when the workgroup's LDS is released
-  if (!role_b || !live) return;
-  T* orow = (T*)p.out + b.z * p.sout[0] + h * p.sout[1] + n * p.sout[2];
-#pragma unroll
-  for (int u = 0; u < DT; ++u)
-#pragma unroll
-    for (int gr = 0; gr < 4; ++gr) {
-      V4 y;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) y[e] = (T)(dq[u][4 * gr + e] * p.scale);
-      *reinterpret_cast<V4*>(orow + 32 * u + 8 * gr + 4 * h2) = y;
-    }
-}
-
 // ---- dK / dV -------------------------------------------------------------------------------------
 // A workgroup owns RW tiles of 32 keys and walks the query tiles that see any of them, head after head of
 // the group: the sum over shared heads stays in registers. Key blocks that hold first keys are seen by every later query, an
@@ -778,19 +568,16 @@ struct KeyBlocks {
   }
 };
 
-template <typename T, int D, int RW, int CS, int OCC>
+template <typename T, int D, int RW, int CS, int TP, int OCC>
 __global__ __launch_bounds__(RW * CS * 64, OCC) void window_dkdv_kernel(const WindowParams p) {
   using H = H16<T>;
   using V8 = typename H::V8;
   using V2 = typename H::V2;
-  constexpr int NW = RW * CS, NSD = D / 16, DT = (D + 31) / 32;
-  // At head dim 128 the accumulators take 128 registers: V's operands then stay in LDS.
-  constexpr bool VLDS = D == 128;
-  using R = WinRing<D, NW, CS>;
+  constexpr int NW = RW * CS, NT = CS * TP, NSD = D / 16, DT = (D + 31) / 32;
+  using R = WinRing<D, NW, NT>;
   __shared__ __attribute__((aligned(1024))) char s0[R::STAGE];
   __shared__ __attribute__((aligned(1024))) char s1[R::STAGE];
-  __shared__ __attribute__((aligned(1024))) char sv[VLDS ? RW * R::TILE : 16];
-  __shared__ __attribute__((aligned(16))) float md[NW][2][64];  // per wave and parity: M[32], -delta[32]
+  __shared__ __attribute__((aligned(16))) float md[NW][2][TP][64];  // per wave, parity and tile: M[32], -delta[32]
 
   const int tid = threadIdx.x;
   const int lane = tid & 63, h2 = lane >> 5, l32 = lane & 31;
@@ -812,9 +599,9 @@ __global__ __launch_bounds__(RW * CS * 64, OCC) void window_dkdv_kernel(const Wi
   const int total = nq * p.G;
   const int i0 = parted ? (int)((int64_t)total * split / p.splits) : 0;
   const int i1 = parted ? (int)((int64_t)total * (split + 1) / p.splits) : total;
-  const int nsteps = (i1 - i0 + CS - 1) / CS;
+  const int nsteps = (i1 - i0 + NT - 1) / NT;
 
-  WinLoader<D, NW, CS> ld;
+  WinLoader<D, NW, NT> ld;
   ld.init(p.sq[2], p.sd[2], wu, lane);
   const char* qbase = ld.second ? (const char*)((const T*)p.dout + z * p.sd[0] + (int64_t)hk * p.G * p.sd[1])
                                 : (const char*)((const T*)p.q + z * p.sq[0] + (int64_t)hk * p.G * p.sq[1]);
@@ -823,7 +610,7 @@ __global__ __launch_bounds__(RW * CS * 64, OCC) void window_dkdv_kernel(const Wi
   auto issue = [&](char* stage, int step) __attribute__((always_inline)) {
 #pragma unroll
     for (int x = 0; x < R::TW; ++x) {
-      const int k = i0 + step * CS + ld.first + x;
+      const int k = i0 + step * NT + ld.first + x;
       if (k >= i1) break;
       const int g = k / nq, qt = qt0 + k % nq;
       // Rows past the head's last query lie past the end of its slice and read as zero.
@@ -835,14 +622,25 @@ __global__ __launch_bounds__(RW * CS * 64, OCC) void window_dkdv_kernel(const Wi
   if (nsteps > 0) issue(s0, 0);
   // Lanes 0-31 fetch M and lanes 32-63 -delta of the wave's tile; zero past the end.
   const float* mdsrc = (h2 ? p.delta : p.m) + ((int64_t)z * p.H + hk * p.G) * p.N;
-  auto md_load = [&](int step) {
-    const int k = i0 + step * CS + cs;
-    const int q = k < i1 ? 32 * (qt0 + k % nq) + l32 : p.N;
-    return q < p.N ? mdsrc[(int64_t)(k / nq) * p.N + q] : 0.0f;
+  auto md_load = [&](int step, float (&x)[TP]) __attribute__((always_inline)) {
+#pragma unroll
+    for (int t = 0; t < TP; ++t) {
+      const int k = i0 + step * NT + cs + t * CS;
+      const int q = k < i1 ? 32 * (qt0 + k % nq) + l32 : p.N;
+      x[t] = q < p.N ? mdsrc[(int64_t)(k / nq) * p.N + q] : 0.0f;
+    }
   };
-  md[wu][0][lane] = nsteps > 0 ? md_load(0) : 0.0f;
+  auto md_store = [&](int par, const float (&x)[TP]) __attribute__((always_inline)) {
+#pragma unroll
+    for (int t = 0; t < TP; ++t) md[wu][par][t][lane] = x[t];
+  };
+  float mdn[TP];
+  if (nsteps > 0) {
+    md_load(0, mdn);
+    md_store(0, mdn);
+  }
   const int kt = kb * RW + rw, key = 32 * kt + l32;
-  V8 kop[NSD], vop[VLDS ? 1 : NSD];
+  V8 kop[NSD], vop[NSD];
   {
     const T* ks = (const T*)p.k + z * p.sk[0] + hk * p.sk[1] + (int64_t)(key < p.S ? key : 0) * p.sk[2] + 8 * h2;
     const T* vs = (const T*)p.v + z * p.sv[0] + hk * p.sv[1] + (int64_t)(key < p.S ? key : 0) * p.sv[2] + 8 * h2;
@@ -851,12 +649,7 @@ __global__ __launch_bounds__(RW * CS * 64, OCC) void window_dkdv_kernel(const Wi
       const V8 a = *reinterpret_cast<const V8*>(ks + 16 * s);
       const V8 b = *reinterpret_cast<const V8*>(vs + 16 * s);
       kop[s] = key < p.S ? a : V8{};
-      const V8 x = key < p.S ? b : V8{};
-      if constexpr (VLDS) {
-        if (cs == 0) *reinterpret_cast<TATTN_LDS V8*>((TATTN_LDS char*)sv + rw * R::TILE + Swz<D>::addr(l32, (16 * s + 8 * h2) * 2)) = x;
-      } else {
-        vop[s] = x;
-      }
+      vop[s] = key < p.S ? b : V8{};
     }
   }
   WinOp<D> at;
@@ -883,10 +676,7 @@ __global__ __launch_bounds__(RW * CS * 64, OCC) void window_dkdv_kernel(const Wi
 #pragma unroll
     for (int sd = 0; sd < NSD; ++sd) {
       s = Elt<T>::mfma(lds8<T>(st + at.nat[sd]), kop[sd], s);
-      V8 vo;
-      if constexpr (VLDS) vo = lds8<T>(sv + rw * R::TILE + at.nat[sd] - cs * R::TILE);
-      else vo = vop[sd];
-      dp = Elt<T>::mfma(lds8<T>(st + R::HALF + at.nat[sd]), vo, dp);
+      dp = Elt<T>::mfma(lds8<T>(st + R::HALF + at.nat[sd]), vop[sd], dp);
     }
     if (masked) ColMask(off + 32 * qt - key, key, p.N - 32 * qt, h2, p.window, p.sinks).hide(s, hidden);
 #pragma unroll
@@ -916,19 +706,19 @@ __global__ __launch_bounds__(RW * CS * 64, OCC) void window_dkdv_kernel(const Wi
   };
   const int wk0 = 32 * kt, wk1 = wk0 + 31;
   auto step = [&](int i, char* cur, char* nxt, int par) __attribute__((always_inline)) {
-    float mdn = 0.0f;
     if (i + 1 < nsteps) {
       issue(nxt, i + 1);
-      mdn = md_load(i + 1);
+      md_load(i + 1, mdn);
     }
-    const int k = i0 + i * CS + cs;
-    if (k < i1 && wk0 < p.S) {
-      const int qt = qt0 + k % nq, q0 = off + 32 * qt, q1 = q0 + 31;
-      if (q1 >= wk0 && (q0 - wk1 < p.window || wk0 < p.sinks)) {
-        tile(cur, md[wu][par], qt, q0 < wk1 || (q1 - wk0 >= p.window && wk1 >= p.sinks) || 32 * qt + 32 > p.N);
-      }
+    const int k = i0 + i * NT + cs;
+#pragma unroll 1
+    for (int x = 0; x < TP; ++x) {
+      if (k + x * CS >= i1 || wk0 >= p.S) break;
+      const int qt = qt0 + (k + x * CS) % nq, q0 = off + 32 * qt, q1 = q0 + 31;
+      if (q1 >= wk0 && (q0 - wk1 < p.window || wk0 < p.sinks))
+        tile(cur + x * CS * R::TILE, md[wu][par][x], qt, q0 < wk1 || (q1 - wk0 >= p.window && wk1 >= p.sinks) || 32 * qt + 32 > p.N);
     }
-    md[wu][par ^ 1][lane] = mdn;  // the wave's own rows: no barrier needed
+    if (i + 1 < nsteps) md_store(par ^ 1, mdn);  // the wave's own rows: no barrier needed
     all_landed_barrier();
   };
   all_landed_barrier();
@@ -1306,17 +1096,14 @@ int bwd_d(WindowParams p, hipStream_t st) {
   p.runs = in_runs(p);
   p.nblk = (int)((rows + 32 * S::RW - 1) / (32 * S::RW));
   if ((rc = grid_of(slices, p.nblk, &blocks))) return rc;
-  if constexpr (D >= 64)
-    window_dq_pair_kernel<T, D, D == 64 ? 4 : 2><<<dim3(blocks), dim3(512), 0, st>>>(p);
-  else
-    window_dq_kernel<T, D, S::RW, 1, S::TP, 4><<<dim3(blocks), dim3(S::RW * 64), 0, st>>>(p);
+  window_dq_kernel<T, D, S::RW, 1, S::TP, D >= 64 ? 2 : 4><<<dim3(blocks), dim3(S::RW * 64), 0, st>>>(p);
   if ((rc = check_launch("tattn_window_bwd"))) return rc;
   const KeyBlocks<K::RW> kbs(p.S, p.sinks, splits);
   if ((rc = grid_of(slices, kbs.items, &blocks))) return rc;
   if constexpr (D >= 64)
     window_dkdv_pair_kernel<T, D, D == 64 ? 4 : 2><<<dim3(blocks), dim3(512), 0, st>>>(p);
   else
-    window_dkdv_kernel<T, D, K::RW, K::CS, D == 32 ? 3 : 4><<<dim3(blocks), dim3(K::RW * K::CS * 64), 0, st>>>(p);
+    window_dkdv_kernel<T, D, K::RW, K::CS, 1, D == 32 ? 3 : 4><<<dim3(blocks), dim3(K::RW * K::CS * 64), 0, st>>>(p);
   if ((rc = check_launch("tattn_window_bwd")) || !kbs.sink_blocks) return rc;
   const int64_t n = slices * kbs.sink_blocks * 2 * 32 * K::RW * D;
   window_first_keys_kernel<T, D, K::RW><<<dim3((unsigned)((n + 255) / 256)), dim3(256), 0, st>>>(p);

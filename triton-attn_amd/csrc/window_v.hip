@@ -1,0 +1,1182 @@
+// Attention over a sliding window and the first keys, 16-bit, forward and backward, on gfx950.
+//
+// A workgroup's NW = RW * CS waves own RW 32-row tiles; a step stages CS * TP tiles of the other dimension by LDS DMA
+// (buffer_load ... lds, swizzled rows) into one of two stages while the other is worked on. With many rows CS is 1 and each wave
+// works on all TP tiles of a step for its own rows; with few, wave (rw, cs) takes every CS-th tile, and the CS partial
+// results of a row tile are added through LDS at the end. Only tiles that some row of the workgroup sees are walked
+// (TileList), only those at the ends of a row's window pay for masks, and a wave passes over tiles that none of its own rows sees.
+//
+// Rows that nobody in the workgroup sees (before the window, behind the last key) are fetched from beyond the end of
+// the buffer, which reads as zero: whatever a cache holds there cannot reach a sum.
+#include <algorithm>
+#include <type_traits>
+
+#include "window.h"
+
+namespace tattn {
+namespace {
+
+// A stage: NT tiles of each of two tensors. Each wave fetches TW whole tiles of a step, the first half of the waves of
+// the first tensor.
+template <int D, int NW, int NT>
+struct WinRing {
+  static constexpr int RB = Swz<D>::RB, TILE = 32 * RB, PIECES = TILE / 1024;  // 1 KB DMA pieces
+  static constexpr int HALF = NT * TILE;  // bytes of one tensor's tiles
+  static constexpr int STAGE = 2 * HALF;
+  static constexpr int TW = 2 * NT / NW;
+  static_assert(TW >= 1 && TW * NW == 2 * NT && NW % 2 == 0, "whole tiles, one tensor per wave");
+};
+
+constexpr uint32_t kBeyond = 0x7fffffffu;  // byte offset past every slice: reads as zero
+
+template <int D, int NW, int NT>
+struct WinLoader {
+  using R = WinRing<D, NW, NT>;
+  uint32_t go[R::PIECES];
+  uint32_t tile_bytes;
+  int first, base, lane;  // first tile of the wave's TW, and its place in a stage
+  bool second;
+  __device__ __forceinline__ void init(int64_t sa, int64_t sb, int wu, int lane_) {
+    lane = lane_;
+    second = wu >= NW / 2;
+    const int64_t st = second ? sb : sa;
+    tile_bytes = uniform32((uint32_t)(st * 64));
+    first = wu % (NW / 2) * R::TW;
+    base = (second ? R::HALF : 0) + first * R::TILE;
+    constexpr int CPR = R::RB / 16;
+#pragma unroll
+    for (int i = 0; i < R::PIECES; ++i) {
+      const int j = 64 * i + lane;
+      const int row = j / CPR, cc = ((j % CPR) ^ Swz<D>::f(row)) & (D / 8 - 1);
+      go[i] = (uint32_t)(perm32(row) * st * 2 + cc * 16);
+    }
+  }
+  // Row of a tile that the lane fetches in piece i.
+  __device__ __forceinline__ int row(int i) const { return perm32((64 * i + lane) / (R::RB / 16)); }
+  __device__ __forceinline__ void fetch(__amdgpu_buffer_rsrc_t rs, char* stage, int x, int i, uint32_t off) const {
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (TATTN_LDS void*)(stage + base + x * R::TILE + 1024 * i), 16, (int)off, 0, 0, 0);
+  }
+};
+
+// Operand addresses within one tile at byte `base`: natural rows, and the transposed reads of 16-row slice 0 (the
+// swizzle depends on a row's index mod 16, so slice 1 is a constant further).
+template <int D>
+struct WinOp {
+  static constexpr int NSD = D / 16, DT = (D + 31) / 32;
+  int nat[NSD], lo[DT], hi[DT];
+  __device__ __forceinline__ void init(int base, int lane) {
+    const int l32 = lane & 31, h2 = lane >> 5;
+#pragma unroll
+    for (int s = 0; s < NSD; ++s) nat[s] = base + Swz<D>::addr(l32, (16 * s + 8 * h2) * 2);
+#pragma unroll
+    for (int u = 0; u < DT; ++u) {
+      tr_addrs<D>(0, u, lane, lo[u], hi[u]);
+      lo[u] += base;
+      hi[u] += base;
+    }
+  }
+  template <typename T>
+  __device__ __forceinline__ typename H16<T>::V8 tr(const char* st, int sl, int u) const {
+    return tr_pair<T>(st + 16 * sl * Swz<D>::RB, lo[u], hi[u]);
+  }
+};
+
+// The rows of a workgroup and of its waves, and the key tiles they see.
+struct WinRows {
+  int z, hk, slice, len, off;
+  int rows;      // N * G
+  int tile0;     // first row tile of the workgroup
+  int p0, p1;    // positions of the workgroup's rows
+  int top;       // last key any of them sees
+  __device__ __forceinline__ void init(const WindowParams& p, int slice_, int blk, int rw) {
+    slice = slice_;
+    z = slice / p.Hk;
+    hk = slice % p.Hk;
+    len = p.lens ? min(max(p.lens[z], 0), p.S) : p.S;
+    off = len - p.N;
+    rows = p.N * p.G;
+    tile0 = blk * rw;
+    p0 = off + (32 * tile0) / p.G;
+    p1 = off + min(32 * (tile0 + rw) - 1, rows - 1) / p.G;
+    top = p1;
+  }
+};
+
+template <typename T, int D>
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t win_rsrc(const void* base, int64_t off, int64_t rows, int64_t stride) {
+  return slice_rsrc((const T*)base + off, rows > 0 ? slice_bytes(rows, stride, D) : 0);
+}
+
+// K and V tiles of list entries [i0, i0 + NT) into `stage`; entries from i1 on are not fetched.
+template <int D, int NW, int NT>
+__device__ __forceinline__ void fetch_keys(const WinLoader<D, NW, NT>& ld, __amdgpu_buffer_rsrc_t rs, char* stage,
+                                           const TileList& list, int i0, int i1, int top, int sinks) {
+  using R = WinRing<D, NW, NT>;
+#pragma unroll
+  for (int x = 0; x < R::TW; ++x) {
+    const int at = i0 + ld.first + x;
+    if (at >= i1) break;
+    const int t = list.at(at);
+    const uint32_t o = (uint32_t)t * ld.tile_bytes;
+    if (32 * t + 31 > top || (32 * t < list.lo && 32 * t + 31 >= sinks)) {
+#pragma unroll
+      for (int i = 0; i < R::PIECES; ++i) {
+        const int key = 32 * t + ld.row(i);
+        const bool dead = key > top || (key < list.lo && key >= sinks);
+        ld.fetch(rs, stage, x, i, dead ? kBeyond : ld.go[i] + o);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < R::PIECES; ++i) ld.fetch(rs, stage, x, i, ld.go[i] + o);
+    }
+  }
+}
+
+// ---- forward -----------------------------------------------------------------------------------
+template <typename T, int D, int RW, int CS, int TP, int OCC, bool SPLIT>
+__global__ __launch_bounds__(RW * CS * 64, OCC) void window_fwd_kernel(const WindowParams p) {
+  using H = H16<T>;
+  using V8 = typename H::V8;
+  using V4 = typename H::V4;
+  using V2 = typename H::V2;
+  constexpr int NW = RW * CS, NT = CS * TP, NSD = D / 16, DT = (D + 31) / 32;
+  using R = WinRing<D, NW, NT>;
+  // Two arrays: a DMA into one stage does not alias reads of the other.
+  __shared__ __attribute__((aligned(1024))) char s0[R::STAGE];
+  __shared__ __attribute__((aligned(1024))) char s1[R::STAGE];
+  __shared__ float red[2][CS > 1 || SPLIT ? NW : 1][32];
+
+  const int tid = threadIdx.x;
+  const int lane = tid & 63, h2 = lane >> 5, l32 = lane & 31;
+  const int wu = (int)uniform32((uint32_t)(tid >> 6));
+  const int rw = wu / CS, cs = wu % CS;
+  const float c = p.c;
+  int slice, blk, split = 0;
+  if (!window_coord(p.Z * p.Hk, p.nblk * (SPLIT ? p.splits : 1), p.runs, slice, blk)) return;
+  if (SPLIT) split = blk % p.splits, blk /= p.splits;
+  WinRows b;
+  b.init(p, slice, p.nblk - 1 - blk, RW);  // longest rows first
+  TileList list;
+  list.init(b.p0, b.p1, p.window, p.sinks);
+  const int i0 = SPLIT ? (int)((int64_t)list.n * split / p.splits) : 0;
+  const int i1 = SPLIT ? (int)((int64_t)list.n * (split + 1) / p.splits) : list.n;
+  const int nsteps = (i1 - i0 + NT - 1) / NT;
+
+  WinLoader<D, NW, NT> ld;
+  ld.init(p.sk[2], p.sv[2], wu, lane);
+  const __amdgpu_buffer_rsrc_t rs =
+      ld.second ? win_rsrc<T, D>(p.v, b.z * p.sv[0] + b.hk * p.sv[1], b.len, p.sv[2])
+                : win_rsrc<T, D>(p.k, b.z * p.sk[0] + b.hk * p.sk[1], b.len, p.sk[2]);
+  auto issue = [&](char* stage, int step) __attribute__((always_inline)) {
+    fetch_keys<D, NW, NT>(ld, rs, stage, list, i0 + step * NT, i1, b.top, p.sinks);
+  };
+  if (nsteps > 0) issue(s0, 0);
+
+  const int tile0 = 32 * (b.tile0 + rw);
+  const int row = tile0 + l32;
+  const bool live = row < b.rows;
+  const int n = (live ? row : 0) / p.G, g = (live ? row : 0) % p.G;
+  const int pos = b.off + n;
+  // The wave's positions; a wave without rows sees no tile.
+  const int wp0 = b.off + tile0 / p.G, wp1 = tile0 < b.rows ? b.off + min(tile0 + 31, b.rows - 1) / p.G : -1;
+  V8 qop[NSD];
+  {
+    const T* src = (const T*)p.q + b.z * p.sq[0] + (b.hk * p.G + g) * p.sq[1] + n * p.sq[2] + 8 * h2;
+#pragma unroll
+    for (int s = 0; s < NSD; ++s) {
+      const V8 x = *reinterpret_cast<const V8*>(src + 16 * s);
+      qop[s] = live ? x : V8{};
+    }
+  }
+  WinOp<D> at;
+  at.init(cs * R::TILE, lane);
+
+  const float hidden = hidden_score(c);
+  float mrow = kNoMax, lrow = 0.0f;
+  f32x16 acc[DT];
+#pragma unroll
+  for (int u = 0; u < DT; ++u) acc[u] = f32x16{};
+
+  // Tile t, staged in `st`. Probabilities against the running max as it stands; a lane whose 16 probabilities sum above
+  // 2^12 (its first visible tile among them) sends the wave through the row max and a rescale. The branches are
+  // one-sided (state updated first, undone inside): two-sided ones make the allocator hold two copies of it and copy the
+  // accumulators in every tile.
+  auto tile = [&](const char* st, int t) __attribute__((always_inline)) {
+    f32x16 s = f32x16{};
+#pragma unroll
+    for (int sd = 0; sd < NSD; ++sd) s = Elt<T>::mfma(lds8<T>(st + at.nat[sd]), qop[sd], s);
+    if (tile_masked(wp0, wp1, t, p.window, p.sinks)) RowMask(pos, t, h2, p.window, p.sinks).hide(s, hidden);
+    V8 x[2];
+    auto probs = [&]() __attribute__((always_inline)) {
+      float ps = 0.0f;
+#pragma unroll
+      for (int sg = 0; sg < 2; ++sg)
+#pragma unroll
+        for (int i = 0; i < 8; i += 2) {
+          const int r = 8 * sg + i;
+          const V2 pr = H::pack(fast_exp2(__builtin_fmaf(s[r], c, -mrow)), fast_exp2(__builtin_fmaf(s[r + 1], c, -mrow)));
+          ps = H::sum2(pr, ps);
+          x[sg][i] = pr[0];
+          x[sg][i + 1] = pr[1];
+        }
+      return ps;
+    };
+    const float lprev = lrow;
+    const float ps = probs();
+    lrow += ps;
+    if (__builtin_amdgcn_ballot_w64(!(ps <= 4096.0f))) {
+      float mx = kNoMax;
+#pragma unroll
+      for (int r = 0; r < 16; ++r) mx = __builtin_fmaxf(mx, s[r] * c);
+      const float cand = max_halves(mx);
+      const float mnew = cand > mrow + kRescaleLog2 ? cand : mrow;
+      const float alpha = fast_exp2(mrow - mnew);
+      mrow = mnew;
+      const float again = probs();
+      lrow = lprev * alpha + again;
+#pragma unroll
+      for (int u = 0; u < DT; ++u) acc[u] *= alpha;
+    }
+#pragma unroll
+    for (int sg = 0; sg < 2; ++sg)
+#pragma unroll
+      for (int u = 0; u < DT; ++u) {
+        V8 va = at.template tr<T>(st + R::HALF, sg, u);
+        if (D < 32 && 16 * ((lane >> 4) & 1) >= D) va = V8{};
+        acc[u] = Elt<T>::mfma(va, x[sg], acc[u]);
+      }
+  };
+  auto step = [&](int i, char* cur, char* nxt) __attribute__((always_inline)) {
+    if (i + 1 < nsteps) issue(nxt, i + 1);
+    const int k = i0 + i * NT + cs;
+#pragma unroll 1
+    for (int x = 0; x < TP; ++x) {
+      if (k + x * CS >= i1) break;
+      const int t = list.at(k + x * CS);
+      if (tile_hidden(wp0, wp1, t, p.window, p.sinks)) continue;
+      tile(cur + x * CS * R::TILE, t);
+    }
+    all_landed_barrier();
+  };
+  all_landed_barrier();
+  int i = 0;
+  for (; i + 1 < nsteps; i += 2) {
+    step(i, s0, s1);
+    step(i + 1, s1, s0);
+  }
+  if (i < nsteps) step(i, s0, s1);
+
+  // Merge the CS partial rows of each row tile (the stages are free: every wave passed the last barrier and no
+  // DMA is in flight). A split keeps the sums as they are; otherwise they are divided by the row's sum, and rows
+  // that see no key become 0.
+  const float lt = sum_halves(lrow);
+  if constexpr (CS == 1 && !SPLIT) {
+    const float inv = lt == 0.0f ? 0.0f : 1.0f / lt;
+    if (!live) return;
+    T* orow = (T*)p.out + b.z * p.sout[0] + (b.hk * p.G + g) * p.sout[1] + n * p.sout[2];
+#pragma unroll
+    for (int u = 0; u < DT; ++u)
+#pragma unroll
+      for (int gr = 0; gr < 4; ++gr) {
+        const int d0 = 32 * u + 8 * gr + 4 * h2;
+        if (d0 >= D) continue;
+        V4 y;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) y[e] = (T)(acc[u][4 * gr + e] * inv);
+        *reinterpret_cast<V4*>(orow + d0) = y;
+      }
+    if (h2 == 0 && p.m) p.m[((int64_t)b.z * p.H + b.hk * p.G + g) * p.N + n] = mrow + __log2f(lt);
+    return;
+  }
+  if (h2 == 0) {
+    red[0][wu][l32] = mrow;
+    red[1][wu][l32] = lt;
+  }
+  __syncthreads();
+  float mall = kNoMax;
+#pragma unroll
+  for (int k = 0; k < CS; ++k) mall = __builtin_fmaxf(mall, red[0][rw * CS + k][l32]);
+  float lall = 0.0f;
+#pragma unroll
+  for (int k = 0; k < CS; ++k) lall += fast_exp2(red[0][rw * CS + k][l32] - mall) * red[1][rw * CS + k][l32];
+  float wgt = fast_exp2(mrow - mall);
+  if (!SPLIT) wgt = lall == 0.0f ? 0.0f : wgt / lall;
+  constexpr int PART = DT * 16 * 64 * 4;  // bytes of one wave's partial O^T
+  constexpr int PER = R::STAGE / PART;    // partials per stage array
+  static_assert((CS == 1 && !SPLIT) || 2 * PER >= NW, "partials fit the stages");
+  auto part = [&](int k) { return (TATTN_LDS float*)(k < PER ? s0 + k * PART : s1 + (k - PER) * PART); };
+  {
+    TATTN_LDS float* dst = part(wu) + lane;
+#pragma unroll
+    for (int u = 0; u < DT; ++u)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) dst[(16 * u + r) * 64] = acc[u][r] * wgt;
+  }
+  __syncthreads();
+  if (!live) return;
+  const int64_t prow = ((int64_t)b.slice * (SPLIT ? p.splits : 1) + split) * b.rows + row;
+  T* orow = (T*)p.out + b.z * p.sout[0] + (b.hk * p.G + g) * p.sout[1] + n * p.sout[2];
+  float* frow = p.part + prow * D;
+  for (int gr = cs; gr < DT * 4; gr += CS) {  // four consecutive columns per register group
+    const int d0 = 8 * gr + 4 * h2;
+    if (d0 < D) {
+      f32x4 x = f32x4{};
+#pragma unroll
+      for (int k = 0; k < CS; ++k) {
+        const TATTN_LDS float* src = part(rw * CS + k) + lane + 4 * gr * 64;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[e] += src[64 * e];
+      }
+      if (SPLIT) {
+        *reinterpret_cast<f32x4*>(frow + d0) = x;
+      } else {
+        V4 y;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) y[e] = (T)x[e];
+        *reinterpret_cast<V4*>(orow + d0) = y;
+      }
+    }
+  }
+  if (cs == 0 && h2 == 0) {
+    if (SPLIT) {
+      float* ml = p.part + (int64_t)p.Z * p.Hk * p.splits * b.rows * D + prow * 2;
+      ml[0] = mall;
+      ml[1] = lall;
+    } else if (p.m) {
+      p.m[((int64_t)b.z * p.H + b.hk * p.G + g) * p.N + n] = mall + __log2f(lall);
+    }
+  }
+}
+
+// ---- rows whose keys were split ------------------------------------------------------------------
+// O = sum_s 2^(m_s - m) O_s / sum_s 2^(m_s - m) l_s, D / 4 lanes per row.
+template <typename T, int D>
+__global__ __launch_bounds__(256) void combine_kernel(const float* part, T* out, float* m, int64_t sz, int64_t sh, int64_t sn,
+                                                      int64_t slices, int Hk, int G, int N, int splits) {
+  typedef T V4 __attribute__((ext_vector_type(4)));
+  constexpr int LPR = D / 4;
+  const int rows = N * G;
+  const int64_t r = (int64_t)blockIdx.x * (256 / LPR) + threadIdx.x / LPR;
+  if (r >= slices * rows) return;
+  const int64_t slice = r / rows;
+  const int row = (int)(r % rows), d0 = threadIdx.x % LPR * 4;
+  const float* ml = part + slices * splits * rows * D;
+  const int64_t first = slice * splits * rows + row;
+  float mall = kNoMax;
+  for (int s = 0; s < splits; ++s) mall = __builtin_fmaxf(mall, ml[(first + (int64_t)s * rows) * 2]);
+  f32x4 x = f32x4{};
+  float l = 0.0f;
+#pragma unroll 4
+  for (int s = 0; s < splits; ++s) {
+    const int64_t at = first + (int64_t)s * rows;
+    const float w = fast_exp2(ml[at * 2] - mall), ls = ml[at * 2 + 1];
+    if (ls == 0.0f) continue;  // no visible key: the sums of such a part may not be there
+    l = __builtin_fmaf(w, ls, l);
+    const f32x4 y = *reinterpret_cast<const f32x4*>(part + at * D + d0);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) x[e] = __builtin_fmaf(w, y[e], x[e]);
+  }
+  const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+  const int64_t z = slice / Hk, h = slice % Hk * G + row % G, n = row / G;
+  V4 y;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) y[e] = (T)(l == 0.0f ? 0.0f : x[e] * inv);
+  *reinterpret_cast<V4*>(out + z * sz + h * sh + n * sn + d0) = y;
+  if (m && d0 == 0) m[(z * Hk * G + h) * N + n] = mall + __log2f(l);
+}
+
+// ---- dQ ------------------------------------------------------------------------------------------
+// Rows and key tiles as in the forward; computes delta = rowsum(dO * O) on the way and stores -delta for dK / dV.
+template <typename T, int D, int RW, int CS, int TP, int OCC>
+__global__ __launch_bounds__(RW * CS * 64, OCC) void window_dq_kernel(const WindowParams p) {
+  using H = H16<T>;
+  using V8 = typename H::V8;
+  using V4 = typename H::V4;
+  using V2 = typename H::V2;
+  constexpr int NW = RW * CS, NT = CS * TP, NSD = D / 16, DT = (D + 31) / 32;
+  using R = WinRing<D, NW, NT>;
+  __shared__ __attribute__((aligned(1024))) char s0[R::STAGE];
+  __shared__ __attribute__((aligned(1024))) char s1[R::STAGE];
+
+  const int tid = threadIdx.x;
+  const int lane = tid & 63, h2 = lane >> 5, l32 = lane & 31;
+  const int wu = (int)uniform32((uint32_t)(tid >> 6));
+  const int rw = wu / CS, cs = wu % CS;
+  const float c = p.c;
+  int slice, blk;
+  if (!window_coord(p.Z * p.Hk, p.nblk, p.runs, slice, blk)) return;
+  WinRows b;
+  b.init(p, slice, p.nblk - 1 - blk, RW);
+  TileList list;
+  list.init(b.p0, b.p1, p.window, p.sinks);
+  const int nsteps = (list.n + NT - 1) / NT;
+
+  WinLoader<D, NW, NT> ld;
+  ld.init(p.sk[2], p.sv[2], wu, lane);
+  const __amdgpu_buffer_rsrc_t rs =
+      ld.second ? win_rsrc<T, D>(p.v, b.z * p.sv[0] + b.hk * p.sv[1], b.len, p.sv[2])
+                : win_rsrc<T, D>(p.k, b.z * p.sk[0] + b.hk * p.sk[1], b.len, p.sk[2]);
+  auto issue = [&](char* stage, int step) __attribute__((always_inline)) {
+    fetch_keys<D, NW, NT>(ld, rs, stage, list, step * NT, list.n, b.top, p.sinks);
+  };
+  if (nsteps > 0) issue(s0, 0);
+
+  const int tile0 = 32 * (b.tile0 + rw);
+  const int row = tile0 + l32;
+  const bool live = row < b.rows;
+  const int n = (live ? row : 0) / p.G, g = (live ? row : 0) % p.G, h = b.hk * p.G + g;
+  const int pos = b.off + n;
+  const int wp0 = b.off + tile0 / p.G, wp1 = tile0 < b.rows ? b.off + min(tile0 + 31, b.rows - 1) / p.G : -1;
+  const int64_t mrow = ((int64_t)b.z * p.H + h) * p.N + n;
+  V8 qop[NSD], dop[NSD];
+  float dl;
+  {
+    const T* qs = (const T*)p.q + b.z * p.sq[0] + h * p.sq[1] + n * p.sq[2] + 8 * h2;
+    const T* ds = (const T*)p.dout + b.z * p.sd[0] + h * p.sd[1] + n * p.sd[2] + 8 * h2;
+    const T* os = (const T*)p.o + b.z * p.so[0] + h * p.so[1] + n * p.so[2] + 8 * h2;
+    float sd[NSD];
+#pragma unroll
+    for (int s = 0; s < NSD; ++s) {
+      const V8 x = *reinterpret_cast<const V8*>(qs + 16 * s), y = *reinterpret_cast<const V8*>(ds + 16 * s);
+      qop[s] = live ? x : V8{};
+      dop[s] = live ? y : V8{};
+      sd[s] = chunk_dot(*reinterpret_cast<const V8*>(os + 16 * s), y);
+    }
+    dl = row_delta(sd);
+    if (live && h2 == 0 && cs == 0) p.delta[mrow] = -dl;
+    if (!live) dl = 0.0f;
+  }
+  const float nm = live ? -p.m[mrow] : 0.0f;
+  WinOp<D> at;
+  at.init(cs * R::TILE, lane);
+  f32x16 dq[DT];
+#pragma unroll
+  for (int u = 0; u < DT; ++u) dq[u] = f32x16{};
+
+  const float hidden = hidden_score(c);
+  auto tile = [&](const char* st, int t) __attribute__((always_inline)) {
+    f32x16 s = f32x16{}, dp;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) dp[r] = -dl;  // seeds dP - delta
+#pragma unroll
+    for (int sd = 0; sd < NSD; ++sd) {
+      s = Elt<T>::mfma(lds8<T>(st + at.nat[sd]), qop[sd], s);
+      dp = Elt<T>::mfma(lds8<T>(st + R::HALF + at.nat[sd]), dop[sd], dp);
+    }
+    if (tile_masked(wp0, wp1, t, p.window, p.sinks)) RowMask(pos, t, h2, p.window, p.sinks).hide(s, hidden);
+#pragma unroll
+    for (int r = 0; r < 16; ++r) s[r] = fast_exp2(__builtin_fmaf(s[r], c, nm)) * dp[r];
+    V8 ds[2];
+#pragma unroll
+    for (int sl = 0; sl < 2; ++sl)
+#pragma unroll
+      for (int i = 0; i < 8; i += 2) {
+        const V2 dh = H::pack(s[8 * sl + i], s[8 * sl + i + 1]);
+        ds[sl][i] = dh[0];
+        ds[sl][i + 1] = dh[1];
+      }
+#pragma unroll
+    for (int sl = 0; sl < 2; ++sl)
+#pragma unroll
+      for (int u = 0; u < DT; ++u) {
+        V8 a = at.template tr<T>(st, sl, u);
+        if (D < 32 && 16 * ((lane >> 4) & 1) >= D) a = V8{};
+        dq[u] = Elt<T>::mfma(a, ds[sl], dq[u]);
+      }
+  };
+  auto step = [&](int i, char* cur, char* nxt) __attribute__((always_inline)) {
+    if (i + 1 < nsteps) issue(nxt, i + 1);
+    const int k = i * NT + cs;
+#pragma unroll 1
+    for (int x = 0; x < TP; ++x) {
+      if (k + x * CS >= list.n) break;
+      const int t = list.at(k + x * CS);
+      if (tile_hidden(wp0, wp1, t, p.window, p.sinks)) continue;
+      tile(cur + x * CS * R::TILE, t);
+    }
+    all_landed_barrier();
+  };
+  all_landed_barrier();
+  int i = 0;
+  for (; i + 1 < nsteps; i += 2) {
+    step(i, s0, s1);
+    step(i + 1, s1, s0);
+  }
+  if (i < nsteps) step(i, s0, s1);
+
+  if constexpr (CS == 1) {
+    if (!live) return;
+    T* orow = (T*)p.out + b.z * p.sout[0] + h * p.sout[1] + n * p.sout[2];
+#pragma unroll
+    for (int u = 0; u < DT; ++u)
+#pragma unroll
+      for (int gr = 0; gr < 4; ++gr) {
+        const int d0 = 32 * u + 8 * gr + 4 * h2;
+        if (d0 >= D) continue;
+        V4 y;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) y[e] = (T)(dq[u][4 * gr + e] * p.scale);
+        *reinterpret_cast<V4*>(orow + d0) = y;
+      }
+    return;
+  }
+  constexpr int PART = DT * 16 * 64 * 4;
+  constexpr int PER = R::STAGE / PART;
+  static_assert(CS == 1 || 2 * PER >= NW, "partials fit the stages");
+  auto part = [&](int k) { return (TATTN_LDS float*)(k < PER ? s0 + k * PART : s1 + (k - PER) * PART); };
+  {
+    TATTN_LDS float* dst = part(wu) + lane;
+#pragma unroll
+    for (int u = 0; u < DT; ++u)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) dst[(16 * u + r) * 64] = dq[u][r];
+  }
+  __syncthreads();
+  if (!live) return;
+  T* orow = (T*)p.out + b.z * p.sout[0] + h * p.sout[1] + n * p.sout[2];
+  for (int gr = cs; gr < DT * 4; gr += CS) {
+    const int d0 = 8 * gr + 4 * h2;
+    if (d0 < D) {
+      f32x4 x = f32x4{};
+#pragma unroll
+      for (int k = 0; k < CS; ++k) {
+        const TATTN_LDS float* src = part(rw * CS + k) + lane + 4 * gr * 64;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[e] += src[64 * e];
+      }
+      V4 y;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) y[e] = (T)(x[e] * p.scale);
+      *reinterpret_cast<V4*>(orow + d0) = y;
+    }
+  }
+}
+
+// ---- dK / dV -------------------------------------------------------------------------------------
+// A workgroup owns RW tiles of 32 keys and walks the query tiles that see any of them, head after head of
+// the group: the sum over shared heads stays in registers. Key blocks that hold first keys are seen by every later query, an
+// N / window-fold of the others' work: their list is cut into `splits` parts (WindowParams), which write float32 sums that
+// window_first_keys_kernel adds in order.
+template <int RW>
+struct KeyBlocks {
+  int sink_blocks, items;  // per slice: sink_blocks * splits parts, then the other blocks
+  __host__ __device__ KeyBlocks(int S, int sinks, int splits) {
+    const int blocks = (S + 32 * RW - 1) / (32 * RW);
+    sink_blocks = splits > 1 ? (sinks + 32 * RW - 1) / (32 * RW) : 0;
+    if (sink_blocks > blocks) sink_blocks = blocks;
+    items = sink_blocks * splits + blocks - sink_blocks;
+  }
+};
+
+template <typename T, int D, int RW, int CS, int TP, int OCC>
+__global__ __launch_bounds__(RW * CS * 64, OCC) void window_dkdv_kernel(const WindowParams p) {
+  using H = H16<T>;
+  using V8 = typename H::V8;
+  using V2 = typename H::V2;
+  constexpr int NW = RW * CS, NT = CS * TP, NSD = D / 16, DT = (D + 31) / 32;
+  using R = WinRing<D, NW, NT>;
+  __shared__ __attribute__((aligned(1024))) char s0[R::STAGE];
+  __shared__ __attribute__((aligned(1024))) char s1[R::STAGE];
+  __shared__ __attribute__((aligned(16))) float md[NW][2][TP][64];  // per wave, parity and tile: M[32], -delta[32]
+
+  const int tid = threadIdx.x;
+  const int lane = tid & 63, h2 = lane >> 5, l32 = lane & 31;
+  const int wu = (int)uniform32((uint32_t)(tid >> 6));
+  const int rw = wu / CS, cs = wu % CS;
+  const float c = p.c;
+  const KeyBlocks<RW> kbs(p.S, p.sinks, p.splits);
+  int slice, kb, split = 0;
+  if (!window_coord(p.Z * p.Hk, kbs.items, p.runs, slice, kb)) return;
+  const bool parted = kb < kbs.sink_blocks * p.splits;
+  if (parted) split = kb % p.splits, kb /= p.splits;
+  else kb = kb - kbs.sink_blocks * p.splits + kbs.sink_blocks;
+  const int z = slice / p.Hk, hk = slice % p.Hk, off = p.S - p.N;
+  const int k0 = 32 * RW * kb, k1 = k0 + 32 * RW - 1;
+  // Queries that see a key of the block, as tiles of 32 of each head in turn.
+  const int nlo = max(0, k0 - off);
+  const int nhi = k0 < p.sinks ? p.N - 1 : min(p.N - 1, k1 + p.window - 1 - off);
+  const int qt0 = nlo >> 5, nq = nhi < nlo ? 0 : (nhi >> 5) - qt0 + 1;
+  const int total = nq * p.G;
+  const int i0 = parted ? (int)((int64_t)total * split / p.splits) : 0;
+  const int i1 = parted ? (int)((int64_t)total * (split + 1) / p.splits) : total;
+  const int nsteps = (i1 - i0 + NT - 1) / NT;
+
+  WinLoader<D, NW, NT> ld;
+  ld.init(p.sq[2], p.sd[2], wu, lane);
+  const char* qbase = ld.second ? (const char*)((const T*)p.dout + z * p.sd[0] + (int64_t)hk * p.G * p.sd[1])
+                                : (const char*)((const T*)p.q + z * p.sq[0] + (int64_t)hk * p.G * p.sq[1]);
+  const int64_t head_bytes = (ld.second ? p.sd[1] : p.sq[1]) * 2;
+  const uint32_t qbytes = (uint32_t)slice_bytes(p.N, ld.second ? p.sd[2] : p.sq[2], D);
+  auto issue = [&](char* stage, int step) __attribute__((always_inline)) {
+#pragma unroll
+    for (int x = 0; x < R::TW; ++x) {
+      const int k = i0 + step * NT + ld.first + x;
+      if (k >= i1) break;
+      const int g = k / nq, qt = qt0 + k % nq;
+      // Rows past the head's last query lie past the end of its slice and read as zero.
+      const __amdgpu_buffer_rsrc_t rs = slice_rsrc(qbase + g * head_bytes, qbytes);
+#pragma unroll
+      for (int i = 0; i < R::PIECES; ++i) ld.fetch(rs, stage, x, i, ld.go[i] + (uint32_t)qt * ld.tile_bytes);
+    }
+  };
+  if (nsteps > 0) issue(s0, 0);
+  // Lanes 0-31 fetch M and lanes 32-63 -delta of the wave's tile; zero past the end.
+  const float* mdsrc = (h2 ? p.delta : p.m) + ((int64_t)z * p.H + hk * p.G) * p.N;
+  auto md_load = [&](int step, float (&x)[TP]) __attribute__((always_inline)) {
+#pragma unroll
+    for (int t = 0; t < TP; ++t) {
+      const int k = i0 + step * NT + cs + t * CS;
+      const int q = k < i1 ? 32 * (qt0 + k % nq) + l32 : p.N;
+      x[t] = q < p.N ? mdsrc[(int64_t)(k / nq) * p.N + q] : 0.0f;
+    }
+  };
+  auto md_store = [&](int par, const float (&x)[TP]) __attribute__((always_inline)) {
+#pragma unroll
+    for (int t = 0; t < TP; ++t) md[wu][par][t][lane] = x[t];
+  };
+  float mdn[TP];
+  if (nsteps > 0) {
+    md_load(0, mdn);
+    md_store(0, mdn);
+  }
+  const int kt = kb * RW + rw, key = 32 * kt + l32;
+  V8 kop[NSD], vop[NSD];
+  {
+    const T* ks = (const T*)p.k + z * p.sk[0] + hk * p.sk[1] + (int64_t)(key < p.S ? key : 0) * p.sk[2] + 8 * h2;
+    const T* vs = (const T*)p.v + z * p.sv[0] + hk * p.sv[1] + (int64_t)(key < p.S ? key : 0) * p.sv[2] + 8 * h2;
+#pragma unroll
+    for (int s = 0; s < NSD; ++s) {
+      const V8 a = *reinterpret_cast<const V8*>(ks + 16 * s);
+      const V8 b = *reinterpret_cast<const V8*>(vs + 16 * s);
+      kop[s] = key < p.S ? a : V8{};
+      vop[s] = key < p.S ? b : V8{};
+    }
+  }
+  WinOp<D> at;
+  at.init(cs * R::TILE, lane);
+  f32x16 dk[DT], dv[DT];
+#pragma unroll
+  for (int u = 0; u < DT; ++u) dk[u] = dv[u] = f32x16{};
+
+  const float hidden = hidden_score(c);
+  auto tile = [&](const char* st, const float* mdw, int qt, bool masked) __attribute__((always_inline)) {
+    f32x16 s = f32x16{}, dp;
+    float mv[16];
+#pragma unroll
+    for (int a = 0; a < 4; ++a) {
+      const int o = 16 * (a >> 1) + 8 * h2 + 4 * (a & 1);
+      const f32x4 x = *reinterpret_cast<const TATTN_LDS f32x4*>((const TATTN_LDS float*)mdw + o);
+      const f32x4 y = *reinterpret_cast<const TATTN_LDS f32x4*>((const TATTN_LDS float*)mdw + 32 + o);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        mv[4 * a + i] = x[i];
+        dp[4 * a + i] = y[i];
+      }
+    }
+#pragma unroll
+    for (int sd = 0; sd < NSD; ++sd) {
+      s = Elt<T>::mfma(lds8<T>(st + at.nat[sd]), kop[sd], s);
+      dp = Elt<T>::mfma(lds8<T>(st + R::HALF + at.nat[sd]), vop[sd], dp);
+    }
+    if (masked) ColMask(off + 32 * qt - key, key, p.N - 32 * qt, h2, p.window, p.sinks).hide(s, hidden);
+#pragma unroll
+    for (int r = 0; r < 16; ++r) s[r] = fast_exp2(__builtin_fmaf(s[r], c, -mv[r]));
+    V8 pp[2], ds[2];
+#pragma unroll
+    for (int sl = 0; sl < 2; ++sl)
+#pragma unroll
+      for (int i = 0; i < 8; i += 2) {
+        const int r = 8 * sl + i;
+        const V2 ph = H::pack(s[r], s[r + 1]), dh = H::pack(s[r] * dp[r], s[r + 1] * dp[r + 1]);
+        pp[sl][i] = ph[0];
+        pp[sl][i + 1] = ph[1];
+        ds[sl][i] = dh[0];
+        ds[sl][i + 1] = dh[1];
+      }
+#pragma unroll
+    for (int sl = 0; sl < 2; ++sl)
+#pragma unroll
+      for (int u = 0; u < DT; ++u) {
+        V8 dob = at.template tr<T>(st + R::HALF, sl, u);
+        V8 qb = at.template tr<T>(st, sl, u);
+        if (D < 32 && 16 * ((lane >> 4) & 1) >= D) dob = qb = V8{};
+        dv[u] = Elt<T>::mfma(pp[sl], dob, dv[u]);
+        dk[u] = Elt<T>::mfma(ds[sl], qb, dk[u]);
+      }
+  };
+  const int wk0 = 32 * kt, wk1 = wk0 + 31;
+  auto step = [&](int i, char* cur, char* nxt, int par) __attribute__((always_inline)) {
+    if (i + 1 < nsteps) {
+      issue(nxt, i + 1);
+      md_load(i + 1, mdn);
+    }
+    const int k = i0 + i * NT + cs;
+#pragma unroll 1
+    for (int x = 0; x < TP; ++x) {
+      if (k + x * CS >= i1 || wk0 >= p.S) break;
+      const int qt = qt0 + (k + x * CS) % nq, q0 = off + 32 * qt, q1 = q0 + 31;
+      if (q1 >= wk0 && (q0 - wk1 < p.window || wk0 < p.sinks))
+        tile(cur + x * CS * R::TILE, md[wu][par][x], qt, q0 < wk1 || (q1 - wk0 >= p.window && wk1 >= p.sinks) || 32 * qt + 32 > p.N);
+    }
+    if (i + 1 < nsteps) md_store(par ^ 1, mdn);  // the wave's own rows: no barrier needed
+    all_landed_barrier();
+  };
+  all_landed_barrier();
+  int i = 0;
+  for (; i + 1 < nsteps; i += 2) {
+    step(i, s0, s1, 0);
+    step(i + 1, s1, s0, 1);
+  }
+  if (i < nsteps) step(i, s0, s1, 0);
+
+  // Sum the CS partials of each key tile, dK then dV: wave 0 of a tile keeps its own in registers. C register r of
+  // a lane: key 8 (r / 4) + 4 h2 + r % 4 of the tile, column 32 u + l32.
+  constexpr int PART = DT * 16 * 64 * 4;
+  constexpr int PER = R::STAGE / PART;
+  static_assert(2 * PER >= RW * (CS - 1), "partials fit the stages");
+  auto part = [&](int k) { return (TATTN_LDS float*)(k < PER ? s0 + k * PART : s1 + (k - PER) * PART); };
+  // A part's sums: [slice][sink block][split][dK, dV][32 RW keys][D] float32.
+  float* fdst = p.part + (((int64_t)slice * kbs.sink_blocks + kb) * p.splits + split) * (2 * 32 * RW * D);
+  auto reduce = [&](const f32x16 (&a)[DT], float mul, T* dst, int64_t stride, float* fpart) __attribute__((always_inline)) {
+    if (cs > 0) {
+      TATTN_LDS float* mine = part(rw * (CS - 1) + cs - 1) + lane;
+#pragma unroll
+      for (int u = 0; u < DT; ++u)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) mine[(16 * u + r) * 64] = a[u][r];
+    }
+    __syncthreads();
+    if (cs == 0) {
+#pragma unroll
+      for (int u = 0; u < DT; ++u)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          float x = a[u][r];
+#pragma unroll
+          for (int k = 0; k < CS - 1; ++k) x += (part(rw * (CS - 1) + k) + lane)[(16 * u + r) * 64];
+          const int in = 8 * (r >> 2) + 4 * h2 + (r & 3), d = 32 * u + l32;
+          if (d >= D) continue;
+          if (parted) fpart[(32 * rw + in) * D + d] = x;
+          else if (wk0 + in < p.S) dst[(int64_t)(wk0 + in) * stride + d] = (T)(x * mul);
+        }
+    }
+  };
+  reduce(dk, p.scale, (T*)p.dk + z * p.sdk[0] + hk * p.sdk[1], p.sdk[2], fdst);
+  __syncthreads();
+  reduce(dv, 1.0f, (T*)p.dv + z * p.sdv[0] + hk * p.sdv[1], p.sdv[2], fdst + 32 * RW * D);
+}
+
+// dK / dV at head dims 64 and 128: two waves per 32-key tile. Over each 32-query tile wave j (role A) computes S = Q K^T,
+// P = 2^(S c - M), dV += P^T dO, and wave j + 4 (role B) dP - delta = dO V^T - delta, dS = P (dP - delta), dK += dS^T Q,
+// taking P from A through LDS in float32. Each keeps one of K / V and one accumulator set: half the registers of a wave that
+// does both, so that two (head dim 128) or four waves (64) share a SIMD; as many matrix instructions in either role.
+// Step i, one barrier each: A takes tile i, B tile i - 1, and tiles i + 1 and i + 2 are on their way. Nothing is
+// pipelined inside a wave: the waves of a SIMD overlap each other's matrix and vector work.
+template <typename T, int D, int OCC>
+__global__ __launch_bounds__(512, OCC) void window_dkdv_pair_kernel(const WindowParams p) {
+  using H = H16<T>;
+  using V8 = typename H::V8;
+  using V2 = typename H::V2;
+  constexpr int RW = 4, NW = 8, NSD = D / 16, DT = D / 32, RB = Swz<D>::RB, TILE = 32 * RB;
+  constexpr int PW = 2 * TILE / 1024 / NW;          // 1 KB pieces per wave and step
+  constexpr int STAGE = 2 * TILE + 256;             // Q, dO, M[32], -delta[32]
+  constexpr int XB = 32 * 32 * 4;                   // P of a pair
+  // Arrays of their own: a DMA into one does not alias reads of the others.
+  __shared__ __attribute__((aligned(1024))) char st0[STAGE], st1[STAGE], st2[STAGE], st3[STAGE];
+  __shared__ __attribute__((aligned(1024))) char x0[RW * XB], x1[RW * XB];
+  auto stage = [&](auto tag) __attribute__((always_inline)) -> char* {
+    constexpr int I = decltype(tag)::value & 3;
+    return I == 0 ? st0 : I == 1 ? st1 : I == 2 ? st2 : st3;
+  };
+
+  const int tid = threadIdx.x;
+  const int lane = tid & 63, h2 = lane >> 5, l32 = lane & 31;
+  const int wu = (int)uniform32((uint32_t)(tid >> 6));
+  const int pr = wu & 3;
+  const bool role_b = wu >= 4;
+  const float c = p.c;
+  const KeyBlocks<RW> kbs(p.S, p.sinks, p.splits);
+  int slice, kb, split = 0;
+  if (!window_coord(p.Z * p.Hk, kbs.items, p.runs, slice, kb)) return;
+  const bool parted = kb < kbs.sink_blocks * p.splits;
+  if (parted) split = kb % p.splits, kb /= p.splits;
+  else kb = kb - kbs.sink_blocks * p.splits + kbs.sink_blocks;
+  const int z = slice / p.Hk, hk = slice % p.Hk, off = p.S - p.N;
+  const int k0 = 32 * RW * kb, k1 = k0 + 32 * RW - 1;
+  // Queries that see a key of the block, as tiles of 32 of each head in turn.
+  const int nlo = max(0, k0 - off);
+  const int nhi = k0 < p.sinks ? p.N - 1 : min(p.N - 1, k1 + p.window - 1 - off);
+  const int qt0 = nlo >> 5, nq = nhi < nlo ? 0 : (nhi >> 5) - qt0 + 1;
+  const int total = nq * p.G;
+  const int i0 = parted ? (int)((int64_t)total * split / p.splits) : 0;
+  const int i1 = parted ? (int)((int64_t)total * (split + 1) / p.splits) : total;
+  const int n = i1 - i0;
+  const int wk0 = 32 * (kb * RW + pr), wk1 = wk0 + 31, key = wk0 + l32;
+
+  // The wave's operand: K rows (A) or V rows (B).
+  V8 kv[NSD];
+  {
+    const T* src = role_b ? (const T*)p.v + z * p.sv[0] + hk * p.sv[1] + (int64_t)(key < p.S ? key : 0) * p.sv[2]
+                          : (const T*)p.k + z * p.sk[0] + hk * p.sk[1] + (int64_t)(key < p.S ? key : 0) * p.sk[2];
+#pragma unroll
+    for (int s = 0; s < NSD; ++s) {
+      const V8 a = *reinterpret_cast<const V8*>(src + 16 * s + 8 * h2);
+      kv[s] = key < p.S ? a : V8{};
+    }
+  }
+
+  // Fetching: pieces wu * PW .. of the step's Q tile (waves 0-3) and dO tile (4-7), and by wave 0 M and -delta.
+  const int64_t head = (role_b ? p.sd[1] : p.sq[1]) * 2, rowst = role_b ? p.sd[2] : p.sq[2];
+  const char* base = role_b ? (const char*)((const T*)p.dout + z * p.sd[0] + (int64_t)hk * p.G * p.sd[1])
+                            : (const char*)((const T*)p.q + z * p.sq[0] + (int64_t)hk * p.G * p.sq[1]);
+  const uint32_t bytes = (uint32_t)slice_bytes(p.N, rowst, D), tile_bytes = uniform32((uint32_t)(rowst * 64));
+  const float* md = (h2 ? p.delta : p.m) + ((int64_t)z * p.H + hk * p.G) * p.N;
+  uint32_t go[PW];
+#pragma unroll
+  for (int i = 0; i < PW; ++i) {
+    constexpr int CPR = RB / 16;
+    const int j = 64 * ((wu & 3) * PW + i) + lane, row = j / CPR;
+    go[i] = (uint32_t)(perm32(row) * rowst * 2 + (((j % CPR) ^ Swz<D>::f(row)) & (D / 8 - 1)) * 16);
+  }
+  // Next tile to fetch. Past the last one its rows come again, into a stage that nobody reads: every step has as many
+  // loads in flight.
+  int fg = nq > 0 ? i0 / nq : 0, fq = qt0 + (nq > 0 ? i0 % nq : 0), fi = 1;
+  auto fetch = [&](char* st) __attribute__((always_inline)) {
+    const __amdgpu_buffer_rsrc_t rs = slice_rsrc(base + fg * head, bytes);  // rows past the last query read as zero
+#pragma unroll
+    for (int i = 0; i < PW; ++i)
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (TATTN_LDS void*)(st + (wu * PW + i) * 1024), 16,
+                                               (int)(go[i] + (uint32_t)fq * tile_bytes), 0, 0, 0);
+    if (wu == 0) {
+      const float* src = md + (int64_t)fg * p.N + min(32 * fq + l32, p.N - 1);
+      __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)src,
+                                       (TATTN_LDS void*)(st + 2 * TILE), 4, 0, 0);
+    }
+    if (fi < n) {
+      ++fi;
+      if (++fq == qt0 + nq) fq = qt0, ++fg;
+    }
+  };
+  // End of a step: the loads of the step before have landed, this step's may stay in flight; LDS accesses are done.
+  auto step_end = [&]() __attribute__((always_inline)) {
+    if (wu == 0) __builtin_amdgcn_s_waitcnt(0x0070 | (PW + 1));
+    else __builtin_amdgcn_s_waitcnt(0x0070 | PW);
+    __atomic_signal_fence(__ATOMIC_SEQ_CST);
+    __builtin_amdgcn_s_barrier();
+    __atomic_signal_fence(__ATOMIC_SEQ_CST);
+  };
+
+  int nat[NSD], lo[DT], hi[DT];
+#pragma unroll
+  for (int s = 0; s < NSD; ++s) nat[s] = Swz<D>::addr(l32, (16 * s + 8 * h2) * 2);
+#pragma unroll
+  for (int u = 0; u < DT; ++u) tr_addrs<D>(0, u, lane, lo[u], hi[u]);
+  const float hidden = hidden_score(c);
+  f32x16 acc[DT];  // dV (A) or dK (B)
+#pragma unroll
+  for (int u = 0; u < DT; ++u) acc[u] = f32x16{};
+
+  // What the pair does with a query tile: nothing, all of it, or with a mask.
+  struct Look {
+    int qt;
+    bool live, masked;
+  };
+  auto look = [&](int qt, bool in) __attribute__((always_inline)) {
+    const int q0 = off + 32 * qt, q1 = q0 + 31;
+    Look l;
+    l.qt = qt;
+    l.live = in && wk0 < p.S && q1 >= wk0 && (q0 - wk1 < p.window || wk0 < p.sinks);
+    l.masked = q0 < wk1 || (q1 - wk0 >= p.window && wk1 >= p.sinks) || 32 * qt + 32 > p.N;
+    return l;
+  };
+
+  auto run = [&](auto role_tag) __attribute__((always_inline)) {
+    constexpr bool RB_ = decltype(role_tag)::value;
+    // S (A) of a stage's tile, or dP - delta (B).
+    auto first = [&](f32x16& s, const char* st) __attribute__((always_inline)) {
+      if constexpr (RB_) {
+        const TATTN_LDS char* nd = (const TATTN_LDS char*)st + 2 * TILE + 128 + 32 * h2;
+#pragma unroll
+        for (int a = 0; a < 4; ++a) {
+          const f32x4 v = *reinterpret_cast<const TATTN_LDS f32x4*>(nd + 64 * (a >> 1) + 16 * (a & 1));
+#pragma unroll
+          for (int e = 0; e < 4; ++e) s[4 * a + e] = v[e];
+        }
+      } else {
+        s = f32x16{};
+      }
+#pragma unroll
+      for (int sd = 0; sd < NSD; ++sd) s = Elt<T>::mfma(lds8<T>(st + (RB_ ? TILE : 0) + nat[sd]), kv[sd], s);
+    };
+    // dV += P^T dO (A), dK += dS^T Q (B).
+    auto grad = [&](const V8 (&op)[2], const char* st) __attribute__((always_inline)) {
+#pragma unroll
+      for (int sl = 0; sl < 2; ++sl)
+#pragma unroll
+        for (int u = 0; u < DT; ++u)
+          acc[u] = Elt<T>::mfma(op[sl], tr_pair<T>(st + (RB_ ? 0 : TILE) + 16 * sl * RB, lo[u], hi[u]), acc[u]);
+    };
+    auto probs = [&](const f32x16& s, V8 (&pp)[2], const char* st, char* x) __attribute__((always_inline)) {
+#pragma unroll
+      for (int a = 0; a < 4; ++a) {
+        const f32x4 m = *reinterpret_cast<const TATTN_LDS f32x4*>((const TATTN_LDS char*)st + 2 * TILE + 32 * h2 + 64 * (a >> 1) + 16 * (a & 1));
+        f32x4 pv;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) pv[e] = fast_exp2(__builtin_fmaf(s[4 * a + e], c, -m[e]));
+        *reinterpret_cast<TATTN_LDS f32x4*>((TATTN_LDS char*)x + pr * XB + 1024 * a + 16 * lane) = pv;
+        const V2 a0 = H::pack(pv[0], pv[1]), a1 = H::pack(pv[2], pv[3]);
+        V8& o8 = pp[a >> 1];
+        o8[4 * (a & 1)] = a0[0], o8[4 * (a & 1) + 1] = a0[1], o8[4 * (a & 1) + 2] = a1[0], o8[4 * (a & 1) + 3] = a1[1];
+      }
+    };
+    auto dsv = [&](const f32x16& dp, V8 (&ds)[2], const char* x) __attribute__((always_inline)) {
+#pragma unroll
+      for (int a = 0; a < 4; ++a) {
+        const f32x4 pv = *reinterpret_cast<const TATTN_LDS f32x4*>((const TATTN_LDS char*)x + pr * XB + 1024 * a + 16 * lane);
+        float d[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) d[e] = pv[e] * dp[4 * a + e];
+        const V2 a0 = H::pack(d[0], d[1]), a1 = H::pack(d[2], d[3]);
+        V8& o8 = ds[a >> 1];
+        o8[4 * (a & 1)] = a0[0], o8[4 * (a & 1) + 1] = a0[1], o8[4 * (a & 1) + 2] = a1[0], o8[4 * (a & 1) + 3] = a1[1];
+      }
+    };
+    int q = nq > 0 ? qt0 + i0 % nq : 0;
+    Look prev{0, false, false};
+    auto step = [&](int i, auto tag) __attribute__((always_inline)) {
+      constexpr int I = decltype(tag)::value;
+      if (i > n) return;
+      fetch(stage(IC<I + 2>{}));
+      const Look cur = look(q, i < n);
+      q = q + 1 == qt0 + nq ? qt0 : q + 1;
+      if constexpr (!RB_) {
+        if (cur.live) {
+          f32x16 s;
+          V8 pp[2];
+          first(s, stage(IC<I>{}));
+          if (cur.masked) ColMask(off + 32 * cur.qt - key, key, p.N - 32 * cur.qt, h2, p.window, p.sinks).hide(s, hidden);
+          probs(s, pp, stage(IC<I>{}), (I & 1) ? x1 : x0);
+          grad(pp, stage(IC<I>{}));
+        }
+      } else if (prev.live) {
+        f32x16 dp;
+        V8 ds[2];
+        first(dp, stage(IC<I + 3>{}));
+        dsv(dp, ds, (I & 1) ? x0 : x1);
+        grad(ds, stage(IC<I + 3>{}));
+      }
+      prev = cur;
+      step_end();
+    };
+    for (int i = 0; i <= n; i += 4) {  // in step n B finishes the last tile; none follows
+      step(i, IC<0>{});
+      step(i + 1, IC<1>{});
+      step(i + 2, IC<2>{});
+      step(i + 3, IC<3>{});
+    }
+  };
+  if (n > 0) {
+    fetch(st0);
+    fetch(st1);
+    all_landed_barrier();
+    if (role_b) run(std::true_type{});
+    else run(std::false_type{});
+    all_landed_barrier();
+  }
+
+  // Every wave has passed the last barrier and nothing is in flight. C register r of a lane: key 8 (r / 4) + 4 h2 + r % 4 of
+  // the tile, column 32 u + l32. A part's sums go out in float32; otherwise the tile is turned into rows through LDS.
+  const float mul = role_b ? p.scale : 1.0f;
+  if (parted) {
+    float* dst = p.part + (((int64_t)slice * kbs.sink_blocks + kb) * p.splits + split) * (2 * 32 * RW * D) +
+                 (role_b ? 0 : 32 * RW * D) + (int64_t)32 * pr * D;
+#pragma unroll
+    for (int u = 0; u < DT; ++u)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) dst[(8 * (r >> 2) + 4 * h2 + (r & 3)) * D + 32 * u + l32] = acc[u][r];
+    return;
+  }
+  T* dst = role_b ? (T*)p.dk + z * p.sdk[0] + hk * p.sdk[1] : (T*)p.dv + z * p.sdv[0] + hk * p.sdv[1];
+  const int64_t dst_row = role_b ? p.sdk[2] : p.sdv[2];
+  constexpr int PER = STAGE / TILE;  // whole tiles per stage array: 2
+  static_assert(PER * 4 >= NW, "a block of rows per wave");
+  char* mine = (wu >> 1) == 0 ? st0 : (wu >> 1) == 1 ? st1 : (wu >> 1) == 2 ? st2 : st3;
+  mine += (wu & 1) * TILE;
+#pragma unroll
+  for (int u = 0; u < DT; ++u)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      const int row = 8 * (r >> 2) + 4 * h2 + (r & 3);
+      *reinterpret_cast<TATTN_LDS T*>((TATTN_LDS char*)mine + Swz<D>::addr(row, (32 * u + l32) * 2)) = (T)(acc[u][r] * mul);
+    }
+  constexpr int CPR = D / 8;
+#pragma unroll
+  for (int i = 0; i < 32 * CPR / 64; ++i) {
+    const int j = 64 * i + lane, row = j / CPR, cc = j % CPR;
+    const u32x4 v = *reinterpret_cast<const TATTN_LDS u32x4*>((const TATTN_LDS char*)mine + Swz<D>::addr(row, 16 * cc));
+    if (wk0 + row < p.S) st16(dst + (int64_t)(wk0 + row) * dst_row + 8 * cc, v);
+  }
+}
+
+// dK and dV of the key blocks whose queries were cut into parts.
+template <typename T, int D, int RW>
+__global__ __launch_bounds__(256) void window_first_keys_kernel(const WindowParams p) {
+  const KeyBlocks<RW> kbs(p.S, p.sinks, p.splits);
+  constexpr int BLOCK = 32 * RW * D;
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const int64_t per = 2ll * BLOCK;
+  if (i >= (int64_t)p.Z * p.Hk * kbs.sink_blocks * per) return;
+  const int64_t block = i / per;
+  const int e = (int)(i % per), which = e / BLOCK, in = e % BLOCK / D, d = e % D;
+  const int slice = (int)(block / kbs.sink_blocks), kb = (int)(block % kbs.sink_blocks);
+  const int key = 32 * RW * kb + in;
+  if (key >= p.S) return;
+  float x = 0.0f;
+#pragma unroll 4
+  for (int s = 0; s < p.splits; ++s) x += p.part[(block * p.splits + s) * per + e];
+  const int z = slice / p.Hk, hk = slice % p.Hk;
+  if (which) ((T*)p.dv)[z * p.sdv[0] + hk * p.sdv[1] + (int64_t)key * p.sdv[2] + d] = (T)x;
+  else ((T*)p.dk)[z * p.sdk[0] + hk * p.sdk[1] + (int64_t)key * p.sdk[2] + d] = (T)(x * p.scale);
+}
+
+// ---- launch ----------------------------------------------------------------------------------------
+// Row tiles per workgroup and key tiles per step.
+template <int D> struct WinShape { static constexpr int RW = 4, TP = 2, OCC = D == 128 ? 2 : 4; };
+template <int D> struct KeyShape { static constexpr int RW = D >= 64 ? 4 : 2, CS = 4; };
+
+int grid_of(int64_t slices, int64_t per_slice, unsigned* out) {
+  const int64_t blocks = slices * per_slice + 8;
+  if (blocks > 0x7ffffff) return set_error(TATTN_E_ARG, "grid too large: %lld workgroups", (long long)blocks);
+  *out = (unsigned)((slices * per_slice + 7) / 8 * 8);
+  return TATTN_OK;
+}
+
+// Whether consecutive blocks of a slice share an XCD: windows much shorter than the rows make blocks equal; else the
+// later ones are longer, and only whole slices per XCD keep the XCDs level.
+int in_runs(const WindowParams& p) { return ((int64_t)p.Z * p.Hk) % 8 == 0 || (int64_t)p.window * 4 <= p.S; }
+
+// Key tiles that a block of 32 rows walks at most.
+int64_t most_tiles(const WindowParams& p) {
+  const int64_t seen = std::min<int64_t>(p.S, (int64_t)p.window + 32 / p.G + std::min(p.sinks, p.S));
+  return (seen + 31) / 32 + 1;
+}
+
+template <typename T, int D>
+int fwd_d(WindowParams p, hipStream_t st) {
+  const int64_t slices = (int64_t)p.Z * p.Hk, rows = (int64_t)p.N * p.G;
+  unsigned blocks;
+  int rc;
+  p.runs = in_runs(p);
+  if (p.splits > 0) {
+    p.nblk = (int)((rows + 31) / 32);
+    if ((rc = grid_of(slices, (int64_t)p.nblk * p.splits, &blocks))) return rc;
+    if (p.splits == 1) {
+      window_fwd_kernel<T, D, 1, 4, 1, D == 128 ? 1 : 2, false><<<dim3(blocks), dim3(256), 0, st>>>(p);
+      return check_launch("tattn_window_fwd");
+    }
+    window_fwd_kernel<T, D, 1, 4, 1, D == 128 ? 1 : 2, true><<<dim3(blocks), dim3(256), 0, st>>>(p);
+    if ((rc = check_launch("tattn_window_fwd"))) return rc;
+    return launch_combine(p.part, p.out, p.m, p.sout, slices, p.Hk, p.G, p.N, p.splits, D, std::is_same_v<T, bf16> ? 2 : 0, st);
+  }
+  using S = WinShape<D>;
+  p.nblk = (int)((rows + 32 * S::RW - 1) / (32 * S::RW));
+  if ((rc = grid_of(slices, p.nblk, &blocks))) return rc;
+  window_fwd_kernel<T, D, S::RW, 1, S::TP, S::OCC, false><<<dim3(blocks), dim3(S::RW * 64), 0, st>>>(p);
+  return check_launch("tattn_window_fwd");
+}
+
+template <typename T, int D>
+int bwd_d(WindowParams p, hipStream_t st) {
+  using S = WinShape<D>;
+  using K = KeyShape<D>;
+  const int64_t slices = (int64_t)p.Z * p.Hk, rows = (int64_t)p.N * p.G;
+  const int splits = p.splits;
+  unsigned blocks;
+  int rc;
+  p.runs = in_runs(p);
+  p.nblk = (int)((rows + 32 * S::RW - 1) / (32 * S::RW));
+  if ((rc = grid_of(slices, p.nblk, &blocks))) return rc;
+  window_dq_kernel<T, D, S::RW, 1, S::TP, D >= 64 ? 2 : 4><<<dim3(blocks), dim3(S::RW * 64), 0, st>>>(p);
+  if ((rc = check_launch("tattn_window_bwd"))) return rc;
+  const KeyBlocks<K::RW> kbs(p.S, p.sinks, splits);
+  if ((rc = grid_of(slices, kbs.items, &blocks))) return rc;
+  if constexpr (D == 64)
+    window_dkdv_kernel<T, 64, 4, 1, KTP, KOC><<<dim3(blocks), dim3(256), 0, st>>>(p);
+  else if constexpr (D >= 64)
+    window_dkdv_pair_kernel<T, D, D == 64 ? 4 : 2><<<dim3(blocks), dim3(512), 0, st>>>(p);
+  else
+    window_dkdv_kernel<T, D, K::RW, K::CS, 1, D == 32 ? 3 : 4><<<dim3(blocks), dim3(K::RW * K::CS * 64), 0, st>>>(p);
+  if ((rc = check_launch("tattn_window_bwd")) || !kbs.sink_blocks) return rc;
+  const int64_t n = slices * kbs.sink_blocks * 2 * 32 * K::RW * D;
+  window_first_keys_kernel<T, D, K::RW><<<dim3((unsigned)((n + 255) / 256)), dim3(256), 0, st>>>(p);
+  return check_launch("tattn_window_bwd");
+}
+
+#define TATTN_WIN_SWITCH(FN)                                                     \
+  switch (D) {                                                                   \
+    case 16: return dtype == 0 ? FN<f16, 16>(p, st) : FN<bf16, 16>(p, st);       \
+    case 32: return dtype == 0 ? FN<f16, 32>(p, st) : FN<bf16, 32>(p, st);       \
+    case 64: return dtype == 0 ? FN<f16, 64>(p, st) : FN<bf16, 64>(p, st);       \
+    case 128: return dtype == 0 ? FN<f16, 128>(p, st) : FN<bf16, 128>(p, st);    \
+  }                                                                              \
+  return set_error(TATTN_E_ARG, "head dim must be 16, 32, 64 or 128, got %d", D);
+
+template <typename T, int D>
+int combine_d(const float* part, void* out, float* m, const int64_t so[3], int64_t slices, int Hk, int G, int N, int splits,
+              hipStream_t st) {
+  const int64_t rows = slices * N * G;
+  constexpr int PER = 256 / (D / 4);
+  combine_kernel<T, D><<<dim3((unsigned)((rows + PER - 1) / PER)), dim3(256), 0, st>>>(part, (T*)out, m, so[0], so[1], so[2],
+                                                                                       slices, Hk, G, N, splits);
+  return check_launch("combine");
+}
+
+}  // namespace
+
+// Few rows: one row tile per workgroup, and its keys cut into parts until the chip has two workgroups per CU, each with
+// at least eight tiles. 0: enough rows for the blocks of two row tiles.
+int window_fwd_splits(const WindowParams& p) {
+  const int64_t slices = (int64_t)p.Z * p.Hk, rows = (int64_t)p.N * p.G;
+  if (slices * ((rows + 63) / 64) >= 256) return 0;
+  const int64_t blocks = slices * ((rows + 31) / 32);
+  return (int)std::max<int64_t>(1, std::min<int64_t>((512 + blocks - 1) / blocks, most_tiles(p) / 8));
+}
+
+// Parts of the first keys' dK and dV: each about as long as another key block's list, or as an even share of all
+// work over four workgroups per CU where that is more.
+int window_bwd_splits(const WindowParams& p, int D) {
+  if (p.sinks == 0) return 1;
+  const int64_t rw = D >= 64 ? KeyShape<64>::RW : KeyShape<32>::RW, keys = 32 * rw;
+  const int64_t all = (int64_t)p.G * ((p.N + 31) / 32);
+  const int64_t list = std::min<int64_t>(all, (int64_t)p.G * (std::min<int64_t>(p.window, p.S) / 32 + rw + 1));
+  const int64_t share = (int64_t)p.Z * p.Hk * ((p.S + keys - 1) / keys) * list / 1024;
+  const int64_t part = std::max<int64_t>(std::max<int64_t>(list, share), 32);
+  return (int)std::max<int64_t>(1, std::min<int64_t>((all + part - 1) / part, 256));
+}
+
+int64_t window_bwd_part_floats(const WindowParams& p, int D) {
+  const int splits = window_bwd_splits(p, D);
+  if (splits == 1) return 0;
+  const int64_t rw = D >= 64 ? KeyShape<64>::RW : KeyShape<32>::RW;
+  const int64_t blocks = D >= 64 ? KeyBlocks<KeyShape<64>::RW>(p.S, p.sinks, splits).sink_blocks
+                                 : KeyBlocks<KeyShape<32>::RW>(p.S, p.sinks, splits).sink_blocks;
+  return (int64_t)p.Z * p.Hk * blocks * splits * 2 * 32 * rw * D;
+}
+
+int launch_window_fwd(WindowParams p, int D, int dtype, hipStream_t st) { TATTN_WIN_SWITCH(fwd_d) }
+int launch_window_bwd(WindowParams p, int D, int dtype, hipStream_t st) { TATTN_WIN_SWITCH(bwd_d) }
+
+int launch_combine(const float* part, void* out, float* m, const int64_t so[3], int64_t slices, int Hk, int G, int N,
+                   int splits, int D, int dtype, hipStream_t st) {
+  switch (D) {
+#define TATTN_COMBINE(D_)                                                                               \
+  case D_:                                                                                              \
+    return dtype == 0 ? combine_d<f16, D_>(part, out, m, so, slices, Hk, G, N, splits, st)              \
+                      : combine_d<bf16, D_>(part, out, m, so, slices, Hk, G, N, splits, st);
+    TATTN_COMBINE(16) TATTN_COMBINE(32) TATTN_COMBINE(64) TATTN_COMBINE(128)
+#undef TATTN_COMBINE
+  }
+  return set_error(TATTN_E_ARG, "head dim must be 16, 32, 64 or 128, got %d", D);
+}
+
+}  // namespace tattn
