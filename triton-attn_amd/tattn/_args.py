@@ -2,9 +2,9 @@
 
 from __future__ import annotations
 
-import torch
+import ctypes
 
-from tattn import _lib
+import torch
 
 
 def same_device(first: torch.Tensor, **others: torch.Tensor | None) -> None:
@@ -22,21 +22,46 @@ def check_index(name: str, t: torch.Tensor, dtype: torch.dtype, shape: tuple) ->
         raise ValueError(f"{name} must be {dtype_name(dtype)} of shape {list(shape)}, got {dtype_name(t.dtype)} {list(t.shape)}")
 
 
+def rows_apart(t: torch.Tensor) -> bool:
+    """Whether the kernels cannot read t's rows where they lie: unit d stride, strides of whole 16-byte chunks."""
+    vec, st = 16 // t.element_size(), t.stride()
+    return st[-1] != 1 or any(size > 1 and s % vec for size, s in zip(t.shape[:-1], st))
+
+
 def rows(t: torch.Tensor) -> torch.Tensor:
-    """t itself where the kernels read its rows (unit d stride, 16-byte aligned), else an aligned contiguous copy."""
-    vec = 16 // t.element_size()
-    st = t.stride()
-    if (st[-1] == 1 or t.shape[-1] <= 1) and t.data_ptr() % 16 == 0:
-        for size, s in zip(t.shape[:-1], st):
-            if size > 1 and s % vec:
-                break
-        else:
-            return t
-    return t.clone(memory_format=torch.contiguous_format)
+    """t itself where the kernels read its rows, else an aligned contiguous copy."""
+    return aligned(t, rows_apart(t))
+
+
+def layout(t: torch.Tensor | None) -> tuple:
+    """What the checks of a call and its launch arguments depend on, but for the data's address."""
+    return () if t is None else (t.shape, t.stride(), t.dtype, t.device)
+
+
+def remember(plans: dict, key: tuple, plan: tuple) -> tuple:
+    """Keeps what the checks of a call made of its tensors' layouts, for calls with the same ones."""
+    if len(plans) >= 1024:
+        plans.clear()
+    plans[key] = plan
+    return plan
+
+
+def aligned(t: torch.Tensor, copy: bool) -> torch.Tensor:
+    """t, or an aligned contiguous copy where its layout asks for one or its data does not start on 16 bytes."""
+    return t.clone(memory_format=torch.contiguous_format) if copy or t.data_ptr() & 15 else t
+
+
+_stride_arrays: dict[tuple, tuple] = {}
 
 
 def strides(*ts: torch.Tensor) -> tuple:
     """An array with each tensor's four strides (missing dimensions and those of one entry have stride 0), to be held
     until the call is made, and the address of each tensor's four."""
-    key = tuple(tuple(s if n > 1 else 0 for n, s in zip(t.shape, t.stride())) for t in ts)
-    return _lib.stride_rows(key)
+    key = tuple([(t.shape, t.stride()) for t in ts])
+    hit = _stride_arrays.get(key)
+    if hit is None:
+        flat = [s for shape, st in key for s in ([s if n > 1 else 0 for n, s in zip(shape, st)] + [0] * 4)[:4]]
+        arr = (ctypes.c_int64 * len(flat))(*flat)
+        base = ctypes.addressof(arr)
+        hit = remember(_stride_arrays, key, (arr, [base + 32 * i for i in range(len(ts))]))
+    return hit

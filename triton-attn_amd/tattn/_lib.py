@@ -149,18 +149,6 @@ def stride_block(*ts: torch.Tensor):
     return hit
 
 
-def stride_rows(key: tuple) -> tuple:
-    """The same for tuples of up to four strides (missing ones are 0)."""
-    hit = _stride_blocks.get(key)
-    if hit is None:
-        if len(_stride_blocks) > 1024:
-            _stride_blocks.clear()
-        arr = (ctypes.c_int64 * (4 * len(key)))(*(s for st in key for s in (*st, 0, 0, 0, 0)[:4]))
-        base = ctypes.addressof(arr)
-        hit = _stride_blocks[key] = (arr, [base + 32 * i for i in range(len(key))])
-    return hit
-
-
 def num_configs(kernel: int, d: int, dtype: int) -> int:
     return load().tattn_num_configs(kernel, d, dtype)
 

@@ -14,7 +14,7 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from tattn import _lib
-from tattn._args import check_index, rows, same_device, strides
+from tattn._args import aligned, check_index, layout, remember, rows, rows_apart, same_device, strides
 from tattn.api import _DTYPES, _on_device, _require_gpu, _stream
 
 
@@ -45,18 +45,24 @@ def _check(q, k, q_weight, k_weight, cos, sin, positions) -> None:
     same_device(q, k=k, q_weight=q_weight, k_weight=k_weight, cos=cos, sin=sin, positions=positions)
 
 
-def _aligned(t: torch.Tensor) -> torch.Tensor:
-    return t if t.is_contiguous() and t.data_ptr() % 16 == 0 else t.clone(memory_format=torch.contiguous_format)
+_plans: dict[tuple, tuple] = {}
 
 
-def _scalars(q, k, qw, cos, positions, eps, interleaved) -> tuple:
+def _plan(q, k, qw, kw, cos, sin, positions, interleaved) -> tuple:
+    """Checks a call; what later calls with these layouts need: which tensors to copy, and the sizes among the
+    launch's arguments."""
+    _check(q, k, qw, kw, cos, sin, positions)
+    copies = (rows_apart(q), rows_apart(k), *(not t.is_contiguous() for t in (qw, kw, cos, sin)))
+    return copies, _scalars(q, k, qw, cos, positions, interleaved)
+
+
+def _scalars(q, k, qw, cos, positions, interleaved) -> tuple:
     z, h, n, d = q.shape
     pos_stride = n if positions is not None and positions.dim() == 2 else 0
-    return (pos_stride, z, h, k.shape[1], n, d, cos.shape[0], _DTYPES[q.dtype], _DTYPES[qw.dtype], int(interleaved), eps)
+    return pos_stride, z, h, k.shape[1], n, d, cos.shape[0], _DTYPES[q.dtype], _DTYPES[qw.dtype], int(interleaved)
 
 
-def _forward(q, k, qw, kw, cos, sin, positions, eps, interleaved) -> tuple[torch.Tensor, torch.Tensor]:
-    q, k = rows(q), rows(k)
+def _forward(q, k, qw, kw, cos, sin, positions, eps, scalars) -> tuple[torch.Tensor, torch.Tensor]:
     qo, ko = torch.empty_like(q), torch.empty_like(k)
     if q.numel() == 0:
         return qo, ko
@@ -64,18 +70,18 @@ def _forward(q, k, qw, kw, cos, sin, positions, eps, interleaved) -> tuple[torch
     with _on_device(q):
         rc = _lib.load().tattn_norm_rope_fwd(
             q.data_ptr(), k.data_ptr(), qw.data_ptr(), kw.data_ptr(), cos.data_ptr(), sin.data_ptr(),
-            None if positions is None else positions.data_ptr(), qo.data_ptr(), ko.data_ptr(), *st,
-            *_scalars(q, k, qw, cos, positions, eps, interleaved), _stream(q))
-    _lib.check(rc, "tattn_norm_rope_fwd")
+            None if positions is None else positions.data_ptr(), qo.data_ptr(), ko.data_ptr(), *st, *scalars, eps, _stream(q))
+    if rc:
+        _lib.check(rc, "tattn_norm_rope_fwd")
     return qo, ko
 
 
 class _NormRope(torch.autograd.Function):
     @staticmethod
-    def forward(ctx: Any, q, k, qw, kw, cos, sin, positions, eps, interleaved):
+    def forward(ctx: Any, q, k, qw, kw, cos, sin, positions, eps, scalars):
         ctx.save_for_backward(q, k, qw, kw, cos, sin, positions)
-        ctx.eps, ctx.interleaved = eps, interleaved
-        return _forward(q, k, qw, kw, cos, sin, positions, eps, interleaved)
+        ctx.eps, ctx.scalars = eps, scalars
+        return _forward(rows(q), rows(k), qw, kw, cos, sin, positions, eps, scalars)
 
     @staticmethod
     @once_differentiable
@@ -96,7 +102,7 @@ class _NormRope(torch.autograd.Function):
                 q.data_ptr(), k.data_ptr(), qw.data_ptr(), kw.data_ptr(), cos.data_ptr(), sin.data_ptr(),
                 None if positions is None else positions.data_ptr(), gq.data_ptr(), gk.data_ptr(), dq.data_ptr(),
                 dk.data_ptr(), *(None if t is None else t.data_ptr() for t in (dqw, dkw, partial)), *st,
-                *_scalars(q, k, qw, cos, positions, ctx.eps, ctx.interleaved), _stream(q))
+                *ctx.scalars, ctx.eps, _stream(q))
         _lib.check(rc, "tattn_norm_rope_bwd")
         return dq, dk, dqw, dkw, None, None, None, None, None
 
@@ -111,11 +117,17 @@ def qk_norm_rope(
     [any, dim / 2]). positions: int32 [seq] or [batch, seq]; None: 0, 1, ... A position outside the tables gives a row of
     NaN. Outputs keep their input's strides. Differentiable in q, k and both weights; float16, bfloat16 or float32, all
     arithmetic in float32, each result rounded once. Any batch, head and sequence strides are read in place."""
-    _check(q, k, q_weight, k_weight, cos, sin, positions)
-    _require_gpu(q)
-    qw, kw, cos, sin = _aligned(q_weight), _aligned(k_weight), _aligned(cos), _aligned(sin)
+    key = (layout(q), layout(k), layout(q_weight), layout(k_weight), layout(cos), layout(sin), layout(positions), interleaved)
+    plan = _plans.get(key)
+    if plan is None:
+        plan = _plan(q, k, q_weight, k_weight, cos, sin, positions, interleaved)
+        _require_gpu(q)
+        remember(_plans, key, plan)
+    copies, scalars = plan
+    qw, kw = aligned(q_weight, copies[2]), aligned(k_weight, copies[3])
+    cos, sin = aligned(cos, copies[4]), aligned(sin, copies[5])
     if positions is not None:
         positions = positions.contiguous()
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or q_weight.requires_grad or k_weight.requires_grad):
-        return _NormRope.apply(q, k, qw, kw, cos, sin, positions, float(eps), bool(interleaved))
-    return _forward(q, k, qw, kw, cos, sin, positions, float(eps), bool(interleaved))
+        return _NormRope.apply(q, k, qw, kw, cos, sin, positions, float(eps), scalars)
+    return _forward(aligned(q, copies[0]), aligned(k, copies[1]), qw, kw, cos, sin, positions, float(eps), scalars)

@@ -9,7 +9,6 @@ No counterpart in the reference, whose attention is causal over all keys or unma
 from __future__ import annotations
 
 import ctypes
-import functools
 import math
 from typing import Any
 
@@ -17,7 +16,7 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from tattn import _lib
-from tattn._args import check_index, rows, same_device, strides
+from tattn._args import aligned, check_index, layout, remember, rows_apart, same_device, strides
 from tattn.api import _on_device, _require_gpu, _stream
 
 _DTYPES = {torch.float16: _lib.F16, torch.bfloat16: _lib.BF16}
@@ -44,81 +43,90 @@ def _check(q, k, v, window, sinks, lens) -> None:
         raise ValueError(f"{n} queries for {s} keys: the queries are the last of the keys' positions")
 
 
-def _tiles(t: torch.Tensor) -> torch.Tensor:
-    """t itself where the kernels read its rows in tiles (aligned rows that do not overlap, heads within 31-bit
-    offsets), else an aligned contiguous copy."""
-    t = rows(t)
+def _tiles_apart(t: torch.Tensor) -> bool:
+    """Whether the kernels cannot read t in tiles of rows where it lies: aligned rows that do not overlap, heads within
+    31-bit offsets."""
     n, st, d = t.shape[2], t.stride(2), t.shape[3]
-    if n > 1 and (st < d or st > 1 << 24 or (n + 256) * st * 2 >= 0x7FFFFF00):
-        t = t.clone(memory_format=torch.contiguous_format)
-    return t
+    return rows_apart(t) or (n > 1 and (st < d or st > 1 << 24 or (n + 256) * st * 2 >= 0x7FFFFF00))
 
 
-@functools.lru_cache(maxsize=4096)
-def _workspace(backward: bool, z: int, h: int, hk: int, n: int, s: int, d: int, window: int, sinks: int) -> int:
+def _tiles(t: torch.Tensor) -> torch.Tensor:
+    return aligned(t, _tiles_apart(t))
+
+
+def _workspace(backward: bool, sizes: tuple) -> int:
     """Float32 values of workspace that a call of these sizes needs."""
     out = ctypes.c_int64()
-    _lib.check(_lib.load().tattn_window_workspace(int(backward), z, h, hk, n, s, d, window, sinks, ctypes.byref(out)),
-               "tattn_window_workspace")
+    _lib.check(_lib.load().tattn_window_workspace(int(backward), *sizes, ctypes.byref(out)), "tattn_window_workspace")
     return out.value
 
 
-def _sizes(q, k, window, sinks) -> tuple:
+_plans: dict[tuple, tuple] = {}
+
+
+def _plan(q, k, v, window, sinks, lens) -> tuple:
+    """Checks a call; which of q, k, v are copied, the float32 values of workspace of forward and backward, and the sizes
+    among the launches' arguments (None: nothing to see)."""
+    _check(q, k, v, window, sinks, lens)
+    _require_gpu(q)
+    copies = tuple(_tiles_apart(t) for t in (q, k, v))
     z, h, n, d = q.shape
     hk, s = k.shape[1:3]
-    return z, h, hk, n, s, d, min(window, s), min(sinks, s)
+    if q.numel() == 0 or s == 0:
+        return copies, 0, 0, None
+    sizes = (z, h, hk, n, s, d, min(window, s), min(sinks, s))
+    return copies, _workspace(False, sizes), _workspace(True, sizes) if lens is None else 0, (*sizes, _DTYPES[q.dtype])
 
 
-def _forward(q, k, v, window, sinks, scale, lens, save_lse) -> tuple[torch.Tensor, torch.Tensor | None]:
-    q, k, v = _tiles(q), _tiles(k), _tiles(v)
+def _forward(q, k, v, plan, scale, lens, save_lse) -> tuple[torch.Tensor, torch.Tensor | None]:
+    copies, floats, _, sizes = plan
+    q, k, v = aligned(q, copies[0]), aligned(k, copies[1]), aligned(v, copies[2])
     o = torch.empty_like(q)
     m = q.new_empty(q.shape[:3], dtype=torch.float32) if save_lse else None
-    if q.numel() == 0 or k.shape[2] == 0:
+    if sizes is None:
         return o.zero_(), m
-    sizes = _sizes(q, k, window, sinks)
-    n = _workspace(False, *sizes)
-    work = q.new_empty(n, dtype=torch.float32) if n else None
+    work = q.new_empty(floats, dtype=torch.float32) if floats else None
     _, st = strides(q, k, v, o)
     with _on_device(q):
         rc = _lib.load().tattn_window_fwd(
             q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), None if m is None else m.data_ptr(),
-            None if lens is None else lens.data_ptr(), None if work is None else work.data_ptr(), *st, *sizes,
-            _DTYPES[q.dtype], scale, _stream(q))
-    _lib.check(rc, "tattn_window_fwd")
+            None if lens is None else lens.data_ptr(), None if work is None else work.data_ptr(), *st, *sizes, scale, _stream(q))
+    if rc:
+        _lib.check(rc, "tattn_window_fwd")
     return o, m
 
 
-def _backward(q, k, v, o, m, do, window, sinks, scale) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+def _backward(q, k, v, o, m, do, plan, scale) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    _, _, floats, sizes = plan
     q, k, v, o, do = _tiles(q), _tiles(k), _tiles(v), _tiles(o), _tiles(do)
     dq, dk, dv = torch.empty_like(q), torch.empty_like(k), torch.empty_like(v)
-    if q.numel() == 0 or k.numel() == 0:
+    if sizes is None:
         return dq.zero_(), dk.zero_(), dv.zero_()
     delta = torch.empty_like(m)
-    sizes = _sizes(q, k, window, sinks)
-    n = _workspace(True, *sizes)
-    work = q.new_empty(n, dtype=torch.float32) if n else None
+    work = q.new_empty(floats, dtype=torch.float32) if floats else None
     _, st = strides(q, k, v, o, do, dq, dk, dv)
     with _on_device(q):
         rc = _lib.load().tattn_window_bwd(
             q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), do.data_ptr(), dq.data_ptr(), dk.data_ptr(),
-            dv.data_ptr(), m.data_ptr(), delta.data_ptr(), None if work is None else work.data_ptr(), *st, *sizes,
-            _DTYPES[q.dtype], scale, _stream(q))
-    _lib.check(rc, "tattn_window_bwd")
+            dv.data_ptr(), m.data_ptr(), delta.data_ptr(), None if work is None else work.data_ptr(), *st, *sizes, scale,
+            _stream(q))
+    if rc:
+        _lib.check(rc, "tattn_window_bwd")
     return dq, dk, dv
 
 
 class _Window(torch.autograd.Function):
     @staticmethod
-    def forward(ctx: Any, q, k, v, window, sinks, scale):
-        o, m = _forward(q, k, v, window, sinks, scale, None, True)
+    def forward(ctx: Any, q, k, v, plan, scale):
+        o, m = _forward(q, k, v, plan, scale, None, True)
         ctx.save_for_backward(q, k, v, o, m)
-        ctx.args = window, sinks, scale
+        ctx.args = plan, scale
         return o
 
     @staticmethod
     @once_differentiable
     def backward(ctx: Any, do):
-        return (*_backward(*ctx.saved_tensors, do, *ctx.args), None, None, None)
+        return (*_backward(*ctx.saved_tensors, do, *ctx.args), None, None)
 
 
 def window_attention(
@@ -135,14 +143,14 @@ def window_attention(
     zeros. sm_scale defaults to 1 / sqrt(dim). Differentiable in q, k and v without lens; with lens the call is for serving
     and refuses inputs that require gradients. A key or value that is infinite or NaN makes the rows that see it
     NaN, and may make NaN of rows up to 64 positions before it or after its window that do not see it."""
-    _check(q, k, v, window, sinks, lens)
-    needs = torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad)
+    key = (layout(q), layout(k), layout(v), layout(lens), window, sinks)
+    plan = _plans.get(key)
+    needs = (q.requires_grad or k.requires_grad or v.requires_grad) and torch.is_grad_enabled()
     if needs and lens is not None:
         raise ValueError("no gradients with lens: call it under torch.no_grad(), or without lens")
-    _require_gpu(q)
+    if plan is None:
+        plan = remember(_plans, key, _plan(q, k, v, int(window), int(sinks), lens))
     scale = float(sm_scale) if sm_scale is not None else 1.0 / math.sqrt(q.shape[3])
-    if lens is not None:
-        lens = lens.contiguous()
     if needs:
-        return _Window.apply(q, k, v, int(window), int(sinks), scale)
-    return _forward(q, k, v, int(window), int(sinks), scale, lens, False)[0]
+        return _Window.apply(q, k, v, plan, scale)
+    return _forward(q, k, v, plan, scale, None if lens is None else lens.contiguous(), False)[0]
