@@ -71,13 +71,22 @@ struct ColMask {
   }
 };
 
-// Whether rows at positions [p0, p1] see nothing of tile t, or all of it.
-__device__ __forceinline__ bool tile_hidden(int p0, int p1, int t, int window, int sinks) {
-  return 32 * t > p1 || (32 * t + 31 < p0 - window + 1 && 32 * t >= sinks);
-}
-__device__ __forceinline__ bool tile_masked(int p0, int p1, int t, int window, int sinks) {
-  return 32 * t + 31 > p0 || (32 * t < p1 - window + 1 && 32 * t + 31 >= sinks);
-}
+// What a wave whose rows are at positions [p0, p1] sees of the tiles: nothing of a tile (live() is false), or some of it
+// (masked()), or all. p1 < 0: no rows.
+struct WaveTiles {
+  int lo, hi, sinks;                 // live: t <= hi, from lo on or with first keys
+  int full_lo, full_hi, full_sinks;  // seen by all rows
+  __device__ __forceinline__ void init(int p0, int p1, int window, int sinks_) {
+    hi = p1 < 0 ? -1 : p1 >> 5;
+    lo = max(0, p0 - window + 1) >> 5;
+    sinks = (sinks_ + 31) >> 5;
+    full_hi = ((p0 + 1) >> 5) - 1;
+    full_lo = (max(0, p1 - window + 1) + 31) >> 5;
+    full_sinks = sinks_ >> 5;
+  }
+  __device__ __forceinline__ bool live(int t) const { return t <= hi && (t >= lo || t < sinks); }
+  __device__ __forceinline__ bool masked(int t) const { return t > full_hi || (t < full_lo && t >= full_sinks); }
+};
 
 // Everything this wave has in flight has landed, its LDS reads are done, then the barrier.
 __device__ __forceinline__ void all_landed_barrier() {

@@ -178,7 +178,8 @@ __global__ __launch_bounds__(RW * CS * 64, OCC) void window_fwd_kernel(const Win
   const int n = (live ? row : 0) / p.G, g = (live ? row : 0) % p.G;
   const int pos = b.off + n;
   // The wave's positions; a wave without rows sees no tile.
-  const int wp0 = b.off + tile0 / p.G, wp1 = tile0 < b.rows ? b.off + min(tile0 + 31, b.rows - 1) / p.G : -1;
+  WaveTiles sees;
+  sees.init(b.off + tile0 / p.G, tile0 < b.rows ? b.off + min(tile0 + 31, b.rows - 1) / p.G : -1, p.window, p.sinks);
   V8 qop[NSD];
   {
     const T* src = (const T*)p.q + b.z * p.sq[0] + (b.hk * p.G + g) * p.sq[1] + n * p.sq[2] + 8 * h2;
@@ -205,7 +206,7 @@ __global__ __launch_bounds__(RW * CS * 64, OCC) void window_fwd_kernel(const Win
     f32x16 s = f32x16{};
 #pragma unroll
     for (int sd = 0; sd < NSD; ++sd) s = Elt<T>::mfma(lds8<T>(st + at.nat[sd]), qop[sd], s);
-    if (tile_masked(wp0, wp1, t, p.window, p.sinks)) RowMask(pos, t, h2, p.window, p.sinks).hide(s, hidden);
+    if (sees.masked(t)) RowMask(pos, t, h2, p.window, p.sinks).hide(s, hidden);
     V8 x[2];
     auto probs = [&]() __attribute__((always_inline)) {
       float ps = 0.0f;
@@ -249,11 +250,11 @@ __global__ __launch_bounds__(RW * CS * 64, OCC) void window_fwd_kernel(const Win
   auto step = [&](int i, char* cur, char* nxt) __attribute__((always_inline)) {
     if (i + 1 < nsteps) issue(nxt, i + 1);
     const int k = i0 + i * NT + cs;
-#pragma unroll 1
+#pragma unroll
     for (int x = 0; x < TP; ++x) {
       if (k + x * CS >= i1) break;
       const int t = list.at(k + x * CS);
-      if (tile_hidden(wp0, wp1, t, p.window, p.sinks)) continue;
+      if (!sees.live(t)) continue;
       tile(cur + x * CS * R::TILE, t);
     }
     all_landed_barrier();
@@ -426,7 +427,8 @@ __global__ __launch_bounds__(RW * CS * 64, OCC) void window_dq_kernel(const Wind
   const bool live = row < b.rows;
   const int n = (live ? row : 0) / p.G, g = (live ? row : 0) % p.G, h = b.hk * p.G + g;
   const int pos = b.off + n;
-  const int wp0 = b.off + tile0 / p.G, wp1 = tile0 < b.rows ? b.off + min(tile0 + 31, b.rows - 1) / p.G : -1;
+  WaveTiles sees;
+  sees.init(b.off + tile0 / p.G, tile0 < b.rows ? b.off + min(tile0 + 31, b.rows - 1) / p.G : -1, p.window, p.sinks);
   const int64_t mrow = ((int64_t)b.z * p.H + h) * p.N + n;
   V8 qop[NSD], dop[NSD];
   float dl;
@@ -463,7 +465,7 @@ __global__ __launch_bounds__(RW * CS * 64, OCC) void window_dq_kernel(const Wind
       s = Elt<T>::mfma(lds8<T>(st + at.nat[sd]), qop[sd], s);
       dp = Elt<T>::mfma(lds8<T>(st + R::HALF + at.nat[sd]), dop[sd], dp);
     }
-    if (tile_masked(wp0, wp1, t, p.window, p.sinks)) RowMask(pos, t, h2, p.window, p.sinks).hide(s, hidden);
+    if (sees.masked(t)) RowMask(pos, t, h2, p.window, p.sinks).hide(s, hidden);
 #pragma unroll
     for (int r = 0; r < 16; ++r) s[r] = fast_exp2(__builtin_fmaf(s[r], c, nm)) * dp[r];
     V8 ds[2];
@@ -487,11 +489,11 @@ __global__ __launch_bounds__(RW * CS * 64, OCC) void window_dq_kernel(const Wind
   auto step = [&](int i, char* cur, char* nxt) __attribute__((always_inline)) {
     if (i + 1 < nsteps) issue(nxt, i + 1);
     const int k = i * NT + cs;
-#pragma unroll 1
+#pragma unroll
     for (int x = 0; x < TP; ++x) {
       if (k + x * CS >= list.n) break;
       const int t = list.at(k + x * CS);
-      if (tile_hidden(wp0, wp1, t, p.window, p.sinks)) continue;
+      if (!sees.live(t)) continue;
       tile(cur + x * CS * R::TILE, t);
     }
     all_landed_barrier();
