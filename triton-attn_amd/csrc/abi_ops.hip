@@ -280,7 +280,7 @@ int tattn_window_workspace(int backward, int64_t Z, int64_t H, int64_t Hk, int64
   if (backward) {
     *floats = window_bwd_part_floats(p, (int)D);
   } else {
-    const int splits = window_fwd_splits(p);
+    const int splits = window_fwd_splits(p, (int)D);
     *floats = splits > 1 ? window_part_floats(Z * Hk, N * p.G, splits, D) : 0;
   }
   return TATTN_OK;
@@ -297,7 +297,7 @@ int tattn_window_fwd(const void* q, const void* k, const void* v, void* o, float
       (rc = check_tiles("v", v, v_strides, S, D, p.sv)) || (rc = check_tiles("o", o, o_strides, N, D, p.sout)) ||
       (rc = check_ptr("m", m, 0, 4)) || (rc = check_ptr("lens", lens, 0, 4)))
     return rc;
-  p.splits = window_fwd_splits(p);
+  p.splits = window_fwd_splits(p, (int)D);
   if ((rc = check_ptr("workspace", workspace, p.splits > 1, 16)) || (rc = require_device())) return rc;
   p.q = q; p.k = k; p.v = v; p.out = o; p.m = m; p.lens = lens; p.part = workspace;
   p.c = window_exponent_scale(sm_scale);

@@ -99,7 +99,7 @@ struct WindowParams {
 inline int64_t window_part_floats(int64_t slices, int64_t rows, int64_t splits, int64_t D) {
   return slices * rows * splits * (D + 2);
 }
-int window_fwd_splits(const WindowParams& p);  // 0: no parts and two row tiles per workgroup
+int window_fwd_splits(const WindowParams& p, int D);  // 0: no parts and two row tiles per workgroup
 int window_bwd_splits(const WindowParams& p, int D);
 int64_t window_bwd_part_floats(const WindowParams& p, int D);
 int launch_window_fwd(WindowParams p, int D, int dtype, hipStream_t st);

@@ -1,8 +1,8 @@
 // Attention over a sliding window and the first keys, 16-bit, forward and backward, on gfx950.
 //
-// A workgroup's NW = RW * CS waves own RW 32-row tiles; a step stages CS * TP tiles of the other dimension by LDS DMA
+// A workgroup's NW = RW * CS waves own RW 32-row tiles; a step stages CS tiles of the other dimension by LDS DMA
 // (buffer_load ... lds, swizzled rows) into one of two stages while the other is worked on. With many rows CS is 1 and each wave
-// works on all TP tiles of a step for its own rows; with few, wave (rw, cs) takes every CS-th tile, and the CS partial
+// works on every tile for its own rows; with few, wave (rw, cs) takes every CS-th tile, and the CS partial
 // results of a row tile are added through LDS at the end. Only tiles that some row of the workgroup sees are walked
 // (TileList), only those at the ends of a row's window pay for masks, and a wave passes over tiles that none of its own rows sees.
 //
@@ -16,15 +16,16 @@
 namespace tattn {
 namespace {
 
-// A stage: NT tiles of each of two tensors. Each wave fetches TW whole tiles of a step, the first half of the waves of
-// the first tensor.
+// A stage: NT tiles of each of two tensors. Each wave fetches PPW 1 KB pieces of a step, TW whole tiles or a part of one,
+// the first half of the waves of the first tensor.
 template <int D, int NW, int NT>
 struct WinRing {
-  static constexpr int RB = Swz<D>::RB, TILE = 32 * RB, PIECES = TILE / 1024;  // 1 KB DMA pieces
+  static constexpr int RB = Swz<D>::RB, TILE = 32 * RB, PIECES = TILE / 1024;
   static constexpr int HALF = NT * TILE;  // bytes of one tensor's tiles
   static constexpr int STAGE = 2 * HALF;
-  static constexpr int TW = 2 * NT / NW;
-  static_assert(TW >= 1 && TW * NW == 2 * NT && NW % 2 == 0, "whole tiles, one tensor per wave");
+  static constexpr int PPW = 2 * NT * PIECES / NW;
+  static constexpr int TW = PPW > PIECES ? PPW / PIECES : 1, PPT = PPW / TW;  // pieces per tile
+  static_assert(PPW >= 1 && TW * PPT * NW == 2 * NT * PIECES && PIECES % PPT == 0 && NW % 2 == 0, "whole pieces, one tensor per wave");
 };
 
 constexpr uint32_t kBeyond = 0x7fffffffu;  // byte offset past every slice: reads as zero
@@ -32,27 +33,28 @@ constexpr uint32_t kBeyond = 0x7fffffffu;  // byte offset past every slice: read
 template <int D, int NW, int NT>
 struct WinLoader {
   using R = WinRing<D, NW, NT>;
-  uint32_t go[R::PIECES];
+  uint32_t go[R::PPT];
   uint32_t tile_bytes;
-  int first, base, lane;  // first tile of the wave's TW, and its place in a stage
+  int first, piece0, base, lane;  // first tile of the wave's TW, first piece of it, and its place in a stage
   bool second;
   __device__ __forceinline__ void init(int64_t sa, int64_t sb, int wu, int lane_) {
     lane = lane_;
     second = wu >= NW / 2;
     const int64_t st = second ? sb : sa;
     tile_bytes = uniform32((uint32_t)(st * 64));
-    first = wu % (NW / 2) * R::TW;
-    base = (second ? R::HALF : 0) + first * R::TILE;
+    first = wu % (NW / 2) * R::PPW / R::PIECES;
+    piece0 = wu % (NW / 2) * R::PPW % R::PIECES;
+    base = (second ? R::HALF : 0) + first * R::TILE + 1024 * piece0;
     constexpr int CPR = R::RB / 16;
 #pragma unroll
-    for (int i = 0; i < R::PIECES; ++i) {
-      const int j = 64 * i + lane;
+    for (int i = 0; i < R::PPT; ++i) {
+      const int j = 64 * (piece0 + i) + lane;
       const int row = j / CPR, cc = ((j % CPR) ^ Swz<D>::f(row)) & (D / 8 - 1);
       go[i] = (uint32_t)(perm32(row) * st * 2 + cc * 16);
     }
   }
-  // Row of a tile that the lane fetches in piece i.
-  __device__ __forceinline__ int row(int i) const { return perm32((64 * i + lane) / (R::RB / 16)); }
+  // Row of a tile that the lane fetches in the wave's piece i.
+  __device__ __forceinline__ int row(int i) const { return perm32((64 * (piece0 + i) + lane) / (R::RB / 16)); }
   __device__ __forceinline__ void fetch(__amdgpu_buffer_rsrc_t rs, char* stage, int x, int i, uint32_t off) const {
     __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (TATTN_LDS void*)(stage + base + x * R::TILE + 1024 * i), 16, (int)off, 0, 0, 0);
   }
@@ -120,27 +122,27 @@ __device__ __forceinline__ void fetch_keys(const WinLoader<D, NW, NT>& ld, __amd
     const uint32_t o = (uint32_t)t * ld.tile_bytes;
     if (32 * t + 31 > top || (32 * t < list.lo && 32 * t + 31 >= sinks)) {
 #pragma unroll
-      for (int i = 0; i < R::PIECES; ++i) {
+      for (int i = 0; i < R::PPT; ++i) {
         const int key = 32 * t + ld.row(i);
         const bool dead = key > top || (key < list.lo && key >= sinks);
         ld.fetch(rs, stage, x, i, dead ? kBeyond : ld.go[i] + o);
       }
     } else {
 #pragma unroll
-      for (int i = 0; i < R::PIECES; ++i) ld.fetch(rs, stage, x, i, ld.go[i] + o);
+      for (int i = 0; i < R::PPT; ++i) ld.fetch(rs, stage, x, i, ld.go[i] + o);
     }
   }
 }
 
 // ---- forward -----------------------------------------------------------------------------------
-template <typename T, int D, int RW, int CS, int TP, int OCC, bool SPLIT>
+template <typename T, int D, int RW, int CS, int OCC, bool SPLIT>
 __global__ __launch_bounds__(RW * CS * 64, OCC) void window_fwd_kernel(const WindowParams p) {
   using H = H16<T>;
   using V8 = typename H::V8;
   using V4 = typename H::V4;
   using V2 = typename H::V2;
-  constexpr int NW = RW * CS, NT = CS * TP, NSD = D / 16, DT = (D + 31) / 32;
-  using R = WinRing<D, NW, NT>;
+  constexpr int NW = RW * CS, NSD = D / 16, DT = (D + 31) / 32;
+  using R = WinRing<D, NW, CS>;
   // Two arrays: a DMA into one stage does not alias reads of the other.
   __shared__ __attribute__((aligned(1024))) char s0[R::STAGE];
   __shared__ __attribute__((aligned(1024))) char s1[R::STAGE];
@@ -160,15 +162,15 @@ __global__ __launch_bounds__(RW * CS * 64, OCC) void window_fwd_kernel(const Win
   list.init(b.p0, b.p1, p.window, p.sinks);
   const int i0 = SPLIT ? (int)((int64_t)list.n * split / p.splits) : 0;
   const int i1 = SPLIT ? (int)((int64_t)list.n * (split + 1) / p.splits) : list.n;
-  const int nsteps = (i1 - i0 + NT - 1) / NT;
+  const int nsteps = (i1 - i0 + CS - 1) / CS;
 
-  WinLoader<D, NW, NT> ld;
+  WinLoader<D, NW, CS> ld;
   ld.init(p.sk[2], p.sv[2], wu, lane);
   const __amdgpu_buffer_rsrc_t rs =
       ld.second ? win_rsrc<T, D>(p.v, b.z * p.sv[0] + b.hk * p.sv[1], b.len, p.sv[2])
                 : win_rsrc<T, D>(p.k, b.z * p.sk[0] + b.hk * p.sk[1], b.len, p.sk[2]);
   auto issue = [&](char* stage, int step) __attribute__((always_inline)) {
-    fetch_keys<D, NW, NT>(ld, rs, stage, list, i0 + step * NT, i1, b.top, p.sinks);
+    fetch_keys<D, NW, CS>(ld, rs, stage, list, i0 + step * CS, i1, b.top, p.sinks);
   };
   if (nsteps > 0) issue(s0, 0);
 
@@ -249,13 +251,10 @@ __global__ __launch_bounds__(RW * CS * 64, OCC) void window_fwd_kernel(const Win
   };
   auto step = [&](int i, char* cur, char* nxt) __attribute__((always_inline)) {
     if (i + 1 < nsteps) issue(nxt, i + 1);
-    const int k = i0 + i * NT + cs;
-#pragma unroll
-    for (int x = 0; x < TP; ++x) {
-      if (k + x * CS >= i1) break;
-      const int t = list.at(k + x * CS);
-      if (!sees.live(t)) continue;
-      tile(cur + x * CS * R::TILE, t);
+    const int k = i0 + i * CS + cs;
+    if (k < i1) {
+      const int t = list.at(k);
+      if (sees.live(t)) tile(cur, t);
     }
     all_landed_barrier();
   };
@@ -388,14 +387,14 @@ __global__ __launch_bounds__(256) void combine_kernel(const float* part, T* out,
 
 // ---- dQ ------------------------------------------------------------------------------------------
 // Rows and key tiles as in the forward; computes delta = rowsum(dO * O) on the way and stores -delta for dK / dV.
-template <typename T, int D, int RW, int CS, int TP, int OCC>
+template <typename T, int D, int RW, int CS, int OCC>
 __global__ __launch_bounds__(RW * CS * 64, OCC) void window_dq_kernel(const WindowParams p) {
   using H = H16<T>;
   using V8 = typename H::V8;
   using V4 = typename H::V4;
   using V2 = typename H::V2;
-  constexpr int NW = RW * CS, NT = CS * TP, NSD = D / 16, DT = (D + 31) / 32;
-  using R = WinRing<D, NW, NT>;
+  constexpr int NW = RW * CS, NSD = D / 16, DT = (D + 31) / 32;
+  using R = WinRing<D, NW, CS>;
   __shared__ __attribute__((aligned(1024))) char s0[R::STAGE];
   __shared__ __attribute__((aligned(1024))) char s1[R::STAGE];
 
@@ -410,15 +409,15 @@ __global__ __launch_bounds__(RW * CS * 64, OCC) void window_dq_kernel(const Wind
   b.init(p, slice, p.nblk - 1 - blk, RW);
   TileList list;
   list.init(b.p0, b.p1, p.window, p.sinks);
-  const int nsteps = (list.n + NT - 1) / NT;
+  const int nsteps = (list.n + CS - 1) / CS;
 
-  WinLoader<D, NW, NT> ld;
+  WinLoader<D, NW, CS> ld;
   ld.init(p.sk[2], p.sv[2], wu, lane);
   const __amdgpu_buffer_rsrc_t rs =
       ld.second ? win_rsrc<T, D>(p.v, b.z * p.sv[0] + b.hk * p.sv[1], b.len, p.sv[2])
                 : win_rsrc<T, D>(p.k, b.z * p.sk[0] + b.hk * p.sk[1], b.len, p.sk[2]);
   auto issue = [&](char* stage, int step) __attribute__((always_inline)) {
-    fetch_keys<D, NW, NT>(ld, rs, stage, list, step * NT, list.n, b.top, p.sinks);
+    fetch_keys<D, NW, CS>(ld, rs, stage, list, step * CS, list.n, b.top, p.sinks);
   };
   if (nsteps > 0) issue(s0, 0);
 
@@ -488,13 +487,10 @@ __global__ __launch_bounds__(RW * CS * 64, OCC) void window_dq_kernel(const Wind
   };
   auto step = [&](int i, char* cur, char* nxt) __attribute__((always_inline)) {
     if (i + 1 < nsteps) issue(nxt, i + 1);
-    const int k = i * NT + cs;
-#pragma unroll
-    for (int x = 0; x < TP; ++x) {
-      if (k + x * CS >= list.n) break;
-      const int t = list.at(k + x * CS);
-      if (!sees.live(t)) continue;
-      tile(cur + x * CS * R::TILE, t);
+    const int k = i * CS + cs;
+    if (k < list.n) {
+      const int t = list.at(k);
+      if (sees.live(t)) tile(cur, t);
     }
     all_landed_barrier();
   };
@@ -570,16 +566,16 @@ struct KeyBlocks {
   }
 };
 
-template <typename T, int D, int RW, int CS, int TP, int OCC>
+template <typename T, int D, int RW, int CS, int OCC>
 __global__ __launch_bounds__(RW * CS * 64, OCC) void window_dkdv_kernel(const WindowParams p) {
   using H = H16<T>;
   using V8 = typename H::V8;
   using V2 = typename H::V2;
-  constexpr int NW = RW * CS, NT = CS * TP, NSD = D / 16, DT = (D + 31) / 32;
-  using R = WinRing<D, NW, NT>;
+  constexpr int NW = RW * CS, NSD = D / 16, DT = (D + 31) / 32;
+  using R = WinRing<D, NW, CS>;
   __shared__ __attribute__((aligned(1024))) char s0[R::STAGE];
   __shared__ __attribute__((aligned(1024))) char s1[R::STAGE];
-  __shared__ __attribute__((aligned(16))) float md[NW][2][TP][64];  // per wave, parity and tile: M[32], -delta[32]
+  __shared__ __attribute__((aligned(16))) float md[NW][2][64];  // per wave and parity: M[32], -delta[32]
 
   const int tid = threadIdx.x;
   const int lane = tid & 63, h2 = lane >> 5, l32 = lane & 31;
@@ -601,9 +597,9 @@ __global__ __launch_bounds__(RW * CS * 64, OCC) void window_dkdv_kernel(const Wi
   const int total = nq * p.G;
   const int i0 = parted ? (int)((int64_t)total * split / p.splits) : 0;
   const int i1 = parted ? (int)((int64_t)total * (split + 1) / p.splits) : total;
-  const int nsteps = (i1 - i0 + NT - 1) / NT;
+  const int nsteps = (i1 - i0 + CS - 1) / CS;
 
-  WinLoader<D, NW, NT> ld;
+  WinLoader<D, NW, CS> ld;
   ld.init(p.sq[2], p.sd[2], wu, lane);
   const char* qbase = ld.second ? (const char*)((const T*)p.dout + z * p.sd[0] + (int64_t)hk * p.G * p.sd[1])
                                 : (const char*)((const T*)p.q + z * p.sq[0] + (int64_t)hk * p.G * p.sq[1]);
@@ -612,35 +608,24 @@ __global__ __launch_bounds__(RW * CS * 64, OCC) void window_dkdv_kernel(const Wi
   auto issue = [&](char* stage, int step) __attribute__((always_inline)) {
 #pragma unroll
     for (int x = 0; x < R::TW; ++x) {
-      const int k = i0 + step * NT + ld.first + x;
+      const int k = i0 + step * CS + ld.first + x;
       if (k >= i1) break;
       const int g = k / nq, qt = qt0 + k % nq;
       // Rows past the head's last query lie past the end of its slice and read as zero.
       const __amdgpu_buffer_rsrc_t rs = slice_rsrc(qbase + g * head_bytes, qbytes);
 #pragma unroll
-      for (int i = 0; i < R::PIECES; ++i) ld.fetch(rs, stage, x, i, ld.go[i] + (uint32_t)qt * ld.tile_bytes);
+      for (int i = 0; i < R::PPT; ++i) ld.fetch(rs, stage, x, i, ld.go[i] + (uint32_t)qt * ld.tile_bytes);
     }
   };
   if (nsteps > 0) issue(s0, 0);
   // Lanes 0-31 fetch M and lanes 32-63 -delta of the wave's tile; zero past the end.
   const float* mdsrc = (h2 ? p.delta : p.m) + ((int64_t)z * p.H + hk * p.G) * p.N;
-  auto md_load = [&](int step, float (&x)[TP]) __attribute__((always_inline)) {
-#pragma unroll
-    for (int t = 0; t < TP; ++t) {
-      const int k = i0 + step * NT + cs + t * CS;
-      const int q = k < i1 ? 32 * (qt0 + k % nq) + l32 : p.N;
-      x[t] = q < p.N ? mdsrc[(int64_t)(k / nq) * p.N + q] : 0.0f;
-    }
+  auto md_load = [&](int step) __attribute__((always_inline)) {
+    const int k = i0 + step * CS + cs;
+    const int q = k < i1 ? 32 * (qt0 + k % nq) + l32 : p.N;
+    return q < p.N ? mdsrc[(int64_t)(k / nq) * p.N + q] : 0.0f;
   };
-  auto md_store = [&](int par, const float (&x)[TP]) __attribute__((always_inline)) {
-#pragma unroll
-    for (int t = 0; t < TP; ++t) md[wu][par][t][lane] = x[t];
-  };
-  float mdn[TP];
-  if (nsteps > 0) {
-    md_load(0, mdn);
-    md_store(0, mdn);
-  }
+  md[wu][0][lane] = nsteps > 0 ? md_load(0) : 0.0f;
   const int kt = kb * RW + rw, key = 32 * kt + l32;
   V8 kop[NSD], vop[NSD];
   {
@@ -708,19 +693,18 @@ __global__ __launch_bounds__(RW * CS * 64, OCC) void window_dkdv_kernel(const Wi
   };
   const int wk0 = 32 * kt, wk1 = wk0 + 31;
   auto step = [&](int i, char* cur, char* nxt, int par) __attribute__((always_inline)) {
+    float mdn = 0.0f;
     if (i + 1 < nsteps) {
       issue(nxt, i + 1);
-      md_load(i + 1, mdn);
+      mdn = md_load(i + 1);
     }
-    const int k = i0 + i * NT + cs;
-#pragma unroll 1
-    for (int x = 0; x < TP; ++x) {
-      if (k + x * CS >= i1 || wk0 >= p.S) break;
-      const int qt = qt0 + (k + x * CS) % nq, q0 = off + 32 * qt, q1 = q0 + 31;
+    const int k = i0 + i * CS + cs;
+    if (k < i1 && wk0 < p.S) {
+      const int qt = qt0 + k % nq, q0 = off + 32 * qt, q1 = q0 + 31;
       if (q1 >= wk0 && (q0 - wk1 < p.window || wk0 < p.sinks))
-        tile(cur + x * CS * R::TILE, md[wu][par][x], qt, q0 < wk1 || (q1 - wk0 >= p.window && wk1 >= p.sinks) || 32 * qt + 32 > p.N);
+        tile(cur, md[wu][par], qt, q0 < wk1 || (q1 - wk0 >= p.window && wk1 >= p.sinks) || 32 * qt + 32 > p.N);
     }
-    if (i + 1 < nsteps) md_store(par ^ 1, mdn);  // the wave's own rows: no barrier needed
+    md[wu][par ^ 1][lane] = mdn;  // the wave's own rows: no barrier needed
     all_landed_barrier();
   };
   all_landed_barrier();
@@ -1042,8 +1026,9 @@ __global__ __launch_bounds__(256) void window_first_keys_kernel(const WindowPara
 }
 
 // ---- launch ----------------------------------------------------------------------------------------
-// Row tiles per workgroup and key tiles per step.
-template <int D> struct WinShape { static constexpr int RW = 4, TP = 2, OCC = D == 128 ? 2 : 4; };
+// Row tiles per workgroup, and waves per SIMD of the forward. One key tile per step: its 32 KB of stages at head dim 128 let three
+// workgroups share a CU (two tiles and two workgroups: 1,129 us against 1,048 at 16,384 x 32/8 x 128, window 4,096).
+template <int D> struct WinShape { static constexpr int RW = 4, OCC = D == 128 ? 3 : 4; };
 template <int D> struct KeyShape { static constexpr int RW = D >= 64 ? 4 : 2, CS = 4; };
 
 int grid_of(int64_t slices, int64_t per_slice, unsigned* out) {
@@ -1073,17 +1058,17 @@ int fwd_d(WindowParams p, hipStream_t st) {
     p.nblk = (int)((rows + 31) / 32);
     if ((rc = grid_of(slices, (int64_t)p.nblk * p.splits, &blocks))) return rc;
     if (p.splits == 1) {
-      window_fwd_kernel<T, D, 1, 4, 1, D == 128 ? 1 : 2, false><<<dim3(blocks), dim3(256), 0, st>>>(p);
+      window_fwd_kernel<T, D, 1, 4, D == 128 ? 1 : 2, false><<<dim3(blocks), dim3(256), 0, st>>>(p);
       return check_launch("tattn_window_fwd");
     }
-    window_fwd_kernel<T, D, 1, 4, 1, D == 128 ? 1 : 2, true><<<dim3(blocks), dim3(256), 0, st>>>(p);
+    window_fwd_kernel<T, D, 1, 4, D == 128 ? 1 : 2, true><<<dim3(blocks), dim3(256), 0, st>>>(p);
     if ((rc = check_launch("tattn_window_fwd"))) return rc;
     return launch_combine(p.part, p.out, p.m, p.sout, slices, p.Hk, p.G, p.N, p.splits, D, std::is_same_v<T, bf16> ? 2 : 0, st);
   }
   using S = WinShape<D>;
   p.nblk = (int)((rows + 32 * S::RW - 1) / (32 * S::RW));
   if ((rc = grid_of(slices, p.nblk, &blocks))) return rc;
-  window_fwd_kernel<T, D, S::RW, 1, S::TP, S::OCC, false><<<dim3(blocks), dim3(S::RW * 64), 0, st>>>(p);
+  window_fwd_kernel<T, D, S::RW, 1, S::OCC, false><<<dim3(blocks), dim3(S::RW * 64), 0, st>>>(p);
   return check_launch("tattn_window_fwd");
 }
 
@@ -1098,14 +1083,14 @@ int bwd_d(WindowParams p, hipStream_t st) {
   p.runs = in_runs(p);
   p.nblk = (int)((rows + 32 * S::RW - 1) / (32 * S::RW));
   if ((rc = grid_of(slices, p.nblk, &blocks))) return rc;
-  window_dq_kernel<T, D, S::RW, 1, S::TP, D >= 64 ? 2 : 4><<<dim3(blocks), dim3(S::RW * 64), 0, st>>>(p);
+  window_dq_kernel<T, D, S::RW, 1, D >= 64 ? 2 : 4><<<dim3(blocks), dim3(S::RW * 64), 0, st>>>(p);
   if ((rc = check_launch("tattn_window_bwd"))) return rc;
   const KeyBlocks<K::RW> kbs(p.S, p.sinks, splits);
   if ((rc = grid_of(slices, kbs.items, &blocks))) return rc;
   if constexpr (D >= 64)
     window_dkdv_pair_kernel<T, D, D == 64 ? 4 : 2><<<dim3(blocks), dim3(512), 0, st>>>(p);
   else
-    window_dkdv_kernel<T, D, K::RW, K::CS, 1, D == 32 ? 3 : 4><<<dim3(blocks), dim3(K::RW * K::CS * 64), 0, st>>>(p);
+    window_dkdv_kernel<T, D, K::RW, K::CS, D == 32 ? 3 : 4><<<dim3(blocks), dim3(K::RW * K::CS * 64), 0, st>>>(p);
   if ((rc = check_launch("tattn_window_bwd")) || !kbs.sink_blocks) return rc;
   const int64_t n = slices * kbs.sink_blocks * 2 * 32 * K::RW * D;
   window_first_keys_kernel<T, D, K::RW><<<dim3((unsigned)((n + 255) / 256)), dim3(256), 0, st>>>(p);
@@ -1133,13 +1118,15 @@ int combine_d(const float* part, void* out, float* m, const int64_t so[3], int64
 
 }  // namespace
 
-// Few rows: one row tile per workgroup, and its keys cut into parts until the chip has two workgroups per CU, each with
-// at least eight tiles. 0: enough rows for the blocks of two row tiles.
-int window_fwd_splits(const WindowParams& p) {
+// Few rows (a single row tile per slice, or fewer blocks of four than CUs): one row tile per workgroup, and its keys cut into
+// parts of at least eight tiles until the chip holds no more workgroups at once, one per CU at head dim 128 (128 KB of
+// stages), two below. (32 x 32/8 heads x 8,192 keys x 128, window 2,048: 51.5 us at one per CU, 59 at two, 68 at four.) 0:
+// blocks of four row tiles.
+int window_fwd_splits(const WindowParams& p, int D) {
   const int64_t slices = (int64_t)p.Z * p.Hk, rows = (int64_t)p.N * p.G;
-  if (slices * ((rows + 63) / 64) >= 256) return 0;
-  const int64_t blocks = slices * ((rows + 31) / 32);
-  return (int)std::max<int64_t>(1, std::min<int64_t>((512 + blocks - 1) / blocks, most_tiles(p) / 8));
+  if (rows > 32 && slices * ((rows + 127) / 128) >= 256) return 0;
+  const int64_t blocks = slices * ((rows + 31) / 32), want = D == 128 ? 256 : 512;
+  return (int)std::max<int64_t>(1, std::min<int64_t>((want + blocks - 1) / blocks, most_tiles(p) / 8));
 }
 
 // Parts of the first keys' dK and dV: each about as long as another key block's list, or as an even share of all
