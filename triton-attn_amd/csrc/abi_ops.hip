@@ -152,7 +152,7 @@ int cache4_attn_common(Cache4AttnParams& p, int64_t R, int64_t H, int64_t Hk, in
   if (width * page_size > 0x7fffffff - 4096)
     return set_error(TATTN_E_ARG, "a table row of %lld pages holds 2^31 tokens or more", (long long)width);
   if (window < 0 || sinks < 0) return set_error(TATTN_E_ARG, "window and sinks must not be negative");
-  p.R = (int32_t)R; p.Hk = (int32_t)Hk; p.G = (int32_t)(H / Hk); p.groups = (p.G + 31) / 32;
+  p.R = (int32_t)R; p.Hk = (int32_t)Hk; p.G = (int32_t)(H / Hk); p.groups = (p.G + 15) / 16;
   if ((double)R * (double)Hk * p.groups > 67108864.0) return set_error(TATTN_E_ARG, "too many requests: %lld", (long long)R);
   p.most = (int32_t)(width * page_size);
   p.window = window == 0 || window > p.most ? p.most + 1 : (int32_t)window;
@@ -361,7 +361,7 @@ int tattn_cache4_attention(const void* q, void* o, const uint8_t* codes, const u
   for (int i = 0; i < 2; ++i) p.sq[i] = q_strides[i], p.so[i] = o_strides[i];
   p.table_stride = table_stride;
   p.pages = (int32_t)pages;
-  p.c = sm_scale * kLog2e;
+  p.c = window_exponent_scale(sm_scale);
   return launch_cache4_attention(p, (int)D, dtype, (hipStream_t)stream);
 }
 

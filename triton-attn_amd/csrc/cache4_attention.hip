@@ -1,12 +1,16 @@
 // Attention of one token per request over a paged cache in 4 bits, on gfx950.
 //
-// Bound by the cache's bytes: 17/32 D for a key and as many for a value, read once for all G query heads that share
-// them, whose rows fill the 32 columns of a matrix instruction (unused columns cost nothing that bounds the kernel).
-// A wave takes 32 keys at a time, alone: lane (key, half of d) loads that half row's codes of K and of V,
-// converts two codes an instruction (v_cvt_scalef32_pk, which also applies the block's power of two), and
-//   S^T = K Q^T     K's codes become operands in the lane that loaded them: the order of d within a dot product is
-//                   free, so each lane half owns one contiguous half of d, for Q as well
-//   O^T += V^T P^T  V's values go through the wave's own 32 rows of LDS, swizzled, and come back transposed
+// Bound by the cache's bytes: 17/32 D for a key and as many for a value, read once for up to 16 query heads that share
+// them, whose rows are the columns of 16 x 16 x 32 matrix instructions (unused columns cost nothing that bounds the kernel).
+//   v_mfma_f32_16x16x32: A lane holds A[m = lane % 16][k = 8 (lane / 16) + i], B lane B[k = 8 (lane / 16) + i][n = lane % 16],
+//   C lane holds C[m = 4 (lane / 16) + r][n = lane % 16], r < 4
+// A wave takes 32 keys at a time, alone. Lane (l, g) = (lane % 16, lane / 16) loads a quarter row, codes of K and of V and
+// their exponent, of two keys, 8 (l / 4) + 4 a + l % 4 of the tile for a = 0, 1, converts two codes an instruction
+// (v_cvt_scalef32_pk, which also applies the block's power of two), and
+//   S^T = K Q^T     two 16-key tiles. K's codes become operands in the lane that loaded them: the order of d within a dot
+//                   product is free, so lane group g owns the g-th quarter of d, for Q as well. With the keys above, a lane's
+//                   8 scores are those of keys 8 g .. 8 g + 7: the B operand of
+//   O^T += V^T P^T  V's values go through the wave's own 32 rows of LDS, swizzled, and come back transposed.
 // The next tile's codes and the page numbers of the one after are on their way meanwhile; waves meet only at the end. A
 // workgroup of four waves takes `chunk` consecutive tiles of one request and key head; requests of many tiles are cut into
 // equal chunks, whatever their lengths, and joined by combine_kernel.
@@ -18,36 +22,45 @@
 namespace tattn {
 namespace {
 
+__device__ __forceinline__ f32x4 mfma16(f16x8 a, f16x8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
+__device__ __forceinline__ f32x4 mfma16(bf16x8 a, bf16x8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
+
+constexpr int kRows = 16;  // query heads per workgroup
+
 template <int D>
 struct C4 {
-  static constexpr int W = D / 16;              // words of codes per lane and tensor: half a row
-  static constexpr int NSD = D / 16, DT = (D + 31) / 32;
-  static constexpr int BLOCKS = D >= 64 ? D / 64 : 1;  // blocks of 32 values in half a row (D = 32: half a block)
-  static constexpr int TILE = 32 * Swz<D>::RB;
-  static constexpr int MERGE = 4 * 16 * 64 * 4;  // one 32-row d tile of every wave
-  static constexpr int LDS = 4 * TILE > MERGE ? 4 * TILE : MERGE;
+  static constexpr int W = D / 32;   // words of codes in a quarter row, and matrix instructions over d
+  static constexpr int DT = D / 16;  // 16-row tiles of O^T
+  static constexpr int RB = 2 * D;   // bytes of a row of V in LDS
+  static constexpr int TILE = 32 * RB;
+  // Chunk swizzle of V's rows: the 16 rows that a lane group writes at one chunk, and the 16 rows x 32 bytes of a
+  // transposed read, spread over all banks.
+  static __device__ __forceinline__ int f(int row) {
+    if constexpr (D == 128) return (row & 3) | (((row >> 3) & 3) << 2);
+    else if constexpr (D == 64) return ((row >> 1) & 1) | (((row >> 3) & 3) << 1);
+    else return (row >> 3) & 3;
+  }
+  static __device__ __forceinline__ int addr(int row, int byte) { return row * RB + ((((byte >> 4) ^ f(row)) << 4) | (byte & 15)); }
 };
 
-// One tile's codes of the lane's key and half of d.
+// The lane's quarter rows of its two keys of a tile.
 template <int D>
 struct Codes {
-  uint32_t k[C4<D>::W], v[C4<D>::W];
-  uint32_t ks, vs;  // exponents, a byte per block
-  bool ok;          // the key is visible and its page is one of the cache's
+  uint32_t k[2][C4<D>::W], v[2][C4<D>::W];
+  uint32_t ks[2], vs[2];  // exponents
+  bool ok[2];             // the key is visible and its page is one of the cache's
 };
 
 template <int W>
 __device__ __forceinline__ void load_words(const uint8_t* p, uint32_t (&x)[W]) {
-  if constexpr (W == 2) {
+  if constexpr (W == 4) {
+    const u32x4 a = *reinterpret_cast<const u32x4*>(p);
+    x[0] = a[0], x[1] = a[1], x[2] = a[2], x[3] = a[3];
+  } else if constexpr (W == 2) {
     const u32x2 a = *reinterpret_cast<const u32x2*>(p);
     x[0] = a[0], x[1] = a[1];
   } else {
-#pragma unroll
-    for (int i = 0; i < W; i += 4) {
-      const u32x4 a = *reinterpret_cast<const u32x4*>(p + 4 * i);
-#pragma unroll
-      for (int j = 0; j < 4; ++j) x[i + j] = a[j];
-    }
+    x[0] = *reinterpret_cast<const uint32_t*>(p);
   }
 }
 
@@ -59,23 +72,27 @@ __device__ __forceinline__ typename H16<T>::V8 values8(uint32_t codes, float sca
                                   Fp4<T>::template unpack<2>(codes, scale), Fp4<T>::template unpack<3>(codes, scale)});
 }
 
+// Over the four lanes that hold a column's rows.
+__device__ __forceinline__ float max_groups(float x) { return max_halves(__builtin_fmaxf(x, __shfl_xor(x, 16))); }
+__device__ __forceinline__ float sum_groups(float x) { return sum_halves(x + __shfl_xor(x, 16)); }
+
 template <typename T, int D>
-__global__ __launch_bounds__(256, 2) void cache4_attention_kernel(const Cache4AttnParams p) {
+__global__ __launch_bounds__(256, D == 128 ? 3 : 4) void cache4_attention_kernel(const Cache4AttnParams p) {
   using H = H16<T>;
   using V8 = typename H::V8;
   using V4 = typename H::V4;
   using V2 = typename H::V2;
   using C = C4<D>;
-  __shared__ __attribute__((aligned(1024))) char smem[C::LDS];
-  __shared__ float red[2][4][32];
+  __shared__ __attribute__((aligned(1024))) char smem[4 * C::TILE];
+  __shared__ float red[2][4][kRows];
 
   const int tid = threadIdx.x;
-  const int lane = tid & 63, h2 = lane >> 5, l32 = lane & 31;
+  const int lane = tid & 63, g = lane >> 4, l16 = lane & 15;
   const int w = (int)uniform32((uint32_t)(tid >> 6));
-  const int units = p.R * p.Hk * p.groups;  // requests x key heads x groups of up to 32 query heads
+  const int units = p.R * p.Hk * p.groups;  // requests x key heads x groups of up to 16 query heads
   const int unit = blockIdx.x % units, chunk = blockIdx.x / units;
   const int rg = unit % p.groups, hk = unit / p.groups % p.Hk, r = unit / p.groups / p.Hk;
-  const int row = 32 * rg + l32;  // of the key head's G
+  const int row = kRows * rg + l16;  // of the key head's G
   const bool live = row < p.G;
 
   const int len = min(max(p.lens[r], 0), p.most);
@@ -87,110 +104,130 @@ __global__ __launch_bounds__(256, 2) void cache4_attention_kernel(const Cache4At
   const int64_t prow = (slice * p.splits + chunk) * p.G + row;
   float* ml = p.part + (int64_t)p.R * p.Hk * p.splits * p.G * D + prow * 2;
   if (i0 >= i1 && p.splits > 1) {  // nothing here: an empty part
-    if (w == 0 && h2 == 0 && live) ml[0] = kNoMax, ml[1] = 0.0f;
+    if (w == 0 && g == 0 && live) ml[0] = kNoMax, ml[1] = 0.0f;
     return;
   }
 
-  V8 qop[C::NSD];
+  V8 qop[C::W];
   {
-    const T* src = (const T*)p.q + r * p.sq[0] + (hk * p.G + (live ? row : 0)) * p.sq[1] + h2 * (D / 2);
+    const T* src = (const T*)p.q + r * p.sq[0] + (hk * p.G + (live ? row : 0)) * p.sq[1] + g * (D / 4);
 #pragma unroll
-    for (int s = 0; s < C::NSD; ++s) {
+    for (int s = 0; s < C::W; ++s) {
       const V8 x = *reinterpret_cast<const V8*>(src + 8 * s);
       qop[s] = live ? x : V8{};
     }
   }
-  const float c = p.c;
+  const float c = p.c, hidden = hidden_score(c);
   const int32_t* table = p.tables + r * p.table_stride;
-  const int page = 1 << p.shift;
-  const int in_tile = perm32(l32);  // the lane's key of a tile, so that S^T comes out in the order of P^T's operand
+  const int in_page = (1 << p.shift) - 1;
+  const int key0 = 8 * (l16 >> 2) + (l16 & 3);  // the lane's keys of a tile: key0 and key0 + 4
+  // Byte offsets are (page number) * (bytes of a page) + what follows; a tile starts a page, or lies within one.
+  const uint32_t page_rows = (uint32_t)p.Hk * 2 << p.shift;
+  const uint8_t* codes = p.codes + ((int64_t)hk * 2 << p.shift) * (D / 2) + g * (D / 8);
+  const uint8_t* scales = p.scales + ((int64_t)hk * 2 << p.shift) * (D / 32) + (D == 128 ? g : D == 64 ? g >> 1 : 0);
 
-  // Page of the lane's key in list entry i; -1 where the key is hidden.
-  auto page_of = [&](int i) __attribute__((always_inline)) {
-    const int key = 32 * list.at(min(i, i1 - 1)) + in_tile;
-    const bool see = i < i1 && key <= pos && (key >= list.lo || key < p.sinks);
-    return see ? table[key >> p.shift] : -1;
+  // Pages of the lane's keys in list entry i; -1 where a key is hidden.
+  auto pages_of = [&](int i, int (&pg)[2]) __attribute__((always_inline)) {
+    const int t = list.at(min(i, i1 - 1));
+    const bool inner = i < i1 && 32 * t + 31 <= pos && (32 * t >= list.lo || 32 * t + 31 < p.sinks);
+#pragma unroll
+    for (int a = 0; a < 2; ++a) {
+      const int key = 32 * t + key0 + 4 * a;
+      const bool see = inner || (i < i1 && key <= pos && (key >= list.lo || key < p.sinks));
+      pg[a] = see ? table[key >> p.shift] : -1;
+    }
   };
-  auto load = [&](int i, int pg) __attribute__((always_inline)) {
+  auto load = [&](int i, const int (&pg)[2]) __attribute__((always_inline)) {
     Codes<D> x;
-    const int key = 32 * list.at(min(i, i1 - 1)) + in_tile;
-    x.ok = (uint32_t)pg < (uint32_t)p.pages;
-    const int64_t at = (((int64_t)(x.ok ? pg : 0) * p.Hk + hk) * 2 << p.shift) + (x.ok ? key & (page - 1) : 0);
-    const uint8_t* codes = p.codes + at * (D / 2) + h2 * (D / 4);
-    load_words(codes, x.k);
-    load_words(codes + ((D / 2) << p.shift), x.v);
-    const uint8_t* sc = p.scales + at * (D / 32) + (D >= 64 ? h2 * (D / 64) : 0);
-    const uint8_t* sv = sc + ((D / 32) << p.shift);
-    if constexpr (D == 128) {
-      x.ks = *reinterpret_cast<const uint16_t*>(sc);
-      x.vs = *reinterpret_cast<const uint16_t*>(sv);
-    } else {
-      x.ks = *sc;
-      x.vs = *sv;
+    const int t0 = 32 * list.at(min(i, i1 - 1));
+#pragma unroll
+    for (int a = 0; a < 2; ++a) {
+      x.ok[a] = (uint32_t)pg[a] < (uint32_t)p.pages;
+      const uint64_t at = (uint64_t)(x.ok[a] ? (uint32_t)pg[a] : 0u) * page_rows + (uint32_t)((t0 + key0 + 4 * a) & in_page);
+      const uint8_t* pc = codes + at * (D / 2);
+      const uint8_t* ps = scales + at * (D / 32);
+      load_words(pc, x.k[a]);
+      load_words(pc + ((D / 2) << p.shift), x.v[a]);
+      x.ks[a] = ps[0];
+      x.vs[a] = ps[(D / 32) << p.shift];
     }
     return x;
   };
 
-  TATTN_LDS char* vrows = (TATTN_LDS char*)(smem + w * C::TILE);
+  char* vrows = smem + w * C::TILE;
+  // Transposed reads: lane s of a group at row 8 g + s / 4 (+ 4 for the second read), column 4 (s % 4) of 16.
   int lo[C::DT], hi[C::DT];
 #pragma unroll
-  for (int u = 0; u < C::DT; ++u) tr_addrs<D>(0, u, lane, lo[u], hi[u]);
+  for (int u = 0; u < C::DT; ++u) {
+    lo[u] = C::addr(8 * g + (l16 >> 2), 32 * u + 8 * (l16 & 3));
+    hi[u] = C::addr(8 * g + 4 + (l16 >> 2), 32 * u + 8 * (l16 & 3));
+  }
   float mrow = kNoMax, lrow = 0.0f;
-  f32x16 acc[C::DT];
+  f32x4 acc[C::DT];
 #pragma unroll
-  for (int u = 0; u < C::DT; ++u) acc[u] = f32x16{};
+  for (int u = 0; u < C::DT; ++u) acc[u] = f32x4{};
 
   auto tile = [&](Codes<D>& x) __attribute__((always_inline)) {
-    const uint64_t see = __builtin_amdgcn_ballot_w64(x.ok);  // both halves alike: bit m is row m of S^T
-    if (see == 0) return;
-    const bool masked = see != ~0ull;
-    if (masked && !x.ok) {
-      // What lies at a hidden key's place reaches nothing.
+    const uint64_t see0 = __builtin_amdgcn_ballot_w64(x.ok[0]), see1 = __builtin_amdgcn_ballot_w64(x.ok[1]);
+    if ((see0 | see1) == 0) return;
+    if ((see0 & see1) != ~0ull) {  // what lies at a hidden key's place reaches nothing
 #pragma unroll
-      for (int i = 0; i < C::W; ++i) x.k[i] = x.v[i] = 0;
-      x.ks = x.vs = 0x7f7f;
-    }
-    f32x16 s = f32x16{};
+      for (int a = 0; a < 2; ++a)
+        if (!x.ok[a]) {
 #pragma unroll
-    for (int i = 0; i < C::NSD; ++i) {
-      const float scale = __builtin_bit_cast(float, ((x.ks >> (8 * (i / 4))) & 255) << 23);
-      s = Elt<T>::mfma(values8<T>(x.k[i], scale), qop[i], s);
+          for (int i = 0; i < C::W; ++i) x.k[a][i] = x.v[a][i] = 0;
+          x.ks[a] = x.vs[a] = 127;
+        }
+    }
+    f32x4 s[2];
+#pragma unroll
+    for (int a = 0; a < 2; ++a) {
+      s[a] = f32x4{};
+      const float scale = __builtin_bit_cast(float, x.ks[a] << 23);
+#pragma unroll
+      for (int i = 0; i < C::W; ++i) s[a] = mfma16(values8<T>(x.k[a][i], scale), qop[i], s[a]);
     }
 #pragma unroll
-    for (int i = 0; i < C::W; ++i) {
-      const float scale = __builtin_bit_cast(float, ((x.vs >> (8 * (i / 4))) & 255) << 23);
-      *reinterpret_cast<TATTN_LDS V8*>(vrows + Swz<D>::addr(l32, h2 * D + 16 * i)) = values8<T>(x.v[i], scale);
+    for (int a = 0; a < 2; ++a) {
+      const float scale = __builtin_bit_cast(float, x.vs[a] << 23);
+#pragma unroll
+      for (int i = 0; i < C::W; ++i)
+        *reinterpret_cast<TATTN_LDS V8*>((TATTN_LDS char*)vrows + C::addr(key0 + 4 * a, g * (D / 2) + 16 * i)) = values8<T>(x.v[a][i], scale);
     }
-    // Bit 8 (r / 4) + r % 4 of the half's mask: whether register r's key is visible.
-    const uint32_t bits = (uint32_t)see >> (4 * h2);
-    V8 pr[2];
+    if ((see0 & see1) != ~0ull) {  // row m of tile a is lane m's key a: the lane's scores are rows 4 g + e
+#pragma unroll
+      for (int a = 0; a < 2; ++a) {
+        const uint32_t bits = (uint32_t)(a ? see1 : see0) >> (4 * g);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[a][e] = bits >> e & 1 ? s[a][e] : hidden;
+      }
+    }
+    V8 pr;
     auto probs = [&]() __attribute__((always_inline)) {
       float ps = 0.0f;
 #pragma unroll
-      for (int sg = 0; sg < 2; ++sg)
+      for (int a = 0; a < 2; ++a)
 #pragma unroll
-        for (int i = 0; i < 8; i += 2) {
-          const int a = 8 * sg + i;
-          float e0 = fast_exp2(__builtin_fmaf(s[a], c, -mrow)), e1 = fast_exp2(__builtin_fmaf(s[a + 1], c, -mrow));
-          if (masked) {
-            e0 = bits >> (8 * (a / 4) + a % 4) & 1 ? e0 : 0.0f;
-            e1 = bits >> (8 * ((a + 1) / 4) + (a + 1) % 4) & 1 ? e1 : 0.0f;
-          }
-          const V2 two = H::pack(e0, e1);
+        for (int e = 0; e < 4; e += 2) {
+          const V2 two = H::pack(fast_exp2(__builtin_fmaf(s[a][e], c, -mrow)), fast_exp2(__builtin_fmaf(s[a][e + 1], c, -mrow)));
           ps = H::sum2(two, ps);
-          pr[sg][i] = two[0];
-          pr[sg][i + 1] = two[1];
+          pr[4 * a + e] = two[0];
+          pr[4 * a + e + 1] = two[1];
         }
       return ps;
     };
+    // Probabilities against the running max as it stands; a sum above 2^12 (the first visible tile among them) sends the
+    // wave through the row max and a rescale. One-sided: state first, undone inside.
     const float lprev = lrow;
     const float ps = probs();
     lrow += ps;
     if (__builtin_amdgcn_ballot_w64(!(ps <= 4096.0f))) {
       float mx = kNoMax;
 #pragma unroll
-      for (int a = 0; a < 16; ++a) mx = bits >> (8 * (a / 4) + a % 4) & 1 ? __builtin_fmaxf(mx, s[a] * c) : mx;
-      const float cand = max_halves(mx);
+      for (int a = 0; a < 2; ++a)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) mx = __builtin_fmaxf(mx, s[a][e] * c);
+      const float cand = max_groups(mx);
       const float mnew = cand > mrow + kRescaleLog2 ? cand : mrow;
       const float alpha = fast_exp2(mrow - mnew);
       mrow = mnew;
@@ -200,65 +237,62 @@ __global__ __launch_bounds__(256, 2) void cache4_attention_kernel(const Cache4At
       for (int u = 0; u < C::DT; ++u) acc[u] *= alpha;
     }
 #pragma unroll
-    for (int sg = 0; sg < 2; ++sg)
-#pragma unroll
-      for (int u = 0; u < C::DT; ++u)
-        acc[u] = Elt<T>::mfma(tr_pair<T>((const char*)smem + w * C::TILE + 16 * sg * Swz<D>::RB, lo[u], hi[u]), pr[sg], acc[u]);
+    for (int u = 0; u < C::DT; ++u) acc[u] = mfma16(tr_pair<T>(vrows, lo[u], hi[u]), pr, acc[u]);
   };
 
   int i = i0 + w;
   if (i < i1) {
-    Codes<D> cur = load(i, page_of(i));
-    int pg = page_of(i + 4);
-    for (; i < i1; i += 4) {
-      Codes<D> nxt = load(i + 4, pg);
-      pg = page_of(i + 8);
-      tile(cur);
-      cur = nxt;
+    int pg[2];
+    pages_of(i, pg);
+    Codes<D> x = load(i, pg);
+    pages_of(i + 4, pg);
+    for (; i < i1; i += 8) {
+      Codes<D> y = load(i + 4, pg);
+      pages_of(i + 8, pg);
+      tile(x);
+      if (i + 4 >= i1) break;
+      x = load(i + 8, pg);
+      pages_of(i + 12, pg);
+      tile(y);
     }
   }
 
-  // Join the four waves, one 32-row tile of d at a time; wave w adds four of its columns for every row.
-  const float lt = sum_halves(lrow);
-  if (h2 == 0) {
-    red[0][w][l32] = mrow;
-    red[1][w][l32] = lt;
+  // Join the four waves: register e of tile u is column d = 16 u + 4 g + e of row l16; wave w adds tiles w, w + 4, ...
+  const float lt = sum_groups(lrow);
+  if (g == 0) {
+    red[0][w][l16] = mrow;
+    red[1][w][l16] = lt;
   }
   __syncthreads();
   float mall = kNoMax, lall = 0.0f;
 #pragma unroll
-  for (int k = 0; k < 4; ++k) mall = __builtin_fmaxf(mall, red[0][k][l32]);
+  for (int k = 0; k < 4; ++k) mall = __builtin_fmaxf(mall, red[0][k][l16]);
 #pragma unroll
-  for (int k = 0; k < 4; ++k) lall += fast_exp2(red[0][k][l32] - mall) * red[1][k][l32];
+  for (int k = 0; k < 4; ++k) lall += fast_exp2(red[0][k][l16] - mall) * red[1][k][l16];
   const bool parts = p.splits > 1;
   float wgt = fast_exp2(mrow - mall);
   if (!parts) wgt = lall == 0.0f ? 0.0f : wgt / lall;
+  static_assert(C::DT * 1024 == C::TILE, "a wave's sums fit its rows of V");
+#pragma unroll
+  for (int u = 0; u < C::DT; ++u) *reinterpret_cast<TATTN_LDS f32x4*>((TATTN_LDS char*)vrows + 1024 * u + 16 * lane) = acc[u] * wgt;
+  __syncthreads();
   T* orow = (T*)p.out + r * p.so[0] + (hk * p.G + row) * p.so[1];
-#pragma unroll
-  for (int u = 0; u < C::DT; ++u) {
-    TATTN_LDS float* mine = (TATTN_LDS float*)smem + w * 1024 + lane;
-#pragma unroll
-    for (int a = 0; a < 16; ++a) mine[a * 64] = acc[u][a] * wgt;
-    __syncthreads();
+  for (int u = w; u < C::DT; u += 4) {
     f32x4 x = f32x4{};
 #pragma unroll
-    for (int k = 0; k < 4; ++k)
+    for (int k = 0; k < 4; ++k) x += *reinterpret_cast<const TATTN_LDS f32x4*>((const TATTN_LDS char*)smem + k * C::TILE + 1024 * u + 16 * lane);
+    const int d0 = 16 * u + 4 * g;
+    if (!live) continue;
+    if (parts) {
+      *reinterpret_cast<f32x4*>(p.part + prow * D + d0) = x;
+    } else {
+      V4 y;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) x[e] += ((TATTN_LDS float*)smem + k * 1024 + lane)[(4 * w + e) * 64];
-    const int d0 = 32 * u + 8 * w + 4 * h2;
-    if (live) {
-      if (parts) {
-        *reinterpret_cast<f32x4*>(p.part + prow * D + d0) = x;
-      } else {
-        V4 y;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) y[e] = (T)x[e];
-        *reinterpret_cast<V4*>(orow + d0) = y;
-      }
+      for (int e = 0; e < 4; ++e) y[e] = (T)x[e];
+      *reinterpret_cast<V4*>(orow + d0) = y;
     }
-    __syncthreads();
   }
-  if (parts && w == 0 && h2 == 0 && live) ml[0] = mall, ml[1] = lall;
+  if (parts && w == 0 && g == 0 && live) ml[0] = mall, ml[1] = lall;
 }
 
 template <typename T, int D>
@@ -278,8 +312,8 @@ int run(const Cache4AttnParams& p, hipStream_t st) {
 void cache4_chunks(Cache4AttnParams& p) {
   const int64_t seen = std::min<int64_t>(p.most, (int64_t)p.window + p.sinks + 31);
   const int64_t tiles = std::max<int64_t>(1, (seen + 31) / 32 + 1), units = (int64_t)p.R * p.Hk * p.groups;
-  int64_t chunk = tiles * units / 1024;
-  chunk = std::min<int64_t>(128, std::max<int64_t>(4, (chunk + 3) / 4 * 4));
+  int64_t chunk = tiles * units / 512;
+  chunk = std::min<int64_t>(64, std::max<int64_t>(4, (chunk + 3) / 4 * 4));
   p.chunk = (int32_t)chunk;
   p.splits = (int32_t)((tiles + chunk - 1) / chunk);
 }

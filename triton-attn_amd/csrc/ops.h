@@ -120,7 +120,7 @@ struct Cache4AttnParams {
   int64_t sq[2], so[2];
   int64_t table_stride;
   int32_t R, Hk, G, pages;
-  int32_t groups;  // of 32 query heads of a key head
+  int32_t groups;  // of 16 query heads of a key head
   int32_t shift;   // log2 of the page size
   int32_t most;    // tokens that a table row holds
   int32_t window, sinks;

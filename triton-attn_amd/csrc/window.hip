@@ -349,32 +349,49 @@ __global__ __launch_bounds__(RW * CS * 64, OCC) void window_fwd_kernel(const Win
 }
 
 // ---- rows whose keys were split ------------------------------------------------------------------
-// O = sum_s 2^(m_s - m) O_s / sum_s 2^(m_s - m) l_s, D / 4 lanes per row.
+// O = sum_s 2^(m_s - m) O_s / sum_s 2^(m_s - m) l_s. A workgroup takes one row: D / 4 lanes over the columns, the parts dealt
+// to the 1024 / D groups of them, whose sums are added in order through LDS (a group walking all of 125 parts took 60 us).
 template <typename T, int D>
 __global__ __launch_bounds__(256) void combine_kernel(const float* part, T* out, float* m, int64_t sz, int64_t sh, int64_t sn,
-                                                      int64_t slices, int Hk, int G, int N, int splits) {
+                                                      int Hk, int G, int N, int splits) {
   typedef T V4 __attribute__((ext_vector_type(4)));
-  constexpr int LPR = D / 4;
-  const int rows = N * G;
-  const int64_t r = (int64_t)blockIdx.x * (256 / LPR) + threadIdx.x / LPR;
-  if (r >= slices * rows) return;
-  const int64_t slice = r / rows;
-  const int row = (int)(r % rows), d0 = threadIdx.x % LPR * 4;
+  constexpr int LPR = D / 4, GROUPS = 256 / LPR;
+  __shared__ float red[4];
+  __shared__ __attribute__((aligned(16))) float sums[GROUPS][D];
+  __shared__ float ls[GROUPS];
+  const int tid = threadIdx.x, rows = N * G;
+  const int64_t slice = blockIdx.x / rows, slices = gridDim.x / rows;
+  const int row = (int)(blockIdx.x % rows), d0 = tid % LPR * 4, g = tid / LPR;
   const float* ml = part + slices * splits * rows * D;
   const int64_t first = slice * splits * rows + row;
   float mall = kNoMax;
-  for (int s = 0; s < splits; ++s) mall = __builtin_fmaxf(mall, ml[(first + (int64_t)s * rows) * 2]);
+  for (int s = tid; s < splits; s += 256) mall = __builtin_fmaxf(mall, ml[(first + (int64_t)s * rows) * 2]);
+#pragma unroll
+  for (int i = 1; i < 64; i <<= 1) mall = __builtin_fmaxf(mall, __shfl_xor(mall, i));
+  red[tid >> 6] = mall;
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < 4; ++i) mall = __builtin_fmaxf(mall, red[i]);
   f32x4 x = f32x4{};
   float l = 0.0f;
 #pragma unroll 4
-  for (int s = 0; s < splits; ++s) {
+  for (int s = g; s < splits; s += GROUPS) {
     const int64_t at = first + (int64_t)s * rows;
-    const float w = fast_exp2(ml[at * 2] - mall), ls = ml[at * 2 + 1];
-    if (ls == 0.0f) continue;  // no visible key: the sums of such a part may not be there
-    l = __builtin_fmaf(w, ls, l);
+    const float w = fast_exp2(ml[at * 2] - mall), part_l = ml[at * 2 + 1];
+    if (part_l == 0.0f) continue;  // no visible key: the sums of such a part may not be there
+    l = __builtin_fmaf(w, part_l, l);
     const f32x4 y = *reinterpret_cast<const f32x4*>(part + at * D + d0);
 #pragma unroll
     for (int e = 0; e < 4; ++e) x[e] = __builtin_fmaf(w, y[e], x[e]);
+  }
+  *reinterpret_cast<f32x4*>(&sums[g][d0]) = x;
+  if (d0 == 0) ls[g] = l;
+  __syncthreads();
+  if (g > 0) return;
+  for (int i = 1; i < min(GROUPS, splits); ++i) {
+    l += ls[i];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) x[e] += sums[i][d0 + e];
   }
   const float inv = l == 0.0f ? 0.0f : 1.0f / l;
   const int64_t z = slice / Hk, h = slice % Hk * G + row % G, n = row / G;
@@ -1110,9 +1127,8 @@ template <typename T, int D>
 int combine_d(const float* part, void* out, float* m, const int64_t so[3], int64_t slices, int Hk, int G, int N, int splits,
               hipStream_t st) {
   const int64_t rows = slices * N * G;
-  constexpr int PER = 256 / (D / 4);
-  combine_kernel<T, D><<<dim3((unsigned)((rows + PER - 1) / PER)), dim3(256), 0, st>>>(part, (T*)out, m, so[0], so[1], so[2],
-                                                                                       slices, Hk, G, N, splits);
+  if (rows > 0x7fffffff) return set_error(TATTN_E_ARG, "grid too large: %lld rows", (long long)rows);
+  combine_kernel<T, D><<<dim3((unsigned)rows), dim3(256), 0, st>>>(part, (T*)out, m, so[0], so[1], so[2], Hk, G, N, splits);
   return check_launch("combine");
 }
 
