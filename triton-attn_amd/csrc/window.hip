@@ -843,21 +843,22 @@ __global__ __launch_bounds__(512, OCC) void window_dkdv_pair_kernel(const Window
   }
   // Next tile to fetch. Past the last one its rows come again, into a stage that nobody reads: every step has as many
   // loads in flight.
-  int fg = nq > 0 ? i0 / nq : 0, fq = qt0 + (nq > 0 ? i0 % nq : 0), fi = 1;
+  const int fg0 = nq > 0 ? i0 / nq : 0, fq0 = qt0 + (nq > 0 ? i0 % nq : 0), q_end = qt0 + nq;
+  const char* fbase = base + fg0 * head;  // of the head being fetched
+  const float* fmd = md + (int64_t)fg0 * p.N;
+  int fq = fq0, fi = 1;
   auto fetch = [&](char* st) __attribute__((always_inline)) {
-    const __amdgpu_buffer_rsrc_t rs = slice_rsrc(base + fg * head, bytes);  // rows past the last query read as zero
+    const __amdgpu_buffer_rsrc_t rs = slice_rsrc(fbase, bytes);  // rows past the last query read as zero
+    const uint32_t o = (uint32_t)fq * tile_bytes;
 #pragma unroll
     for (int i = 0; i < PW; ++i)
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (TATTN_LDS void*)(st + (wu * PW + i) * 1024), 16,
-                                               (int)(go[i] + (uint32_t)fq * tile_bytes), 0, 0, 0);
-    if (wu == 0) {
-      const float* src = md + (int64_t)fg * p.N + min(32 * fq + l32, p.N - 1);
-      __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)src,
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (TATTN_LDS void*)(st + (wu * PW + i) * 1024), 16, (int)(go[i] + o), 0, 0, 0);
+    if (wu == 0)
+      __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(fmd + min(32 * fq + l32, p.N - 1)),
                                        (TATTN_LDS void*)(st + 2 * TILE), 4, 0, 0);
-    }
     if (fi < n) {
       ++fi;
-      if (++fq == qt0 + nq) fq = qt0, ++fg;
+      if (++fq == q_end) fq = qt0, fbase += head, fmd += p.N;
     }
   };
   // End of a step: the loads of the step before have landed, this step's may stay in flight; LDS accesses are done.
@@ -879,19 +880,11 @@ __global__ __launch_bounds__(512, OCC) void window_dkdv_pair_kernel(const Window
 #pragma unroll
   for (int u = 0; u < DT; ++u) acc[u] = f32x16{};
 
-  // What the pair does with a query tile: nothing, all of it, or with a mask.
-  struct Look {
-    int qt;
-    bool live, masked;
-  };
-  auto look = [&](int qt, bool in) __attribute__((always_inline)) {
-    const int q0 = off + 32 * qt, q1 = q0 + 31;
-    Look l;
-    l.qt = qt;
-    l.live = in && wk0 < p.S && q1 >= wk0 && (q0 - wk1 < p.window || wk0 < p.sinks);
-    l.masked = q0 < wk1 || (q1 - wk0 >= p.window && wk1 >= p.sinks) || 32 * qt + 32 > p.N;
-    return l;
-  };
+  // Query tiles of which the pair's keys see something, and those that see all of them (or are seen by all).
+  const int far = 0x3fffffff;
+  const int live_lo = wk0 < p.S ? (wk0 - off) >> 5 : far, live_hi = wk0 < p.sinks ? far : (p.window + wk1 - off - 1) >> 5;
+  const int full_lo = (wk1 - off + 31) >> 5;
+  const int full_hi = min((p.N >> 5) - 1, wk1 < p.sinks ? far : (p.window + wk0 - off - 32) >> 5);
 
   auto run = [&](auto role_tag) __attribute__((always_inline)) {
     constexpr bool RB_ = decltype(role_tag)::value;
@@ -944,31 +937,31 @@ __global__ __launch_bounds__(512, OCC) void window_dkdv_pair_kernel(const Window
         o8[4 * (a & 1)] = a0[0], o8[4 * (a & 1) + 1] = a0[1], o8[4 * (a & 1) + 2] = a1[0], o8[4 * (a & 1) + 3] = a1[1];
       }
     };
-    int q = nq > 0 ? qt0 + i0 % nq : 0;
-    Look prev{0, false, false};
+    int q = fq0;
+    bool prev = false;
     auto step = [&](int i, auto tag) __attribute__((always_inline)) {
       constexpr int I = decltype(tag)::value;
       if (i > n) return;
       fetch(stage(IC<I + 2>{}));
-      const Look cur = look(q, i < n);
-      q = q + 1 == qt0 + nq ? qt0 : q + 1;
+      const bool live = i < n && q >= live_lo && q <= live_hi;
       if constexpr (!RB_) {
-        if (cur.live) {
+        if (live) {
           f32x16 s;
           V8 pp[2];
           first(s, stage(IC<I>{}));
-          if (cur.masked) ColMask(off + 32 * cur.qt - key, key, p.N - 32 * cur.qt, h2, p.window, p.sinks).hide(s, hidden);
+          if (q < full_lo || q > full_hi) ColMask(off + 32 * q - key, key, p.N - 32 * q, h2, p.window, p.sinks).hide(s, hidden);
           probs(s, pp, stage(IC<I>{}), (I & 1) ? x1 : x0);
           grad(pp, stage(IC<I>{}));
         }
-      } else if (prev.live) {
+      } else if (prev) {
         f32x16 dp;
         V8 ds[2];
         first(dp, stage(IC<I + 3>{}));
         dsv(dp, ds, (I & 1) ? x0 : x1);
         grad(ds, stage(IC<I + 3>{}));
       }
-      prev = cur;
+      prev = live;
+      if (++q == q_end) q = qt0;
       step_end();
     };
     for (int i = 0; i <= n; i += 4) {  // in step n B finishes the last tile; none follows
