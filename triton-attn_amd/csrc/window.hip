@@ -572,12 +572,11 @@ __global__ __launch_bounds__(RW * CS * 64, OCC) void window_dq_kernel(const Wind
 // the group: the sum over shared heads stays in registers. Key blocks that hold first keys are seen by every later query, an
 // N / window-fold of the others' work: their list is cut into `splits` parts (WindowParams), which write float32 sums that
 // window_first_keys_kernel adds in order.
-template <int RW>
 struct KeyBlocks {
   int sink_blocks, items;  // per slice: sink_blocks * splits parts, then the other blocks
-  __host__ __device__ KeyBlocks(int S, int sinks, int splits) {
-    const int blocks = (S + 32 * RW - 1) / (32 * RW);
-    sink_blocks = splits > 1 ? (sinks + 32 * RW - 1) / (32 * RW) : 0;
+  __host__ __device__ KeyBlocks(int rw, int S, int sinks, int splits) {
+    const int blocks = (S + 32 * rw - 1) / (32 * rw);
+    sink_blocks = splits > 1 ? (sinks + 32 * rw - 1) / (32 * rw) : 0;
     if (sink_blocks > blocks) sink_blocks = blocks;
     items = sink_blocks * splits + blocks - sink_blocks;
   }
@@ -599,7 +598,7 @@ __global__ __launch_bounds__(RW * CS * 64, OCC) void window_dkdv_kernel(const Wi
   const int wu = (int)uniform32((uint32_t)(tid >> 6));
   const int rw = wu / CS, cs = wu % CS;
   const float c = p.c;
-  const KeyBlocks<RW> kbs(p.S, p.sinks, p.splits);
+  const KeyBlocks kbs(RW, p.S, p.sinks, p.splits);
   int slice, kb, split = 0;
   if (!window_coord(p.Z * p.Hk, kbs.items, p.runs, slice, kb)) return;
   const bool parted = kb < kbs.sink_blocks * p.splits;
@@ -770,35 +769,35 @@ __global__ __launch_bounds__(RW * CS * 64, OCC) void window_dkdv_kernel(const Wi
 }
 
 // dK / dV at head dims 64 and 128: two waves per 32-key tile. Over each 32-query tile wave j (role A) computes S = Q K^T,
-// P = 2^(S c - M), dV += P^T dO, and wave j + 4 (role B) dP - delta = dO V^T - delta, dS = P (dP - delta), dK += dS^T Q,
+// P = 2^(S c - M), dV += P^T dO, and wave j + RW (role B) dP - delta = dO V^T - delta, dS = P (dP - delta), dK += dS^T Q,
 // taking P from A through LDS in float32. Each keeps one of K / V and one accumulator set: half the registers of a wave that
 // does both, so that two (head dim 128) or four waves (64) share a SIMD; as many matrix instructions in either role.
-// Step i, one barrier each: A takes tile i, B tile i - 1, and tiles i + 1 and i + 2 are on their way. Nothing is
+// Step i, one barrier each: A takes tile i, B tile i - 1, and tile i + 1 (with four stages i + 2 too) is on its way. Nothing is
 // pipelined inside a wave: the waves of a SIMD overlap each other's matrix and vector work.
-template <typename T, int D, int OCC>
-__global__ __launch_bounds__(512, OCC) void window_dkdv_pair_kernel(const WindowParams p) {
+template <typename T, int D, int RW, int NST, int OCC>
+__global__ __launch_bounds__(RW * 128, OCC) void window_dkdv_pair_kernel(const WindowParams p) {
   using H = H16<T>;
   using V8 = typename H::V8;
   using V2 = typename H::V2;
-  constexpr int RW = 4, NW = 8, NSD = D / 16, DT = D / 32, RB = Swz<D>::RB, TILE = 32 * RB;
+  constexpr int NW = 2 * RW, NSD = D / 16, DT = D / 32, RB = Swz<D>::RB, TILE = 32 * RB;
   constexpr int PW = 2 * TILE / 1024 / NW;          // 1 KB pieces per wave and step
   constexpr int STAGE = 2 * TILE + 256;             // Q, dO, M[32], -delta[32]
   constexpr int XB = 32 * 32 * 4;                   // P of a pair
   // Arrays of their own: a DMA into one does not alias reads of the others.
-  __shared__ __attribute__((aligned(1024))) char st0[STAGE], st1[STAGE], st2[STAGE], st3[STAGE];
-  __shared__ __attribute__((aligned(1024))) char x0[RW * XB], x1[RW * XB];
+  __shared__ __attribute__((aligned(256))) char st0[STAGE], st1[STAGE], st2[STAGE], st3[NST == 4 ? STAGE : 16];
+  __shared__ __attribute__((aligned(256))) char xbuf[2 * RW * XB];
   auto stage = [&](auto tag) __attribute__((always_inline)) -> char* {
-    constexpr int I = decltype(tag)::value & 3;
+    constexpr int I = decltype(tag)::value % NST;
     return I == 0 ? st0 : I == 1 ? st1 : I == 2 ? st2 : st3;
   };
 
   const int tid = threadIdx.x;
   const int lane = tid & 63, h2 = lane >> 5, l32 = lane & 31;
   const int wu = (int)uniform32((uint32_t)(tid >> 6));
-  const int pr = wu & 3;
-  const bool role_b = wu >= 4;
+  const int pr = wu % RW;
+  const bool role_b = wu >= RW;
   const float c = p.c;
-  const KeyBlocks<RW> kbs(p.S, p.sinks, p.splits);
+  const KeyBlocks kbs(RW, p.S, p.sinks, p.splits);
   int slice, kb, split = 0;
   if (!window_coord(p.Z * p.Hk, kbs.items, p.runs, slice, kb)) return;
   const bool parted = kb < kbs.sink_blocks * p.splits;
@@ -838,7 +837,7 @@ __global__ __launch_bounds__(512, OCC) void window_dkdv_pair_kernel(const Window
 #pragma unroll
   for (int i = 0; i < PW; ++i) {
     constexpr int CPR = RB / 16;
-    const int j = 64 * ((wu & 3) * PW + i) + lane, row = j / CPR;
+    const int j = 64 * (pr * PW + i) + lane, row = j / CPR;
     go[i] = (uint32_t)(perm32(row) * rowst * 2 + (((j % CPR) ^ Swz<D>::f(row)) & (D / 8 - 1)) * 16);
   }
   // Next tile to fetch. Past the last one its rows come again, into a stage that nobody reads: every step has as many
@@ -861,9 +860,11 @@ __global__ __launch_bounds__(512, OCC) void window_dkdv_pair_kernel(const Window
       if (++fq == q_end) fq = qt0, fbase += head, fmd += p.N;
     }
   };
-  // End of a step: the loads of the step before have landed, this step's may stay in flight; LDS accesses are done.
+  // End of a step: with four stages the loads of the step before have landed and this step's may stay in flight, with
+  // three all have landed; LDS accesses are done.
   auto step_end = [&]() __attribute__((always_inline)) {
-    if (wu == 0) __builtin_amdgcn_s_waitcnt(0x0070 | (PW + 1));
+    if (NST == 3) __builtin_amdgcn_s_waitcnt(0x0070);
+    else if (wu == 0) __builtin_amdgcn_s_waitcnt(0x0070 | (PW + 1));
     else __builtin_amdgcn_s_waitcnt(0x0070 | PW);
     __atomic_signal_fence(__ATOMIC_SEQ_CST);
     __builtin_amdgcn_s_barrier();
@@ -942,7 +943,10 @@ __global__ __launch_bounds__(512, OCC) void window_dkdv_pair_kernel(const Window
     auto step = [&](int i, auto tag) __attribute__((always_inline)) {
       constexpr int I = decltype(tag)::value;
       if (i > n) return;
-      fetch(stage(IC<I + 2>{}));
+      fetch(stage(IC<I + NST - 2>{}));
+      const int odd = (NST == 4 ? I : i) & 1;
+      char* xc = xbuf + odd * (RW * XB);
+      const char* xp = xbuf + (odd ^ 1) * (RW * XB);
       const bool live = i < n && q >= live_lo && q <= live_hi;
       if constexpr (!RB_) {
         if (live) {
@@ -950,30 +954,30 @@ __global__ __launch_bounds__(512, OCC) void window_dkdv_pair_kernel(const Window
           V8 pp[2];
           first(s, stage(IC<I>{}));
           if (q < full_lo || q > full_hi) ColMask(off + 32 * q - key, key, p.N - 32 * q, h2, p.window, p.sinks).hide(s, hidden);
-          probs(s, pp, stage(IC<I>{}), (I & 1) ? x1 : x0);
+          probs(s, pp, stage(IC<I>{}), xc);
           grad(pp, stage(IC<I>{}));
         }
       } else if (prev) {
         f32x16 dp;
         V8 ds[2];
-        first(dp, stage(IC<I + 3>{}));
-        dsv(dp, ds, (I & 1) ? x0 : x1);
-        grad(ds, stage(IC<I + 3>{}));
+        first(dp, stage(IC<I + NST - 1>{}));
+        dsv(dp, ds, xp);
+        grad(ds, stage(IC<I + NST - 1>{}));
       }
       prev = live;
       if (++q == q_end) q = qt0;
       step_end();
     };
-    for (int i = 0; i <= n; i += 4) {  // in step n B finishes the last tile; none follows
+    for (int i = 0; i <= n; i += NST) {  // in step n B finishes the last tile; none follows
       step(i, IC<0>{});
       step(i + 1, IC<1>{});
       step(i + 2, IC<2>{});
-      step(i + 3, IC<3>{});
+      if constexpr (NST == 4) step(i + 3, IC<3>{});
     }
   };
   if (n > 0) {
     fetch(st0);
-    fetch(st1);
+    if (NST == 4) fetch(st1);
     all_landed_barrier();
     if (role_b) run(std::true_type{});
     else run(std::false_type{});
@@ -994,8 +998,7 @@ __global__ __launch_bounds__(512, OCC) void window_dkdv_pair_kernel(const Window
   }
   T* dst = role_b ? (T*)p.dk + z * p.sdk[0] + hk * p.sdk[1] : (T*)p.dv + z * p.sdv[0] + hk * p.sdv[1];
   const int64_t dst_row = role_b ? p.sdk[2] : p.sdv[2];
-  constexpr int PER = STAGE / TILE;  // whole tiles per stage array: 2
-  static_assert(PER * 4 >= NW, "a block of rows per wave");
+  static_assert(2 * NST >= NW, "a block of rows per wave, two in a stage");
   char* mine = (wu >> 1) == 0 ? st0 : (wu >> 1) == 1 ? st1 : (wu >> 1) == 2 ? st2 : st3;
   mine += (wu & 1) * TILE;
 #pragma unroll
@@ -1017,7 +1020,7 @@ __global__ __launch_bounds__(512, OCC) void window_dkdv_pair_kernel(const Window
 // dK and dV of the key blocks whose queries were cut into parts.
 template <typename T, int D, int RW>
 __global__ __launch_bounds__(256) void window_first_keys_kernel(const WindowParams p) {
-  const KeyBlocks<RW> kbs(p.S, p.sinks, p.splits);
+  const KeyBlocks kbs(RW, p.S, p.sinks, p.splits);
   constexpr int BLOCK = 32 * RW * D;
   const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
   const int64_t per = 2ll * BLOCK;
@@ -1039,7 +1042,11 @@ __global__ __launch_bounds__(256) void window_first_keys_kernel(const WindowPara
 // Row tiles per workgroup, and waves per SIMD of the forward. One key tile per step: its 32 KB of stages at head dim 128 let three
 // workgroups share a CU (two tiles and two workgroups: 1,129 us against 1,048 at 16,384 x 32/8 x 128, window 4,096).
 template <int D> struct WinShape { static constexpr int RW = 4, OCC = D == 128 ? 3 : 4; };
-template <int D> struct KeyShape { static constexpr int RW = D >= 64 ? 4 : 2, CS = 4; };
+// Key tiles per workgroup of dK / dV. At head dim 128 two pairs and three stages let two workgroups share a CU, whose barriers do
+// not wait for each other, and a last round of few workgroups is shorter (four pairs, four stages, one workgroup: 149 us
+// against 125 at 11 x 12/4 x 1,500, window 500); at 64 four pairs have the CU full (two pairs: 269 against 205 us at
+// 4 x 16 x 4,096, window 1,024).
+constexpr int key_tiles(int D) { return D == 64 ? 4 : 2; }
 
 int grid_of(int64_t slices, int64_t per_slice, unsigned* out) {
   const int64_t blocks = slices * per_slice + 8;
@@ -1085,7 +1092,7 @@ int fwd_d(WindowParams p, hipStream_t st) {
 template <typename T, int D>
 int bwd_d(WindowParams p, hipStream_t st) {
   using S = WinShape<D>;
-  using K = KeyShape<D>;
+  constexpr int RW = key_tiles(D);
   const int64_t slices = (int64_t)p.Z * p.Hk, rows = (int64_t)p.N * p.G;
   const int splits = p.splits;
   unsigned blocks;
@@ -1095,15 +1102,15 @@ int bwd_d(WindowParams p, hipStream_t st) {
   if ((rc = grid_of(slices, p.nblk, &blocks))) return rc;
   window_dq_kernel<T, D, S::RW, 1, D >= 64 ? 2 : 4><<<dim3(blocks), dim3(S::RW * 64), 0, st>>>(p);
   if ((rc = check_launch("tattn_window_bwd"))) return rc;
-  const KeyBlocks<K::RW> kbs(p.S, p.sinks, splits);
+  const KeyBlocks kbs(RW, p.S, p.sinks, splits);
   if ((rc = grid_of(slices, kbs.items, &blocks))) return rc;
   if constexpr (D >= 64)
-    window_dkdv_pair_kernel<T, D, D == 64 ? 4 : 2><<<dim3(blocks), dim3(512), 0, st>>>(p);
+    window_dkdv_pair_kernel<T, D, RW, D == 128 ? 3 : 4, D == 128 ? 2 : 4><<<dim3(blocks), dim3(RW * 128), 0, st>>>(p);
   else
-    window_dkdv_kernel<T, D, K::RW, K::CS, D == 32 ? 3 : 4><<<dim3(blocks), dim3(K::RW * K::CS * 64), 0, st>>>(p);
+    window_dkdv_kernel<T, D, RW, 4, D == 32 ? 3 : 4><<<dim3(blocks), dim3(RW * 256), 0, st>>>(p);
   if ((rc = check_launch("tattn_window_bwd")) || !kbs.sink_blocks) return rc;
-  const int64_t n = slices * kbs.sink_blocks * 2 * 32 * K::RW * D;
-  window_first_keys_kernel<T, D, K::RW><<<dim3((unsigned)((n + 255) / 256)), dim3(256), 0, st>>>(p);
+  const int64_t n = slices * kbs.sink_blocks * 2 * 32 * RW * D;
+  window_first_keys_kernel<T, D, RW><<<dim3((unsigned)((n + 255) / 256)), dim3(256), 0, st>>>(p);
   return check_launch("tattn_window_bwd");
 }
 
@@ -1142,7 +1149,7 @@ int window_fwd_splits(const WindowParams& p, int D) {
 // work over four workgroups per CU where that is more.
 int window_bwd_splits(const WindowParams& p, int D) {
   if (p.sinks == 0) return 1;
-  const int64_t rw = D >= 64 ? KeyShape<64>::RW : KeyShape<32>::RW, keys = 32 * rw;
+  const int64_t rw = key_tiles(D), keys = 32 * rw;
   const int64_t all = (int64_t)p.G * ((p.N + 31) / 32);
   const int64_t list = std::min<int64_t>(all, (int64_t)p.G * (std::min<int64_t>(p.window, p.S) / 32 + rw + 1));
   const int64_t share = (int64_t)p.Z * p.Hk * ((p.S + keys - 1) / keys) * list / 1024;
@@ -1153,9 +1160,7 @@ int window_bwd_splits(const WindowParams& p, int D) {
 int64_t window_bwd_part_floats(const WindowParams& p, int D) {
   const int splits = window_bwd_splits(p, D);
   if (splits == 1) return 0;
-  const int64_t rw = D >= 64 ? KeyShape<64>::RW : KeyShape<32>::RW;
-  const int64_t blocks = D >= 64 ? KeyBlocks<KeyShape<64>::RW>(p.S, p.sinks, splits).sink_blocks
-                                 : KeyBlocks<KeyShape<32>::RW>(p.S, p.sinks, splits).sink_blocks;
+  const int64_t rw = key_tiles(D), blocks = KeyBlocks((int)rw, p.S, p.sinks, splits).sink_blocks;
   return (int64_t)p.Z * p.Hk * blocks * splits * 2 * 32 * rw * D;
 }
 
