@@ -220,6 +220,26 @@ def test_lengths_and_garbage_behind_them(z, h, hk, n, s, d, window, sinks, dtype
     assert (clean.transpose(1, 2)[empty] == 0).all()
 
 
+@pytest.mark.parametrize("d", [32, 64, 128])
+def test_garbage_in_keys_that_no_query_sees(d):
+    """The last queries of longer keys: NaN and infinities before the first window (and behind the first keys) change nothing,
+    and their gradients are zeros."""
+    from tattn import window_attention
+
+    q, k, v, do = make(1, 6, 2, 100, 700, d, torch.float16, seed=9)
+    unseen = ~visible(1, 100, 700, 77, 5)[0].any(0)
+    assert 500 < unseen.sum() < 700
+    runs = []
+    for fill in (0.0, math.nan, math.inf):
+        kk, vv = (torch.where(unseen[None, None, :, None], torch.full_like(t, fill), t).requires_grad_() for t in (k, v))
+        qq = q.clone().requires_grad_()
+        o = window_attention(qq, kk, vv, 77, 5)
+        runs.append((o.detach(), *torch.autograd.grad(o, (qq, kk, vv), do)))
+    for a, b, c in zip(*runs):
+        assert torch.equal(a, b) and torch.equal(a, c)
+    assert (runs[1][2][:, :, unseen] == 0).all() and (runs[1][3][:, :, unseen] == 0).all()
+
+
 def test_lens_of_whole_rows_are_the_plain_call():
     from tattn import window_attention
 

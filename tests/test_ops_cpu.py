@@ -175,6 +175,7 @@ def test_qk_norm_rope_has_no_cpu_path():
     (dict(D=48), "head dim"), (dict(dtype=9), "unknown dtype"), (dict(wd=_lib.BF16), "weights must be"), (dict(Hk=0), "heads must be positive"),
     (dict(q=8), "q must be 16-byte aligned"), (dict(cos=None), "cos is a null pointer"), (dict(P=0), "no rows"),
     (dict(ks=(ctypes.c_int64 * 4)(64, 60, 32, 1)), "k stride"), (dict(ko=None), "k_out is a null pointer"),
+    (dict(qos=(ctypes.c_int64 * 4)(1024, 256, 32, 2)), "q_out d stride must be 1"),
     (dict(Z=1 << 20, N=1 << 20), "too many tokens"),
 ])
 def test_norm_rope_entry_point_refuses(bad, msg):
@@ -230,7 +231,7 @@ def test_window_attention_has_no_cpu_path():
     (dict(window=0), "window must be positive"), (dict(sinks=-1), "sinks must not be negative"), (dict(N=0), "positive"),
     (dict(k=None), "k is a null pointer"), (dict(v=8), "v must be 16-byte aligned"),
     (dict(ks=(ctypes.c_int64 * 4)(512, 256, 16, 1)), "k rows overlap"), (dict(ks=(ctypes.c_int64 * 4)(512, 256, 36, 1)), "multiple of"),
-    (dict(ks=(ctypes.c_int64 * 4)(512, 256, 1 << 25, 1)), "2 GiB"), (dict(os=None), "o strides are null"),
+    (dict(ks=(ctypes.c_int64 * 4)(512, 256, 1 << 25, 1)), "2 GiB"), (dict(vs=(ctypes.c_int64 * 4)(512, 256, 32, 0)), "v d stride must be 1"), (dict(os=None), "o strides are null"),
     (dict(Z=1 << 20, H=1 << 20, Hk=1), "too many rows"),
 ])
 def test_window_entry_point_refuses(bad, msg):
@@ -252,6 +253,16 @@ def test_window_workspace_is_asked_for_where_keys_are_split():
     assert lib.tattn_window_workspace(1, 1, 8, 2, 16384, 16384, 64, 128, 4, ctypes.byref(n)) == 0 and n.value > 0
     assert lib.tattn_window_workspace(1, 1, 8, 2, 16384, 16384, 64, 128, 0, ctypes.byref(n)) == 0 and n.value == 0
     assert lib.tattn_window_workspace(1, 1, 8, 2, 16384, 100, 64, 128, 0, ctypes.byref(n)) == 1
+
+
+@pytest.mark.parametrize("z,h,hk", [(1, 1, 1), (1, 8, 2), (64, 8, 8)])
+@pytest.mark.parametrize("n,window,sinks", [(16384, 128, 16384), (16384, 1, 4), (4096, 64, 64), (65536, 1024, 128)])
+def test_window_backward_workspace_stays_small(z, h, hk, n, window, sinks):
+    """Parts of the first keys' sums: about a thousand of 64 or 128 keys, whatever the sizes."""
+    for d in (16, 32, 64, 128):
+        out = ctypes.c_int64(-1)
+        assert _lib.load().tattn_window_workspace(1, z, h, hk, n, n, d, window, sinks, ctypes.byref(out)) == 0
+        assert out.value <= (z * hk * ((min(n, sinks) + 63) // 64) + 2048) * 2 * 128 * d
 
 
 # ---- cache4_attention ----------------------------------------------------------------------------

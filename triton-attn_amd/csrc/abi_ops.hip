@@ -17,9 +17,10 @@ int check_ptr(const char* name, const void* p, int64_t elements, unsigned align)
   return TATTN_OK;
 }
 
-// Strides (in elements) of dimensions before the unit-stride d: whole 16-byte rows.
+// Strides (in elements) of dimensions before the unit-stride d (given as the last of four): whole 16-byte rows.
 int check_rows(const char* name, const int64_t* st, int n, int sz) {
   if (!st) return set_error(TATTN_E_ARG, "%s strides are null", name);
+  if (n == 3 && st[3] != 1) return set_error(TATTN_E_ARG, "%s d stride must be 1, got %lld", name, (long long)st[3]);
   for (int i = 0; i < n; ++i)
     if (st[i] < 0 || (st[i] * sz) % 16 != 0)
       return set_error(TATTN_E_ARG, "%s stride %lld must be a multiple of %d elements", name, (long long)st[i], 16 / sz);
@@ -47,6 +48,7 @@ int cache4_common(Cache4Params& p, const void* codes, const void* scales, const 
   if ((rc = check_page(page_size, &p.shift)) || (rc = check_count("tokens", T)) || (rc = check_count("heads", H)) ||
       (rc = check_count("pages", pages)))
     return rc;
+  if (H > 65536) return set_error(TATTN_E_ARG, "heads out of range: %lld", (long long)H);
   if ((rc = check_ptr("codes", codes, pages * H, 16)) || (rc = check_ptr("scales", scales, pages * H, 4)) ||
       (rc = check_ptr("slots", slots, T, 8)))
     return rc;
@@ -147,7 +149,7 @@ int cache4_attn_common(Cache4AttnParams& p, int64_t R, int64_t H, int64_t Hk, in
   if ((rc = check_page(page_size, &p.shift)) || (rc = check_count("requests", R)) || (rc = check_count("heads", H)) ||
       (rc = check_count("table width", width)))
     return rc;
-  if (Hk < 1 || H < 1 || H % Hk)
+  if (Hk < 1 || H < 1 || H > 65536 || H % Hk)
     return set_error(TATTN_E_ARG, "%lld heads do not share %lld key heads evenly", (long long)H, (long long)Hk);
   if (width * page_size > 0x7fffffff - 4096)
     return set_error(TATTN_E_ARG, "a table row of %lld pages holds 2^31 tokens or more", (long long)width);

@@ -582,6 +582,11 @@ struct KeyBlocks {
   }
 };
 
+// Whether any query sees the key: what lies at another is taken as zero.
+__device__ __forceinline__ bool key_seen(const WindowParams& p, int off, int key) {
+  return key < p.S && (key < p.sinks || off - key < p.window);
+}
+
 template <typename T, int D, int RW, int CS, int OCC>
 __global__ __launch_bounds__(RW * CS * 64, OCC) void window_dkdv_kernel(const WindowParams p) {
   using H = H16<T>;
@@ -643,6 +648,7 @@ __global__ __launch_bounds__(RW * CS * 64, OCC) void window_dkdv_kernel(const Wi
   };
   md[wu][0][lane] = nsteps > 0 ? md_load(0) : 0.0f;
   const int kt = kb * RW + rw, key = 32 * kt + l32;
+  const bool seen = key_seen(p, off, key);
   V8 kop[NSD], vop[NSD];
   {
     const T* ks = (const T*)p.k + z * p.sk[0] + hk * p.sk[1] + (int64_t)(key < p.S ? key : 0) * p.sk[2] + 8 * h2;
@@ -651,8 +657,8 @@ __global__ __launch_bounds__(RW * CS * 64, OCC) void window_dkdv_kernel(const Wi
     for (int s = 0; s < NSD; ++s) {
       const V8 a = *reinterpret_cast<const V8*>(ks + 16 * s);
       const V8 b = *reinterpret_cast<const V8*>(vs + 16 * s);
-      kop[s] = key < p.S ? a : V8{};
-      vop[s] = key < p.S ? b : V8{};
+      kop[s] = seen ? a : V8{};
+      vop[s] = seen ? b : V8{};
     }
   }
   WinOp<D> at;
@@ -816,6 +822,7 @@ __global__ __launch_bounds__(RW * 128, OCC) void window_dkdv_pair_kernel(const W
   const int wk0 = 32 * (kb * RW + pr), wk1 = wk0 + 31, key = wk0 + l32;
 
   // The wave's operand: K rows (A) or V rows (B).
+  const bool seen = key_seen(p, off, key);
   V8 kv[NSD];
   {
     const T* src = role_b ? (const T*)p.v + z * p.sv[0] + hk * p.sv[1] + (int64_t)(key < p.S ? key : 0) * p.sv[2]
@@ -823,7 +830,7 @@ __global__ __launch_bounds__(RW * 128, OCC) void window_dkdv_pair_kernel(const W
 #pragma unroll
     for (int s = 0; s < NSD; ++s) {
       const V8 a = *reinterpret_cast<const V8*>(src + 16 * s + 8 * h2);
-      kv[s] = key < p.S ? a : V8{};
+      kv[s] = seen ? a : V8{};
     }
   }
 
@@ -1146,13 +1153,14 @@ int window_fwd_splits(const WindowParams& p, int D) {
 }
 
 // Parts of the first keys' dK and dV: each about as long as another key block's list, or as an even share of all
-// work over four workgroups per CU where that is more.
+// work over four workgroups per CU where that is more, so that all parts together stay near a thousand.
 int window_bwd_splits(const WindowParams& p, int D) {
   if (p.sinks == 0) return 1;
   const int64_t rw = key_tiles(D), keys = 32 * rw;
   const int64_t all = (int64_t)p.G * ((p.N + 31) / 32);
   const int64_t list = std::min<int64_t>(all, (int64_t)p.G * (std::min<int64_t>(p.window, p.S) / 32 + rw + 1));
-  const int64_t share = (int64_t)p.Z * p.Hk * ((p.S + keys - 1) / keys) * list / 1024;
+  const int64_t blocks = (p.S + keys - 1) / keys, first = std::min<int64_t>(blocks, (p.sinks + keys - 1) / keys);
+  const int64_t share = (int64_t)p.Z * p.Hk * (first * all + (blocks - first) * list) / 1024;
   const int64_t part = std::max<int64_t>(std::max<int64_t>(list, share), 32);
   return (int)std::max<int64_t>(1, std::min<int64_t>((all + part - 1) / part, 256));
 }
