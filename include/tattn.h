@@ -230,14 +230,14 @@ int tattn_norm_rope_bwd(const void* q, const void* k, const void* q_weight, cons
 
 /*
  * Causal attention over a sliding window and the first keys, grouped heads: q, o [Z, H, N, D], k, v [Z, Hk, S, D],
- * H a multiple of Hk (query head h reads key head h / (H / Hk)), TATTN_F16 or TATTN_BF16, D = 16, 32, 64 or 128.
+ * H a multiple of Hk (query head h reads key head h / (H / Hk)), any dtype, D = 16, 32, 64 or 128.
  * The queries are the last N of len_z positions, len_z = lens[z] (clamped to [0, S]) or S where lens is null: query n
  * is at position len_z - N + n and sees key j <= position with position - j < window or j < sinks. Rows that see no
  * key (positions below 0) give zeros; keys that no query of a block sees are not read into any sum. Strides per tensor
  * (z, h, n, d) in elements, unit d stride, 16-byte aligned rows that do not overlap; a head spans less than 2 GiB.
  *
  * m: [Z, H, N] float32 base-2 log-sum-exp for the backward, or null. workspace: float32, 16-byte aligned, as many
- * as tattn_window_workspace gives for the same sizes (may be null where that is 0); calls that may overlap need one each.
+ * as tattn_window_workspace gives for the same sizes (may be null where that is 0, and in TATTN_F32); calls that may overlap need one each.
  * The backward (no lens, S >= N) sums dk and dv over the heads of a group, without atomics; delta: [Z, H, N] scratch.
  */
 int tattn_window_workspace(int backward, int64_t Z, int64_t H, int64_t Hk, int64_t N, int64_t S, int64_t D, int64_t window,

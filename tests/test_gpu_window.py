@@ -3,8 +3,8 @@
 Bounds, element by element, from the roundings the kernels make (u: half a step of the element type, s = 2^-24 of
 float32, f = 2^-25 in float16, where probabilities below its normal range are rounded to steps of 2^-24; 0 in bfloat16).
 A score is a float32 sum of D products: e = (D + 4) s sum |q k| |scale| + 2^-20 relative in its probability (the rest
-is the exponential's own error). Probabilities are rounded once, relative to a maximum of at least 1, and divided by
-the sum of the rounded ones:
+is the exponential's own error). float32 has the same terms with u = s. Probabilities are rounded once, relative to a
+maximum of at least 1, and divided by the sum of the rounded ones:
   dO_row   <= sum_j p_j |v_j| (2u + 2e) + f sum_j |v_j| + u |o|
 The backward's P = 2^(S - M) has that sum's error through M, and is rounded once as dV's operand; dS = P (dP - delta) has P's,
 that of dP (float32) and of delta = dO . O (from the rounded O), and is rounded once:
@@ -121,6 +121,13 @@ TRAIN = [
     (1, 4, 4, 1, 150, 128, 20, 10, torch.bfloat16, "tokens"),
     (1, 9, 3, 77, 400, 32, 150, 0, torch.float16, "tokens"),
     (9, 16, 16, 128, 128, 64, 40, 4, torch.float16, "heads"),
+    (1, 1, 1, 1, 1, 16, 1, 0, torch.float32, "heads"),
+    (2, 3, 1, 45, 45, 16, 9, 2, torch.float32, "tokens"),
+    (1, 6, 2, 200, 200, 32, 31, 0, torch.float32, "tokens"),
+    (2, 4, 4, 257, 257, 64, 100, 4, torch.float32, "heads"),
+    (1, 5, 1, 300, 300, 128, 64, 40, torch.float32, "tokens"),
+    (1, 4, 2, 77, 500, 64, 150, 3, torch.float32, "heads"),
+    (1, 2, 1, 400, 400, 128, 1000, 0, torch.float32, "heads"),
 ]
 
 
@@ -190,6 +197,8 @@ LENS = [
     (1, 16, 2, 1, 9000, 128, 100000, 0, torch.bfloat16, "heads"),
     (1, 64, 1, 2, 700, 32, 200, 70, torch.float16, "heads"),
     (40, 8, 8, 3, 130, 16, 50, 2, torch.bfloat16, "tokens"),
+    (5, 6, 2, 1, 300, 64, 90, 4, torch.float32, "heads"),
+    (7, 4, 1, 2, 150, 128, 1000, 0, torch.float32, "tokens"),
 ]
 
 
@@ -220,13 +229,13 @@ def test_lengths_and_garbage_behind_them(z, h, hk, n, s, d, window, sinks, dtype
     assert (clean.transpose(1, 2)[empty] == 0).all()
 
 
-@pytest.mark.parametrize("d", [32, 64, 128])
-def test_garbage_in_keys_that_no_query_sees(d):
+@pytest.mark.parametrize("d,dtype", [(32, torch.float16), (64, torch.bfloat16), (128, torch.float16), (64, torch.float32)])
+def test_garbage_in_keys_that_no_query_sees(d, dtype):
     """The last queries of longer keys: NaN and infinities before the first window (and behind the first keys) change nothing,
     and their gradients are zeros."""
     from tattn import window_attention
 
-    q, k, v, do = make(1, 6, 2, 100, 700, d, torch.float16, seed=9)
+    q, k, v, do = make(1, 6, 2, 100, 700, d, dtype, seed=9)
     unseen = ~visible(1, 100, 700, 77, 5)[0].any(0)
     assert 500 < unseen.sum() < 700
     runs = []

@@ -209,6 +209,7 @@ def _window(**kw):
     (dict(q=torch.zeros(2, 4, 9, 32).half()), "9 queries for 8 keys"),
     (dict(q=torch.zeros(2, 4, 8, 48).half(), k=torch.zeros(2, 2, 8, 48).half(), v=torch.zeros(2, 2, 8, 48).half()), "head dim"),
     (dict(q=torch.zeros(2, 4, 8, 32)), "dtype"),
+    (dict(q=torch.zeros(2, 4, 8, 32).double(), k=torch.zeros(2, 2, 8, 32).double(), v=torch.zeros(2, 2, 8, 32).double()), "dtype"),
     (dict(window=0), "window must be positive"),
     (dict(sinks=-1), "sinks not negative"),
     (dict(lens=torch.zeros(2, dtype=torch.int64)), "lens must be int32"),
@@ -227,7 +228,7 @@ def test_window_attention_has_no_cpu_path():
 
 
 @pytest.mark.parametrize("bad,msg", [
-    (dict(D=48), "head dim"), (dict(dtype=_lib.F32), "dtype"), (dict(Hk=3), "evenly"), (dict(S=7), "8 queries for 7 keys"),
+    (dict(D=48), "head dim"), (dict(dtype=5), "dtype"), (dict(Hk=3), "evenly"), (dict(S=7), "8 queries for 7 keys"),
     (dict(window=0), "window must be positive"), (dict(sinks=-1), "sinks must not be negative"), (dict(N=0), "positive"),
     (dict(k=None), "k is a null pointer"), (dict(v=8), "v must be 16-byte aligned"),
     (dict(ks=(ctypes.c_int64 * 4)(512, 256, 16, 1)), "k rows overlap"), (dict(ks=(ctypes.c_int64 * 4)(512, 256, 36, 1)), "multiple of"),

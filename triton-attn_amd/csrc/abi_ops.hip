@@ -116,18 +116,20 @@ int window_common(WindowParams& p, int64_t Z, int64_t H, int64_t Hk, int64_t N, 
   p.Z = (int32_t)Z; p.H = (int32_t)H; p.Hk = (int32_t)Hk; p.G = (int32_t)(H / Hk); p.N = (int32_t)N; p.S = (int32_t)S;
   p.window = (int32_t)(window < S ? window : S);
   p.sinks = (int32_t)(sinks < S ? sinks : S);
+  p.runs = window_runs(p);
   return TATTN_OK;
 }
 
 // A tensor that the kernels read in tiles of 32 rows: strides (z, h, n), rows that do not overlap, slices that 31-bit
 // byte offsets span with a step's rows to spare. A dimension of one row gets the stride of whole rows.
-int check_tiles(const char* name, const void* ptr, const int64_t* st, int64_t rows, int64_t D, int64_t (&out)[3]) {
+int check_tiles(const char* name, const void* ptr, const int64_t* st, int64_t rows, int64_t D, int dtype, int64_t (&out)[3]) {
+  const int sz = dtype == TATTN_F32 ? 4 : 2;
   int rc;
-  if ((rc = check_ptr(name, ptr, 1, 16)) || (rc = check_rows(name, st, 3, 2))) return rc;
+  if ((rc = check_ptr(name, ptr, 1, 16)) || (rc = check_rows(name, st, 3, sz))) return rc;
   for (int i = 0; i < 3; ++i) out[i] = st[i];
   if (rows == 1) out[2] = D;
   if (out[2] < D) return set_error(TATTN_E_ARG, "%s rows overlap: stride %lld", name, (long long)out[2]);
-  if (out[2] > (1ll << 24) || (rows + 256) * out[2] * 2 >= 0x7fffff00ll)
+  if (out[2] > (1ll << 24) || (rows + 256) * out[2] * sz >= 0x7fffff00ll)
     return set_error(TATTN_E_ARG, "a head of %s spans 2 GiB or more", name);
   return TATTN_OK;
 }
@@ -135,6 +137,11 @@ int check_tiles(const char* name, const void* ptr, const int64_t* st, int64_t ro
 // Scores to base-2 exponents. A scale of 0 becomes one so small that all exponents are 0 for finite scores below 1e22, because
 // hidden keys are marked by scores whose scaled value is -inf.
 float window_exponent_scale(float sm_scale) { return sm_scale == 0.0f ? 1.0e-30f : sm_scale * kLog2e; }
+
+int check_dtype(int dtype) {
+  if (dtype != TATTN_F16 && dtype != TATTN_F32 && dtype != TATTN_BF16) return set_error(TATTN_E_ARG, "unknown dtype %d", dtype);
+  return TATTN_OK;
+}
 
 int check_16bit(int dtype) {
   if (dtype != TATTN_F16 && dtype != TATTN_BF16)
@@ -294,16 +301,17 @@ int tattn_window_fwd(const void* q, const void* k, const void* v, void* o, float
                      int64_t window, int64_t sinks, int dtype, float sm_scale, void* stream) {
   WindowParams p{};
   int rc;
-  if ((rc = window_common(p, Z, H, Hk, N, S, D, window, sinks, lens != nullptr)) || (rc = check_16bit(dtype)) ||
-      (rc = check_tiles("q", q, q_strides, N, D, p.sq)) || (rc = check_tiles("k", k, k_strides, S, D, p.sk)) ||
-      (rc = check_tiles("v", v, v_strides, S, D, p.sv)) || (rc = check_tiles("o", o, o_strides, N, D, p.sout)) ||
+  if ((rc = window_common(p, Z, H, Hk, N, S, D, window, sinks, lens != nullptr)) || (rc = check_dtype(dtype)) ||
+      (rc = check_tiles("q", q, q_strides, N, D, dtype, p.sq)) || (rc = check_tiles("k", k, k_strides, S, D, dtype, p.sk)) ||
+      (rc = check_tiles("v", v, v_strides, S, D, dtype, p.sv)) || (rc = check_tiles("o", o, o_strides, N, D, dtype, p.sout)) ||
       (rc = check_ptr("m", m, 0, 4)) || (rc = check_ptr("lens", lens, 0, 4)))
     return rc;
-  p.splits = window_fwd_splits(p, (int)D);
+  p.splits = dtype == TATTN_F32 ? 0 : window_fwd_splits(p, (int)D);
   if ((rc = check_ptr("workspace", workspace, p.splits > 1, 16)) || (rc = require_device())) return rc;
   p.q = q; p.k = k; p.v = v; p.out = o; p.m = m; p.lens = lens; p.part = workspace;
   p.c = window_exponent_scale(sm_scale);
   p.scale = sm_scale;
+  if (dtype == TATTN_F32) return launch_window_f32(p, (int)D, false, (hipStream_t)stream);
   return launch_window_fwd(p, (int)D, dtype, (hipStream_t)stream);
 }
 
@@ -315,14 +323,14 @@ int tattn_window_bwd(const void* q, const void* k, const void* v, const void* o,
                      int64_t window, int64_t sinks, int dtype, float sm_scale, void* stream) {
   WindowParams p{};
   int rc;
-  if ((rc = window_common(p, Z, H, Hk, N, S, D, window, sinks, false)) || (rc = check_16bit(dtype)) ||
-      (rc = check_tiles("q", q, q_strides, N, D, p.sq)) || (rc = check_tiles("k", k, k_strides, S, D, p.sk)) ||
-      (rc = check_tiles("v", v, v_strides, S, D, p.sv)) || (rc = check_tiles("o", o, o_strides, N, D, p.so)) ||
-      (rc = check_tiles("do", dout, do_strides, N, D, p.sd)) || (rc = check_tiles("dq", dq, dq_strides, N, D, p.sout)) ||
-      (rc = check_tiles("dk", dk, dk_strides, S, D, p.sdk)) || (rc = check_tiles("dv", dv, dv_strides, S, D, p.sdv)) ||
+  if ((rc = window_common(p, Z, H, Hk, N, S, D, window, sinks, false)) || (rc = check_dtype(dtype)) ||
+      (rc = check_tiles("q", q, q_strides, N, D, dtype, p.sq)) || (rc = check_tiles("k", k, k_strides, S, D, dtype, p.sk)) ||
+      (rc = check_tiles("v", v, v_strides, S, D, dtype, p.sv)) || (rc = check_tiles("o", o, o_strides, N, D, dtype, p.so)) ||
+      (rc = check_tiles("do", dout, do_strides, N, D, dtype, p.sd)) || (rc = check_tiles("dq", dq, dq_strides, N, D, dtype, p.sout)) ||
+      (rc = check_tiles("dk", dk, dk_strides, S, D, dtype, p.sdk)) || (rc = check_tiles("dv", dv, dv_strides, S, D, dtype, p.sdv)) ||
       (rc = check_ptr("m", m, 1, 4)) || (rc = check_ptr("delta", delta, 1, 4)))
     return rc;
-  p.splits = window_bwd_splits(p, (int)D);
+  p.splits = dtype == TATTN_F32 ? 1 : window_bwd_splits(p, (int)D);
   if ((rc = check_ptr("workspace", workspace, p.splits > 1, 16)) || (rc = require_device())) return rc;
   p.q = q; p.k = k; p.v = v; p.o = o; p.dout = dout; p.out = dq; p.dk = dk; p.dv = dv;
   p.m = const_cast<float*>(m);
@@ -330,6 +338,7 @@ int tattn_window_bwd(const void* q, const void* k, const void* v, const void* o,
   p.part = workspace;
   p.c = window_exponent_scale(sm_scale);
   p.scale = sm_scale;
+  if (dtype == TATTN_F32) return launch_window_f32(p, (int)D, true, (hipStream_t)stream);
   return launch_window_bwd(p, (int)D, dtype, (hipStream_t)stream);
 }
 

@@ -102,8 +102,12 @@ inline int64_t window_part_floats(int64_t slices, int64_t rows, int64_t splits, 
 int window_fwd_splits(const WindowParams& p, int D);  // 0: no parts and two row tiles per workgroup
 int window_bwd_splits(const WindowParams& p, int D);
 int64_t window_bwd_part_floats(const WindowParams& p, int D);
-int launch_window_fwd(WindowParams p, int D, int dtype, hipStream_t st);
+// Whether consecutive blocks of a slice share an XCD (window_coord): windows much shorter than the rows make blocks equal;
+// else the later ones are longer, and only whole slices per XCD keep the XCDs level.
+inline int window_runs(const WindowParams& p) { return ((int64_t)p.Z * p.Hk) % 8 == 0 || (int64_t)p.window * 4 <= p.S; }
+int launch_window_fwd(WindowParams p, int D, int dtype, hipStream_t st);  // 16-bit
 int launch_window_bwd(WindowParams p, int D, int dtype, hipStream_t st);
+int launch_window_f32(const WindowParams& p, int D, bool bwd, hipStream_t st);  // no parts, no workspace
 // O of rows whose keys were split: part as laid out above, out [slices / Hk, H, N, D] with strides (z, h, n).
 int launch_combine(const float* part, void* out, float* m, const int64_t so[3], int64_t slices, int Hk, int G, int N,
                    int splits, int D, int dtype, hipStream_t st);

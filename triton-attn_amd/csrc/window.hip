@@ -1062,10 +1062,6 @@ int grid_of(int64_t slices, int64_t per_slice, unsigned* out) {
   return TATTN_OK;
 }
 
-// Whether consecutive blocks of a slice share an XCD: windows much shorter than the rows make blocks equal; else the
-// later ones are longer, and only whole slices per XCD keep the XCDs level.
-int in_runs(const WindowParams& p) { return ((int64_t)p.Z * p.Hk) % 8 == 0 || (int64_t)p.window * 4 <= p.S; }
-
 // Key tiles that a block of 32 rows walks at most.
 int64_t most_tiles(const WindowParams& p) {
   const int64_t seen = std::min<int64_t>(p.S, (int64_t)p.window + 32 / p.G + std::min(p.sinks, p.S));
@@ -1077,7 +1073,6 @@ int fwd_d(WindowParams p, hipStream_t st) {
   const int64_t slices = (int64_t)p.Z * p.Hk, rows = (int64_t)p.N * p.G;
   unsigned blocks;
   int rc;
-  p.runs = in_runs(p);
   if (p.splits > 0) {
     p.nblk = (int)((rows + 31) / 32);
     if ((rc = grid_of(slices, (int64_t)p.nblk * p.splits, &blocks))) return rc;
@@ -1104,7 +1099,6 @@ int bwd_d(WindowParams p, hipStream_t st) {
   const int splits = p.splits;
   unsigned blocks;
   int rc;
-  p.runs = in_runs(p);
   p.nblk = (int)((rows + 32 * S::RW - 1) / (32 * S::RW));
   if ((rc = grid_of(slices, p.nblk, &blocks))) return rc;
   window_dq_kernel<T, D, S::RW, 1, D >= 64 ? 2 : 4><<<dim3(blocks), dim3(S::RW * 64), 0, st>>>(p);

@@ -17,9 +17,7 @@ from torch.autograd.function import once_differentiable
 
 from tattn import _lib
 from tattn._args import aligned, check_index, layout, remember, rows_apart, same_device, strides
-from tattn.api import _on_device, _require_gpu, _stream
-
-_DTYPES = {torch.float16: _lib.F16, torch.bfloat16: _lib.BF16}
+from tattn.api import _DTYPES, _on_device, _require_gpu, _stream
 
 
 def _check(q, k, v, window, sinks, lens) -> None:
@@ -33,7 +31,7 @@ def _check(q, k, v, window, sinks, lens) -> None:
     if hk < 1 or h < 1 or h % hk:
         raise ValueError(f"heads must be a multiple of kv heads, got {h} and {hk}")
     if not (q.dtype == k.dtype == v.dtype) or q.dtype not in _DTYPES:
-        raise ValueError(f"q, k, v must share dtype float16 or bfloat16, got {q.dtype}, {k.dtype}, {v.dtype}")
+        raise ValueError(f"q, k, v must share dtype float16, bfloat16 or float32, got {q.dtype}, {k.dtype}, {v.dtype}")
     if window < 1 or sinks < 0:
         raise ValueError(f"window must be positive and sinks not negative, got {window} and {sinks}")
     same_device(q, k=k, v=v, lens=lens)
@@ -47,7 +45,7 @@ def _tiles_apart(t: torch.Tensor) -> bool:
     """Whether the kernels cannot read t in tiles of rows where it lies: aligned rows that do not overlap, heads within
     31-bit offsets."""
     n, st, d = t.shape[2], t.stride(2), t.shape[3]
-    return rows_apart(t) or (n > 1 and (st < d or st > 1 << 24 or (n + 256) * st * 2 >= 0x7FFFFF00))
+    return rows_apart(t) or (n > 1 and (st < d or st > 1 << 24 or (n + 256) * st * t.element_size() >= 0x7FFFFF00))
 
 
 def _tiles(t: torch.Tensor) -> torch.Tensor:
@@ -75,7 +73,9 @@ def _plan(q, k, v, window, sinks, lens) -> tuple:
     if q.numel() == 0 or s == 0:
         return copies, 0, 0, None
     sizes = (z, h, hk, n, s, d, min(window, s), min(sinks, s))
-    return copies, _workspace(False, sizes), _workspace(True, sizes) if lens is None else 0, (*sizes, _DTYPES[q.dtype])
+    half = q.dtype != torch.float32  # float32 is never split
+    return (copies, _workspace(False, sizes) if half else 0, _workspace(True, sizes) if half and lens is None else 0,
+            (*sizes, _DTYPES[q.dtype]))
 
 
 def _forward(q, k, v, plan, scale, lens, save_lse) -> tuple[torch.Tensor, torch.Tensor | None]:
@@ -135,7 +135,7 @@ def window_attention(
 ) -> torch.Tensor:
     """Causal attention in which a query sees the last `window` keys, its own included, and the first `sinks` keys.
 
-    q [batch, heads, queries, dim]; k, v [batch, kv heads, keys, dim]; float16 or bfloat16; heads a multiple of kv heads,
+    q [batch, heads, queries, dim]; k, v [batch, kv heads, keys, dim]; float16, bfloat16 or float32; heads a multiple of kv heads,
     consecutive heads sharing one; any strides. The queries are the last ones of the keys' positions: query n of a
     sequence with len keys is at position len - queries + n and sees key j <= position with position - j < window or
     j < sinks. len is keys, or lens[batch] (int32, on the GPU, clamped to [0, keys]) where a cache is filled to
