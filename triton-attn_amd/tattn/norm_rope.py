@@ -115,8 +115,9 @@ def qk_norm_rope(
     weights [dim] (the tensors' dtype, or float32), then the position rotation: pairs (i, i + dim / 2), or (2i, 2i + 1)
     when `interleaved`, turned by the angle with cosine cos[position, i] and sine sin[position, i] (float32
     [any, dim / 2]). positions: int32 [seq] or [batch, seq]; None: 0, 1, ... A position outside the tables gives a row of
-    NaN. Outputs keep their input's strides. Differentiable in q, k and both weights; float16, bfloat16 or float32, all
-    arithmetic in float32, each result rounded once. Any batch, head and sequence strides are read in place."""
+    NaN. Outputs keep the order of their input's strides. Differentiable in q, k and both weights (cos and sin get no
+    gradients); float16, bfloat16 or float32, all arithmetic in float32, each result rounded once. Any batch, head and
+    sequence strides are read in place."""
     key = (layout(q), layout(k), layout(q_weight), layout(k_weight), layout(cos), layout(sin), layout(positions), interleaved)
     plan = _plans.get(key)
     if plan is None:

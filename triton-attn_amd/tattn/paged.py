@@ -94,7 +94,8 @@ class Cache4:
     codes: uint8 [pages, kv_heads, 2, page_size, head_dim / 2] (2: keys, values; an even d in the low half of a
     byte), e2m1 codes (sign, two exponent bits, one mantissa bit: 0, 0.5, 1, 1.5, 2, 3, 4, 6). scales: uint8 [pages,
     kv_heads, 2, page_size, head_dim / 32], biased exponents of the blocks of 32 values along the head: the smallest power
-    of two at which the block's largest magnitude rounds to 6 or less (and 6 times which is finite in dtype). A block that held an infinity or a NaN reads as NaN.
+    of two at which the block's largest magnitude rounds to 6 or less (and 6 times which is finite in dtype). A block that
+    held an infinity or a NaN reads as NaN.
     dtype: float16 or bfloat16, the type of the values written and read, and of the queries over them.
     """
 

@@ -135,9 +135,9 @@ def window_attention(
 ) -> torch.Tensor:
     """Causal attention in which a query sees the last `window` keys, its own included, and the first `sinks` keys.
 
-    q [batch, heads, queries, dim]; k, v [batch, kv heads, keys, dim]; float16, bfloat16 or float32; heads a multiple of kv heads,
-    consecutive heads sharing one; any strides. The queries are the last ones of the keys' positions: query n of a
-    sequence with len keys is at position len - queries + n and sees key j <= position with position - j < window or
+    q [batch, heads, queries, dim]; k, v [batch, kv heads, keys, dim]; float16, bfloat16 or float32; heads a multiple of
+    kv heads, consecutive heads sharing one; any strides. The queries are the last ones of the keys' positions: query n of
+    a sequence with len keys is at position len - queries + n and sees key j <= position with position - j < window or
     j < sinks. len is keys, or lens[batch] (int32, on the GPU, clamped to [0, keys]) where a cache is filled to
     different lengths; what lies behind it, or before every window, reaches no result. Rows at positions below 0 give
     zeros. sm_scale defaults to 1 / sqrt(dim). Differentiable in q, k and v without lens; with lens the call is for serving
