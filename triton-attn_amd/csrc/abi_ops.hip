@@ -116,7 +116,6 @@ int window_common(WindowParams& p, int64_t Z, int64_t H, int64_t Hk, int64_t N, 
   p.Z = (int32_t)Z; p.H = (int32_t)H; p.Hk = (int32_t)Hk; p.G = (int32_t)(H / Hk); p.N = (int32_t)N; p.S = (int32_t)S;
   p.window = (int32_t)(window < S ? window : S);
   p.sinks = (int32_t)(sinks < S ? sinks : S);
-  p.runs = window_runs(p);
   return TATTN_OK;
 }
 

@@ -34,7 +34,6 @@ struct TileList {
 // (the entry points replace a scale of 0, where no such score exists, by a tiny one).
 __device__ __forceinline__ float hidden_score(float c) { return c < 0.0f ? __builtin_inff() : -__builtin_inff(); }
 
-
 // What a lane's row at position p hides in a tile of S^T: register r of lane-half h2 is key 32 t + 8 h2 + 16 (r / 8) + r % 8.
 struct RowMask {
   int hi, lb, sk;
@@ -96,16 +95,24 @@ __device__ __forceinline__ void all_landed_barrier() {
   __atomic_signal_fence(__ATOMIC_SEQ_CST);
 }
 
-// Workgroup -> (slice, block); false past the last. Workgroups go round-robin over the 8 XCDs. runs: an XCD takes
-// consecutive blocks, which read overlapping keys through its L2; else consecutive workgroups take consecutive slices.
-__device__ __forceinline__ bool window_coord(int slices, int nblk, bool runs, int& slice, int& blk) {
-  const int64_t total = (int64_t)slices * nblk;
+// Workgroup -> (slice, block); false past the last. Workgroups go round-robin over the 8 XCDs. The first blocks of the slices,
+// all but `tail` of each, are equally long: an XCD takes consecutive ones, which read overlapping rows through its
+// L2. The last `tail` are shorter and shorter: they come after all others, the longer ones first.
+__device__ __forceinline__ bool window_coord(int slices, int nblk, int tail, int& slice, int& blk) {
+  const int even = nblk - tail;
+  const int64_t total = (int64_t)slices * even, chunk = (total + 7) >> 3;
   int64_t i = blockIdx.x;
-  if (runs) i = (i & 7) * ((total + 7) >> 3) + (i >> 3);
-  if (i >= total) return false;
-  if (!runs) i = (i % slices) * nblk + i / slices;
-  slice = (int)(i / nblk);
-  blk = (int)(i % nblk);
+  if (i < 8 * chunk) {
+    i = (i & 7) * chunk + (i >> 3);
+    if (i >= total) return false;
+    slice = (int)(i / even);
+    blk = (int)(i % even);
+    return true;
+  }
+  i -= 8 * chunk;
+  if (i >= (int64_t)slices * tail) return false;
+  slice = (int)(i % slices);
+  blk = even + (int)(i / slices);
   return true;
 }
 

@@ -154,7 +154,7 @@ __global__ __launch_bounds__(RW * CS * 64, OCC) void window_fwd_kernel(const Win
   const int rw = wu / CS, cs = wu % CS;
   const float c = p.c;
   int slice, blk, split = 0;
-  if (!window_coord(p.Z * p.Hk, p.nblk * (SPLIT ? p.splits : 1), p.runs, slice, blk)) return;
+  if (!window_coord(p.Z * p.Hk, p.nblk * (SPLIT ? p.splits : 1), p.tail, slice, blk)) return;
   if (SPLIT) split = blk % p.splits, blk /= p.splits;
   WinRows b;
   b.init(p, slice, p.nblk - 1 - blk, RW);  // longest rows first
@@ -421,7 +421,7 @@ __global__ __launch_bounds__(RW * CS * 64, OCC) void window_dq_kernel(const Wind
   const int rw = wu / CS, cs = wu % CS;
   const float c = p.c;
   int slice, blk;
-  if (!window_coord(p.Z * p.Hk, p.nblk, p.runs, slice, blk)) return;
+  if (!window_coord(p.Z * p.Hk, p.nblk, p.tail, slice, blk)) return;
   WinRows b;
   b.init(p, slice, p.nblk - 1 - blk, RW);
   TileList list;
@@ -605,7 +605,7 @@ __global__ __launch_bounds__(RW * CS * 64, OCC) void window_dkdv_kernel(const Wi
   const float c = p.c;
   const KeyBlocks kbs(RW, p.S, p.sinks, p.splits);
   int slice, kb, split = 0;
-  if (!window_coord(p.Z * p.Hk, kbs.items, p.runs, slice, kb)) return;
+  if (!window_coord(p.Z * p.Hk, kbs.items, p.tail, slice, kb)) return;
   const bool parted = kb < kbs.sink_blocks * p.splits;
   if (parted) split = kb % p.splits, kb /= p.splits;
   else kb = kb - kbs.sink_blocks * p.splits + kbs.sink_blocks;
@@ -805,7 +805,7 @@ __global__ __launch_bounds__(RW * 128, OCC) void window_dkdv_pair_kernel(const W
   const float c = p.c;
   const KeyBlocks kbs(RW, p.S, p.sinks, p.splits);
   int slice, kb, split = 0;
-  if (!window_coord(p.Z * p.Hk, kbs.items, p.runs, slice, kb)) return;
+  if (!window_coord(p.Z * p.Hk, kbs.items, p.tail, slice, kb)) return;
   const bool parted = kb < kbs.sink_blocks * p.splits;
   if (parted) split = kb % p.splits, kb /= p.splits;
   else kb = kb - kbs.sink_blocks * p.splits + kbs.sink_blocks;
@@ -1055,13 +1055,6 @@ template <int D> struct WinShape { static constexpr int RW = 4, OCC = D == 128 ?
 // 4 x 16 x 4,096, window 1,024).
 constexpr int key_tiles(int D) { return D == 64 ? 4 : 2; }
 
-int grid_of(int64_t slices, int64_t per_slice, unsigned* out) {
-  const int64_t blocks = slices * per_slice + 8;
-  if (blocks > 0x7ffffff) return set_error(TATTN_E_ARG, "grid too large: %lld workgroups", (long long)blocks);
-  *out = (unsigned)((slices * per_slice + 7) / 8 * 8);
-  return TATTN_OK;
-}
-
 // Key tiles that a block of 32 rows walks at most.
 int64_t most_tiles(const WindowParams& p) {
   const int64_t seen = std::min<int64_t>(p.S, (int64_t)p.window + 32 / p.G + std::min(p.sinks, p.S));
@@ -1075,7 +1068,8 @@ int fwd_d(WindowParams p, hipStream_t st) {
   int rc;
   if (p.splits > 0) {
     p.nblk = (int)((rows + 31) / 32);
-    if ((rc = grid_of(slices, (int64_t)p.nblk * p.splits, &blocks))) return rc;
+    p.tail = 0;
+    if ((rc = window_grid(slices, (int64_t)p.nblk * p.splits, 0, &blocks))) return rc;
     if (p.splits == 1) {
       window_fwd_kernel<T, D, 1, 4, D == 128 ? 1 : 2, false><<<dim3(blocks), dim3(256), 0, st>>>(p);
       return check_launch("tattn_window_fwd");
@@ -1086,7 +1080,8 @@ int fwd_d(WindowParams p, hipStream_t st) {
   }
   using S = WinShape<D>;
   p.nblk = (int)((rows + 32 * S::RW - 1) / (32 * S::RW));
-  if ((rc = grid_of(slices, p.nblk, &blocks))) return rc;
+  p.tail = window_row_tail(p, 32 * S::RW, p.nblk);
+  if ((rc = window_grid(slices, p.nblk, p.tail, &blocks))) return rc;
   window_fwd_kernel<T, D, S::RW, 1, S::OCC, false><<<dim3(blocks), dim3(S::RW * 64), 0, st>>>(p);
   return check_launch("tattn_window_fwd");
 }
@@ -1100,11 +1095,13 @@ int bwd_d(WindowParams p, hipStream_t st) {
   unsigned blocks;
   int rc;
   p.nblk = (int)((rows + 32 * S::RW - 1) / (32 * S::RW));
-  if ((rc = grid_of(slices, p.nblk, &blocks))) return rc;
+  p.tail = window_row_tail(p, 32 * S::RW, p.nblk);
+  if ((rc = window_grid(slices, p.nblk, p.tail, &blocks))) return rc;
   window_dq_kernel<T, D, S::RW, 1, D >= 64 ? 2 : 4><<<dim3(blocks), dim3(S::RW * 64), 0, st>>>(p);
   if ((rc = check_launch("tattn_window_bwd"))) return rc;
   const KeyBlocks kbs(RW, p.S, p.sinks, splits);
-  if ((rc = grid_of(slices, kbs.items, &blocks))) return rc;
+  p.tail = window_key_tail(p, 32 * RW, kbs.items - kbs.sink_blocks * splits);
+  if ((rc = window_grid(slices, kbs.items, p.tail, &blocks))) return rc;
   if constexpr (D >= 64)
     window_dkdv_pair_kernel<T, D, RW, D == 128 ? 3 : 4, D == 128 ? 2 : 4><<<dim3(blocks), dim3(RW * 128), 0, st>>>(p);
   else

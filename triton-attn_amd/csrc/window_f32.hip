@@ -91,7 +91,7 @@ struct Rows32 {
   WaveTiles sees;
   __device__ __forceinline__ void init(const WindowParams& p, int w, int l32) {
     int blk;
-    ok = window_coord(p.Z * p.Hk, p.nblk, p.runs, slice, blk);
+    ok = window_coord(p.Z * p.Hk, p.nblk, p.tail, slice, blk);
     if (!ok) return;
     blk = p.nblk - 1 - blk;  // longest rows first
     z = slice / p.Hk;
@@ -265,7 +265,7 @@ __global__ __launch_bounds__(256, 1) void window_dkdv_f32_kernel(const WindowPar
   __shared__ __attribute__((aligned(16))) float md[2][32];  // M, -delta
   const int tid = threadIdx.x, lane = tid & 63, h2 = lane >> 5, l32 = lane & 31, w = (int)uniform32(tid >> 6);
   int slice, kb;
-  if (!window_coord(p.Z * p.Hk, p.nblk, p.runs, slice, kb)) return;
+  if (!window_coord(p.Z * p.Hk, p.nblk, p.tail, slice, kb)) return;
   const int z = slice / p.Hk, hk = slice % p.Hk, off = p.S - p.N;
   const int k0 = 128 * kb, k1 = k0 + 127;
   const int nlo = max(0, k0 - off), nhi = k0 < p.sinks ? p.N - 1 : min(p.N - 1, k1 + p.window - 1 - off);
@@ -330,17 +330,12 @@ __global__ __launch_bounds__(256, 1) void window_dkdv_f32_kernel(const WindowPar
     }
 }
 
-int grid_f32(int64_t slices, int64_t per_slice, unsigned* out) {
-  if (slices * per_slice + 8 > 0x7ffffff) return set_error(TATTN_E_ARG, "grid too large: %lld workgroups", (long long)(slices * per_slice));
-  *out = (unsigned)((slices * per_slice + 7) / 8 * 8);
-  return TATTN_OK;
-}
-
 template <int D>
 int fwd_d(WindowParams p, hipStream_t st) {
   unsigned blocks;
   p.nblk = (int)(((int64_t)p.N * p.G + 127) / 128);
-  if (int rc = grid_f32((int64_t)p.Z * p.Hk, p.nblk, &blocks)) return rc;
+  p.tail = window_row_tail(p, 128, p.nblk);
+  if (int rc = window_grid((int64_t)p.Z * p.Hk, p.nblk, p.tail, &blocks)) return rc;
   window_fwd_f32_kernel<D, D == 128 ? 1 : 2><<<dim3(blocks), dim3(256), 0, st>>>(p);
   return check_launch("tattn_window_fwd");
 }
@@ -350,11 +345,13 @@ int bwd_d(WindowParams p, hipStream_t st) {
   unsigned blocks;
   int rc;
   p.nblk = (int)(((int64_t)p.N * p.G + 127) / 128);
-  if ((rc = grid_f32((int64_t)p.Z * p.Hk, p.nblk, &blocks))) return rc;
+  p.tail = window_row_tail(p, 128, p.nblk);
+  if ((rc = window_grid((int64_t)p.Z * p.Hk, p.nblk, p.tail, &blocks))) return rc;
   window_dq_f32_kernel<D, D == 128 ? 1 : 2><<<dim3(blocks), dim3(256), 0, st>>>(p);
   if ((rc = check_launch("tattn_window_bwd"))) return rc;
   p.nblk = (p.S + 127) / 128;
-  if ((rc = grid_f32((int64_t)p.Z * p.Hk, p.nblk, &blocks))) return rc;
+  p.tail = window_key_tail(p, 128, p.nblk);
+  if ((rc = window_grid((int64_t)p.Z * p.Hk, p.nblk, p.tail, &blocks))) return rc;
   window_dkdv_f32_kernel<D><<<dim3(blocks), dim3(256), 0, st>>>(p);
   return check_launch("tattn_window_bwd");
 }
