@@ -92,7 +92,7 @@ struct WindowParams {
   int32_t window, sinks;
   int32_t nblk;
   int32_t splits;  // forward: parts of a row's keys; backward: parts of the first keys' queries
-  int32_t tail;    // blocks of a slice that are placed last (window_coord)
+  int32_t head, tail;  // blocks of a slice that are placed first and last (window_coord)
   float c, scale;
 };
 
@@ -116,9 +116,9 @@ inline int window_row_tail(const WindowParams& p, int rows, int blocks) {
 inline int window_key_tail(const WindowParams& p, int keys, int blocks) {
   return window_tail((std::min<int64_t>(p.window, p.S) + keys - 1) / keys, blocks);
 }
-// Workgroups of a launch over `slices` slices of `blocks` blocks, `tail` of them placed last (window_coord).
-inline int window_grid(int64_t slices, int64_t blocks, int64_t tail, unsigned* out) {
-  const int64_t n = (slices * (blocks - tail) + 7) / 8 * 8 + slices * tail;
+// Workgroups of a launch over `slices` slices of `blocks` blocks, `apart` of them placed first or last (window_coord).
+inline int window_grid(int64_t slices, int64_t blocks, int64_t apart, unsigned* out) {
+  const int64_t n = (slices * (blocks - apart) + 7) / 8 * 8 + slices * apart;
   if (n > 0x7ffffff) return set_error(TATTN_E_ARG, "grid too large: %lld workgroups", (long long)n);
   *out = (unsigned)n;
   return TATTN_OK;

@@ -95,24 +95,29 @@ __device__ __forceinline__ void all_landed_barrier() {
   __atomic_signal_fence(__ATOMIC_SEQ_CST);
 }
 
-// Workgroup -> (slice, block); false past the last. Workgroups go round-robin over the 8 XCDs. The first blocks of the slices,
-// all but `tail` of each, are equally long: an XCD takes consecutive ones, which read overlapping rows through its
-// L2. The last `tail` are shorter and shorter: they come after all others, the longer ones first.
-__device__ __forceinline__ bool window_coord(int slices, int nblk, int tail, int& slice, int& blk) {
-  const int even = nblk - tail;
-  const int64_t total = (int64_t)slices * even, chunk = (total + 7) >> 3;
+// Workgroup -> (slice, block); false past the last. Workgroups go round-robin over the 8 XCDs. The first `head` blocks of the
+// slices come before all others and the last `tail`, which are shorter and shorter, after them, the longer ones first; those
+// between are equally long: an XCD takes consecutive ones, which read overlapping rows through its L2.
+__device__ __forceinline__ bool window_coord(int slices, int nblk, int head, int tail, int& slice, int& blk) {
+  const int even = nblk - head - tail;
+  const int64_t ahead = (int64_t)slices * head, total = (int64_t)slices * even, chunk = (total + 7) >> 3;
   int64_t i = blockIdx.x;
-  if (i < 8 * chunk) {
-    i = (i & 7) * chunk + (i >> 3);
-    if (i >= total) return false;
-    slice = (int)(i / even);
-    blk = (int)(i % even);
-    return true;
+  blk = 0;
+  if (i >= ahead) {
+    i -= ahead;
+    if (i < 8 * chunk) {
+      i = (i & 7) * chunk + (i >> 3);
+      if (i >= total) return false;
+      slice = (int)(i / even);
+      blk = head + (int)(i % even);
+      return true;
+    }
+    i -= 8 * chunk;
+    if (i >= (int64_t)slices * tail) return false;
+    blk = nblk - tail;
   }
-  i -= 8 * chunk;
-  if (i >= (int64_t)slices * tail) return false;
   slice = (int)(i % slices);
-  blk = even + (int)(i / slices);
+  blk += (int)(i / slices);
   return true;
 }
 

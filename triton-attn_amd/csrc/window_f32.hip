@@ -91,7 +91,7 @@ struct Rows32 {
   WaveTiles sees;
   __device__ __forceinline__ void init(const WindowParams& p, int w, int l32) {
     int blk;
-    ok = window_coord(p.Z * p.Hk, p.nblk, p.tail, slice, blk);
+    ok = window_coord(p.Z * p.Hk, p.nblk, p.head, p.tail, slice, blk);
     if (!ok) return;
     blk = p.nblk - 1 - blk;  // longest rows first
     z = slice / p.Hk;
@@ -265,7 +265,7 @@ __global__ __launch_bounds__(256, 1) void window_dkdv_f32_kernel(const WindowPar
   __shared__ __attribute__((aligned(16))) float md[2][32];  // M, -delta
   const int tid = threadIdx.x, lane = tid & 63, h2 = lane >> 5, l32 = lane & 31, w = (int)uniform32(tid >> 6);
   int slice, kb;
-  if (!window_coord(p.Z * p.Hk, p.nblk, p.tail, slice, kb)) return;
+  if (!window_coord(p.Z * p.Hk, p.nblk, p.head, p.tail, slice, kb)) return;
   const int z = slice / p.Hk, hk = slice % p.Hk, off = p.S - p.N;
   const int k0 = 128 * kb, k1 = k0 + 127;
   const int nlo = max(0, k0 - off), nhi = k0 < p.sinks ? p.N - 1 : min(p.N - 1, k1 + p.window - 1 - off);
