@@ -121,6 +121,11 @@ TRAIN = [
     (1, 4, 4, 1, 150, 128, 20, 10, torch.bfloat16, "tokens"),
     (1, 9, 3, 77, 400, 32, 150, 0, torch.float16, "tokens"),
     (9, 16, 16, 128, 128, 64, 40, 4, torch.float16, "heads"),
+    (1, 8, 1, 700, 700, 64, 300, 0, torch.float16, "tokens"),     # few key blocks, long lists: in parts
+    (1, 8, 1, 900, 900, 128, 5000, 0, torch.bfloat16, "heads"),
+    (1, 16, 1, 500, 500, 32, 200, 70, torch.float16, "heads"),
+    (1, 12, 1, 300, 900, 128, 400, 3, torch.bfloat16, "tokens"),
+    (1, 32, 1, 100, 100, 16, 100, 0, torch.float16, "tokens"),
     (1, 1, 1, 1, 1, 16, 1, 0, torch.float32, "heads"),
     (2, 3, 1, 45, 45, 16, 9, 2, torch.float32, "tokens"),
     (1, 6, 2, 200, 200, 32, 31, 0, torch.float32, "tokens"),

@@ -252,7 +252,8 @@ def test_window_workspace_is_asked_for_where_keys_are_split():
     assert lib.tattn_window_fwd(16, 16, 16, 16, None, None, None, st, st, st, st, 1, 8, 2, 1, 8192, 64, 8192, 0, _lib.F16, 0.1, None) == 1
     assert "workspace is a null pointer" in _lib.last_error()
     assert lib.tattn_window_workspace(1, 1, 8, 2, 16384, 16384, 64, 128, 4, ctypes.byref(n)) == 0 and n.value > 0
-    assert lib.tattn_window_workspace(1, 1, 8, 2, 16384, 16384, 64, 128, 0, ctypes.byref(n)) == 0 and n.value == 0
+    assert lib.tattn_window_workspace(1, 8, 8, 2, 16384, 16384, 64, 128, 0, ctypes.byref(n)) == 0 and n.value == 0
+    assert lib.tattn_window_workspace(1, 1, 8, 1, 8192, 8192, 128, 1024, 0, ctypes.byref(n)) == 0 and n.value > 0  # few key blocks
     assert lib.tattn_window_workspace(1, 1, 8, 2, 16384, 100, 64, 128, 0, ctypes.byref(n)) == 1
 
 

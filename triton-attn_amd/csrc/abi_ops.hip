@@ -286,6 +286,7 @@ int tattn_window_workspace(int backward, int64_t Z, int64_t H, int64_t Hk, int64
   if (!floats) return set_error(TATTN_E_ARG, "floats is a null pointer");
   if ((rc = window_common(p, Z, H, Hk, N, S, D, window, sinks, !backward))) return rc;
   if (backward) {
+    window_bwd_parts(p, (int)D);
     *floats = window_bwd_part_floats(p, (int)D);
   } else {
     const int splits = window_fwd_splits(p, (int)D);
@@ -329,8 +330,9 @@ int tattn_window_bwd(const void* q, const void* k, const void* v, const void* o,
       (rc = check_tiles("dk", dk, dk_strides, S, D, dtype, p.sdk)) || (rc = check_tiles("dv", dv, dv_strides, S, D, dtype, p.sdv)) ||
       (rc = check_ptr("m", m, 1, 4)) || (rc = check_ptr("delta", delta, 1, 4)))
     return rc;
-  p.splits = dtype == TATTN_F32 ? 1 : window_bwd_splits(p, (int)D);
-  if ((rc = check_ptr("workspace", workspace, p.splits > 1, 16)) || (rc = require_device())) return rc;
+  p.splits = p.parts = 1;
+  if (dtype != TATTN_F32) window_bwd_parts(p, (int)D);
+  if ((rc = check_ptr("workspace", workspace, p.splits > 1 || p.parts > 1, 16)) || (rc = require_device())) return rc;
   p.q = q; p.k = k; p.v = v; p.o = o; p.dout = dout; p.out = dq; p.dk = dk; p.dv = dv;
   p.m = const_cast<float*>(m);
   p.delta = delta;

@@ -92,6 +92,7 @@ struct WindowParams {
   int32_t window, sinks;
   int32_t nblk;
   int32_t splits;  // forward: parts of a row's keys; backward: parts of the first keys' queries
+  int32_t parts;   // backward: parts of the other keys' queries
   int32_t head, tail;  // blocks of a slice that are placed first and last (window_coord)
   float c, scale;
 };
@@ -101,7 +102,7 @@ inline int64_t window_part_floats(int64_t slices, int64_t rows, int64_t splits, 
   return slices * rows * splits * (D + 2);
 }
 int window_fwd_splits(const WindowParams& p, int D);  // 0: no parts and two row tiles per workgroup
-int window_bwd_splits(const WindowParams& p, int D);
+void window_bwd_parts(WindowParams& p, int D);  // sets splits and parts
 int64_t window_bwd_part_floats(const WindowParams& p, int D);
 // How many of a slice's `blocks` row blocks (of `rows` rows with their heads) or key blocks (of `keys` keys) are placed last
 // (window_coord): those that the ends of the sequence make shorter, queries before a whole window and keys that fewer than a

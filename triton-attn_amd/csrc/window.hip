@@ -579,16 +579,29 @@ __global__ __launch_bounds__(RW * CS * 64, OCC) void window_dq_kernel(const Wind
 // ---- dK / dV -------------------------------------------------------------------------------------
 // A workgroup owns RW tiles of 32 keys and walks the query tiles that see any of them, head after head of
 // the group: the sum over shared heads stays in registers. Key blocks that hold first keys are seen by every later query, an
-// N / window-fold of the others' work: their list is cut into `splits` parts (WindowParams), which write float32 sums that
-// window_first_keys_kernel adds in order.
+// N / window-fold of the others' work: their list is cut into `splits` parts. Where all blocks of all slices would fill the
+// chip only in part, the others' lists are cut into `parts`. Parts write float32 sums that window_parts_kernel adds in order.
 struct KeyBlocks {
-  int sink_blocks, items;  // per slice: sink_blocks * splits parts, then the other blocks
-  __host__ __device__ KeyBlocks(int rw, int S, int sinks, int splits) {
-    const int blocks = (S + 32 * rw - 1) / (32 * rw);
-    sink_blocks = splits > 1 ? (sinks + 32 * rw - 1) / (32 * rw) : 0;
+  int sink_blocks, splits, parts;
+  int blocks, items;  // per slice: sink_blocks * splits parts, then the other blocks' parts
+  __host__ __device__ explicit KeyBlocks(int rw, const WindowParams& p) : splits(p.splits), parts(p.parts) {
+    blocks = (p.S + 32 * rw - 1) / (32 * rw);
+    sink_blocks = splits > 1 ? (p.sinks + 32 * rw - 1) / (32 * rw) : 0;
     if (sink_blocks > blocks) sink_blocks = blocks;
-    items = sink_blocks * splits + blocks - sink_blocks;
+    items = sink_blocks * splits + (blocks - sink_blocks) * parts;
   }
+  // Key block, part and number of parts of an item.
+  __device__ __forceinline__ void block(int item, int& kb, int& part, int& of) const {
+    const int rest = item - sink_blocks * splits;
+    of = rest < 0 ? splits : parts;
+    const int i = rest < 0 ? item : rest;
+    kb = i / of + (rest < 0 ? 0 : sink_blocks);
+    part = i % of;
+  }
+  __host__ __device__ int first(int kb) const {  // item of its first part
+    return kb < sink_blocks ? kb * splits : sink_blocks * splits + (kb - sink_blocks) * parts;
+  }
+  __host__ __device__ int parted() const { return parts > 1 ? blocks : sink_blocks; }  // blocks in parts, the first ones
 };
 
 // Whether any query sees the key: what lies at another is taken as zero.
@@ -612,12 +625,11 @@ __global__ __launch_bounds__(RW * CS * 64, OCC) void window_dkdv_kernel(const Wi
   const int wu = (int)uniform32((uint32_t)(tid >> 6));
   const int rw = wu / CS, cs = wu % CS;
   const float c = p.c;
-  const KeyBlocks kbs(RW, p.S, p.sinks, p.splits);
-  int slice, kb, split = 0;
-  if (!window_coord(p.Z * p.Hk, kbs.items, p.head, p.tail, slice, kb)) return;
-  const bool parted = kb < kbs.sink_blocks * p.splits;
-  if (parted) split = kb % p.splits, kb /= p.splits;
-  else kb = kb - kbs.sink_blocks * p.splits + kbs.sink_blocks;
+  const KeyBlocks kbs(RW, p);
+  int slice, item, kb, split, splits;
+  if (!window_coord(p.Z * p.Hk, kbs.items, p.head, p.tail, slice, item)) return;
+  kbs.block(item, kb, split, splits);
+  const bool parted = splits > 1;
   const int z = slice / p.Hk, hk = slice % p.Hk, off = p.S - p.N;
   const int k0 = 32 * RW * kb, k1 = k0 + 32 * RW - 1;
   // Queries that see a key of the block, as tiles of 32 of each head in turn.
@@ -625,8 +637,7 @@ __global__ __launch_bounds__(RW * CS * 64, OCC) void window_dkdv_kernel(const Wi
   const int nhi = k0 < p.sinks ? p.N - 1 : min(p.N - 1, k1 + p.window - 1 - off);
   const int qt0 = nlo >> 5, nq = nhi < nlo ? 0 : (nhi >> 5) - qt0 + 1;
   const int total = nq * p.G;
-  const int i0 = parted ? (int)((int64_t)total * split / p.splits) : 0;
-  const int i1 = parted ? (int)((int64_t)total * (split + 1) / p.splits) : total;
+  const int i0 = (int)((int64_t)total * split / splits), i1 = (int)((int64_t)total * (split + 1) / splits);
   const int nsteps = (i1 - i0 + CS - 1) / CS;
 
   WinLoader<D, NW, CS> ld;
@@ -752,8 +763,8 @@ __global__ __launch_bounds__(RW * CS * 64, OCC) void window_dkdv_kernel(const Wi
   constexpr int PER = R::STAGE / PART;
   static_assert(2 * PER >= RW * (CS - 1), "partials fit the stages");
   auto part = [&](int k) { return (TATTN_LDS float*)(k < PER ? s0 + k * PART : s1 + (k - PER) * PART); };
-  // A part's sums: [slice][sink block][split][dK, dV][32 RW keys][D] float32.
-  float* fdst = p.part + (((int64_t)slice * kbs.sink_blocks + kb) * p.splits + split) * (2 * 32 * RW * D);
+  // A part's sums: [slice][item][dK, dV][32 RW keys][D] float32.
+  float* fdst = p.part + ((int64_t)slice * kbs.first(kbs.parted()) + item) * (2 * 32 * RW * D);
   auto reduce = [&](const f32x16 (&a)[DT], float mul, T* dst, int64_t stride, float* fpart) __attribute__((always_inline)) {
     if (cs > 0) {
       TATTN_LDS float* mine = part(rw * (CS - 1) + cs - 1) + lane;
@@ -812,12 +823,11 @@ __global__ __launch_bounds__(RW * 128, OCC) void window_dkdv_pair_kernel(const W
   const int pr = wu % RW;
   const bool role_b = wu >= RW;
   const float c = p.c;
-  const KeyBlocks kbs(RW, p.S, p.sinks, p.splits);
-  int slice, kb, split = 0;
-  if (!window_coord(p.Z * p.Hk, kbs.items, p.head, p.tail, slice, kb)) return;
-  const bool parted = kb < kbs.sink_blocks * p.splits;
-  if (parted) split = kb % p.splits, kb /= p.splits;
-  else kb = kb - kbs.sink_blocks * p.splits + kbs.sink_blocks;
+  const KeyBlocks kbs(RW, p);
+  int slice, item, kb, split, splits;
+  if (!window_coord(p.Z * p.Hk, kbs.items, p.head, p.tail, slice, item)) return;
+  kbs.block(item, kb, split, splits);
+  const bool parted = splits > 1;
   const int z = slice / p.Hk, hk = slice % p.Hk, off = p.S - p.N;
   const int k0 = 32 * RW * kb, k1 = k0 + 32 * RW - 1;
   // Queries that see a key of the block, as tiles of 32 of each head in turn.
@@ -825,8 +835,7 @@ __global__ __launch_bounds__(RW * 128, OCC) void window_dkdv_pair_kernel(const W
   const int nhi = k0 < p.sinks ? p.N - 1 : min(p.N - 1, k1 + p.window - 1 - off);
   const int qt0 = nlo >> 5, nq = nhi < nlo ? 0 : (nhi >> 5) - qt0 + 1;
   const int total = nq * p.G;
-  const int i0 = parted ? (int)((int64_t)total * split / p.splits) : 0;
-  const int i1 = parted ? (int)((int64_t)total * (split + 1) / p.splits) : total;
+  const int i0 = (int)((int64_t)total * split / splits), i1 = (int)((int64_t)total * (split + 1) / splits);
   const int n = i1 - i0;
   const int wk0 = 32 * (kb * RW + pr), wk1 = wk0 + 31, key = wk0 + l32;
 
@@ -1004,7 +1013,7 @@ __global__ __launch_bounds__(RW * 128, OCC) void window_dkdv_pair_kernel(const W
   // the tile, column 32 u + l32. A part's sums go out in float32; otherwise the tile is turned into rows through LDS.
   const float mul = role_b ? p.scale : 1.0f;
   if (parted) {
-    float* dst = p.part + (((int64_t)slice * kbs.sink_blocks + kb) * p.splits + split) * (2 * 32 * RW * D) +
+    float* dst = p.part + ((int64_t)slice * kbs.first(kbs.parted()) + item) * (2 * 32 * RW * D) +
                  (role_b ? 0 : 32 * RW * D) + (int64_t)32 * pr * D;
 #pragma unroll
     for (int u = 0; u < DT; ++u)
@@ -1033,25 +1042,32 @@ __global__ __launch_bounds__(RW * 128, OCC) void window_dkdv_pair_kernel(const W
   }
 }
 
-// dK and dV of the key blocks whose queries were cut into parts.
+// dK and dV of the key blocks whose queries were cut into parts: four consecutive columns a thread.
 template <typename T, int D, int RW>
-__global__ __launch_bounds__(256) void window_first_keys_kernel(const WindowParams p) {
-  const KeyBlocks kbs(RW, p.S, p.sinks, p.splits);
+__global__ __launch_bounds__(256) void window_parts_kernel(const WindowParams p) {
+  typedef T V4 __attribute__((ext_vector_type(4)));
+  const KeyBlocks kbs(RW, p);
+  const int blocks = kbs.parted();
   constexpr int BLOCK = 32 * RW * D;
-  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  const int64_t per = 2ll * BLOCK;
-  if (i >= (int64_t)p.Z * p.Hk * kbs.sink_blocks * per) return;
+  const int64_t per = 2ll * BLOCK, i = 4 * ((int64_t)blockIdx.x * 256 + threadIdx.x);
+  if (i >= (int64_t)p.Z * p.Hk * blocks * per) return;
   const int64_t block = i / per;
   const int e = (int)(i % per), which = e / BLOCK, in = e % BLOCK / D, d = e % D;
-  const int slice = (int)(block / kbs.sink_blocks), kb = (int)(block % kbs.sink_blocks);
+  const int slice = (int)(block / blocks), kb = (int)(block % blocks);
   const int key = 32 * RW * kb + in;
   if (key >= p.S) return;
-  float x = 0.0f;
+  const int first = kbs.first(kb), n = kbs.first(kb + 1) - first;
+  const float* src = p.part + ((int64_t)slice * kbs.first(blocks) + first) * per + e;
+  f32x4 x = f32x4{};
 #pragma unroll 4
-  for (int s = 0; s < p.splits; ++s) x += p.part[(block * p.splits + s) * per + e];
+  for (int s = 0; s < n; ++s) x += *reinterpret_cast<const f32x4*>(src + s * per);
   const int z = slice / p.Hk, hk = slice % p.Hk;
-  if (which) ((T*)p.dv)[z * p.sdv[0] + hk * p.sdv[1] + (int64_t)key * p.sdv[2] + d] = (T)x;
-  else ((T*)p.dk)[z * p.sdk[0] + hk * p.sdk[1] + (int64_t)key * p.sdk[2] + d] = (T)(x * p.scale);
+  T* dst = which ? (T*)p.dv + z * p.sdv[0] + hk * p.sdv[1] + (int64_t)key * p.sdv[2] + d
+                 : (T*)p.dk + z * p.sdk[0] + hk * p.sdk[1] + (int64_t)key * p.sdk[2] + d;
+  V4 y;
+#pragma unroll
+  for (int k = 0; k < 4; ++k) y[k] = (T)(x[k] * (which ? 1.0f : p.scale));
+  *reinterpret_cast<V4*>(dst) = y;
 }
 
 // ---- launch ----------------------------------------------------------------------------------------
@@ -1100,7 +1116,6 @@ int bwd_d(WindowParams p, hipStream_t st) {
   using S = WinShape<D>;
   constexpr int RW = key_tiles(D);
   const int64_t slices = (int64_t)p.Z * p.Hk, rows = (int64_t)p.N * p.G;
-  const int splits = p.splits;
   unsigned blocks;
   int rc;
   p.nblk = (int)((rows + 32 * S::RW - 1) / (32 * S::RW));
@@ -1108,17 +1123,17 @@ int bwd_d(WindowParams p, hipStream_t st) {
   if ((rc = window_grid(slices, p.nblk, p.tail, &blocks))) return rc;
   window_dq_kernel<T, D, S::RW, 1, D >= 64 ? 2 : 4><<<dim3(blocks), dim3(S::RW * 64), 0, st>>>(p);
   if ((rc = check_launch("tattn_window_bwd"))) return rc;
-  const KeyBlocks kbs(RW, p.S, p.sinks, splits);
-  p.head = kbs.sink_blocks * splits;  // the longest: 84 -> 73 us for the whole backward at 4/4 x 16,384 x 64, window 512
-  p.tail = window_key_tail(p, 32 * RW, kbs.items - p.head);
+  const KeyBlocks kbs(RW, p);
+  p.head = kbs.sink_blocks * p.splits;  // the longest: 84 -> 73 us for the whole backward at 4/4 x 16,384 x 64, window 512
+  p.tail = window_key_tail(p, 32 * RW, kbs.blocks - kbs.sink_blocks) * p.parts;
   if ((rc = window_grid(slices, kbs.items, p.head + p.tail, &blocks))) return rc;
   if constexpr (D >= 64)
     window_dkdv_pair_kernel<T, D, RW, D == 128 ? 3 : 4, D == 128 ? 2 : 4><<<dim3(blocks), dim3(RW * 128), 0, st>>>(p);
   else
     window_dkdv_kernel<T, D, RW, 4, D == 32 ? 3 : 4><<<dim3(blocks), dim3(RW * 256), 0, st>>>(p);
-  if ((rc = check_launch("tattn_window_bwd")) || !kbs.sink_blocks) return rc;
-  const int64_t n = slices * kbs.sink_blocks * 2 * 32 * RW * D;
-  window_first_keys_kernel<T, D, RW><<<dim3((unsigned)((n + 255) / 256)), dim3(256), 0, st>>>(p);
+  if ((rc = check_launch("tattn_window_bwd")) || !kbs.parted()) return rc;
+  const int64_t n = slices * kbs.parted() * 2 * 32 * RW * D / 4;
+  window_parts_kernel<T, D, RW><<<dim3((unsigned)((n + 255) / 256)), dim3(256), 0, st>>>(p);
   return check_launch("tattn_window_bwd");
 }
 
@@ -1153,24 +1168,26 @@ int window_fwd_splits(const WindowParams& p, int D) {
   return (int)std::max<int64_t>(1, std::min<int64_t>((want + blocks - 1) / blocks, most_tiles(p) / 8));
 }
 
-// Parts of the first keys' dK and dV: each about as long as another key block's list, or as an even share of all
-// work over four workgroups per CU where that is more, so that all parts together stay near a thousand.
-int window_bwd_splits(const WindowParams& p, int D) {
-  if (p.sinks == 0) return 1;
-  const int64_t rw = key_tiles(D), keys = 32 * rw;
+// Parts that the queries of dK / dV are cut into. `parts`, of every key block's: where all blocks together are at most half of
+// what the chip holds at once (two workgroups a CU), as many as fill it, of at least 16 steps each (whole backward of 1 x 32/2
+// x 4,096 x 64, causal, 1,364 -> 309 us; 1 x 8/1 x 8,192 x 128, window 1,024, 283 -> 184). `splits`, of those that hold first keys: each about as long as another block's part, or as an even share of all work over four
+// workgroups per CU where that is more, so that all parts together stay near a thousand.
+void window_bwd_parts(WindowParams& p, int D) {
+  const int64_t rw = key_tiles(D), keys = 32 * rw, slices = (int64_t)p.Z * p.Hk;
   const int64_t all = (int64_t)p.G * ((p.N + 31) / 32);
   const int64_t list = std::min<int64_t>(all, (int64_t)p.G * (std::min<int64_t>(p.window, p.S) / 32 + rw + 1));
   const int64_t blocks = (p.S + keys - 1) / keys, first = std::min<int64_t>(blocks, (p.sinks + keys - 1) / keys);
-  const int64_t share = (int64_t)p.Z * p.Hk * (first * all + (blocks - first) * list) / 1024;
-  const int64_t part = std::max<int64_t>(std::max<int64_t>(list, share), 32);
-  return (int)std::max<int64_t>(1, std::min<int64_t>((all + part - 1) / part, 256));
+  p.parts = (int32_t)std::max<int64_t>(1, std::min<int64_t>(512 / (slices * blocks), list / 16));
+  p.splits = p.parts;
+  if (p.sinks == 0) return;
+  const int64_t share = slices * (first * all + (blocks - first) * list) / 1024;
+  const int64_t part = std::max<int64_t>(std::max<int64_t>(list / p.parts, share), 32);
+  p.splits = (int32_t)std::max<int64_t>(p.parts, std::min<int64_t>((all + part - 1) / part, 256));
 }
 
 int64_t window_bwd_part_floats(const WindowParams& p, int D) {
-  const int splits = window_bwd_splits(p, D);
-  if (splits == 1) return 0;
-  const int64_t rw = key_tiles(D), blocks = KeyBlocks((int)rw, p.S, p.sinks, splits).sink_blocks;
-  return (int64_t)p.Z * p.Hk * blocks * splits * 2 * 32 * rw * D;
+  const KeyBlocks kbs(key_tiles(D), p);
+  return (int64_t)p.Z * p.Hk * kbs.first(kbs.parted()) * 2 * 32 * key_tiles(D) * D;
 }
 
 int launch_window_fwd(WindowParams p, int D, int dtype, hipStream_t st) { TATTN_WIN_SWITCH(fwd_d) }
