@@ -1157,21 +1157,27 @@ int combine_d(const float* part, void* out, float* m, const int64_t so[3], int64
 
 }  // namespace
 
-// Few rows (a single row tile per slice, or fewer blocks of four than CUs): one row tile per workgroup, and its keys cut into
-// parts of at least eight tiles until the chip holds no more workgroups at once, one per CU at head dim 128 (128 KB of
-// stages), two below. (32 x 32/8 heads x 8,192 keys x 128, window 2,048: 51.5 us at one per CU, 59 at two, 68 at four.) 0:
-// blocks of four row tiles.
+// Few rows (a single row tile per slice, or few blocks of four tiles): one row tile per workgroup, whose waves share its keys.
+// Against blocks of four, us by head dim and number of such blocks, at windows of 300, 1,000 and 4,000 keys:
+//   128: 64 blocks 11, 18, 25 (19, 33, 50); 128: 20, 33, 67 (19, 34, 94); 250: 37, 64, 166 (21, 37, 102)
+//    64: 128 blocks 11, 15, 28 (14, 25, 65); 250: 17, 27, 64 (15, 26, 70); 300: 21, 33, 80 (19, 33, 71)
+//    32: 250 blocks 11, 18, 41 (13, 21, 56); 384: 15, 24, 58 (16, 27, 70); 500: 19, 30, 72 (16, 28, 74)
+// Its keys are cut into parts until the chip holds no more workgroups at once, one per CU at head dim 128 (128 KB of stages), two
+// below (32 x 32/8 heads x 8,192 keys x 128, window 2,048: 51.5 us at one per CU, 59 at two, 68 at four); of at least eight
+// tiles, and of more where many rows have to be joined (a workgroup each: 4 x 1,024 rows x 64 over 1,000
+// keys take 17 us in parts of eight tiles and 12 whole). 0: blocks of four row tiles.
 int window_fwd_splits(const WindowParams& p, int D) {
   const int64_t slices = (int64_t)p.Z * p.Hk, rows = (int64_t)p.N * p.G;
-  if (rows > 32 && slices * ((rows + 127) / 128) >= 256) return 0;
+  if (rows > 32 && slices * ((rows + 127) / 128) > (D == 128 ? 128 : D == 64 ? 256 : 400)) return 0;
   const int64_t blocks = slices * ((rows + 31) / 32), want = D == 128 ? 256 : 512;
-  return (int)std::max<int64_t>(1, std::min<int64_t>((want + blocks - 1) / blocks, most_tiles(p) / 8));
+  return (int)std::max<int64_t>(1, std::min<int64_t>(want / blocks, most_tiles(p) / std::max<int64_t>(8, slices * rows / 128)));
 }
 
 // Parts that the queries of dK / dV are cut into. `parts`, of every key block's: where all blocks together are at most half of
 // what the chip holds at once (two workgroups a CU), as many as fill it, of at least 16 steps each (whole backward of 1 x 32/2
-// x 4,096 x 64, causal, 1,364 -> 309 us; 1 x 8/1 x 8,192 x 128, window 1,024, 283 -> 184). `splits`, of those that hold first keys: each about as long as another block's part, or as an even share of all work over four
-// workgroups per CU where that is more, so that all parts together stay near a thousand.
+// x 4,096 x 64, causal, 1,364 -> 309 us; 1 x 8/1 x 8,192 x 128, window 1,024, 283 -> 184). `splits`, of those that hold first
+// keys: each about as long as another block's part, or as an even share of all work over four workgroups per CU where that is
+// more, so that all parts together stay near a thousand.
 void window_bwd_parts(WindowParams& p, int D) {
   const int64_t rw = key_tiles(D), keys = 32 * rw, slices = (int64_t)p.Z * p.Hk;
   const int64_t all = (int64_t)p.G * ((p.N + 31) / 32);
