@@ -33,9 +33,9 @@ def rows(t: torch.Tensor) -> torch.Tensor:
     return aligned(t, rows_apart(t))
 
 
-def layout(t: torch.Tensor | None) -> tuple:
-    """What the checks of a call and its launch arguments depend on, but for the data's address."""
-    return () if t is None else (t.shape, t.stride(), t.dtype, t.device)
+def layouts(*ts: torch.Tensor | None) -> tuple:
+    """What the checks of a call and its launch arguments depend on, but for the data's addresses."""
+    return tuple([None if t is None else (t.shape, t.stride(), t.dtype, t.device) for t in ts])
 
 
 def remember(plans: dict, key: tuple, plan: tuple) -> tuple:

@@ -14,7 +14,7 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from tattn import _lib
-from tattn._args import aligned, check_index, layout, remember, rows, rows_apart, same_device, strides
+from tattn._args import aligned, check_index, layouts, remember, rows, rows_apart, same_device, strides
 from tattn.api import _DTYPES, _on_device, _require_gpu, _stream
 
 
@@ -49,11 +49,13 @@ _plans: dict[tuple, tuple] = {}
 
 
 def _plan(q, k, qw, kw, cos, sin, positions, interleaved) -> tuple:
-    """Checks a call; what later calls with these layouts need: which tensors to copy, and the sizes among the
-    launch's arguments."""
+    """Checks a call; what later calls with these layouts need: which tensors to copy, the strides of inputs and outputs (None
+    where q or k is copied), and the sizes among the launch's arguments."""
     _check(q, k, qw, kw, cos, sin, positions)
+    _require_gpu(q)
     copies = (rows_apart(q), rows_apart(k), *(not t.is_contiguous() for t in (qw, kw, cos, sin)))
-    return copies, _scalars(q, k, qw, cos, positions, interleaved)
+    st = None if copies[0] or copies[1] else strides(q, k, torch.empty_like(q), torch.empty_like(k))
+    return copies, st, _scalars(q, k, qw, cos, positions, interleaved)
 
 
 def _scalars(q, k, qw, cos, positions, interleaved) -> tuple:
@@ -62,11 +64,14 @@ def _scalars(q, k, qw, cos, positions, interleaved) -> tuple:
     return pos_stride, z, h, k.shape[1], n, d, cos.shape[0], _DTYPES[q.dtype], _DTYPES[qw.dtype], int(interleaved)
 
 
-def _forward(q, k, qw, kw, cos, sin, positions, eps, scalars) -> tuple[torch.Tensor, torch.Tensor]:
+def _forward(q, k, qw, kw, cos, sin, positions, eps, plan) -> tuple[torch.Tensor, torch.Tensor]:
+    copies, held, scalars = plan
+    q0, k0 = q, k
+    q, k = aligned(q, copies[0]), aligned(k, copies[1])
     qo, ko = torch.empty_like(q), torch.empty_like(k)
     if q.numel() == 0:
         return qo, ko
-    _, st = strides(q, k, qo, ko)
+    _, st = held if q is q0 and k is k0 and held else strides(q, k, qo, ko)
     with _on_device(q):
         rc = _lib.load().tattn_norm_rope_fwd(
             q.data_ptr(), k.data_ptr(), qw.data_ptr(), kw.data_ptr(), cos.data_ptr(), sin.data_ptr(),
@@ -78,10 +83,10 @@ def _forward(q, k, qw, kw, cos, sin, positions, eps, scalars) -> tuple[torch.Ten
 
 class _NormRope(torch.autograd.Function):
     @staticmethod
-    def forward(ctx: Any, q, k, qw, kw, cos, sin, positions, eps, scalars):
+    def forward(ctx: Any, q, k, qw, kw, cos, sin, positions, eps, plan):
         ctx.save_for_backward(q, k, qw, kw, cos, sin, positions)
-        ctx.eps, ctx.scalars = eps, scalars
-        return _forward(rows(q), rows(k), qw, kw, cos, sin, positions, eps, scalars)
+        ctx.eps, ctx.scalars = eps, plan[2]
+        return _forward(q, k, qw, kw, cos, sin, positions, eps, plan)
 
     @staticmethod
     @once_differentiable
@@ -118,17 +123,15 @@ def qk_norm_rope(
     NaN. Outputs keep the order of their input's strides. Differentiable in q, k and both weights (cos and sin get no
     gradients); float16, bfloat16 or float32, all arithmetic in float32, each result rounded once. Any batch, head and
     sequence strides are read in place."""
-    key = (layout(q), layout(k), layout(q_weight), layout(k_weight), layout(cos), layout(sin), layout(positions), interleaved)
+    key = (layouts(q, k, q_weight, k_weight, cos, sin, positions), interleaved)
     plan = _plans.get(key)
     if plan is None:
-        plan = _plan(q, k, q_weight, k_weight, cos, sin, positions, interleaved)
-        _require_gpu(q)
-        remember(_plans, key, plan)
-    copies, scalars = plan
+        plan = remember(_plans, key, _plan(q, k, q_weight, k_weight, cos, sin, positions, interleaved))
+    copies = plan[0]
     qw, kw = aligned(q_weight, copies[2]), aligned(k_weight, copies[3])
     cos, sin = aligned(cos, copies[4]), aligned(sin, copies[5])
     if positions is not None:
         positions = positions.contiguous()
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or q_weight.requires_grad or k_weight.requires_grad):
-        return _NormRope.apply(q, k, qw, kw, cos, sin, positions, float(eps), scalars)
-    return _forward(aligned(q, copies[0]), aligned(k, copies[1]), qw, kw, cos, sin, positions, float(eps), scalars)
+        return _NormRope.apply(q, k, qw, kw, cos, sin, positions, float(eps), plan)
+    return _forward(q, k, qw, kw, cos, sin, positions, float(eps), plan)

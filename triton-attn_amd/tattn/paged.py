@@ -18,7 +18,7 @@ from typing import NamedTuple
 import torch
 
 from tattn import _lib
-from tattn._args import aligned, check_index, layout, remember, rows_apart, same_device, strides
+from tattn._args import aligned, check_index, layouts, remember, rows_apart, same_device, strides
 from tattn.api import _on_device, _require_gpu, _stream
 
 _DTYPES = {torch.float16: _lib.F16, torch.bfloat16: _lib.BF16}
@@ -69,7 +69,7 @@ def page_tables(lens: torch.Tensor, new_tokens: torch.Tensor, tables: torch.Tens
     """
     if not 0 <= tokens < (1 << 31) - 4096:
         raise ValueError(f"tokens out of range: {tokens}")
-    key = (layout(lens), layout(new_tokens), layout(tables), layout(free_pages), page_size)
+    key = (layouts(lens, new_tokens, tables, free_pages), page_size)
     plan = _table_plans.get(key)
     if plan is None:
         _check_tables(lens, new_tokens, tables, free_pages, page_size)
@@ -133,9 +133,9 @@ def cache4_write(cache: Cache4, k: torch.Tensor, v: torch.Tensor, slots: torch.T
     """Writes keys and values [tokens, kv_heads, head_dim] (the cache's dtype, any token and head strides) into
     `slots` (int64 [tokens], as page_tables gives them). Slots outside the cache, such as a padded token's -1,
     are skipped. No two tokens of a call may share a slot."""
-    key = (layout(k), layout(v), layout(slots), cache.layout)
-    copies = _write_plans.get(key)
-    if copies is None:
+    key = (layouts(k, v, slots), cache.layout)
+    plan = _write_plans.get(key)
+    if plan is None:
         if k.dim() != 3 or k.shape != v.shape or tuple(k.shape[1:]) != (cache.kv_heads, cache.head_dim):
             raise ValueError(f"expected k, v of shape [tokens, {cache.kv_heads}, {cache.head_dim}]; got {list(k.shape)}, {list(v.shape)}")
         if k.dtype != cache.dtype or v.dtype != cache.dtype:
@@ -143,9 +143,10 @@ def cache4_write(cache: Cache4, k: torch.Tensor, v: torch.Tensor, slots: torch.T
         check_index("slots", slots, torch.int64, (k.shape[0],))
         same_device(cache.codes, k=k, v=v, slots=slots)
         _require_gpu(k)
-        copies = remember(_write_plans, key, (rows_apart(k), rows_apart(v)))
-    k, v, slots = aligned(k, copies[0]), aligned(v, copies[1]), slots.contiguous()
-    _, st = strides(k, v)
+        plan = remember(_write_plans, key, (rows_apart(k), rows_apart(v), strides(k, v)))
+    given = k, v
+    k, v, slots = aligned(k, plan[0]), aligned(v, plan[1]), slots.contiguous()
+    _, st = plan[2] if k is given[0] and v is given[1] else strides(k, v)
     with _on_device(k):
         rc = _lib.load().tattn_cache4_write(
             cache.codes.data_ptr(), cache.scales.data_ptr(), k.data_ptr(), v.data_ptr(), slots.data_ptr(), *st, k.shape[0],
@@ -178,8 +179,8 @@ _attention_plans: dict[tuple, tuple] = {}
 
 
 def _attention_plan(q, cache, tables, lens, window, sinks) -> tuple:
-    """Checks a call of cache4_attention; whether q and tables are copied, the float32 values of workspace, and the sizes
-    among the launch's arguments (None: nothing to see)."""
+    """Checks a call of cache4_attention; whether q and tables are copied, the strides of q and the output (None where q is
+    copied), the float32 values of workspace, and the sizes among the launch's arguments (None: nothing to see)."""
     if q.dim() != 3 or q.shape[2] != cache.head_dim or q.shape[1] < 1 or q.shape[1] % cache.kv_heads:
         raise ValueError(f"expected q [requests, heads, {cache.head_dim}] with a multiple of {cache.kv_heads} heads; got {list(q.shape)}")
     r, h, d = q.shape
@@ -195,13 +196,14 @@ def _attention_plan(q, cache, tables, lens, window, sinks) -> tuple:
     same_device(q, cache=cache.codes, tables=tables, lens=lens)
     _require_gpu(q)
     if q.numel() == 0 or width == 0 or cache.pages == 0:
-        return rows_apart(q), False, 0, None
+        return rows_apart(q), False, None, 0, None
     held = width * cache.page_size
     window, sinks = 0 if window is None else min(window, held), min(sinks, held)
     out = ctypes.c_int64()
     _lib.check(_lib.load().tattn_cache4_attention_workspace(r, h, cache.kv_heads, d, width, cache.page_size, window, sinks,
                                                             ctypes.byref(out)), "tattn_cache4_attention_workspace")
-    return (rows_apart(q), width > 1 and tables.stride(1) != 1, out.value,
+    return (rows_apart(q), width > 1 and tables.stride(1) != 1,
+            None if rows_apart(q) else strides(q, torch.empty_like(q)), out.value,
             (r, h, cache.kv_heads, d, width, cache.pages, cache.page_size, window, sinks, _DTYPES[cache.dtype]))
 
 
@@ -217,11 +219,12 @@ def cache4_attention(
     that sees nothing gives zeros. sm_scale defaults to 1 / sqrt(head_dim). For serving: refuses a q that requires gradients."""
     if q.requires_grad and torch.is_grad_enabled():
         raise ValueError("cache4_attention has no gradients: call it under torch.no_grad()")
-    key = (layout(q), layout(tables), layout(lens), cache.layout, window, sinks)
+    key = (layouts(q, tables, lens), cache.layout, window, sinks)
     plan = _attention_plans.get(key)
     if plan is None:
         plan = remember(_attention_plans, key, _attention_plan(q, cache, tables, lens, window, sinks))
-    copy_q, copy_tables, floats, sizes = plan
+    copy_q, copy_tables, held, floats, sizes = plan
+    given = q
     q, lens = aligned(q, copy_q), lens.contiguous()
     o = torch.empty_like(q)
     if sizes is None:
@@ -229,7 +232,7 @@ def cache4_attention(
     if copy_tables:
         tables = tables.contiguous()
     work = q.new_empty(floats, dtype=torch.float32) if floats else None
-    _, st = strides(q, o)
+    _, st = held if held and q is given else strides(q, o)
     with _on_device(q):
         rc = _lib.load().tattn_cache4_attention(
             q.data_ptr(), o.data_ptr(), cache.codes.data_ptr(), cache.scales.data_ptr(), tables.data_ptr(), lens.data_ptr(),

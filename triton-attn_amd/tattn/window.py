@@ -16,7 +16,7 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from tattn import _lib
-from tattn._args import aligned, check_index, layout, remember, rows_apart, same_device, strides
+from tattn._args import aligned, check_index, layouts, remember, rows_apart, same_device, strides
 from tattn.api import _DTYPES, _on_device, _require_gpu, _stream
 
 
@@ -63,30 +63,31 @@ _plans: dict[tuple, tuple] = {}
 
 
 def _plan(q, k, v, window, sinks, lens) -> tuple:
-    """Checks a call; which of q, k, v are copied, the float32 values of workspace of forward and backward, and the sizes
-    among the launches' arguments (None: nothing to see)."""
+    """Checks a call; which of q, k, v are copied, the strides of inputs and output (None where one is copied), the float32
+    values of workspace of forward and backward, and the sizes among the launches' arguments (None: nothing to see)."""
     _check(q, k, v, window, sinks, lens)
     _require_gpu(q)
     copies = tuple(_tiles_apart(t) for t in (q, k, v))
     z, h, n, d = q.shape
     hk, s = k.shape[1:3]
     if q.numel() == 0 or s == 0:
-        return copies, 0, 0, None
+        return copies, None, 0, 0, None
     sizes = (z, h, hk, n, s, d, min(window, s), min(sinks, s))
     half = q.dtype != torch.float32  # float32 is never split
-    return (copies, _workspace(False, sizes) if half else 0, _workspace(True, sizes) if half and lens is None else 0,
-            (*sizes, _DTYPES[q.dtype]))
+    return (copies, None if any(copies) else strides(q, k, v, torch.empty_like(q)), _workspace(False, sizes) if half else 0,
+            _workspace(True, sizes) if half and lens is None else 0, (*sizes, _DTYPES[q.dtype]))
 
 
 def _forward(q, k, v, plan, scale, lens, save_lse) -> tuple[torch.Tensor, torch.Tensor | None]:
-    copies, floats, _, sizes = plan
+    copies, held, floats, _, sizes = plan
+    given = q, k, v
     q, k, v = aligned(q, copies[0]), aligned(k, copies[1]), aligned(v, copies[2])
     o = torch.empty_like(q)
     m = q.new_empty(q.shape[:3], dtype=torch.float32) if save_lse else None
     if sizes is None:
         return o.zero_(), m
     work = q.new_empty(floats, dtype=torch.float32) if floats else None
-    _, st = strides(q, k, v, o)
+    _, st = held if held and q is given[0] and k is given[1] and v is given[2] else strides(q, k, v, o)
     with _on_device(q):
         rc = _lib.load().tattn_window_fwd(
             q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), None if m is None else m.data_ptr(),
@@ -97,7 +98,7 @@ def _forward(q, k, v, plan, scale, lens, save_lse) -> tuple[torch.Tensor, torch.
 
 
 def _backward(q, k, v, o, m, do, plan, scale) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
-    _, _, floats, sizes = plan
+    floats, sizes = plan[3:]
     q, k, v, o, do = _tiles(q), _tiles(k), _tiles(v), _tiles(o), _tiles(do)
     dq, dk, dv = torch.empty_like(q), torch.empty_like(k), torch.empty_like(v)
     if sizes is None:
@@ -143,7 +144,7 @@ def window_attention(
     zeros. sm_scale defaults to 1 / sqrt(dim). Differentiable in q, k and v without lens; with lens the call is for serving
     and refuses inputs that require gradients. A key or value that is infinite or NaN makes the rows that see it
     NaN, and may make NaN of rows up to 64 positions before it or after its window that do not see it."""
-    key = (layout(q), layout(k), layout(v), layout(lens), window, sinks)
+    key = (layouts(q, k, v, lens), window, sinks)
     plan = _plans.get(key)
     needs = (q.requires_grad or k.requires_grad or v.requires_grad) and torch.is_grad_enabled()
     if needs and lens is not None:
