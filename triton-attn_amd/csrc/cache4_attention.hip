@@ -128,30 +128,31 @@ __global__ __launch_bounds__(256, D == 128 ? 3 : 4) void cache4_attention_kernel
   const uint8_t* codes = p.codes + ((int64_t)hk * 2 << p.shift) * (D / 2) + g * (D / 8);
   const uint8_t* scales = p.scales + ((int64_t)hk * 2 << p.shift) * (D / 32) + (D == 128 ? g : D == 64 ? g >> 1 : 0);
 
-  // Pages of the lane's keys in list entry i; -1 where a key is hidden.
-  auto pages_of = [&](int i, int (&pg)[2]) __attribute__((always_inline)) {
+  // The page of the lane's keys in list entry i (pages hold multiples of 16 keys: both lie in one; -1 where both are
+  // hidden), and which of them are visible.
+  auto page_of = [&](int i, bool (&see)[2]) __attribute__((always_inline)) {
     const int t = list.at(min(i, i1 - 1));
     const bool inner = i < i1 && 32 * t + 31 <= pos && (32 * t >= list.lo || 32 * t + 31 < p.sinks);
 #pragma unroll
     for (int a = 0; a < 2; ++a) {
       const int key = 32 * t + key0 + 4 * a;
-      const bool see = inner || (i < i1 && key <= pos && (key >= list.lo || key < p.sinks));
-      pg[a] = see ? table[key >> p.shift] : -1;
+      see[a] = inner || (i < i1 && key <= pos && (key >= list.lo || key < p.sinks));
     }
+    return see[0] || see[1] ? table[(32 * t + key0) >> p.shift] : -1;
   };
-  auto load = [&](int i, const int (&pg)[2]) __attribute__((always_inline)) {
+  auto load = [&](int i, int page, const bool (&see)[2]) __attribute__((always_inline)) {
     Codes<D> x;
-    const int t0 = 32 * list.at(min(i, i1 - 1));
+    const bool held = (uint32_t)page < (uint32_t)p.pages;
+    const uint64_t at = (uint64_t)(held ? (uint32_t)page : 0u) * page_rows + (uint32_t)((32 * list.at(min(i, i1 - 1)) + key0) & in_page);
+    const uint8_t* pc = codes + at * (D / 2);
+    const uint8_t* ps = scales + at * (D / 32);
 #pragma unroll
     for (int a = 0; a < 2; ++a) {
-      x.ok[a] = (uint32_t)pg[a] < (uint32_t)p.pages;
-      const uint64_t at = (uint64_t)(x.ok[a] ? (uint32_t)pg[a] : 0u) * page_rows + (uint32_t)((t0 + key0 + 4 * a) & in_page);
-      const uint8_t* pc = codes + at * (D / 2);
-      const uint8_t* ps = scales + at * (D / 32);
-      load_words(pc, x.k[a]);
-      load_words(pc + ((D / 2) << p.shift), x.v[a]);
-      x.ks[a] = ps[0];
-      x.vs[a] = ps[(D / 32) << p.shift];
+      x.ok[a] = held && see[a];
+      load_words(pc + 4 * a * (D / 2), x.k[a]);
+      load_words(pc + 4 * a * (D / 2) + ((D / 2) << p.shift), x.v[a]);
+      x.ks[a] = ps[4 * a * (D / 32)];
+      x.vs[a] = ps[4 * a * (D / 32) + ((D / 32) << p.shift)];
     }
     return x;
   };
@@ -244,17 +245,17 @@ __global__ __launch_bounds__(256, D == 128 ? 3 : 4) void cache4_attention_kernel
 
   int i = i0 + w;
   if (i < i1) {
-    int pg[2];
-    pages_of(i, pg);
-    Codes<D> x = load(i, pg);
-    pages_of(i + 4, pg);
+    bool see[2];
+    int page = page_of(i, see);
+    Codes<D> x = load(i, page, see);
+    page = page_of(i + 4, see);
     for (; i < i1; i += 8) {
-      Codes<D> y = load(i + 4, pg);
-      pages_of(i + 8, pg);
+      Codes<D> y = load(i + 4, page, see);
+      page = page_of(i + 8, see);
       tile(x);
       if (i + 4 >= i1) break;
-      x = load(i + 8, pg);
-      pages_of(i + 12, pg);
+      x = load(i + 8, page, see);
+      page = page_of(i + 12, see);
       tile(y);
     }
   }
