@@ -14,7 +14,7 @@
 // The next tile's codes and the page numbers of the one after are on their way meanwhile; waves meet only at the end. A
 // workgroup of four waves takes `chunk` consecutive tiles of one request and key head; requests of many tiles are cut into
 // equal chunks, whatever their lengths, and joined by combine_kernel. 64 requests of up to 16,384 tokens with 32/8 heads x 128
-// take 152 us, 4.7 TB/s of the cache's bytes, a large copy's rate (32 x 32 x 16 instructions, with twice the unused columns:
+// take 147 us, 4.9 TB/s of the cache's bytes, a large copy's rate (32 x 32 x 16 instructions, with twice the unused columns:
 // 163 us).
 #include <algorithm>
 
