@@ -8,7 +8,7 @@
 // their exponent, of two keys, 8 (l / 4) + 4 a + l % 4 of the tile for a = 0, 1, converts two codes an instruction
 // (v_cvt_scalef32_pk, which also applies the block's power of two), and
 //   S^T = K Q^T     two 16-key tiles. K's codes become operands in the lane that loaded them: the order of d within a dot
-//                   product is free, so lane group g owns the g-th quarter of d, for Q as well. With the keys above, a lane's
+//                   product is free, so a lane group owns a quarter of d, for Q as well. With the keys above, a lane's
 //                   8 scores are those of keys 8 g .. 8 g + 7: the B operand of
 //   O^T += V^T P^T  V's values go through the wave's own 32 rows of LDS, swizzled, and come back transposed.
 // The next tile's codes and the page numbers of the one after are on their way meanwhile; waves meet only at the end. A
@@ -74,21 +74,30 @@ struct Scales {
 // The lane's quarter rows of its two keys of a tile.
 template <int D>
 struct Codes {
-  uint32_t k[2][C4<D>::W], v[2][C4<D>::W];
+  uint32_t k[2 * C4<D>::W], v[2 * C4<D>::W];
   Scales<D> scale[2];     // exponents of K and of V
   bool ok[2];             // the key is visible and its page is one of the cache's
 };
 
 template <int W>
-__device__ __forceinline__ void load_words(const uint8_t* p, uint32_t (&x)[W]) {
+__device__ __forceinline__ void load_words(const uint8_t* p, uint32_t* x) {
   if constexpr (W == 4) {
     const u32x4 a = *reinterpret_cast<const u32x4*>(p);
     x[0] = a[0], x[1] = a[1], x[2] = a[2], x[3] = a[3];
-  } else if constexpr (W == 2) {
+  } else {
     const u32x2 a = *reinterpret_cast<const u32x2*>(p);
     x[0] = a[0], x[1] = a[1];
-  } else {
-    x[0] = *reinterpret_cast<const uint32_t*>(p);
+  }
+}
+
+// Half rows of two keys as loaded (lanes 0-31 of the first key, the others of the second) -> a quarter row of either.
+template <int W>
+__device__ __forceinline__ void quarters(uint32_t (&x)[2 * W]) {
+#pragma unroll
+  for (int i = 0; i < W; ++i) {
+    const auto y = __builtin_amdgcn_permlane32_swap(x[i], x[W + i], false, false);
+    x[i] = y[0];
+    x[W + i] = y[1];
   }
 }
 
@@ -111,6 +120,9 @@ __global__ __launch_bounds__(256, D == 128 ? 3 : 4) void cache4_attention_kernel
   using V4 = typename H::V4;
   using V2 = typename H::V2;
   using C = C4<D>;
+  // Below head dim 128 a lane loads half a row of one of its two keys and swaps a quarter with the lane 32 away: half as many
+  // loads, each twice as wide (64 x 16,384 x 32/8 x 64: 90 -> 85 us; 112 x 11,401 x 3 x 32: 63 -> 32).
+  constexpr bool HALVES = D < 128;
   __shared__ __attribute__((aligned(1024))) char smem[4 * C::TILE];
   __shared__ float red[2][4][kRows];
 
@@ -136,9 +148,10 @@ __global__ __launch_bounds__(256, D == 128 ? 3 : 4) void cache4_attention_kernel
     return;
   }
 
+  const int quarter = HALVES ? 2 * (g & 1) + (g >> 1) : g;  // of d, that the lane's group owns
   V8 qop[C::W];
   {
-    const T* src = (const T*)p.q + r * p.sq[0] + (hk * p.G + (live ? row : 0)) * p.sq[1] + g * (D / 4);
+    const T* src = (const T*)p.q + r * p.sq[0] + (hk * p.G + (live ? row : 0)) * p.sq[1] + quarter * (D / 4);
 #pragma unroll
     for (int s = 0; s < C::W; ++s) {
       const V8 x = *reinterpret_cast<const V8*>(src + 8 * s);
@@ -151,9 +164,9 @@ __global__ __launch_bounds__(256, D == 128 ? 3 : 4) void cache4_attention_kernel
   const int key0 = 8 * (l16 >> 2) + (l16 & 3);  // the lane's keys of a tile: key0 and key0 + 4
   // Byte offsets are (page number) * (bytes of a page) + what follows; a tile starts a page, or lies within one.
   const uint32_t page_rows = (uint32_t)p.Hk * 2 << p.shift;
-  const uint8_t* codes = p.codes + ((int64_t)hk * 2 << p.shift) * (D / 2) + g * (D / 8);
+  const uint8_t* codes = p.codes + ((int64_t)hk * 2 << p.shift) * (D / 2) + (HALVES ? (g & 1) * (D / 4) + 2 * D * (g >> 1) : g * (D / 8));
   const uint8_t* scales = p.scales + ((int64_t)hk * 2 << p.shift) * (D / 32) + (D == 128 ? g : 0);
-  const uint32_t pick = 2 * (l16 & 3) + (g >> 1);
+  const uint32_t pick = 2 * (l16 & 3) + (quarter >> 1);
 
   // The page of the lane's keys in list entry i (pages hold multiples of 16 keys: both lie in one; -1 where both are
   // hidden), and which of them are visible.
@@ -176,8 +189,14 @@ __global__ __launch_bounds__(256, D == 128 ? 3 : 4) void cache4_attention_kernel
 #pragma unroll
     for (int a = 0; a < 2; ++a) {
       x.ok[a] = held && see[a];
-      load_words(pc + 4 * a * (D / 2), x.k[a]);
-      load_words(pc + 4 * a * (D / 2) + ((D / 2) << p.shift), x.v[a]);
+      if constexpr (!HALVES) {
+        load_words<C::W>(pc + 4 * a * (D / 2), x.k + a * C::W);
+        load_words<C::W>(pc + 4 * a * (D / 2) + ((D / 2) << p.shift), x.v + a * C::W);
+      }
+    }
+    if constexpr (HALVES) {
+      load_words<2 * C::W>(pc, x.k);
+      load_words<2 * C::W>(pc + ((D / 2) << p.shift), x.v);
     }
 #pragma unroll
     for (int v = 0; v < 2; ++v) x.scale[v].load(ps + (v ? (D / 32) << p.shift : 0));
@@ -200,12 +219,16 @@ __global__ __launch_bounds__(256, D == 128 ? 3 : 4) void cache4_attention_kernel
   auto tile = [&](Codes<D>& x) __attribute__((always_inline)) {
     const uint64_t see0 = __builtin_amdgcn_ballot_w64(x.ok[0]), see1 = __builtin_amdgcn_ballot_w64(x.ok[1]);
     if ((see0 | see1) == 0) return;
+    if constexpr (HALVES) {
+      quarters<C::W>(x.k);
+      quarters<C::W>(x.v);
+    }
     if ((see0 & see1) != ~0ull) {  // what lies at a hidden key's place reaches nothing
 #pragma unroll
       for (int a = 0; a < 2; ++a)
         if (!x.ok[a]) {
 #pragma unroll
-          for (int i = 0; i < C::W; ++i) x.k[a][i] = x.v[a][i] = 0;
+          for (int i = 0; i < C::W; ++i) x.k[a * C::W + i] = x.v[a * C::W + i] = 0;
           x.scale[0].hide(a);
           x.scale[1].hide(a);
         }
@@ -216,14 +239,14 @@ __global__ __launch_bounds__(256, D == 128 ? 3 : 4) void cache4_attention_kernel
       s[a] = f32x4{};
       const float scale = x.scale[0].of(a, pick);
 #pragma unroll
-      for (int i = 0; i < C::W; ++i) s[a] = mfma16(values8<T>(x.k[a][i], scale), qop[i], s[a]);
+      for (int i = 0; i < C::W; ++i) s[a] = mfma16(values8<T>(x.k[a * C::W + i], scale), qop[i], s[a]);
     }
 #pragma unroll
     for (int a = 0; a < 2; ++a) {
       const float scale = x.scale[1].of(a, pick);
 #pragma unroll
       for (int i = 0; i < C::W; ++i)
-        *reinterpret_cast<TATTN_LDS V8*>((TATTN_LDS char*)vrows + C::addr(key0 + 4 * a, g * (D / 2) + 16 * i)) = values8<T>(x.v[a][i], scale);
+        *reinterpret_cast<TATTN_LDS V8*>((TATTN_LDS char*)vrows + C::addr(key0 + 4 * a, quarter * (D / 2) + 16 * i)) = values8<T>(x.v[a * C::W + i], scale);
     }
     if ((see0 & see1) != ~0ull) {  // row m of tile a is lane m's key a: the lane's scores are rows 4 g + e
 #pragma unroll
