@@ -138,7 +138,7 @@ __global__ __launch_bounds__(256, D == 128 ? 3 : 4) void cache4_attention_kernel
   const int len = min(max(p.lens[r], 0), p.most);
   const int pos = len - 1;
   TileList list;
-  list.init(pos, pos, p.window, p.sinks);
+  list.init(pos, pos, pos, p.window, p.sinks);
   const int i0 = chunk * p.chunk, i1 = min(list.n, i0 + p.chunk);
   const int64_t slice = (int64_t)r * p.Hk + hk;
   const int64_t prow = (slice * p.splits + chunk) * p.G + row;

@@ -17,17 +17,29 @@ namespace tattn {
 constexpr float kNoMax = -3.0e38f;
 
 // The key tiles (32 keys) that rows at positions [p0, p1] see: the tiles of the first `sinks` keys, then those of
-// the window.
+// the window. `last` is the position of the first row of the last wave. Where the tile in which the first keys end lies in the
+// window of the first wave's rows and before the last's, it comes twice: of its other keys nothing may be there for waves that
+// see none of them (a hidden key's probability is 0, but 0 times a NaN in its value is not), so these waves take an entry
+// among the first keys', in which the other keys are zeros, and those whose window holds the tile take it whole.
 struct TileList {
   int lo;     // first key of the window
   int sink_tiles, first, n;
-  __device__ __forceinline__ void init(int p0, int p1, int window, int sinks) {
+  int extra;  // the entry of that tile among the first keys', or -1
+  __device__ __forceinline__ void init(int p0, int p1, int last, int window, int sinks) {
     lo = max(0, p0 - window + 1);
     first = lo >> 5;
     sink_tiles = min((min(sinks, lo) + 31) >> 5, first);
+    const int end = sinks >> 5;
+    extra = -1;
+    if ((sinks & 31) != 0 && first <= end && end < (last - window + 1) >> 5) {
+      extra = first = end;  // the tiles before it hold first keys alone
+      sink_tiles = end + 1;
+    }
     n = p1 < 0 ? 0 : sink_tiles + (p1 >> 5) - first + 1;
   }
   __device__ __forceinline__ int at(int i) const { return i < sink_tiles ? i : i - sink_tiles + first; }
+  // Keys below are zeros in entry i, but for the first keys.
+  __device__ __forceinline__ int low(int i) const { return i == extra ? 0x7fffffff : lo; }
 };
 
 // The raw score of a hidden key: its scaled value is -inf, so its probability is 0 whatever the row's max or log-sum-exp
@@ -74,16 +86,19 @@ struct ColMask {
 // (masked()), or all. p1 < 0: no rows.
 struct WaveTiles {
   int lo, hi, sinks;                 // live: t <= hi, from lo on or with first keys
+  int skip;                          // the entry that is not the wave's of a tile that comes twice
   int full_lo, full_hi, full_sinks;  // seen by all rows
-  __device__ __forceinline__ void init(int p0, int p1, int window, int sinks_) {
+  __device__ __forceinline__ void init(const TileList& list, int p0, int p1, int window, int sinks_) {
     hi = p1 < 0 ? -1 : p1 >> 5;
     lo = max(0, p0 - window + 1) >> 5;
     sinks = (sinks_ + 31) >> 5;
+    skip = list.extra < 0 || list.first >= lo ? list.extra : list.sink_tiles;
     full_hi = ((p0 + 1) >> 5) - 1;
     full_lo = (max(0, p1 - window + 1) + 31) >> 5;
     full_sinks = sinks_ >> 5;
   }
-  __device__ __forceinline__ bool live(int t) const { return t <= hi && (t >= lo || t < sinks); }
+  // Entry i of the list, tile t.
+  __device__ __forceinline__ bool live(int i, int t) const { return t <= hi && (t >= lo || t < sinks) && i != skip; }
   __device__ __forceinline__ bool masked(int t) const { return t > full_hi || (t < full_lo && t >= full_sinks); }
 };
 

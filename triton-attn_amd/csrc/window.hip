@@ -98,6 +98,7 @@ struct WinRows {
   int rows;      // N * G
   int tile0;     // first row tile of the workgroup
   int p0, p1;    // positions of the workgroup's rows
+  int last;      // position of the last row tile's first row
   int top;       // last key any of them sees
   __device__ __forceinline__ void init(const WindowParams& p, int slice_, int blk, int rw) {
     slice = slice_;
@@ -109,6 +110,7 @@ struct WinRows {
     tile0 = blk * rw;
     p0 = off + (32 * tile0) / p.G;
     p1 = off + min(32 * (tile0 + rw) - 1, rows - 1) / p.G;
+    last = off + min(32 * (tile0 + rw - 1), rows - 1) / p.G;
     top = p1;
   }
 };
@@ -127,13 +129,13 @@ __device__ __forceinline__ void fetch_keys(const WinLoader<D, NW, NT>& ld, __amd
   for (int x = 0; x < R::TW; ++x) {
     const int at = i0 + ld.first + x;
     if (at >= i1) break;
-    const int t = list.at(at);
+    const int t = list.at(at), low = list.low(at);
     const uint32_t o = (uint32_t)t * ld.tile_bytes;
-    if (32 * t + 31 > top || (32 * t < list.lo && 32 * t + 31 >= sinks)) {
+    if (32 * t + 31 > top || (32 * t < low && 32 * t + 31 >= sinks)) {
 #pragma unroll
       for (int i = 0; i < R::PPT; ++i) {
         const int key = 32 * t + ld.row(i);
-        const bool dead = key > top || (key < list.lo && key >= sinks);
+        const bool dead = key > top || (key < low && key >= sinks);
         ld.fetch(rs, stage, x, i, dead ? kBeyond : ld.go[i] + o);
       }
     } else {
@@ -168,7 +170,7 @@ __global__ __launch_bounds__(RW * CS * 64, OCC) void window_fwd_kernel(const Win
   WinRows b;
   b.init(p, slice, p.nblk - 1 - blk, RW);  // longest rows first
   TileList list;
-  list.init(b.p0, b.p1, p.window, p.sinks);
+  list.init(b.p0, b.p1, b.last, p.window, p.sinks);
   const int i0 = SPLIT ? (int)((int64_t)list.n * split / p.splits) : 0;
   const int i1 = SPLIT ? (int)((int64_t)list.n * (split + 1) / p.splits) : list.n;
   const int nsteps = (i1 - i0 + CS - 1) / CS;
@@ -190,7 +192,7 @@ __global__ __launch_bounds__(RW * CS * 64, OCC) void window_fwd_kernel(const Win
   const int pos = b.off + n;
   // The wave's positions; a wave without rows sees no tile.
   WaveTiles sees;
-  sees.init(b.off + tile0 / p.G, tile0 < b.rows ? b.off + min(tile0 + 31, b.rows - 1) / p.G : -1, p.window, p.sinks);
+  sees.init(list, b.off + tile0 / p.G, tile0 < b.rows ? b.off + min(tile0 + 31, b.rows - 1) / p.G : -1, p.window, p.sinks);
   V8 qop[NSD];
   {
     const T* src = (const T*)p.q + b.z * p.sq[0] + (b.hk * p.G + g) * p.sq[1] + n * p.sq[2] + 8 * h2;
@@ -263,7 +265,7 @@ __global__ __launch_bounds__(RW * CS * 64, OCC) void window_fwd_kernel(const Win
     const int k = i0 + i * CS + cs;
     if (k < i1) {
       const int t = list.at(k);
-      if (sees.live(t)) tile(cur, t);
+      if (sees.live(k, t)) tile(cur, t);
     }
     all_landed_barrier();
   };
@@ -434,7 +436,7 @@ __global__ __launch_bounds__(RW * CS * 64, OCC) void window_dq_kernel(const Wind
   WinRows b;
   b.init(p, slice, p.nblk - 1 - blk, RW);
   TileList list;
-  list.init(b.p0, b.p1, p.window, p.sinks);
+  list.init(b.p0, b.p1, b.last, p.window, p.sinks);
   const int nsteps = (list.n + CS - 1) / CS;
 
   WinLoader<D, NW, CS> ld;
@@ -453,7 +455,7 @@ __global__ __launch_bounds__(RW * CS * 64, OCC) void window_dq_kernel(const Wind
   const int n = (live ? row : 0) / p.G, g = (live ? row : 0) % p.G, h = b.hk * p.G + g;
   const int pos = b.off + n;
   WaveTiles sees;
-  sees.init(b.off + tile0 / p.G, tile0 < b.rows ? b.off + min(tile0 + 31, b.rows - 1) / p.G : -1, p.window, p.sinks);
+  sees.init(list, b.off + tile0 / p.G, tile0 < b.rows ? b.off + min(tile0 + 31, b.rows - 1) / p.G : -1, p.window, p.sinks);
   const int64_t mrow = ((int64_t)b.z * p.H + h) * p.N + n;
   V8 qop[NSD], dop[NSD];
   float dl;
@@ -516,7 +518,7 @@ __global__ __launch_bounds__(RW * CS * 64, OCC) void window_dq_kernel(const Wind
     const int k = i * CS + cs;
     if (k < list.n) {
       const int t = list.at(k);
-      if (sees.live(t)) tile(cur, t);
+      if (sees.live(k, t)) tile(cur, t);
     }
     all_landed_barrier();
   };

@@ -101,16 +101,16 @@ struct Rows32 {
     rows = p.N * p.G;
     const int p0 = off + 128 * blk / p.G;
     top = off + min(128 * blk + 127, rows - 1) / p.G;
-    list.init(p0, top, p.window, p.sinks);
+    list.init(p0, top, off + min(128 * blk + 96, rows - 1) / p.G, p.window, p.sinks);
     const int tile0 = 128 * blk + 32 * w, row = tile0 + l32;
     live = row < rows;
     n = (live ? row : 0) / p.G;
     g = (live ? row : 0) % p.G;
     pos = off + n;
-    sees.init(off + tile0 / p.G, tile0 < rows ? off + min(tile0 + 31, rows - 1) / p.G : -1, p.window, p.sinks);
+    sees.init(list, off + tile0 / p.G, tile0 < rows ? off + min(tile0 + 31, rows - 1) / p.G : -1, p.window, p.sinks);
   }
-  // Whether any row of the workgroup sees the key.
-  __device__ __forceinline__ bool key(int k, int sinks) const { return k <= top && (k >= list.lo || k < sinks); }
+  // Whether entry i of the list has the key: some row of the workgroup sees it.
+  __device__ __forceinline__ bool key(int i, int k, int sinks) const { return k <= top && (k >= list.low(i) || k < sinks); }
 };
 
 template <int D, int OCC>
@@ -131,8 +131,8 @@ __global__ __launch_bounds__(256, OCC) void window_fwd_f32_kernel(const WindowPa
 #pragma unroll
   for (int u = 0; u < C::DT; ++u) acc[u] = f32x16{};
   Tile32<D> kn, vn;
-  auto seen = [&](int key) { return b.key(key, p.sinks); };
   auto load = [&](int i) {
+    auto seen = [&](int key) { return b.key(i, key, p.sinks); };
     kn.load(K, p.sk[2], 32 * b.list.at(i), seen);
     vn.load(V, p.sv[2], 32 * b.list.at(i), seen);
   };
@@ -144,7 +144,7 @@ __global__ __launch_bounds__(256, OCC) void window_fwd_f32_kernel(const WindowPa
     __syncthreads();
     if (i + 1 < b.list.n) load(i + 1);
     const int t = b.list.at(i);
-    if (!b.sees.live(t)) continue;
+    if (!b.sees.live(i, t)) continue;
     f32x16 s = rows_dot<D>(ks, q, f32x16{}, l32, h2);
     if (b.sees.masked(t)) RowMask(b.pos, t, h2, p.window, p.sinks).hide(s, hidden);
     float mx = kNoMax;
@@ -216,8 +216,8 @@ __global__ __launch_bounds__(256, OCC) void window_dq_f32_kernel(const WindowPar
 #pragma unroll
   for (int u = 0; u < C::DT; ++u) dq[u] = f32x16{};
   Tile32<D> kn, vn;
-  auto seen = [&](int key) { return b.key(key, p.sinks); };
   auto load = [&](int i) {
+    auto seen = [&](int key) { return b.key(i, key, p.sinks); };
     kn.load(K, p.sk[2], 32 * b.list.at(i), seen);
     vn.load(V, p.sv[2], 32 * b.list.at(i), seen);
   };
@@ -229,7 +229,7 @@ __global__ __launch_bounds__(256, OCC) void window_dq_f32_kernel(const WindowPar
     __syncthreads();
     if (i + 1 < b.list.n) load(i + 1);
     const int t = b.list.at(i);
-    if (!b.sees.live(t)) continue;
+    if (!b.sees.live(i, t)) continue;
     f32x16 s = rows_dot<D>(ks, q, f32x16{}, l32, h2), dp;
 #pragma unroll
     for (int r = 0; r < 16; ++r) dp[r] = -dl;
