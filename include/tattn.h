@@ -26,7 +26,7 @@
 extern "C" {
 #endif
 
-#define TATTN_ABI_VERSION 2
+#define TATTN_ABI_VERSION 3
 
 /* TATTN_BF16 has no counterpart in the reference, which accepts fp16 and fp32 only
  * (src/tattn/api.py:55-56); it runs the fp16 kernels with bf16 MFMAs and bf16 rounding points. */

@@ -13,7 +13,7 @@ from pathlib import Path
 import torch  # noqa: F401  (must be imported before the library is loaded, see above)
 
 LIB_PATH = Path(__file__).resolve().with_name("libtattn_hip.so")
-ABI_VERSION = 2
+ABI_VERSION = 3
 
 F16, F32, BF16 = 0, 1, 2
 K_FWD, K_BWD_DKDV, K_BWD_DQ = 0, 1, 2
@@ -106,13 +106,13 @@ def load() -> ctypes.CDLL:
                     "(or __graft_entry__.build()) first"
                 )
             lib = ctypes.CDLL(str(LIB_PATH))
+            got = lib.tattn_abi_version()  # first: another version need not have the other names
+            if got != ABI_VERSION:
+                raise RuntimeError(f"{LIB_PATH}: ABI version {got}, expected {ABI_VERSION}")
             for name, (res, args) in _SIGS.items():
                 fn = getattr(lib, name)
                 fn.restype = res
                 fn.argtypes = args
-            got = lib.tattn_abi_version()
-            if got != ABI_VERSION:
-                raise RuntimeError(f"{LIB_PATH}: ABI version {got}, expected {ABI_VERSION}")
             _lib = lib
     return _lib
 
