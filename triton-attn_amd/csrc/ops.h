@@ -84,7 +84,7 @@ struct WindowParams {
   void* dk;
   void* dv;
   float* m;      // [Z, H, N] base-2 log-sum-exp, or null
-  float* delta;  // [Z, H, N]
+  float* delta;  // [Z, H, N], then in fp16 [Z, Hk, window_norm_blocks] largest squared norms of dO's rows
   const int32_t* lens;  // [Z] keys of each sequence, or null: S
   float* part;          // partial rows of a split forward, see window_part_floats; partial dK, dV of the first keys
   int64_t sq[3], sk[3], sv[3], so[3], sd[3], sout[3], sdk[3], sdv[3];
@@ -101,6 +101,8 @@ struct WindowParams {
 inline int64_t window_part_floats(int64_t slices, int64_t rows, int64_t splits, int64_t D) {
   return slices * rows * splits * (D + 2);
 }
+// Blocks of 128 rows (queries with their heads) of a slice, as dQ's workgroups take them.
+__host__ __device__ inline int window_norm_blocks(int64_t N, int64_t G) { return (int)((N * G + 127) / 128); }
 int window_fwd_splits(const WindowParams& p, int D);  // 0: no parts and two row tiles per workgroup
 void window_bwd_parts(WindowParams& p, int D);  // sets splits and parts
 int64_t window_bwd_part_floats(const WindowParams& p, int D);

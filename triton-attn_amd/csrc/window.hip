@@ -414,7 +414,8 @@ __global__ __launch_bounds__(256) void combine_kernel(const float* part, T* out,
 }
 
 // ---- dQ ------------------------------------------------------------------------------------------
-// Rows and key tiles as in the forward; computes delta = rowsum(dO * O) on the way and stores -delta for dK / dV.
+// Rows and key tiles as in the forward; computes delta = rowsum(dO * O) on the way and stores -delta for dK / dV, in float16 also
+// the block's largest norm of a row of dO.
 template <typename T, int D, int RW, int CS, int OCC>
 __global__ __launch_bounds__(RW * CS * 64, OCC) void window_dq_kernel(const WindowParams p) {
   using H = H16<T>;
@@ -423,8 +424,10 @@ __global__ __launch_bounds__(RW * CS * 64, OCC) void window_dq_kernel(const Wind
   using V2 = typename H::V2;
   constexpr int NW = RW * CS, NSD = D / 16, DT = (D + 31) / 32;
   using R = WinRing<D, NW, CS>;
+  constexpr bool LIFT = std::is_same_v<T, f16>;
   __shared__ __attribute__((aligned(1024))) char s0[R::STAGE];
   __shared__ __attribute__((aligned(1024))) char s1[R::STAGE];
+  __shared__ uint32_t norms[LIFT ? NW : 1];
 
   const int tid = threadIdx.x;
   const int lane = tid & 63, h2 = lane >> 5, l32 = lane & 31;
@@ -433,8 +436,9 @@ __global__ __launch_bounds__(RW * CS * 64, OCC) void window_dq_kernel(const Wind
   const float c = p.c;
   int slice, blk;
   if (!window_coord(p.Z * p.Hk, p.nblk, p.head, p.tail, slice, blk)) return;
+  blk = p.nblk - 1 - blk;
   WinRows b;
-  b.init(p, slice, p.nblk - 1 - blk, RW);
+  b.init(p, slice, blk, RW);
   TileList list;
   list.init(b.p0, b.p1, b.last, p.window, p.sinks);
   const int nsteps = (list.n + CS - 1) / CS;
@@ -459,23 +463,31 @@ __global__ __launch_bounds__(RW * CS * 64, OCC) void window_dq_kernel(const Wind
   const int64_t mrow = ((int64_t)b.z * p.H + h) * p.N + n;
   V8 qop[NSD], dop[NSD];
   float dl;
+  int lift = 0;  // dS is scaled by 2^lift
   {
     const T* qs = (const T*)p.q + b.z * p.sq[0] + h * p.sq[1] + n * p.sq[2] + 8 * h2;
     const T* ds = (const T*)p.dout + b.z * p.sd[0] + h * p.sd[1] + n * p.sd[2] + 8 * h2;
     const T* os = (const T*)p.o + b.z * p.so[0] + h * p.so[1] + n * p.so[2] + 8 * h2;
-    float sd[NSD];
+    float sd[NSD], norm = 0.0f;
 #pragma unroll
     for (int s = 0; s < NSD; ++s) {
       const V8 x = *reinterpret_cast<const V8*>(qs + 16 * s), y = *reinterpret_cast<const V8*>(ds + 16 * s);
       qop[s] = live ? x : V8{};
       dop[s] = live ? y : V8{};
       sd[s] = chunk_dot(*reinterpret_cast<const V8*>(os + 16 * s), y);
+      if (LIFT) norm += chunk_dot(dop[s], dop[s]);
+    }
+    if constexpr (LIFT) {
+      const uint32_t bits = __builtin_bit_cast(uint32_t, sum_halves(norm));
+      lift = small_gradient_lift(bits, 60);
+      norms[wu] = max_wave(bits);  // NaN above all
     }
     dl = row_delta(sd);
     if (live && h2 == 0 && cs == 0) p.delta[mrow] = -dl;
     if (!live) dl = 0.0f;
   }
-  const float nm = live ? -p.m[mrow] : 0.0f;
+  const float nm = live ? (float)lift - p.m[mrow] : 0.0f;
+  const float scale = LIFT ? p.scale * unlift_of(lift) : p.scale;
   WinOp<D> at;
   at.init(cs * R::TILE, lane);
   f32x16 dq[DT];
@@ -523,6 +535,14 @@ __global__ __launch_bounds__(RW * CS * 64, OCC) void window_dq_kernel(const Wind
     all_landed_barrier();
   };
   all_landed_barrier();
+  if constexpr (LIFT) {  // for dK / dV
+    if (tid == 0) {
+      uint32_t top = norms[0];
+#pragma unroll
+      for (int k = 1; k < NW; ++k) top = max(top, norms[k]);
+      p.delta[(int64_t)p.Z * p.H * p.N + (int64_t)b.slice * p.nblk + blk] = __builtin_bit_cast(float, top);
+    }
+  }
   int i = 0;
   for (; i + 1 < nsteps; i += 2) {
     step(i, s0, s1);
@@ -541,7 +561,7 @@ __global__ __launch_bounds__(RW * CS * 64, OCC) void window_dq_kernel(const Wind
         if (d0 >= D) continue;
         V4 y;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) y[e] = (T)(dq[u][4 * gr + e] * p.scale);
+        for (int e = 0; e < 4; ++e) y[e] = (T)(dq[u][4 * gr + e] * scale);
         *reinterpret_cast<V4*>(orow + d0) = y;
       }
     return;
@@ -572,7 +592,7 @@ __global__ __launch_bounds__(RW * CS * 64, OCC) void window_dq_kernel(const Wind
       }
       V4 y;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) y[e] = (T)(x[e] * p.scale);
+      for (int e = 0; e < 4; ++e) y[e] = (T)(x[e] * scale);
       *reinterpret_cast<V4*>(orow + d0) = y;
     }
   }
@@ -610,6 +630,27 @@ struct KeyBlocks {
 __device__ __forceinline__ bool key_seen(const WindowParams& p, int off, int key) {
   return key < p.S && (key < p.sinks || off - key < p.window);
 }
+
+// What dS of a block of keys that queries nlo .. nhi see is scaled by (small_gradient_lift), the same for all lanes. Loaded
+// first and looked at once the first tiles are on their way.
+struct KeysLift {
+  const uint32_t* norms;
+  int i, last;
+  uint32_t top;
+  __device__ __forceinline__ KeysLift(const WindowParams& p, int slice, int nlo, int nhi, int lane) {
+    norms = (const uint32_t*)p.delta + (int64_t)p.Z * p.H * p.N + (int64_t)slice * window_norm_blocks(p.N, p.G);
+    i = (nlo * p.G >> 7) + lane;
+    last = (nhi * p.G + p.G - 1) >> 7;
+    top = i <= last ? norms[i] : 0;
+  }
+  __device__ __forceinline__ int lift() {
+    for (i += 64; i <= last; i += 256) {  // four loads at a time
+      const uint32_t a = norms[i], b = norms[min(i + 64, last)], c = norms[min(i + 128, last)], d = norms[min(i + 192, last)];
+      top = max(top, max(max(a, b), max(c, d)));
+    }
+    return small_gradient_lift(max_wave(top), 15);
+  }
+};
 
 template <typename T, int D, int RW, int CS, int OCC>
 __global__ __launch_bounds__(RW * CS * 64, OCC) void window_dkdv_kernel(const WindowParams p) {
@@ -660,6 +701,8 @@ __global__ __launch_bounds__(RW * CS * 64, OCC) void window_dkdv_kernel(const Wi
       for (int i = 0; i < R::PPT; ++i) ld.fetch(rs, stage, x, i, ld.go[i] + (uint32_t)qt * ld.tile_bytes);
     }
   };
+  constexpr bool LIFT = std::is_same_v<T, f16>;
+  KeysLift kl(p, slice, nlo, LIFT ? nhi : -1, lane);
   if (nsteps > 0) issue(s0, 0);
   // Lanes 0-31 fetch M and lanes 32-63 -delta of the wave's tile; zero past the end.
   const float* mdsrc = (h2 ? p.delta : p.m) + ((int64_t)z * p.H + hk * p.G) * p.N;
@@ -668,7 +711,7 @@ __global__ __launch_bounds__(RW * CS * 64, OCC) void window_dkdv_kernel(const Wi
     const int q = k < i1 ? 32 * (qt0 + k % nq) + l32 : p.N;
     return q < p.N ? mdsrc[(int64_t)(k / nq) * p.N + q] : 0.0f;
   };
-  md[wu][0][lane] = nsteps > 0 ? md_load(0) : 0.0f;
+  const float md0 = nsteps > 0 ? md_load(0) : 0.0f;
   const int kt = kb * RW + rw, key = 32 * kt + l32;
   const bool seen = key_seen(p, off, key);
   V8 kop[NSD], vop[NSD];
@@ -683,6 +726,10 @@ __global__ __launch_bounds__(RW * CS * 64, OCC) void window_dkdv_kernel(const Wi
       vop[s] = seen ? b : V8{};
     }
   }
+  // P, and with it dS, is scaled by 2^lift through M.
+  const int by = LIFT ? kl.lift() : 0;
+  const float unlift = unlift_of(by), lift = LIFT && h2 == 0 ? (float)by : 0.0f;
+  md[wu][0][lane] = md0 - lift;
   WinOp<D> at;
   at.init(cs * R::TILE, lane);
   f32x16 dk[DT], dv[DT];
@@ -748,7 +795,7 @@ __global__ __launch_bounds__(RW * CS * 64, OCC) void window_dkdv_kernel(const Wi
       if (q1 >= wk0 && (q0 - wk1 < p.window || wk0 < p.sinks))
         tile(cur, md[wu][par], qt, q0 < wk1 || (q1 - wk0 >= p.window && wk1 >= p.sinks) || 32 * qt + 32 > p.N);
     }
-    md[wu][par ^ 1][lane] = mdn;  // the wave's own rows: no barrier needed
+    md[wu][par ^ 1][lane] = mdn - lift;  // the wave's own rows: no barrier needed
     all_landed_barrier();
   };
   all_landed_barrier();
@@ -786,14 +833,14 @@ __global__ __launch_bounds__(RW * CS * 64, OCC) void window_dkdv_kernel(const Wi
           for (int k = 0; k < CS - 1; ++k) x += (part(rw * (CS - 1) + k) + lane)[(16 * u + r) * 64];
           const int in = 8 * (r >> 2) + 4 * h2 + (r & 3), d = 32 * u + l32;
           if (d >= D) continue;
-          if (parted) fpart[(32 * rw + in) * D + d] = x;
+          if (parted) fpart[(32 * rw + in) * D + d] = x * unlift;
           else if (wk0 + in < p.S) dst[(int64_t)(wk0 + in) * stride + d] = (T)(x * mul);
         }
     }
   };
-  reduce(dk, p.scale, (T*)p.dk + z * p.sdk[0] + hk * p.sdk[1], p.sdk[2], fdst);
+  reduce(dk, p.scale * unlift, (T*)p.dk + z * p.sdk[0] + hk * p.sdk[1], p.sdk[2], fdst);
   __syncthreads();
-  reduce(dv, 1.0f, (T*)p.dv + z * p.sdv[0] + hk * p.sdv[1], p.sdv[2], fdst + 32 * RW * D);
+  reduce(dv, unlift, (T*)p.dv + z * p.sdv[0] + hk * p.sdv[1], p.sdv[2], fdst + 32 * RW * D);
 }
 
 // dK / dV at head dims 64 and 128: two waves per 32-key tile. Over each 32-query tile wave j (role A) computes S = Q K^T,
@@ -840,6 +887,9 @@ __global__ __launch_bounds__(RW * 128, OCC) void window_dkdv_pair_kernel(const W
   const int i0 = (int)((int64_t)total * split / splits), i1 = (int)((int64_t)total * (split + 1) / splits);
   const int n = i1 - i0;
   const int wk0 = 32 * (kb * RW + pr), wk1 = wk0 + 31, key = wk0 + l32;
+  constexpr bool LIFT = std::is_same_v<T, f16>;
+  KeysLift kl(p, slice, nlo, LIFT && role_b ? nhi : -1, lane);
+  int lift = 0;  // dS is scaled by 2^lift
 
   // The wave's operand: K rows (A) or V rows (B).
   const bool seen = key_seen(p, off, key);
@@ -915,7 +965,8 @@ __global__ __launch_bounds__(RW * 128, OCC) void window_dkdv_pair_kernel(const W
   const int full_hi = min((p.N >> 5) - 1, wk1 < p.sinks ? far : (p.window + wk0 - off - 32) >> 5);
 
   auto run = [&](auto role_tag) __attribute__((always_inline)) {
-    constexpr bool RB_ = decltype(role_tag)::value;
+    constexpr int ROLE = decltype(role_tag)::value;  // 0: A, 1: B, 2: B with dS scaled up
+    constexpr bool RB_ = ROLE > 0;
     // S (A) of a stage's tile, or dP - delta (B).
     auto first = [&](f32x16& s, const char* st) __attribute__((always_inline)) {
       if constexpr (RB_) {
@@ -988,6 +1039,10 @@ __global__ __launch_bounds__(RW * 128, OCC) void window_dkdv_pair_kernel(const W
         f32x16 dp;
         V8 ds[2];
         first(dp, stage(IC<I + NST - 1>{}));
+        if constexpr (ROLE == 2) {
+#pragma unroll
+          for (int r = 0; r < 16; ++r) dp[r] *= unlift_of(-lift);
+        }
         dsv(dp, ds, xp);
         grad(ds, stage(IC<I + NST - 1>{}));
       }
@@ -1006,21 +1061,23 @@ __global__ __launch_bounds__(RW * 128, OCC) void window_dkdv_pair_kernel(const W
     fetch(st0);
     if (NST == 4) fetch(st1);
     all_landed_barrier();
-    if (role_b) run(std::true_type{});
-    else run(std::false_type{});
+    if (LIFT && role_b) lift = kl.lift();  // while A takes its first tile
+    if (!role_b) run(IC<0>{});
+    else if (!LIFT || lift == 0) run(IC<1>{});
+    else run(IC<2>{});
     all_landed_barrier();
   }
 
   // Every wave has passed the last barrier and nothing is in flight. C register r of a lane: key 8 (r / 4) + 4 h2 + r % 4 of
   // the tile, column 32 u + l32. A part's sums go out in float32; otherwise the tile is turned into rows through LDS.
-  const float mul = role_b ? p.scale : 1.0f;
+  const float unlift = role_b ? unlift_of(lift) : 1.0f, mul = role_b ? p.scale * unlift : 1.0f;
   if (parted) {
     float* dst = p.part + ((int64_t)slice * kbs.first(kbs.parted()) + item) * (2 * 32 * RW * D) +
                  (role_b ? 0 : 32 * RW * D) + (int64_t)32 * pr * D;
 #pragma unroll
     for (int u = 0; u < DT; ++u)
 #pragma unroll
-      for (int r = 0; r < 16; ++r) dst[(8 * (r >> 2) + 4 * h2 + (r & 3)) * D + 32 * u + l32] = acc[u][r];
+      for (int r = 0; r < 16; ++r) dst[(8 * (r >> 2) + 4 * h2 + (r & 3)) * D + 32 * u + l32] = acc[u][r] * unlift;
     return;
   }
   T* dst = role_b ? (T*)p.dk + z * p.sdk[0] + hk * p.sdk[1] : (T*)p.dv + z * p.sdv[0] + hk * p.sdv[1];

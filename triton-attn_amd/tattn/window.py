@@ -64,22 +64,23 @@ _plans: dict[tuple, tuple] = {}
 
 def _plan(q, k, v, window, sinks, lens) -> tuple:
     """Checks a call; which of q, k, v are copied, the strides of inputs and output (None where one is copied), the float32
-    values of workspace of forward and backward, and the sizes among the launches' arguments (None: nothing to see)."""
+    values of workspace of forward and backward and of delta, and the sizes among the launches' arguments (None: nothing to see)."""
     _check(q, k, v, window, sinks, lens)
     _require_gpu(q)
     copies = tuple(_tiles_apart(t) for t in (q, k, v))
     z, h, n, d = q.shape
     hk, s = k.shape[1:3]
     if q.numel() == 0 or s == 0:
-        return copies, None, 0, 0, None
+        return copies, None, 0, 0, 0, None
     sizes = (z, h, hk, n, s, d, min(window, s), min(sinks, s))
     half = q.dtype != torch.float32  # float32 is never split
+    norms = z * hk * ((n * (h // hk) + 127) // 128) if q.dtype == torch.float16 else 0
     return (copies, None if any(copies) else strides(q, k, v, torch.empty_like(q)), _workspace(False, sizes) if half else 0,
-            _workspace(True, sizes) if half and lens is None else 0, (*sizes, _DTYPES[q.dtype]))
+            _workspace(True, sizes) if half and lens is None else 0, z * h * n + norms, (*sizes, _DTYPES[q.dtype]))
 
 
 def _forward(q, k, v, plan, scale, lens, save_lse) -> tuple[torch.Tensor, torch.Tensor | None]:
-    copies, held, floats, _, sizes = plan
+    copies, held, floats, _, _, sizes = plan
     given = q, k, v
     q, k, v = aligned(q, copies[0]), aligned(k, copies[1]), aligned(v, copies[2])
     o = torch.empty_like(q)
@@ -98,12 +99,12 @@ def _forward(q, k, v, plan, scale, lens, save_lse) -> tuple[torch.Tensor, torch.
 
 
 def _backward(q, k, v, o, m, do, plan, scale) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
-    floats, sizes = plan[3:]
+    floats, rows, sizes = plan[3:]
     q, k, v, o, do = _tiles(q), _tiles(k), _tiles(v), _tiles(o), _tiles(do)
     dq, dk, dv = torch.empty_like(q), torch.empty_like(k), torch.empty_like(v)
     if sizes is None:
         return dq.zero_(), dk.zero_(), dv.zero_()
-    delta = torch.empty_like(m)
+    delta = m.new_empty(rows)
     work = q.new_empty(floats, dtype=torch.float32) if floats else None
     _, st = strides(q, k, v, o, do, dq, dk, dv)
     with _on_device(q):
