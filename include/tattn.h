@@ -244,6 +244,9 @@ int tattn_norm_rope_bwd(const void* q, const void* k, const void* q_weight, cons
  */
 int tattn_window_workspace(int backward, int64_t Z, int64_t H, int64_t Hk, int64_t N, int64_t S, int64_t D, int64_t window,
                            int64_t sinks, int64_t* floats);
+/* What a 16-bit forward of these sizes runs: 0 for workgroups of four row tiles, otherwise one row tile per workgroup and the
+ * number of parts that its keys are cut into; -1 for sizes that it refuses. */
+int tattn_window_picked(int64_t Z, int64_t H, int64_t Hk, int64_t N, int64_t S, int64_t D, int64_t window, int64_t sinks);
 int tattn_window_fwd(const void* q, const void* k, const void* v, void* o, float* m, const int32_t* lens, float* workspace,
                      const int64_t q_strides[4], const int64_t k_strides[4], const int64_t v_strides[4],
                      const int64_t o_strides[4], int64_t Z, int64_t H, int64_t Hk, int64_t N, int64_t S, int64_t D,

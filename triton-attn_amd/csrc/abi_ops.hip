@@ -295,6 +295,12 @@ int tattn_window_workspace(int backward, int64_t Z, int64_t H, int64_t Hk, int64
   return TATTN_OK;
 }
 
+int tattn_window_picked(int64_t Z, int64_t H, int64_t Hk, int64_t N, int64_t S, int64_t D, int64_t window, int64_t sinks) {
+  WindowParams p{};
+  if (window_common(p, Z, H, Hk, N, S, D, window, sinks, true)) return -1;
+  return window_fwd_splits(p, (int)D);
+}
+
 int tattn_window_fwd(const void* q, const void* k, const void* v, void* o, float* m, const int32_t* lens, float* workspace,
                      const int64_t q_strides[4], const int64_t k_strides[4], const int64_t v_strides[4],
                      const int64_t o_strides[4], int64_t Z, int64_t H, int64_t Hk, int64_t N, int64_t S, int64_t D,

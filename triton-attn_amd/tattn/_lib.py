@@ -25,7 +25,8 @@ EXPORTS = (
     "tattn_bwd_preprocess", "tattn_bwd_dkdv", "tattn_bwd_dq", "tattn_bwd", "tattn_bwd_layouts", "tattn_bwd_noalloc",
     "tattn_num_configs", "tattn_config_desc", "tattn_pick_config", "tattn_picked",
     "tattn_page_tables", "tattn_cache4_write", "tattn_cache4_read",
-    "tattn_norm_rope_fwd", "tattn_norm_rope_bwd", "tattn_window_workspace", "tattn_window_fwd", "tattn_window_bwd",
+    "tattn_norm_rope_fwd", "tattn_norm_rope_bwd",
+    "tattn_window_workspace", "tattn_window_picked", "tattn_window_fwd", "tattn_window_bwd",
     "tattn_cache4_attention_workspace", "tattn_cache4_attention",
 )
 
@@ -80,6 +81,7 @@ _SIGS = {
     "tattn_cache4_attention_workspace": (_I, [_I64] * 8 + [ctypes.POINTER(_I64)]),
     "tattn_cache4_attention": (_I, [_P] * 7 + [_STR4] * 2 + [_I64] * 10 + [_I, _F, _P]),
     "tattn_window_workspace": (_I, [_I] + [_I64] * 8 + [ctypes.POINTER(_I64)]),
+    "tattn_window_picked": (_I, [_I64] * 8),
     "tattn_window_fwd": (_I, [_P] * 7 + [_STR4] * 4 + [_I64] * 8 + [_I, _F, _P]),
     "tattn_window_bwd": (_I, [_P] * 11 + [_STR4] * 8 + [_I64] * 8 + [_I, _F, _P]),
     "tattn_norm_rope_bwd": (_I, [_P] * 14 + [_STR4] * 6 + [_I64] * 7 + [_I, _I, _I, _F, _P]),
