@@ -1,0 +1,86 @@
+"""Arguments of the operators around attention that are no plain numbers or carry derivatives: refused before anything reaches a
+GPU, or taken at their value in every call."""
+
+import pytest
+import torch
+import torch.autograd.forward_ad as forward_ad
+
+import tattn
+
+
+def half(*shape):
+    return torch.zeros(*shape, dtype=torch.float16)
+
+
+def i32(*x):
+    return torch.tensor(x, dtype=torch.int32)
+
+
+def window(**kw):
+    a = dict(q=half(2, 4, 8, 32), k=half(2, 2, 8, 32), v=half(2, 2, 8, 32), window=4)
+    a.update(kw)
+    return tattn.window_attention(**a)
+
+
+def norm_rope(**kw):
+    a = dict(q=torch.zeros(2, 4, 8, 32), k=torch.zeros(2, 2, 8, 32), q_weight=torch.ones(32), k_weight=torch.ones(32),
+             cos=torch.ones(8, 16), sin=torch.ones(8, 16))
+    a.update(kw)
+    return tattn.qk_norm_rope(**a)
+
+
+def cache():
+    return tattn.Cache4.empty(3, 16, 2, 64, dtype=torch.float16, device="cpu")
+
+
+def attend(**kw):
+    a = dict(q=half(2, 4, 64), cache=cache(), tables=torch.zeros(2, 3, dtype=torch.int32), lens=i32(0, 0))
+    a.update(kw)
+    return tattn.cache4_attention(**a)
+
+
+def tables(**kw):
+    a = dict(lens=i32(3, 0), new_tokens=i32(1, 5), tables=torch.zeros(2, 4, dtype=torch.int32), free_pages=i32(5, 6, 7),
+             page_size=16, tokens=8)
+    a.update(kw)
+    return tattn.page_tables(**a)
+
+
+# ---- sizes ---------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("call,bad", [
+    (window, dict(window=2.5)), (window, dict(sinks=1.5)), (window, dict(window="4")), (window, dict(sinks=None)),
+    (window, dict(window=torch.tensor(2.5))), (window, dict(window=torch.tensor([1, 2]))), (window, dict(window=float("nan"))),
+    (attend, dict(window=2.5)), (attend, dict(sinks=0.5)), (tables, dict(page_size=16.5)), (tables, dict(tokens=8.5)),
+])
+def test_sizes_are_whole_numbers(call, bad):
+    with pytest.raises(ValueError, match="must be a whole number"):
+        call(**bad)
+
+
+@pytest.mark.parametrize("call,good", [
+    (window, dict(window=4.0)), (window, dict(sinks=True)), (window, dict(window=torch.tensor(4))), (attend, dict(window=3.0)),
+    (tables, dict(page_size=16.0, tokens=torch.tensor(8))),
+])
+def test_whole_numbers_of_other_types_pass_the_checks(call, good):
+    with pytest.raises(RuntimeError, match="gfx950"):
+        call(**good)
+
+
+@pytest.mark.gpu
+def test_sizes_in_tensors_are_read_in_every_call():
+    if not torch.cuda.is_available():
+        pytest.skip("no GPU")
+    g = torch.Generator().manual_seed(0)
+    q, k, v = (torch.randn(1, 2, 40, 32, generator=g).to("cuda", torch.float16) for _ in range(3))
+    size, first = torch.tensor(4), torch.tensor(0)
+    for w, s in ((4, 0), (9, 0), (9, 3)):
+        size.fill_(w)
+        first.fill_(s)
+        assert torch.equal(tattn.window_attention(q, k, v, size, first), tattn.window_attention(q, k, v, w, s))
+    cos, sin = (torch.rand(40, 16, generator=g).cuda() for _ in range(2))
+    ones, turn = torch.ones(32, dtype=torch.float16, device="cuda"), torch.tensor(False)
+    for il in (False, True):
+        turn.fill_(il)
+        got = tattn.qk_norm_rope(q, k, ones, ones, cos, sin, interleaved=turn)
+        assert torch.equal(got[0], tattn.qk_norm_rope(q, k, ones, ones, cos, sin, interleaved=il)[0])

@@ -17,6 +17,19 @@ def dtype_name(dtype: torch.dtype) -> str:
     return str(dtype).removeprefix("torch.")
 
 
+def whole(name: str, x) -> int:
+    """x's value now as a plain int, fit to be kept in a key: numbers of other types, and tensors, may change or compare by identity."""
+    if type(x) is int:
+        return x
+    try:
+        n = int(x)
+    except (TypeError, ValueError):
+        n = None
+    if n is None or n != x:
+        raise ValueError(f"{name} must be a whole number, got {x!r}")
+    return n
+
+
 def check_index(name: str, t: torch.Tensor, dtype: torch.dtype, shape: tuple) -> None:
     if t.dtype != dtype or tuple(t.shape) != shape:
         raise ValueError(f"{name} must be {dtype_name(dtype)} of shape {list(shape)}, got {dtype_name(t.dtype)} {list(t.shape)}")

@@ -123,6 +123,7 @@ def qk_norm_rope(
     NaN. Outputs keep the order of their input's strides. Differentiable in q, k and both weights (cos and sin get no
     gradients); float16, bfloat16 or float32, all arithmetic in float32, each result rounded once. Any batch, head and
     sequence strides are read in place."""
+    interleaved = bool(interleaved)
     key = (layouts(q, k, q_weight, k_weight, cos, sin, positions), interleaved)
     plan = _plans.get(key)
     if plan is None:

@@ -18,7 +18,7 @@ from typing import NamedTuple
 import torch
 
 from tattn import _lib
-from tattn._args import aligned, check_index, layouts, remember, rows_apart, same_device, strides
+from tattn._args import aligned, check_index, layouts, remember, rows_apart, same_device, strides, whole
 from tattn.api import _on_device, _require_gpu, _stream
 
 _DTYPES = {torch.float16: _lib.F16, torch.bfloat16: _lib.BF16}
@@ -67,6 +67,7 @@ def page_tables(lens: torch.Tensor, new_tokens: torch.Tensor, tables: torch.Tens
     tokens past it are not placed (no slot, no page). lens and free_pages are not changed: the caller adds new_tokens
     and skips `taken` pages. Where free pages or a table row run out, tokens have slot -1 (and `taken` exceeds the list).
     """
+    page_size, tokens = whole("page_size", page_size), whole("tokens", tokens)
     if not 0 <= tokens < (1 << 31) - 4096:
         raise ValueError(f"tokens out of range: {tokens}")
     key = (layouts(lens, new_tokens, tables, free_pages), page_size)
@@ -219,6 +220,7 @@ def cache4_attention(
     that sees nothing gives zeros. sm_scale defaults to 1 / sqrt(head_dim). For serving: refuses a q that requires gradients."""
     if q.requires_grad and torch.is_grad_enabled():
         raise ValueError("cache4_attention has no gradients: call it under torch.no_grad()")
+    window, sinks = None if window is None else whole("window", window), whole("sinks", sinks)
     key = (layouts(q, tables, lens), cache.layout, window, sinks)
     plan = _attention_plans.get(key)
     if plan is None:

@@ -16,7 +16,7 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from tattn import _lib
-from tattn._args import aligned, check_index, layouts, remember, rows_apart, same_device, strides
+from tattn._args import aligned, check_index, layouts, remember, rows_apart, same_device, strides, whole
 from tattn.api import _DTYPES, _on_device, _require_gpu, _stream
 
 
@@ -145,13 +145,14 @@ def window_attention(
     zeros. sm_scale defaults to 1 / sqrt(dim). Differentiable in q, k and v without lens; with lens the call is for serving
     and refuses inputs that require gradients. A key or value that is infinite or NaN makes the rows that see it
     NaN, and may make NaN of rows up to 64 positions before it or after its window that do not see it."""
+    window, sinks = whole("window", window), whole("sinks", sinks)
     key = (layouts(q, k, v, lens), window, sinks)
     plan = _plans.get(key)
     needs = (q.requires_grad or k.requires_grad or v.requires_grad) and torch.is_grad_enabled()
     if needs and lens is not None:
         raise ValueError("no gradients with lens: call it under torch.no_grad(), or without lens")
     if plan is None:
-        plan = remember(_plans, key, _plan(q, k, v, int(window), int(sinks), lens))
+        plan = remember(_plans, key, _plan(q, k, v, window, sinks, lens))
     scale = float(sm_scale) if sm_scale is not None else 1.0 / math.sqrt(q.shape[3])
     if needs:
         return _Window.apply(q, k, v, plan, scale)
