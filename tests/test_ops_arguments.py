@@ -84,3 +84,36 @@ def test_sizes_in_tensors_are_read_in_every_call():
         turn.fill_(il)
         got = tattn.qk_norm_rope(q, k, ones, ones, cos, sin, interleaved=turn)
         assert torch.equal(got[0], tattn.qk_norm_rope(q, k, ones, ones, cos, sin, interleaved=il)[0])
+
+
+# ---- forward-mode derivatives ----------------------------------------------------------------------
+
+def dual(t):
+    return forward_ad.make_dual(t, torch.ones_like(t))
+
+
+@pytest.mark.parametrize("call,arg,t", [
+    (window, "q", half(2, 4, 8, 32)), (window, "k", half(2, 2, 8, 32)), (window, "v", half(2, 2, 8, 32)),
+    (norm_rope, "q", torch.zeros(2, 4, 8, 32)), (norm_rope, "k", torch.zeros(2, 2, 8, 32)),
+    (norm_rope, "q_weight", torch.ones(32)), (norm_rope, "k_weight", torch.ones(32)),
+    (norm_rope, "cos", torch.ones(8, 16)), (norm_rope, "sin", torch.ones(8, 16)), (attend, "q", half(2, 4, 64)),
+])
+def test_tangents_are_refused_not_lost(call, arg, t):
+    made = {"cache": cache()} if call is attend else {}
+    with forward_ad.dual_level():
+        with pytest.raises(ValueError, match="forward-mode"):
+            call(**{arg: dual(t)}, **made)
+        with torch.no_grad(), pytest.raises(ValueError, match="forward-mode"):
+            call(**{arg: dual(t)}, **made)
+        with pytest.raises(RuntimeError, match="gfx950"):  # none of its arguments has one
+            call()
+    with pytest.raises(ValueError, match="forward-mode"):
+        torch.func.jvp(lambda x: call(**{arg: x}, **made), (t,), (t,))
+
+
+def test_tangents_of_what_a_cache_is_given_are_refused():
+    k = half(5, 2, 64)
+    with forward_ad.dual_level():
+        for a in ((dual(k), k), (k, dual(k))):
+            with pytest.raises(ValueError, match="forward-mode"):
+                tattn.cache4_write(cache(), *a, torch.zeros(5, dtype=torch.int64))

@@ -5,6 +5,7 @@ from __future__ import annotations
 import ctypes
 
 import torch
+from torch.autograd import forward_ad
 
 
 def same_device(first: torch.Tensor, **others: torch.Tensor | None) -> None:
@@ -15,6 +16,12 @@ def same_device(first: torch.Tensor, **others: torch.Tensor | None) -> None:
 
 def dtype_name(dtype: torch.dtype) -> str:
     return str(dtype).removeprefix("torch.")
+
+
+def no_tangents(*ts: torch.Tensor | None) -> None:
+    """Refuses dual tensors: the kernels would lose their tangents. Outside a level of forward-mode AD there are none."""
+    if forward_ad._current_level >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in ts):
+        raise ValueError("no forward-mode derivatives: the tensors must not carry tangents")
 
 
 def whole(name: str, x) -> int:

@@ -1,7 +1,8 @@
 """Norms of queries and keys for each head, with the position rotation in the same pass.
 
     q, k = qk_norm_rope(q, k, q_weight, k_weight, cos, sin, positions)
-    o = attention(q, k, v, causal=True)
+    o = attention(q, k, v, causal=True)                              # as many key heads as query heads
+    o = window_attention(q, k, v, window=k.shape[2])                 # fewer key heads; or a true window
 
 No counterpart in the reference.
 """
@@ -14,7 +15,7 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from tattn import _lib
-from tattn._args import aligned, check_index, layouts, remember, rows, rows_apart, same_device, strides
+from tattn._args import aligned, check_index, layouts, no_tangents, remember, rows, rows_apart, same_device, strides
 from tattn.api import _DTYPES, _on_device, _require_gpu, _stream
 
 
@@ -121,8 +122,9 @@ def qk_norm_rope(
     when `interleaved`, turned by the angle with cosine cos[position, i] and sine sin[position, i] (float32
     [any, dim / 2]). positions: int32 [seq] or [batch, seq]; None: 0, 1, ... A position outside the tables gives a row of
     NaN. Outputs keep the order of their input's strides. Differentiable in q, k and both weights (cos and sin get no
-    gradients); float16, bfloat16 or float32, all arithmetic in float32, each result rounded once. Any batch, head and
-    sequence strides are read in place."""
+    gradients; forward-mode derivatives are refused); float16, bfloat16 or float32, all arithmetic in float32, each result
+    rounded once. Any batch, head and sequence strides are read in place."""
+    no_tangents(q, k, q_weight, k_weight, cos, sin)
     interleaved = bool(interleaved)
     key = (layouts(q, k, q_weight, k_weight, cos, sin, positions), interleaved)
     plan = _plans.get(key)

@@ -18,7 +18,7 @@ from typing import NamedTuple
 import torch
 
 from tattn import _lib
-from tattn._args import aligned, check_index, layouts, remember, rows_apart, same_device, strides, whole
+from tattn._args import aligned, check_index, layouts, no_tangents, remember, rows_apart, same_device, strides, whole
 from tattn.api import _on_device, _require_gpu, _stream
 
 _DTYPES = {torch.float16: _lib.F16, torch.bfloat16: _lib.BF16}
@@ -133,7 +133,9 @@ _write_plans: dict[tuple, tuple] = {}
 def cache4_write(cache: Cache4, k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor) -> None:
     """Writes keys and values [tokens, kv_heads, head_dim] (the cache's dtype, any token and head strides) into
     `slots` (int64 [tokens], as page_tables gives them). Slots outside the cache, such as a padded token's -1,
-    are skipped. No two tokens of a call may share a slot."""
+    are skipped. No two tokens of a call may share a slot. Gradients do not flow through the cache; forward-mode derivatives
+    are refused."""
+    no_tangents(k, v)
     key = (layouts(k, v, slots), cache.layout)
     plan = _write_plans.get(key)
     if plan is None:
@@ -217,7 +219,9 @@ def cache4_attention(
     as page_tables keeps them, lens int32 [requests]: tokens each request sees, the newest one included (clamped to what its
     table row holds). With a window only the last `window` tokens and the first `sinks` are seen, and pages without a seen
     token are not looked up (they may have been given away). Tokens on a page number outside the cache are hidden; a request
-    that sees nothing gives zeros. sm_scale defaults to 1 / sqrt(head_dim). For serving: refuses a q that requires gradients."""
+    that sees nothing gives zeros. sm_scale defaults to 1 / sqrt(head_dim). For serving: refuses a q that requires gradients or
+    carries forward-mode ones."""
+    no_tangents(q)
     if q.requires_grad and torch.is_grad_enabled():
         raise ValueError("cache4_attention has no gradients: call it under torch.no_grad()")
     window, sinks = None if window is None else whole("window", window), whole("sinks", sinks)

@@ -16,7 +16,7 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from tattn import _lib
-from tattn._args import aligned, check_index, layouts, remember, rows_apart, same_device, strides, whole
+from tattn._args import aligned, check_index, layouts, no_tangents, remember, rows_apart, same_device, strides, whole
 from tattn.api import _DTYPES, _on_device, _require_gpu, _stream
 
 
@@ -143,8 +143,10 @@ def window_attention(
     j < sinks. len is keys, or lens[batch] (int32, on the GPU, clamped to [0, keys]) where a cache is filled to
     different lengths; what lies behind it, or before every window, reaches no result. Rows at positions below 0 give
     zeros. sm_scale defaults to 1 / sqrt(dim). Differentiable in q, k and v without lens; with lens the call is for serving
-    and refuses inputs that require gradients. A key or value that is infinite or NaN makes the rows that see it
-    NaN, and may make NaN of rows up to 64 positions before it or after its window that do not see it."""
+    and refuses inputs that require gradients. Forward-mode derivatives are refused. A key or value that is infinite or NaN
+    makes the rows that see it NaN, and may make NaN of rows up to 64 positions before it or after its window that do not see
+    it."""
+    no_tangents(q, k, v)
     window, sinks = whole("window", window), whole("sinks", sinks)
     key = (layouts(q, k, v, lens), window, sinks)
     plan = _plans.get(key)
