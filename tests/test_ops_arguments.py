@@ -34,9 +34,9 @@ def cache():
 
 
 def attend(**kw):
-    a = dict(q=half(2, 4, 64), cache=cache(), tables=torch.zeros(2, 3, dtype=torch.int32), lens=i32(0, 0))
+    a = dict(q=half(2, 4, 64), tables=torch.zeros(2, 3, dtype=torch.int32), lens=i32(0, 0))
     a.update(kw)
-    return tattn.cache4_attention(**a)
+    return tattn.cache4_attention(**a, **({} if "cache" in kw else {"cache": cache()}))
 
 
 def tables(**kw):
