@@ -117,3 +117,12 @@ def test_tangents_of_what_a_cache_is_given_are_refused():
         for a in ((dual(k), k), (k, dual(k))):
             with pytest.raises(ValueError, match="forward-mode"):
                 tattn.cache4_write(cache(), *a, torch.zeros(5, dtype=torch.int64))
+
+
+# ---- a cache without heads -------------------------------------------------------------------------
+
+def test_a_cache_has_a_head():
+    with pytest.raises(ValueError, match="at least one kv head"):
+        tattn.Cache4.empty(3, 16, 0, 64, dtype=torch.float16, device="cpu")
+    with pytest.raises(ValueError, match="at least one kv head"):
+        tattn.Cache4(torch.zeros(3, 0, 2, 16, 32, dtype=torch.uint8), torch.zeros(3, 0, 2, 16, 2, dtype=torch.uint8), torch.float16)

@@ -106,6 +106,8 @@ class Cache4:
         pages, heads, _, page, half = codes.shape
         if 2 * half not in (32, 64, 128):
             raise ValueError(f"head dim must be 32, 64 or 128, got {2 * half}")
+        if heads < 1:
+            raise ValueError("expected at least one kv head")
         check_index("scales", scales, torch.uint8, (pages, heads, 2, page, half // 16))
         _check_page_size(page)
         if dtype not in _DTYPES:
