@@ -97,9 +97,8 @@ struct WinRows {
   int z, hk, slice, len, off;
   int rows;      // N * G
   int tile0;     // first row tile of the workgroup
-  int p0, p1;    // positions of the workgroup's rows
+  int p0, p1;    // positions of the workgroup's rows; p1 is also the last key any of them sees
   int last;      // position of the last row tile's first row
-  int top;       // last key any of them sees
   __device__ __forceinline__ void init(const WindowParams& p, int slice_, int blk, int rw) {
     slice = slice_;
     z = slice / p.Hk;
@@ -111,7 +110,6 @@ struct WinRows {
     p0 = off + (32 * tile0) / p.G;
     p1 = off + min(32 * (tile0 + rw) - 1, rows - 1) / p.G;
     last = off + min(32 * (tile0 + rw - 1), rows - 1) / p.G;
-    top = p1;
   }
 };
 
@@ -181,7 +179,7 @@ __global__ __launch_bounds__(RW * CS * 64, OCC) void window_fwd_kernel(const Win
       ld.second ? win_rsrc<T, D>(p.v, b.z * p.sv[0] + b.hk * p.sv[1], b.len, p.sv[2])
                 : win_rsrc<T, D>(p.k, b.z * p.sk[0] + b.hk * p.sk[1], b.len, p.sk[2]);
   auto issue = [&](char* stage, int step) __attribute__((always_inline)) {
-    fetch_keys<D, NW, CS>(ld, rs, stage, list, i0 + step * CS, i1, b.top, p.sinks);
+    fetch_keys<D, NW, CS>(ld, rs, stage, list, i0 + step * CS, i1, b.p1, p.sinks);
   };
   if (nsteps > 0) issue(s0, 0);
 
@@ -416,23 +414,22 @@ __global__ __launch_bounds__(256) void combine_kernel(const float* part, T* out,
 // ---- dQ ------------------------------------------------------------------------------------------
 // Rows and key tiles as in the forward; computes delta = rowsum(dO * O) on the way and stores -delta for dK / dV, in float16 also
 // the block's largest norm of a row of dO.
-template <typename T, int D, int RW, int CS, int OCC>
-__global__ __launch_bounds__(RW * CS * 64, OCC) void window_dq_kernel(const WindowParams p) {
+template <typename T, int D, int RW, int OCC>
+__global__ __launch_bounds__(RW * 64, OCC) void window_dq_kernel(const WindowParams p) {
   using H = H16<T>;
   using V8 = typename H::V8;
   using V4 = typename H::V4;
   using V2 = typename H::V2;
-  constexpr int NW = RW * CS, NSD = D / 16, DT = (D + 31) / 32;
-  using R = WinRing<D, NW, CS>;
+  constexpr int NSD = D / 16, DT = (D + 31) / 32;
+  using R = WinRing<D, RW, 1>;
   constexpr bool LIFT = std::is_same_v<T, f16>;
   __shared__ __attribute__((aligned(1024))) char s0[R::STAGE];
   __shared__ __attribute__((aligned(1024))) char s1[R::STAGE];
-  __shared__ uint32_t norms[LIFT ? NW : 1];
+  __shared__ uint32_t norms[LIFT ? RW : 1];
 
   const int tid = threadIdx.x;
   const int lane = tid & 63, h2 = lane >> 5, l32 = lane & 31;
   const int wu = (int)uniform32((uint32_t)(tid >> 6));
-  const int rw = wu / CS, cs = wu % CS;
   const float c = p.c;
   int slice, blk;
   if (!window_coord(p.Z * p.Hk, p.nblk, p.head, p.tail, slice, blk)) return;
@@ -441,19 +438,18 @@ __global__ __launch_bounds__(RW * CS * 64, OCC) void window_dq_kernel(const Wind
   b.init(p, slice, blk, RW);
   TileList list;
   list.init(b.p0, b.p1, b.last, p.window, p.sinks);
-  const int nsteps = (list.n + CS - 1) / CS;
 
-  WinLoader<D, NW, CS> ld;
+  WinLoader<D, RW, 1> ld;
   ld.init(p.sk[2], p.sv[2], wu, lane);
   const __amdgpu_buffer_rsrc_t rs =
       ld.second ? win_rsrc<T, D>(p.v, b.z * p.sv[0] + b.hk * p.sv[1], b.len, p.sv[2])
                 : win_rsrc<T, D>(p.k, b.z * p.sk[0] + b.hk * p.sk[1], b.len, p.sk[2]);
-  auto issue = [&](char* stage, int step) __attribute__((always_inline)) {
-    fetch_keys<D, NW, CS>(ld, rs, stage, list, step * CS, list.n, b.top, p.sinks);
+  auto issue = [&](char* stage, int i) __attribute__((always_inline)) {
+    fetch_keys<D, RW, 1>(ld, rs, stage, list, i, list.n, b.p1, p.sinks);
   };
-  if (nsteps > 0) issue(s0, 0);
+  if (list.n > 0) issue(s0, 0);
 
-  const int tile0 = 32 * (b.tile0 + rw);
+  const int tile0 = 32 * (b.tile0 + wu);
   const int row = tile0 + l32;
   const bool live = row < b.rows;
   const int n = (live ? row : 0) / p.G, g = (live ? row : 0) % p.G, h = b.hk * p.G + g;
@@ -483,13 +479,13 @@ __global__ __launch_bounds__(RW * CS * 64, OCC) void window_dq_kernel(const Wind
       norms[wu] = max_wave(bits);  // NaN above all
     }
     dl = row_delta(sd);
-    if (live && h2 == 0 && cs == 0) p.delta[mrow] = -dl;
+    if (live && h2 == 0) p.delta[mrow] = -dl;
     if (!live) dl = 0.0f;
   }
   const float nm = live ? (float)lift - p.m[mrow] : 0.0f;
   const float scale = LIFT ? p.scale * unlift_of(lift) : p.scale;
   WinOp<D> at;
-  at.init(cs * R::TILE, lane);
+  at.init(0, lane);
   f32x16 dq[DT];
 #pragma unroll
   for (int u = 0; u < DT; ++u) dq[u] = f32x16{};
@@ -526,12 +522,9 @@ __global__ __launch_bounds__(RW * CS * 64, OCC) void window_dq_kernel(const Wind
       }
   };
   auto step = [&](int i, char* cur, char* nxt) __attribute__((always_inline)) {
-    if (i + 1 < nsteps) issue(nxt, i + 1);
-    const int k = i * CS + cs;
-    if (k < list.n) {
-      const int t = list.at(k);
-      if (sees.live(k, t)) tile(cur, t);
-    }
+    if (i + 1 < list.n) issue(nxt, i + 1);
+    const int t = list.at(i);
+    if (sees.live(i, t)) tile(cur, t);
     all_landed_barrier();
   };
   all_landed_barrier();
@@ -539,63 +532,30 @@ __global__ __launch_bounds__(RW * CS * 64, OCC) void window_dq_kernel(const Wind
     if (tid == 0) {
       uint32_t top = norms[0];
 #pragma unroll
-      for (int k = 1; k < NW; ++k) top = max(top, norms[k]);
+      for (int k = 1; k < RW; ++k) top = max(top, norms[k]);
       p.delta[(int64_t)p.Z * p.H * p.N + (int64_t)b.slice * p.nblk + blk] = __builtin_bit_cast(float, top);
     }
   }
   int i = 0;
-  for (; i + 1 < nsteps; i += 2) {
+  for (; i + 1 < list.n; i += 2) {
     step(i, s0, s1);
     step(i + 1, s1, s0);
   }
-  if (i < nsteps) step(i, s0, s1);
+  if (i < list.n) step(i, s0, s1);
 
-  if constexpr (CS == 1) {
-    if (!live) return;
-    T* orow = (T*)p.out + b.z * p.sout[0] + h * p.sout[1] + n * p.sout[2];
-#pragma unroll
-    for (int u = 0; u < DT; ++u)
-#pragma unroll
-      for (int gr = 0; gr < 4; ++gr) {
-        const int d0 = 32 * u + 8 * gr + 4 * h2;
-        if (d0 >= D) continue;
-        V4 y;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) y[e] = (T)(dq[u][4 * gr + e] * scale);
-        *reinterpret_cast<V4*>(orow + d0) = y;
-      }
-    return;
-  }
-  constexpr int PART = DT * 16 * 64 * 4;
-  constexpr int PER = R::STAGE / PART;
-  static_assert(CS == 1 || 2 * PER >= NW, "partials fit the stages");
-  auto part = [&](int k) { return (TATTN_LDS float*)(k < PER ? s0 + k * PART : s1 + (k - PER) * PART); };
-  {
-    TATTN_LDS float* dst = part(wu) + lane;
-#pragma unroll
-    for (int u = 0; u < DT; ++u)
-#pragma unroll
-      for (int r = 0; r < 16; ++r) dst[(16 * u + r) * 64] = dq[u][r];
-  }
-  __syncthreads();
   if (!live) return;
   T* orow = (T*)p.out + b.z * p.sout[0] + h * p.sout[1] + n * p.sout[2];
-  for (int gr = cs; gr < DT * 4; gr += CS) {
-    const int d0 = 8 * gr + 4 * h2;
-    if (d0 < D) {
-      f32x4 x = f32x4{};
 #pragma unroll
-      for (int k = 0; k < CS; ++k) {
-        const TATTN_LDS float* src = part(rw * CS + k) + lane + 4 * gr * 64;
+  for (int u = 0; u < DT; ++u)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) x[e] += src[64 * e];
-      }
+    for (int gr = 0; gr < 4; ++gr) {
+      const int d0 = 32 * u + 8 * gr + 4 * h2;
+      if (d0 >= D) continue;
       V4 y;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) y[e] = (T)(x[e] * scale);
+      for (int e = 0; e < 4; ++e) y[e] = (T)(dq[u][4 * gr + e] * scale);
       *reinterpret_cast<V4*>(orow + d0) = y;
     }
-  }
 }
 
 // ---- dK / dV -------------------------------------------------------------------------------------
@@ -1180,7 +1140,7 @@ int bwd_d(WindowParams p, hipStream_t st) {
   p.nblk = (int)((rows + 32 * S::RW - 1) / (32 * S::RW));
   p.tail = window_row_tail(p, 32 * S::RW, p.nblk);
   if ((rc = window_grid(slices, p.nblk, p.tail, &blocks))) return rc;
-  window_dq_kernel<T, D, S::RW, 1, D >= 64 ? 2 : 4><<<dim3(blocks), dim3(S::RW * 64), 0, st>>>(p);
+  window_dq_kernel<T, D, S::RW, D >= 64 ? 2 : 4><<<dim3(blocks), dim3(S::RW * 64), 0, st>>>(p);
   if ((rc = check_launch("tattn_window_bwd"))) return rc;
   const KeyBlocks kbs(RW, p);
   p.head = kbs.sink_blocks * p.splits;  // the longest: 84 -> 73 us for the whole backward at 4/4 x 16,384 x 64, window 512
