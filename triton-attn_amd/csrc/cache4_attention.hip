@@ -14,8 +14,12 @@
 // The next tile's codes and the page numbers of the one after are on their way meanwhile; waves meet only at the end. A
 // workgroup of four waves takes `chunk` consecutive tiles of one request and key head; requests of many tiles are cut into
 // equal chunks, whatever their lengths, and joined by combine_kernel. 64 requests of up to 16,384 tokens with 32/8 heads x 128
-// take 147 us, 4.9 TB/s of the cache's bytes, a large copy's rate (32 x 32 x 16 instructions, with twice the unused columns:
-// 163 us).
+// take 147-153 us, 4.7-4.9 TB/s of the cache's bytes, where a kernel that only reads has 6.3 (32 x 32 x 16 instructions, with
+// twice the unused columns: 163 us).
+//
+// Roundings: K and V are what the cache holds, exact in either type; P is rounded to it as the second product's operand, its sum
+// taken from the rounded values; scores, maxima, sums and accumulators are float32 (relative to 64 bits, in norm, in bf16:
+// 2.3e-3, a float32 computation rounded once 1.7e-3).
 #include <algorithm>
 
 #include "fp4.h"

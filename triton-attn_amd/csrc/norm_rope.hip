@@ -13,7 +13,8 @@
 // lane holds 16 bytes of the row's lower half and the 16 bytes D/2 further, so either kind of pair lies in one lane
 // and the row's sum takes at most four lane swaps. A lane group takes up to four heads of one token, whose
 // position, cosines, sines and weights it loads once, and has all their loads in flight together. At 4 x 32/8 x 4,096 x 128
-// in bf16 the forward takes 61 us (5.5 TB/s) and the backward 104 and 4 us (4.8 TB/s); a large copy has 4.8 TB/s.
+// in bf16 the forward takes 61-65 us (5.3-5.5 TB/s) and the backward 104 and 5 us (4.8 TB/s), in float32 124 (5.5) and
+// 203 us (5.0); a kernel that copies has 5.7 TB/s.
 #include <algorithm>
 
 #include "common.h"

@@ -146,7 +146,8 @@ __global__ __launch_bounds__(256) void page_tables_kernel(const TablesParams p) 
 //
 // Bound by bytes: 16 values a thread (two 16-byte loads, one 8-byte store), a workgroup takes one head of
 // 2048 / D consecutive tokens, keys and values, so that its codes and exponents fill whole lines of a page. 16,384 tokens
-// of 8 heads x 128 in bf16 are written in 13.6 us and read in 16.6 (6.2 and 5.1 TB/s of their 85 MB; a large copy has 4.8).
+// of 8 heads x 128 in bf16 are written in 13.6-14.5 us and read in 16.5 (5.9-6.2 and 5.1 TB/s of their 85 MB; a kernel that copies has
+// 5.7, one that writes 6.0).
 
 // Row x of a workgroup's 256 / (D / 16) rows: token, K (0) or V (1), and the thread's 16 values.
 template <int D>

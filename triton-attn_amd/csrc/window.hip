@@ -9,14 +9,22 @@
 // Rows that nobody in the workgroup sees (before the window, behind the last key) are fetched from beyond the end of
 // the buffer, which reads as zero: whatever a cache holds there cannot reach a sum.
 //
+// Roundings: the operands of the second products, P and dS, are rounded to the element type, as the matrix instruction takes them
+// (what a second operand for the rest would add: as many products again), P's sum is taken from the rounded values, and
+// delta from the stored O. Scores, maxima, sums and accumulators are float32. That leaves errors 1.1 to 1.5 times those
+// of a float32 computation rounded once (relative to 64 bits, in norm, all outputs: 4 x 16 x 4,096 x 64 in fp16 3.1e-4 for 2.1e-4,
+// 11 x 12/4 x 1,500 x 128 in bf16 2.5e-3 for 1.7e-3). dS in fp16 is scaled first (small_gradient_lift).
+//
 // Bound by the issue of matrix and vector instructions and by the latency of a tile's chain (scores, exponentials, second product),
 // which the 8 to 16 waves of a CU overlap only in part: at head dim 64 the forward keeps the matrix cores busy 31% and the vector
-// units 49% of the time. us (rate of the products that count, for dQ and dK / dV of the backward's ten per forward four):
-//                                                  forward        dQ    dK / dV
-//   4 x 16 x 4,096 x 64 fp16, window 1,024, 4 sinks   100 (600 TF)  124   199 (both: 466 TF)
-//   11 x 12/4 x 1,500 x 128 bf16, window 500           74 (570 TF)  103   135 (both: 443 TF)
-//   1 x 32/8 x 16,384 x 128 bf16, window 4,096        877 (1,100 TF)
-//   32 x 32/8 x 128, one token, window 2,048           51 (5.2 TB/s of the keys and values)
+// units 49% of the time. us (rate of the products that count); whole calls, and in a profiler's trace, which clocks lower,
+// the kernels one by one:
+//                                                    call         forward       with gradients  |  traced: forward   dQ   dK / dV
+//   4 x 16 x 4,096 x 64 fp16, window 1,024, 4 first keys            89 (680 TF)   380 (556 TF)  |           102    126     204
+//   11 x 12/4 x 1,500 x 128 bf16, window 500                        64 (660 TF)   283 (522 TF)  |            79    109     143
+//   1 x 32/8 x 16,384 x 128 bf16, window 4,096, 4 first keys       892 (1,080 TF)               |         1,003
+//   32 x 32/8 x 128, one token, window 2,048, 4 first keys          51 (5.2 TB/s of the keys and values)  |  49
+// Each row was measured in one session; sessions differ by up to 6%.
 #include <algorithm>
 #include <type_traits>
 

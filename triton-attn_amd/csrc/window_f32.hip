@@ -9,9 +9,9 @@
 // 16-byte LDS read feeds four instructions. Tiles are read in perm32 order, which gives a lane's 16 results the
 // keys (or queries) kappa(r, h): what the second product needs as its operand, with no lane exchange and no rounding.
 // Bound by the matrix instruction: 2,048 multiply-adds in 64 cycles, 157 TFLOP/s in all. 4 x 16 x 4,096 x 64 at window 1,024
-// takes 0.70 ms forward (87 TFLOP/s) and 3.2 ms backward (67 with its seven products); 11 x 12/4 x 1,500 x 128 at window
-// 512 0.53 and 2.1 ms. Keys are not split between workgroups, so few rows over many keys leave the chip partly idle
-// (8 x 32/8 x 128, one query over a window of 4,096: 0.61 ms).
+// takes 0.58 ms forward (104 TFLOP/s) and 2.9 ms backward (52 with the five products that count, 73 with its seven);
+// 11 x 12/4 x 1,500 x 128 at window 512 0.51 and 1.9 ms. Keys are not split between workgroups, so few rows over many keys
+// leave the chip partly idle (8 x 32/8 x 128, one query over a window of 4,096: 0.62 ms).
 #include "window.h"
 
 namespace tattn {
