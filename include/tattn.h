@@ -239,8 +239,8 @@ int tattn_norm_rope_bwd(const void* q, const void* k, const void* q_weight, cons
  * m: [Z, H, N] float32 base-2 log-sum-exp for the backward, or null. workspace: float32, 16-byte aligned, as many
  * as tattn_window_workspace gives for the same sizes (may be null where that is 0, and in TATTN_F32); calls that may
  * overlap need one each.
- * The backward (no lens, S >= N) sums dk and dv over the heads of a group, without atomics; delta: float32 scratch of Z H N values,
- * in TATTN_F16 with Z Hk ceil(N (H / Hk) / 128) more.
+ * The backward (no lens, S >= N) sums dk and dv over the heads of a group, without atomics; delta: float32 scratch, 8-byte aligned, of
+ * Z H N values, in TATTN_F16 of Z H N rounded up to an even number and 2 Z Hk ceil(N (H / Hk) / 128) more.
  */
 int tattn_window_workspace(int backward, int64_t Z, int64_t H, int64_t Hk, int64_t N, int64_t S, int64_t D, int64_t window,
                            int64_t sinks, int64_t* floats);

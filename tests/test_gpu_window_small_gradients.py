@@ -134,3 +134,19 @@ def test_small_gradients_of_values_far_above_one(d):
     for name, got in zip(("dq", "dk", "dv"), gradients(q, k, v, do, 100, 4, d ** -0.5)):
         assert got.isfinite().all()
         close(name, got, *want[name])
+
+
+@pytest.mark.parametrize("window", [2, 100, 5000])
+@pytest.mark.parametrize("d", [16, 32, 64, 128])
+def test_small_gradients_of_values_near_the_largest(d, window):
+    """Values of 60,000 either way, along the gradients: dS of their size is not scaled past float16's largest."""
+    q, k, v, do = make(1, 4, 2, 400, 400, d, torch.float16, seed=45)
+    sign = torch.where(torch.arange(400, device=DEV) % 3 == 0, 1.0, -1.0)[None, None, :, None]
+    v = (60000 * sign).expand_as(v).to(torch.float16).contiguous()
+    v[:, :, 300:] /= 1024  # ordinary ones
+    do = torch.full_like(do, 2.0 ** -12)
+    do[:, :, 100:150] *= 2.0 ** -3
+    want = bounds(q, k, v, do, window, 4, d ** -0.5)
+    for name, got in zip(("dq", "dk", "dv"), gradients(q, k, v, do, window, 4, d ** -0.5)):
+        assert got.isfinite().all(), name
+        close(name, got, *want[name])

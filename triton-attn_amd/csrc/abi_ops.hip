@@ -334,7 +334,7 @@ int tattn_window_bwd(const void* q, const void* k, const void* v, const void* o,
       (rc = check_tiles("v", v, v_strides, S, D, dtype, p.sv)) || (rc = check_tiles("o", o, o_strides, N, D, dtype, p.so)) ||
       (rc = check_tiles("do", dout, do_strides, N, D, dtype, p.sd)) || (rc = check_tiles("dq", dq, dq_strides, N, D, dtype, p.sout)) ||
       (rc = check_tiles("dk", dk, dk_strides, S, D, dtype, p.sdk)) || (rc = check_tiles("dv", dv, dv_strides, S, D, dtype, p.sdv)) ||
-      (rc = check_ptr("m", m, 1, 4)) || (rc = check_ptr("delta", delta, 1, 4)))
+      (rc = check_ptr("m", m, 1, 4)) || (rc = check_ptr("delta", delta, 1, 8)))
     return rc;
   p.splits = p.parts = 1;
   if (dtype != TATTN_F32) window_bwd_parts(p, (int)D);
@@ -342,6 +342,7 @@ int tattn_window_bwd(const void* q, const void* k, const void* v, const void* o,
   p.q = q; p.k = k; p.v = v; p.o = o; p.dout = dout; p.out = dq; p.dk = dk; p.dv = dv;
   p.m = const_cast<float*>(m);
   p.delta = delta;
+  p.norms = delta + (Z * H * N + 1) / 2 * 2;
   p.part = workspace;
   p.c = window_exponent_scale(sm_scale);
   p.scale = sm_scale;

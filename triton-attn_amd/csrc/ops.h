@@ -84,7 +84,8 @@ struct WindowParams {
   void* dk;
   void* dv;
   float* m;      // [Z, H, N] base-2 log-sum-exp, or null
-  float* delta;  // [Z, H, N], then in fp16 [Z, Hk, window_norm_blocks] largest squared norms of dO's rows
+  float* delta;  // [Z, H, N]
+  float* norms;  // fp16 backward: [Z, Hk, window_norm_blocks, 2], largest squared norm of dO's rows, largest |delta|
   const int32_t* lens;  // [Z] keys of each sequence, or null: S
   float* part;          // partial rows of a split forward, see window_part_floats; partial dK, dV of the first keys
   int64_t sq[3], sk[3], sv[3], so[3], sd[3], sout[3], sdk[3], sdv[3];

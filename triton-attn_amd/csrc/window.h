@@ -105,12 +105,12 @@ struct WaveTiles {
 };
 
 // In float16 dS is rounded to steps of 2^-24 below 2^-14, where that of small losses lies. It is scaled up by a power of two
-// before it is rounded, 2^lift with lift = -floor(log2 |dO|) from the (largest) squared norm of the rows: |dS| <= 2 |dO| max|v|
-// stays finite for values up to |v| = 2^14. (4 x 16 x 4,096 x 64, window 1,024, dO near 1: 0.3% of the step's time.)
-__device__ __forceinline__ int small_gradient_lift(uint32_t norm2, int most) {  // the norm's float32 bits
-  const int e = (int)(norm2 >> 23) - 127;  // floor(log2); NaN and infinity: 128
-  return min(max(-(e >> 1), 0), most);
-}
+// before it is rounded, 2^lift with lift = -floor(log2 |dO|), |dO| the (largest) norm of the rows. |dS| <= |dO| |v| + |delta| must
+// stay finite: dK takes its keys' |v| and the rows' |delta| into account, dQ, whose rows see many keys, starts over without a
+// factor where a sum is not finite. Of a step's time this is 0.2% at 4 x 16 x 4,096 x 64, window 1,024 (1.7% where dO is small), 1% at
+// 16/4 x 32,768 x 64, window 128, and 3% at 4 x 16 x 8,192 x 32, window 512, whose workgroups are short.
+__device__ __forceinline__ int norm_exponent(uint32_t norm2) { return ((int)(norm2 >> 23) - 127) >> 1; }  // of a squared norm's bits; NaN: 64
+__device__ __forceinline__ int small_gradient_lift(int exponent, int most) { return min(max(-exponent, 0), most); }
 __device__ __forceinline__ float unlift_of(int lift) { return __builtin_bit_cast(float, (uint32_t)(127 - lift) << 23); }
 
 // Over the wave, uniform.

@@ -421,7 +421,7 @@ __global__ __launch_bounds__(256) void combine_kernel(const float* part, T* out,
 
 // ---- dQ ------------------------------------------------------------------------------------------
 // Rows and key tiles as in the forward; computes delta = rowsum(dO * O) on the way and stores -delta for dK / dV, in float16 also
-// the block's largest norm of a row of dO.
+// the largest squared norm of the block's rows of dO and its largest |delta|.
 template <typename T, int D, int RW, int OCC>
 __global__ __launch_bounds__(RW * 64, OCC) void window_dq_kernel(const WindowParams p) {
   using H = H16<T>;
@@ -433,7 +433,7 @@ __global__ __launch_bounds__(RW * 64, OCC) void window_dq_kernel(const WindowPar
   constexpr bool LIFT = std::is_same_v<T, f16>;
   __shared__ __attribute__((aligned(1024))) char s0[R::STAGE];
   __shared__ __attribute__((aligned(1024))) char s1[R::STAGE];
-  __shared__ uint32_t norms[LIFT ? RW : 1];
+  __shared__ uint32_t norms[3][LIFT ? RW : 1];  // per wave: largest squared norm, |delta|, whether a row is lifted
 
   const int tid = threadIdx.x;
   const int lane = tid & 63, h2 = lane >> 5, l32 = lane & 31;
@@ -468,6 +468,7 @@ __global__ __launch_bounds__(RW * 64, OCC) void window_dq_kernel(const WindowPar
   V8 qop[NSD], dop[NSD];
   float dl;
   int lift = 0;  // dS is scaled by 2^lift
+  uint32_t top = 0;
   {
     const T* qs = (const T*)p.q + b.z * p.sq[0] + h * p.sq[1] + n * p.sq[2] + 8 * h2;
     const T* ds = (const T*)p.dout + b.z * p.sd[0] + h * p.sd[1] + n * p.sd[2] + 8 * h2;
@@ -483,20 +484,24 @@ __global__ __launch_bounds__(RW * 64, OCC) void window_dq_kernel(const WindowPar
     }
     if constexpr (LIFT) {
       const uint32_t bits = __builtin_bit_cast(uint32_t, sum_halves(norm));
-      lift = small_gradient_lift(bits, 60);
-      norms[wu] = max_wave(bits);  // NaN above all
+      lift = small_gradient_lift(norm_exponent(bits), 60);
+      top = max_wave(bits);  // NaN above all
+      norms[0][wu] = top;
+      norms[2][wu] = __builtin_amdgcn_ballot_w64(lift > 0) != 0;
     }
     dl = row_delta(sd);
     if (live && h2 == 0) p.delta[mrow] = -dl;
     if (!live) dl = 0.0f;
+    if constexpr (LIFT) {  // delta counts where all rows are small
+      norms[1][wu] = 0;
+      if (norm_exponent(top) < 0) norms[1][wu] = max_wave(__builtin_bit_cast(uint32_t, __builtin_fabsf(dl)));
+    }
   }
-  const float nm = live ? (float)lift - p.m[mrow] : 0.0f;
-  const float scale = LIFT ? p.scale * unlift_of(lift) : p.scale;
+  const float m = live ? p.m[mrow] : 0.0f;
+  float nm = live ? (float)lift - m : 0.0f;
   WinOp<D> at;
   at.init(0, lane);
   f32x16 dq[DT];
-#pragma unroll
-  for (int u = 0; u < DT; ++u) dq[u] = f32x16{};
 
   const float hidden = hidden_score(c);
   auto tile = [&](const char* st, int t) __attribute__((always_inline)) {
@@ -536,20 +541,40 @@ __global__ __launch_bounds__(RW * 64, OCC) void window_dq_kernel(const WindowPar
     all_landed_barrier();
   };
   all_landed_barrier();
-  if constexpr (LIFT) {  // for dK / dV
-    if (tid == 0) {
-      uint32_t top = norms[0];
+  uint32_t lifted = 0;
+  if constexpr (LIFT) {
+    if (tid < 2) {  // for dK / dV
+      top = norms[tid][0];
 #pragma unroll
-      for (int k = 1; k < RW; ++k) top = max(top, norms[k]);
-      p.delta[(int64_t)p.Z * p.H * p.N + (int64_t)b.slice * p.nblk + blk] = __builtin_bit_cast(float, top);
+      for (int k = 1; k < RW; ++k) top = max(top, norms[tid][k]);
+      p.norms[2 * ((int64_t)b.slice * p.nblk + blk) + tid] = __builtin_bit_cast(float, top);
     }
+#pragma unroll
+    for (int k = 0; k < RW; ++k) lifted |= norms[2][k];
+    lifted = uniform32(lifted);
   }
-  int i = 0;
-  for (; i + 1 < list.n; i += 2) {
-    step(i, s0, s1);
-    step(i + 1, s1, s0);
+  for (;;) {
+#pragma unroll
+    for (int u = 0; u < DT; ++u) dq[u] = f32x16{};
+    int i = 0;
+    for (; i + 1 < list.n; i += 2) {
+      step(i, s0, s1);
+      step(i + 1, s1, s0);
+    }
+    if (i < list.n) step(i, s0, s1);
+    if (!LIFT || !lifted) break;
+    float zero = 0.0f;  // times every sum: NaN where one is not finite
+#pragma unroll
+    for (int u = 0; u < DT; ++u)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) zero = __builtin_fmaf(dq[u][r], 0.0f, zero);
+    if (!__syncthreads_or(lift > 0 && zero != 0.0f)) break;
+    lifted = lift = 0;
+    nm = -m;
+    issue(s0, 0);
+    all_landed_barrier();
   }
-  if (i < list.n) step(i, s0, s1);
+  const float scale = LIFT ? p.scale * unlift_of(lift) : p.scale;
 
   if (!live) return;
   T* orow = (T*)p.out + b.z * p.sout[0] + h * p.sout[1] + n * p.sout[2];
@@ -602,21 +627,31 @@ __device__ __forceinline__ bool key_seen(const WindowParams& p, int off, int key
 // What dS of a block of keys that queries nlo .. nhi see is scaled by (small_gradient_lift), the same for all lanes. Loaded
 // first and looked at once the first tiles are on their way.
 struct KeysLift {
-  const uint32_t* norms;
+  const u32x2* norms;
   int i, last;
-  uint32_t top;
+  u32x2 top;  // squared norm of dO, |delta|
   __device__ __forceinline__ KeysLift(const WindowParams& p, int slice, int nlo, int nhi, int lane) {
-    norms = (const uint32_t*)p.delta + (int64_t)p.Z * p.H * p.N + (int64_t)slice * window_norm_blocks(p.N, p.G);
+    norms = reinterpret_cast<const u32x2*>(p.norms) + (int64_t)slice * window_norm_blocks(p.N, p.G);
     i = (nlo * p.G >> 7) + lane;
     last = (nhi * p.G + p.G - 1) >> 7;
-    top = i <= last ? norms[i] : 0;
+    top = i <= last ? norms[i] : u32x2{};
   }
-  __device__ __forceinline__ int lift() {
+  template <typename V8, int N>
+  __device__ __forceinline__ int lift(const V8 (&v)[N]) {  // v: the lane's half of its key's value
     for (i += 64; i <= last; i += 256) {  // four loads at a time
-      const uint32_t a = norms[i], b = norms[min(i + 64, last)], c = norms[min(i + 128, last)], d = norms[min(i + 192, last)];
-      top = max(top, max(max(a, b), max(c, d)));
+      const u32x2 a = norms[i], b = norms[min(i + 64, last)], c = norms[min(i + 128, last)], d = norms[min(i + 192, last)];
+#pragma unroll
+      for (int k = 0; k < 2; ++k) top[k] = max(top[k], max(max(a[k], b[k]), max(c[k], d[k])));
     }
-    return small_gradient_lift(max_wave(top), 15);
+    const int row = norm_exponent(max_wave(top[0]));
+    if (row >= 0) return 0;
+    float norm = 0.0f;
+#pragma unroll
+    for (int s = 0; s < N; ++s) norm += chunk_dot(v[s], v[s]);
+    const int key = norm_exponent(max_wave(__builtin_bit_cast(uint32_t, sum_halves(norm))));
+    const int delta = (int)(max_wave(top[1]) >> 23) - 127;
+    // |dS| < 2^(row + key + 2) + 2^(delta + 1)
+    return min(small_gradient_lift(row, 15), max(min(12 - row - key, 13 - delta), 0));
   }
 };
 
@@ -695,7 +730,7 @@ __global__ __launch_bounds__(RW * CS * 64, OCC) void window_dkdv_kernel(const Wi
     }
   }
   // P, and with it dS, is scaled by 2^lift through M.
-  const int by = LIFT ? kl.lift() : 0;
+  const int by = LIFT ? kl.lift(vop) : 0;
   const float unlift = unlift_of(by), lift = LIFT && h2 == 0 ? (float)by : 0.0f;
   md[wu][0][lane] = md0 - lift;
   WinOp<D> at;
@@ -1028,8 +1063,8 @@ __global__ __launch_bounds__(RW * 128, OCC) void window_dkdv_pair_kernel(const W
   if (n > 0) {
     fetch(st0);
     if (NST == 4) fetch(st1);
+    if (LIFT && role_b) lift = kl.lift(kv);
     all_landed_barrier();
-    if (LIFT && role_b) lift = kl.lift();  // while A takes its first tile
     if (!role_b) run(IC<0>{});
     else if (!LIFT || lift == 0) run(IC<1>{});
     else run(IC<2>{});

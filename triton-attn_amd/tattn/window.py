@@ -74,7 +74,7 @@ def _plan(q, k, v, window, sinks, lens) -> tuple:
         return copies, None, 0, 0, 0, None
     sizes = (z, h, hk, n, s, d, min(window, s), min(sinks, s))
     half = q.dtype != torch.float32  # float32 is never split
-    norms = z * hk * ((n * (h // hk) + 127) // 128) if q.dtype == torch.float16 else 0
+    norms = 1 + 2 * z * hk * ((n * (h // hk) + 127) // 128) if q.dtype == torch.float16 else 0
     return (copies, None if any(copies) else strides(q, k, v, torch.empty_like(q)), _workspace(False, sizes) if half else 0,
             _workspace(True, sizes) if half and lens is None else 0, z * h * n + norms, (*sizes, _DTYPES[q.dtype]))
 
