@@ -26,7 +26,7 @@
 extern "C" {
 #endif
 
-#define TATTN_ABI_VERSION 3
+#define TATTN_ABI_VERSION 4
 
 /* TATTN_BF16 has no counterpart in the reference, which accepts fp16 and fp32 only
  * (src/tattn/api.py:55-56); it runs the fp16 kernels with bf16 MFMAs and bf16 rounding points. */
@@ -272,6 +272,66 @@ int tattn_cache4_attention(const void* q, void* o, const uint8_t* codes, const u
                            const int32_t* lens, float* workspace, const int64_t q_strides[2], const int64_t o_strides[2],
                            int64_t table_stride, int64_t R, int64_t H, int64_t Hk, int64_t D, int64_t width, int64_t pages,
                            int64_t page_size, int64_t window, int64_t sinks, int dtype, float sm_scale, void* stream);
+
+/*
+ * Attention over keys of another length, an encoder's states, without a causal mask, grouped heads: q, o [Z, H, N, D], k, v
+ * [Z, Hk, S, D], H a multiple of Hk (query head h reads key head h / (H / Hk)), any dtype, D = 16, 32, 64 or 128. Every query of
+ * sequence z sees its first lens[z] keys (clamped to [0, S]; lens null: S); where that is none, rows of o are zeros. What lies at
+ * or past lens[z] reaches nothing. Strides per tensor (z, h, n, d) in elements, unit d stride, 16-byte aligned rows; rows of k
+ * and v, and in the backward of all tensors, do not overlap and a head of them spans less than 2 GiB.
+ *
+ * m: [Z, H, N] float32 base-2 log-sum-exp for the backward, or null. workspace: float32, 16-byte aligned, as many as
+ * tattn_cross_workspace gives for the same sizes (null where 0); calls that may overlap need one each.
+ * The backward sums dk and dv over the heads of a group, without atomics; keys at or past lens[z] get zeros.
+ */
+int tattn_cross_workspace(int backward, int64_t Z, int64_t H, int64_t Hk, int64_t N, int64_t S, int64_t D, int dtype,
+                          int64_t* floats);
+int tattn_cross_fwd(const void* q, const void* k, const void* v, void* o, float* m, const int32_t* lens, float* workspace,
+                    const int64_t q_strides[4], const int64_t k_strides[4], const int64_t v_strides[4],
+                    const int64_t o_strides[4], int64_t Z, int64_t H, int64_t Hk, int64_t N, int64_t S, int64_t D, int dtype,
+                    float sm_scale, void* stream);
+int tattn_cross_bwd(const void* q, const void* k, const void* v, const void* o, const void* dout, void* dq, void* dk, void* dv,
+                    const float* m, const int32_t* lens, float* workspace, const int64_t q_strides[4],
+                    const int64_t k_strides[4], const int64_t v_strides[4], const int64_t o_strides[4],
+                    const int64_t do_strides[4], const int64_t dq_strides[4], const int64_t dk_strides[4],
+                    const int64_t dv_strides[4], int64_t Z, int64_t H, int64_t Hk, int64_t N, int64_t S, int64_t D, int dtype,
+                    float sm_scale, void* stream);
+
+/*
+ * Attention of the newest N tokens of sequences behind shared prefixes (TATTN_F16 or TATTN_BF16; D = 16, 32, 64 or 128): q, o
+ * [groups * members, H, N, D], prefix_k, prefix_v [groups, Hk, P, D], k, v [groups * members, Hk, S, D]. Sequence z belongs to
+ * group z / members. Its query n is at position lens[z] - N + n (lens clamped to [0, S]) of its own keys and sees all
+ * prefix_lens[group] keys of the prefix (clamped to [0, P]; null: P) and its own keys up to its position; at a position below 0 it
+ * sees nothing and its row is zeros. P and S may be 0. Strides and workspace as above (tattn_prefix_workspace).
+ */
+int tattn_prefix_workspace(int64_t groups, int64_t members, int64_t H, int64_t Hk, int64_t N, int64_t P, int64_t S, int64_t D,
+                           int64_t* floats);
+int tattn_prefix_attention(const void* q, const void* prefix_k, const void* prefix_v, const void* k, const void* v, void* o,
+                           const int32_t* prefix_lens, const int32_t* lens, float* workspace, const int64_t q_strides[4],
+                           const int64_t pk_strides[4], const int64_t pv_strides[4], const int64_t k_strides[4],
+                           const int64_t v_strides[4], const int64_t o_strides[4], int64_t groups, int64_t members, int64_t H,
+                           int64_t Hk, int64_t N, int64_t P, int64_t S, int64_t D, int dtype, float sm_scale, void* stream);
+
+/*
+ * The rotation of tattn_norm_rope_* by positions on several axes: pair i of a token is turned by the angle whose cosine and sine
+ * are cos[x][i], sin[x][i] (float32 [R, D / 2], contiguous) with x the token's position on axis axes[i]. axes: host array of
+ * D / 2 entries, each in [0, num_axes), num_axes <= 8, or -1 for a pair that is not turned. positions: [num_axes, N] (pos_stride
+ * 0) or [num_axes, Z, N], axis_stride and pos_stride apart. A position outside [0, R) makes the pairs of its axis NaN. Without
+ * weights (both null) there is no norm: eps is not read, the backward reads no q and k and gives no gradients of weights.
+ */
+int tattn_rope_axes_fwd(const void* q, const void* k, const void* q_weight, const void* k_weight, const float* cos,
+                        const float* sin, const int32_t* positions, const int32_t* axes, void* q_out, void* k_out,
+                        const int64_t q_strides[4], const int64_t k_strides[4], const int64_t qo_strides[4],
+                        const int64_t ko_strides[4], int64_t num_axes, int64_t axis_stride, int64_t pos_stride, int64_t Z,
+                        int64_t H, int64_t Hk, int64_t N, int64_t D, int64_t R, int dtype, int w_dtype, int interleaved,
+                        float eps, void* stream);
+int tattn_rope_axes_bwd(const void* q, const void* k, const void* q_weight, const void* k_weight, const float* cos,
+                        const float* sin, const int32_t* positions, const int32_t* axes, const void* dq_out,
+                        const void* dk_out, void* dq, void* dk, void* dq_weight, void* dk_weight, float* workspace,
+                        const int64_t q_strides[4], const int64_t k_strides[4], const int64_t dqo_strides[4],
+                        const int64_t dko_strides[4], const int64_t dq_strides[4], const int64_t dk_strides[4],
+                        int64_t num_axes, int64_t axis_stride, int64_t pos_stride, int64_t Z, int64_t H, int64_t Hk, int64_t N,
+                        int64_t D, int64_t R, int dtype, int w_dtype, int interleaved, float eps, void* stream);
 
 #ifdef __cplusplus
 }

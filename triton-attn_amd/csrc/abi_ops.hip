@@ -133,6 +133,57 @@ int check_tiles(const char* name, const void* ptr, const int64_t* st, int64_t ro
   return TATTN_OK;
 }
 
+// Sizes of attention over keys of another length; sequences z belong to Zs groups of B.
+int cross_common(CrossParams& p, int64_t Zs, int64_t B, int64_t H, int64_t Hk, int64_t N, int64_t S, int64_t D, int64_t least) {
+  int rc;
+  if (D != 16 && D != 32 && D != 64 && D != 128)
+    return set_error(TATTN_E_ARG, "head dim must be 16, 32, 64 or 128, got %lld", (long long)D);
+  if ((rc = check_count("batch", Zs)) || (rc = check_count("batch", B)) || (rc = check_count("heads", H)) ||
+      (rc = check_count("length", N)) || (rc = check_count("key length", S)))
+    return rc;
+  if (Zs < 1 || B < 1 || H < 1 || N < 1 || S < least) return set_error(TATTN_E_ARG, "sizes must be positive");
+  if (Hk < 1 || H % Hk) return set_error(TATTN_E_ARG, "%lld heads do not share %lld key heads evenly", (long long)H, (long long)Hk);
+  if ((double)B * (double)H * (double)N > 1073741824.0 || (double)Zs * (double)B * (double)H * (double)((N + 31) / 32) > 67108864.0 ||
+      (double)Zs * (double)Hk * (double)((S + 127) / 128) > 67108864.0)
+    return set_error(TATTN_E_ARG, "too many rows: %lld x %lld x %lld over %lld keys", (long long)(Zs * B), (long long)H,
+                     (long long)N, (long long)S);
+  p.Zs = (int32_t)Zs; p.B = (int32_t)B; p.H = (int32_t)H; p.Hk = (int32_t)Hk; p.G = (int32_t)(H / Hk);
+  p.N = (int32_t)N; p.S = (int32_t)S;
+  return TATTN_OK;
+}
+
+// A tensor whose rows are read or written one by one: strides (z, h, n).
+int check_lone_rows(const char* name, const void* ptr, const int64_t* st, int dtype, int64_t (&out)[3]) {
+  int rc;
+  if ((rc = check_ptr(name, ptr, 1, 16)) || (rc = check_rows(name, st, 3, dtype == TATTN_F32 ? 4 : 2))) return rc;
+  for (int i = 0; i < 3; ++i) out[i] = st[i];
+  return TATTN_OK;
+}
+
+// Axes of pairs and positions, after norm_rope_common.
+int rope_axes_common(RopeAxesParams& p, const int32_t* axes, const int32_t* positions, int64_t num_axes, int64_t axis_stride,
+                     int64_t D, int64_t rows) {
+  if (num_axes < 1 || num_axes > 8) return set_error(TATTN_E_ARG, "there must be 1 to 8 axes, got %lld", (long long)num_axes);
+  if (!axes) return set_error(TATTN_E_ARG, "axes is a null pointer");
+  if (rows > 0 && !positions) return set_error(TATTN_E_ARG, "positions is a null pointer");
+  p.quads = 1;
+  for (int i = 0; i < (int)D / 2; ++i) {
+    if (axes[i] < -1 || axes[i] >= num_axes)
+      return set_error(TATTN_E_ARG, "axis of pair %d must be -1 to %lld, got %d", i, (long long)num_axes - 1, (int)axes[i]);
+    p.axes[i / 2] |= (uint8_t)((axes[i] < 0 ? kNoAxis : (uint32_t)axes[i]) << (i % 2 * 4));
+    if (axes[i] != axes[i / 4 * 4]) p.quads = 0;
+  }
+  p.axis_stride = axis_stride;
+  p.sign = 1.0f;
+  return TATTN_OK;
+}
+
+// Both weights or none; without, a stand-in passes the checks of the norm.
+int check_weights(const void* qw, const void* kw) {
+  if ((qw == nullptr) != (kw == nullptr)) return set_error(TATTN_E_ARG, "give both weights or neither");
+  return TATTN_OK;
+}
+
 // Scores to base-2 exponents. A scale of 0 becomes one so small that all exponents are 0 for finite scores below 1e22, because
 // hidden keys are marked by scores whose scaled value is -inf.
 float window_exponent_scale(float sm_scale) { return sm_scale == 0.0f ? 1.0e-30f : sm_scale * kLog2e; }
@@ -382,6 +433,177 @@ int tattn_cache4_attention(const void* q, void* o, const uint8_t* codes, const u
   p.pages = (int32_t)pages;
   p.c = window_exponent_scale(sm_scale);
   return launch_cache4_attention(p, (int)D, dtype, (hipStream_t)stream);
+}
+
+int tattn_cross_workspace(int backward, int64_t Z, int64_t H, int64_t Hk, int64_t N, int64_t S, int64_t D, int dtype,
+                          int64_t* floats) {
+  CrossParams p{};
+  int rc;
+  if (!floats) return set_error(TATTN_E_ARG, "floats is a null pointer");
+  if ((rc = cross_common(p, Z, 1, H, Hk, N, S, D, 1)) || (rc = check_dtype(dtype))) return rc;
+  if (backward) {
+    cross_bwd_plan(p, (int)D, dtype);
+    *floats = cross_bwd_floats(p, (int)D, dtype);
+  } else {
+    cross_fwd_plan(p, (int)D, dtype);
+    *floats = p.splits > 1 ? cross_part_floats(p.slices(), p.rows(), p.splits, D) : 0;
+  }
+  return TATTN_OK;
+}
+
+int tattn_cross_fwd(const void* q, const void* k, const void* v, void* o, float* m, const int32_t* lens, float* workspace,
+                    const int64_t q_strides[4], const int64_t k_strides[4], const int64_t v_strides[4],
+                    const int64_t o_strides[4], int64_t Z, int64_t H, int64_t Hk, int64_t N, int64_t S, int64_t D, int dtype,
+                    float sm_scale, void* stream) {
+  CrossParams p{};
+  int rc;
+  if ((rc = cross_common(p, Z, 1, H, Hk, N, S, D, 1)) || (rc = check_dtype(dtype)) ||
+      (rc = check_lone_rows("q", q, q_strides, dtype, p.sq)) || (rc = check_tiles("k", k, k_strides, S, D, dtype, p.sk)) ||
+      (rc = check_tiles("v", v, v_strides, S, D, dtype, p.sv)) || (rc = check_lone_rows("o", o, o_strides, dtype, p.sout)) ||
+      (rc = check_ptr("m", m, 0, 4)) || (rc = check_ptr("lens", lens, 0, 4)))
+    return rc;
+  cross_fwd_plan(p, (int)D, dtype);
+  if ((rc = check_ptr("workspace", workspace, p.splits > 1, 16)) || (rc = require_device())) return rc;
+  p.q = q; p.k = k; p.v = v; p.out = o; p.m = m; p.lens = lens; p.part = workspace;
+  p.c = window_exponent_scale(sm_scale);
+  p.scale = sm_scale;
+  if (dtype == TATTN_F32) return launch_cross_f32(p, (int)D, false, (hipStream_t)stream);
+  return launch_cross_fwd(p, (int)D, dtype, (hipStream_t)stream);
+}
+
+int tattn_cross_bwd(const void* q, const void* k, const void* v, const void* o, const void* dout, void* dq, void* dk, void* dv,
+                    const float* m, const int32_t* lens, float* workspace, const int64_t q_strides[4],
+                    const int64_t k_strides[4], const int64_t v_strides[4], const int64_t o_strides[4],
+                    const int64_t do_strides[4], const int64_t dq_strides[4], const int64_t dk_strides[4],
+                    const int64_t dv_strides[4], int64_t Z, int64_t H, int64_t Hk, int64_t N, int64_t S, int64_t D, int dtype,
+                    float sm_scale, void* stream) {
+  CrossParams p{};
+  int rc;
+  if ((rc = cross_common(p, Z, 1, H, Hk, N, S, D, 1)) || (rc = check_dtype(dtype)) ||
+      (rc = check_tiles("q", q, q_strides, N, D, dtype, p.sq)) || (rc = check_tiles("k", k, k_strides, S, D, dtype, p.sk)) ||
+      (rc = check_tiles("v", v, v_strides, S, D, dtype, p.sv)) || (rc = check_tiles("o", o, o_strides, N, D, dtype, p.so)) ||
+      (rc = check_tiles("do", dout, do_strides, N, D, dtype, p.sd)) || (rc = check_tiles("dq", dq, dq_strides, N, D, dtype, p.sout)) ||
+      (rc = check_tiles("dk", dk, dk_strides, S, D, dtype, p.sdk)) || (rc = check_tiles("dv", dv, dv_strides, S, D, dtype, p.sdv)) ||
+      (rc = check_ptr("m", m, 1, 4)) || (rc = check_ptr("lens", lens, 0, 4)) || (rc = check_ptr("workspace", workspace, 1, 16)))
+    return rc;
+  cross_bwd_plan(p, (int)D, dtype);
+  if ((rc = require_device())) return rc;
+  p.q = q; p.k = k; p.v = v; p.o = o; p.dout = dout; p.out = dq; p.dk = dk; p.dv = dv; p.lens = lens;
+  p.m = const_cast<float*>(m);
+  cross_bwd_workspace(p, (int)D, dtype, workspace);
+  p.c = window_exponent_scale(sm_scale);
+  p.scale = sm_scale;
+  if (dtype == TATTN_F32) return launch_cross_f32(p, (int)D, true, (hipStream_t)stream);
+  return launch_cross_bwd(p, (int)D, dtype, (hipStream_t)stream);
+}
+
+int tattn_prefix_workspace(int64_t groups, int64_t members, int64_t H, int64_t Hk, int64_t N, int64_t P, int64_t S, int64_t D,
+                           int64_t* floats) {
+  PrefixParams p{};
+  int rc;
+  if (!floats) return set_error(TATTN_E_ARG, "floats is a null pointer");
+  if ((rc = cross_common(p.pre, groups, members, H, Hk, N, P, D, 0)) ||
+      (rc = cross_common(p.own, groups * members, 1, H, Hk, N, S, D, 0)))
+    return rc;
+  prefix_plan(p, (int)D);
+  *floats = prefix_floats(p, (int)D);
+  return TATTN_OK;
+}
+
+int tattn_prefix_attention(const void* q, const void* prefix_k, const void* prefix_v, const void* k, const void* v, void* o,
+                           const int32_t* prefix_lens, const int32_t* lens, float* workspace, const int64_t q_strides[4],
+                           const int64_t pk_strides[4], const int64_t pv_strides[4], const int64_t k_strides[4],
+                           const int64_t v_strides[4], const int64_t o_strides[4], int64_t groups, int64_t members, int64_t H,
+                           int64_t Hk, int64_t N, int64_t P, int64_t S, int64_t D, int dtype, float sm_scale, void* stream) {
+  PrefixParams p{};
+  CrossParams &a = p.pre, &b = p.own;
+  int rc;
+  if ((rc = cross_common(a, groups, members, H, Hk, N, P, D, 0)) || (rc = cross_common(b, groups * members, 1, H, Hk, N, S, D, 0)) ||
+      (rc = check_16bit(dtype)) || (rc = check_lone_rows("q", q, q_strides, dtype, a.sq)) ||
+      (rc = check_lone_rows("o", o, o_strides, dtype, a.sout)) || (rc = check_ptr("prefix_lens", prefix_lens, 0, 4)) ||
+      (rc = check_ptr("lens", lens, 1, 4)) || (rc = check_ptr("workspace", workspace, 1, 16)))
+    return rc;
+  if (P > 0 && ((rc = check_tiles("prefix_k", prefix_k, pk_strides, P, D, dtype, a.sk)) ||
+                (rc = check_tiles("prefix_v", prefix_v, pv_strides, P, D, dtype, a.sv))))
+    return rc;
+  if (S > 0 && ((rc = check_tiles("k", k, k_strides, S, D, dtype, b.sk)) || (rc = check_tiles("v", v, v_strides, S, D, dtype, b.sv))))
+    return rc;
+  if ((rc = require_device())) return rc;
+  prefix_plan(p, (int)D);
+  for (int i = 0; i < 3; ++i) b.sq[i] = a.sq[i], b.sout[i] = a.sout[i];
+  a.q = b.q = q; a.out = b.out = o;
+  a.c = b.c = window_exponent_scale(sm_scale);
+  a.k = prefix_k; a.v = prefix_v; a.lens = prefix_lens;
+  b.k = k; b.v = v; b.lens = lens;
+  a.part = workspace;
+  b.part = workspace + cross_part_floats(a.slices(), a.rows(), a.splits, D);
+  return launch_prefix(p, (int)D, dtype, (hipStream_t)stream);
+}
+
+int tattn_rope_axes_fwd(const void* q, const void* k, const void* q_weight, const void* k_weight, const float* cos,
+                        const float* sin, const int32_t* positions, const int32_t* axes, void* q_out, void* k_out,
+                        const int64_t q_strides[4], const int64_t k_strides[4], const int64_t qo_strides[4],
+                        const int64_t ko_strides[4], int64_t num_axes, int64_t axis_stride, int64_t pos_stride, int64_t Z,
+                        int64_t H, int64_t Hk, int64_t N, int64_t D, int64_t R, int dtype, int w_dtype, int interleaved,
+                        float eps, void* stream) {
+  RopeAxesParams p{};
+  int rc;
+  const void *qw = q_weight ? q_weight : cos, *kw = k_weight ? k_weight : cos;
+  if ((rc = check_weights(q_weight, k_weight)) ||
+      (rc = norm_rope_common(p, q, k, qw, kw, cos, sin, positions, q_strides, k_strides, pos_stride, Z, H, Hk, N, D, R, dtype,
+                             w_dtype, eps)) ||
+      (rc = rope_axes_common(p, axes, positions, num_axes, axis_stride, D, Z * N)))
+    return rc;
+  const int sz = dtype == TATTN_F32 ? 4 : 2;
+  if ((rc = check_ptr("q_out", q_out, Z * N, 16)) || (rc = check_ptr("k_out", k_out, Z * N, 16)) ||
+      (rc = check_rows("q_out", qo_strides, 3, sz)) || (rc = check_rows("k_out", ko_strides, 3, sz)) || (rc = require_device()))
+    return rc;
+  if (Z == 0 || N == 0) return TATTN_OK;
+  p.qw = q_weight; p.kw = k_weight; p.qo = q_out; p.ko = k_out;
+  for (int i = 0; i < 3; ++i) p.sqo[i] = qo_strides[i], p.sko[i] = ko_strides[i];
+  return launch_rope_axes(p, (int)D, dtype, interleaved != 0, false, (hipStream_t)stream);
+}
+
+int tattn_rope_axes_bwd(const void* q, const void* k, const void* q_weight, const void* k_weight, const float* cos,
+                        const float* sin, const int32_t* positions, const int32_t* axes, const void* dq_out,
+                        const void* dk_out, void* dq, void* dk, void* dq_weight, void* dk_weight, float* workspace,
+                        const int64_t q_strides[4], const int64_t k_strides[4], const int64_t dqo_strides[4],
+                        const int64_t dko_strides[4], const int64_t dq_strides[4], const int64_t dk_strides[4],
+                        int64_t num_axes, int64_t axis_stride, int64_t pos_stride, int64_t Z, int64_t H, int64_t Hk, int64_t N,
+                        int64_t D, int64_t R, int dtype, int w_dtype, int interleaved, float eps, void* stream) {
+  RopeAxesParams p{};
+  int rc;
+  const bool norm = q_weight != nullptr;
+  // Without norms the gradients take the place of q and k: the rotation back reads nothing else.
+  if ((rc = check_weights(q_weight, k_weight)) ||
+      (rc = norm_rope_common(p, norm ? q : dq_out, norm ? k : dk_out, norm ? q_weight : cos, norm ? k_weight : cos, cos, sin,
+                             positions, norm ? q_strides : dqo_strides, norm ? k_strides : dko_strides, pos_stride, Z, H, Hk, N,
+                             D, R, dtype, w_dtype, eps)) ||
+      (rc = rope_axes_common(p, axes, positions, num_axes, axis_stride, D, Z * N)))
+    return rc;
+  const int sz = dtype == TATTN_F32 ? 4 : 2;
+  const int64_t rows = Z * N;
+  if ((rc = check_ptr("dq_out", dq_out, rows, 16)) || (rc = check_ptr("dk_out", dk_out, rows, 16)) ||
+      (rc = check_ptr("dq", dq, rows, 16)) || (rc = check_ptr("dk", dk, rows, 16)) ||
+      (rc = check_rows("dq_out", dqo_strides, 3, sz)) || (rc = check_rows("dk_out", dko_strides, 3, sz)) ||
+      (rc = check_rows("dq", dq_strides, 3, sz)) || (rc = check_rows("dk", dk_strides, 3, sz)))
+    return rc;
+  if (norm && workspace) {
+    if ((rc = check_ptr("dq_weight", dq_weight, 1, 2)) || (rc = check_ptr("dk_weight", dk_weight, 1, 2)) ||
+        (rc = check_ptr("workspace", workspace, 1, 16)))
+      return rc;
+  } else if (dq_weight || dk_weight) {
+    return set_error(TATTN_E_ARG, "weight gradients need the weights and the workspace");
+  }
+  if ((rc = require_device())) return rc;
+  if (rows == 0) return TATTN_OK;
+  p.qw = q_weight; p.kw = k_weight; p.gq = dq_out; p.gk = dk_out; p.qo = dq; p.ko = dk;
+  p.dqw = dq_weight; p.dkw = dk_weight; p.partial = norm ? workspace : nullptr;
+  p.sign = -1.0f;
+  for (int i = 0; i < 3; ++i) {
+    p.sqo[i] = dq_strides[i]; p.sko[i] = dk_strides[i]; p.sgq[i] = dqo_strides[i]; p.sgk[i] = dko_strides[i];
+  }
+  return launch_rope_axes(p, (int)D, dtype, interleaved != 0, true, (hipStream_t)stream);
 }
 
 }  // extern "C"

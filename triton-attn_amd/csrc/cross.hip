@@ -1,0 +1,424 @@
+// Attention over keys of another length, 16-bit forward, and one step behind a shared prefix, on gfx950.
+//
+//   O = softmax(c' Q K^T) V over the first len keys, one pass over the keys with the running max and sum of the softmax
+//
+// Few rows (`rows_block`): four waves share 32 QT rows, and each takes every fourth key tile by itself, staged by LDS DMA
+// into its own two stages: no barrier until the four partial results are added. The keys are cut into parts where rows are few, and
+// `combine_kernel` joins the parts in order.
+//
+// Roundings: P is rounded to the element type, as the matrix instruction takes it, and its sum is taken from the rounded values.
+// Scores, maxima, sums and accumulators are float32.
+#include <algorithm>
+#include <type_traits>
+
+#include "cross.h"
+
+namespace tattn {
+namespace {
+
+constexpr int kWaves = 4;  // of a workgroup of rows_block
+
+template <int D>
+struct RowsLds {
+  static constexpr int STAGE = kWaves * 2 * CrossTile<D>::BYTES;  // each wave's K and V tile
+};
+
+// The part `split` of the keys for row block blk of a slice. CAUSAL: query n is at position len - N + n and sees no key after it.
+template <typename T, int D, int QT, bool CAUSAL>
+__device__ __forceinline__ void rows_block(const CrossParams& p, int slice, int blk, int split, char* s0, char* s1,
+                                           float (*red)[kWaves][64]) {
+  using V4 = typename H16<T>::V4;
+  using V8 = typename H16<T>::V8;
+  using Tile = CrossTile<D>;
+  constexpr int NSD = D / 16, DT = (D + 31) / 32, PIECES = Tile::PIECES;
+  const int tid = threadIdx.x;
+  const int lane = tid & 63, h2 = lane >> 5, l32 = lane & 31;
+  const int wu = (int)uniform32((uint32_t)(tid >> 6));
+  const CrossSlice sl(p, slice);
+  const int tiles = (sl.len + 31) >> 5;
+  const int i0 = (int)((int64_t)tiles * split / p.splits), i1 = (int)((int64_t)tiles * (split + 1) / p.splits);
+  const int rows = p.B * p.G * p.N;
+  const float c = p.c, hidden = hidden_score(c);
+
+  const __amdgpu_buffer_rsrc_t krs = rows_rsrc<T, D>(p.k, sl.zs * p.sk[0] + sl.hk * p.sk[1], sl.len, p.sk[2]);
+  const __amdgpu_buffer_rsrc_t vrs = rows_rsrc<T, D>(p.v, sl.zs * p.sv[0] + sl.hk * p.sv[1], sl.len, p.sv[2]);
+  const uint32_t kb = uniform32((uint32_t)(p.sk[2] * 64)), vb = uniform32((uint32_t)(p.sv[2] * 64));
+  uint32_t gk[PIECES], gv[PIECES];
+#pragma unroll
+  for (int i = 0; i < PIECES; ++i) {
+    gk[i] = Tile::source(i, lane, p.sk[2]);
+    gv[i] = Tile::source(i, lane, p.sv[2]);
+  }
+  const int mine = wu * 2 * Tile::BYTES;
+  auto issue = [&](char* st, int t) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < PIECES; ++i) dma16(krs, st + mine + 1024 * i, gk[i] + (uint32_t)t * kb);
+#pragma unroll
+    for (int i = 0; i < PIECES; ++i) dma16(vrs, st + mine + Tile::BYTES + 1024 * i, gv[i] + (uint32_t)t * vb);
+  };
+  int t = i0 + wu;
+  if (t < i1) issue(s0, t);
+
+  V8 qop[QT][NSD];
+  int last[QT];  // last key that the lane's row sees
+#pragma unroll
+  for (int j = 0; j < QT; ++j) {
+    const int row = 32 * (QT * blk + j) + l32;
+    const bool live = row < rows;
+    const CrossRow r(p, sl, live ? row : 0);
+    const T* src = (const T*)p.q + r.at(p.sq) + 8 * h2;
+    last[j] = CAUSAL ? sl.len - p.N + r.n : sl.len - 1;
+#pragma unroll
+    for (int s = 0; s < NSD; ++s) {
+      const V8 x = *reinterpret_cast<const V8*>(src + 16 * s);
+      qop[j][s] = live ? x : V8{};
+    }
+  }
+  // Tiles from here on hold keys that some row does not see.
+  const int masked = (CAUSAL ? max(0, sl.len - p.N + 1) : sl.len) >> 5;
+  CrossOp<D> at;
+  at.init(lane);
+
+  float mrow[QT], lrow[QT];
+  f32x16 acc[QT][DT];
+#pragma unroll
+  for (int j = 0; j < QT; ++j) {
+    mrow[j] = kNoMax;
+    lrow[j] = 0.0f;
+#pragma unroll
+    for (int u = 0; u < DT; ++u) acc[j][u] = f32x16{};
+  }
+
+  // Probabilities against the running max as it stands; a lane whose 16 sum above 2^12 (its first tile among them) sends the
+  // wave through the row max and a rescale, a one-sided branch (two-sided ones make the compiler hold the accumulators twice).
+  auto tile = [&](const char* st, int t) __attribute__((always_inline)) {
+    f32x16 s[QT];
+#pragma unroll
+    for (int j = 0; j < QT; ++j) s[j] = f32x16{};
+#pragma unroll
+    for (int sd = 0; sd < NSD; ++sd) {
+      const V8 ka = lds8<T>(st + mine + at.nat[sd]);
+#pragma unroll
+      for (int j = 0; j < QT; ++j) s[j] = Elt<T>::mfma(ka, qop[j][sd], s[j]);
+    }
+    if (t >= masked) {
+#pragma unroll
+      for (int j = 0; j < QT; ++j) hide_after(s[j], last[j], t, h2, hidden);
+    }
+    V8 x[QT][2];
+    float ps[QT], before[QT];
+    bool over = false;
+#pragma unroll
+    for (int j = 0; j < QT; ++j) {
+      ps[j] = tile_probs<T>(s[j], x[j], c, -mrow[j]);
+      before[j] = lrow[j];
+      lrow[j] += ps[j];
+      over |= !(ps[j] <= 4096.0f);
+    }
+    if (__builtin_amdgcn_ballot_w64(over)) {
+#pragma unroll
+      for (int j = 0; j < QT; ++j) {
+        const float mnew = moved_max(s[j], c, mrow[j]), alpha = fast_exp2(mrow[j] - mnew);
+        mrow[j] = mnew;
+        lrow[j] = before[j] * alpha + tile_probs<T>(s[j], x[j], c, -mnew);
+#pragma unroll
+        for (int u = 0; u < DT; ++u) acc[j][u] *= alpha;
+      }
+    }
+#pragma unroll
+    for (int sg = 0; sg < 2; ++sg)
+#pragma unroll
+      for (int u = 0; u < DT; ++u) {
+        const V8 va = at.template tr<T>(st + mine + Tile::BYTES, sg, u, lane);
+#pragma unroll
+        for (int j = 0; j < QT; ++j) acc[j][u] = Elt<T>::mfma(va, x[j][sg], acc[j][u]);
+      }
+  };
+  // The next tile's loads start once this wave's reads of that stage are done, and stay in flight over this tile.
+  auto step = [&](char* cur, char* nxt) __attribute__((always_inline)) {
+    if (t + kWaves < i1) {
+      __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0)
+      __atomic_signal_fence(__ATOMIC_SEQ_CST);
+      issue(nxt, t + kWaves);
+      wave_landed<2 * PIECES>();
+    } else {
+      wave_landed<0>();
+    }
+    tile(cur, t);
+    t += kWaves;
+  };
+  while (t < i1) {
+    step(s0, s1);
+    if (t >= i1) break;
+    step(s1, s0);
+  }
+
+  // The waves' results, tile by tile of rows through LDS: every wave is done with its stages, and nothing is in flight.
+  float lsum[QT];
+#pragma unroll
+  for (int j = 0; j < QT; ++j) {
+    lsum[j] = sum_halves(lrow[j]);
+    if (h2 == 0) {
+      red[0][wu][32 * j + l32] = mrow[j];
+      red[1][wu][32 * j + l32] = lsum[j];
+    }
+  }
+  __syncthreads();
+  constexpr int PART = DT * 16 * 64;  // floats of one wave's tile
+  static_assert(kWaves * PART * 4 <= RowsLds<D>::STAGE, "a stage holds a row tile of every wave");
+  const bool parted = p.splits > 1;
+  float mall[QT], lall[QT];
+#pragma unroll
+  for (int j = 0; j < QT; ++j) {
+    mall[j] = kNoMax;
+    lall[j] = 0.0f;
+#pragma unroll
+    for (int k = 0; k < kWaves; ++k) mall[j] = __builtin_fmaxf(mall[j], red[0][k][32 * j + l32]);
+#pragma unroll
+    for (int k = 0; k < kWaves; ++k) lall[j] += fast_exp2(red[0][k][32 * j + l32] - mall[j]) * red[1][k][32 * j + l32];
+    float wgt = fast_exp2(mrow[j] - mall[j]);
+    if (!parted) wgt = lall[j] == 0.0f ? 0.0f : wgt / lall[j];
+    TATTN_LDS float* dst = (TATTN_LDS float*)(j ? s1 : s0) + wu * PART + lane;
+#pragma unroll
+    for (int u = 0; u < DT; ++u)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) dst[(16 * u + r) * 64] = acc[j][u][r] * wgt;
+  }
+  __syncthreads();
+#pragma unroll
+  for (int j = 0; j < QT; ++j) {
+    const int row = 32 * (QT * blk + j) + l32;
+    if (row >= rows) continue;
+    const CrossRow r(p, sl, row);
+    T* orow = (T*)p.out + r.at(p.sout);
+    const int64_t prow = ((int64_t)slice * p.splits + split) * rows + row;
+    const TATTN_LDS float* src = (const TATTN_LDS float*)(j ? s1 : s0) + lane;
+    for (int g = wu; g < DT * 4; g += kWaves) {  // four consecutive columns per register group
+      const int d0 = 8 * g + 4 * h2;
+      if (d0 >= D) continue;
+      f32x4 x = f32x4{};
+#pragma unroll
+      for (int k = 0; k < kWaves; ++k)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[e] += src[k * PART + (4 * g + e) * 64];
+      if (parted) {
+        *reinterpret_cast<f32x4*>(p.part + prow * D + d0) = x;
+      } else {
+        V4 y;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) y[e] = (T)x[e];
+        *reinterpret_cast<V4*>(orow + d0) = y;
+      }
+    }
+    if (wu == 0 && h2 == 0) {
+      if (parted) {
+        float* ml = p.part + (int64_t)p.Zs * p.Hk * p.splits * rows * D + prow * 2;
+        ml[0] = mall[j];
+        ml[1] = lall[j];
+      } else if (p.m) {
+        p.m[r.index(p)] = mall[j] + __log2f(lall[j]);
+      }
+    }
+  }
+}
+
+template <typename T, int D, int QT, int OCC>
+__global__ __launch_bounds__(kWaves * 64, OCC) void cross_rows_kernel(const CrossParams p) {
+  __shared__ __attribute__((aligned(1024))) char s0[RowsLds<D>::STAGE];
+  __shared__ __attribute__((aligned(1024))) char s1[RowsLds<D>::STAGE];
+  __shared__ float red[2][kWaves][64];
+  int slice, blk;
+  if (!window_coord(p.Zs * p.Hk, p.nblk * p.splits, 0, 0, slice, blk)) return;
+  rows_block<T, D, QT, false>(p, slice, blk / p.splits, blk % p.splits, s0, s1, red);
+}
+
+// The prefix's parts first, which are the longer ones, then each sequence's own keys.
+template <typename T, int D, int QT, int OCC>
+__global__ __launch_bounds__(kWaves * 64, OCC) void prefix_rows_kernel(const PrefixParams p) {
+  __shared__ __attribute__((aligned(1024))) char s0[RowsLds<D>::STAGE];
+  __shared__ __attribute__((aligned(1024))) char s1[RowsLds<D>::STAGE];
+  __shared__ float red[2][kWaves][64];
+  const int shared = p.pre.nblk * p.pre.splits, total = p.pre.Zs * p.pre.Hk * shared;
+  int i = blockIdx.x;
+  if (i < total) {
+    const int blk = i % shared;
+    rows_block<T, D, QT, false>(p.pre, i / shared, blk / p.pre.splits, blk % p.pre.splits, s0, s1, red);
+    return;
+  }
+  i -= total;
+  const int per = p.own.nblk * p.own.splits, blk = i % per;
+  rows_block<T, D, 1, true>(p.own, i / per, blk / p.own.splits, blk % p.own.splits, s0, s1, red);
+}
+
+// ---- rows whose keys were cut into parts ---------------------------------------------------------
+struct CombineParams {
+  const float* part[2];  // of the slices' rows; of each sequence's own rows, or null
+  int32_t splits[2];
+  void* out;
+  float* m;
+  const int32_t* lens;  // own keys of each sequence: rows at positions below 0 become 0
+  int64_t st[3];
+  int64_t slices;
+  int32_t Hk, B, G, N, S;
+  int32_t dealt;  // groups of lanes that a row's parts are dealt to
+};
+
+// O = sum_s 2^(m_s - m) O_s / sum_s 2^(m_s - m) l_s. D / 4 lanes hold a row's columns; `dealt` such groups share a row's parts
+// and are added in order through LDS.
+template <typename T, int D>
+__global__ __launch_bounds__(256) void combine_kernel(const CombineParams p) {
+  typedef T V4 __attribute__((ext_vector_type(4)));
+  constexpr int LPR = D / 4, GROUPS = 256 / LPR;
+  __shared__ __attribute__((aligned(16))) float sums[GROUPS][D];
+  __shared__ float ml[GROUPS][2];
+  const int tid = threadIdx.x, g = tid / LPR, d0 = tid % LPR * 4, deal = g % p.dealt;
+  const int rows = p.B * p.G * p.N;
+  const int64_t i = (int64_t)blockIdx.x * (GROUPS / p.dealt) + g / p.dealt;
+  const bool live = i < p.slices * rows;
+  const int64_t slice = live ? i / rows : 0;
+  const int row = live ? (int)(i % rows) : 0, b = row / (p.G * p.N), rest = row % (p.G * p.N);
+  const int64_t zs = slice / p.Hk, hk = slice % p.Hk, z = zs * p.B + b;
+  const int n = rest % p.N;
+  float m = kNoMax, l = 0.0f;
+  f32x4 x = f32x4{};
+  auto add = [&](float ms, float ls, f32x4 y) __attribute__((always_inline)) {
+    const float mn = __builtin_fmaxf(m, ms), a = fast_exp2(m - mn), w = fast_exp2(ms - mn);
+    m = mn;
+    l = l * a + ls * w;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) x[e] = x[e] * a + y[e] * w;
+  };
+  auto take = [&](const float* part, int splits, int first, int64_t slices, int64_t slice, int rows, int row) __attribute__((always_inline)) {
+    const float* tail = part + slices * splits * rows * D;
+#pragma unroll 4
+    for (int s = first; s < splits; s += p.dealt) {
+      const int64_t at = (slice * splits + s) * rows + row;
+      const f32x2 v = *reinterpret_cast<const f32x2*>(tail + 2 * at);
+      add(v[0], v[1], *reinterpret_cast<const f32x4*>(part + at * D + d0));
+    }
+  };
+  if (live) {
+    take(p.part[0], p.splits[0], deal, p.slices, slice, rows, row);
+    if (p.part[1]) take(p.part[1], p.splits[1], deal, p.slices * p.B, z * p.Hk + hk, p.G * p.N, rest);
+  }
+  if (p.dealt > 1) {
+    *reinterpret_cast<f32x4*>(&sums[g][d0]) = x;
+    if (d0 == 0) ml[g][0] = m, ml[g][1] = l;
+    __syncthreads();
+    if (deal > 0) return;
+    for (int k = 1; k < p.dealt; ++k) add(ml[g + k][0], ml[g + k][1], *reinterpret_cast<const f32x4*>(&sums[g + k][d0]));
+  }
+  if (!live) return;
+  if (p.lens && min(max(p.lens[z], 0), p.S) - p.N + n < 0) l = 0.0f;
+  const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+  V4 y;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) y[e] = (T)(l == 0.0f ? 0.0f : x[e] * inv);
+  const int64_t h = hk * p.G + rest / p.N;
+  *reinterpret_cast<V4*>((T*)p.out + z * p.st[0] + h * p.st[1] + n * p.st[2] + d0) = y;
+  if (p.m && d0 == 0) p.m[(z * p.Hk * p.G + h) * p.N + n] = m + __log2f(l);
+}
+
+template <typename T, int D>
+int combine(CombineParams p, hipStream_t st, const char* what) {
+  constexpr int GROUPS = 256 / (D / 4);
+  const int most = std::max(p.splits[0], p.part[1] ? p.splits[1] : 0);
+  for (p.dealt = 1; p.dealt < GROUPS && 4 * p.dealt < most; p.dealt *= 2) {}
+  const int64_t rows = p.slices * p.B * p.G * p.N, per = GROUPS / p.dealt, blocks = (rows + per - 1) / per;
+  if (blocks > 0x7fffffff) return set_error(TATTN_E_ARG, "grid too large: %lld rows", (long long)rows);
+  combine_kernel<T, D><<<dim3((unsigned)blocks), dim3(256), 0, st>>>(p);
+  return check_launch(what);
+}
+
+CombineParams combine_params(const CrossParams& p) {
+  CombineParams c{};
+  c.part[0] = p.part;
+  c.splits[0] = p.splits;
+  c.out = p.out;
+  c.m = p.m;
+  for (int i = 0; i < 3; ++i) c.st[i] = p.sout[i];
+  c.slices = p.slices();
+  c.Hk = p.Hk; c.B = p.B; c.G = p.G; c.N = p.N;
+  return c;
+}
+
+template <typename T, int D>
+int combine_cross(const CrossParams& p, hipStream_t st) { return combine<T, D>(combine_params(p), st, "tattn_cross_fwd"); }
+
+// Workgroups of rows_block that a CU holds (128 KB of stages at head dim 128).
+constexpr int rows_occ(int D) { return D == 128 ? 1 : 2; }
+
+template <typename T, int D>
+int fwd_d(const CrossParams& p, hipStream_t st) {
+  unsigned blocks;
+  int rc;
+  if ((rc = window_grid(p.slices(), (int64_t)p.nblk * p.splits, 0, &blocks))) return rc;
+  cross_rows_kernel<T, D, 1, rows_occ(D)><<<dim3(blocks), dim3(kWaves * 64), 0, st>>>(p);
+  if ((rc = check_launch("tattn_cross_fwd")) || p.splits == 1) return rc;
+  return combine_cross<T, D>(p, st);
+}
+
+template <typename T, int D>
+int prefix_d(const PrefixParams& p, hipStream_t st) {
+  const int64_t blocks = p.pre.slices() * p.pre.nblk * p.pre.splits + p.own.slices() * p.own.nblk * p.own.splits;
+  if (blocks > 0x7ffffff) return set_error(TATTN_E_ARG, "grid too large: %lld workgroups", (long long)blocks);
+  prefix_rows_kernel<T, D, 2, rows_occ(D)><<<dim3((unsigned)blocks), dim3(kWaves * 64), 0, st>>>(p);
+  int rc = check_launch("tattn_prefix_attention");
+  if (rc) return rc;
+  CombineParams c = combine_params(p.pre);
+  c.part[1] = p.own.part;
+  c.splits[1] = p.own.splits;
+  c.lens = p.own.lens;
+  c.S = p.own.S;
+  return combine<T, D>(c, st, "tattn_prefix_attention");
+}
+
+}  // namespace
+
+// One row tile per workgroup (four in float32); its keys are cut into parts until the chip holds no more workgroups at once, of at least eight tiles.
+void cross_fwd_plan(CrossParams& p, int D, int dtype) {
+  const int64_t tiles = ((int64_t)p.S + 31) / 32, block = dtype == 1 ? 128 : 32;
+  p.nblk = (int)((p.rows() + block - 1) / block);
+  const int64_t blocks = p.slices() * p.nblk, want = 256 * rows_occ(D);
+  p.splits = (int)std::max<int64_t>(1, std::min<int64_t>(want / blocks, tiles / 8));
+}
+
+// The parts of all rows together, prefixes and own keys, are about as many as the chip holds at once; none has less than eight
+// tiles. Both kinds are always joined, so each has a part at least.
+void prefix_plan(PrefixParams& p, int D) {
+  const int64_t pt = std::max<int64_t>(1, ((int64_t)p.pre.S + 31) / 32), ot = std::max<int64_t>(1, ((int64_t)p.own.S + 31) / 32);
+  p.pre.nblk = (int)((p.pre.rows() + 63) / 64);
+  p.own.nblk = (int)((p.own.rows() + 31) / 32);
+  const int64_t pb = p.pre.slices() * p.pre.nblk, ob = p.own.slices() * p.own.nblk;
+  const int64_t chunk = std::max<int64_t>(8, (pb * pt + ob * ot) / (256 * rows_occ(D)));
+  p.pre.splits = (int)std::max<int64_t>(2, (pt + chunk - 1) / chunk);
+  p.own.splits = (int)std::max<int64_t>(2, (ot + chunk - 1) / chunk);
+}
+int64_t prefix_floats(const PrefixParams& p, int D) {
+  return cross_part_floats(p.pre.slices(), p.pre.rows(), p.pre.splits, D) + cross_part_floats(p.own.slices(), p.own.rows(), p.own.splits, D);
+}
+
+#define TATTN_CROSS_SWITCH(FN)                                                   \
+  switch (D) {                                                                   \
+    case 16: return dtype == 0 ? FN<f16, 16>(p, st) : FN<bf16, 16>(p, st);       \
+    case 32: return dtype == 0 ? FN<f16, 32>(p, st) : FN<bf16, 32>(p, st);       \
+    case 64: return dtype == 0 ? FN<f16, 64>(p, st) : FN<bf16, 64>(p, st);       \
+    case 128: return dtype == 0 ? FN<f16, 128>(p, st) : FN<bf16, 128>(p, st);    \
+  }                                                                              \
+  return set_error(TATTN_E_ARG, "head dim must be 16, 32, 64 or 128, got %d", D);
+
+int launch_cross_fwd(const CrossParams& p, int D, int dtype, hipStream_t st) { TATTN_CROSS_SWITCH(fwd_d) }
+int launch_prefix(const PrefixParams& p, int D, int dtype, hipStream_t st) { TATTN_CROSS_SWITCH(prefix_d) }
+int launch_cross_combine(const CrossParams& p, int D, int dtype, hipStream_t st) {
+  if (dtype == 1) {
+    switch (D) {
+      case 16: return combine_cross<float, 16>(p, st);
+      case 32: return combine_cross<float, 32>(p, st);
+      case 64: return combine_cross<float, 64>(p, st);
+      case 128: return combine_cross<float, 128>(p, st);
+    }
+  }
+  TATTN_CROSS_SWITCH(combine_cross)
+}
+
+}  // namespace tattn

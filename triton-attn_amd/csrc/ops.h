@@ -1,5 +1,5 @@
 // Host-side launchers of the operators around attention: page bookkeeping, the cache in 4 bits,
-// norms with rotation, window attention. Arguments are checked by the entry points (abi_ops.hip).
+// norms with rotation, window attention, attention over other lengths and shared prefixes. Arguments are checked by the entry points (abi_ops.hip).
 #pragma once
 
 #include <algorithm>
@@ -72,6 +72,17 @@ struct NormRopeParams {
   int32_t blocks_q, blocks_k;
 };
 int launch_norm_rope(const NormRopeParams& p, int D, int dtype, bool interleaved, bool bwd, hipStream_t st);
+int launch_norm_rope_dw(const NormRopeParams& p, int D, int dtype, hipStream_t st);
+
+// The same with several axes: positions [axes, N] or [axes, Z, N], an axis for each pair; the norm is left out without weights.
+constexpr uint32_t kNoAxis = 15;
+struct RopeAxesParams : NormRopeParams {
+  alignas(4) uint8_t axes[32];  // four bits a pair, the first in the low ones; kNoAxis: not turned
+  int64_t axis_stride;
+  int32_t quads;  // pairs 4 i .. 4 i + 3 share an axis
+  float sign;     // without norms: -1 turns back
+};
+int launch_rope_axes(const RopeAxesParams& p, int D, int dtype, bool interleaved, bool bwd, hipStream_t st);
 
 // Attention over a window and the first keys (window.h). q, o, do, dq: [Z, H, N, D]; k, v, dk, dv: [Z, Hk, S, D].
 struct WindowParams {
@@ -133,6 +144,54 @@ int launch_window_f32(const WindowParams& p, int D, bool bwd, hipStream_t st);  
 // O of rows whose keys were split: part as laid out above, out [slices / Hk, H, N, D] with strides (z, h, n).
 int launch_combine(const float* part, void* out, float* m, const int64_t so[3], int64_t slices, int Hk, int G, int N,
                    int splits, int D, int dtype, hipStream_t st);
+
+// Attention over keys of another length (cross.h). q, o, do, dq: [Zs B, H, N, D]; k, v, dk, dv: [Zs, Hk, S, D].
+struct CrossParams {
+  const void* q;
+  const void* k;
+  const void* v;
+  const void* o;  // backward: the forward's output
+  const void* dout;
+  void* out;  // forward: O; backward: dQ
+  void* dk;
+  void* dv;
+  float* m;             // [Zs B, H, N] base-2 log-sum-exp, or null
+  float* delta;         // backward: [slices, rows], minus rowsum(dO * O)
+  float* norms;         // fp16 backward: [slices, cross_norm_blocks, 2], largest squared norm of dO's rows, largest |delta|
+  const int32_t* lens;  // [Zs] keys that each sequence (or group) sees, or null: S
+  float* part;          // forward: partial rows, see cross_part_floats; backward: partial dQ
+  float* kpart;         // backward: partial dK, dV
+  int64_t sq[3], sk[3], sv[3], so[3], sd[3], sout[3], sdk[3], sdv[3];
+  int32_t Zs, B, H, Hk, G, N, S;
+  int32_t nblk, splits;   // row blocks of a slice, parts of their keys
+  int32_t kblk, parts;    // backward: key blocks of a slice, parts of their rows
+  float c, scale;
+  int64_t slices() const { return (int64_t)Zs * Hk; }
+  int64_t rows() const { return (int64_t)B * G * N; }  // of a slice
+};
+// Partial rows of a forward split `splits` ways: for each slice, part and row D sums, then for each its max and sum.
+inline int64_t cross_part_floats(int64_t slices, int64_t rows, int64_t splits, int64_t D) { return slices * rows * splits * (D + 2); }
+// Blocks of 128 rows of a slice, as dQ's workgroups take them.
+__host__ __device__ inline int cross_norm_blocks(int64_t rows) { return (int)((rows + 127) / 128); }
+void cross_fwd_plan(CrossParams& p, int D, int dtype);  // sets nblk and splits
+void cross_bwd_plan(CrossParams& p, int D, int dtype);  // sets nblk, splits, kblk and parts
+int64_t cross_bwd_floats(const CrossParams& p, int D, int dtype);  // workspace of a planned backward
+void cross_bwd_workspace(CrossParams& p, int D, int dtype, float* work);  // lays out delta, norms, part and kpart
+int launch_cross_fwd(const CrossParams& p, int D, int dtype, hipStream_t st);
+int launch_cross_bwd(const CrossParams& p, int D, int dtype, hipStream_t st);
+int launch_cross_f32(const CrossParams& p, int D, bool bwd, hipStream_t st);
+int launch_cross_combine(const CrossParams& p, int D, int dtype, hipStream_t st);  // joins the forward's parts
+// Adds the parts of dQ, or of dK and dV for key blocks of `block` keys.
+int launch_cross_sum(const CrossParams& p, int D, int dtype, bool keys, int block, hipStream_t st);
+
+// One step behind a shared prefix: `pre` holds a group's rows (B sequences) over the prefix, `own` each sequence's over its
+// keys, causal. Both write parts (own.part lies behind pre.part), which are joined.
+struct PrefixParams {
+  CrossParams pre, own;
+};
+void prefix_plan(PrefixParams& p, int D);
+int64_t prefix_floats(const PrefixParams& p, int D);
+int launch_prefix(const PrefixParams& p, int D, int dtype, hipStream_t st);
 
 // One token per request over the cache in 4 bits.
 struct Cache4AttnParams {

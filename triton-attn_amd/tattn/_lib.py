@@ -13,7 +13,7 @@ from pathlib import Path
 import torch  # noqa: F401  (must be imported before the library is loaded, see above)
 
 LIB_PATH = Path(__file__).resolve().with_name("libtattn_hip.so")
-ABI_VERSION = 3
+ABI_VERSION = 4
 
 F16, F32, BF16 = 0, 1, 2
 K_FWD, K_BWD_DKDV, K_BWD_DQ = 0, 1, 2
@@ -28,6 +28,8 @@ EXPORTS = (
     "tattn_norm_rope_fwd", "tattn_norm_rope_bwd",
     "tattn_window_workspace", "tattn_window_picked", "tattn_window_fwd", "tattn_window_bwd",
     "tattn_cache4_attention_workspace", "tattn_cache4_attention",
+    "tattn_cross_workspace", "tattn_cross_fwd", "tattn_cross_bwd", "tattn_prefix_workspace", "tattn_prefix_attention",
+    "tattn_rope_axes_fwd", "tattn_rope_axes_bwd",
 )
 
 # Kernels outside the tables, as `picked` reports them.
@@ -84,6 +86,13 @@ _SIGS = {
     "tattn_window_picked": (_I, [_I64] * 8),
     "tattn_window_fwd": (_I, [_P] * 7 + [_STR4] * 4 + [_I64] * 8 + [_I, _F, _P]),
     "tattn_window_bwd": (_I, [_P] * 11 + [_STR4] * 8 + [_I64] * 8 + [_I, _F, _P]),
+    "tattn_cross_workspace": (_I, [_I] + [_I64] * 6 + [_I, ctypes.POINTER(_I64)]),
+    "tattn_cross_fwd": (_I, [_P] * 7 + [_STR4] * 4 + [_I64] * 6 + [_I, _F, _P]),
+    "tattn_cross_bwd": (_I, [_P] * 11 + [_STR4] * 8 + [_I64] * 6 + [_I, _F, _P]),
+    "tattn_prefix_workspace": (_I, [_I64] * 8 + [ctypes.POINTER(_I64)]),
+    "tattn_prefix_attention": (_I, [_P] * 9 + [_STR4] * 6 + [_I64] * 8 + [_I, _F, _P]),
+    "tattn_rope_axes_fwd": (_I, [_P] * 10 + [_STR4] * 4 + [_I64] * 9 + [_I, _I, _I, _F, _P]),
+    "tattn_rope_axes_bwd": (_I, [_P] * 15 + [_STR4] * 6 + [_I64] * 9 + [_I, _I, _I, _F, _P]),
     "tattn_norm_rope_bwd": (_I, [_P] * 14 + [_STR4] * 6 + [_I64] * 7 + [_I, _I, _I, _F, _P]),
 }
 
