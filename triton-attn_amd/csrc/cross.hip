@@ -228,7 +228,7 @@ __global__ __launch_bounds__(kWaves * 64, OCC) void cross_rows_kernel(const Cros
   __shared__ __attribute__((aligned(1024))) char s1[RowsLds<D>::STAGE];
   __shared__ float red[2][kWaves][64];
   int slice, blk;
-  if (!window_coord(p.Zs * p.Hk, p.nblk * p.splits, 0, 0, slice, blk)) return;
+  if (!cross_coord(p.Zs * p.Hk, p.nblk * p.splits, slice, blk)) return;
   rows_block<T, D, QT, false>(p, slice, blk / p.splits, blk % p.splits, s0, s1, red);
 }
 
@@ -352,7 +352,11 @@ template <typename T, int D>
 int fwd_d(const CrossParams& p, hipStream_t st) {
   unsigned blocks;
   int rc;
-  if ((rc = window_grid(p.slices(), (int64_t)p.nblk * p.splits, 0, &blocks))) return rc;
+  if (p.pipe) {
+    if ((rc = launch_cross_pipe(p, D, std::is_same_v<T, f16> ? 0 : 2, st)) || p.splits == 1) return rc;
+    return combine_cross<T, D>(p, st);
+  }
+  if ((rc = cross_grid(p.slices(), (int64_t)p.nblk * p.splits, &blocks))) return rc;
   cross_rows_kernel<T, D, 1, rows_occ(D)><<<dim3(blocks), dim3(kWaves * 64), 0, st>>>(p);
   if ((rc = check_launch("tattn_cross_fwd")) || p.splits == 1) return rc;
   return combine_cross<T, D>(p, st);
@@ -375,11 +379,14 @@ int prefix_d(const PrefixParams& p, hipStream_t st) {
 
 }  // namespace
 
-// One row tile per workgroup (four in float32); its keys are cut into parts until the chip holds no more workgroups at once, of at least eight tiles.
+// Up to two row tiles: one per workgroup (rows_block). More: blocks of cross_pipe_rows. Keys are cut into parts until the chip
+// holds no more workgroups at once, of at least eight tiles.
 void cross_fwd_plan(CrossParams& p, int D, int dtype) {
-  const int64_t tiles = ((int64_t)p.S + 31) / 32, block = dtype == 1 ? 128 : 32;
+  const int64_t tiles = ((int64_t)p.S + 31) / 32;
+  p.pipe = dtype != 1 && p.rows() > 64;
+  const int64_t block = dtype == 1 ? 128 : p.pipe ? cross_pipe_rows(D) : 32;
   p.nblk = (int)((p.rows() + block - 1) / block);
-  const int64_t blocks = p.slices() * p.nblk, want = 256 * rows_occ(D);
+  const int64_t blocks = p.slices() * p.nblk, want = 256 * (p.pipe ? 2 : rows_occ(D));
   p.splits = (int)std::max<int64_t>(1, std::min<int64_t>(want / blocks, tiles / 8));
 }
 

@@ -78,7 +78,7 @@ __global__ __launch_bounds__(NW * 64, OCC) void cross_dq_kernel(const CrossParam
   const int wu = (int)uniform32((uint32_t)(tid >> 6));
   const float c = p.c;
   int slice, blk;
-  if (!window_coord(p.Zs * p.Hk, p.nblk * p.splits, 0, 0, slice, blk)) return;
+  if (!cross_coord(p.Zs * p.Hk, p.nblk * p.splits, slice, blk)) return;
   const int split = blk % p.splits;
   blk /= p.splits;
   const CrossSlice sl(p, slice);
@@ -283,7 +283,7 @@ __global__ __launch_bounds__(NW * 64, OCC) void cross_dkdv_kernel(const CrossPar
   const int wu = (int)uniform32((uint32_t)(tid >> 6));
   const float c = p.c;
   int slice, item;
-  if (!window_coord(p.Zs * p.Hk, p.kblk * p.parts, 0, 0, slice, item)) return;
+  if (!cross_coord(p.Zs * p.Hk, p.kblk * p.parts, slice, item)) return;
   const int kbi = item / p.parts, part = item % p.parts;
   const CrossSlice sl(p, slice);
   const int kw0 = KEYS * kbi + 32 * wu, key = kw0 + l32;
@@ -544,11 +544,11 @@ template <typename T, int D>
 int bwd_d(const CrossParams& p, hipStream_t st) {
   unsigned blocks;
   int rc;
-  if ((rc = window_grid(p.slices(), (int64_t)p.nblk * p.splits, 0, &blocks))) return rc;
+  if ((rc = cross_grid(p.slices(), (int64_t)p.nblk * p.splits, &blocks))) return rc;
   cross_dq_kernel<T, D, kRowWaves, bwd_occ(D)><<<dim3(blocks), dim3(kRowWaves * 64), 0, st>>>(p);
   if ((rc = check_launch("tattn_cross_bwd")) || (p.splits > 1 && (rc = sum_d<T, D>(p, false, 0, st)))) return rc;
   constexpr int KW = key_waves(D);
-  if ((rc = window_grid(p.slices(), (int64_t)p.kblk * p.parts, 0, &blocks))) return rc;
+  if ((rc = cross_grid(p.slices(), (int64_t)p.kblk * p.parts, &blocks))) return rc;
   cross_dkdv_kernel<T, D, KW, bwd_occ(D)><<<dim3(blocks), dim3(KW * 64), 0, st>>>(walked(p));
   if ((rc = check_launch("tattn_cross_bwd")) || p.parts == 1) return rc;
   return sum_d<T, D>(p, true, 32 * KW, st);

@@ -13,7 +13,7 @@ struct CrossRows32 {
   int slice, blk, split, row, rows, i0, i1;
   bool ok, live;
   __device__ __forceinline__ CrossRows32(const CrossParams& p, int w, int l32) {
-    ok = window_coord(p.Zs * p.Hk, p.nblk * p.splits, 0, 0, slice, blk);
+    ok = cross_coord(p.Zs * p.Hk, p.nblk * p.splits, slice, blk);
     if (!ok) return;
     split = blk % p.splits;
     blk /= p.splits;
@@ -160,7 +160,7 @@ __global__ __launch_bounds__(256, 1) void cross_dkdv_f32_kernel(const CrossParam
   __shared__ __attribute__((aligned(16))) float md[2][32];  // M, -delta
   const int tid = threadIdx.x, lane = tid & 63, h2 = lane >> 5, l32 = lane & 31, w = (int)uniform32(tid >> 6);
   int slice, item;
-  if (!window_coord(p.Zs * p.Hk, p.kblk * p.parts, 0, 0, slice, item)) return;
+  if (!cross_coord(p.Zs * p.Hk, p.kblk * p.parts, slice, item)) return;
   const int kb = item / p.parts, part = item % p.parts;
   const CrossSlice sl(p, slice);
   const int nq = (p.N + 31) >> 5, total = 128 * kb < sl.len ? nq * p.G : 0;
@@ -234,7 +234,7 @@ template <int D>
 int fwd_d(const CrossParams& p, hipStream_t st) {
   unsigned blocks;
   int rc;
-  if ((rc = window_grid(p.slices(), (int64_t)p.nblk * p.splits, 0, &blocks))) return rc;
+  if ((rc = cross_grid(p.slices(), (int64_t)p.nblk * p.splits, &blocks))) return rc;
   cross_fwd_f32_kernel<D, D == 128 ? 1 : 2><<<dim3(blocks), dim3(256), 0, st>>>(p);
   if ((rc = check_launch("tattn_cross_fwd")) || p.splits == 1) return rc;
   return launch_cross_combine(p, D, 1, st);
@@ -244,10 +244,10 @@ template <int D>
 int bwd_d(const CrossParams& p, hipStream_t st) {
   unsigned blocks;
   int rc;
-  if ((rc = window_grid(p.slices(), (int64_t)p.nblk * p.splits, 0, &blocks))) return rc;
+  if ((rc = cross_grid(p.slices(), (int64_t)p.nblk * p.splits, &blocks))) return rc;
   cross_dq_f32_kernel<D, D == 128 ? 1 : 2><<<dim3(blocks), dim3(256), 0, st>>>(p);
   if ((rc = check_launch("tattn_cross_bwd")) || (p.splits > 1 && (rc = launch_cross_sum(p, D, 1, false, 0, st)))) return rc;
-  if ((rc = window_grid(p.slices(), (int64_t)p.kblk * p.parts, 0, &blocks))) return rc;
+  if ((rc = cross_grid(p.slices(), (int64_t)p.kblk * p.parts, &blocks))) return rc;
   cross_dkdv_f32_kernel<D><<<dim3(blocks), dim3(256), 0, st>>>(p);
   if ((rc = check_launch("tattn_cross_bwd")) || p.parts == 1) return rc;
   return launch_cross_sum(p, D, 1, true, 128, st);

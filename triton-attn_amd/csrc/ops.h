@@ -157,13 +157,14 @@ struct CrossParams {
   void* dv;
   float* m;             // [Zs B, H, N] base-2 log-sum-exp, or null
   float* delta;         // backward: [slices, rows], minus rowsum(dO * O)
-  float* norms;         // fp16 backward: [slices, cross_norm_blocks, 2], largest squared norm of dO's rows, largest |delta|
+  float* norms;         // fp16 backward: [slices, nblk, 2], largest squared norm of dO's rows, largest |delta|
   const int32_t* lens;  // [Zs] keys that each sequence (or group) sees, or null: S
   float* part;          // forward: partial rows, see cross_part_floats; backward: partial dQ
   float* kpart;         // backward: partial dK, dV
   int64_t sq[3], sk[3], sv[3], so[3], sd[3], sout[3], sdk[3], sdv[3];
   int32_t Zs, B, H, Hk, G, N, S;
   int32_t nblk, splits;   // row blocks of a slice, parts of their keys
+  int32_t pipe;           // forward: row blocks of cross_pipe_rows rows, walked by all waves together
   int32_t kblk, parts;    // backward: key blocks of a slice, parts of their rows
   float c, scale;
   int64_t slices() const { return (int64_t)Zs * Hk; }
@@ -171,13 +172,21 @@ struct CrossParams {
 };
 // Partial rows of a forward split `splits` ways: for each slice, part and row D sums, then for each its max and sum.
 inline int64_t cross_part_floats(int64_t slices, int64_t rows, int64_t splits, int64_t D) { return slices * rows * splits * (D + 2); }
-// Blocks of 128 rows of a slice, as dQ's workgroups take them.
-__host__ __device__ inline int cross_norm_blocks(int64_t rows) { return (int)((rows + 127) / 128); }
+// Whether slices are dealt out to the XCDs (cross_coord): an eighth of the places at most is left idle.
+__host__ __device__ inline bool cross_dealt(int64_t slices) { return ((slices + 7) / 8 * 8 - slices) * 8 <= slices; }
+inline int cross_grid(int64_t slices, int64_t blocks, unsigned* out) {
+  return window_grid(cross_dealt(slices) ? (slices + 7) / 8 * 8 : slices, blocks, 0, out);
+}
 void cross_fwd_plan(CrossParams& p, int D, int dtype);  // sets nblk and splits
 void cross_bwd_plan(CrossParams& p, int D, int dtype);  // sets nblk, splits, kblk and parts
 int64_t cross_bwd_floats(const CrossParams& p, int D, int dtype);  // workspace of a planned backward
 void cross_bwd_workspace(CrossParams& p, int D, int dtype, float* work);  // lays out delta, norms, part and kpart
 int launch_cross_fwd(const CrossParams& p, int D, int dtype, hipStream_t st);
+int launch_cross_pipe(const CrossParams& p, int D, int dtype, hipStream_t st);  // without the joining of parts
+// Waves of a workgroup of the forward for many rows, and row tiles of each.
+constexpr int cross_pipe_waves(int D) { return 4; }
+constexpr int cross_pipe_tiles(int D) { return D == 128 ? 1 : 2; }
+constexpr int cross_pipe_rows(int D) { return 32 * cross_pipe_waves(D) * cross_pipe_tiles(D); }
 int launch_cross_bwd(const CrossParams& p, int D, int dtype, hipStream_t st);
 int launch_cross_f32(const CrossParams& p, int D, bool bwd, hipStream_t st);
 int launch_cross_combine(const CrossParams& p, int D, int dtype, hipStream_t st);  // joins the forward's parts
