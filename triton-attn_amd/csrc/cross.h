@@ -15,10 +15,10 @@ namespace tattn {
 
 // Workgroup -> (slice, block); false past the last. Workgroups go round-robin over the 8 XCDs. Blocks of a slice stay on one, whose
 // L2 then holds its keys, and the slices are dealt out one by one, so that sequences of other lengths meet on every XCD
-// (at 8 x 16 x 1,024 rows over 375 to 1,500 keys x 64 a sequence an XCD took 53 us forward and 200 backward, dealt out 47 and
-// 185). Where that would leave XCDs
-// idle each takes a run of all blocks.
-__device__ __forceinline__ bool cross_coord(int slices, int nblk, int& slice, int& blk) {
+// (cross_dealt); where that would leave XCDs idle each takes a run of all blocks. 8 x 16 x 1,024 rows over 375 to 1,500 keys x 64, us
+// forward and backward: runs 53 and 200, dealt out 47 and 185 (long sequences first, or long and short ones side by side: no faster).
+__device__ __forceinline__ bool cross_coord(const CrossParams& p, int nblk, int& slice, int& blk) {
+  const int slices = p.Zs * p.Hk;
   if (!cross_dealt(slices)) return window_coord(slices, nblk, 0, 0, slice, blk);
   const int l = (int)(blockIdx.x >> 3);
   slice = 8 * (l / nblk) + (int)(blockIdx.x & 7);

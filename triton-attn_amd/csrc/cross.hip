@@ -228,7 +228,7 @@ __global__ __launch_bounds__(kWaves * 64, OCC) void cross_rows_kernel(const Cros
   __shared__ __attribute__((aligned(1024))) char s1[RowsLds<D>::STAGE];
   __shared__ float red[2][kWaves][64];
   int slice, blk;
-  if (!cross_coord(p.Zs * p.Hk, p.nblk * p.splits, slice, blk)) return;
+  if (!cross_coord(p, p.nblk * p.splits, slice, blk)) return;
   rows_block<T, D, QT, false>(p, slice, blk / p.splits, blk % p.splits, s0, s1, red);
 }
 

@@ -3,8 +3,8 @@
 //   P = 2^(S c - M),  dS = P (dP - delta),  dP = dO V^T,  delta = rowsum(dO * O)
 //   dQ = dS K scale,  dK = dS^T Q scale,  dV = P^T dO,  the last two summed over the query heads of a key head
 //
-// Two kernels, no atomics: `cross_dq_kernel` owns rows and walks the keys (it also computes delta), `cross_dkdv_kernel` owns
-// keys and walks the rows of all heads. A wave keeps 32 rows (keys) in registers. Per step of 32 keys (rows) it issues the
+// Two kernels, no atomics: `cross_dq_kernel` (cross_dq.hip) owns rows and walks the keys (it also computes delta),
+// `cross_dkdv_kernel` owns keys and walks the rows of all heads. A wave keeps 32 rows (keys) in registers. Per step of 32 keys (rows) it issues the
 // first products of the next step and the second products of the one before, none of which wait for the step's exponentials. Tiles
 // come through registers into a ring of four LDS stages, one barrier per step. Where there are too few blocks to fill the
 // chip, the walked dimension is cut into parts, whose float32 sums `cross_sum_kernel` adds in order.
@@ -16,232 +16,10 @@
 #include <algorithm>
 #include <type_traits>
 
-#include "cross.h"
+#include "cross_bwd.h"
 
 namespace tattn {
 namespace {
-
-// A step's rows on their way from memory to LDS: two tiles of 32 rows, NT threads.
-template <int D, int NT>
-struct StepRows {
-  using B = BwdPipe<D>;
-  static constexpr int CPT = (B::CHUNKS + NT - 1) / NT;
-  uint32_t goff[2][CPT];
-  int ldst[CPT];
-  u32x4 x[2][CPT];
-  __device__ __forceinline__ void init(int tid, int64_t sa, int64_t sb) {
-#pragma unroll
-    for (int i = 0; i < CPT; ++i) {
-      const int ch = min(tid + i * NT, B::CHUNKS - 1), row = ch / B::CPR, cb = (ch % B::CPR) * 16;
-      goff[0][i] = (uint32_t)(row * sa * 2 + cb);
-      goff[1][i] = (uint32_t)(row * sb * 2 + cb);
-      ldst[i] = Swz<D>::addr(perm32(row), cb);
-    }
-  }
-  __device__ __forceinline__ void load(__amdgpu_buffer_rsrc_t a, __amdgpu_buffer_rsrc_t b, uint32_t oa, uint32_t ob) {
-#pragma unroll
-    for (int i = 0; i < CPT; ++i) {
-      x[0][i] = rsrc_load(a, goff[0][i] + oa);
-      x[1][i] = rsrc_load(b, goff[1][i] + ob);
-    }
-  }
-  __device__ __forceinline__ void store(char* stage, int tid) const {
-#pragma unroll
-    for (int i = 0; i < CPT; ++i)
-      if (B::CHUNKS % NT == 0 || tid + i * NT < B::CHUNKS) {
-        st16(stage + ldst[i], x[0][i]);
-        st16(stage + B::TILE + ldst[i], x[1][i]);
-      }
-  }
-  __device__ __forceinline__ void clear(char* stage, int tid) const {
-#pragma unroll
-    for (int i = 0; i < CPT; ++i)
-      if (B::CHUNKS % NT == 0 || tid + i * NT < B::CHUNKS) {
-        st16(stage + ldst[i], u32x4{});
-        st16(stage + B::TILE + ldst[i], u32x4{});
-      }
-  }
-};
-
-// ---- dQ ------------------------------------------------------------------------------------------
-template <typename T, int D, int NW, int OCC>
-__global__ __launch_bounds__(NW * 64, OCC) void cross_dq_kernel(const CrossParams p) {
-  using V8 = typename H16<T>::V8;
-  using B = BwdPipe<D>;
-  constexpr int NSD = B::NSD, DT = B::DT, STAGE = B::DQ_STAGE;
-  constexpr bool LIFT = std::is_same_v<T, f16>;
-  __shared__ __attribute__((aligned(16))) char smem[B::NST * STAGE];
-  __shared__ uint32_t norms[3][LIFT ? NW : 1];  // per wave: largest squared norm, |delta|, whether a row is lifted
-
-  const int tid = threadIdx.x;
-  const int lane = tid & 63, h2 = lane >> 5, l32 = lane & 31;
-  const int wu = (int)uniform32((uint32_t)(tid >> 6));
-  const float c = p.c;
-  int slice, blk;
-  if (!cross_coord(p.Zs * p.Hk, p.nblk * p.splits, slice, blk)) return;
-  const int split = blk % p.splits;
-  blk /= p.splits;
-  const CrossSlice sl(p, slice);
-  const int tiles = (sl.len + 31) >> 5;
-  const int i0 = (int)((int64_t)tiles * split / p.splits), i1 = (int)((int64_t)tiles * (split + 1) / p.splits);
-  const int nsteps = i1 - i0, rows = p.G * p.N;
-
-  const __amdgpu_buffer_rsrc_t krs = rows_rsrc<T, D>(p.k, sl.zs * p.sk[0] + sl.hk * p.sk[1], sl.len, p.sk[2]);
-  const __amdgpu_buffer_rsrc_t vrs = rows_rsrc<T, D>(p.v, sl.zs * p.sv[0] + sl.hk * p.sv[1], sl.len, p.sv[2]);
-  const uint32_t kb = uniform32((uint32_t)(p.sk[2] * 64)), vb = uniform32((uint32_t)(p.sv[2] * 64));
-  StepRows<D, NW * 64> next, second;
-  next.init(tid, p.sk[2], p.sv[2]);
-  second = next;
-  next.load(krs, vrs, (uint32_t)i0 * kb, (uint32_t)i0 * vb);
-  second.load(krs, vrs, (uint32_t)(i0 + 1) * kb, (uint32_t)(i0 + 1) * vb);
-
-  const int row = 32 * (blk * NW + wu) + l32;
-  const bool live = row < rows;
-  const CrossRow r(p, sl, live ? row : 0);
-  V8 qop[NSD], dop[NSD];
-  float dl;
-  int lift = 0;  // dS is scaled by 2^lift
-  uint32_t top = 0;
-  {
-    const T* qs = (const T*)p.q + r.at(p.sq) + 8 * h2;
-    const T* ds = (const T*)p.dout + r.at(p.sd) + 8 * h2;
-    const T* os = (const T*)p.o + r.at(p.so) + 8 * h2;
-    float sd[NSD], norm = 0.0f;
-#pragma unroll
-    for (int s = 0; s < NSD; ++s) {
-      const V8 x = *reinterpret_cast<const V8*>(qs + 16 * s), y = *reinterpret_cast<const V8*>(ds + 16 * s);
-      qop[s] = live ? x : V8{};
-      dop[s] = live ? y : V8{};
-      sd[s] = chunk_dot(*reinterpret_cast<const V8*>(os + 16 * s), y);
-      if (LIFT) norm += chunk_dot(dop[s], dop[s]);
-    }
-    dl = row_delta(sd);
-    if (!live) dl = 0.0f;
-    if (live && h2 == 0 && split == 0) p.delta[(int64_t)slice * rows + row] = -dl;
-    if constexpr (LIFT) {
-      const uint32_t bits = __builtin_bit_cast(uint32_t, sum_halves(norm));
-      lift = small_gradient_lift(norm_exponent(bits), 60);
-      top = max_wave(bits);  // NaN above all
-      norms[0][wu] = top;
-      norms[1][wu] = max_wave(__builtin_bit_cast(uint32_t, __builtin_fabsf(dl)));
-      norms[2][wu] = __builtin_amdgcn_ballot_w64(lift > 0) != 0;
-    }
-  }
-  const float m = live ? p.m[r.index(p)] : 0.0f;
-  float nm = live ? (float)lift - m : 0.0f;
-  CrossOp<D> at;
-  at.init(lane);
-  f32x16 dq[DT];
-
-  // S^T and dP^T - delta of a stage's 32 keys (lane = row, register r = key kappa(r, h2)).
-  auto first = [&](f32x16& s, f32x16& dp, int st) __attribute__((always_inline)) {
-    const char* base = smem + st * STAGE;
-    s = f32x16{};
-#pragma unroll
-    for (int i = 0; i < 16; ++i) dp[i] = -dl;
-#pragma unroll
-    for (int sd = 0; sd < NSD; ++sd) {
-      s = Elt<T>::mfma(lds8<T>(base + at.nat[sd]), qop[sd], s);
-      dp = Elt<T>::mfma(lds8<T>(base + B::TILE + at.nat[sd]), dop[sd], dp);
-    }
-  };
-  auto grad = [&](const V8 (&ds)[2], int st) __attribute__((always_inline)) {
-#pragma unroll
-    for (int g = 0; g < 2; ++g)
-#pragma unroll
-      for (int u = 0; u < DT; ++u) dq[u] = Elt<T>::mfma(at.template tr<T>(smem + st * STAGE, g, u, lane), ds[g], dq[u]);
-  };
-  auto dsv = [&](const f32x16& s, const f32x16& dp, V8 (&ds)[2], int left, auto mask_tag) __attribute__((always_inline)) {
-    constexpr bool MASK = decltype(mask_tag)::value;
-#pragma unroll
-    for (int a = 0; a < 2; ++a)
-#pragma unroll
-      for (int i = 0; i < 8; i += 2) {
-        float x[2];
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const int g = 8 * a + i + e;
-          float pr = fast_exp2(__builtin_fmaf(s[g], c, nm));
-          if constexpr (MASK) pr = kappa(g, h2) >= left ? 0.0f : pr;
-          x[e] = pr * dp[g];
-        }
-        const auto y = H16<T>::pack(x[0], x[1]);
-        ds[a][i] = y[0];
-        ds[a][i + 1] = y[1];
-      }
-  };
-
-  next.clear(smem + 3 * STAGE, tid);  // read by the first step together with all-zero dS
-  next.store(smem, tid);
-  second.store(smem + STAGE, tid);
-  __syncthreads();
-  uint32_t lifted = 0;
-  if constexpr (LIFT) {
-    if (tid < 2 && split == 0) {  // for dK / dV
-      top = norms[tid][0];
-#pragma unroll
-      for (int k = 1; k < NW; ++k) top = max(top, norms[tid][k]);
-      p.norms[2 * ((int64_t)slice * p.nblk + blk) + tid] = __builtin_bit_cast(float, top);
-    }
-#pragma unroll
-    for (int k = 0; k < NW; ++k) lifted |= norms[2][k];
-    lifted = uniform32(lifted);
-  }
-  // Steps whose 32 keys are all there.
-  const int n_full = min(nsteps, (sl.len >> 5) - i0);
-  for (;;) {
-#pragma unroll
-    for (int u = 0; u < DT; ++u) dq[u] = f32x16{};
-    f32x16 sa, da, sb, db;
-    V8 ea[2] = {}, eb[2];
-    if (nsteps > 0) first(sa, da, 0);
-    auto step = [&](int i, int st, f32x16& s0, f32x16& d0, f32x16& s1, f32x16& d1, const V8 (&e0)[2], V8 (&e1)[2], auto mask_tag)
-                    __attribute__((always_inline)) {
-      next.load(krs, vrs, (uint32_t)(i0 + i + 2) * kb, (uint32_t)(i0 + i + 2) * vb);
-      first(s1, d1, (st + 1) & 3);
-      grad(e0, (st + 3) & 3);
-      dsv(s0, d0, e1, sl.len - 32 * (i0 + i), mask_tag);
-      next.store(smem + ((st + 2) & 3) * STAGE, tid);
-      __syncthreads();
-    };
-    int i = 0;
-    for (; i + 3 < n_full; i += 4) {
-      step(i, 0, sa, da, sb, db, ea, eb, std::false_type{});
-      step(i + 1, 1, sb, db, sa, da, eb, ea, std::false_type{});
-      step(i + 2, 2, sa, da, sb, db, ea, eb, std::false_type{});
-      step(i + 3, 3, sb, db, sa, da, eb, ea, std::false_type{});
-    }
-    for (; i < nsteps; ++i) {
-      step(i, i & 3, sa, da, sb, db, ea, eb, std::true_type{});
-      sa = sb;
-      da = db;
-      ea[0] = eb[0];
-      ea[1] = eb[1];
-    }
-    if (nsteps > 0) grad(ea, (nsteps - 1) & 3);
-    if (!LIFT || !lifted) break;
-    float zero = 0.0f;  // times every sum: NaN where one is not finite
-#pragma unroll
-    for (int u = 0; u < DT; ++u)
-#pragma unroll
-      for (int g = 0; g < 16; ++g) zero = __builtin_fmaf(dq[u][g], 0.0f, zero);
-    if (!__syncthreads_or(lift > 0 && zero != 0.0f)) break;
-    lifted = lift = 0;  // once more without a factor
-    nm = -m;
-    next.load(krs, vrs, (uint32_t)i0 * kb, (uint32_t)i0 * vb);
-    second.load(krs, vrs, (uint32_t)(i0 + 1) * kb, (uint32_t)(i0 + 1) * vb);
-    next.clear(smem + 3 * STAGE, tid);
-    next.store(smem, tid);
-    second.store(smem + STAGE, tid);
-    __syncthreads();
-  }
-  if (!live) return;
-  const float unlift = LIFT ? unlift_of(lift) : 1.0f;
-  if (p.splits > 1)
-    store_row_t<float, D>(p.part + (((int64_t)slice * p.splits + split) * rows + row) * D, dq, unlift, h2);
-  else
-    store_row_t<T, D>((T*)p.out + r.at(p.sout), dq, p.scale * unlift, h2);
-}
 
 // ---- dK / dV -------------------------------------------------------------------------------------
 // What dS of a block of keys is scaled by, the same for the workgroup: up to the largest norm of the slice's rows of dO, and
@@ -283,7 +61,7 @@ __global__ __launch_bounds__(NW * 64, OCC) void cross_dkdv_kernel(const CrossPar
   const int wu = (int)uniform32((uint32_t)(tid >> 6));
   const float c = p.c;
   int slice, item;
-  if (!cross_coord(p.Zs * p.Hk, p.kblk * p.parts, slice, item)) return;
+  if (!cross_coord(p, p.kblk * p.parts, slice, item)) return;
   const int kbi = item / p.parts, part = item % p.parts;
   const CrossSlice sl(p, slice);
   const int kw0 = KEYS * kbi + 32 * wu, key = kw0 + l32;
@@ -519,8 +297,10 @@ int sum_d(const CrossParams& p, bool keys, int block, hipStream_t st) {
 }
 
 // ---- launch --------------------------------------------------------------------------------------
-constexpr int kRowWaves = 4;                            // row tiles of a dQ workgroup
-constexpr int key_waves(int D) { return D == 128 ? 4 : 8; }  // key tiles of a dK / dV workgroup
+constexpr int kRowTiles = 4;  // row tiles of a dQ workgroup
+// Key tiles of a dK / dV workgroup. Eight take 145 us where four take 121 (whole backward, 16 x 8 x 4,096 over 77 x 64), 184 for 175
+// (8 x 16 x 1,024 over 375 to 1,500 x 64), 1,012 for 995 (4 x 16 x 4,096 over 4,096 x 64).
+constexpr int kKeyTiles = 4;
 constexpr int bwd_occ(int D) { return D == 128 ? 1 : 2; }
 
 // Rows that lie at one stride, whatever head they belong to, are walked as one head's: no tile holds the end of a head.
@@ -544,14 +324,12 @@ template <typename T, int D>
 int bwd_d(const CrossParams& p, hipStream_t st) {
   unsigned blocks;
   int rc;
-  if ((rc = cross_grid(p.slices(), (int64_t)p.nblk * p.splits, &blocks))) return rc;
-  cross_dq_kernel<T, D, kRowWaves, bwd_occ(D)><<<dim3(blocks), dim3(kRowWaves * 64), 0, st>>>(p);
-  if ((rc = check_launch("tattn_cross_bwd")) || (p.splits > 1 && (rc = sum_d<T, D>(p, false, 0, st)))) return rc;
-  constexpr int KW = key_waves(D);
+  if ((rc = launch_cross_dq(p, D, std::is_same_v<T, f16> ? 0 : 2, st))) return rc;
+  if (p.splits > 1 && (rc = sum_d<T, D>(p, false, 0, st))) return rc;
   if ((rc = cross_grid(p.slices(), (int64_t)p.kblk * p.parts, &blocks))) return rc;
-  cross_dkdv_kernel<T, D, KW, bwd_occ(D)><<<dim3(blocks), dim3(KW * 64), 0, st>>>(walked(p));
+  cross_dkdv_kernel<T, D, kKeyTiles, bwd_occ(D)><<<dim3(blocks), dim3(64 * kKeyTiles), 0, st>>>(walked(p));
   if ((rc = check_launch("tattn_cross_bwd")) || p.parts == 1) return rc;
-  return sum_d<T, D>(p, true, 32 * KW, st);
+  return sum_d<T, D>(p, true, 32 * kKeyTiles, st);
 }
 
 }  // namespace
@@ -559,8 +337,8 @@ int bwd_d(const CrossParams& p, hipStream_t st) {
 // Blocks are cut into parts while all of them together leave half of the chip's places empty (two workgroups a CU, one at head dim
 // 128); a part has at least 8 tiles of keys or 16 of rows.
 void cross_bwd_plan(CrossParams& p, int D, int dtype) {
-  const int64_t slices = p.slices(), places = 256 * bwd_occ(D), keys = dtype == 1 ? 128 : 32 * key_waves(D);
-  p.nblk = (int)((p.rows() + 32 * kRowWaves - 1) / (32 * kRowWaves));
+  const int64_t slices = p.slices(), places = 256 * bwd_occ(D), keys = 32 * kKeyTiles;
+  p.nblk = (int)((p.rows() + 32 * kRowTiles - 1) / (32 * kRowTiles));
   p.kblk = (int)((p.S + keys - 1) / keys);
   const int64_t rt = (int64_t)p.G * ((p.N + 31) / 32), kt = ((int64_t)p.S + 31) / 32;
   p.splits = (int)std::max<int64_t>(1, std::min<int64_t>(places / (slices * p.nblk), kt / 8));
@@ -569,13 +347,12 @@ void cross_bwd_plan(CrossParams& p, int D, int dtype) {
 
 namespace {
 int64_t even(int64_t x) { return (x + 3) / 4 * 4; }
-int64_t key_block(int D, int dtype) { return dtype == 1 ? 128 : 32 * key_waves(D); }
 }  // namespace
 
 int64_t cross_bwd_floats(const CrossParams& p, int D, int dtype) {
   const int64_t rows = p.slices() * p.rows();
   return even(rows) + (dtype == 0 ? even(2 * p.slices() * p.nblk) : 0) + (p.splits > 1 ? rows * p.splits * D : 0) +
-         (p.parts > 1 ? p.slices() * p.kblk * p.parts * 2 * key_block(D, dtype) * D : 0);
+         (p.parts > 1 ? p.slices() * p.kblk * p.parts * 2 * 32 * kKeyTiles * D : 0);
 }
 
 void cross_bwd_workspace(CrossParams& p, int D, int dtype, float* work) {

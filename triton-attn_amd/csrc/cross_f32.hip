@@ -13,7 +13,7 @@ struct CrossRows32 {
   int slice, blk, split, row, rows, i0, i1;
   bool ok, live;
   __device__ __forceinline__ CrossRows32(const CrossParams& p, int w, int l32) {
-    ok = cross_coord(p.Zs * p.Hk, p.nblk * p.splits, slice, blk);
+    ok = cross_coord(p, p.nblk * p.splits, slice, blk);
     if (!ok) return;
     split = blk % p.splits;
     blk /= p.splits;
@@ -160,7 +160,7 @@ __global__ __launch_bounds__(256, 1) void cross_dkdv_f32_kernel(const CrossParam
   __shared__ __attribute__((aligned(16))) float md[2][32];  // M, -delta
   const int tid = threadIdx.x, lane = tid & 63, h2 = lane >> 5, l32 = lane & 31, w = (int)uniform32(tid >> 6);
   int slice, item;
-  if (!cross_coord(p.Zs * p.Hk, p.kblk * p.parts, slice, item)) return;
+  if (!cross_coord(p, p.kblk * p.parts, slice, item)) return;
   const int kb = item / p.parts, part = item % p.parts;
   const CrossSlice sl(p, slice);
   const int nq = (p.N + 31) >> 5, total = 128 * kb < sl.len ? nq * p.G : 0;

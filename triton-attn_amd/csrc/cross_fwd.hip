@@ -37,7 +37,7 @@ __global__ __launch_bounds__(NW * 64, OCC) void cross_pipe_kernel(const CrossPar
   const int wu = (int)uniform32((uint32_t)(tid >> 6));
   const float c = p.c;
   int slice, blk;
-  if (!cross_coord(p.Zs * p.Hk, p.nblk * p.splits, slice, blk)) return;
+  if (!cross_coord(p, p.nblk * p.splits, slice, blk)) return;
   const int split = blk % p.splits;
   blk /= p.splits;
   const CrossSlice sl(p, slice);

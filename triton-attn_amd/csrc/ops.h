@@ -188,6 +188,7 @@ constexpr int cross_pipe_waves(int D) { return 4; }
 constexpr int cross_pipe_tiles(int D) { return D == 128 ? 1 : 2; }
 constexpr int cross_pipe_rows(int D) { return 32 * cross_pipe_waves(D) * cross_pipe_tiles(D); }
 int launch_cross_bwd(const CrossParams& p, int D, int dtype, hipStream_t st);
+int launch_cross_dq(const CrossParams& p, int D, int dtype, hipStream_t st);  // 16-bit; dQ (its parts) and delta
 int launch_cross_f32(const CrossParams& p, int D, bool bwd, hipStream_t st);
 int launch_cross_combine(const CrossParams& p, int D, int dtype, hipStream_t st);  // joins the forward's parts
 // Adds the parts of dQ, or of dK and dV for key blocks of `block` keys.

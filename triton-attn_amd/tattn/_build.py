@@ -21,19 +21,24 @@ LIB = PKG / "libtattn_hip.so"
 SOURCES = ["abi.hip", "fwd.hip", "fwd_persist_causal.hip", "bwd.hip", "bwd_dq_persist.hip", "bwd_dkdv_persist.hip",
            "bwd_split.hip", "short.hip", "coop.hip", "f32_split.hip",
            "abi_ops.hip", "paged.hip", "norm_rope.hip", "window.hip",
-           "window_f32.hip", "cache4_attention.hip", "cross.hip", "cross_fwd.hip", "cross_bwd.hip", "cross_f32.hip", "rope_axes.hip"]
+           "window_f32.hip", "cache4_attention.hip", "cross.hip", "cross_fwd.hip", "cross_bwd.hip", "cross_dq.hip", "cross_f32.hip", "rope_axes.hip"]
 # Per-source flags. fwd.hip: keep each step's softmax work in the step that issues the
 # independent MFMAs it interleaves with (machine sinking would move it to its first use).
 # fwd_persist_causal.hip (persistent causal forward, two tiles per wave), bwd_dq_persist.hip
 # (persistent dQ) and bwd_split.hip (paired-wave dK/dV and dQ) hold one kernel family each so
 # that they can take the LLVM instruction scheduler that measured fastest for them, and window.hip
-# takes the same (head dim 128: dQ 5% faster, the rest 1-2%); the other kernels are slower under either.
+# takes the same (head dim 128: dQ 5% faster, the rest 1-2%); the other kernels are slower under either. Attention over
+# another length: cross_fwd.hip as fwd.hip; dK / dV (cross_bwd.hip) are 2-8% faster under iterative-ilp and 5-9% slower under max-ilp,
+# dQ by pairs of waves (cross_dq.hip) takes 419 us under max-ilp, 457 under the default and 481 under iterative-ilp
+# (2 x 16 x 4,096 over 4,096 x 128).
 SOURCE_FLAGS = {
     "fwd.hip": ["-mllvm", "-disable-machine-sink"],
     "fwd_persist_causal.hip": ["-mllvm", "-disable-machine-sink", "-mllvm", "-amdgpu-sched-strategy=iterative-ilp"],
     "bwd_dq_persist.hip": ["-mllvm", "-amdgpu-sched-strategy=max-ilp"],
     "bwd_split.hip": ["-mllvm", "-amdgpu-sched-strategy=iterative-ilp"],
     "window.hip": ["-mllvm", "-amdgpu-sched-strategy=iterative-ilp"],
+    "cross_dq.hip": ["-mllvm", "-amdgpu-sched-strategy=max-ilp"],
+    "cross_bwd.hip": ["-mllvm", "-amdgpu-sched-strategy=iterative-ilp"],
     "cross_fwd.hip": ["-mllvm", "-disable-machine-sink"],
 }
 ARCH = "gfx950"
