@@ -352,6 +352,7 @@ template <typename T, int D>
 int fwd_d(const CrossParams& p, hipStream_t st) {
   unsigned blocks;
   int rc;
+  if (cross_short(p, D, std::is_same_v<T, f16> ? 0 : 2, false)) return launch_cross_short(p, D, std::is_same_v<T, f16> ? 0 : 2, false, st);
   if (p.pipe) {
     if ((rc = launch_cross_pipe(p, D, std::is_same_v<T, f16> ? 0 : 2, st)) || p.splits == 1) return rc;
     return combine_cross<T, D>(p, st);
@@ -380,14 +381,20 @@ int prefix_d(const PrefixParams& p, hipStream_t st) {
 }  // namespace
 
 // Up to two row tiles: one per workgroup (rows_block). More: blocks of cross_pipe_rows. Keys are cut into parts until the chip
-// holds no more workgroups at once, of at least eight tiles.
+// holds no more workgroups at once, of at least eight tiles (in float32, where a tile takes eight times as long, three).
 void cross_fwd_plan(CrossParams& p, int D, int dtype) {
+  if (cross_short(p, D, dtype, false)) {  // row tiles of a slice in parts, four a workgroup for a wave at least
+    const int64_t tiles = (p.rows() + 31) / 32;
+    p.nblk = (int)std::max<int64_t>(1, std::min<int64_t>(1024 / p.slices(), tiles / 16));
+    p.splits = 1;
+    return;
+  }
   const int64_t tiles = ((int64_t)p.S + 31) / 32;
   p.pipe = dtype != 1 && p.rows() > 64;
   const int64_t block = dtype == 1 ? 128 : p.pipe ? cross_pipe_rows(D) : 32;
   p.nblk = (int)((p.rows() + block - 1) / block);
   const int64_t blocks = p.slices() * p.nblk, want = 256 * (p.pipe ? 2 : rows_occ(D));
-  p.splits = (int)std::max<int64_t>(1, std::min<int64_t>(want / blocks, tiles / 8));
+  p.splits = (int)std::max<int64_t>(1, std::min<int64_t>(want / blocks, tiles / (dtype == 1 ? 3 : 8)));
 }
 
 // The parts of all rows together, prefixes and own keys, are about as many as the chip holds at once; none has less than eight

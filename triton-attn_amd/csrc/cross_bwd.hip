@@ -324,6 +324,7 @@ template <typename T, int D>
 int bwd_d(const CrossParams& p, hipStream_t st) {
   unsigned blocks;
   int rc;
+  if (cross_short(p, D, std::is_same_v<T, f16> ? 0 : 2, true)) return launch_cross_short(p, D, std::is_same_v<T, f16> ? 0 : 2, true, st);
   if ((rc = launch_cross_dq(p, D, std::is_same_v<T, f16> ? 0 : 2, st))) return rc;
   if (p.splits > 1 && (rc = sum_d<T, D>(p, false, 0, st))) return rc;
   if ((rc = cross_grid(p.slices(), (int64_t)p.kblk * p.parts, &blocks))) return rc;
@@ -335,14 +336,20 @@ int bwd_d(const CrossParams& p, hipStream_t st) {
 }  // namespace
 
 // Blocks are cut into parts while all of them together leave half of the chip's places empty (two workgroups a CU, one at head dim
-// 128); a part has at least 8 tiles of keys or 16 of rows.
+// 128); a part has at least 8 tiles of keys or 16 of rows, in float32, where a tile takes eight times as long, three.
 void cross_bwd_plan(CrossParams& p, int D, int dtype) {
   const int64_t slices = p.slices(), places = 256 * bwd_occ(D), keys = 32 * kKeyTiles;
+  if (cross_short(p, D, dtype, true)) {  // row tiles of a slice in as many parts as the chip holds at once, two a wave at least
+    const int nt = (p.S + 31) / 32;
+    p.nblk = p.splits = p.kblk = 1;
+    p.parts = (int)std::max<int64_t>(1, std::min<int64_t>(256 * cross_short_occ(D, nt) / slices, (p.rows() + 31) / 32 / 8));
+    return;
+  }
   p.nblk = (int)((p.rows() + 32 * kRowTiles - 1) / (32 * kRowTiles));
   p.kblk = (int)((p.S + keys - 1) / keys);
   const int64_t rt = (int64_t)p.G * ((p.N + 31) / 32), kt = ((int64_t)p.S + 31) / 32;
-  p.splits = (int)std::max<int64_t>(1, std::min<int64_t>(places / (slices * p.nblk), kt / 8));
-  p.parts = (int)std::max<int64_t>(1, std::min<int64_t>(places / (slices * p.kblk), rt / 16));
+  p.splits = (int)std::max<int64_t>(1, std::min<int64_t>(places / (slices * p.nblk), kt / (dtype == 1 ? 3 : 8)));
+  p.parts = (int)std::max<int64_t>(1, std::min<int64_t>(places / (slices * p.kblk), rt / (dtype == 1 ? 3 : 16)));
 }
 
 namespace {
@@ -351,12 +358,17 @@ int64_t even(int64_t x) { return (x + 3) / 4 * 4; }
 
 int64_t cross_bwd_floats(const CrossParams& p, int D, int dtype) {
   const int64_t rows = p.slices() * p.rows();
+  if (cross_short(p, D, dtype, true)) return p.parts > 1 ? p.slices() * p.parts * 2 * ((p.S + 31) / 32 * 32) * D : 4;
   return even(rows) + (dtype == 0 ? even(2 * p.slices() * p.nblk) : 0) + (p.splits > 1 ? rows * p.splits * D : 0) +
          (p.parts > 1 ? p.slices() * p.kblk * p.parts * 2 * 32 * kKeyTiles * D : 0);
 }
 
 void cross_bwd_workspace(CrossParams& p, int D, int dtype, float* work) {
   const int64_t rows = p.slices() * p.rows();
+  if (cross_short(p, D, dtype, true)) {
+    p.kpart = work;
+    return;
+  }
   p.delta = work;
   p.norms = p.delta + even(rows);
   p.part = p.norms + (dtype == 0 ? even(2 * p.slices() * p.nblk) : 0);

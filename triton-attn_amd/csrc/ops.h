@@ -188,6 +188,11 @@ constexpr int cross_pipe_waves(int D) { return 4; }
 constexpr int cross_pipe_tiles(int D) { return D == 128 ? 1 : 2; }
 constexpr int cross_pipe_rows(int D) { return 32 * cross_pipe_waves(D) * cross_pipe_tiles(D); }
 int launch_cross_bwd(const CrossParams& p, int D, int dtype, hipStream_t st);
+// Up to four tiles of keys (backward two at head dim 128, for the registers of a wave): cross_short.hip.
+constexpr int cross_short_tiles(int D, bool bwd) { return D == 128 && bwd ? 2 : 4; }
+constexpr int cross_short_occ(int D, int tiles) { return tiles * ((D + 31) / 32) <= 3 ? 2 : 1; }  // waves per SIMD of the backward
+inline bool cross_short(const CrossParams& p, int D, int dtype, bool bwd) { return dtype != 1 && p.S <= 32 * cross_short_tiles(D, bwd); }
+int launch_cross_short(const CrossParams& p, int D, int dtype, bool bwd, hipStream_t st);
 int launch_cross_dq(const CrossParams& p, int D, int dtype, hipStream_t st);  // 16-bit; dQ (its parts) and delta
 int launch_cross_f32(const CrossParams& p, int D, bool bwd, hipStream_t st);
 int launch_cross_combine(const CrossParams& p, int D, int dtype, hipStream_t st);  // joins the forward's parts

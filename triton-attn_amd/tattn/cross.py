@@ -18,7 +18,7 @@ from torch.autograd.function import once_differentiable
 from tattn import _lib
 from tattn._args import aligned, check_index, layouts, no_tangents, remember, rows_apart, same_device, strides
 from tattn.api import _DTYPES, _on_device, _require_gpu, _stream
-from tattn.window import _tiles, _tiles_apart
+from tattn.window import _tiles_apart
 
 
 def _check_heads(q, k, v, names: str) -> None:
@@ -55,21 +55,22 @@ _plans: dict[tuple, tuple] = {}
 
 def _plan(q, k, v, lens) -> tuple:
     """Checks a call; which of q, k, v are copied, the strides of inputs and output (None where one is copied), the float32
-    values of workspace of forward and backward, and the sizes among the launches' arguments (None: nothing to see)."""
+    values of workspace of forward and backward, the sizes among the launches' arguments (None: nothing to see), and what the
+    backward found for gradients of each layout: which of its five inputs are copied, and all strides."""
     _check_cross(q, k, v, lens)
     _require_gpu(q)
     copies = rows_apart(q), _tiles_apart(k), _tiles_apart(v)
     z, h, n, d = q.shape
     hk, s = k.shape[1:3]
     if q.numel() == 0 or s == 0:
-        return copies, None, 0, 0, None
+        return copies, None, 0, 0, None, {}
     sizes = (z, h, hk, n, s, d, _DTYPES[q.dtype])
     return (copies, None if any(copies) else strides(q, k, v, torch.empty_like(q)), _workspace(False, sizes),
-            _workspace(True, sizes), sizes)
+            _workspace(True, sizes), sizes, {})
 
 
 def _forward(q, k, v, lens, plan, scale, save_lse) -> tuple[torch.Tensor, torch.Tensor | None]:
-    copies, held, floats, _, sizes = plan
+    copies, held, floats, _, sizes, _ = plan
     given = q, k, v
     q, k, v = aligned(q, copies[0]), aligned(k, copies[1]), aligned(v, copies[2])
     o = torch.empty_like(q)
@@ -88,13 +89,25 @@ def _forward(q, k, v, lens, plan, scale, save_lse) -> tuple[torch.Tensor, torch.
 
 
 def _backward(q, k, v, o, m, lens, do, plan, scale) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
-    floats, sizes = plan[3:]
-    q, k, v, o, do = _tiles(q), _tiles(k), _tiles(v), _tiles(o), _tiles(do)
+    floats, sizes, layouts_of = plan[3:]
+    given = q, k, v, o, do
+    key = o.stride(), do.stride()
+    hit = layouts_of.get(key)
+    copies = hit[0] if hit else tuple([_tiles_apart(t) for t in given])
+    tensors = tuple([aligned(t, c) for t, c in zip(given, copies)])
+    q, k, v, o, do = tensors
     dq, dk, dv = torch.empty_like(q), torch.empty_like(k), torch.empty_like(v)
     if sizes is None:
         return dq.zero_(), dk.zero_(), dv.zero_()
     work = m.new_empty(floats)
-    _, st = strides(q, k, v, o, do, dq, dk, dv)
+    in_place = q is given[0] and k is given[1] and v is given[2] and o is given[3] and do is given[4]
+    if hit and hit[1] and in_place:
+        held = hit[1]
+    else:
+        held = strides(*tensors, dq, dk, dv)
+        if hit is None or in_place:
+            remember(layouts_of, key, (copies, held if in_place else None))
+    _, st = held
     with _on_device(q):
         rc = _lib.load().tattn_cross_bwd(
             q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), do.data_ptr(), dq.data_ptr(), dk.data_ptr(),
@@ -196,18 +209,20 @@ def prefix_attention(
     Query n is at position lens - queries + n of its sequence's own keys and sees the whole prefix and its own keys up to its
     position; rows at positions below 0 give zeros. What lies behind the lengths reaches nothing. sm_scale defaults to
     1 / sqrt(dim). For serving: refuses inputs that require gradients or carry forward-mode ones."""
-    tensors = q, prefix_k, prefix_v, k, v
-    no_tangents(*tensors)
-    if torch.is_grad_enabled() and any(t.requires_grad for t in tensors):
+    no_tangents(q, prefix_k, prefix_v, k, v)
+    if torch.is_grad_enabled() and (q.requires_grad or prefix_k.requires_grad or prefix_v.requires_grad or k.requires_grad
+                                    or v.requires_grad):
         raise ValueError("prefix_attention has no gradients: call it under torch.no_grad()")
-    key = layouts(*tensors, lens, prefix_lens)
+    key = layouts(q, prefix_k, prefix_v, k, v, lens, prefix_lens)
     plan = _prefix_plans.get(key)
     if plan is None:
-        plan = remember(_prefix_plans, key, _prefix_plan(*tensors, lens, prefix_lens))
+        plan = remember(_prefix_plans, key, _prefix_plan(q, prefix_k, prefix_v, k, v, lens, prefix_lens))
     copies, held, floats, sizes = plan
-    given = tensors
-    tensors = tuple([aligned(t, c) for t, c in zip(tensors, copies)])
-    q, prefix_k, prefix_v, k, v = tensors
+    pointers = [q.data_ptr(), prefix_k.data_ptr(), prefix_v.data_ptr(), k.data_ptr(), v.data_ptr()]
+    if held is None or (pointers[0] | pointers[1] | pointers[2] | pointers[3] | pointers[4]) & 15:
+        tensors = [aligned(t, c) for t, c in zip((q, prefix_k, prefix_v, k, v), copies)]
+        q, pointers = tensors[0], [t.data_ptr() for t in tensors]
+        held = strides(*tensors, torch.empty_like(q))
     o = torch.empty_like(q)
     if sizes is None:
         return o
@@ -215,13 +230,10 @@ def prefix_attention(
     if prefix_lens is not None:
         prefix_lens = prefix_lens.contiguous()
     work = q.new_empty(floats, dtype=torch.float32)
-    same = held and all([a is b for a, b in zip(tensors, given)])
-    _, st = held if same else strides(*tensors, o)
     with _on_device(q):
         rc = _lib.load().tattn_prefix_attention(
-            q.data_ptr(), prefix_k.data_ptr(), prefix_v.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(),
-            None if prefix_lens is None else prefix_lens.data_ptr(), lens.data_ptr(), work.data_ptr(), *st, *sizes,
-            float(sm_scale) if sm_scale is not None else 1.0 / math.sqrt(q.shape[3]), _stream(q))
+            *pointers, o.data_ptr(), None if prefix_lens is None else prefix_lens.data_ptr(), lens.data_ptr(), work.data_ptr(),
+            *held[1], *sizes, float(sm_scale) if sm_scale is not None else 1.0 / math.sqrt(q.shape[3]), _stream(q))
     if rc:
         _lib.check(rc, "tattn_prefix_attention")
     return o

@@ -125,7 +125,9 @@ def qk_rope_axes(
     rounded once. Any batch, head and sequence strides are read in place."""
     no_tangents(q, k, q_weight, k_weight, cos, sin)
     interleaved = bool(interleaved)
-    axes = tuple([whole("axis", a) for a in axes])
+    axes = tuple(axes)
+    if set(map(type, axes)) != {int}:
+        axes = tuple([whole("axis", a) for a in axes])
     key = (layouts(q, k, q_weight, k_weight, cos, sin, positions), axes, interleaved)
     plan = _plans.get(key)
     if plan is None:
