@@ -99,6 +99,12 @@ __device__ __forceinline__ void wave_landed() {
   __atomic_signal_fence(__ATOMIC_SEQ_CST);
 }
 
+// This wave's LDS reads are done: a load into what it read may start.
+__device__ __forceinline__ void reads_done() {
+  __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0)
+  __atomic_signal_fence(__ATOMIC_SEQ_CST);
+}
+
 // Hides the keys past a row's last one in a tile of S^T: register r of lane half h2 is key 32 t + 8 h2 + 16 (r / 8) + r % 8.
 __device__ __forceinline__ void hide_after(f32x16& s, int last, int t, int h2, float hidden) {
   const int hi = last - 32 * t - 8 * h2;

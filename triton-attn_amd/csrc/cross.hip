@@ -2,8 +2,8 @@
 //
 //   O = softmax(c' Q K^T) V over the first len keys, one pass over the keys with the running max and sum of the softmax
 //
-// Few rows (`rows_block`): four waves share 32 QT rows, and each takes every fourth key tile by itself, staged by LDS DMA
-// into its own two stages: no barrier until the four partial results are added. The keys are cut into parts where rows are few, and
+// Few rows (`rows_block`): four waves share 32 rows, and each takes every fourth key tile by itself, staged by LDS DMA
+// into LDS of its own: no barrier until the four partial results are added. The keys are cut into parts where rows are few, and
 // `combine_kernel` joins the parts in order.
 //
 // Roundings: P is rounded to the element type, as the matrix instruction takes it, and its sum is taken from the rounded values.
@@ -18,15 +18,10 @@ namespace {
 
 constexpr int kWaves = 4;  // of a workgroup of rows_block
 
-template <int D>
-struct RowsLds {
-  static constexpr int STAGE = kWaves * 2 * CrossTile<D>::BYTES;  // each wave's K and V tile
-};
-
-// The part `split` of the keys for row block blk of a slice. CAUSAL: query n is at position len - N + n and sees no key after it.
-template <typename T, int D, int QT, bool CAUSAL>
-__device__ __forceinline__ void rows_block(const CrossParams& p, int slice, int blk, int split, char* s0, char* s1,
-                                           float (*red)[kWaves][64]) {
+// The part `split` of the keys for 32 rows of a slice. CAUSAL: query n is at position len - N + n and sees no key after it.
+template <typename T, int D, bool CAUSAL>
+__device__ __forceinline__ void rows_block(const CrossParams& p, int slice, int blk, int split, char* kbuf, char* vbuf,
+                                           float (*red)[kWaves][32]) {
   using V4 = typename H16<T>::V4;
   using V8 = typename H16<T>::V8;
   using Tile = CrossTile<D>;
@@ -49,29 +44,33 @@ __device__ __forceinline__ void rows_block(const CrossParams& p, int slice, int 
     gk[i] = Tile::source(i, lane, p.sk[2]);
     gv[i] = Tile::source(i, lane, p.sv[2]);
   }
-  const int mine = wu * 2 * Tile::BYTES;
-  auto issue = [&](char* st, int t) __attribute__((always_inline)) {
+  char *kt = kbuf + wu * Tile::BYTES, *vt = vbuf + wu * Tile::BYTES;
+  auto fetch_k = [&](int t) __attribute__((always_inline)) {
 #pragma unroll
-    for (int i = 0; i < PIECES; ++i) dma16(krs, st + mine + 1024 * i, gk[i] + (uint32_t)t * kb);
+    for (int i = 0; i < PIECES; ++i) dma16(krs, kt + 1024 * i, gk[i] + (uint32_t)t * kb);
+  };
+  auto fetch_v = [&](int t) __attribute__((always_inline)) {
 #pragma unroll
-    for (int i = 0; i < PIECES; ++i) dma16(vrs, st + mine + Tile::BYTES + 1024 * i, gv[i] + (uint32_t)t * vb);
+    for (int i = 0; i < PIECES; ++i) dma16(vrs, vt + 1024 * i, gv[i] + (uint32_t)t * vb);
   };
   int t = i0 + wu;
-  if (t < i1) issue(s0, t);
+  if (t < i1) {
+    fetch_k(t);
+    fetch_v(t);
+  }
 
-  V8 qop[QT][NSD];
-  int last[QT];  // last key that the lane's row sees
-#pragma unroll
-  for (int j = 0; j < QT; ++j) {
-    const int row = 32 * (QT * blk + j) + l32;
+  const int row = 32 * blk + l32;
+  V8 qop[NSD];
+  int last = sl.len - 1;  // key that the lane's row sees
+  {
     const bool live = row < rows;
     const CrossRow r(p, sl, live ? row : 0);
+    if (CAUSAL) last = sl.len - p.N + r.n;
     const T* src = (const T*)p.q + r.at(p.sq) + 8 * h2;
-    last[j] = CAUSAL ? sl.len - p.N + r.n : sl.len - 1;
 #pragma unroll
     for (int s = 0; s < NSD; ++s) {
       const V8 x = *reinterpret_cast<const V8*>(src + 16 * s);
-      qop[j][s] = live ? x : V8{};
+      qop[s] = live ? x : V8{};
     }
   }
   // Tiles from here on hold keys that some row does not see.
@@ -79,120 +78,76 @@ __device__ __forceinline__ void rows_block(const CrossParams& p, int slice, int 
   CrossOp<D> at;
   at.init(lane);
 
-  float mrow[QT], lrow[QT];
-  f32x16 acc[QT][DT];
+  float mrow = kNoMax, lrow = 0.0f;
+  f32x16 acc[DT];
 #pragma unroll
-  for (int j = 0; j < QT; ++j) {
-    mrow[j] = kNoMax;
-    lrow[j] = 0.0f;
-#pragma unroll
-    for (int u = 0; u < DT; ++u) acc[j][u] = f32x16{};
-  }
+  for (int u = 0; u < DT; ++u) acc[u] = f32x16{};
 
-  // Probabilities against the running max as it stands; a lane whose 16 sum above 2^12 (its first tile among them) sends the
-  // wave through the row max and a rescale, a one-sided branch (two-sided ones make the compiler hold the accumulators twice).
-  auto tile = [&](const char* st, int t) __attribute__((always_inline)) {
-    f32x16 s[QT];
+  // A wave has one tile of each: K of the next tile is on its way from the end of this one's scores on, V from the end of its products
+  // on. (Past the last tile it comes again, so that as many loads are in flight in every step.) Probabilities are taken against
+  // the running max as it stands; a lane whose 16 sum above 2^12 (its first tile among them) sends the wave through the row max
+  // and a rescale, a one-sided branch (two-sided ones make the compiler hold the accumulators twice).
+  auto step = [&]() __attribute__((always_inline)) {
+    const int after = t + kWaves < i1 ? t + kWaves : t;
+    wave_landed<PIECES>();  // V is still in flight
+    f32x16 s = f32x16{};
 #pragma unroll
-    for (int j = 0; j < QT; ++j) s[j] = f32x16{};
+    for (int sd = 0; sd < NSD; ++sd) s = Elt<T>::mfma(lds8<T>(kt + at.nat[sd]), qop[sd], s);
+    reads_done();
+    fetch_k(after);
+    if (t >= masked) hide_after(s, last, t, h2, hidden);
+    V8 x[2];
+    const float ps = tile_probs<T>(s, x, c, -mrow), before = lrow;
+    lrow += ps;
+    if (__builtin_amdgcn_ballot_w64(!(ps <= 4096.0f))) {
+      const float mnew = moved_max(s, c, mrow), alpha = fast_exp2(mrow - mnew);
+      mrow = mnew;
+      lrow = before * alpha + tile_probs<T>(s, x, c, -mnew);
 #pragma unroll
-    for (int sd = 0; sd < NSD; ++sd) {
-      const V8 ka = lds8<T>(st + mine + at.nat[sd]);
-#pragma unroll
-      for (int j = 0; j < QT; ++j) s[j] = Elt<T>::mfma(ka, qop[j][sd], s[j]);
+      for (int u = 0; u < DT; ++u) acc[u] *= alpha;
     }
-    if (t >= masked) {
-#pragma unroll
-      for (int j = 0; j < QT; ++j) hide_after(s[j], last[j], t, h2, hidden);
-    }
-    V8 x[QT][2];
-    float ps[QT], before[QT];
-    bool over = false;
-#pragma unroll
-    for (int j = 0; j < QT; ++j) {
-      ps[j] = tile_probs<T>(s[j], x[j], c, -mrow[j]);
-      before[j] = lrow[j];
-      lrow[j] += ps[j];
-      over |= !(ps[j] <= 4096.0f);
-    }
-    if (__builtin_amdgcn_ballot_w64(over)) {
-#pragma unroll
-      for (int j = 0; j < QT; ++j) {
-        const float mnew = moved_max(s[j], c, mrow[j]), alpha = fast_exp2(mrow[j] - mnew);
-        mrow[j] = mnew;
-        lrow[j] = before[j] * alpha + tile_probs<T>(s[j], x[j], c, -mnew);
-#pragma unroll
-        for (int u = 0; u < DT; ++u) acc[j][u] *= alpha;
-      }
-    }
+    wave_landed<PIECES>();  // the next K is still in flight
 #pragma unroll
     for (int sg = 0; sg < 2; ++sg)
 #pragma unroll
-      for (int u = 0; u < DT; ++u) {
-        const V8 va = at.template tr<T>(st + mine + Tile::BYTES, sg, u, lane);
-#pragma unroll
-        for (int j = 0; j < QT; ++j) acc[j][u] = Elt<T>::mfma(va, x[j][sg], acc[j][u]);
-      }
-  };
-  // The next tile's loads start once this wave's reads of that stage are done, and stay in flight over this tile.
-  auto step = [&](char* cur, char* nxt) __attribute__((always_inline)) {
-    if (t + kWaves < i1) {
-      __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0)
-      __atomic_signal_fence(__ATOMIC_SEQ_CST);
-      issue(nxt, t + kWaves);
-      wave_landed<2 * PIECES>();
-    } else {
-      wave_landed<0>();
-    }
-    tile(cur, t);
+      for (int u = 0; u < DT; ++u) acc[u] = Elt<T>::mfma(at.template tr<T>(vt, sg, u, lane), x[sg], acc[u]);
+    reads_done();
+    fetch_v(after);
     t += kWaves;
   };
-  while (t < i1) {
-    step(s0, s1);
-    if (t >= i1) break;
-    step(s1, s0);
-  }
+  while (t < i1) step();  // (as a plain loop body it takes 30 more registers)
+  wave_landed<0>();
 
-  // The waves' results, tile by tile of rows through LDS: every wave is done with its stages, and nothing is in flight.
-  float lsum[QT];
-#pragma unroll
-  for (int j = 0; j < QT; ++j) {
-    lsum[j] = sum_halves(lrow[j]);
+  // The waves' results through LDS.
+  {
+    const float lsum = sum_halves(lrow);
     if (h2 == 0) {
-      red[0][wu][32 * j + l32] = mrow[j];
-      red[1][wu][32 * j + l32] = lsum[j];
+      red[0][wu][l32] = mrow;
+      red[1][wu][l32] = lsum;
     }
   }
+  constexpr int PART = DT * 16 * 64;  // floats of one wave's rows: two tiles of K or V
+  static_assert(PART * 4 == 2 * Tile::BYTES && kWaves == 4, "the buffers hold the rows of every wave");
+  const bool parted = p.splits > 1 || p.joined;
+  auto part = [&](int k) { return (TATTN_LDS float*)(k < 2 ? kbuf : vbuf) + (k & 1) * PART + lane; };
+  __syncthreads();  // every wave is done with its tiles, nothing is in flight
+  float mall = kNoMax, lall = 0.0f;
+#pragma unroll
+  for (int k = 0; k < kWaves; ++k) mall = __builtin_fmaxf(mall, red[0][k][l32]);
+#pragma unroll
+  for (int k = 0; k < kWaves; ++k) lall += fast_exp2(red[0][k][l32] - mall) * red[1][k][l32];
+  float wgt = fast_exp2(mrow - mall);
+  if (!parted) wgt = lall == 0.0f ? 0.0f : wgt / lall;  // no keys: zeros
+  TATTN_LDS float* dst = part(wu);
+#pragma unroll
+  for (int u = 0; u < DT; ++u)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) dst[(16 * u + i) * 64] = acc[u][i] * wgt;
   __syncthreads();
-  constexpr int PART = DT * 16 * 64;  // floats of one wave's tile
-  static_assert(kWaves * PART * 4 <= RowsLds<D>::STAGE, "a stage holds a row tile of every wave");
-  const bool parted = p.splits > 1;
-  float mall[QT], lall[QT];
-#pragma unroll
-  for (int j = 0; j < QT; ++j) {
-    mall[j] = kNoMax;
-    lall[j] = 0.0f;
-#pragma unroll
-    for (int k = 0; k < kWaves; ++k) mall[j] = __builtin_fmaxf(mall[j], red[0][k][32 * j + l32]);
-#pragma unroll
-    for (int k = 0; k < kWaves; ++k) lall[j] += fast_exp2(red[0][k][32 * j + l32] - mall[j]) * red[1][k][32 * j + l32];
-    float wgt = fast_exp2(mrow[j] - mall[j]);
-    if (!parted) wgt = lall[j] == 0.0f ? 0.0f : wgt / lall[j];
-    TATTN_LDS float* dst = (TATTN_LDS float*)(j ? s1 : s0) + wu * PART + lane;
-#pragma unroll
-    for (int u = 0; u < DT; ++u)
-#pragma unroll
-      for (int r = 0; r < 16; ++r) dst[(16 * u + r) * 64] = acc[j][u][r] * wgt;
-  }
-  __syncthreads();
-#pragma unroll
-  for (int j = 0; j < QT; ++j) {
-    const int row = 32 * (QT * blk + j) + l32;
-    if (row >= rows) continue;
+  if (row < rows) {
     const CrossRow r(p, sl, row);
     T* orow = (T*)p.out + r.at(p.sout);
     const int64_t prow = ((int64_t)slice * p.splits + split) * rows + row;
-    const TATTN_LDS float* src = (const TATTN_LDS float*)(j ? s1 : s0) + lane;
     for (int g = wu; g < DT * 4; g += kWaves) {  // four consecutive columns per register group
       const int d0 = 8 * g + 4 * h2;
       if (d0 >= D) continue;
@@ -200,7 +155,7 @@ __device__ __forceinline__ void rows_block(const CrossParams& p, int slice, int 
 #pragma unroll
       for (int k = 0; k < kWaves; ++k)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) x[e] += src[k * PART + (4 * g + e) * 64];
+        for (int e = 0; e < 4; ++e) x[e] += part(k)[(4 * g + e) * 64];
       if (parted) {
         *reinterpret_cast<f32x4*>(p.part + prow * D + d0) = x;
       } else {
@@ -213,41 +168,45 @@ __device__ __forceinline__ void rows_block(const CrossParams& p, int slice, int 
     if (wu == 0 && h2 == 0) {
       if (parted) {
         float* ml = p.part + (int64_t)p.Zs * p.Hk * p.splits * rows * D + prow * 2;
-        ml[0] = mall[j];
-        ml[1] = lall[j];
+        ml[0] = mall;
+        ml[1] = lall;
       } else if (p.m) {
-        p.m[r.index(p)] = mall[j] + __log2f(lall[j]);
+        p.m[r.index(p)] = mall + __log2f(lall);
       }
     }
   }
 }
 
-template <typename T, int D, int QT, int OCC>
+template <typename T, int D, int OCC>
 __global__ __launch_bounds__(kWaves * 64, OCC) void cross_rows_kernel(const CrossParams p) {
-  __shared__ __attribute__((aligned(1024))) char s0[RowsLds<D>::STAGE];
-  __shared__ __attribute__((aligned(1024))) char s1[RowsLds<D>::STAGE];
-  __shared__ float red[2][kWaves][64];
+  __shared__ __attribute__((aligned(1024))) char kbuf[kWaves * CrossTile<D>::BYTES];
+  __shared__ __attribute__((aligned(1024))) char vbuf[kWaves * CrossTile<D>::BYTES];
+  __shared__ float red[2][kWaves][32];
   int slice, blk;
   if (!cross_coord(p, p.nblk * p.splits, slice, blk)) return;
-  rows_block<T, D, QT, false>(p, slice, blk / p.splits, blk % p.splits, s0, s1, red);
+  rows_block<T, D, false>(p, slice, blk / p.splits, blk % p.splits, kbuf, vbuf, red);
 }
 
+// Workgroups over the prefix, the row blocks that read one part of it on one XCD, whose L2 hands it to the others.
+__host__ __device__ inline int64_t prefix_blocks(const CrossParams& p) { return ((int64_t)p.Zs * p.Hk * p.splits + 7) / 8 * 8 * p.nblk; }
+
 // The prefix's parts first, which are the longer ones, then each sequence's own keys.
-template <typename T, int D, int QT, int OCC>
+template <typename T, int D, int OCC>
 __global__ __launch_bounds__(kWaves * 64, OCC) void prefix_rows_kernel(const PrefixParams p) {
-  __shared__ __attribute__((aligned(1024))) char s0[RowsLds<D>::STAGE];
-  __shared__ __attribute__((aligned(1024))) char s1[RowsLds<D>::STAGE];
-  __shared__ float red[2][kWaves][64];
-  const int shared = p.pre.nblk * p.pre.splits, total = p.pre.Zs * p.pre.Hk * shared;
+  __shared__ __attribute__((aligned(1024))) char kbuf[kWaves * CrossTile<D>::BYTES];
+  __shared__ __attribute__((aligned(1024))) char vbuf[kWaves * CrossTile<D>::BYTES];
+  __shared__ float red[2][kWaves][32];
+  const int total = (int)prefix_blocks(p.pre);
   int i = blockIdx.x;
   if (i < total) {
-    const int blk = i % shared;
-    rows_block<T, D, QT, false>(p.pre, i / shared, blk / p.pre.splits, blk % p.pre.splits, s0, s1, red);
+    const int l = i >> 3, unit = 8 * (l / p.pre.nblk) + (i & 7), slice = unit / p.pre.splits;
+    if (slice < p.pre.Zs * p.pre.Hk)
+      rows_block<T, D, false>(p.pre, slice, l % p.pre.nblk, unit % p.pre.splits, kbuf, vbuf, red);
     return;
   }
   i -= total;
   const int per = p.own.nblk * p.own.splits, blk = i % per;
-  rows_block<T, D, 1, true>(p.own, i / per, blk / p.own.splits, blk % p.own.splits, s0, s1, red);
+  rows_block<T, D, true>(p.own, i / per, blk / p.own.splits, blk % p.own.splits, kbuf, vbuf, red);
 }
 
 // ---- rows whose keys were cut into parts ---------------------------------------------------------
@@ -345,8 +304,8 @@ CombineParams combine_params(const CrossParams& p) {
 template <typename T, int D>
 int combine_cross(const CrossParams& p, hipStream_t st) { return combine<T, D>(combine_params(p), st, "tattn_cross_fwd"); }
 
-// Workgroups of rows_block that a CU holds (128 KB of stages at head dim 128).
-constexpr int rows_occ(int D) { return D == 128 ? 1 : 2; }
+// Workgroups of rows_block that a CU holds: 64 KB of tiles at head dim 128, 128 registers below.
+constexpr int rows_occ(int D) { return D == 128 ? 2 : 4; }
 
 template <typename T, int D>
 int fwd_d(const CrossParams& p, hipStream_t st) {
@@ -358,18 +317,18 @@ int fwd_d(const CrossParams& p, hipStream_t st) {
     return combine_cross<T, D>(p, st);
   }
   if ((rc = cross_grid(p.slices(), (int64_t)p.nblk * p.splits, &blocks))) return rc;
-  cross_rows_kernel<T, D, 1, rows_occ(D)><<<dim3(blocks), dim3(kWaves * 64), 0, st>>>(p);
+  cross_rows_kernel<T, D, rows_occ(D)><<<dim3(blocks), dim3(kWaves * 64), 0, st>>>(p);
   if ((rc = check_launch("tattn_cross_fwd")) || p.splits == 1) return rc;
   return combine_cross<T, D>(p, st);
 }
 
 template <typename T, int D>
 int prefix_d(const PrefixParams& p, hipStream_t st) {
-  const int64_t blocks = p.pre.slices() * p.pre.nblk * p.pre.splits + p.own.slices() * p.own.nblk * p.own.splits;
+  int rc;
+  const int64_t blocks = prefix_blocks(p.pre) + p.own.slices() * p.own.nblk * p.own.splits;
   if (blocks > 0x7ffffff) return set_error(TATTN_E_ARG, "grid too large: %lld workgroups", (long long)blocks);
-  prefix_rows_kernel<T, D, 2, rows_occ(D)><<<dim3((unsigned)blocks), dim3(kWaves * 64), 0, st>>>(p);
-  int rc = check_launch("tattn_prefix_attention");
-  if (rc) return rc;
+  prefix_rows_kernel<T, D, rows_occ(D)><<<dim3((unsigned)blocks), dim3(kWaves * 64), 0, st>>>(p);
+  if ((rc = check_launch("tattn_prefix_attention"))) return rc;
   CombineParams c = combine_params(p.pre);
   c.part[1] = p.own.part;
   c.splits[1] = p.own.splits;
@@ -397,16 +356,21 @@ void cross_fwd_plan(CrossParams& p, int D, int dtype) {
   p.splits = (int)std::max<int64_t>(1, std::min<int64_t>(want / blocks, tiles / (dtype == 1 ? 3 : 8)));
 }
 
-// The parts of all rows together, prefixes and own keys, are about as many as the chip holds at once; none has less than eight
-// tiles. Both kinds are always joined, so each has a part at least.
+// Parts of the prefix as long as an even share of all tiles over the places that the chip has, those of a sequence's own keys half
+// of that, as later workgroups fill the places that fall free; none has less than eight tiles. us at shares of (prefix, own) (1/2, 1/2),
+// (1, 1/2), (1, 1), (3/2, 1/2):
+//   64 requests x 32/8 x 128, prefix 8,192, up to 1,024 own keys   49, 44, 44, 68
+//   8 x 16 samples x 16/4 x 128, prefix 4,096, up to 2,048          81, 77, 83, 77
+//   128 x 16 x 5 queries x 128, prefix 8,192, up to 64               90, 85, 85, 86
 void prefix_plan(PrefixParams& p, int D) {
   const int64_t pt = std::max<int64_t>(1, ((int64_t)p.pre.S + 31) / 32), ot = std::max<int64_t>(1, ((int64_t)p.own.S + 31) / 32);
-  p.pre.nblk = (int)((p.pre.rows() + 63) / 64);
+  p.pre.nblk = (int)((p.pre.rows() + 31) / 32);
   p.own.nblk = (int)((p.own.rows() + 31) / 32);
-  const int64_t pb = p.pre.slices() * p.pre.nblk, ob = p.own.slices() * p.own.nblk;
-  const int64_t chunk = std::max<int64_t>(8, (pb * pt + ob * ot) / (256 * rows_occ(D)));
-  p.pre.splits = (int)std::max<int64_t>(2, (pt + chunk - 1) / chunk);
-  p.own.splits = (int)std::max<int64_t>(2, (ot + chunk - 1) / chunk);
+  const int64_t share = (p.pre.slices() * p.pre.nblk * pt + p.own.slices() * p.own.nblk * ot) / (256 * rows_occ(D));
+  const int64_t shared = std::max<int64_t>(8, share), own = std::max<int64_t>(8, share / 2);
+  p.pre.splits = (int)((pt + shared - 1) / shared);
+  p.own.splits = (int)((ot + own - 1) / own);
+  p.pre.joined = p.own.joined = 1;
 }
 int64_t prefix_floats(const PrefixParams& p, int D) {
   return cross_part_floats(p.pre.slices(), p.pre.rows(), p.pre.splits, D) + cross_part_floats(p.own.slices(), p.own.rows(), p.own.splits, D);

@@ -164,6 +164,7 @@ struct CrossParams {
   int64_t sq[3], sk[3], sv[3], so[3], sd[3], sout[3], sdk[3], sdv[3];
   int32_t Zs, B, H, Hk, G, N, S;
   int32_t nblk, splits;   // row blocks of a slice, parts of their keys
+  int32_t joined;         // forward: results are parts even where there is one
   int32_t pipe;           // forward: row blocks of cross_pipe_rows rows, walked by all waves together
   int32_t kblk, parts;    // backward: key blocks of a slice, parts of their rows
   float c, scale;
