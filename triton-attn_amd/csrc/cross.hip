@@ -2,8 +2,8 @@
 //
 //   O = softmax(c' Q K^T) V over the first len keys, one pass over the keys with the running max and sum of the softmax
 //
-// Few rows (`rows_block`): four waves share 32 rows, and each takes every fourth key tile by itself, staged by LDS DMA
-// into LDS of its own: no barrier until the four partial results are added. The keys are cut into parts where rows are few, and
+// Few rows (`rows_block`): the waves of a workgroup share 32 rows, and each takes its own key tiles by itself, staged by LDS DMA
+// into LDS of its own: no barrier until their partial results are added. The keys are cut into parts where rows are few, and
 // `combine_kernel` joins the parts in order.
 //
 // Roundings: P is rounded to the element type, as the matrix instruction takes it, and its sum is taken from the rounded values.
@@ -16,12 +16,10 @@
 namespace tattn {
 namespace {
 
-constexpr int kWaves = 4;  // of a workgroup of rows_block
-
 // The part `split` of the keys for 32 rows of a slice. CAUSAL: query n is at position len - N + n and sees no key after it.
-template <typename T, int D, bool CAUSAL>
+template <typename T, int D, int W, bool CAUSAL>
 __device__ __forceinline__ void rows_block(const CrossParams& p, int slice, int blk, int split, char* kbuf, char* vbuf,
-                                           float (*red)[kWaves][32]) {
+                                           float (*red)[W][32]) {
   using V4 = typename H16<T>::V4;
   using V8 = typename H16<T>::V8;
   using Tile = CrossTile<D>;
@@ -88,7 +86,7 @@ __device__ __forceinline__ void rows_block(const CrossParams& p, int slice, int 
   // the running max as it stands; a lane whose 16 sum above 2^12 (its first tile among them) sends the wave through the row max
   // and a rescale, a one-sided branch (two-sided ones make the compiler hold the accumulators twice).
   auto step = [&]() __attribute__((always_inline)) {
-    const int after = t + kWaves < i1 ? t + kWaves : t;
+    const int after = t + W < i1 ? t + W : t;
     wave_landed<PIECES>();  // V is still in flight
     f32x16 s = f32x16{};
 #pragma unroll
@@ -113,7 +111,7 @@ __device__ __forceinline__ void rows_block(const CrossParams& p, int slice, int 
       for (int u = 0; u < DT; ++u) acc[u] = Elt<T>::mfma(at.template tr<T>(vt, sg, u, lane), x[sg], acc[u]);
     reads_done();
     fetch_v(after);
-    t += kWaves;
+    t += W;
   };
   while (t < i1) step();  // (as a plain loop body it takes 30 more registers)
   wave_landed<0>();
@@ -127,15 +125,15 @@ __device__ __forceinline__ void rows_block(const CrossParams& p, int slice, int 
     }
   }
   constexpr int PART = DT * 16 * 64;  // floats of one wave's rows: two tiles of K or V
-  static_assert(PART * 4 == 2 * Tile::BYTES && kWaves == 4, "the buffers hold the rows of every wave");
+  static_assert(PART * 4 == 2 * Tile::BYTES && W % 2 == 0, "the buffers hold the rows of every wave");
   const bool parted = p.splits > 1 || p.joined;
-  auto part = [&](int k) { return (TATTN_LDS float*)(k < 2 ? kbuf : vbuf) + (k & 1) * PART + lane; };
+  auto part = [&](int k) { return (TATTN_LDS float*)(k < W / 2 ? kbuf : vbuf) + k % (W / 2) * PART + lane; };
   __syncthreads();  // every wave is done with its tiles, nothing is in flight
   float mall = kNoMax, lall = 0.0f;
 #pragma unroll
-  for (int k = 0; k < kWaves; ++k) mall = __builtin_fmaxf(mall, red[0][k][l32]);
+  for (int k = 0; k < W; ++k) mall = __builtin_fmaxf(mall, red[0][k][l32]);
 #pragma unroll
-  for (int k = 0; k < kWaves; ++k) lall += fast_exp2(red[0][k][l32] - mall) * red[1][k][l32];
+  for (int k = 0; k < W; ++k) lall += fast_exp2(red[0][k][l32] - mall) * red[1][k][l32];
   float wgt = fast_exp2(mrow - mall);
   if (!parted) wgt = lall == 0.0f ? 0.0f : wgt / lall;  // no keys: zeros
   TATTN_LDS float* dst = part(wu);
@@ -148,12 +146,12 @@ __device__ __forceinline__ void rows_block(const CrossParams& p, int slice, int 
     const CrossRow r(p, sl, row);
     T* orow = (T*)p.out + r.at(p.sout);
     const int64_t prow = ((int64_t)slice * p.splits + split) * rows + row;
-    for (int g = wu; g < DT * 4; g += kWaves) {  // four consecutive columns per register group
+    for (int g = wu; g < DT * 4; g += W) {  // four consecutive columns per register group
       const int d0 = 8 * g + 4 * h2;
       if (d0 >= D) continue;
       f32x4 x = f32x4{};
 #pragma unroll
-      for (int k = 0; k < kWaves; ++k)
+      for (int k = 0; k < W; ++k)
 #pragma unroll
         for (int e = 0; e < 4; ++e) x[e] += part(k)[(4 * g + e) * 64];
       if (parted) {
@@ -177,14 +175,14 @@ __device__ __forceinline__ void rows_block(const CrossParams& p, int slice, int 
   }
 }
 
-template <typename T, int D, int OCC>
-__global__ __launch_bounds__(kWaves * 64, OCC) void cross_rows_kernel(const CrossParams p) {
-  __shared__ __attribute__((aligned(1024))) char kbuf[kWaves * CrossTile<D>::BYTES];
-  __shared__ __attribute__((aligned(1024))) char vbuf[kWaves * CrossTile<D>::BYTES];
-  __shared__ float red[2][kWaves][32];
+template <typename T, int D, int W, int OCC>
+__global__ __launch_bounds__(W * 64, OCC) void cross_rows_kernel(const CrossParams p) {
+  __shared__ __attribute__((aligned(1024))) char kbuf[W * CrossTile<D>::BYTES];
+  __shared__ __attribute__((aligned(1024))) char vbuf[W * CrossTile<D>::BYTES];
+  __shared__ float red[2][W][32];
   int slice, blk;
   if (!cross_coord(p, p.nblk * p.splits, slice, blk)) return;
-  rows_block<T, D, false>(p, slice, blk / p.splits, blk % p.splits, kbuf, vbuf, red);
+  rows_block<T, D, W, false>(p, slice, blk / p.splits, blk % p.splits, kbuf, vbuf, red);
 }
 
 // Workgroups over the prefix, the row blocks that read one part of it on one XCD, whose L2 hands it to the others.
@@ -192,21 +190,21 @@ __host__ __device__ inline int64_t prefix_blocks(const CrossParams& p) { return 
 
 // The prefix's parts first, which are the longer ones, then each sequence's own keys.
 template <typename T, int D, int OCC>
-__global__ __launch_bounds__(kWaves * 64, OCC) void prefix_rows_kernel(const PrefixParams p) {
-  __shared__ __attribute__((aligned(1024))) char kbuf[kWaves * CrossTile<D>::BYTES];
-  __shared__ __attribute__((aligned(1024))) char vbuf[kWaves * CrossTile<D>::BYTES];
-  __shared__ float red[2][kWaves][32];
+__global__ __launch_bounds__(4 * 64, OCC) void prefix_rows_kernel(const PrefixParams p) {
+  __shared__ __attribute__((aligned(1024))) char kbuf[4 * CrossTile<D>::BYTES];
+  __shared__ __attribute__((aligned(1024))) char vbuf[4 * CrossTile<D>::BYTES];
+  __shared__ float red[2][4][32];
   const int total = (int)prefix_blocks(p.pre);
   int i = blockIdx.x;
   if (i < total) {
     const int l = i >> 3, unit = 8 * (l / p.pre.nblk) + (i & 7), slice = unit / p.pre.splits;
     if (slice < p.pre.Zs * p.pre.Hk)
-      rows_block<T, D, false>(p.pre, slice, l % p.pre.nblk, unit % p.pre.splits, kbuf, vbuf, red);
+      rows_block<T, D, 4, false>(p.pre, slice, l % p.pre.nblk, unit % p.pre.splits, kbuf, vbuf, red);
     return;
   }
   i -= total;
   const int per = p.own.nblk * p.own.splits, blk = i % per;
-  rows_block<T, D, true>(p.own, i / per, blk / p.own.splits, blk % p.own.splits, kbuf, vbuf, red);
+  rows_block<T, D, 4, true>(p.own, i / per, blk / p.own.splits, blk % p.own.splits, kbuf, vbuf, red);
 }
 
 // ---- rows whose keys were cut into parts ---------------------------------------------------------
@@ -317,7 +315,8 @@ int fwd_d(const CrossParams& p, hipStream_t st) {
     return combine_cross<T, D>(p, st);
   }
   if ((rc = cross_grid(p.slices(), (int64_t)p.nblk * p.splits, &blocks))) return rc;
-  cross_rows_kernel<T, D, rows_occ(D)><<<dim3(blocks), dim3(kWaves * 64), 0, st>>>(p);
+  if (p.waves == 8) cross_rows_kernel<T, D, 8, rows_occ(D)><<<dim3(blocks), dim3(512), 0, st>>>(p);
+  else cross_rows_kernel<T, D, 4, rows_occ(D)><<<dim3(blocks), dim3(256), 0, st>>>(p);
   if ((rc = check_launch("tattn_cross_fwd")) || p.splits == 1) return rc;
   return combine_cross<T, D>(p, st);
 }
@@ -327,7 +326,7 @@ int prefix_d(const PrefixParams& p, hipStream_t st) {
   int rc;
   const int64_t blocks = prefix_blocks(p.pre) + p.own.slices() * p.own.nblk * p.own.splits;
   if (blocks > 0x7ffffff) return set_error(TATTN_E_ARG, "grid too large: %lld workgroups", (long long)blocks);
-  prefix_rows_kernel<T, D, rows_occ(D)><<<dim3((unsigned)blocks), dim3(kWaves * 64), 0, st>>>(p);
+  prefix_rows_kernel<T, D, rows_occ(D)><<<dim3((unsigned)blocks), dim3(4 * 64), 0, st>>>(p);
   if ((rc = check_launch("tattn_prefix_attention"))) return rc;
   CombineParams c = combine_params(p.pre);
   c.part[1] = p.own.part;
@@ -354,6 +353,11 @@ void cross_fwd_plan(CrossParams& p, int D, int dtype) {
   p.nblk = (int)((p.rows() + block - 1) / block);
   const int64_t blocks = p.slices() * p.nblk, want = 256 * (p.pipe ? 2 : rows_occ(D));
   p.splits = (int)std::max<int64_t>(1, std::min<int64_t>(want / blocks, tiles / (dtype == 1 ? 3 : 8)));
+  p.waves = 4;
+  if (!p.pipe && dtype != 1 && p.splits > 1) {  // eight waves share the rows before the keys are cut: fewer parts to join, or none
+    p.waves = 8;
+    p.splits = (int)std::max<int64_t>(1, std::min<int64_t>(want / 2 / blocks, tiles / 16));
+  }
 }
 
 // Parts of the prefix as long as an even share of all tiles over the places that the chip has, those of a sequence's own keys half

@@ -165,6 +165,7 @@ struct CrossParams {
   int32_t Zs, B, H, Hk, G, N, S;
   int32_t nblk, splits;   // row blocks of a slice, parts of their keys
   int32_t joined;         // forward: results are parts even where there is one
+  int32_t waves;          // forward: of a workgroup where rows are few
   int32_t pipe;           // forward: row blocks of cross_pipe_rows rows, walked by all waves together
   int32_t kblk, parts;    // backward: key blocks of a slice, parts of their rows
   float c, scale;
