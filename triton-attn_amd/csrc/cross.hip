@@ -1,179 +1,19 @@
-// Attention over keys of another length, 16-bit forward, and one step behind a shared prefix, on gfx950.
+// Attention over keys of another length, 16-bit forward, on gfx950: few rows, the choice between the kernels, and the sum of parts.
 //
 //   O = softmax(c' Q K^T) V over the first len keys, one pass over the keys with the running max and sum of the softmax
 //
-// Few rows (`rows_block`): the waves of a workgroup share 32 rows, and each takes its own key tiles by itself, staged by LDS DMA
-// into LDS of its own: no barrier until their partial results are added. The keys are cut into parts where rows are few, and
-// `combine_kernel` joins the parts in order.
+// Few rows: cross_rows.h. Many: cross_pipe.h. Few keys: cross_short.hip. The keys are cut into parts where workgroups are few, and
+// combine_kernel joins the parts in order.
 //
 // Roundings: P is rounded to the element type, as the matrix instruction takes it, and its sum is taken from the rounded values.
 // Scores, maxima, sums and accumulators are float32.
 #include <algorithm>
 #include <type_traits>
 
-#include "cross.h"
+#include "cross_rows.h"
 
 namespace tattn {
 namespace {
-
-// The part `split` of the keys for 32 rows of a slice. CAUSAL: query n is at position len - N + n and sees no key after it.
-template <typename T, int D, int W, bool CAUSAL>
-__device__ __forceinline__ void rows_block(const CrossParams& p, int slice, int blk, int split, char* kbuf, char* vbuf,
-                                           float (*red)[W][32]) {
-  using V4 = typename H16<T>::V4;
-  using V8 = typename H16<T>::V8;
-  using Tile = CrossTile<D>;
-  constexpr int NSD = D / 16, DT = (D + 31) / 32, PIECES = Tile::PIECES;
-  const int tid = threadIdx.x;
-  const int lane = tid & 63, h2 = lane >> 5, l32 = lane & 31;
-  const int wu = (int)uniform32((uint32_t)(tid >> 6));
-  const CrossSlice sl(p, slice);
-  const int tiles = (sl.len + 31) >> 5;
-  const int i0 = (int)((int64_t)tiles * split / p.splits), i1 = (int)((int64_t)tiles * (split + 1) / p.splits);
-  const int rows = p.B * p.G * p.N;
-  const float c = p.c, hidden = hidden_score(c);
-
-  const __amdgpu_buffer_rsrc_t krs = rows_rsrc<T, D>(p.k, sl.zs * p.sk[0] + sl.hk * p.sk[1], sl.len, p.sk[2]);
-  const __amdgpu_buffer_rsrc_t vrs = rows_rsrc<T, D>(p.v, sl.zs * p.sv[0] + sl.hk * p.sv[1], sl.len, p.sv[2]);
-  const uint32_t kb = uniform32((uint32_t)(p.sk[2] * 64)), vb = uniform32((uint32_t)(p.sv[2] * 64));
-  uint32_t gk[PIECES], gv[PIECES];
-#pragma unroll
-  for (int i = 0; i < PIECES; ++i) {
-    gk[i] = Tile::source(i, lane, p.sk[2]);
-    gv[i] = Tile::source(i, lane, p.sv[2]);
-  }
-  char *kt = kbuf + wu * Tile::BYTES, *vt = vbuf + wu * Tile::BYTES;
-  auto fetch_k = [&](int t) __attribute__((always_inline)) {
-#pragma unroll
-    for (int i = 0; i < PIECES; ++i) dma16(krs, kt + 1024 * i, gk[i] + (uint32_t)t * kb);
-  };
-  auto fetch_v = [&](int t) __attribute__((always_inline)) {
-#pragma unroll
-    for (int i = 0; i < PIECES; ++i) dma16(vrs, vt + 1024 * i, gv[i] + (uint32_t)t * vb);
-  };
-  int t = i0 + wu;
-  if (t < i1) {
-    fetch_k(t);
-    fetch_v(t);
-  }
-
-  const int row = 32 * blk + l32;
-  V8 qop[NSD];
-  int last = sl.len - 1;  // key that the lane's row sees
-  {
-    const bool live = row < rows;
-    const CrossRow r(p, sl, live ? row : 0);
-    if (CAUSAL) last = sl.len - p.N + r.n;
-    const T* src = (const T*)p.q + r.at(p.sq) + 8 * h2;
-#pragma unroll
-    for (int s = 0; s < NSD; ++s) {
-      const V8 x = *reinterpret_cast<const V8*>(src + 16 * s);
-      qop[s] = live ? x : V8{};
-    }
-  }
-  // Tiles from here on hold keys that some row does not see.
-  const int masked = (CAUSAL ? max(0, sl.len - p.N + 1) : sl.len) >> 5;
-  CrossOp<D> at;
-  at.init(lane);
-
-  float mrow = kNoMax, lrow = 0.0f;
-  f32x16 acc[DT];
-#pragma unroll
-  for (int u = 0; u < DT; ++u) acc[u] = f32x16{};
-
-  // A wave has one tile of each: K of the next tile is on its way from the end of this one's scores on, V from the end of its products
-  // on. (Past the last tile it comes again, so that as many loads are in flight in every step.) Probabilities are taken against
-  // the running max as it stands; a lane whose 16 sum above 2^12 (its first tile among them) sends the wave through the row max
-  // and a rescale, a one-sided branch (two-sided ones make the compiler hold the accumulators twice).
-  auto step = [&]() __attribute__((always_inline)) {
-    const int after = t + W < i1 ? t + W : t;
-    wave_landed<PIECES>();  // V is still in flight
-    f32x16 s = f32x16{};
-#pragma unroll
-    for (int sd = 0; sd < NSD; ++sd) s = Elt<T>::mfma(lds8<T>(kt + at.nat[sd]), qop[sd], s);
-    reads_done();
-    fetch_k(after);
-    if (t >= masked) hide_after(s, last, t, h2, hidden);
-    V8 x[2];
-    const float ps = tile_probs<T>(s, x, c, -mrow), before = lrow;
-    lrow += ps;
-    if (__builtin_amdgcn_ballot_w64(!(ps <= 4096.0f))) {
-      const float mnew = moved_max(s, c, mrow), alpha = fast_exp2(mrow - mnew);
-      mrow = mnew;
-      lrow = before * alpha + tile_probs<T>(s, x, c, -mnew);
-#pragma unroll
-      for (int u = 0; u < DT; ++u) acc[u] *= alpha;
-    }
-    wave_landed<PIECES>();  // the next K is still in flight
-#pragma unroll
-    for (int sg = 0; sg < 2; ++sg)
-#pragma unroll
-      for (int u = 0; u < DT; ++u) acc[u] = Elt<T>::mfma(at.template tr<T>(vt, sg, u, lane), x[sg], acc[u]);
-    reads_done();
-    fetch_v(after);
-    t += W;
-  };
-  while (t < i1) step();  // (as a plain loop body it takes 30 more registers)
-  wave_landed<0>();
-
-  // The waves' results through LDS.
-  {
-    const float lsum = sum_halves(lrow);
-    if (h2 == 0) {
-      red[0][wu][l32] = mrow;
-      red[1][wu][l32] = lsum;
-    }
-  }
-  constexpr int PART = DT * 16 * 64;  // floats of one wave's rows: two tiles of K or V
-  static_assert(PART * 4 == 2 * Tile::BYTES && W % 2 == 0, "the buffers hold the rows of every wave");
-  const bool parted = p.splits > 1 || p.joined;
-  auto part = [&](int k) { return (TATTN_LDS float*)(k < W / 2 ? kbuf : vbuf) + k % (W / 2) * PART + lane; };
-  __syncthreads();  // every wave is done with its tiles, nothing is in flight
-  float mall = kNoMax, lall = 0.0f;
-#pragma unroll
-  for (int k = 0; k < W; ++k) mall = __builtin_fmaxf(mall, red[0][k][l32]);
-#pragma unroll
-  for (int k = 0; k < W; ++k) lall += fast_exp2(red[0][k][l32] - mall) * red[1][k][l32];
-  float wgt = fast_exp2(mrow - mall);
-  if (!parted) wgt = lall == 0.0f ? 0.0f : wgt / lall;  // no keys: zeros
-  TATTN_LDS float* dst = part(wu);
-#pragma unroll
-  for (int u = 0; u < DT; ++u)
-#pragma unroll
-    for (int i = 0; i < 16; ++i) dst[(16 * u + i) * 64] = acc[u][i] * wgt;
-  __syncthreads();
-  if (row < rows) {
-    const CrossRow r(p, sl, row);
-    T* orow = (T*)p.out + r.at(p.sout);
-    const int64_t prow = ((int64_t)slice * p.splits + split) * rows + row;
-    for (int g = wu; g < DT * 4; g += W) {  // four consecutive columns per register group
-      const int d0 = 8 * g + 4 * h2;
-      if (d0 >= D) continue;
-      f32x4 x = f32x4{};
-#pragma unroll
-      for (int k = 0; k < W; ++k)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) x[e] += part(k)[(4 * g + e) * 64];
-      if (parted) {
-        *reinterpret_cast<f32x4*>(p.part + prow * D + d0) = x;
-      } else {
-        V4 y;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) y[e] = (T)x[e];
-        *reinterpret_cast<V4*>(orow + d0) = y;
-      }
-    }
-    if (wu == 0 && h2 == 0) {
-      if (parted) {
-        float* ml = p.part + (int64_t)p.Zs * p.Hk * p.splits * rows * D + prow * 2;
-        ml[0] = mall;
-        ml[1] = lall;
-      } else if (p.m) {
-        p.m[r.index(p)] = mall + __log2f(lall);
-      }
-    }
-  }
-}
 
 template <typename T, int D, int W, int OCC>
 __global__ __launch_bounds__(W * 64, OCC) void cross_rows_kernel(const CrossParams p) {
@@ -182,29 +22,7 @@ __global__ __launch_bounds__(W * 64, OCC) void cross_rows_kernel(const CrossPara
   __shared__ float red[2][W][32];
   int slice, blk;
   if (!cross_coord(p, p.nblk * p.splits, slice, blk)) return;
-  rows_block<T, D, W, false>(p, slice, blk / p.splits, blk % p.splits, kbuf, vbuf, red);
-}
-
-// Workgroups over the prefix, the row blocks that read one part of it on one XCD, whose L2 hands it to the others.
-__host__ __device__ inline int64_t prefix_blocks(const CrossParams& p) { return ((int64_t)p.Zs * p.Hk * p.splits + 7) / 8 * 8 * p.nblk; }
-
-// The prefix's parts first, which are the longer ones, then each sequence's own keys.
-template <typename T, int D, int OCC>
-__global__ __launch_bounds__(4 * 64, OCC) void prefix_rows_kernel(const PrefixParams p) {
-  __shared__ __attribute__((aligned(1024))) char kbuf[4 * CrossTile<D>::BYTES];
-  __shared__ __attribute__((aligned(1024))) char vbuf[4 * CrossTile<D>::BYTES];
-  __shared__ float red[2][4][32];
-  const int total = (int)prefix_blocks(p.pre);
-  int i = blockIdx.x;
-  if (i < total) {
-    const int l = i >> 3, unit = 8 * (l / p.pre.nblk) + (i & 7), slice = unit / p.pre.splits;
-    if (slice < p.pre.Zs * p.pre.Hk)
-      rows_block<T, D, 4, false>(p.pre, slice, l % p.pre.nblk, unit % p.pre.splits, kbuf, vbuf, red);
-    return;
-  }
-  i -= total;
-  const int per = p.own.nblk * p.own.splits, blk = i % per;
-  rows_block<T, D, 4, true>(p.own, i / per, blk / p.own.splits, blk % p.own.splits, kbuf, vbuf, red);
+  rows_block<T, D, W, false, 1>(p, slice, blk / p.splits, blk % p.splits, {{kbuf}, {vbuf}, red});
 }
 
 // ---- rows whose keys were cut into parts ---------------------------------------------------------
@@ -302,8 +120,15 @@ CombineParams combine_params(const CrossParams& p) {
 template <typename T, int D>
 int combine_cross(const CrossParams& p, hipStream_t st) { return combine<T, D>(combine_params(p), st, "tattn_cross_fwd"); }
 
-// Workgroups of rows_block that a CU holds: 64 KB of tiles at head dim 128, 128 registers below.
-constexpr int rows_occ(int D) { return D == 128 ? 2 : 4; }
+template <typename T, int D>
+int combine_prefix(const PrefixParams& p, hipStream_t st) {
+  CombineParams c = combine_params(p.pre);
+  c.part[1] = p.own.part;
+  c.splits[1] = p.own.splits;
+  c.lens = p.own.lens;
+  c.S = p.own.S;
+  return combine<T, D>(c, st, "tattn_prefix_attention");
+}
 
 template <typename T, int D>
 int fwd_d(const CrossParams& p, hipStream_t st) {
@@ -319,21 +144,6 @@ int fwd_d(const CrossParams& p, hipStream_t st) {
   else cross_rows_kernel<T, D, 4, rows_occ(D)><<<dim3(blocks), dim3(256), 0, st>>>(p);
   if ((rc = check_launch("tattn_cross_fwd")) || p.splits == 1) return rc;
   return combine_cross<T, D>(p, st);
-}
-
-template <typename T, int D>
-int prefix_d(const PrefixParams& p, hipStream_t st) {
-  int rc;
-  const int64_t blocks = prefix_blocks(p.pre) + p.own.slices() * p.own.nblk * p.own.splits;
-  if (blocks > 0x7ffffff) return set_error(TATTN_E_ARG, "grid too large: %lld workgroups", (long long)blocks);
-  prefix_rows_kernel<T, D, rows_occ(D)><<<dim3((unsigned)blocks), dim3(4 * 64), 0, st>>>(p);
-  if ((rc = check_launch("tattn_prefix_attention"))) return rc;
-  CombineParams c = combine_params(p.pre);
-  c.part[1] = p.own.part;
-  c.splits[1] = p.own.splits;
-  c.lens = p.own.lens;
-  c.S = p.own.S;
-  return combine<T, D>(c, st, "tattn_prefix_attention");
 }
 
 }  // namespace
@@ -360,26 +170,6 @@ void cross_fwd_plan(CrossParams& p, int D, int dtype) {
   }
 }
 
-// Parts of the prefix as long as an even share of all tiles over the places that the chip has, those of a sequence's own keys half
-// of that, as later workgroups fill the places that fall free; none has less than eight tiles. us at shares of (prefix, own) (1/2, 1/2),
-// (1, 1/2), (1, 1), (3/2, 1/2):
-//   64 requests x 32/8 x 128, prefix 8,192, up to 1,024 own keys   49, 44, 44, 68
-//   8 x 16 samples x 16/4 x 128, prefix 4,096, up to 2,048          81, 77, 83, 77
-//   128 x 16 x 5 queries x 128, prefix 8,192, up to 64               90, 85, 85, 86
-void prefix_plan(PrefixParams& p, int D) {
-  const int64_t pt = std::max<int64_t>(1, ((int64_t)p.pre.S + 31) / 32), ot = std::max<int64_t>(1, ((int64_t)p.own.S + 31) / 32);
-  p.pre.nblk = (int)((p.pre.rows() + 31) / 32);
-  p.own.nblk = (int)((p.own.rows() + 31) / 32);
-  const int64_t share = (p.pre.slices() * p.pre.nblk * pt + p.own.slices() * p.own.nblk * ot) / (256 * rows_occ(D));
-  const int64_t shared = std::max<int64_t>(8, share), own = std::max<int64_t>(8, share / 2);
-  p.pre.splits = (int)((pt + shared - 1) / shared);
-  p.own.splits = (int)((ot + own - 1) / own);
-  p.pre.joined = p.own.joined = 1;
-}
-int64_t prefix_floats(const PrefixParams& p, int D) {
-  return cross_part_floats(p.pre.slices(), p.pre.rows(), p.pre.splits, D) + cross_part_floats(p.own.slices(), p.own.rows(), p.own.splits, D);
-}
-
 #define TATTN_CROSS_SWITCH(FN)                                                   \
   switch (D) {                                                                   \
     case 16: return dtype == 0 ? FN<f16, 16>(p, st) : FN<bf16, 16>(p, st);       \
@@ -390,7 +180,7 @@ int64_t prefix_floats(const PrefixParams& p, int D) {
   return set_error(TATTN_E_ARG, "head dim must be 16, 32, 64 or 128, got %d", D);
 
 int launch_cross_fwd(const CrossParams& p, int D, int dtype, hipStream_t st) { TATTN_CROSS_SWITCH(fwd_d) }
-int launch_prefix(const PrefixParams& p, int D, int dtype, hipStream_t st) { TATTN_CROSS_SWITCH(prefix_d) }
+int launch_prefix_combine(const PrefixParams& p, int D, int dtype, hipStream_t st) { TATTN_CROSS_SWITCH(combine_prefix) }
 int launch_cross_combine(const CrossParams& p, int D, int dtype, hipStream_t st) {
   if (dtype == 1) {
     switch (D) {

@@ -18,6 +18,10 @@ __global__ __launch_bounds__(NW * 64, OCC) void cross_dq_kernel(const CrossParam
   using B = BwdPipe<D>;
   constexpr int NSD = B::NSD, DT = B::DT, STAGE = B::DQ_STAGE;
   constexpr bool LIFT = std::is_same_v<T, f16>;
+  // dS as a sum of two halves at head dim 16. With few columns the error of delta, which comes from the rounded O, adds to that of a
+  // rounded dS: dQ is then 1.55 times as far off as its last rounding leaves it (1.45 at head dim 64), and 1.1 times with two
+  // halves, at 111 us for 77 (4 x 16 x 2,048 over 2,048 x 16).
+  constexpr int NE = D == 16 ? 4 : 2;
   __shared__ __attribute__((aligned(16))) char smem[B::NST * STAGE];
   __shared__ uint32_t norms[3][LIFT ? NW : 1];  // per wave: largest squared norm, |delta|, whether a row is lifted
 
@@ -93,13 +97,17 @@ __global__ __launch_bounds__(NW * 64, OCC) void cross_dq_kernel(const CrossParam
       dp = Elt<T>::mfma(lds8<T>(base + B::TILE + at.nat[sd]), dop[sd], dp);
     }
   };
-  auto grad = [&](const V8 (&ds)[2], int st) __attribute__((always_inline)) {
+  auto grad = [&](const V8 (&ds)[NE], int st) __attribute__((always_inline)) {
 #pragma unroll
     for (int g = 0; g < 2; ++g)
 #pragma unroll
-      for (int u = 0; u < DT; ++u) dq[u] = Elt<T>::mfma(at.template tr<T>(smem + st * STAGE, g, u, lane), ds[g], dq[u]);
+      for (int u = 0; u < DT; ++u) {
+        const V8 ka = at.template tr<T>(smem + st * STAGE, g, u, lane);
+#pragma unroll
+        for (int e = g; e < NE; e += 2) dq[u] = Elt<T>::mfma(ka, ds[e], dq[u]);
+      }
   };
-  auto dsv = [&](const f32x16& s, const f32x16& dp, V8 (&ds)[2], int left, auto mask_tag) __attribute__((always_inline)) {
+  auto dsv = [&](const f32x16& s, const f32x16& dp, V8 (&ds)[NE], int left, auto mask_tag) __attribute__((always_inline)) {
     constexpr bool MASK = decltype(mask_tag)::value;
 #pragma unroll
     for (int a = 0; a < 2; ++a)
@@ -116,6 +124,11 @@ __global__ __launch_bounds__(NW * 64, OCC) void cross_dq_kernel(const CrossParam
         const auto y = H16<T>::pack(x[0], x[1]);
         ds[a][i] = y[0];
         ds[a][i + 1] = y[1];
+        if constexpr (NE == 4) {
+          const auto low = H16<T>::pack(x[0] - (float)y[0], x[1] - (float)y[1]);
+          ds[2 + a][i] = low[0];
+          ds[2 + a][i + 1] = low[1];
+        }
       }
   };
 
@@ -141,9 +154,9 @@ __global__ __launch_bounds__(NW * 64, OCC) void cross_dq_kernel(const CrossParam
 #pragma unroll
     for (int u = 0; u < DT; ++u) dq[u] = f32x16{};
     f32x16 sa, da, sb, db;
-    V8 ea[2] = {}, eb[2];
+    V8 ea[NE] = {}, eb[NE];
     if (nsteps > 0) first(sa, da, 0);
-    auto step = [&](int i, int st, f32x16& s0, f32x16& d0, f32x16& s1, f32x16& d1, const V8 (&e0)[2], V8 (&e1)[2], auto mask_tag)
+    auto step = [&](int i, int st, f32x16& s0, f32x16& d0, f32x16& s1, f32x16& d1, const V8 (&e0)[NE], V8 (&e1)[NE], auto mask_tag)
                     __attribute__((always_inline)) {
       next.load(krs, vrs, (uint32_t)(i0 + i + 2) * kb, (uint32_t)(i0 + i + 2) * vb);
       first(s1, d1, (st + 1) & 3);
@@ -163,8 +176,8 @@ __global__ __launch_bounds__(NW * 64, OCC) void cross_dq_kernel(const CrossParam
       step(i, i & 3, sa, da, sb, db, ea, eb, std::true_type{});
       sa = sb;
       da = db;
-      ea[0] = eb[0];
-      ea[1] = eb[1];
+#pragma unroll
+      for (int e = 0; e < NE; ++e) ea[e] = eb[e];
     }
     if (nsteps > 0) grad(ea, (nsteps - 1) & 3);
     if (!LIFT || !lifted) break;

@@ -209,6 +209,7 @@ struct PrefixParams {
 void prefix_plan(PrefixParams& p, int D);
 int64_t prefix_floats(const PrefixParams& p, int D);
 int launch_prefix(const PrefixParams& p, int D, int dtype, hipStream_t st);
+int launch_prefix_combine(const PrefixParams& p, int D, int dtype, hipStream_t st);
 
 // One token per request over the cache in 4 bits.
 struct Cache4AttnParams {
