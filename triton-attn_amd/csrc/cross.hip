@@ -5,6 +5,9 @@
 // Few rows: cross_rows.h. Many: cross_pipe.h. Few keys: cross_short.hip. The keys are cut into parts where workgroups are few, and
 // combine_kernel joins the parts in order.
 //
+// Few rows are bound by the keys' bytes. One token of each sequence, keys not in a cache, us (as a copy): 32 x 32/8 over 375 to 1,500 x 128
+// 28 (22), 64 x 32/8 over 1,024 x 128 50 (47), 64 x 32/8 over 1,024 to 4,096 x 64 66 (59), 1 x 32 over 131,072 x 128 367 (377).
+//
 // Roundings: P is rounded to the element type, as the matrix instruction takes it, and its sum is taken from the rounded values.
 // Scores, maxima, sums and accumulators are float32.
 #include <algorithm>
@@ -161,10 +164,12 @@ void cross_fwd_plan(CrossParams& p, int D, int dtype) {
   p.pipe = dtype != 1 && p.rows() > 64;
   const int64_t block = dtype == 1 ? 128 : p.pipe ? cross_pipe_rows(D) : 32;
   p.nblk = (int)((p.rows() + block - 1) / block);
-  const int64_t blocks = p.slices() * p.nblk, want = 256 * (p.pipe ? 2 : rows_occ(D));
+  const int64_t blocks = p.slices() * p.nblk, want = 256 * (dtype == 1 ? (D == 128 ? 1 : 2) : p.pipe ? 2 : rows_occ(D));
   p.splits = (int)std::max<int64_t>(1, std::min<int64_t>(want / blocks, tiles / (dtype == 1 ? 3 : 8)));
   p.waves = 4;
-  if (!p.pipe && dtype != 1 && p.splits > 1) {  // eight waves share the rows before the keys are cut: fewer parts to join, or none
+  // Eight waves share the rows before the keys are cut: fewer parts to join, or none (32 x 32/8 over 375 to 1,500 x 128, one token: 22.5 us
+  // for 24.6, keys in the cache).
+  if (!p.pipe && dtype != 1 && p.splits > 1) {
     p.waves = 8;
     p.splits = (int)std::max<int64_t>(1, std::min<int64_t>(want / 2 / blocks, tiles / 16));
   }

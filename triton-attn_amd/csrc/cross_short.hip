@@ -10,7 +10,9 @@
 // Roundings: P and dS as operands, once. In float16 dS is scaled by the power of two that the largest norms of dO and v allow
 // (|dS| <= 2 |dO| |v|); where a later tile has larger rows, what was summed is scaled down with it.
 //
-// Bound by bytes forward, and by the chain of products of the one wave that a SIMD holds backward: TIMES.
+// Bound by bytes forward, and by the chain of products of the one wave that a SIMD holds backward (dK and dV of 96 keys take 192
+// registers). 16 x 8 x 4,096 over 77 x 64 fp16: forward 34 us (134 MB), backward 80 (201 MB, 34 us as a copy) and 5 for the sum; by
+// the kernels for many keys 46 and 121.
 #include <algorithm>
 #include <type_traits>
 

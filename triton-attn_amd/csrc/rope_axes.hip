@@ -2,7 +2,9 @@
 // gradients, on gfx950. The mathematics and the layout of norm_rope.hip; a pair's angle is that of its own axis's position.
 // Without norms the rotation is linear: the gradient turns dy back by the same kernel and reads no x.
 //
-// Bound by bytes: x in and y out. The angles of a token are looked up once for four heads; their tables stay in the caches.
+// Bound by bytes: x in and y out. The angles of a token are looked up once for four heads; their tables stay in the caches. Forward
+// and gradients with their launches, us (floor of a copy): 2 x 24 + 24 heads x 21,601 x 128 bf16 393 (376); 16 x 16 + 16 x 4,097 x 64 fp16
+// with norms 269 (239).
 #include <type_traits>
 
 #include "norm_rope.h"
