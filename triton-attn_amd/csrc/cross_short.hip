@@ -11,76 +11,16 @@
 // (|dS| <= 2 |dO| |v|); where a later tile has larger rows, what was summed is scaled down with it.
 //
 // Bound by bytes forward, and by the chain of products of the one wave that a SIMD holds backward (dK and dV of 96 keys take 192
-// registers). 16 x 8 x 4,096 over 77 x 64 fp16: forward 34 us (134 MB), backward 80 (201 MB, 34 us as a copy) and 5 for the sum; by
-// the kernels for many keys 46 and 121.
+// registers); cross_short_pipe.hip has the form for two row tiles in a step. us, keys not in a cache: 16 x 8 x 4,096 over 77 x 64 fp16
+// forward 44 (134 MB), backward 76 (201 MB, 35 as a copy) and 5 for the sum; over 128 x 64 45 and 114; over 64 x 128 fp16 60 and 170 (some
+// registers spill; bf16, which needs no factor on dS, 120; by the kernels for many keys 300 and 267).
 #include <algorithm>
 #include <type_traits>
 
-#include "cross_bwd.h"
+#include "cross_short.h"
 
 namespace tattn {
 namespace {
-
-constexpr int kShortWaves = 4;
-
-// K and V of the slice into `tiles` (K's, then V's), rows at or past len as zeros; waits for them.
-template <typename T, int D, int NT>
-__device__ __forceinline__ void stage_keys(const CrossParams& p, const CrossSlice& sl, char* tiles, int wu, int lane) {
-  using Tile = CrossTile<D>;
-  const __amdgpu_buffer_rsrc_t krs = rows_rsrc<T, D>(p.k, sl.zs * p.sk[0] + sl.hk * p.sk[1], sl.len, p.sk[2]);
-  const __amdgpu_buffer_rsrc_t vrs = rows_rsrc<T, D>(p.v, sl.zs * p.sv[0] + sl.hk * p.sv[1], sl.len, p.sv[2]);
-  for (int i = wu; i < NT * Tile::PIECES; i += kShortWaves) {
-    const int t = i / Tile::PIECES, piece = i % Tile::PIECES;
-    dma16(krs, tiles + 1024 * i, Tile::source(piece, lane, p.sk[2]) + (uint32_t)(64 * t * p.sk[2]));
-    dma16(vrs, tiles + NT * Tile::BYTES + 1024 * i, Tile::source(piece, lane, p.sv[2]) + (uint32_t)(64 * t * p.sv[2]));
-  }
-  all_landed_barrier();
-}
-
-// Row tiles of the workgroup's part.
-struct ShortRows {
-  int slice, part, rows, t0, t1;
-  bool ok;
-  __device__ __forceinline__ ShortRows(const CrossParams& p, int parts) {
-    ok = cross_coord(p, parts, slice, part);
-    rows = p.B * p.G * p.N;
-    const int tiles = (rows + 31) >> 5;
-    t0 = (int)((int64_t)tiles * part / parts);
-    t1 = (int)((int64_t)tiles * (part + 1) / parts);
-  }
-};
-
-// What the scores of a tile's keys start from: 0, or -inf for those at or past len, whose K is zeros. One float a key.
-template <int NT>
-__device__ __forceinline__ void stage_mask(const CrossSlice& sl, float* mask) {
-  if (threadIdx.x < 32 * NT) mask[threadIdx.x] = (int)threadIdx.x < sl.len ? 0.0f : -__builtin_inff();
-}
-__device__ __forceinline__ f32x16 masked_start(const float* mask, int k, int h2) {
-  f32x16 s;
-  int at = 8 * h2;
-  asm volatile("" : "+v"(at));  // read where it is used: held over the rows it would take 16 registers a tile
-#pragma unroll
-  for (int a = 0; a < 4; ++a) {
-    const f32x4 x = *reinterpret_cast<const TATTN_LDS f32x4*>((const TATTN_LDS float*)mask + 32 * k + 16 * (a >> 1) + at + 4 * (a & 1));
-#pragma unroll
-    for (int e = 0; e < 4; ++e) s[4 * a + e] = x[e];
-  }
-  return s;
-}
-// Where the scale is negative the signs of q and of the scale change: scores rise with their exponents.
-template <typename V8>
-__device__ __forceinline__ V8 signed_rows(u32x4 x, uint32_t sign) {
-#pragma unroll
-  for (int i = 0; i < 4; ++i) x[i] ^= sign;
-  return __builtin_bit_cast(V8, x);
-}
-
-// The lane's row of a tile as operand chunks (row l32, 16 bytes of every 32).
-template <typename T, int D>
-__device__ __forceinline__ void load_rows(const T* base, int64_t off, int h2, u32x4 (&x)[D / 16]) {
-#pragma unroll
-  for (int s = 0; s < D / 16; ++s) x[s] = ld16(base + off + 16 * s + 8 * h2);
-}
 
 template <typename T, int D, int NT>
 __global__ __launch_bounds__(kShortWaves * 64, 2) void short_fwd_kernel(const CrossParams p) {
@@ -184,13 +124,12 @@ __global__ __launch_bounds__(kShortWaves * 64, OCC) void short_bwd_kernel(const 
   using V8 = typename H16<T>::V8;
   using Tile = CrossTile<D>;
   using Pt = Swz<32>;  // rows of a tile of P or dS: 32 keys
-  constexpr int NSD = D / 16, DT = (D + 31) / 32, TB = Tile::BYTES, CPR = D / 8, KEYS = 32 * NT;
+  constexpr int NSD = D / 16, DT = (D + 31) / 32, TB = Tile::BYTES;
   constexpr bool LIFT = std::is_same_v<T, f16>;
   constexpr bool AHEAD = NT * DT < 8;                    // registers for the next tile's rows
   constexpr int WAVE = 2 * TB + 2 * 32 * Pt::RB;         // Q, dO, P and dS of a wave
-  constexpr int PART = DT * 16 * 64 * 4;                 // a wave's sums for 32 keys
   constexpr int SPACE = 2 * NT * TB + kShortWaves * WAVE;
-  static_assert(kShortWaves * PART <= SPACE, "the waves' sums fit");
+  static_assert(kShortWaves * short_part(D) <= SPACE, "the waves' sums fit");
   __shared__ __attribute__((aligned(1024))) char smem[SPACE];
   __shared__ __attribute__((aligned(16))) float mask[32 * NT];
   const int tid = threadIdx.x, lane = tid & 63, h2 = lane >> 5, l32 = lane & 31;
@@ -358,48 +297,7 @@ __global__ __launch_bounds__(kShortWaves * 64, OCC) void short_bwd_kernel(const 
       store_row_t<T, D>((T*)p.out + CrossRow(p, sl, row).at(p.sout), dq, p.scale * (LIFT ? unlift_of(lift) : 1.0f), h2);
   }
 
-  // The waves' sums, tile by tile of keys: C register r of a lane is key 8 (r / 4) + 4 h2 + r % 4, column 32 u + l32. Keys at or past
-  // len have none: their P and dS are 0.
-  const float unlift = LIFT ? unlift_of(lift) : 1.0f;
-  TATTN_LDS float* sums = (TATTN_LDS float*)smem;
-  float* part = p.kpart + ((int64_t)b.slice * p.parts + b.part) * (2 * KEYS * D);
-#pragma unroll
-  for (int k = 0; k < NT; ++k)
-#pragma unroll
-    for (int which = 0; which < 2; ++which) {
-      __syncthreads();
-#pragma unroll
-      for (int u = 0; u < DT; ++u)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          const int in = 8 * (r >> 2) + 4 * h2 + (r & 3), d = 32 * u + l32;
-          if (d < D) sums[wu * (PART / 4) + in * D + d] = which ? dv[k][u][r] : dk[k][u][r] * unlift;
-        }
-      __syncthreads();
-      for (int i = tid; i < 32 * CPR; i += kShortWaves * 64) {
-        const int in = i / CPR, cc = i % CPR, key = 32 * k + in;
-        if (key >= p.S) continue;
-        f32x4 lo = f32x4{}, hi = f32x4{};
-#pragma unroll
-        for (int w = 0; w < kShortWaves; ++w) {
-          lo += *reinterpret_cast<const TATTN_LDS f32x4*>(sums + w * (PART / 4) + in * D + 8 * cc);
-          hi += *reinterpret_cast<const TATTN_LDS f32x4*>(sums + w * (PART / 4) + in * D + 8 * cc + 4);
-        }
-        if (p.parts > 1) {
-          float* dst = part + (which ? KEYS * D : 0) + key * D + 8 * cc;
-          *reinterpret_cast<f32x4*>(dst) = lo;
-          *reinterpret_cast<f32x4*>(dst + 4) = hi;
-        } else {
-          const float mul = which ? 1.0f : p.scale;
-          V8 y;
-#pragma unroll
-          for (int e = 0; e < 8; ++e) y[e] = (T)((e < 4 ? lo[e & 3] : hi[e & 3]) * mul);
-          T* dst = which ? (T*)p.dv + sl.zs * p.sdv[0] + sl.hk * p.sdv[1] + (int64_t)key * p.sdv[2]
-                         : (T*)p.dk + sl.zs * p.sdk[0] + sl.hk * p.sdk[1] + (int64_t)key * p.sdk[2];
-          *reinterpret_cast<V8*>(dst + 8 * cc) = y;
-        }
-      }
-    }
+  short_sums<T, D, NT, DT>(p, sl, b, smem, dk, dv, LIFT ? unlift_of(lift) : 1.0f);
 }
 
 template <typename T, int D, int NT>
@@ -412,8 +310,12 @@ int short_d(const CrossParams& p, bool bwd, hipStream_t st) {
     return check_launch("tattn_cross_fwd");
   }
   if constexpr (NT <= cross_short_tiles(D, true)) {
-    short_bwd_kernel<T, D, NT, cross_short_occ(D, NT)><<<dim3(blocks), dim3(kShortWaves * 64), 0, st>>>(p);
-    if ((rc = check_launch("tattn_cross_bwd")) || p.parts == 1) return rc;
+    if constexpr (cross_short_piped(D, NT)) rc = launch_cross_short_pipe(p, D, std::is_same_v<T, f16> ? 0 : 2, st);
+    else {
+      short_bwd_kernel<T, D, NT, cross_short_occ(D, NT)><<<dim3(blocks), dim3(kShortWaves * 64), 0, st>>>(p);
+      rc = check_launch("tattn_cross_bwd");
+    }
+    if (rc || p.parts == 1) return rc;
     return launch_cross_sum(p, D, std::is_same_v<T, f16> ? 0 : 2, true, 32 * NT, st);
   }
   return set_error(TATTN_E_ARG, "too many keys: %d", p.S);

@@ -194,7 +194,10 @@ int launch_cross_bwd(const CrossParams& p, int D, int dtype, hipStream_t st);
 constexpr int cross_short_tiles(int D, bool bwd) { return D == 128 && bwd ? 2 : 4; }
 constexpr int cross_short_occ(int D, int tiles) { return tiles * ((D + 31) / 32) <= 3 ? 2 : 1; }  // waves per SIMD of the backward
 inline bool cross_short(const CrossParams& p, int D, int dtype, bool bwd) { return dtype != 1 && p.S <= 32 * cross_short_tiles(D, bwd); }
+// Backward with two row tiles in a step: cross_short_pipe.hip.
+constexpr bool cross_short_piped(int D, int tiles) { return D < 128 && tiles * ((D + 31) / 32) >= 4 && tiles * ((D + 31) / 32) < 8; }
 int launch_cross_short(const CrossParams& p, int D, int dtype, bool bwd, hipStream_t st);
+int launch_cross_short_pipe(const CrossParams& p, int D, int dtype, hipStream_t st);
 int launch_cross_dq(const CrossParams& p, int D, int dtype, hipStream_t st);  // 16-bit; dQ (its parts) and delta
 int launch_cross_f32(const CrossParams& p, int D, bool bwd, hipStream_t st);
 int launch_cross_combine(const CrossParams& p, int D, int dtype, hipStream_t st);  // joins the forward's parts

@@ -21,8 +21,8 @@ LIB = PKG / "libtattn_hip.so"
 SOURCES = ["abi.hip", "fwd.hip", "fwd_persist_causal.hip", "bwd.hip", "bwd_dq_persist.hip", "bwd_dkdv_persist.hip",
            "bwd_split.hip", "short.hip", "coop.hip", "f32_split.hip",
            "abi_ops.hip", "paged.hip", "norm_rope.hip", "window.hip",
-           "window_f32.hip", "cache4_attention.hip", "cross.hip", "cross_fwd.hip", "cross_bwd.hip", "cross_dq.hip", "cross_short.hip", "cross_f32.hip", "prefix.hip",
-           "rope_axes.hip"]
+           "window_f32.hip", "cache4_attention.hip", "cross.hip", "cross_fwd.hip", "cross_bwd.hip", "cross_dq.hip",
+           "cross_short.hip", "cross_short_pipe.hip", "cross_f32.hip", "prefix.hip", "rope_axes.hip"]
 # Per-source flags. fwd.hip: keep each step's softmax work in the step that issues the
 # independent MFMAs it interleaves with (machine sinking would move it to its first use).
 # fwd_persist_causal.hip (persistent causal forward, two tiles per wave), bwd_dq_persist.hip
@@ -31,7 +31,7 @@ SOURCES = ["abi.hip", "fwd.hip", "fwd_persist_causal.hip", "bwd.hip", "bwd_dq_pe
 # takes the same (head dim 128: dQ 5% faster, the rest 1-2%); the other kernels are slower under either. Attention over
 # another length: cross_fwd.hip as fwd.hip; dK / dV (cross_bwd.hip) are 2-8% faster under iterative-ilp and 5-9% slower under max-ilp,
 # dQ by pairs of waves (cross_dq.hip) takes 419 us under max-ilp, 457 under the default and 481 under iterative-ilp
-# (2 x 16 x 4,096 over 4,096 x 128).
+# (2 x 16 x 4,096 over 4,096 x 128), and cross_short_pipe.hip has the registers for two tiles only under max-ilp.
 SOURCE_FLAGS = {
     "fwd.hip": ["-mllvm", "-disable-machine-sink"],
     "fwd_persist_causal.hip": ["-mllvm", "-disable-machine-sink", "-mllvm", "-amdgpu-sched-strategy=iterative-ilp"],
@@ -39,6 +39,7 @@ SOURCE_FLAGS = {
     "bwd_split.hip": ["-mllvm", "-amdgpu-sched-strategy=iterative-ilp"],
     "window.hip": ["-mllvm", "-amdgpu-sched-strategy=iterative-ilp"],
     "cross_dq.hip": ["-mllvm", "-amdgpu-sched-strategy=max-ilp"],
+    "cross_short_pipe.hip": ["-mllvm", "-amdgpu-sched-strategy=max-ilp"],
     "cross_bwd.hip": ["-mllvm", "-amdgpu-sched-strategy=iterative-ilp"],
     "cross_fwd.hip": ["-mllvm", "-disable-machine-sink"],
 }
