@@ -154,9 +154,11 @@ int fwd_d(const CrossParams& p, hipStream_t st) {
 // Up to two row tiles: one per workgroup (rows_block). More: blocks of cross_pipe_rows. Keys are cut into parts until the chip
 // holds no more workgroups at once, of at least eight tiles (in float32, where a tile takes eight times as long, three).
 void cross_fwd_plan(CrossParams& p, int D, int dtype) {
-  if (cross_short(p, D, dtype, false)) {  // row tiles of a slice in parts, four a workgroup for a wave at least
-    const int64_t tiles = (p.rows() + 31) / 32;
-    p.nblk = (int)std::max<int64_t>(1, std::min<int64_t>(1024 / p.slices(), tiles / 16));
+  // Few keys: a slice's row tiles in as many parts as the chip holds workgroups, of four tiles for a wave at least. us at 512, 768 and
+  // 1,024: 16 x 8 x 4,096 over 77 x 64 41, 39, 44; over 64 x 128 57, 62, 59; 16 x 16 x 4,096 over 77 x 32 51, 49, 45.
+  if (cross_short(p, D, dtype, false)) {
+    const int64_t tiles = (p.rows() + 31) / 32, places = 256 * (D == 128 ? 2 : D == 64 ? 3 : 4);
+    p.nblk = (int)std::max<int64_t>(1, std::min<int64_t>(places / p.slices(), tiles / 16));
     p.splits = 1;
     return;
   }

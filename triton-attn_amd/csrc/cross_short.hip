@@ -12,7 +12,7 @@
 //
 // Bound by bytes forward, and by the chain of products of the one wave that a SIMD holds backward (dK and dV of 96 keys take 192
 // registers); cross_short_pipe.hip has the form for two row tiles in a step. us, keys not in a cache: 16 x 8 x 4,096 over 77 x 64 fp16
-// forward 44 (134 MB), backward 76 (201 MB, 35 as a copy) and 5 for the sum; over 128 x 64 45 and 114; over 64 x 128 fp16 60 and 170 (some
+// forward 39 (134 MB), backward 76 (201 MB, 35 as a copy) and 5 for the sum; over 128 x 64 45 and 114; over 64 x 128 fp16 60 and 170 (some
 // registers spill; bf16, which needs no factor on dS, 120; by the kernels for many keys 300 and 267).
 #include <algorithm>
 #include <type_traits>
