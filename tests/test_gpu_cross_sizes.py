@@ -96,6 +96,18 @@ def test_what_is_not_finite_stays_in_its_row_and_head(n, s, d, dtype, value):
         assert not torch.isfinite(got[1, 2:]).any()
 
 
+@pytest.mark.parametrize("dtype", [F16, BF16, F32])
+@pytest.mark.parametrize("h,n,s", [(4, 1, 300), (8, 1, 60), (4, 2, 300), (6, 33, 200)])
+def test_heads_that_share_a_query_or_a_gradient(h, n, s, dtype):
+    """Heads of one address: queries that all heads read, and the gradient of a sum over heads. Scores reach 2 * 64 * 3 * 3, so that a
+    row that is not there would not be of no weight."""
+    q, k, v, do = make(3, h, 2, n, s, 64, dtype)
+    lens = i32(s, 0, s - 5)
+    check(q, k, v, do[:, :1].expand(-1, h, -1, -1), lens, 0.125)
+    check(q[:, :1].expand(-1, h, -1, -1), k, v, do, lens, 2.0, 2.0 ** -94)
+    check(q[:, :1].expand(-1, h, -1, -1), k, v, do[:1, :1, :1].expand(3, h, n, 64), lens, 0.125)
+
+
 def test_rows_far_apart():
     """Batches 2^31 elements apart: offsets pass 32 bits."""
     z, h, n, s, d = 2, 2, 70, 200, 64

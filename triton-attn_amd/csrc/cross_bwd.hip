@@ -306,11 +306,12 @@ constexpr int kRowTiles = 4;  // row tiles of a dQ workgroup
 constexpr int kKeyTiles = 4;
 constexpr int bwd_occ(int D) { return D == 128 ? 1 : 2; }
 
-// Rows that lie at one stride, whatever head they belong to, are walked as one head's: no tile holds the end of a head.
-CrossParams walked(const CrossParams& p) {
+// Rows that lie at one stride, whatever head they belong to, are walked as one head's: no tile holds the end of a head. (Not where
+// heads share an address: rows past the last would be read as it.)
+CrossParams walked(const CrossParams& p, int D) {
   CrossParams w = p;
   const int64_t rows = (int64_t)p.G * p.N, sq = p.N == 1 ? p.sq[1] : p.sq[2], sd = p.N == 1 ? p.sd[1] : p.sd[2];
-  const bool one = p.G > 1 && p.sq[1] == p.N * sq && p.sd[1] == p.N * sd && rows < (1 << 30) &&
+  const bool one = p.G > 1 && p.sq[1] == p.N * sq && p.sd[1] == p.N * sd && sq >= D && sd >= D && rows < (1 << 30) &&
                    (rows + 256) * std::max(sq, sd) * 2 < 0x7fffff00ll;
   if (!one) return w;
   w.N = (int32_t)rows;
@@ -331,7 +332,7 @@ int bwd_d(const CrossParams& p, hipStream_t st) {
   if ((rc = launch_cross_dq(p, D, std::is_same_v<T, f16> ? 0 : 2, st))) return rc;
   if (p.splits > 1 && (rc = sum_d<T, D>(p, false, 0, st))) return rc;
   if ((rc = cross_grid(p.slices(), (int64_t)p.kblk * p.parts, &blocks))) return rc;
-  cross_dkdv_kernel<T, D, kKeyTiles, bwd_occ(D)><<<dim3(blocks), dim3(64 * kKeyTiles), 0, st>>>(walked(p));
+  cross_dkdv_kernel<T, D, kKeyTiles, bwd_occ(D)><<<dim3(blocks), dim3(64 * kKeyTiles), 0, st>>>(walked(p, D));
   if ((rc = check_launch("tattn_cross_bwd")) || p.parts == 1) return rc;
   return sum_d<T, D>(p, true, 32 * kKeyTiles, st);
 }

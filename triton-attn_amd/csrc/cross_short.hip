@@ -65,7 +65,7 @@ __global__ __launch_bounds__(kShortWaves * 64, 2) void short_fwd_kernel(const Cr
 #pragma unroll
       for (int r = 0; r < 16; ++r) mx = __builtin_fmaxf(mx, s[k][r]);
     }
-    const float m = max_halves(mx) * c;
+    const float m = __builtin_fmaxf(max_halves(mx) * c, kNoMax);  // finite where no key is seen, too
     float l = 0.0f, le = 0.0f;  // of the rounded probabilities, for O, and as they are, for M
     f32x16 o[DT];
 #pragma unroll
