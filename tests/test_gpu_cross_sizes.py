@@ -68,6 +68,25 @@ def test_scores_that_climb_and_fall(n, s, d, dtype):
     check(q, k, v, do, i32(s, s - 33), 0.3, 2.0 ** -94)
 
 
+@pytest.mark.parametrize("scale", [-0.3, 0.0, 2.0, -3.0])
+@pytest.mark.parametrize("n,s,d,dtype", [(1, 300, 64, BF16), (40, 1000, 128, F16), (200, 700, 32, F16), (150, 300, 128, BF16), (70, 300, 64, F32),
+                                         (5, 50, 16, F16), (70, 120, 64, BF16)])
+def test_any_scale(n, s, d, dtype, scale):
+    q, k, v, do = make(3, 4, 2, n, s, d, dtype)
+    check(q, k, v, do, i32(s, 0, s - 40), scale, 2.0 ** -94)
+
+
+@pytest.mark.parametrize("scale", [-0.3, 0.0, 2.0, -3.0])
+@pytest.mark.parametrize("members,n", [(5, 3), (40, 1)])
+def test_any_scale_behind_a_prefix(members, n, scale):
+    from tattn import prefix_attention
+
+    args = make_prefix(2, members, 4, 2, n, 500, 60, 64, BF16)
+    lens, prefix_lens = torch.arange(2 * members, dtype=torch.int32, device=DEV) % 61, i32(0, 333)
+    got = prefix_attention(*args, lens, prefix_lens, sm_scale=scale)
+    close("o", got, *want_of(*args, lens, prefix_lens, scale))
+
+
 @pytest.mark.parametrize("value", [math.nan, math.inf])
 @pytest.mark.parametrize("n,s,d,dtype", [(1, 300, 64, BF16), (70, 100, 64, F16), (70, 300, 128, F16), (200, 500, 64, F16), (40, 70, 32, F32)])
 def test_what_is_not_finite_stays_in_its_row_and_head(n, s, d, dtype, value):

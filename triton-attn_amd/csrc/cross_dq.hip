@@ -18,10 +18,10 @@ __global__ __launch_bounds__(NW * 64, OCC) void cross_dq_kernel(const CrossParam
   using B = BwdPipe<D>;
   constexpr int NSD = B::NSD, DT = B::DT, STAGE = B::DQ_STAGE;
   constexpr bool LIFT = std::is_same_v<T, f16>;
-  // dS as a sum of two halves at head dim 16. With few columns the error of delta, which comes from the rounded O, adds to that of a
-  // rounded dS: dQ is then 1.55 times as far off as its last rounding leaves it (1.45 at head dim 64), and 1.1 times with two
-  // halves, at 111 us for 77 (4 x 16 x 2,048 over 2,048 x 16).
-  constexpr int NE = D == 16 ? 4 : 2;
+  // dS as a sum of two halves up to head dim 32. With few columns the error of delta, which comes from the rounded O, adds to that of
+  // a rounded dS: dQ is then 1.55 (head dim 16) and 1.5 times (32) as far off as its last rounding leaves it (1.45 at 64 and 128), and
+  // 1.1 times with two halves, at 111 us for 77 and 125 for 92 (4 x 16 x 2,048 over 2,048).
+  constexpr int NE = D <= 32 ? 4 : 2;
   __shared__ __attribute__((aligned(16))) char smem[B::NST * STAGE];
   __shared__ uint32_t norms[3][LIFT ? NW : 1];  // per wave: largest squared norm, |delta|, whether a row is lifted
 
