@@ -151,7 +151,7 @@ int fwd_d(const CrossParams& p, hipStream_t st) {
 
 }  // namespace
 
-// Up to two row tiles: one per workgroup (rows_block). More: blocks of cross_pipe_rows. Keys are cut into parts until the chip
+// Up to two row tiles: one per workgroup (rows_block; in float32 of one wave). More: blocks of cross_pipe_rows (128 in float32). Keys are cut into parts until the chip
 // holds no more workgroups at once, of at least eight tiles (in float32, where a tile takes eight times as long, three).
 void cross_fwd_plan(CrossParams& p, int D, int dtype) {
   // Few keys: a slice's row tiles in as many parts as the chip holds workgroups, of four tiles for a wave at least. us at 512, 768 and
@@ -164,11 +164,11 @@ void cross_fwd_plan(CrossParams& p, int D, int dtype) {
   }
   const int64_t tiles = ((int64_t)p.S + 31) / 32;
   p.pipe = dtype != 1 && p.rows() > 64;
-  const int64_t block = dtype == 1 ? 128 : p.pipe ? cross_pipe_rows(D) : 32;
+  p.waves = dtype == 1 && p.rows() <= 64 ? 1 : 4;
+  const int64_t block = dtype == 1 ? 32 * p.waves : p.pipe ? cross_pipe_rows(D) : 32;
   p.nblk = (int)((p.rows() + block - 1) / block);
-  const int64_t blocks = p.slices() * p.nblk, want = 256 * (dtype == 1 ? (D == 128 ? 1 : 2) : p.pipe ? 2 : rows_occ(D));
+  const int64_t blocks = p.slices() * p.nblk, want = 256 * (dtype == 1 ? cross_f32_occ(D) * 4 / p.waves : p.pipe ? 2 : rows_occ(D));
   p.splits = (int)std::max<int64_t>(1, std::min<int64_t>(want / blocks, tiles / (dtype == 1 ? 3 : 8)));
-  p.waves = 4;
   // Eight waves share the rows before the keys are cut: fewer parts to join, or none (32 x 32/8 over 375 to 1,500 x 128, one token: 22.5 us
   // for 24.6, keys in the cache).
   if (!p.pipe && dtype != 1 && p.splits > 1) {

@@ -349,10 +349,11 @@ void cross_bwd_plan(CrossParams& p, int D, int dtype) {
     p.parts = (int)std::max<int64_t>(1, std::min<int64_t>(256 * cross_short_occ(D, nt) / slices, (p.rows() + 31) / 32 / 8));
     return;
   }
-  p.nblk = (int)((p.rows() + 32 * kRowTiles - 1) / (32 * kRowTiles));
+  p.waves = dtype == 1 && p.rows() <= 64 ? 1 : kRowTiles;
+  p.nblk = (int)((p.rows() + 32 * p.waves - 1) / (32 * p.waves));
   p.kblk = (int)((p.S + keys - 1) / keys);
   const int64_t rt = (int64_t)p.G * ((p.N + 31) / 32), kt = ((int64_t)p.S + 31) / 32;
-  p.splits = (int)std::max<int64_t>(1, std::min<int64_t>(places / (slices * p.nblk), kt / (dtype == 1 ? 3 : 8)));
+  p.splits = (int)std::max<int64_t>(1, std::min<int64_t>(places * kRowTiles / p.waves / (slices * p.nblk), kt / (dtype == 1 ? 3 : 8)));
   p.parts = (int)std::max<int64_t>(1, std::min<int64_t>(places / (slices * p.kblk), rt / (dtype == 1 ? 3 : 16)));
 }
 

@@ -1,19 +1,22 @@
 // Attention over keys of another length in float32, forward and backward, on gfx950's float32 matrix instruction
 // (f32_tiles.h). The rows, keys and parts of cross.h; four waves of a workgroup own a 32-row tile each (32 keys for dK / dV) and
-// walk the tiles of the other dimension, staged one at a time through registers into LDS, the next one's loads in flight meanwhile.
+// walk the tiles of the other dimension, staged one at a time through registers into LDS, the next one's loads in flight meanwhile. Up
+// to two row tiles are a workgroup of one wave each, over more parts of the keys: all SIMDs then have a tile to work on.
 // Nothing is rounded below float32.
 //
 // Bound by the matrix instruction: 64 cycles for 32 x 32 x 2, 154 TF as a large product reaches it.
 // Traced, 4 x 16 x 1,024 over 1,024 x 64: forward 157 us (110 TF), dQ 216 (119), dK / dV 289 (119; 353 with one
 // wave on a SIMD, as the compiler would have it for 276 registers). 4 x 8 x 1,024 over 1,024 x 128, one wave on a SIMD: 164 (105), 225
-// (115) and 317 (109).
+// (115) and 317 (109). One query of each of 16 x 8 heads over 8,192 x 128, whole calls: forward 264 us (4.1 TB/s; 607 with the
+// workgroups of four), with gradients 1,304 (2,164).
 #include "cross.h"
 #include "f32_tiles.h"
 
 namespace tattn {
 namespace {
 
-// The rows of a workgroup of four row tiles and the lane's, and the part of the keys that is walked.
+// The rows of a workgroup of NW row tiles and the lane's, and the part of the keys that is walked.
+template <int NW>
 struct CrossRows32 {
   int slice, blk, split, row, rows, i0, i1;
   bool ok, live;
@@ -23,7 +26,7 @@ struct CrossRows32 {
     split = blk % p.splits;
     blk /= p.splits;
     rows = p.B * p.G * p.N;
-    row = 128 * blk + 32 * w + l32;
+    row = 32 * (NW * blk + w) + l32;
     live = row < rows;
     const int tiles = (CrossSlice(p, slice).len + 31) >> 5;
     i0 = (int)((int64_t)tiles * split / p.splits);
@@ -31,12 +34,12 @@ struct CrossRows32 {
   }
 };
 
-template <int D, int OCC>
-__global__ __launch_bounds__(256, OCC) void cross_fwd_f32_kernel(const CrossParams p) {
+template <int D, int NW, int OCC>
+__global__ __launch_bounds__(64 * NW, OCC) void cross_fwd_f32_kernel(const CrossParams p) {
   using C = F32<D>;
   __shared__ __attribute__((aligned(16))) float ks[32 * C::LD], vs[32 * C::LD];
   const int lane = threadIdx.x & 63, h2 = lane >> 5, l32 = lane & 31;
-  const CrossRows32 b(p, (int)uniform32(threadIdx.x >> 6), l32);
+  const CrossRows32<NW> b(p, (int)uniform32(threadIdx.x >> 6), l32);
   if (!b.ok) return;
   const CrossSlice sl(p, b.slice);
   const CrossRow r(p, sl, b.live ? b.row : 0);
@@ -49,7 +52,7 @@ __global__ __launch_bounds__(256, OCC) void cross_fwd_f32_kernel(const CrossPara
   f32x16 acc[C::DT];
 #pragma unroll
   for (int u = 0; u < C::DT; ++u) acc[u] = f32x16{};
-  Tile32<D> kn, vn;
+  Tile32<D, 64 * NW> kn, vn;
   auto load = [&](int t) {
     auto seen = [&](int key) { return key < sl.len; };
     kn.load(K, p.sk[2], 32 * t, seen);
@@ -98,12 +101,12 @@ __global__ __launch_bounds__(256, OCC) void cross_fwd_f32_kernel(const CrossPara
   if (h2 == 0 && p.m) p.m[r.index(p)] = mrow + __log2f(lt);
 }
 
-template <int D, int OCC>
-__global__ __launch_bounds__(256, OCC) void cross_dq_f32_kernel(const CrossParams p) {
+template <int D, int NW, int OCC>
+__global__ __launch_bounds__(64 * NW, OCC) void cross_dq_f32_kernel(const CrossParams p) {
   using C = F32<D>;
   __shared__ __attribute__((aligned(16))) float ks[32 * C::LD], vs[32 * C::LD];
   const int lane = threadIdx.x & 63, h2 = lane >> 5, l32 = lane & 31;
-  const CrossRows32 b(p, (int)uniform32(threadIdx.x >> 6), l32);
+  const CrossRows32<NW> b(p, (int)uniform32(threadIdx.x >> 6), l32);
   if (!b.ok) return;
   const CrossSlice sl(p, b.slice);
   const CrossRow r(p, sl, b.live ? b.row : 0);
@@ -125,7 +128,7 @@ __global__ __launch_bounds__(256, OCC) void cross_dq_f32_kernel(const CrossParam
   f32x16 dq[C::DT];
 #pragma unroll
   for (int u = 0; u < C::DT; ++u) dq[u] = f32x16{};
-  Tile32<D> kn, vn;
+  Tile32<D, 64 * NW> kn, vn;
   auto load = [&](int t) {
     auto seen = [&](int key) { return key < sl.len; };
     kn.load(K, p.sk[2], 32 * t, seen);
@@ -240,7 +243,8 @@ int fwd_d(const CrossParams& p, hipStream_t st) {
   unsigned blocks;
   int rc;
   if ((rc = cross_grid(p.slices(), (int64_t)p.nblk * p.splits, &blocks))) return rc;
-  cross_fwd_f32_kernel<D, D == 128 ? 1 : 2><<<dim3(blocks), dim3(256), 0, st>>>(p);
+  if (p.waves == 1) cross_fwd_f32_kernel<D, 1, cross_f32_occ(D)><<<dim3(blocks), dim3(64), 0, st>>>(p);
+  else cross_fwd_f32_kernel<D, 4, cross_f32_occ(D)><<<dim3(blocks), dim3(256), 0, st>>>(p);
   if ((rc = check_launch("tattn_cross_fwd")) || p.splits == 1) return rc;
   return launch_cross_combine(p, D, 1, st);
 }
@@ -250,10 +254,11 @@ int bwd_d(const CrossParams& p, hipStream_t st) {
   unsigned blocks;
   int rc;
   if ((rc = cross_grid(p.slices(), (int64_t)p.nblk * p.splits, &blocks))) return rc;
-  cross_dq_f32_kernel<D, D == 128 ? 1 : 2><<<dim3(blocks), dim3(256), 0, st>>>(p);
+  if (p.waves == 1) cross_dq_f32_kernel<D, 1, cross_f32_occ(D)><<<dim3(blocks), dim3(64), 0, st>>>(p);
+  else cross_dq_f32_kernel<D, 4, cross_f32_occ(D)><<<dim3(blocks), dim3(256), 0, st>>>(p);
   if ((rc = check_launch("tattn_cross_bwd")) || (p.splits > 1 && (rc = launch_cross_sum(p, D, 1, false, 0, st)))) return rc;
   if ((rc = cross_grid(p.slices(), (int64_t)p.kblk * p.parts, &blocks))) return rc;
-  cross_dkdv_f32_kernel<D, D == 128 ? 1 : 2><<<dim3(blocks), dim3(256), 0, st>>>(p);
+  cross_dkdv_f32_kernel<D, cross_f32_occ(D)><<<dim3(blocks), dim3(256), 0, st>>>(p);
   if ((rc = check_launch("tattn_cross_bwd")) || p.parts == 1) return rc;
   return launch_cross_sum(p, D, 1, true, 128, st);
 }

@@ -165,7 +165,7 @@ struct CrossParams {
   int32_t Zs, B, H, Hk, G, N, S;
   int32_t nblk, splits;   // row blocks of a slice, parts of their keys
   int32_t joined;         // forward: results are parts even where there is one
-  int32_t waves;          // forward: of a workgroup where rows are few
+  int32_t waves;          // of a workgroup: forward where rows are few, dQ in float32
   int32_t pipe;           // forward: row blocks of cross_pipe_rows rows, walked by all waves together
   int32_t kblk, parts;    // backward: key blocks of a slice, parts of their rows
   float c, scale;
@@ -199,6 +199,7 @@ constexpr bool cross_short_piped(int D, int tiles) { return D < 128 && tiles * (
 int launch_cross_short(const CrossParams& p, int D, int dtype, bool bwd, hipStream_t st);
 int launch_cross_short_pipe(const CrossParams& p, int D, int dtype, hipStream_t st);
 int launch_cross_dq(const CrossParams& p, int D, int dtype, hipStream_t st);  // 16-bit; dQ (its parts) and delta
+constexpr int cross_f32_occ(int D) { return D == 128 ? 1 : 2; }  // waves per SIMD in float32
 int launch_cross_f32(const CrossParams& p, int D, bool bwd, hipStream_t st);
 int launch_cross_combine(const CrossParams& p, int D, int dtype, hipStream_t st);  // joins the forward's parts
 // Adds the parts of dQ, or of dK and dV for key blocks of `block` keys.
