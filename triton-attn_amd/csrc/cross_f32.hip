@@ -4,16 +4,49 @@
 // to two row tiles are a workgroup of one wave each, over more parts of the keys: all SIMDs then have a tile to work on.
 // Nothing is rounded below float32.
 //
-// Bound by the matrix instruction: 64 cycles for 32 x 32 x 2, 154 TF as a large product reaches it.
-// Traced, 4 x 16 x 1,024 over 1,024 x 64: forward 157 us (110 TF), dQ 216 (119), dK / dV 289 (119; 353 with one
-// wave on a SIMD, as the compiler would have it for 276 registers). 4 x 8 x 1,024 over 1,024 x 128, one wave on a SIMD: 164 (105), 225
-// (115) and 317 (109). One query of each of 16 x 8 heads over 8,192 x 128, whole calls: forward 264 us (4.1 TB/s; 607 with the
+// Bound by the matrix instruction, 64 cycles for 32 x 32 x 2 (154 TF as a large product reaches it), and by the other vector work, which
+// does not overlap it even where a SIMD has two waves. Traced, 4 x 16 x 1,024 over 1,024 x 64: forward 149 us (116 TF), dQ 208 (124),
+// dK / dV 272 (126; with one wave on a SIMD, as the compiler would have it for 276 registers, a fifth more). 4 x 8 x 1,024 over 1,024 x
+// 128, one wave on a SIMD: 154 (112), 215 (120) and 301 (114). One query of each of 16 x 8 heads over 8,192 x 128, whole calls: forward 264 us (4.1 TB/s; 607 with the
 // workgroups of four), with gradients 1,304 (2,164).
 #include "cross.h"
 #include "f32_tiles.h"
 
 namespace tattn {
 namespace {
+
+// A 32-row tile on its way from memory to LDS, by NT threads; rows past the buffer's end are zeros. Offsets of 32 bits, one addition a
+// load: with 64-bit addresses and a check of each row the loads are half of a step's vector instructions (157, 216 and 289 us at 64).
+template <int D, int NT>
+struct RowTile32 {
+  using C = F32<D>;
+  static constexpr int CPT = (32 * C::CPR + NT - 1) / NT;
+  uint32_t off[CPT];
+  u32x4 x[CPT];
+  __device__ __forceinline__ void init(int64_t stride) {
+#pragma unroll
+    for (int i = 0; i < CPT; ++i) {
+      const int ch = threadIdx.x + NT * i;
+      off[i] = (uint32_t)(ch / C::CPR * stride * 4 + 16 * (ch % C::CPR));
+    }
+  }
+  __device__ __forceinline__ void load(__amdgpu_buffer_rsrc_t rs, uint32_t from) {
+#pragma unroll
+    for (int i = 0; i < CPT; ++i) x[i] = rsrc_load(rs, off[i] + from);
+  }
+  __device__ __forceinline__ void store(float* lds) const {
+#pragma unroll
+    for (int i = 0; i < CPT; ++i) {
+      const int ch = threadIdx.x + NT * i, row = ch / C::CPR;
+      if (32 * C::CPR % NT == 0 || row < 32)
+        *reinterpret_cast<TATTN_LDS u32x4*>((TATTN_LDS float*)lds + row * C::LD + 4 * (ch % C::CPR)) = x[i];
+    }
+  }
+};
+template <int D>
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t rows32_rsrc(const void* base, int64_t off, int64_t rows, int64_t stride) {
+  return slice_rsrc((const float*)base + off, rows > 0 ? slice_bytes(rows, 2 * stride, 2 * D) : 0);
+}
 
 // The rows of a workgroup of NW row tiles and the lane's, and the part of the keys that is walked.
 template <int NW>
@@ -44,19 +77,21 @@ __global__ __launch_bounds__(64 * NW, OCC) void cross_fwd_f32_kernel(const Cross
   const CrossSlice sl(p, b.slice);
   const CrossRow r(p, sl, b.live ? b.row : 0);
   const float c = p.c, hidden = hidden_score(c);
-  const float* K = (const float*)p.k + sl.zs * p.sk[0] + sl.hk * p.sk[1];
-  const float* V = (const float*)p.v + sl.zs * p.sv[0] + sl.hk * p.sv[1];
+  const __amdgpu_buffer_rsrc_t krs = rows32_rsrc<D>(p.k, sl.zs * p.sk[0] + sl.hk * p.sk[1], sl.len, p.sk[2]);
+  const __amdgpu_buffer_rsrc_t vrs = rows32_rsrc<D>(p.v, sl.zs * p.sv[0] + sl.hk * p.sv[1], sl.len, p.sv[2]);
+  const uint32_t kb = uniform32((uint32_t)(p.sk[2] * 128)), vb = uniform32((uint32_t)(p.sv[2] * 128));
   float q[C::H];
   own_row<D>((const float*)p.q + r.at(p.sq), b.live, h2, q);
   float mrow = kNoMax, lrow = 0.0f;
   f32x16 acc[C::DT];
 #pragma unroll
   for (int u = 0; u < C::DT; ++u) acc[u] = f32x16{};
-  Tile32<D, 64 * NW> kn, vn;
+  RowTile32<D, 64 * NW> kn, vn;
+  kn.init(p.sk[2]);
+  vn.init(p.sv[2]);
   auto load = [&](int t) {
-    auto seen = [&](int key) { return key < sl.len; };
-    kn.load(K, p.sk[2], 32 * t, seen);
-    vn.load(V, p.sv[2], 32 * t, seen);
+    kn.load(krs, (uint32_t)t * kb);
+    vn.load(vrs, (uint32_t)t * vb);
   };
   if (b.i0 < b.i1) load(b.i0);
   for (int t = b.i0; t < b.i1; ++t) {
@@ -111,8 +146,9 @@ __global__ __launch_bounds__(64 * NW, OCC) void cross_dq_f32_kernel(const CrossP
   const CrossSlice sl(p, b.slice);
   const CrossRow r(p, sl, b.live ? b.row : 0);
   const float c = p.c, hidden = hidden_score(c);
-  const float* K = (const float*)p.k + sl.zs * p.sk[0] + sl.hk * p.sk[1];
-  const float* V = (const float*)p.v + sl.zs * p.sv[0] + sl.hk * p.sv[1];
+  const __amdgpu_buffer_rsrc_t krs = rows32_rsrc<D>(p.k, sl.zs * p.sk[0] + sl.hk * p.sk[1], sl.len, p.sk[2]);
+  const __amdgpu_buffer_rsrc_t vrs = rows32_rsrc<D>(p.v, sl.zs * p.sv[0] + sl.hk * p.sv[1], sl.len, p.sv[2]);
+  const uint32_t kb = uniform32((uint32_t)(p.sk[2] * 128)), vb = uniform32((uint32_t)(p.sv[2] * 128));
   float q[C::H], go[C::H];
   own_row<D>((const float*)p.q + r.at(p.sq), b.live, h2, q);
   own_row<D>((const float*)p.dout + r.at(p.sd), b.live, h2, go);
@@ -128,11 +164,12 @@ __global__ __launch_bounds__(64 * NW, OCC) void cross_dq_f32_kernel(const CrossP
   f32x16 dq[C::DT];
 #pragma unroll
   for (int u = 0; u < C::DT; ++u) dq[u] = f32x16{};
-  Tile32<D, 64 * NW> kn, vn;
+  RowTile32<D, 64 * NW> kn, vn;
+  kn.init(p.sk[2]);
+  vn.init(p.sv[2]);
   auto load = [&](int t) {
-    auto seen = [&](int key) { return key < sl.len; };
-    kn.load(K, p.sk[2], 32 * t, seen);
-    vn.load(V, p.sv[2], 32 * t, seen);
+    kn.load(krs, (uint32_t)t * kb);
+    vn.load(vrs, (uint32_t)t * vb);
   };
   if (b.i0 < b.i1) load(b.i0);
   for (int t = b.i0; t < b.i1; ++t) {
@@ -182,13 +219,15 @@ __global__ __launch_bounds__(256, OCC) void cross_dkdv_f32_kernel(const CrossPar
   f32x16 dk[C::DT], dv[C::DT];
 #pragma unroll
   for (int u = 0; u < C::DT; ++u) dk[u] = dv[u] = f32x16{};
-  Tile32<D> qn, gn;
+  RowTile32<D, 256> qn, gn;
+  qn.init(p.sq[2]);
+  gn.init(p.sd[2]);
+  const uint32_t qb = uniform32((uint32_t)(p.sq[2] * 128)), ob = uniform32((uint32_t)(p.sd[2] * 128));
   float mn = 0.0f;
   auto load = [&](int i) {
     const int g = i / nq, first = 32 * (i % nq);
-    auto in = [&](int n) { return n < p.N; };
-    qn.load((const float*)p.q + sl.zs * p.sq[0] + (sl.hk * p.G + g) * p.sq[1], p.sq[2], first, in);
-    gn.load((const float*)p.dout + sl.zs * p.sd[0] + (sl.hk * p.G + g) * p.sd[1], p.sd[2], first, in);
+    qn.load(rows32_rsrc<D>(p.q, sl.zs * p.sq[0] + (sl.hk * p.G + g) * p.sq[1], p.N, p.sq[2]), (uint32_t)(i % nq) * qb);
+    gn.load(rows32_rsrc<D>(p.dout, sl.zs * p.sd[0] + (sl.hk * p.G + g) * p.sd[1], p.N, p.sd[2]), (uint32_t)(i % nq) * ob);
     if (tid < 64) mn = first + l32 < p.N ? (h2 ? p.delta : p.m)[((int64_t)slice * p.G + g) * p.N + first + l32] : 0.0f;
   };
   if (i0 < i1) load(i0);

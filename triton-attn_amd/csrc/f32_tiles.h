@@ -1,5 +1,5 @@
 // Tiles of 32 rows in float32 for v_mfma_f32_32x32x2f32: A lane holds A[m = lane % 32][k = lane / 32], B lane
-// B[k = lane / 32][n = lane % 32].
+// B[k = lane / 32][n = lane % 32]. Workgroups of 256 threads.
 #pragma once
 
 #include "common.h"
@@ -14,28 +14,28 @@ struct F32 {
   static constexpr int DT = (D + 31) / 32;
   static constexpr int LD = D + 4;              // floats per row in LDS
   static constexpr int CPR = D / 4;             // 16-byte chunks per row
+  static constexpr int CPT = (32 * CPR + 255) / 256;
 };
 
-// A 32-row tile on its way from memory to LDS, by NT threads.
-template <int D, int NT = 256>
+// A 32-row tile on its way from memory to LDS.
+template <int D>
 struct Tile32 {
   using C = F32<D>;
-  static constexpr int CPT = (32 * C::CPR + NT - 1) / NT;
-  f32x4 x[CPT];
+  f32x4 x[C::CPT];
   // Row i of the tile where ok(i), else zeros.
   template <typename Ok>
   __device__ __forceinline__ void load(const float* base, int64_t stride, int first, Ok ok) {
 #pragma unroll
-    for (int i = 0; i < CPT; ++i) {
-      const int ch = threadIdx.x + NT * i, row = ch / C::CPR;
+    for (int i = 0; i < C::CPT; ++i) {
+      const int ch = threadIdx.x + 256 * i, row = ch / C::CPR;
       x[i] = f32x4{};
       if (row < 32 && ok(first + row)) x[i] = *reinterpret_cast<const f32x4*>(base + (int64_t)(first + row) * stride + 4 * (ch % C::CPR));
     }
   }
   __device__ __forceinline__ void store(float* lds) const {
 #pragma unroll
-    for (int i = 0; i < CPT; ++i) {
-      const int ch = threadIdx.x + NT * i, row = ch / C::CPR;
+    for (int i = 0; i < C::CPT; ++i) {
+      const int ch = threadIdx.x + 256 * i, row = ch / C::CPR;
       if (row < 32) *reinterpret_cast<TATTN_LDS f32x4*>((TATTN_LDS float*)lds + row * C::LD + 4 * (ch % C::CPR)) = x[i];
     }
   }
