@@ -5,8 +5,9 @@
 // Few rows: cross_rows.h. Many: cross_pipe.h. Few keys: cross_short.hip. The keys are cut into parts where workgroups are few, and
 // combine_kernel joins the parts in order.
 //
-// Few rows are bound by the keys' bytes. One token of each sequence, keys not in a cache, us (as a copy): 32 x 32/8 over 375 to 1,500 x 128
-// 28 (22), 64 x 32/8 over 1,024 x 128 50 (47), 64 x 32/8 over 1,024 to 4,096 x 64 66 (59), 1 x 32 over 131,072 x 128 367 (377).
+// Few rows are bound by the keys' bytes. One token of each sequence, keys not in a cache, us (as a copy): 32 x 32/8 over 375 to
+// 1,500 x 128 28 (22), 64 x 32/8 over 1,024 x 128 50 (47), 64 x 32/8 over 1,024 to 4,096 x 64 66 (59), 1 x 32 over 131,072 x
+// 128 367 (377).
 //
 // Roundings: P is rounded to the element type, as the matrix instruction takes it, and its sum is taken from the rounded values.
 // Scores, maxima, sums and accumulators are float32.
@@ -151,8 +152,9 @@ int fwd_d(const CrossParams& p, hipStream_t st) {
 
 }  // namespace
 
-// Up to two row tiles: one per workgroup (rows_block; in float32 of one wave). More: blocks of cross_pipe_rows (128 in float32). Keys are cut into parts until the chip
-// holds no more workgroups at once, of at least eight tiles (in float32, where a tile takes eight times as long, three).
+// Up to two row tiles: one per workgroup (rows_block; in float32 of one wave). More: blocks of cross_pipe_rows (128 in
+// float32). Keys are cut into parts until the chip holds no more workgroups at once, of at least eight tiles (in float32, where
+// a tile takes eight times as long, three).
 void cross_fwd_plan(CrossParams& p, int D, int dtype) {
   // Few keys: a slice's row tiles in as many parts as the chip holds workgroups, of four tiles for a wave at least. us at 512, 768 and
   // 1,024: 16 x 8 x 4,096 over 77 x 64 41, 39, 44; over 64 x 128 57, 62, 59; 16 x 16 x 4,096 over 77 x 32 51, 49, 45.
@@ -169,8 +171,8 @@ void cross_fwd_plan(CrossParams& p, int D, int dtype) {
   p.nblk = (int)((p.rows() + block - 1) / block);
   const int64_t blocks = p.slices() * p.nblk, want = 256 * (dtype == 1 ? cross_f32_occ(D) * 4 / p.waves : p.pipe ? 2 : rows_occ(D));
   p.splits = (int)std::max<int64_t>(1, std::min<int64_t>(want / blocks, tiles / (dtype == 1 ? 3 : 8)));
-  // Eight waves share the rows before the keys are cut: fewer parts to join, or none (32 x 32/8 over 375 to 1,500 x 128, one token: 22.5 us
-  // for 24.6, keys in the cache).
+  // Eight waves share the rows before the keys are cut: fewer parts to join, or none (32 x 32/8 over 375 to 1,500 x 128, one
+  // token: 22.5 us for 24.6, keys in the cache).
   if (!p.pipe && dtype != 1 && p.splits > 1) {
     p.waves = 8;
     p.splits = (int)std::max<int64_t>(1, std::min<int64_t>(want / 2 / blocks, tiles / 16));

@@ -4,10 +4,10 @@
 //   dQ = dS K scale,  dK = dS^T Q scale,  dV = P^T dO,  the last two summed over the query heads of a key head
 //
 // Two kernels, no atomics: `cross_dq_kernel` (cross_dq.hip) owns rows and walks the keys (it also computes delta),
-// `cross_dkdv_kernel` owns keys and walks the rows of all heads. A wave keeps 32 rows (keys) in registers. Per step of 32 keys (rows) it issues the
-// first products of the next step and the second products of the one before, none of which wait for the step's exponentials. Tiles
-// come through registers into a ring of four LDS stages, one barrier per step. Where there are too few blocks to fill the
-// chip, the walked dimension is cut into parts, whose float32 sums `cross_sum_kernel` adds in order.
+// `cross_dkdv_kernel` owns keys and walks the rows of all heads. A wave keeps 32 rows (keys) in registers. Per step of 32 keys
+// (rows) it issues the first products of the next step and the second products of the one before, none of which wait for the
+// step's exponentials. Tiles come through registers into a ring of four LDS stages, one barrier per step. Where there are too
+// few blocks to fill the chip, the walked dimension is cut into parts, whose float32 sums `cross_sum_kernel` adds in order.
 //
 // Keys at or past len are fetched as zeros and get zero gradients.
 //
@@ -340,7 +340,8 @@ int bwd_d(const CrossParams& p, hipStream_t st) {
 }  // namespace
 
 // Blocks are cut into parts while all of them together leave half of the chip's places empty (two workgroups a CU, one at head dim
-// 128); a part has at least 8 tiles of keys or 16 of rows, in float32, where a tile takes eight times as long, three.
+// 128, dQ in float32 of up to two row tiles four times as many of one wave); a part has at least 8 tiles of keys or 16 of rows, in
+// float32, where a tile takes eight times as long, three.
 void cross_bwd_plan(CrossParams& p, int D, int dtype) {
   const int64_t slices = p.slices(), places = 256 * bwd_occ(D), keys = 32 * kKeyTiles;
   if (cross_short(p, D, dtype, true)) {  // row tiles of a slice in as many parts as the chip holds at once, two a wave at least

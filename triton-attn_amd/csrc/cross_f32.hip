@@ -4,11 +4,11 @@
 // to two row tiles are a workgroup of one wave each, over more parts of the keys: all SIMDs then have a tile to work on.
 // Nothing is rounded below float32.
 //
-// Bound by the matrix instruction, 64 cycles for 32 x 32 x 2 (154 TF as a large product reaches it), and by the other vector work, which
-// does not overlap it even where a SIMD has two waves. Traced, 4 x 16 x 1,024 over 1,024 x 64: forward 149 us (116 TF), dQ 208 (124),
-// dK / dV 272 (126; with one wave on a SIMD, as the compiler would have it for 276 registers, a fifth more). 4 x 8 x 1,024 over 1,024 x
-// 128, one wave on a SIMD: 154 (112), 215 (120) and 301 (114). One query of each of 16 x 8 heads over 8,192 x 128, whole calls: forward 264 us (4.1 TB/s; 607 with the
-// workgroups of four), with gradients 1,304 (2,164).
+// Bound by the matrix instruction, 64 cycles for 32 x 32 x 2 (154 TF as a large product reaches it), and by the other vector
+// work, which does not overlap it even where a SIMD has two waves. Traced, 4 x 16 x 1,024 over 1,024 x 64: forward 149 us (116
+// TF), dQ 208 (124), dK / dV 272 (126; with one wave on a SIMD, as the compiler would have it for 276 registers, a fifth more).
+// 4 x 8 x 1,024 over 1,024 x 128, one wave on a SIMD: 154 (112), 215 (120) and 301 (114). One query of each of 16 x 8 heads
+// over 8,192 x 128, whole calls: forward 264 us (4.1 TB/s; 607 with the workgroups of four), with gradients 1,304 (2,164).
 #include "cross.h"
 #include "f32_tiles.h"
 

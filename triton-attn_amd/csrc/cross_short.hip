@@ -1,19 +1,19 @@
 // Attention over few keys (a short text that many image tokens read), 16-bit, forward and the whole backward, on gfx950.
 //
-// K and V of a slice stay in LDS as NT tiles of 32 keys, and every wave walks row tiles of its own with no barrier. All scores of a row are in
-// its lane (lane = row, two halves of the keys) before any is turned into a probability, so the softmax takes its exact max and sum.
-// The backward needs neither M nor O then: with p the probabilities, delta = sum_j p_j dP_j, dS = p (dP - delta), dQ = dS K
-// scale; P and dS go through the wave's own LDS rows once to be read transposed, dV += P^T dO, dK += dS^T Q, which stay in
-// registers over all of a wave's rows. Five products run, of which all count, and q and dO are read once. The four waves' dK and dV are added
-// through LDS, and the parts that a slice's rows are cut into by cross_sum_kernel, in order.
+// K and V of a slice stay in LDS as NT tiles of 32 keys, and every wave walks row tiles of its own with no barrier. All scores
+// of a row are in its lane (lane = row, two halves of the keys) before any is turned into a probability, so the softmax takes
+// its exact max and sum. The backward needs neither M nor O then: with p the probabilities, delta = sum_j p_j dP_j, dS = p (dP
+// - delta), dQ = dS K scale; P and dS go through the wave's own LDS rows once to be read transposed, dV += P^T dO, dK += dS^T
+// Q, which stay in registers over all of a wave's rows. Five products run, of which all count, and q and dO are read once. The
+// four waves' dK and dV are added through LDS, and the parts that a slice's rows are cut into by cross_sum_kernel, in order.
 //
 // Roundings: P and dS as operands, once. In float16 dS is scaled by the power of two that the largest norms of dO and v allow
 // (|dS| <= 2 |dO| |v|); where a later tile has larger rows, what was summed is scaled down with it.
 //
 // Bound by bytes forward, and by the chain of products of the one wave that a SIMD holds backward (dK and dV of 96 keys take 192
 // registers); cross_short_pipe.hip has the form for two row tiles in a step. us, keys not in a cache: 16 x 8 x 4,096 over 77 x 64 fp16
-// forward 39 (134 MB), backward 76 (201 MB, 35 as a copy) and 5 for the sum; over 128 x 64 45 and 114; over 64 x 128 fp16 60 and 170 (some
-// registers spill; bf16, which needs no factor on dS, 120; by the kernels for many keys 300 and 267).
+// forward 39 (134 MB), backward 76 (201 MB, 35 as a copy) and 5 for the sum; over 128 x 64 45 and 114; over 64 x 128 fp16 60
+// and 170 (some registers spill; bf16, which needs no factor on dS, 120; by the kernels for many keys 300 and 267).
 #include <algorithm>
 #include <type_traits>
 
