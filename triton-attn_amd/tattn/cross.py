@@ -56,7 +56,7 @@ _plans: dict[tuple, tuple] = {}
 def _plan(q, k, v, lens) -> tuple:
     """Checks a call; which of q, k, v are copied, the strides of inputs and output (None where one is copied), the float32
     values of workspace of forward and backward, the sizes among the launches' arguments (None: nothing to see), and what the
-    backward found for gradients of each layout: which of its five inputs are copied, and all strides."""
+    backward found for its five inputs in each layout: which are copied, and all strides."""
     _check_cross(q, k, v, lens)
     _require_gpu(q)
     copies = rows_apart(q), _tiles_apart(k), _tiles_apart(v)
@@ -91,7 +91,8 @@ def _forward(q, k, v, lens, plan, scale, save_lse) -> tuple[torch.Tensor, torch.
 def _backward(q, k, v, o, m, lens, do, plan, scale) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
     floats, sizes, layouts_of = plan[3:]
     given = q, k, v, o, do
-    key = o.stride(), do.stride()
+    # Saved tensors come back as hooks on them return them, which need not be the layouts that the forward saw.
+    key = q.stride(), k.stride(), v.stride(), o.stride(), do.stride()
     hit = layouts_of.get(key)
     copies = hit[0] if hit else tuple([_tiles_apart(t) for t in given])
     tensors = tuple([aligned(t, c) for t, c in zip(given, copies)])
@@ -99,6 +100,8 @@ def _backward(q, k, v, o, m, lens, do, plan, scale) -> tuple[torch.Tensor, torch
     dq, dk, dv = torch.empty_like(q), torch.empty_like(k), torch.empty_like(v)
     if sizes is None:
         return dq.zero_(), dk.zero_(), dv.zero_()
+    m = m.contiguous()
+    lens = None if lens is None else lens.contiguous()
     work = m.new_empty(floats)
     in_place = q is given[0] and k is given[1] and v is given[2] and o is given[3] and do is given[4]
     if hit and hit[1] and in_place:
