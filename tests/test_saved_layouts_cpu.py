@@ -83,3 +83,48 @@ def step(library, back):
 def test_strides_are_those_of_the_tensors_that_come_back(library, order):
     first = [step(library, back) for back in order]
     assert [step(library, back) for back in order] == first
+
+
+# ---- qk_rope_axes ----------------------------------------------------------------------------------
+
+class RopeLibrary:
+    """Takes a copy of the tables, weights and positions that the backward is given."""
+
+    def tattn_rope_axes_fwd(self, *args):
+        return 0
+
+    def tattn_rope_axes_bwd(self, *args):
+        self.args = args
+
+        def copy(at, kind, count):
+            return list((kind * count).from_address(at))
+
+        self.got = [copy(at, ctypes.c_float, n) for at, n in zip(args[2:6], (32, 32, 9 * 16, 9 * 16))]
+        self.got.append(copy(args[6], ctypes.c_int32, 2 * 3 * 5))
+        return 0
+
+
+def columns(t):
+    """The same values with the last dimension outermost in memory."""
+    return t.transpose(0, -1).contiguous().transpose(0, -1) if t.dim() > 1 else t.repeat_interleave(2)[::2]
+
+
+def test_tables_weights_and_positions_are_read_in_the_layout_that_they_come_back_with(monkeypatch):
+    from tattn import rope_axes
+
+    lib = RopeLibrary()
+    monkeypatch.setattr(_lib, "load", lambda: lib)
+    monkeypatch.setattr(rope_axes, "_plans", {})
+    monkeypatch.setattr(rope_axes, "_require_gpu", lambda q: None)
+    monkeypatch.setattr(rope_axes, "_on_device", lambda q: contextlib.nullcontext())
+    monkeypatch.setattr(rope_axes, "_stream", lambda q: None)
+    gen = torch.Generator().manual_seed(1)
+    q, k = torch.zeros(3, 4, 5, 32, requires_grad=True), torch.zeros(3, 2, 5, 32, requires_grad=True)
+    weights = [torch.randn(32, generator=gen).requires_grad_() for _ in range(2)]
+    cos, sin = (torch.randn(9, 16, generator=gen) for _ in range(2))
+    positions = torch.randint(0, 9, (2, 3, 5), generator=gen).int()
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t, columns):
+        qo, ko = rope_axes.qk_rope_axes(q, k, cos, sin, positions, (0, 1) * 8, q_weight=weights[0], k_weight=weights[1])
+        torch.autograd.grad((qo.sum() + ko.sum()), (q, k, *weights))
+    for got, want in zip(lib.got, (*weights, cos, sin, positions)):
+        assert got == want.detach().flatten().tolist()

@@ -88,7 +88,9 @@ class _RopeAxes(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx: Any, gq, gk):
-        q, k, qw, kw, cos, sin, positions = ctx.saved_tensors
+        # Saved tensors come back as hooks on them return them, which need not be in the layouts that were saved.
+        q, k, *rest = ctx.saved_tensors
+        qw, kw, cos, sin, positions = (t if t is None else aligned(t, not t.is_contiguous()) for t in rest)
         gq, gk = rows(gq), rows(gk)
         norm = qw is not None
         q, k = (rows(q), rows(k)) if norm else (gq, gk)
