@@ -69,7 +69,7 @@ __device__ __forceinline__ void load_rows(const T* base, int64_t off, int h2, u3
 }
 
 // The waves' sums of dK and dV, tile by tile of keys, added through `smem` and stored: C register r of a lane is key 8 (r / 4) + 4 h2 +
-// r % 4, column 32 u + l32. Keys at or past len have none: their P and dS are 0.
+// r % 4, column 32 u + l32. Keys at or past len get zeros: their P and dS are 0, but not their products with what is not finite.
 template <typename T, int D, int NT, int DT>
 __device__ __forceinline__ void short_sums(const CrossParams& p, const CrossSlice& sl, const ShortRows& b, char* smem,
                                            const f32x16 (&dk)[NT][DT], const f32x16 (&dv)[NT][DT], float unlift) {
@@ -101,6 +101,7 @@ __device__ __forceinline__ void short_sums(const CrossParams& p, const CrossSlic
           lo += *reinterpret_cast<const TATTN_LDS f32x4*>(sums + w * (PART / 4) + in * D + 8 * cc);
           hi += *reinterpret_cast<const TATTN_LDS f32x4*>(sums + w * (PART / 4) + in * D + 8 * cc + 4);
         }
+        if (key >= sl.len) lo = hi = f32x4{};
         if (p.parts > 1) {
           float* dst = part + (which ? KEYS * D : 0) + key * D + 8 * cc;
           *reinterpret_cast<f32x4*>(dst) = lo;
