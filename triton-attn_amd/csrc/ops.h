@@ -172,8 +172,11 @@ struct CrossParams {
   int64_t slices() const { return (int64_t)Zs * Hk; }
   int64_t rows() const { return (int64_t)B * G * N; }  // of a slice
 };
-// Partial rows of a forward split `splits` ways: for each slice, part and row D sums, then for each its max and sum.
-inline int64_t cross_part_floats(int64_t slices, int64_t rows, int64_t splits, int64_t D) { return slices * rows * splits * (D + 2); }
+// Partial rows of a forward split `splits` ways: for each slice, part and row D sums, then for each its max and sum; in whole chunks
+// of 16 bytes, so that another region may lie behind.
+inline int64_t cross_part_floats(int64_t slices, int64_t rows, int64_t splits, int64_t D) {
+  return (slices * rows * splits * (D + 2) + 3) / 4 * 4;
+}
 // Whether slices are dealt out to the XCDs (cross_coord): an eighth of the places at most is left idle.
 __host__ __device__ inline bool cross_dealt(int64_t slices) { return ((slices + 7) / 8 * 8 - slices) * 8 <= slices; }
 inline int cross_grid(int64_t slices, int64_t blocks, unsigned* out) {
