@@ -190,16 +190,14 @@ void cross_fwd_plan(CrossParams& p, int D, int dtype) {
 
 int launch_cross_fwd(const CrossParams& p, int D, int dtype, hipStream_t st) { TATTN_CROSS_SWITCH(fwd_d) }
 int launch_prefix_combine(const PrefixParams& p, int D, int dtype, hipStream_t st) { TATTN_CROSS_SWITCH(combine_prefix) }
-int launch_cross_combine(const CrossParams& p, int D, int dtype, hipStream_t st) {
-  if (dtype == 1) {
-    switch (D) {
-      case 16: return combine_cross<float, 16>(p, st);
-      case 32: return combine_cross<float, 32>(p, st);
-      case 64: return combine_cross<float, 64>(p, st);
-      case 128: return combine_cross<float, 128>(p, st);
-    }
+int launch_cross_combine_f32(const CrossParams& p, int D, hipStream_t st) {
+  switch (D) {
+    case 16: return combine_cross<float, 16>(p, st);
+    case 32: return combine_cross<float, 32>(p, st);
+    case 64: return combine_cross<float, 64>(p, st);
+    case 128: return combine_cross<float, 128>(p, st);
   }
-  TATTN_CROSS_SWITCH(combine_cross)
+  return set_error(TATTN_E_ARG, "head dim must be 16, 32, 64 or 128, got %d", D);
 }
 
 }  // namespace tattn

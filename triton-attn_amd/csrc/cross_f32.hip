@@ -285,7 +285,7 @@ int fwd_d(const CrossParams& p, hipStream_t st) {
   if (p.waves == 1) cross_fwd_f32_kernel<D, 1, cross_f32_occ(D)><<<dim3(blocks), dim3(64), 0, st>>>(p);
   else cross_fwd_f32_kernel<D, 4, cross_f32_occ(D)><<<dim3(blocks), dim3(256), 0, st>>>(p);
   if ((rc = check_launch("tattn_cross_fwd")) || p.splits == 1) return rc;
-  return launch_cross_combine(p, D, 1, st);
+  return launch_cross_combine_f32(p, D, st);
 }
 
 template <int D>

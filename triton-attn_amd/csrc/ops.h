@@ -204,7 +204,7 @@ int launch_cross_short_pipe(const CrossParams& p, int D, int dtype, hipStream_t 
 int launch_cross_dq(const CrossParams& p, int D, int dtype, hipStream_t st);  // 16-bit; dQ (its parts) and delta
 constexpr int cross_f32_occ(int D) { return D == 128 ? 1 : 2; }  // waves per SIMD in float32
 int launch_cross_f32(const CrossParams& p, int D, bool bwd, hipStream_t st);
-int launch_cross_combine(const CrossParams& p, int D, int dtype, hipStream_t st);  // joins the forward's parts
+int launch_cross_combine_f32(const CrossParams& p, int D, hipStream_t st);  // joins the parts of a forward in float32
 // Adds the parts of dQ, or of dK and dV for key blocks of `block` keys.
 int launch_cross_sum(const CrossParams& p, int D, int dtype, bool keys, int block, hipStream_t st);
 
