@@ -89,16 +89,17 @@ __device__ __forceinline__ void load_angles(const float* row, int c, float* x) {
   }
 }
 
-// Turns the lane's pairs by their angles (sign = 1) or back (-1).
+// Turns the lane's pairs by their angles (sign = 1) or back (-1), but for those whose bits in `still` are set: a turn by cosine 1 and
+// sine 0 would carry an infinity or a NaN of one of a pair into the other.
 template <int E, bool IL>
-__device__ __forceinline__ void rotate(float* x, const float* cs, const float* sn, float sign) {
+__device__ __forceinline__ void rotate(float* x, const float* cs, const float* sn, float sign, uint32_t still) {
 #pragma unroll
   for (int i = 0; i < E / 2; ++i) {
     float& a = IL ? x[2 * i] : x[i];
     float& b = IL ? x[2 * i + 1] : x[i + E / 2];
     const float s = sign * sn[i], a0 = a, b0 = b;
-    a = a0 * cs[i] - b0 * s;
-    b = b0 * cs[i] + a0 * s;
+    a = still >> i & 1 ? a0 : a0 * cs[i] - b0 * s;
+    b = still >> i & 1 ? b0 : b0 * cs[i] + a0 * s;
   }
 }
 
@@ -119,9 +120,9 @@ __device__ __forceinline__ Unit unit_of(uint32_t u, uint32_t per, int N, int H) 
   return {(int)(token / (uint32_t)N), (int)(token % (uint32_t)N), head, min(kHeads, H - head)};
 }
 
-// Angles of the unit's position; a position outside the table makes them NaN.
+// Angles of the unit's position; a position outside the table makes them NaN. Returns the pairs that are not turned: none.
 template <typename T, int D, bool IL>
-__device__ __forceinline__ void unit_angles(const NormRopeParams& p, const Unit& u, int c, float* cs, float* sn) {
+__device__ __forceinline__ uint32_t unit_angles(const NormRopeParams& p, const Unit& u, int c, float* cs, float* sn) {
   constexpr int EPC = RowCfg<T, D>::EPC;
   const int pos = p.positions ? p.positions[u.z * p.pos_stride + u.n] : u.n;
   const bool ok = pos >= 0 && pos < p.P;
@@ -132,14 +133,16 @@ __device__ __forceinline__ void unit_angles(const NormRopeParams& p, const Unit&
 #pragma unroll
     for (int i = 0; i < EPC; ++i) cs[i] = sn[i] = __builtin_nanf("");
   }
+  return 0;
 }
 
 // Angles of the unit's positions where each pair has an axis of its own. Quads: four pairs in a row share one, and are loaded
-// together. A pair without an axis is not turned; a position outside the table makes its axis's pairs NaN.
+// together. A position outside the table makes its axis's pairs NaN. Returns a bit for each pair without an axis, which is not turned.
 template <typename T, int D, bool IL>
-__device__ __forceinline__ void unit_angles(const RopeAxesParams& p, const Unit& u, int c, float* cs, float* sn) {
+__device__ __forceinline__ uint32_t unit_angles(const RopeAxesParams& p, const Unit& u, int c, float* cs, float* sn) {
   constexpr int EPC = RowCfg<T, D>::EPC, RUN = IL ? EPC / 2 : EPC, W = RUN < 4 ? RUN : 4;  // pairs in a row, and in a load
   const int64_t at = u.z * p.pos_stride + u.n;
+  uint32_t still = 0;
 #pragma unroll
   for (int i0 = 0; i0 < EPC; i0 += W) {
     const int first = IL ? i0 / RUN * (D / 4) + RUN * c + i0 % RUN : RUN * c + i0;  // of the pairs
@@ -152,8 +155,9 @@ __device__ __forceinline__ void unit_angles(const RopeAxesParams& p, const Unit&
       return (int64_t)(ok ? pos : 0) * (D / 2) + first;
     };
     auto put = [&](int i, uint32_t axis, bool ok, float x, float y) __attribute__((always_inline)) {
-      cs[i0 + i] = axis == kNoAxis ? 1.0f : ok ? x : __builtin_nanf("");
-      sn[i0 + i] = axis == kNoAxis ? 0.0f : ok ? y : __builtin_nanf("");
+      cs[i0 + i] = ok ? x : __builtin_nanf("");
+      sn[i0 + i] = ok ? y : __builtin_nanf("");
+      still |= axis == kNoAxis ? 1u << (i0 + i) : 0;
     };
     if (W == 4 && p.quads) {
       bool ok;
@@ -172,6 +176,7 @@ __device__ __forceinline__ void unit_angles(const RopeAxesParams& p, const Unit&
       }
     }
   }
+  return still;
 }
 
 // NORM: the rows are divided by their root mean square and weighted before the rotation; otherwise they are turned by p.sign times
@@ -192,7 +197,7 @@ __global__ __launch_bounds__(256) void norm_rope_fwd_kernel(const P p) {
   float x[kHeads][C::E], w[C::E], cs[C::EPC], sn[C::EPC];
 #pragma unroll
   for (int j = 0; j < kHeads; ++j) load_row<T, D>(src + (j < u.heads ? j : 0) * st[1], c, x[j]);
-  unit_angles<T, D, IL>(p, u, c, cs, sn);
+  const uint32_t still = unit_angles<T, D, IL>(p, u, c, cs, sn);
   if constexpr (NORM) load_weight<T, D>(is_k ? p.kw : p.qw, p.wide_w, c, w);
 #pragma unroll
   for (int j = 0; j < kHeads; ++j) {
@@ -204,9 +209,9 @@ __global__ __launch_bounds__(256) void norm_rope_fwd_kernel(const P p) {
       const float r = rsqrtf(row_sum<C::LPR>(s) * (1.0f / D) + p.eps);
 #pragma unroll
       for (int i = 0; i < C::E; ++i) x[j][i] = x[j][i] * r * w[i];
-      rotate<C::E, IL>(x[j], cs, sn, 1.0f);
+      rotate<C::E, IL>(x[j], cs, sn, 1.0f, still);
     } else {
-      rotate<C::E, IL>(x[j], cs, sn, p.sign);
+      rotate<C::E, IL>(x[j], cs, sn, p.sign, still);
     }
     store_row<T, D>(dst + j * so[1], c, x[j]);
   }
@@ -239,7 +244,7 @@ __global__ __launch_bounds__(kBwdThreads) void norm_rope_bwd_kernel(const P p) {
     const T* grad = (const T*)(is_k ? p.gk : p.gq) + u.z * sg[0] + u.head * sg[1] + u.n * sg[2];
     T* dst = (T*)(is_k ? p.ko : p.qo) + u.z * so[0] + u.head * so[1] + u.n * so[2];
     float cs[C::EPC], sn[C::EPC];
-    unit_angles<T, D, IL>(p, u, c, cs, sn);
+    const uint32_t still = unit_angles<T, D, IL>(p, u, c, cs, sn);
 #pragma unroll
     for (int j0 = 0; j0 < kHeads; j0 += HB) {
       if (j0 >= u.heads) break;
@@ -257,7 +262,7 @@ __global__ __launch_bounds__(kBwdThreads) void norm_rope_bwd_kernel(const P p) {
 #pragma unroll
         for (int i = 0; i < C::E; ++i) s = __builtin_fmaf(x[j][i], x[j][i], s);
         const float r = rsqrtf(row_sum<C::LPR>(s) * (1.0f / D) + p.eps);
-        rotate<C::E, IL>(t[j], cs, sn, -1.0f);
+        rotate<C::E, IL>(t[j], cs, sn, -1.0f, still);
         float m = 0.0f;
 #pragma unroll
         for (int i = 0; i < C::E; ++i) {
