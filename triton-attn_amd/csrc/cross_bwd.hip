@@ -12,7 +12,7 @@
 // Keys at or past len are fetched as zeros and get zero gradients.
 //
 // Roundings: P and dS are rounded to the element type as operands of the second products, everything else is float32. In
-// float16 dS is scaled up by a power of two first where dO is small (small_gradient_lift).
+// float16 dS is scaled by a power of two first: up where dO is small (small_gradient_lift), down where dS would pass the type.
 //
 // Bound by the issue of matrix and vector instructions. Traced, dK / dV: 4 x 16 x 4,096 over 4,096 x 64 fp16 581 us (946 TF of its four
 // products), 2 x 16 x 4,096 over 4,096 x 128 bf16, one wave on a SIMD, 560 (982).
@@ -25,8 +25,8 @@ namespace tattn {
 namespace {
 
 // ---- dK / dV -------------------------------------------------------------------------------------
-// What dS of a block of keys is scaled by, the same for the workgroup: up to the largest norm of the slice's rows of dO, and
-// so that the largest |dS| stays finite, |dS| <= |dO| |v| + |delta|.
+// What dS of a block of keys is scaled by, 2^by, the same for the workgroup: up by the largest norm of the slice's rows of dO, and up or
+// down so far that the largest |dS| stays finite, |dS| <= |dO| |v| + |delta|. Values that are not finite ask for nothing.
 template <int NW, typename V8, int N>
 __device__ __forceinline__ int keys_lift(const CrossParams& p, int slice, const V8 (&v)[N], int wu, int lane, uint32_t (&share)[NW]) {
   const u32x2* norms = reinterpret_cast<const u32x2*>(p.norms) + (int64_t)slice * p.nblk;
@@ -47,7 +47,7 @@ __device__ __forceinline__ int keys_lift(const CrossParams& p, int slice, const 
   for (int k = 1; k < NW; ++k) most = max(most, share[k]);
   const int key = norm_exponent(uniform32(most)), delta = (int)(max_wave(top[1]) >> 23) - 127;
   // |dS| < 2^(row + key + 2) + 2^(delta + 1)
-  return row >= 0 ? 0 : min(small_gradient_lift(row, 15), max(min(12 - row - key, 13 - delta), 0));
+  return row >= 30 || key >= 30 || delta >= 127 ? 0 : min(small_gradient_lift(row, 15), min(12 - row - key, 13 - delta));
 }
 
 template <typename T, int D, int NW, int OCC>
@@ -114,12 +114,23 @@ __global__ __launch_bounds__(NW * 64, OCC) void cross_dkdv_kernel(const CrossPar
       vop[s] = key < sl.len ? b : V8{};
     }
   }
-  int by = 0;  // P, and with it dS, is scaled by 2^by through M
-  if constexpr (LIFT) by = keys_lift<NW>(p, slice, vop, wu, lane, share);
-  const float lift = h2 ? 0.0f : (float)by;
+  // Up, P is scaled with dS, through M. Down, dS alone, through V and delta: P would lose its precision. V then falls below the
+  // normal range only by as much as |dO| is large: dP is off by 2^(row - 32) |dO| |v| or less (row as in keys_lift, 19 at most).
+  int by = 0;
+  if constexpr (LIFT) {
+    by = keys_lift<NW>(p, slice, vop, wu, lane, share);
+    if (by < 0) {
+      const float down = unlift_of(-by);
+#pragma unroll
+      for (int s = 0; s < NSD; ++s)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) vop[s][i] = (T)((float)vop[s][i] * down);
+    }
+  }
+  const float lift = h2 ? 0.0f : (float)max(by, 0), down = h2 ? unlift_of(max(-by, 0)) : 1.0f;
   auto store = [&](const StepRows<D, NW * 64>& from, float md, int st) __attribute__((always_inline)) {
     from.store(smem + st * STAGE, tid);
-    if (md_loader) *reinterpret_cast<float*>(smem + st * STAGE + 2 * B::TILE + 4 * tid) = md - lift;
+    if (md_loader) *reinterpret_cast<float*>(smem + st * STAGE + 2 * B::TILE + 4 * tid) = __builtin_fmaf(md, down, -lift);
   };
   CrossOp<D> at;
   at.init(lane);
@@ -212,7 +223,7 @@ __global__ __launch_bounds__(NW * 64, OCC) void cross_dkdv_kernel(const CrossPar
 
   // C register r of a lane: key 8 (r / 4) + 4 h2 + r % 4 of the tile, column 32 u + l32. Keys past len get zeros: what
   // their lanes hold is of no meaning. Parts go out as float32 sums, tiles in rows through LDS, free after the barrier.
-  const float unlift = unlift_of(by);
+  const float unlift = unlift_of(by), unlift_v = unlift_of(max(by, 0));
   if (p.parts > 1) {
     float* dst = p.kpart + (((int64_t)slice * p.kblk + kbi) * p.parts + part) * (2 * KEYS * D) + 32 * wu * D;
 #pragma unroll
@@ -223,7 +234,7 @@ __global__ __launch_bounds__(NW * 64, OCC) void cross_dkdv_kernel(const CrossPar
         if (d >= D) continue;
         const bool seen = kw0 + in < sl.len;
         dst[in * D + d] = seen ? dk[u][g] * unlift : 0.0f;
-        dst[KEYS * D + in * D + d] = seen ? dv[u][g] * unlift : 0.0f;
+        dst[KEYS * D + in * D + d] = seen ? dv[u][g] * unlift_v : 0.0f;
       }
     return;
   }
@@ -250,7 +261,7 @@ __global__ __launch_bounds__(NW * 64, OCC) void cross_dkdv_kernel(const CrossPar
     }
   };
   rows_out(dk, p.scale * unlift, (T*)p.dk + sl.zs * p.sdk[0] + sl.hk * p.sdk[1], p.sdk[2]);
-  rows_out(dv, unlift, (T*)p.dv + sl.zs * p.sdv[0] + sl.hk * p.sdv[1], p.sdv[2]);
+  rows_out(dv, unlift_v, (T*)p.dv + sl.zs * p.sdv[0] + sl.hk * p.sdv[1], p.sdv[2]);
 }
 
 // ---- sums of parts -------------------------------------------------------------------------------

@@ -11,6 +11,27 @@
 namespace tattn {
 namespace {
 
+// Whether a sum of the lane's row, whose columns lie in both halves of the wave, is not finite.
+template <int DT>
+__device__ __forceinline__ bool row_overflowed(const f32x16 (&dq)[DT], int l32) {
+  float zero = 0.0f;  // times every sum: NaN where one is not finite
+#pragma unroll
+  for (int u = 0; u < DT; ++u)
+#pragma unroll
+    for (int g = 0; g < 16; ++g) zero = __builtin_fmaf(dq[u][g], 0.0f, zero);
+  const uint64_t bad = __builtin_amdgcn_ballot_w64(zero != 0.0f);
+  return ((bad | bad >> 32) >> l32 & 1) != 0;
+}
+
+// What dS of a row in float16 is scaled by, 2^lift, in the next try after one that was not finite; false: there is none. First up where
+// dO is small (small_gradient_lift), then as it is, then down so far that it is finite whatever the values: |dS| <= |dO| (|v| + |o|) <
+// 2^(exponent + 1) 2^21, as norms of at most 128 values of float16 stay below 2^20. A row of dO that is not finite has one try.
+__device__ __forceinline__ bool next_lift(bool overflowed, int exponent, int& lift) {
+  if (!overflowed || lift < 0 || exponent >= 30 || (lift == 0 && exponent <= -7)) return false;
+  lift = lift > 0 ? 0 : -(exponent + 7);
+  return true;
+}
+
 // A wave takes 32 rows.
 template <typename T, int D, int NW, int OCC>
 __global__ __launch_bounds__(NW * 64, OCC) void cross_dq_kernel(const CrossParams p) {
@@ -23,7 +44,7 @@ __global__ __launch_bounds__(NW * 64, OCC) void cross_dq_kernel(const CrossParam
   // 1.1 times with two halves, at 111 us for 77 and 125 for 92 (4 x 16 x 2,048 over 2,048).
   constexpr int NE = D <= 32 ? 4 : 2;
   __shared__ __attribute__((aligned(16))) char smem[B::NST * STAGE];
-  __shared__ uint32_t norms[3][LIFT ? NW : 1];  // per wave: largest squared norm, |delta|, whether a row is lifted
+  __shared__ uint32_t norms[2][LIFT ? NW : 1];  // per wave: largest squared norm, |delta|
 
   const int tid = threadIdx.x;
   const int lane = tid & 63, h2 = lane >> 5, l32 = lane & 31;
@@ -52,7 +73,7 @@ __global__ __launch_bounds__(NW * 64, OCC) void cross_dq_kernel(const CrossParam
   const CrossRow r(p, sl, live ? row : 0);
   V8 qop[NSD], dop[NSD];
   float dl;
-  int lift = 0;  // dS is scaled by 2^lift
+  int lift = 0, exponent = 0;  // dS is scaled by 2^lift; of the norm of the row of dO
   uint32_t top = 0;
   {
     const T* qs = (const T*)p.q + r.at(p.sq) + 8 * h2;
@@ -72,11 +93,11 @@ __global__ __launch_bounds__(NW * 64, OCC) void cross_dq_kernel(const CrossParam
     if (live && h2 == 0 && split == 0) p.delta[(int64_t)slice * rows + row] = -dl;
     if constexpr (LIFT) {
       const uint32_t bits = __builtin_bit_cast(uint32_t, sum_halves(norm));
-      lift = small_gradient_lift(norm_exponent(bits), 60);
+      exponent = norm_exponent(bits);
+      lift = small_gradient_lift(exponent, 60);
       top = max_wave(bits);  // NaN above all
       norms[0][wu] = top;
       norms[1][wu] = max_wave(__builtin_bit_cast(uint32_t, __builtin_fabsf(dl)));
-      norms[2][wu] = __builtin_amdgcn_ballot_w64(lift > 0) != 0;
     }
   }
   const float m = live ? p.m[r.index(p)] : 0.0f;
@@ -136,7 +157,6 @@ __global__ __launch_bounds__(NW * 64, OCC) void cross_dq_kernel(const CrossParam
   next.store(smem, tid);
   second.store(smem + STAGE, tid);
   __syncthreads();
-  uint32_t lifted = 0;
   if constexpr (LIFT) {
     if (tid < 2 && split == 0) {  // for dK / dV
       top = norms[tid][0];
@@ -144,9 +164,6 @@ __global__ __launch_bounds__(NW * 64, OCC) void cross_dq_kernel(const CrossParam
       for (int k = 1; k < NW; ++k) top = max(top, norms[tid][k]);
       p.norms[2 * ((int64_t)slice * p.nblk + blk) + tid] = __builtin_bit_cast(float, top);
     }
-#pragma unroll
-    for (int k = 0; k < NW; ++k) lifted |= norms[2][k];
-    lifted = uniform32(lifted);
   }
   // Steps whose 32 keys are all there.
   const int n_full = min(nsteps, (sl.len >> 5) - i0);
@@ -180,15 +197,10 @@ __global__ __launch_bounds__(NW * 64, OCC) void cross_dq_kernel(const CrossParam
       for (int e = 0; e < NE; ++e) ea[e] = eb[e];
     }
     if (nsteps > 0) grad(ea, (nsteps - 1) & 3);
-    if (!LIFT || !lifted) break;
-    float zero = 0.0f;  // times every sum: NaN where one is not finite
-#pragma unroll
-    for (int u = 0; u < DT; ++u)
-#pragma unroll
-      for (int g = 0; g < 16; ++g) zero = __builtin_fmaf(dq[u][g], 0.0f, zero);
-    if (!__syncthreads_or(lift > 0 && zero != 0.0f)) break;
-    lifted = lift = 0;  // once more without a factor
-    nm = -m;
+    if (!LIFT) break;
+    const bool again = live && next_lift(row_overflowed(dq, l32), exponent, lift);
+    if (!__syncthreads_or(again)) break;
+    nm = live ? (float)lift - m : 0.0f;
     next.clear(smem + 3 * STAGE, tid);
     next.load(krs, vrs, (uint32_t)i0 * kb, (uint32_t)i0 * vb);
     next.store(smem, tid);
@@ -218,7 +230,7 @@ __global__ __launch_bounds__(512, 2) void cross_dq_pair_kernel(const CrossParams
   constexpr bool LIFT = std::is_same_v<T, f16>;
   __shared__ __attribute__((aligned(16))) char smem[B::NST * STAGE];
   __shared__ __attribute__((aligned(16))) char xbuf[2 * NP * XB];
-  __shared__ uint32_t norms[3][NP];  // per pair: largest squared norm, |delta|, whether a row is lifted
+  __shared__ uint32_t norms[2][NP];  // per pair: largest squared norm, |delta|
   __shared__ float lifts[NP][32];
 
   const int tid = threadIdx.x;
@@ -257,7 +269,7 @@ __global__ __launch_bounds__(512, 2) void cross_dq_pair_kernel(const CrossParams
       op[s] = live ? x : V8{};
     }
   }
-  int lift = 0;  // dS is scaled by 2^lift
+  int lift = 0, exponent = 0;  // dS is scaled by 2^lift; of the norm of the row of dO
   float dl = 0.0f;
   if (role_b) {
     const T* os = (const T*)p.o + r.at(p.so) + 8 * h2;
@@ -272,11 +284,11 @@ __global__ __launch_bounds__(512, 2) void cross_dq_pair_kernel(const CrossParams
     if (live && h2 == 0 && split == 0) p.delta[(int64_t)slice * rows + row] = -dl;
     if constexpr (LIFT) {
       const uint32_t bits = __builtin_bit_cast(uint32_t, sum_halves(norm));
-      lift = small_gradient_lift(norm_exponent(bits), 60);
+      exponent = norm_exponent(bits);
+      lift = small_gradient_lift(exponent, 60);
       lifts[pr][l32] = (float)lift;
       norms[0][pr] = max_wave(bits);  // NaN above all
       norms[1][pr] = max_wave(__builtin_bit_cast(uint32_t, __builtin_fabsf(dl)));
-      norms[2][pr] = __builtin_amdgcn_ballot_w64(lift > 0) != 0;
     }
   }
   const float m = live ? p.m[r.index(p)] : 0.0f;
@@ -287,7 +299,6 @@ __global__ __launch_bounds__(512, 2) void cross_dq_pair_kernel(const CrossParams
   next.store(smem, tid);
   second.store(smem + STAGE, tid);
   __syncthreads();
-  uint32_t lifted = 0;
   float nm = -m;
   if constexpr (LIFT) {
     if (tid < 2 && split == 0) {  // for dK / dV
@@ -296,9 +307,6 @@ __global__ __launch_bounds__(512, 2) void cross_dq_pair_kernel(const CrossParams
       for (int k = 1; k < NP; ++k) top = max(top, norms[tid][k]);
       p.norms[2 * ((int64_t)slice * p.nblk + blk) + tid] = __builtin_bit_cast(float, top);
     }
-#pragma unroll
-    for (int k = 0; k < NP; ++k) lifted |= norms[2][k];
-    lifted = uniform32(lifted);
     nm = live ? lifts[pr][l32] - m : 0.0f;
   }
   // Steps whose 32 keys are all there.
@@ -390,15 +398,11 @@ __global__ __launch_bounds__(512, 2) void cross_dq_pair_kernel(const CrossParams
     for (int u = 0; u < DT; ++u) dq[u] = f32x16{};
     if (role_b) run(std::true_type{});
     else run(std::false_type{});
-    if (!LIFT || !lifted) break;
-    float zero = 0.0f;  // times every sum: NaN where one is not finite
-#pragma unroll
-    for (int u = 0; u < DT; ++u)
-#pragma unroll
-      for (int g = 0; g < 16; ++g) zero = __builtin_fmaf(dq[u][g], 0.0f, zero);
-    if (!__syncthreads_or(lift > 0 && zero != 0.0f)) break;
-    lifted = lift = 0;  // once more without a factor
-    nm = -m;
+    if (!LIFT) break;
+    const bool again = role_b && live && next_lift(row_overflowed(dq, l32), exponent, lift);
+    if (again) lifts[pr][l32] = (float)lift;  // A has read it
+    if (!__syncthreads_or(again)) break;
+    nm = live ? lifts[pr][l32] - m : 0.0f;
     next.clear(smem + 3 * STAGE, tid);
     next.load(krs, vrs, (uint32_t)i0 * kb, (uint32_t)i0 * vb);
     next.store(smem, tid);

@@ -212,7 +212,7 @@ __global__ __launch_bounds__(kShortWaves * 64, OCC) void short_bwd_kernel(const 
       for (int s = 0; s < NSD; ++s) norm += chunk_dot(g[s], g[s]);
       const int e = norm_exponent(max_wave(__builtin_bit_cast(uint32_t, sum_halves(norm))));
       // |dS| < 2^(e + ev + 3); rows with an infinity or a NaN, which spoil their own results, ask for nothing.
-      const int most = e >= 30 || ev >= 30 ? 0 : max(12 - e - ev, -20);
+      const int most = e >= 30 || ev >= 30 ? 0 : 12 - e - ev;
       if (most < lift) {
         const float down = unlift_of(lift - most);  // 2^(most - lift)
         lift = most;

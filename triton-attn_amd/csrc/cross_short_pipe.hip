@@ -117,7 +117,7 @@ __global__ __launch_bounds__(kShortWaves * 64, 1) void short_pipe_kernel(const C
       for (int i = 0; i < NSD; ++i) norm += chunk_dot(g[i], g[i]);
       const int e = norm_exponent(max_wave(__builtin_bit_cast(uint32_t, sum_halves(norm))));
       // |dS| < 2^(e + ev + 3); rows with an infinity or a NaN, which spoil their own results, ask for nothing.
-      most = e >= 30 || ev >= 30 ? 0 : max(12 - e - ev, -20);
+      most = e >= 30 || ev >= 30 ? 0 : 12 - e - ev;
     }
 #pragma unroll
     for (int k = 0; k < NT; ++k) {
