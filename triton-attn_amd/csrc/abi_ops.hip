@@ -442,10 +442,10 @@ int tattn_cross_workspace(int backward, int64_t Z, int64_t H, int64_t Hk, int64_
   if (!floats) return set_error(TATTN_E_ARG, "floats is a null pointer");
   if ((rc = cross_common(p, Z, 1, H, Hk, N, S, D, 1)) || (rc = check_dtype(dtype))) return rc;
   if (backward) {
-    cross_bwd_plan(p, (int)D, dtype);
+    if ((rc = cross_bwd_plan(p, (int)D, dtype))) return rc;
     *floats = cross_bwd_floats(p, (int)D, dtype);
   } else {
-    cross_fwd_plan(p, (int)D, dtype);
+    if ((rc = cross_fwd_plan(p, (int)D, dtype))) return rc;
     *floats = p.splits > 1 ? cross_part_floats(p.slices(), p.rows(), p.splits, D) : 0;
   }
   return TATTN_OK;
@@ -462,8 +462,7 @@ int tattn_cross_fwd(const void* q, const void* k, const void* v, void* o, float*
       (rc = check_tiles("v", v, v_strides, S, D, dtype, p.sv)) || (rc = check_lone_rows("o", o, o_strides, dtype, p.sout)) ||
       (rc = check_ptr("m", m, 0, 4)) || (rc = check_ptr("lens", lens, 0, 4)))
     return rc;
-  cross_fwd_plan(p, (int)D, dtype);
-  if ((rc = check_ptr("workspace", workspace, p.splits > 1, 16)) || (rc = require_device())) return rc;
+  if ((rc = cross_fwd_plan(p, (int)D, dtype)) || (rc = check_ptr("workspace", workspace, p.splits > 1, 16)) || (rc = require_device())) return rc;
   p.q = q; p.k = k; p.v = v; p.out = o; p.m = m; p.lens = lens; p.part = workspace;
   p.c = window_exponent_scale(sm_scale);
   p.scale = sm_scale;
@@ -486,8 +485,7 @@ int tattn_cross_bwd(const void* q, const void* k, const void* v, const void* o, 
       (rc = check_tiles("dk", dk, dk_strides, S, D, dtype, p.sdk)) || (rc = check_tiles("dv", dv, dv_strides, S, D, dtype, p.sdv)) ||
       (rc = check_ptr("m", m, 1, 4)) || (rc = check_ptr("lens", lens, 0, 4)) || (rc = check_ptr("workspace", workspace, 1, 16)))
     return rc;
-  cross_bwd_plan(p, (int)D, dtype);
-  if ((rc = require_device())) return rc;
+  if ((rc = cross_bwd_plan(p, (int)D, dtype)) || (rc = require_device())) return rc;
   p.q = q; p.k = k; p.v = v; p.o = o; p.dout = dout; p.out = dq; p.dk = dk; p.dv = dv; p.lens = lens;
   p.m = const_cast<float*>(m);
   cross_bwd_workspace(p, (int)D, dtype, workspace);
@@ -505,7 +503,7 @@ int tattn_prefix_workspace(int64_t groups, int64_t members, int64_t H, int64_t H
   if ((rc = cross_common(p.pre, groups, members, H, Hk, N, P, D, 0)) ||
       (rc = cross_common(p.own, groups * members, 1, H, Hk, N, S, D, 0)))
     return rc;
-  prefix_plan(p, (int)D);
+  if ((rc = prefix_plan(p, (int)D))) return rc;
   *floats = prefix_floats(p, (int)D);
   return TATTN_OK;
 }
@@ -528,8 +526,7 @@ int tattn_prefix_attention(const void* q, const void* prefix_k, const void* pref
     return rc;
   if (S > 0 && ((rc = check_tiles("k", k, k_strides, S, D, dtype, b.sk)) || (rc = check_tiles("v", v, v_strides, S, D, dtype, b.sv))))
     return rc;
-  if ((rc = require_device())) return rc;
-  prefix_plan(p, (int)D);
+  if ((rc = prefix_plan(p, (int)D)) || (rc = require_device())) return rc;
   for (int i = 0; i < 3; ++i) b.sq[i] = a.sq[i], b.sout[i] = a.sout[i];
   a.q = b.q = q; a.out = b.out = o;
   a.c = b.c = window_exponent_scale(sm_scale);

@@ -100,11 +100,8 @@ __global__ __launch_bounds__(256) void combine_kernel(const CombineParams p) {
 
 template <typename T, int D>
 int combine(CombineParams p, hipStream_t st, const char* what) {
-  constexpr int GROUPS = 256 / (D / 4);
-  const int most = std::max(p.splits[0], p.part[1] ? p.splits[1] : 0);
-  for (p.dealt = 1; p.dealt < GROUPS && 4 * p.dealt < most; p.dealt *= 2) {}
-  const int64_t rows = p.slices * p.B * p.G * p.N, per = GROUPS / p.dealt, blocks = (rows + per - 1) / per;
-  if (blocks > 0x7fffffff) return set_error(TATTN_E_ARG, "grid too large: %lld rows", (long long)rows);
+  const int64_t blocks = combine_blocks(p.slices * p.B * p.G * p.N, std::max(p.splits[0], p.part[1] ? p.splits[1] : 0), D, p.dealt);
+  if (int rc = check_grid(blocks, 256)) return rc;
   combine_kernel<T, D><<<dim3((unsigned)blocks), dim3(256), 0, st>>>(p);
   return check_launch(what);
 }
@@ -143,7 +140,7 @@ int fwd_d(const CrossParams& p, hipStream_t st) {
     if ((rc = launch_cross_pipe(p, D, std::is_same_v<T, f16> ? 0 : 2, st)) || p.splits == 1) return rc;
     return combine_cross<T, D>(p, st);
   }
-  if ((rc = cross_grid(p.slices(), (int64_t)p.nblk * p.splits, &blocks))) return rc;
+  if ((rc = cross_grid(p.slices(), (int64_t)p.nblk * p.splits, 64 * p.waves, &blocks))) return rc;
   if (p.waves == 8) cross_rows_kernel<T, D, 8, rows_occ(D)><<<dim3(blocks), dim3(512), 0, st>>>(p);
   else cross_rows_kernel<T, D, 4, rows_occ(D)><<<dim3(blocks), dim3(256), 0, st>>>(p);
   if ((rc = check_launch("tattn_cross_fwd")) || p.splits == 1) return rc;
@@ -155,14 +152,15 @@ int fwd_d(const CrossParams& p, hipStream_t st) {
 // Up to two row tiles: one per workgroup (rows_block; in float32 of one wave). More: blocks of cross_pipe_rows (128 in
 // float32). Keys are cut into parts until the chip holds no more workgroups at once, of at least eight tiles (in float32, where
 // a tile takes eight times as long, three).
-void cross_fwd_plan(CrossParams& p, int D, int dtype) {
+int cross_fwd_plan(CrossParams& p, int D, int dtype) {
+  unsigned launched;
   // Few keys: a slice's row tiles in as many parts as the chip holds workgroups, of four tiles for a wave at least. us at 512, 768 and
   // 1,024: 16 x 8 x 4,096 over 77 x 64 41, 39, 44; over 64 x 128 57, 62, 59; 16 x 16 x 4,096 over 77 x 32 51, 49, 45.
   if (cross_short(p, D, dtype, false)) {
     const int64_t tiles = (p.rows() + 31) / 32, places = 256 * (D == 128 ? 2 : D == 64 ? 3 : 4);
     p.nblk = (int)std::max<int64_t>(1, std::min<int64_t>(places / p.slices(), tiles / 16));
     p.splits = 1;
-    return;
+    return cross_grid(p.slices(), p.nblk, 256, &launched);
   }
   const int64_t tiles = ((int64_t)p.S + 31) / 32;
   p.pipe = dtype != 1 && p.rows() > 64;
@@ -177,6 +175,7 @@ void cross_fwd_plan(CrossParams& p, int D, int dtype) {
     p.waves = 8;
     p.splits = (int)std::max<int64_t>(1, std::min<int64_t>(want / 2 / blocks, tiles / 16));
   }
+  return cross_grid(p.slices(), (int64_t)p.nblk * p.splits, 64 * p.waves, &launched);
 }
 
 #define TATTN_CROSS_SWITCH(FN)                                                   \

@@ -303,8 +303,8 @@ __global__ __launch_bounds__(256) void cross_sum_kernel(const CrossParams p, int
 
 template <typename T, int D>
 int sum_d(const CrossParams& p, bool keys, int block, hipStream_t st) {
-  const int64_t n = keys ? p.slices() * p.kblk * 2 * block * D / 4 : p.slices() * p.rows() * D / 4, blocks = (n + 255) / 256;
-  if (blocks > 0x7fffffff) return set_error(TATTN_E_ARG, "grid too large: %lld workgroups", (long long)blocks);
+  const int64_t blocks = cross_sum_blocks(p, D, keys, block);
+  if (int rc = check_grid(blocks, 256)) return rc;
   if (keys) cross_sum_kernel<T, D, true><<<dim3((unsigned)blocks), dim3(256), 0, st>>>(p, block);
   else cross_sum_kernel<T, D, false><<<dim3((unsigned)blocks), dim3(256), 0, st>>>(p, 0);
   return check_launch("tattn_cross_bwd");
@@ -342,7 +342,7 @@ int bwd_d(const CrossParams& p, hipStream_t st) {
   if (cross_short(p, D, std::is_same_v<T, f16> ? 0 : 2, true)) return launch_cross_short(p, D, std::is_same_v<T, f16> ? 0 : 2, true, st);
   if ((rc = launch_cross_dq(p, D, std::is_same_v<T, f16> ? 0 : 2, st))) return rc;
   if (p.splits > 1 && (rc = sum_d<T, D>(p, false, 0, st))) return rc;
-  if ((rc = cross_grid(p.slices(), (int64_t)p.kblk * p.parts, &blocks))) return rc;
+  if ((rc = cross_grid(p.slices(), (int64_t)p.kblk * p.parts, 64 * kKeyTiles, &blocks))) return rc;
   cross_dkdv_kernel<T, D, kKeyTiles, bwd_occ(D)><<<dim3(blocks), dim3(64 * kKeyTiles), 0, st>>>(walked(p, D));
   if ((rc = check_launch("tattn_cross_bwd")) || p.parts == 1) return rc;
   return sum_d<T, D>(p, true, 32 * kKeyTiles, st);
@@ -353,13 +353,16 @@ int bwd_d(const CrossParams& p, hipStream_t st) {
 // Blocks are cut into parts while all of them together leave half of the chip's places empty (two workgroups a CU, one at head dim
 // 128, dQ in float32 of up to two row tiles four times as many of one wave); a part has at least 8 tiles of keys or 16 of rows, in
 // float32, where a tile takes eight times as long, three.
-void cross_bwd_plan(CrossParams& p, int D, int dtype) {
+int cross_bwd_plan(CrossParams& p, int D, int dtype) {
+  unsigned launched;
+  int rc;
   const int64_t slices = p.slices(), places = 256 * bwd_occ(D), keys = 32 * kKeyTiles;
   if (cross_short(p, D, dtype, true)) {  // row tiles of a slice in as many parts as the chip holds at once, two a wave at least
     const int nt = (p.S + 31) / 32;
     p.nblk = p.splits = p.kblk = 1;
     p.parts = (int)std::max<int64_t>(1, std::min<int64_t>(256 * cross_short_occ(D, nt) / slices, (p.rows() + 31) / 32 / 8));
-    return;
+    if ((rc = cross_grid(slices, p.parts, 256, &launched)) || p.parts == 1) return rc;
+    return check_grid(cross_sum_blocks(p, D, true, 32 * nt), 256);
   }
   p.waves = dtype == 1 && p.rows() <= 64 ? 1 : kRowTiles;
   p.nblk = (int)((p.rows() + 32 * p.waves - 1) / (32 * p.waves));
@@ -367,6 +370,11 @@ void cross_bwd_plan(CrossParams& p, int D, int dtype) {
   const int64_t rt = (int64_t)p.G * ((p.N + 31) / 32), kt = ((int64_t)p.S + 31) / 32;
   p.splits = (int)std::max<int64_t>(1, std::min<int64_t>(places * kRowTiles / p.waves / (slices * p.nblk), kt / (dtype == 1 ? 3 : 8)));
   p.parts = (int)std::max<int64_t>(1, std::min<int64_t>(places / (slices * p.kblk), rt / (dtype == 1 ? 3 : 16)));
+  if ((rc = cross_grid(slices, (int64_t)p.nblk * p.splits, dtype == 1 ? 64 * p.waves : cross_dq_threads(D), &launched)) ||
+      (rc = cross_grid(slices, (int64_t)p.kblk * p.parts, 256, &launched)) ||
+      (p.splits > 1 && (rc = check_grid(cross_sum_blocks(p, D, false, 0), 256))))
+    return rc;
+  return p.parts > 1 ? check_grid(cross_sum_blocks(p, D, true, keys), 256) : TATTN_OK;
 }
 
 namespace {

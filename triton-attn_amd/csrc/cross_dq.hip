@@ -422,8 +422,9 @@ __global__ __launch_bounds__(512, 2) void cross_dq_pair_kernel(const CrossParams
 
 int launch_cross_dq(const CrossParams& p, int D, int dtype, hipStream_t st) {
   unsigned blocks;
-  if (int rc = cross_grid(p.slices(), (int64_t)p.nblk * p.splits, &blocks)) return rc;
-  const dim3 grid(blocks), block(D == 128 ? 512 : 256);
+  const dim3 block(cross_dq_threads(D));
+  if (int rc = cross_grid(p.slices(), (int64_t)p.nblk * p.splits, (int)block.x, &blocks)) return rc;
+  const dim3 grid(blocks);
   switch (D) {
 #define TATTN_DQ(D_)                                                           \
   case D_:                                                                     \

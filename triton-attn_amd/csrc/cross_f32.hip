@@ -281,7 +281,7 @@ template <int D>
 int fwd_d(const CrossParams& p, hipStream_t st) {
   unsigned blocks;
   int rc;
-  if ((rc = cross_grid(p.slices(), (int64_t)p.nblk * p.splits, &blocks))) return rc;
+  if ((rc = cross_grid(p.slices(), (int64_t)p.nblk * p.splits, 64 * p.waves, &blocks))) return rc;
   if (p.waves == 1) cross_fwd_f32_kernel<D, 1, cross_f32_occ(D)><<<dim3(blocks), dim3(64), 0, st>>>(p);
   else cross_fwd_f32_kernel<D, 4, cross_f32_occ(D)><<<dim3(blocks), dim3(256), 0, st>>>(p);
   if ((rc = check_launch("tattn_cross_fwd")) || p.splits == 1) return rc;
@@ -292,11 +292,11 @@ template <int D>
 int bwd_d(const CrossParams& p, hipStream_t st) {
   unsigned blocks;
   int rc;
-  if ((rc = cross_grid(p.slices(), (int64_t)p.nblk * p.splits, &blocks))) return rc;
+  if ((rc = cross_grid(p.slices(), (int64_t)p.nblk * p.splits, 64 * p.waves, &blocks))) return rc;
   if (p.waves == 1) cross_dq_f32_kernel<D, 1, cross_f32_occ(D)><<<dim3(blocks), dim3(64), 0, st>>>(p);
   else cross_dq_f32_kernel<D, 4, cross_f32_occ(D)><<<dim3(blocks), dim3(256), 0, st>>>(p);
   if ((rc = check_launch("tattn_cross_bwd")) || (p.splits > 1 && (rc = launch_cross_sum(p, D, 1, false, 0, st)))) return rc;
-  if ((rc = cross_grid(p.slices(), (int64_t)p.kblk * p.parts, &blocks))) return rc;
+  if ((rc = cross_grid(p.slices(), (int64_t)p.kblk * p.parts, 256, &blocks))) return rc;
   cross_dkdv_f32_kernel<D, cross_f32_occ(D)><<<dim3(blocks), dim3(256), 0, st>>>(p);
   if ((rc = check_launch("tattn_cross_bwd")) || p.parts == 1) return rc;
   return launch_cross_sum(p, D, 1, true, 128, st);

@@ -27,7 +27,7 @@ template <typename T, int D>
 int pipe_d(const CrossParams& p, hipStream_t st) {
   constexpr int NW = cross_pipe_waves(D);
   unsigned blocks;
-  if (int rc = cross_grid(p.slices(), (int64_t)p.nblk * p.splits, &blocks)) return rc;
+  if (int rc = cross_grid(p.slices(), (int64_t)p.nblk * p.splits, 64 * NW, &blocks)) return rc;
   cross_pipe_kernel<T, D, NW, cross_pipe_tiles(D), 2><<<dim3(blocks), dim3(NW * 64), 0, st>>>(p);
   return check_launch("tattn_cross_fwd");
 }

@@ -304,7 +304,7 @@ template <typename T, int D, int NT>
 int short_d(const CrossParams& p, bool bwd, hipStream_t st) {
   unsigned blocks;
   int rc;
-  if ((rc = cross_grid(p.slices(), bwd ? p.parts : p.nblk, &blocks))) return rc;
+  if ((rc = cross_grid(p.slices(), bwd ? p.parts : p.nblk, kShortWaves * 64, &blocks))) return rc;
   if (!bwd) {
     short_fwd_kernel<T, D, NT><<<dim3(blocks), dim3(kShortWaves * 64), 0, st>>>(p);
     return check_launch("tattn_cross_fwd");

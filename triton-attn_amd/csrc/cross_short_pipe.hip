@@ -218,7 +218,7 @@ __global__ __launch_bounds__(kShortWaves * 64, 1) void short_pipe_kernel(const C
 template <typename T, int D, int NT>
 int pipe_nt(const CrossParams& p, hipStream_t st) {
   unsigned blocks;
-  if (int rc = cross_grid(p.slices(), p.parts, &blocks)) return rc;
+  if (int rc = cross_grid(p.slices(), p.parts, kShortWaves * 64, &blocks)) return rc;
   short_pipe_kernel<T, D, NT><<<dim3(blocks), dim3(kShortWaves * 64), 0, st>>>(p);
   return check_launch("tattn_cross_bwd");
 }

@@ -179,11 +179,29 @@ inline int64_t cross_part_floats(int64_t slices, int64_t rows, int64_t splits, i
 }
 // Whether slices are dealt out to the XCDs (cross_coord): an eighth of the places at most is left idle.
 __host__ __device__ inline bool cross_dealt(int64_t slices) { return ((slices + 7) / 8 * 8 - slices) * 8 <= slices; }
-inline int cross_grid(int64_t slices, int64_t blocks, unsigned* out) {
-  return window_grid(cross_dealt(slices) ? (slices + 7) / 8 * 8 : slices, blocks, 0, out);
+// A launch holds fewer than 2^32 threads.
+inline int check_grid(int64_t blocks, int threads) {
+  if (blocks > 0xffffffffll / threads)
+    return set_error(TATTN_E_ARG, "grid too large: %lld workgroups of %d threads", (long long)blocks, threads);
+  return TATTN_OK;
 }
-void cross_fwd_plan(CrossParams& p, int D, int dtype);  // sets nblk and splits
-void cross_bwd_plan(CrossParams& p, int D, int dtype);  // sets nblk, splits, kblk and parts
+inline int cross_grid(int64_t slices, int64_t blocks, int threads, unsigned* out) {
+  const int rc = window_grid(cross_dealt(slices) ? (slices + 7) / 8 * 8 : slices, blocks, 0, out);
+  return rc ? rc : check_grid(*out, threads);
+}
+// Set nblk, splits and waves, and for the backward kblk and parts; refuse what its launches would not hold.
+int cross_fwd_plan(CrossParams& p, int D, int dtype);
+int cross_bwd_plan(CrossParams& p, int D, int dtype);
+// Workgroups that join the parts of so many rows, `most` parts a row at most; `dealt` groups of lanes share a row's parts.
+inline int64_t combine_blocks(int64_t rows, int most, int D, int32_t& dealt) {
+  const int groups = 256 / (D / 4);
+  for (dealt = 1; dealt < groups && 4 * dealt < most; dealt *= 2) {}
+  const int64_t per = groups / dealt;
+  return (rows + per - 1) / per;
+}
+inline int64_t cross_sum_blocks(const CrossParams& p, int D, bool keys, int block) {
+  return ((keys ? p.slices() * p.kblk * 2 * block * D / 4 : p.slices() * p.rows() * D / 4) + 255) / 256;
+}
 int64_t cross_bwd_floats(const CrossParams& p, int D, int dtype);  // workspace of a planned backward
 void cross_bwd_workspace(CrossParams& p, int D, int dtype, float* work);  // lays out delta, norms, part and kpart
 int launch_cross_fwd(const CrossParams& p, int D, int dtype, hipStream_t st);
@@ -201,6 +219,7 @@ inline bool cross_short(const CrossParams& p, int D, int dtype, bool bwd) { retu
 constexpr bool cross_short_piped(int D, int tiles) { return D < 128 && tiles * ((D + 31) / 32) >= 4 && tiles * ((D + 31) / 32) < 8; }
 int launch_cross_short(const CrossParams& p, int D, int dtype, bool bwd, hipStream_t st);
 int launch_cross_short_pipe(const CrossParams& p, int D, int dtype, hipStream_t st);
+constexpr int cross_dq_threads(int D) { return D == 128 ? 512 : 256; }
 int launch_cross_dq(const CrossParams& p, int D, int dtype, hipStream_t st);  // 16-bit; dQ (its parts) and delta
 constexpr int cross_f32_occ(int D) { return D == 128 ? 1 : 2; }  // waves per SIMD in float32
 int launch_cross_f32(const CrossParams& p, int D, bool bwd, hipStream_t st);
@@ -213,7 +232,7 @@ int launch_cross_sum(const CrossParams& p, int D, int dtype, bool keys, int bloc
 struct PrefixParams {
   CrossParams pre, own;
 };
-void prefix_plan(PrefixParams& p, int D);
+int prefix_plan(PrefixParams& p, int D);  // as the plans above
 int64_t prefix_floats(const PrefixParams& p, int D);
 int launch_prefix(const PrefixParams& p, int D, int dtype, hipStream_t st);
 int launch_prefix_combine(const PrefixParams& p, int D, int dtype, hipStream_t st);

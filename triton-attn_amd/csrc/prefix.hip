@@ -15,6 +15,9 @@ constexpr int prefix_occ(int D) { return D == 64 ? 3 : rows_occ(D); }
 // Workgroups over the prefix, the row blocks that read one part of it on one XCD, whose L2 hands it to the others.
 __host__ __device__ inline int64_t prefix_blocks(const CrossParams& p) { return ((int64_t)p.Zs * p.Hk * p.splits + 7) / 8 * 8 * p.nblk; }
 
+// All of a launch.
+int64_t prefix_launch(const PrefixParams& p) { return prefix_blocks(p.pre) + p.own.slices() * p.own.nblk * p.own.splits; }
+
 // The prefix's parts first, then each sequence's own keys.
 template <typename T, int D>
 __global__ __launch_bounds__(4 * 64, prefix_occ(D)) void prefix_kernel(const PrefixParams p) {
@@ -37,8 +40,8 @@ __global__ __launch_bounds__(4 * 64, prefix_occ(D)) void prefix_kernel(const Pre
 
 template <typename T, int D>
 int prefix_d(const PrefixParams& p, hipStream_t st) {
-  const int64_t blocks = prefix_blocks(p.pre) + p.own.slices() * p.own.nblk * p.own.splits;
-  if (blocks > 0x7ffffff) return set_error(TATTN_E_ARG, "grid too large: %lld workgroups", (long long)blocks);
+  const int64_t blocks = prefix_launch(p);
+  if (int rc = check_grid(blocks, 256)) return rc;
   prefix_kernel<T, D><<<dim3((unsigned)blocks), dim3(4 * 64), 0, st>>>(p);
   const int rc = check_launch("tattn_prefix_attention");
   return rc ? rc : launch_prefix_combine(p, D, std::is_same_v<T, f16> ? 0 : 2, st);
@@ -58,7 +61,7 @@ int prefix_d(const PrefixParams& p, hipStream_t st) {
 //   128 x 16 x 5 queries x 128, prefix 8,192, up to 64                                  99         73         73       73         72
 //   8 requests x 32/8 x 128 (32 rows), prefix 32,768, up to 512                         40         39         39       37         41
 //   2 x 32 requests x 16/8 x 128, prefixes of 2,000, up to 500                           -         33         29       29         37
-void prefix_plan(PrefixParams& p, int D) {
+int prefix_plan(PrefixParams& p, int D) {
   const int64_t pt = std::max<int64_t>(1, ((int64_t)p.pre.S + 31) / 32), ot = std::max<int64_t>(1, ((int64_t)p.own.S + 31) / 32);
   p.pre.pipe = p.pre.rows() > 32;
   const int64_t block = p.pre.pipe ? 128 : 32;
@@ -69,11 +72,14 @@ void prefix_plan(PrefixParams& p, int D) {
   p.pre.splits = (int)((pt + shared - 1) / shared);
   p.own.splits = (int)((ot + own - 1) / own);
   p.pre.joined = p.own.joined = 1;
+  const int rc = check_grid(prefix_launch(p), 256);
+  if (rc) return rc;
+  int32_t dealt;
+  return check_grid(combine_blocks(p.pre.slices() * p.pre.rows(), std::max(p.pre.splits, p.own.splits), D, dealt), 256);
 }
 int64_t prefix_floats(const PrefixParams& p, int D) {
   return cross_part_floats(p.pre.slices(), p.pre.rows(), p.pre.splits, D) + cross_part_floats(p.own.slices(), p.own.rows(), p.own.splits, D);
 }
-
 
 int launch_prefix(const PrefixParams& p, int D, int dtype, hipStream_t st) {
   switch (D) {
