@@ -282,7 +282,8 @@ int tattn_cache4_attention(const void* q, void* o, const uint8_t* codes, const u
  *
  * m: [Z, H, N] float32 base-2 log-sum-exp for the backward, or null. workspace: float32, 16-byte aligned, as many as
  * tattn_cross_workspace gives for the same sizes (null where 0); calls that may overlap need one each.
- * The backward sums dk and dv over the heads of a group, without atomics; keys at or past lens[z] get zeros.
+ * The backward sums dk and dv over the heads of a group, without atomics; keys at or past lens[z] get zeros. Calls whose launches would
+ * hold 2^32 threads or more are refused, by the workspace's functions too.
  */
 int tattn_cross_workspace(int backward, int64_t Z, int64_t H, int64_t Hk, int64_t N, int64_t S, int64_t D, int dtype,
                           int64_t* floats);
@@ -315,7 +316,7 @@ int tattn_prefix_attention(const void* q, const void* prefix_k, const void* pref
 /*
  * The rotation of tattn_norm_rope_* by positions on several axes: pair i of a token is turned by the angle whose cosine and sine
  * are cos[x][i], sin[x][i] (float32 [R, D / 2], contiguous) with x the token's position on axis axes[i]. axes: host array of
- * D / 2 entries, each in [0, num_axes), num_axes <= 8, or -1 for a pair that is not turned. positions: [num_axes, N] (pos_stride
+ * D / 2 entries, each in [0, num_axes), num_axes <= 8, or -1 for a pair that stays as it is. positions: [num_axes, N] (pos_stride
  * 0) or [num_axes, Z, N], axis_stride and pos_stride apart. A position outside [0, R) makes the pairs of its axis NaN. Without
  * weights (both null) there is no norm: eps is not read, the backward reads no q and k and gives no gradients of weights.
  */

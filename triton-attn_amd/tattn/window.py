@@ -143,7 +143,8 @@ def window_attention(
     j < sinks. len is keys, or lens[batch] (int32, on the GPU, clamped to [0, keys]) where a cache is filled to
     different lengths; what lies behind it, or before every window, reaches no result. Rows at positions below 0 give
     zeros. sm_scale defaults to 1 / sqrt(dim). Differentiable in q, k and v without lens; with lens the call is for serving
-    and refuses inputs that require gradients. Forward-mode derivatives are refused. A key or value that is infinite or NaN
+    and refuses inputs that require gradients. Forward-mode derivatives are refused. In float16 a gradient of the scores, P (dP - delta),
+    of more than 65,504 makes infinite gradients. A key or value that is infinite or NaN
     makes the rows that see it NaN, and may make NaN of rows up to 64 positions before it or after its window that do not see
     it."""
     no_tangents(q, k, v)
